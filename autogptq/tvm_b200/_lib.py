@@ -62,6 +62,9 @@ _SIGNATURES = {
     "b200gptq_dense_gemv": (_c_int, [_c_void_p] * 3 + [_c_int] * 3 + [_c_void_p]),
     "b200gptq_pick_local": (_c_int, [_c_void_p, _c_int, _c_int, _c_int, ctypes.c_longlong, _c_int, _c_int, _c_void_p,
                                      _c_void_p, ctypes.c_longlong, _c_void_p, _c_void_p]),
+    "b200gptq_attn_workspace_bytes": (ctypes.c_int64, [_c_void_p]),
+    "b200gptq_attn": (_c_int, [_c_void_p, _c_void_p, _c_size_t, _c_void_p]),
+    "b200gptq_adjust_logits": (_c_int, [_c_void_p, _c_void_p]),
     "b200gptq_step_plan_bytes": (_c_size_t, [_c_void_p]),
     "b200gptq_step_table_bytes": (_c_size_t, [_c_int]),
     "b200gptq_step_plan_create": (_c_int, [_c_void_p] * 4),
@@ -83,6 +86,21 @@ class StepLayer(ctypes.Structure):
 class StepShape(ctypes.Structure):
     _fields_ = ([(n, _c_int) for n in ("layers", "batch", "hidden", "heads", "inter", "max_seq", "bits", "group_size", "gated", "rms", "rope")]
                 + [("eps", ctypes.c_float), ("scale", ctypes.c_float)] + [(n, _c_void_p) for n in ("cos_t", "sin_t", "pos")])
+
+
+class AttnArgs(ctypes.Structure):
+    _fields_ = ([(n, _c_void_p) for n in ("q", "k_cache", "v_cache", "k_prefix", "v_prefix", "out", "pos", "counts")]
+                + [(n, ctypes.c_int64 * 3) for n in ("q_stride", "out_stride", "k_stride", "v_stride")]
+                + [(n, ctypes.c_int64 * 2) for n in ("k_prefix_stride", "v_prefix_stride")]
+                + [(n, _c_int) for n in ("dtype", "batch", "tokens", "heads", "kv_heads", "hd", "max_seq", "prefix", "window", "sinks", "pos_each")]
+                + [("scale", ctypes.c_float)])
+
+
+class LogitArgs(ctypes.Structure):
+    _fields_ = ([(n, _c_void_p) for n in ("logits", "out", "history", "lengths", "prompt_lens", "bias_tokens", "repetition", "frequency",
+                                          "presence", "bias_values", "mask")]
+                + [(n, ctypes.c_int64) for n in ("logits_stride", "out_stride", "history_stride", "mask_stride")]
+                + [(n, _c_int) for n in ("dtype", "rows", "vocab", "history_len", "biases")])
 
 
 def _load() -> ctypes.CDLL:

@@ -1,0 +1,69 @@
+// b200gptq_attn: checks of the arguments and choice of the kernel.  See include/b200gptq.h.
+#include <cstdlib>
+
+#include "attn.h"
+#include "common.cuh"
+
+namespace b200gptq {
+
+bool attn_pdl_enabled() {
+    static const bool on = [] {
+        const char* e = std::getenv("B200GPTQ_PDL");
+        return !(e && e[0] == '0');
+    }();
+    return on;
+}
+
+namespace {
+
+constexpr int kMost = 1 << 29;          // of every size, so that positions and their differences are ints
+
+int check_sizes(const b200gptq_attn_args& a) {
+    if (a.dtype != B200GPTQ_F16 && a.dtype != B200GPTQ_BF16) return B200GPTQ_ERR_SHAPE;
+    if (a.batch < 1 || a.tokens < 1 || a.heads < 1 || a.kv_heads < 1 || a.heads % a.kv_heads || (a.hd != 64 && a.hd != 128)) return B200GPTQ_ERR_SHAPE;
+    if (a.max_seq < 1 || a.prefix < 0 || a.window < 0 || a.sinks < 0 || (a.window && a.prefix) || (!a.window && a.sinks)) return B200GPTQ_ERR_SHAPE;
+    if (a.batch > kMost || a.tokens > kMost || a.max_seq > kMost || a.prefix > kMost || a.window > kMost || a.sinks > kMost ||
+        (long long)a.batch * a.tokens > kMost || (long long)a.batch * a.tokens * (a.heads / a.kv_heads) > kMost)
+        return B200GPTQ_ERR_TOO_LARGE;
+    return B200GPTQ_OK;
+}
+
+size_t scratch_bytes(const b200gptq_attn_args& a, const AttnSplit& s) {
+    return (size_t)s.prefix * a.batch * a.tokens * a.heads * (a.hd + 2) * sizeof(float);
+}
+
+}  // namespace
+}  // namespace b200gptq
+
+using namespace b200gptq;
+
+extern "C" {
+
+B200GPTQ_API int64_t b200gptq_attn_workspace_bytes(const b200gptq_attn_args* args) {
+    if (!args) return B200GPTQ_ERR_NULL_POINTER;
+    const int st = check_sizes(*args);
+    return st != B200GPTQ_OK ? st : (int64_t)scratch_bytes(*args, attn_rows_split(*args));
+}
+
+B200GPTQ_API int b200gptq_attn(const b200gptq_attn_args* args, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!args) return B200GPTQ_ERR_NULL_POINTER;
+    const b200gptq_attn_args& a = *args;
+    const int st = check_sizes(a);
+    if (st != B200GPTQ_OK) return st;
+    if (!a.q || !a.k_cache || !a.v_cache || !a.out || !a.pos || (a.prefix && (!a.k_prefix || !a.v_prefix))) return B200GPTQ_ERR_NULL_POINTER;
+    uintptr_t bits = 0;
+    for (const void* p : {a.q, a.k_cache, a.v_cache, (const void*)a.out}) bits |= reinterpret_cast<uintptr_t>(p);
+    if (a.prefix) bits |= reinterpret_cast<uintptr_t>(a.k_prefix) | reinterpret_cast<uintptr_t>(a.v_prefix);
+    for (int i = 0; i < 3; ++i) bits |= (uintptr_t)(2 * (a.q_stride[i] | a.out_stride[i] | a.k_stride[i] | a.v_stride[i]));
+    if (a.prefix)
+        for (int i = 0; i < 2; ++i) bits |= (uintptr_t)(2 * (a.k_prefix_stride[i] | a.v_prefix_stride[i]));
+    if (bits & 15u) return B200GPTQ_ERR_ALIGNMENT;
+    if ((reinterpret_cast<uintptr_t>(a.pos) | reinterpret_cast<uintptr_t>(a.counts)) & 7u) return B200GPTQ_ERR_ALIGNMENT;
+    const AttnSplit s = attn_rows_split(a);
+    const size_t need = scratch_bytes(a, s);
+    if (need && (!workspace || workspace_bytes < need)) return B200GPTQ_ERR_WORKSPACE;
+    if (reinterpret_cast<uintptr_t>(workspace) & 15u) return B200GPTQ_ERR_ALIGNMENT;
+    return attn_rows_dispatch(a, static_cast<float*>(workspace), s, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -1,0 +1,101 @@
+// What the two kernels of b200gptq_attn share: the types' conversions, what a query sees, and the slow exact row.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+
+namespace b200gptq {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <typename T> struct Half;       // the two 16-bit types
+template <> struct Half<__half> {
+    __device__ static __forceinline__ uint32_t pack(float a, float b) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    __device__ static __forceinline__ float2 unpack(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+    __device__ static __forceinline__ __half round(float a) { return __float2half_rn(a); }
+    __device__ static __forceinline__ float wide(__half a) { return __half2float(a); }
+};
+template <> struct Half<__nv_bfloat16> {
+    __device__ static __forceinline__ uint32_t pack(float a, float b) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    __device__ static __forceinline__ float2 unpack(uint32_t u) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u)); }
+    __device__ static __forceinline__ __nv_bfloat16 round(float a) { return __float2bfloat16_rn(a); }
+    __device__ static __forceinline__ float wide(__nv_bfloat16 a) { return __bfloat162float(a); }
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {       // 2^x; 0 for -infinity
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Position of token 0 of sequence b.  Positions far outside the cache behave like those just outside (all sizes are below 2^30).
+__device__ __forceinline__ int attn_pos(const b200gptq_attn_args& a, int b) {
+    const long long p = __ldcg(reinterpret_cast<const long long*>(a.pos) + (a.pos_each ? b : 0));
+    return (int)max(min(p, 1LL << 30), -(1LL << 30));
+}
+__device__ __forceinline__ int attn_count(const b200gptq_attn_args& a, int b) {
+    if (!a.counts) return a.tokens;
+    const long long n = __ldcg(reinterpret_cast<const long long*>(a.counts) + b);
+    return (int)max(min(n, (long long)a.tokens), 0LL);
+}
+// Whether the query at position p sees row j >= 0 of its cache (window is at least 1 here; no window: 2^30).
+__device__ __forceinline__ bool attn_sees(int p, int j, int window, int sinks) { return j <= p && (j > p - window || j < sinks); }
+
+// Rows of a cache that the queries at positions p_lo .. p_hi see between them: [0, s_end) and [w_start, w_end), which do not overlap.
+struct AttnRange { int s_end, w_start, w_end; };
+__device__ __forceinline__ AttnRange attn_range(int p_lo, int p_hi, int window, int sinks, int max_seq) {
+    AttnRange r;
+    r.w_end = max(0, min(p_hi + 1, max_seq));
+    r.w_start = max(0, p_lo - window + 1);
+    r.s_end = max(0, min(sinks, r.w_end));
+    if (r.w_start <= r.s_end) r.w_start = r.s_end = 0;
+    r.w_end = max(r.w_end, r.w_start);
+    return r;
+}
+
+// One query row by one warp, key by key, skipping the rows that it does not see.  The tiles of both kernels multiply weights of zero with whatever
+// the rows hold that other queries of the tile see: where that gives a NaN or an infinity the row is done again here.  A lane owns HD / 32 dims.
+template <typename T, int HD>
+__device__ __noinline__ void attn_row_again(const b200gptq_attn_args& a, int b, int t, int head, int p, int d0, int d1) {
+    constexpr int D = HD / 32;
+    const int lane = threadIdx.x & 31, kh = head / (a.heads / a.kv_heads), window = a.window ? a.window : 1 << 30;
+    const T* q = static_cast<const T*>(a.q) + b * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2] + lane * D;
+    float qf[D], acc[D], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int e = 0; e < D; ++e) { qf[e] = Half<T>::wide(q[e]) * a.scale * kLog2e; acc[e] = 0.f; }
+    auto key = [&](const T* k, const T* v) {
+        float s = 0.f;
+#pragma unroll
+        for (int e = 0; e < D; ++e) s = fmaf(qf[e], Half<T>::wide(k[e]), s);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        const float up = fmaxf(m, s), safe = up == -INFINITY ? 0.f : up, corr = exp2_fast(m - safe), w = exp2_fast(s - safe);
+        m = up;
+        l = l * corr + w;
+#pragma unroll
+        for (int e = 0; e < D; ++e) acc[e] = acc[e] * corr + w * Half<T>::wide(v[e]);
+    };
+    const T *kp = static_cast<const T*>(a.k_prefix) + kh * a.k_prefix_stride[0] + lane * D,
+            *vp = static_cast<const T*>(a.v_prefix) + kh * a.v_prefix_stride[0] + lane * D;
+    for (int j = 0; j < a.prefix; ++j) key(kp + j * a.k_prefix_stride[1], vp + j * a.v_prefix_stride[1]);
+    const T *kc = static_cast<const T*>(a.k_cache) + b * a.k_stride[0] + kh * a.k_stride[1] + lane * D,
+            *vc = static_cast<const T*>(a.v_cache) + b * a.v_stride[0] + kh * a.v_stride[1] + lane * D;
+    const AttnRange r = attn_range(p, p, window, a.sinks, a.max_seq);
+    for (int j = 0; j < r.s_end; ++j) key(kc + j * a.k_stride[2], vc + j * a.v_stride[2]);
+    for (int j = r.w_start; j < r.w_end; ++j) key(kc + j * a.k_stride[2], vc + j * a.v_stride[2]);
+    T* out = static_cast<T*>(a.out) + b * a.out_stride[0] + t * a.out_stride[1] + head * a.out_stride[2];
+#pragma unroll
+    for (int e = 0; e < D; ++e) {
+        const int d = lane * D + e;
+        if (d >= d0 && d < d1) out[d] = Half<T>::round(l != 0.f ? acc[e] / l : 0.f);       // (a NaN stays one)
+    }
+}
+
+}  // namespace b200gptq

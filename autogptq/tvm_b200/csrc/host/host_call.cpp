@@ -12,8 +12,11 @@
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <ATen/core/grad_mode.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
+#include <string>
 #include <unordered_map>
 
 #include "../../../../include/b200gptq.h"
@@ -62,7 +65,7 @@ struct Layer {
 // A reference held for the time of a call.
 struct Held {
     PyObject* o;
-    explicit Held(PyObject* p) : o(p) { Py_XINCREF(o); }
+    explicit Held(PyObject* p, bool own = false) : o(p) { if (!own) Py_XINCREF(o); }      // own: a reference that is handed over
     ~Held() { Py_XDECREF(o); }
     Held(const Held&) = delete;
     Held& operator=(const Held&) = delete;
@@ -384,7 +387,268 @@ PyObject* set_scratch_source(PyObject*, PyObject* fn) {
     Py_RETURN_NONE;
 }
 
+// ---- b200gptq_attn and b200gptq_adjust_logits: the checks that need tensors, the outputs' memory and the call.  There is no other route; what
+//      is wrong is raised here, with the type that ops.py's other checks have. ----
+struct Refusal { PyObject* type; std::string text; };
+[[noreturn]] void refuse(PyObject* type, std::string text) { throw Refusal{type, std::move(text)}; }
+
+const at::Tensor* tensor_or_none(PyObject* o, const char* name) {
+    if (o == Py_None) return nullptr;
+    if (!THPVariable_Check(o)) refuse(PyExc_TypeError, std::string(name) + " must be a tensor");
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (t.key_set().has_any(kNotPlain) || t.layout() != at::kStrided) refuse(PyExc_TypeError, std::string(name) + " must be a plain tensor");
+    if (!t.is_cuda()) refuse(PyExc_RuntimeError, std::string(name) + " must be a CUDA tensor: the B200 GPTQ kernels have no CPU path");
+    return &t;
+}
+const at::Tensor& tensor_of(PyObject* o, const char* name) {
+    const at::Tensor* t = tensor_or_none(o, name);
+    if (!t) refuse(PyExc_TypeError, std::string(name) + " must be a tensor");
+    return *t;
+}
+void need(bool ok, const char* name, const char* what) {
+    if (!ok) refuse(PyExc_ValueError, std::string(name) + " " + what);
+}
+void need_type(const at::Tensor& t, at::ScalarType type, const char* name) {
+    if (t.scalar_type() != type) refuse(PyExc_TypeError, std::string(name) + " must be " + c10::toString(type) + ", got " + c10::toString(t.scalar_type()));
+}
+void need_device(const at::Tensor& t, int device, const char* name) {
+    if (t.get_device() != device) refuse(PyExc_RuntimeError, std::string(name) + " is on another device");
+}
+void need_no_gradient(const at::Tensor& t, const char* name) {
+    if (t.requires_grad() && at::GradMode::is_enabled()) refuse(PyExc_RuntimeError, std::string(name) + " requires a gradient, and this operator has no backward pass");
+}
+const void* data_of(const at::Tensor& t) { return t.unsafeGetTensorImpl()->data(); }
+// Whether the memory between the first and the last element of the two has a byte in common.
+bool overlap(const at::Tensor& x, const at::Tensor& y) {
+    auto span = [](const at::Tensor& t, uintptr_t& lo, uintptr_t& hi) {
+        int64_t last = 0;
+        for (int64_t i = 0; i < t.dim(); ++i) {
+            if (t.size(i) == 0) { lo = hi = 0; return; }
+            last += (t.size(i) - 1) * t.stride(i);
+        }
+        lo = (uintptr_t)data_of(t);
+        hi = lo + (uintptr_t)((last + 1) * t.element_size());
+    };
+    uintptr_t a, b, c, d;
+    span(x, a, b);
+    span(y, c, d);
+    return a < d && c < b;
+}
+int int_of(PyObject* o, const char* name) {
+    const long long v = PyLong_AsLongLong(o);
+    if (v == -1 && PyErr_Occurred()) { PyErr_Clear(); refuse(PyExc_TypeError, std::string(name) + " must be an integer"); }
+    need(v >= 0 && v <= (1 << 29), name, "is out of range");
+    return (int)v;
+}
+// A tensor's strides by dimension; those of dimensions of size one are not used and count as 0.
+template <size_t N> void strides_of(const at::Tensor& t, int64_t (&to)[N], const int (&dims)[N]) {
+    for (size_t i = 0; i < N; ++i) to[i] = t.size(dims[i]) == 1 ? 0 : t.stride(dims[i]);
+}
+void need_rows(const at::Tensor& t, const char* name) {
+    need(t.size(-1) == 1 || t.stride(-1) == 1, name, "must be dense in its last dimension");
+    bool ok = ((uintptr_t)data_of(t) & 15u) == 0;
+    for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && (t.size(i) == 1 || (t.stride(i) * (int64_t)t.element_size()) % 16 == 0);
+    need(ok, name, "must have rows that begin at multiples of 16 bytes");
+}
+// int64 [batch]
+const int64_t* whole_numbers(const at::Tensor* t, int device, int64_t batch, const char* name) {
+    if (!t) return nullptr;
+    need_type(*t, at::kLong, name);
+    need_device(*t, device, name);
+    need(t->dim() == 1 && t->size(0) == batch && (batch == 1 || t->stride(0) == 1), name, "must be int64, dense, one number for each sequence");
+    return static_cast<const int64_t*>(data_of(*t));
+}
+
+// The output (one that was given counts a write in place), or a status code.
+PyObject* answer(at::Tensor out, bool given, int st) {
+    if (st != B200GPTQ_OK) return PyLong_FromLong(st);
+    if (given && !out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
+    return THPVariable_Wrap(std::move(out));
+}
+
+// attn(q, k_prefix, v_prefix, k_cache, v_cache, pos, window, sinks, counts, scale, out): the output, or a status code
+PyObject* attn_checked(PyObject* const* args) {
+    const at::Tensor &q = tensor_of(args[0], "q"), &k = tensor_of(args[3], "k_cache"), &v = tensor_of(args[4], "v_cache"), &pos = tensor_of(args[5], "pos");
+    const at::Tensor *kp = tensor_or_none(args[1], "k_prefix"), *vp = tensor_or_none(args[2], "v_prefix"), *counts = tensor_or_none(args[8], "counts"),
+                     *given = tensor_or_none(args[10], "out");
+    b200gptq_attn_args a = {};
+    const int device = q.get_device();
+    const at::ScalarType type = q.scalar_type();
+    if (type != at::kHalf && type != at::kBFloat16) refuse(PyExc_TypeError, "q must be float16 or bfloat16");
+    a.dtype = type == at::kHalf ? B200GPTQ_F16 : B200GPTQ_BF16;
+    need(q.dim() == 4 && q.numel() > 0, "q", "must be [batch, tokens, heads, head_dim]");
+    need(k.dim() == 4 && k.numel() > 0, "k_cache", "must be [batch, kv_heads, max_seq, head_dim]");
+    const int64_t B = q.size(0), T = q.size(1), H = q.size(2), hd = q.size(3), KV = k.size(1), S = k.size(2);
+    need(hd == 64 || hd == 128, "q", "must have heads of 64 or 128 dims");
+    need(k.size(0) == B && k.size(3) == hd && H % KV == 0, "k_cache", "must be [batch, kv_heads, max_seq, head_dim], kv_heads a divisor of q's heads");
+    need(v.sizes() == k.sizes(), "v_cache", "must have the shape of k_cache");
+    need(B * T <= (1 << 29) && B * T * (H / KV) <= (1 << 29) && S <= (1 << 29), "q", "is too large");
+    for (auto [t, name] : {std::pair{&k, "k_cache"}, std::pair{&v, "v_cache"}}) { need_type(*t, type, name); need_device(*t, device, name); need_rows(*t, name); need_no_gradient(*t, name); }
+    need_rows(q, "q");
+    need_no_gradient(q, "q");
+    need_type(pos, at::kLong, "pos");
+    need_device(pos, device, "pos");
+    need(pos.dim() == 1 && (pos.size(0) == B || pos.size(0) == 1) && (pos.size(0) == 1 || pos.stride(0) == 1), "pos", "must be int64, dense, one number or one for each sequence");
+    a.pos = static_cast<const int64_t*>(data_of(pos));
+    a.pos_each = pos.size(0) > 1;
+    a.counts = whole_numbers(counts, device, B, "counts");
+    a.batch = (int)B; a.tokens = (int)T; a.heads = (int)H; a.kv_heads = (int)KV; a.hd = (int)hd; a.max_seq = (int)S;
+    a.q = data_of(q); a.k_cache = data_of(k); a.v_cache = data_of(v);
+    strides_of(q, a.q_stride, {0, 1, 2});
+    strides_of(k, a.k_stride, {0, 1, 2});
+    strides_of(v, a.v_stride, {0, 1, 2});
+    if (kp || vp) {
+        need(kp && vp, "k_prefix", "and v_prefix come together");
+        need(kp->dim() == 3 && kp->size(0) == KV && kp->size(2) == hd && kp->size(1) <= (1 << 29), "k_prefix", "must be [kv_heads, positions, head_dim]");
+        need(vp->sizes() == kp->sizes(), "v_prefix", "must have the shape of k_prefix");
+        for (auto [t, name] : {std::pair{kp, "k_prefix"}, std::pair{vp, "v_prefix"}}) { need_type(*t, type, name); need_device(*t, device, name); need_no_gradient(*t, name); }
+        a.prefix = (int)kp->size(1);
+        if (a.prefix) {
+            need_rows(*kp, "k_prefix");
+            need_rows(*vp, "v_prefix");
+            a.k_prefix = data_of(*kp); a.v_prefix = data_of(*vp);
+            strides_of(*kp, a.k_prefix_stride, {0, 1});
+            strides_of(*vp, a.v_prefix_stride, {0, 1});
+        }
+    } else {
+        a.window = int_of(args[6], "window");
+        a.sinks = int_of(args[7], "sinks");
+        need(a.window >= 1, "window", "must be at least 1");
+    }
+    if (args[9] == Py_None) {
+        a.scale = (float)(1.0 / std::sqrt((double)hd));
+    } else {
+        a.scale = (float)PyFloat_AsDouble(args[9]);
+        if (PyErr_Occurred()) { PyErr_Clear(); refuse(PyExc_TypeError, "scale must be a number"); }
+    }
+    if (given) {
+        need_type(*given, type, "out");
+        need_device(*given, device, "out");
+        need(given->sizes() == q.sizes(), "out", "must have the shape of q");
+        need_rows(*given, "out");
+        need_no_gradient(*given, "out");
+        bool apart = !overlap(*given, q) && !overlap(*given, k) && !overlap(*given, v) && !overlap(*given, pos) && !(counts && overlap(*given, *counts));
+        if (a.prefix) apart = apart && !overlap(*given, *kp) && !overlap(*given, *vp);
+        for (int i = 0; i < 3; ++i) apart = apart && (given->size(i) == 1 || given->stride(i) != 0);
+        need(apart, "out", "must not overlap what is read, nor itself");
+    }
+    // (rows of padding that nobody has given a value)
+    if (counts && !given) refuse(PyExc_ValueError, "counts needs out: the rows of padding keep what it holds");
+    const at::Device on(at::kCUDA, (c10::DeviceIndex)device);
+    const c10::cuda::OptionalCUDAGuard guard(c10::cuda::current_device() != device ? std::optional<at::Device>(on) : std::nullopt);
+    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
+    at::Tensor out, scratch;
+    int st;
+    {
+        const WithoutGil released;
+        out = given ? *given : at::Tensor(at::detail::empty_cuda(q.sizes(), type, on, std::nullopt));
+        a.out = out.unsafeGetTensorImpl()->mutable_data();
+        strides_of(out, a.out_stride, {0, 1, 2});
+        const int64_t bytes = b200gptq_attn_workspace_bytes(&a);
+        if (bytes > 0) scratch = at::detail::empty_cuda({bytes}, at::kByte, on, std::nullopt);
+        st = bytes < 0 ? (int)bytes : b200gptq_attn(&a, bytes > 0 ? scratch.unsafeGetTensorImpl()->mutable_data() : nullptr, (size_t)bytes, stream);
+    }
+    return answer(std::move(out), given != nullptr, st);
+}
+
+// adjust_logits(logits, history, lengths, prompt_lens, repetition, frequency, presence, bias_tokens, bias_values, mask, out)
+PyObject* logits_checked(PyObject* const* args) {
+    const at::Tensor& x = tensor_of(args[0], "logits");
+    const char* names[11] = {"logits", "history", "lengths", "prompt_lens", "repetition", "frequency", "presence", "bias_tokens", "bias_values", "mask", "out"};
+    const at::Tensor* t[11];
+    const int device = x.get_device();
+    for (int i = 1; i < 11; ++i) {
+        t[i] = tensor_or_none(args[i], names[i]);
+        if (t[i]) need_device(*t[i], device, names[i]);
+    }
+    b200gptq_logit_args a = {};
+    const at::ScalarType type = x.scalar_type();
+    if (type != at::kHalf && type != at::kBFloat16 && type != at::kFloat) refuse(PyExc_TypeError, "logits must be float16, bfloat16 or float32");
+    a.dtype = type == at::kHalf ? B200GPTQ_F16 : type == at::kBFloat16 ? B200GPTQ_BF16 : B200GPTQ_F32;
+    need(x.dim() == 2 && x.numel() > 0 && (x.size(1) == 1 || x.stride(1) == 1) && x.size(0) <= INT32_MAX && x.size(1) <= (1 << 30), "logits", "must be [rows, vocab], dense in its last dimension");
+    need_no_gradient(x, "logits");
+    const int64_t R = x.size(0), V = x.size(1);
+    a.rows = (int)R; a.vocab = (int)V;
+    a.logits = data_of(x);
+    a.logits_stride = R == 1 ? 0 : x.stride(0);
+    need((t[1] != nullptr) == (t[2] != nullptr), "history", "and lengths come together");
+    need(t[1] || (!t[3] && !t[4] && !t[5] && !t[6]), "history", "is needed for penalties");
+    if (t[1]) {
+        need_type(*t[1], at::kLong, "history");
+        need(t[1]->dim() == 2 && t[1]->size(0) == R && t[1]->size(1) <= (1 << 30) && (t[1]->size(1) <= 1 || t[1]->stride(1) == 1), "history", "must be [rows, positions], dense in its last dimension");
+        a.history_len = (int)t[1]->size(1);
+        a.history = a.history_len ? static_cast<const int64_t*>(data_of(*t[1])) : nullptr;
+        a.history_stride = R == 1 ? 0 : t[1]->stride(0);
+    }
+    a.lengths = whole_numbers(t[2], device, R, "lengths");
+    a.prompt_lens = whole_numbers(t[3], device, R, "prompt_lens");
+    const float** params[3] = {&a.repetition, &a.frequency, &a.presence};
+    for (int i = 4; i < 7; ++i)
+        if (t[i]) {
+            need_type(*t[i], at::kFloat, names[i]);
+            need(t[i]->dim() == 1 && t[i]->size(0) == R && (R == 1 || t[i]->stride(0) == 1), names[i], "must be float32, dense, one number for each row");
+            *params[i - 4] = static_cast<const float*>(data_of(*t[i]));
+        }
+    need((t[7] != nullptr) == (t[8] != nullptr), "bias_tokens", "and bias_values come together");
+    if (t[7]) {
+        need_type(*t[7], at::kLong, "bias_tokens");
+        need_type(*t[8], at::kFloat, "bias_values");
+        need(t[7]->dim() == 2 && t[7]->size(0) == R && t[7]->size(1) < (1 << 30) && t[7]->is_contiguous(), "bias_tokens", "must be [rows, entries], contiguous");
+        need(t[8]->sizes() == t[7]->sizes() && t[8]->is_contiguous(), "bias_values", "must have the shape of bias_tokens, contiguous");
+        a.biases = (int)t[7]->size(1);
+        if (a.biases) { a.bias_tokens = static_cast<const int64_t*>(data_of(*t[7])); a.bias_values = static_cast<const float*>(data_of(*t[8])); }
+    }
+    if (t[9]) {
+        need_type(*t[9], at::kInt, "mask");
+        need(t[9]->dim() == 2 && (t[9]->size(0) == R || t[9]->size(0) == 1) && t[9]->size(1) == (V + 31) / 32 && (t[9]->size(1) == 1 || t[9]->stride(1) == 1), "mask",
+             "must be [rows or 1, ceil(vocab / 32)], dense in its last dimension");
+        a.mask = static_cast<const int32_t*>(data_of(*t[9]));
+        a.mask_stride = t[9]->size(0) == 1 ? 0 : t[9]->stride(0);
+    }
+    if (t[10]) {
+        const at::Tensor& o = *t[10];
+        need_type(o, type, "out");
+        need(o.sizes() == x.sizes() && (V == 1 || o.stride(1) == 1) && (R == 1 || o.stride(0) >= V), "out", "must have the shape of logits, rows apart and dense in its last dimension");
+        need_no_gradient(o, "out");
+        bool apart = (data_of(o) == data_of(x) && (R == 1 || o.stride(0) == x.stride(0))) || !overlap(o, x);
+        for (int i = 1; i < 10; ++i) apart = apart && !(t[i] && overlap(o, *t[i]));
+        need(apart, "out", "must be logits itself or overlap nothing that is read");
+    }
+    const at::Device on(at::kCUDA, (c10::DeviceIndex)device);
+    const c10::cuda::OptionalCUDAGuard guard(c10::cuda::current_device() != device ? std::optional<at::Device>(on) : std::nullopt);
+    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
+    at::Tensor out;
+    int st;
+    {
+        const WithoutGil released;
+        out = t[10] ? *t[10] : at::Tensor(at::detail::empty_cuda({R, V}, type, on, std::nullopt));
+        a.out = out.unsafeGetTensorImpl()->mutable_data();
+        a.out_stride = R == 1 ? 0 : out.stride(0);
+        st = b200gptq_adjust_logits(&a, stream);
+    }
+    return answer(std::move(out), t[10] != nullptr, st);
+}
+
+PyObject* raising(PyObject* (*call)(PyObject* const*), PyObject* const* args, Py_ssize_t nargs) {
+    if (nargs != 11) { PyErr_SetString(PyExc_TypeError, "11 arguments"); return nullptr; }
+    try {
+        return call(args);
+    } catch (const Refusal& r) {
+        PyErr_SetString(r.type, r.text.c_str());
+    } catch (const c10::OutOfMemoryError& e) {
+        const Held torch(PyImport_ImportModule("torch"), true), type(torch.o ? PyObject_GetAttrString(torch.o, "OutOfMemoryError") : nullptr, true);
+        if (type.o) PyErr_SetString(type.o, e.what_without_backtrace());
+    } catch (const std::exception& e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+    }
+    return nullptr;
+}
+PyObject* attn(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return raising(attn_checked, args, nargs); }
+PyObject* adjust_logits(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return raising(logits_checked, args, nargs); }
+
 PyMethodDef module_methods[] = {
+    {"attn", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attn)), METH_FASTCALL, nullptr},
+    {"adjust_logits", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adjust_logits)), METH_FASTCALL, nullptr},
     {"pack", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(pack)), METH_FASTCALL, nullptr},
     {"set_scratch", set_scratch, METH_VARARGS, nullptr},
     {"set_scratch_source", set_scratch_source, METH_O, nullptr},

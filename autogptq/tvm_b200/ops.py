@@ -447,6 +447,50 @@ def attn_step(qkv, cos_t, sin_t, pos, k_cache, v_cache, out, heads: int, hd: int
     return out
 
 
+def _checked(r, where: str):
+    if isinstance(r, int):
+        _lib.check(r, where)
+    return r
+
+
+def attn_window(q, k_cache, v_cache, pos, window: int, sinks: int = 0, counts=None, scale: Optional[float] = None, out=None):
+    """Attention of new tokens that sees the last ``window`` positions, the token's own among them, and the first ``sinks``
+    (``b200gptq_attn``), for single tokens of a decode step and for prompts or chunks of them.
+
+    ``q`` ``[B, T, heads, hd]`` fp16 or bf16, hd 64 or 128; caches ``[B, kv_heads, max_seq, hd]`` of the same type, which hold the new tokens' own keys
+    and values already; ``pos`` int64 ``[1]`` or ``[B]`` on the device: position of token 0 (token t is at ``pos + t``); ``counts`` int64 ``[B]``:
+    how many of a sequence's T tokens are no padding, the rows of ``out`` behind them are left as they were.  ``scale`` is ``hd ** -0.5`` where not
+    given.  Views are taken as long as rows begin at multiples of 16 bytes.  A query before position 0 sees nothing and gets zeros; one
+    behind the cache sees what its window has of it.  There is no backward pass.  Returns ``[B, T, heads, hd]``."""
+    return _checked(_lib._host.attn(q, None, None, k_cache, v_cache, pos, window, sinks, counts, scale, out), "b200gptq_attn")
+
+
+def attn_prefix(q, k_prefix, v_prefix, k_cache, v_cache, pos, counts=None, scale: Optional[float] = None, out=None):
+    """Attention of a batch whose sequences begin with the same text: ``k_prefix`` / ``v_prefix`` ``[kv_heads, P, hd]`` are held and read once
+    for all (P may be 0), the rest of each sequence is in its own rows of the caches ``[B, kv_heads, max_seq, hd]``.  A query sees all P rows and rows
+    ``0 .. pos + t`` of its own; ``pos`` counts the sequence's own rows (-1: none).  Otherwise as :func:`attn_window`."""
+    if k_prefix is None or v_prefix is None:
+        raise TypeError("k_prefix and v_prefix must be tensors")
+    return _checked(_lib._host.attn(q, k_prefix, v_prefix, k_cache, v_cache, pos, 0, 0, counts, scale, out), "b200gptq_attn")
+
+
+def adjust_logits(logits, history=None, lengths=None, prompt_lens=None, repetition=None, frequency=None, presence=None,
+                  bias_tokens=None, bias_values=None, mask=None, out=None):
+    """Rules on next-token logits before the pick, in one launch (``b200gptq_adjust_logits``).  ``logits`` ``[rows, vocab]`` fp16, bf16 or
+    fp32; per row:
+
+    * a token that stands in ``history[:lengths]`` (int64 ``[rows, L]``): ``x / repetition`` if ``x > 0`` else ``x * repetition``;
+    * a token that stands n > 0 times in ``history[prompt_lens:lengths]``: ``x - frequency * n - presence``;
+    * ``bias_values`` (fp32 ``[rows, N]``) is added to the tokens ``bias_tokens`` (int64; -1: no token; the last of several entries
+      for one token counts);
+    * bit ``v % 32`` of ``mask[:, v // 32]`` (int32 ``[rows or 1, ceil(vocab / 32)]``) clear: minus infinity.
+
+    ``repetition`` / ``frequency`` / ``presence`` are fp32 ``[rows]``.  ``out`` may be ``logits``.  A row whose mask leaves nothing is minus infinity
+    throughout.  Evaluated in fp32, rounded once."""
+    return _checked(_lib._host.adjust_logits(logits, history, lengths, prompt_lens, repetition, frequency, presence, bias_tokens,
+                                             bias_values, mask, out), "b200gptq_adjust_logits")
+
+
 def act(u, out, inter: int, gated: bool):
     with torch.cuda.device(u.device):
         st = _lib.lib.b200gptq_act(_ptr(u), _ptr(out), u.shape[0], inter, 1 if gated else 0, _stream(u.device))

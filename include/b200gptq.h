@@ -428,6 +428,65 @@ B200GPTQ_API int b200gptq_pick_final(const void* slots, int rows, int world, lon
                                      long long* pos_inc, void* stream);
 
 /*
+ * Attention of new tokens over a KV cache with a sliding window and sinks, or behind a prefix that the whole batch shares.  No
+ * counterpart in the reference, which leaves attention to transformers' modules
+ * (end2end/autogptq-generation-inference-benchmark.py:26-49); b200gptq_attn_decode above sees the whole cache of one head layout.
+ *
+ *   out[b, t, h, :] = sum_j w_j v_j,  w = softmax over the visible j of (scale * q[b, t, h, :] . k_j)
+ *
+ * The query of token t of sequence b is at position p = pos[b] + t of the sequence's own cache [b, kv_heads, max_seq, hd] and
+ * reads key head h / (heads / kv_heads).  It sees the rows j of the cache with 0 <= j <= p, j < max_seq and (j > p - window or j < sinks)
+ * (window 0: all of 0 <= j <= p), and all `prefix` rows of k_prefix / v_prefix [kv_heads, prefix, hd], which stand in front of every sequence.  A query that
+ * sees nothing gets zeros.  What lies in rows that it does not see does not matter, NaN and infinities included.  The new tokens' own keys and
+ * values are in the cache before the call.  window and prefix are not combined: one of them is 0.
+ *
+ *   dtype      B200GPTQ_F16 or B200GPTQ_BF16, of q, caches, prefix and out.  Sums and softmax statistics are fp32; the weights are
+ *              rounded to dtype before they multiply v, the result once at the end
+ *   hd         64 or 128;  kv_heads divides heads
+ *   pos        device int64 [batch], or one for all (pos_each 0);  counts  device int64 [batch] or NULL: tokens t >= counts[b] are padding, and
+ *              out is left as it was there
+ *   strides    in elements, multiples of 8: q and out {batch, token, head}, caches {batch, head, row}, prefix {head, row}; the last
+ *              dimension is dense.  All addresses 16-byte aligned.  out overlaps nothing that is read
+ * b200gptq_attn_workspace_bytes: scratch of a call (0 without a prefix; its contents on entry do not matter and nothing is kept there, so
+ * calls that may overlap need scratch of their own).  Negative: a B200GPTQ_ERR_* code for the sizes.
+ */
+typedef struct {
+    const void *q, *k_cache, *v_cache, *k_prefix, *v_prefix;
+    void* out;
+    const int64_t *pos, *counts;
+    int64_t q_stride[3], out_stride[3], k_stride[3], v_stride[3], k_prefix_stride[2], v_prefix_stride[2];
+    int dtype, batch, tokens, heads, kv_heads, hd, max_seq, prefix, window, sinks, pos_each;
+    float scale;
+} b200gptq_attn_args;
+B200GPTQ_API int64_t b200gptq_attn_workspace_bytes(const b200gptq_attn_args* args);
+B200GPTQ_API int b200gptq_attn(const b200gptq_attn_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Rules on the logits of the next token, before the pick (the reference leaves them to transformers' generate()).  Per row, for token v with logit x:
+ *   1. v among history[0 .. length):              x = x > 0 ? x / repetition : x * repetition
+ *   2. v n times (n > 0) in history[prompt_len .. length):   x = x - frequency * n - presence
+ *   3. v among bias_tokens:                       x = x + its value in bias_values (the last entry where v stands there several times)
+ *   4. bit v % 32 of mask word v / 32 is 0:       x = -infinity
+ * evaluated in fp32 and rounded once.  Tokens outside [0, vocab), in history or among the biases, count for nothing (padding: -1).
+ *   dtype      B200GPTQ_F16, _BF16 or _F32, of logits and out [rows, vocab] with row strides (elements); out may be logits itself
+ *   history    device int64 [rows, history_len], row stride history_stride; lengths / prompt_lens device int64 [rows], held to
+ *              [0, history_len]; prompt_lens NULL: 0.  history NULL: rules 1 and 2 are left out
+ *   repetition, frequency, presence  device fp32 [rows], each NULL for 1, 0, 0
+ *   bias_tokens int64 and bias_values fp32 [rows, biases], dense, or NULL;  mask int32 [rows, ceil(vocab / 32)], row stride mask_stride (0: one mask for
+ *              all rows), or NULL
+ */
+typedef struct {
+    const void* logits;
+    void* out;
+    const int64_t *history, *lengths, *prompt_lens, *bias_tokens;
+    const float *repetition, *frequency, *presence, *bias_values;
+    const int32_t* mask;
+    int64_t logits_stride, out_stride, history_stride, mask_stride;
+    int dtype, rows, vocab, history_len, biases;
+} b200gptq_logit_args;
+B200GPTQ_API int b200gptq_adjust_logits(const b200gptq_logit_args* args, void* stream);
+
+/*
  * The decoder layers of one decode step of one sequence as ONE cooperative launch: per layer norm, q|k|v, rotary embedding +
  * cache write + attention, output projection, residual sum, norm, first FFN linear, activation, second FFN linear, residual sum: the
  * arithmetic of the helpers above and of b200gptq_gemv.  The reference has no counterpart (its loop is transformers' generate(),

@@ -84,3 +84,68 @@ def test_attention_refuses_caches_that_are_not_aligned():
         for hd in (64, 128):
             assert _lib.lib.b200gptq_attn_decode(a, k, v, a, a, 1, 8, hd, 256, 1.0, None) == -4
             assert _lib.lib.b200gptq_attn_step(a, a, a, a, k, v, a, 1, 8, hd, 256, 1, 1.0, None) == -4
+
+
+def test_attention_with_a_window_or_a_prefix_refuses_on_the_host():
+    """Every check comes before anything is launched (the addresses are made up)."""
+    import ctypes
+    from autogptq.tvm_b200 import _lib
+    A = 0x100000
+    good = dict(q=A, k_cache=A, v_cache=A, out=A, pos=A, dtype=0, batch=2, tokens=1, heads=8, kv_heads=2, hd=64, max_seq=40, window=4, scale=1.0)
+
+    def call(fn=_lib.lib.b200gptq_attn, ws=None, ws_bytes=0, **change):
+        a = _lib.AttnArgs(**{k: v for k, v in dict(good, **change).items() if "stride" not in k})
+        for n in ("q_stride", "out_stride", "k_stride", "v_stride"):
+            setattr(a, n, (ctypes.c_int64 * 3)(*change.get(n, (512, 64, 64))))
+        for n in ("k_prefix_stride", "v_prefix_stride"):
+            setattr(a, n, (ctypes.c_int64 * 2)(*change.get(n, (512, 64))))
+        return fn(ctypes.byref(a), ws, ws_bytes, None) if fn is _lib.lib.b200gptq_attn else fn(ctypes.byref(a))
+
+    assert _lib.lib.b200gptq_attn(None, None, 0, None) == -1 and _lib.lib.b200gptq_attn_workspace_bytes(None) == -1
+    for change, status in [
+        (dict(q=None), -1), (dict(k_cache=None), -1), (dict(v_cache=None), -1), (dict(out=None), -1), (dict(pos=None), -1),
+        (dict(window=0, prefix=5), -1), (dict(window=0, prefix=5, k_prefix=A), -1),
+        (dict(dtype=2), -3), (dict(dtype=-1), -3), (dict(batch=0), -3), (dict(tokens=0), -3), (dict(heads=0), -3), (dict(kv_heads=3), -3), (dict(kv_heads=0), -3),
+        (dict(hd=80), -3), (dict(max_seq=0), -3), (dict(window=-1), -3), (dict(sinks=-1), -3), (dict(prefix=-1), -3), (dict(prefix=5), -3),
+        (dict(window=0, sinks=3), -3), (dict(batch=1 << 20, tokens=1 << 20), -8), (dict(max_seq=(1 << 29) + 1), -8), (dict(window=(1 << 29) + 1), -8),
+        (dict(q=A + 8), -4), (dict(k_cache=A + 2), -4), (dict(v_cache=A + 8), -4), (dict(out=A + 8), -4), (dict(pos=A + 4), -4), (dict(counts=A + 4), -4),
+        (dict(q_stride=(512, 64, 68)), -4), (dict(k_stride=(4, 64, 64)), -4), (dict(v_stride=(512, 4, 64)), -4), (dict(out_stride=(512, 64, 1)), -4),
+        (dict(window=0, prefix=5, k_prefix=A, v_prefix=A + 8), -4), (dict(window=0, prefix=5, k_prefix=A, v_prefix=A, v_prefix_stride=(512, 4)), -4),
+        (dict(window=0, prefix=5, k_prefix=A, v_prefix=A), -5),
+    ]:
+        assert call(**change) == status, change
+    assert call(fn=_lib.lib.b200gptq_attn_workspace_bytes) == 0
+    need = call(fn=_lib.lib.b200gptq_attn_workspace_bytes, window=0, prefix=500)
+    assert need > 0 and need % (2 * 8 * 66 * 4) == 0
+    assert call(window=0, prefix=500, k_prefix=A, v_prefix=A, ws=A, ws_bytes=need - 1) == -5
+    assert call(window=0, prefix=500, k_prefix=A, v_prefix=A, ws=A + 8, ws_bytes=need) == -4
+    assert call(fn=_lib.lib.b200gptq_attn_workspace_bytes, hd=96) == -3
+
+
+def test_logit_rules_refuse_on_the_host():
+    import ctypes
+    from autogptq.tvm_b200 import _lib
+    A = 0x100000
+    good = dict(logits=A, out=A, history=A, lengths=A, bias_tokens=A, bias_values=A, dtype=0, rows=2, vocab=100, history_len=5, biases=2, logits_stride=100, out_stride=100)
+    assert _lib.lib.b200gptq_adjust_logits(None, None) == -1
+    for change, status in [(dict(logits=None), -1), (dict(out=None), -1), (dict(lengths=None), -1), (dict(bias_tokens=None), -1), (dict(bias_values=None), -1),
+                           (dict(rows=0), -3), (dict(vocab=0), -3), (dict(history_len=-1), -3), (dict(biases=-1), -3), (dict(dtype=3), -3), (dict(logits_stride=-1), -3),
+                           (dict(logits=A + 1), -4), (dict(out=A + 2, dtype=2), -4), (dict(history=A + 4), -4), (dict(lengths=A + 4), -4)]:
+        assert _lib.lib.b200gptq_adjust_logits(ctypes.byref(_lib.LogitArgs(**dict(good, **change))), None) == status, change
+
+
+def test_attention_and_logit_rules_refuse_cpu_tensors():
+    import pytest
+    import torch
+    from autogptq.tvm_b200 import ops
+    q, k, p = torch.zeros(1, 1, 2, 64).half(), torch.zeros(1, 2, 8, 64).half(), torch.zeros(1).long()
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.attn_window(q, k, k, p, 4)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.attn_prefix(q, k[0], k[0], k, k, p)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.adjust_logits(torch.zeros(1, 8))
+    with pytest.raises(TypeError):
+        ops.attn_window(None, k, k, p, 4)
+    with pytest.raises(TypeError):
+        ops.attn_prefix(q, None, None, k, k, p)
