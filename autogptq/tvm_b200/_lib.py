@@ -89,7 +89,7 @@ class StepShape(ctypes.Structure):
 
 
 class AttnArgs(ctypes.Structure):
-    _fields_ = ([(n, _c_void_p) for n in ("q", "k_cache", "v_cache", "k_prefix", "v_prefix", "out", "pos", "counts")]
+    _fields_ = ([(n, _c_void_p) for n in ("q", "k_cache", "v_cache", "k_prefix", "v_prefix", "out", "pos", "counts", "status")]
                 + [(n, ctypes.c_int64 * 3) for n in ("q_stride", "out_stride", "k_stride", "v_stride")]
                 + [(n, ctypes.c_int64 * 2) for n in ("k_prefix_stride", "v_prefix_stride")]
                 + [(n, _c_int) for n in ("dtype", "batch", "tokens", "heads", "kv_heads", "hd", "max_seq", "prefix", "window", "sinks", "pos_each")]

@@ -1,4 +1,5 @@
 // b200gptq_attn: checks of the arguments and choice of the kernel.  See include/b200gptq.h.
+#include <algorithm>
 #include <cstdlib>
 
 #include "attn.h"
@@ -16,7 +17,7 @@ bool attn_pdl_enabled() {
 
 namespace {
 
-constexpr int kMost = 1 << 29;          // of every size, so that positions and their differences are ints
+constexpr int kMost = 1 << 29;      // of every size, so that positions and their differences are ints
 
 int check_sizes(const b200gptq_attn_args& a) {
     if (a.dtype != B200GPTQ_F16 && a.dtype != B200GPTQ_BF16) return B200GPTQ_ERR_SHAPE;
@@ -28,8 +29,35 @@ int check_sizes(const b200gptq_attn_args& a) {
     return B200GPTQ_OK;
 }
 
-size_t scratch_bytes(const b200gptq_attn_args& a, const AttnSplit& s) {
-    return (size_t)s.prefix * a.batch * a.tokens * a.heads * (a.hd + 2) * sizeof(float);
+AttnPlan plan_of(const b200gptq_attn_args& a) {
+    AttnPlan p = {};
+    const long long rows = (long long)a.tokens * (a.heads / a.kv_heads), all = rows * a.batch, sms = sm_count();
+    if (rows >= 64 && attn_tiles_maps(a, false) && (!a.prefix || attn_tiles_maps(a, true))) {
+        p.tiles = true;
+        return p;
+    }
+    // As many CTAs as the SMs hold (one each), as long as every warp has a block of keys.
+    const long long units = (rows <= 16 ? 1 : (rows + 31) / 32) * a.kv_heads * a.batch;
+    const long long keys = a.window ? std::min<long long>(a.max_seq, (long long)a.window + a.sinks + a.tokens) : a.max_seq;
+    p.own = 1;
+    while (p.own < kAttnMaxSplit && units * p.own * 2 <= sms && keys > p.own * kAttnRowsKeys) p.own *= 2;
+    if (a.prefix) {
+        p.prefix_tiles = all > 32 && attn_tiles_maps(a, true);
+        if (p.prefix_tiles) {
+            const bool pairs = all <= 128;            // two runs of each CTA
+            const long long tiles = (a.prefix + 127) / 128, ctas = (all + 255) / 256 * a.kv_heads;
+            const long long splits = std::max<long long>(1, std::min(sms / ctas, tiles / 2));
+            p.parts = (int)(pairs ? 2 * splits : splits);
+        } else {
+            const long long ctas = (all <= 16 ? 1 : (all + 31) / 32) * a.kv_heads;
+            p.parts = (int)std::max<long long>(1, std::min<long long>(std::min<long long>(2 * sms / ctas, 64), a.prefix / kAttnRowsKeys));
+        }
+    }
+    return p;
+}
+
+size_t scratch_bytes(const b200gptq_attn_args& a, const AttnPlan& p) {
+    return (size_t)p.parts * a.batch * a.tokens * a.heads * (a.hd + 2) * sizeof(float);
 }
 
 }  // namespace
@@ -42,7 +70,7 @@ extern "C" {
 B200GPTQ_API int64_t b200gptq_attn_workspace_bytes(const b200gptq_attn_args* args) {
     if (!args) return B200GPTQ_ERR_NULL_POINTER;
     const int st = check_sizes(*args);
-    return st != B200GPTQ_OK ? st : (int64_t)scratch_bytes(*args, attn_rows_split(*args));
+    return st != B200GPTQ_OK ? st : (int64_t)scratch_bytes(*args, plan_of(*args));
 }
 
 B200GPTQ_API int b200gptq_attn(const b200gptq_attn_args* args, void* workspace, size_t workspace_bytes, void* stream) {
@@ -58,12 +86,19 @@ B200GPTQ_API int b200gptq_attn(const b200gptq_attn_args* args, void* workspace, 
     if (a.prefix)
         for (int i = 0; i < 2; ++i) bits |= (uintptr_t)(2 * (a.k_prefix_stride[i] | a.v_prefix_stride[i]));
     if (bits & 15u) return B200GPTQ_ERR_ALIGNMENT;
-    if ((reinterpret_cast<uintptr_t>(a.pos) | reinterpret_cast<uintptr_t>(a.counts)) & 7u) return B200GPTQ_ERR_ALIGNMENT;
-    const AttnSplit s = attn_rows_split(a);
-    const size_t need = scratch_bytes(a, s);
+    if ((reinterpret_cast<uintptr_t>(a.pos) | reinterpret_cast<uintptr_t>(a.counts)) & 7u || reinterpret_cast<uintptr_t>(a.status) & 3u) return B200GPTQ_ERR_ALIGNMENT;
+    const AttnPlan p = plan_of(a);
+    const size_t need = scratch_bytes(a, p);
     if (need && (!workspace || workspace_bytes < need)) return B200GPTQ_ERR_WORKSPACE;
     if (reinterpret_cast<uintptr_t>(workspace) & 15u) return B200GPTQ_ERR_ALIGNMENT;
-    return attn_rows_dispatch(a, static_cast<float*>(workspace), s, static_cast<cudaStream_t>(stream));
+    const cudaStream_t at = static_cast<cudaStream_t>(stream);
+    float* part = static_cast<float*>(workspace);
+    if (p.tiles) return attn_tiles_dispatch(a, at);
+    if (p.prefix_tiles) {
+        const int before = attn_tiles_prefix(a, part, p.parts, at);
+        if (before != B200GPTQ_OK) return before;
+    }
+    return attn_rows_dispatch(a, part, p, at);
 }
 
 }  // extern "C"

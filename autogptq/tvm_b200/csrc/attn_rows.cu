@@ -26,7 +26,8 @@
 namespace b200gptq {
 namespace {
 
-constexpr int kWarps = 8, kThreads = kWarps * 32, kBlock = 16, kMaxSplit = 8;
+constexpr int kWarps = 8, kThreads = kWarps * 32, kBlock = 16, kMaxSplit = kAttnMaxSplit;
+static_assert(kWarps * kBlock == kAttnRowsKeys, "");
 
 template <typename T>
 __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -56,7 +57,7 @@ template <int HD, int MT> struct Lay {
 // (and the sums of the prefix).  A row tile is blockIdx.x / splits % row_tiles.
 template <typename T, int HD, int MT, bool PREFIX>
 __global__ void __launch_bounds__(kThreads, 1)
-attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict__ part, int splits, int row_tiles, int prefix_splits) {
+attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict__ part, int splits, int row_tiles, int parts) {
     using L = Lay<HD, MT>;
     constexpr int R = L::R, SEG = HD / 32, HH = HD / 64;
     extern __shared__ __align__(16) float sm[];
@@ -283,20 +284,20 @@ attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict
     if (a.prefix) asm volatile("griddepcontrol.wait;" ::: "memory");                        // the prefix's sums
     // ---- this CTA's slice of the dims ----
     int* flags = reinterpret_cast<int*>(sm + L::flags);
-    const float* part_ml = part + prefix_splits * rows_total * HD;
+    const float* part_ml = part + parts * rows_total * HD;
     for (int x = threadIdx.x; x < nrows * slice; x += kThreads) {
         const int row = x / slice, d = x - row * slice, idx = row0 + row, t = idx / G, head = kh * G + idx % G;
         const long long at = ((long long)b0 * a.tokens + t) * a.heads + head;
         float tm = -INFINITY, tl = 0.f, ta = 0.f;
         for (int r = 0; r < splits; ++r) tm = fmaxf(tm, sm[L::slice_ml + 2 * (r * R + row)]);
-        for (int r = 0; r < prefix_splits; ++r) tm = fmaxf(tm, __ldcg(part_ml + 2 * (r * rows_total + at)));
+        for (int r = 0; r < parts; ++r) tm = fmaxf(tm, __ldcg(part_ml + 2 * (r * rows_total + at)));
         const float safe = tm == -INFINITY ? 0.f : tm;
         for (int r = 0; r < splits; ++r) {
             const float e = exp2_fast(sm[L::slice_ml + 2 * (r * R + row)] - safe);
             tl += sm[L::slice_ml + 2 * (r * R + row) + 1] * e;
             ta += sm[L::slice + (r * R + row) * slice + d] * e;
         }
-        for (int r = 0; r < prefix_splits; ++r) {
+        for (int r = 0; r < parts; ++r) {
             const float2 ml = __ldcg(reinterpret_cast<const float2*>(part_ml + 2 * (r * rows_total + at)));
             const float e = exp2_fast(ml.x - safe);
             tl += ml.y * e;
@@ -319,7 +320,7 @@ attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict
 
 template <typename K>
 int launch(K* kernel, const b200gptq_attn_args& a, int smem, long long ctas, int cluster, bool pdl, float* part, int splits, int row_tiles,
-           int prefix_splits, cudaStream_t stream) {
+           int parts, cudaStream_t stream) {
     if (ctas > 0x7fffffff) return B200GPTQ_ERR_TOO_LARGE;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)ctas);
@@ -341,12 +342,12 @@ int launch(K* kernel, const b200gptq_attn_args& a, int smem, long long ctas, int
     }
     cfg.attrs = attr;
     cfg.numAttrs = n;
-    B200GPTQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a, part, splits, row_tiles, prefix_splits));
+    B200GPTQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a, part, splits, row_tiles, parts));
     return B200GPTQ_OK;
 }
 
 template <typename T, int HD, int MT, bool PREFIX>
-int run(const b200gptq_attn_args& a, float* part, const AttnSplit& s, cudaStream_t stream) {
+int run(const b200gptq_attn_args& a, float* part, const AttnPlan& s, cudaStream_t stream) {
     static std::once_flag once[64];
     static cudaError_t result[64];
     auto* kernel = attn_rows_kernel<T, HD, MT, PREFIX>;
@@ -359,14 +360,14 @@ int run(const b200gptq_attn_args& a, float* part, const AttnSplit& s, cudaStream
     const long long rows = (long long)a.tokens * (a.heads / a.kv_heads) * (PREFIX ? a.batch : 1);
     const int tiles = (int)((rows + 16 * MT - 1) / (16 * MT));
     const long long units = (long long)tiles * a.kv_heads * (PREFIX ? 1 : a.batch);
-    const int splits = PREFIX ? s.prefix : s.own;
-    return launch(kernel, a, smem, units * splits, PREFIX ? 1 : splits, attn_pdl_enabled(), part, splits, tiles, s.prefix, stream);
+    const int splits = PREFIX ? s.parts : s.own;
+    return launch(kernel, a, smem, units * splits, PREFIX ? 1 : splits, attn_pdl_enabled(), part, splits, tiles, s.parts, stream);
 }
 
 template <typename T, int HD>
-int run_all(const b200gptq_attn_args& a, float* part, const AttnSplit& s, cudaStream_t stream) {
+int run_all(const b200gptq_attn_args& a, float* part, const AttnPlan& s, cudaStream_t stream) {
     const long long per_sequence = (long long)a.tokens * (a.heads / a.kv_heads);
-    if (a.prefix) {
+    if (a.prefix && !s.prefix_tiles) {
         const int st = per_sequence * a.batch <= 16 ? run<T, HD, 1, true>(a, part, s, stream) : run<T, HD, 2, true>(a, part, s, stream);
         if (st != B200GPTQ_OK) return st;
     }
@@ -375,21 +376,7 @@ int run_all(const b200gptq_attn_args& a, float* part, const AttnSplit& s, cudaSt
 
 }  // namespace
 
-// How far the key ranges are split.  A CTA fills an SM, so as many as the SMs hold, as long as every warp has a block of keys.
-AttnSplit attn_rows_split(const b200gptq_attn_args& a) {
-    AttnSplit s = {1, 0};
-    const long long rows = (long long)a.tokens * (a.heads / a.kv_heads), sms = sm_count();
-    const long long units = (rows <= 16 ? 1 : (rows + 31) / 32) * a.kv_heads * a.batch;
-    const long long keys = a.window ? std::min<long long>(a.max_seq, (long long)a.window + a.sinks + a.tokens) : a.max_seq;
-    while (s.own < kMaxSplit && units * s.own * 2 <= sms && keys > s.own * kWarps * kBlock) s.own *= 2;
-    if (a.prefix) {
-        const long long all = rows * a.batch, tiles = (all <= 16 ? 1 : (all + 31) / 32) * a.kv_heads;
-        s.prefix = (int)std::max<long long>(1, std::min<long long>(std::min<long long>(2 * sms / tiles, 64), a.prefix / (kWarps * kBlock)));
-    }
-    return s;
-}
-
-int attn_rows_dispatch(const b200gptq_attn_args& a, float* part, const AttnSplit& s, cudaStream_t stream) {
+int attn_rows_dispatch(const b200gptq_attn_args& a, float* part, const AttnPlan& s, cudaStream_t stream) {
     if (a.dtype == B200GPTQ_F16) return a.hd == 128 ? run_all<__half, 128>(a, part, s, stream) : run_all<__half, 64>(a, part, s, stream);
     return a.hd == 128 ? run_all<__nv_bfloat16, 128>(a, part, s, stream) : run_all<__nv_bfloat16, 64>(a, part, s, stream);
 }

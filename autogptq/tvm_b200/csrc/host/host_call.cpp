@@ -537,6 +537,10 @@ PyObject* attn_checked(PyObject* const* args) {
     const at::Device on(at::kCUDA, (c10::DeviceIndex)device);
     const c10::cuda::OptionalCUDAGuard guard(c10::cuda::current_device() != device ? std::optional<at::Device>(on) : std::nullopt);
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
+    Scratch ws;                 // (for its status word: what a wait that runs out raises)
+    if (!scratch_for(device, stream, B200GPTQ_STATUS_BYTES, &ws)) return nullptr;
+    const Held owner(ws.owner);
+    a.status = reinterpret_cast<unsigned int*>(static_cast<char*>(ws.ptr) + B200GPTQ_STATUS_BYTES) - 1;
     at::Tensor out, scratch;
     int st;
     {

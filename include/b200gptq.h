@@ -88,6 +88,7 @@ B200GPTQ_API size_t b200gptq_workspace_bytes(int op, int M, int K, int N, int bi
  * stream.  0 = no wait ever ran out since the buffer was zero-filled.  (The word is the last 32-bit word of
  * the first 16 KiB of the buffer; b200gptq_gemv_static_status is the same query for the scratch built into the library.)
  */
+#define B200GPTQ_STATUS_BYTES 16384
 B200GPTQ_API int b200gptq_workspace_status(const void* workspace, void* stream, unsigned int* host_out);
 
 /*
@@ -447,6 +448,7 @@ B200GPTQ_API int b200gptq_pick_final(const void* slots, int rows, int world, lon
  *              out is left as it was there
  *   strides    in elements, multiples of 8: q and out {batch, token, head}, caches {batch, head, row}, prefix {head, row}; the last
  *              dimension is dense.  All addresses 16-byte aligned.  out overlaps nothing that is read
+ *   status      device word (b200gptq_workspace_status's, or any) that a bounded wait which runs out sets to 1, or NULL
  * b200gptq_attn_workspace_bytes: scratch of a call (0 without a prefix; its contents on entry do not matter and nothing is kept there, so
  * calls that may overlap need scratch of their own).  Negative: a B200GPTQ_ERR_* code for the sizes.
  */
@@ -454,6 +456,7 @@ typedef struct {
     const void *q, *k_cache, *v_cache, *k_prefix, *v_prefix;
     void* out;
     const int64_t *pos, *counts;
+    unsigned int* status;
     int64_t q_stride[3], out_stride[3], k_stride[3], v_stride[3], k_prefix_stride[2], v_prefix_stride[2];
     int dtype, batch, tokens, heads, kv_heads, hd, max_seq, prefix, window, sinks, pos_each;
     float scale;
