@@ -44,10 +44,8 @@ AttnPlan plan_of(const b200gptq_attn_args& a) {
     if (a.prefix) {
         p.prefix_tiles = all > 32 && attn_tiles_maps(a, true);
         if (p.prefix_tiles) {
-            const bool pairs = all <= 128;            // two runs of each CTA
-            const long long tiles = (a.prefix + 127) / 128, ctas = (all + 255) / 256 * a.kv_heads;
-            const long long splits = std::max<long long>(1, std::min(sms / ctas, tiles / 2));
-            p.parts = (int)(pairs ? 2 * splits : splits);
+            const long long units = (a.prefix + kAttnTilesKeys - 1) / kAttnTilesKeys, ctas = (all + 255) / 256 * a.kv_heads;
+            p.parts = (int)std::max<long long>(1, std::min(sms / ctas, units / 4));
         } else {
             const long long ctas = (all <= 16 ? 1 : (all + 31) / 32) * a.kv_heads;
             p.parts = (int)std::max<long long>(1, std::min<long long>(std::min<long long>(2 * sms / ctas, 64), a.prefix / kAttnRowsKeys));

@@ -11,7 +11,7 @@ namespace b200gptq {
 // prefix goes before it in `parts` runs (sums in scratch), by the tcgen05 kernel (prefix_tiles) or by the rows kernel.
 struct AttnPlan { bool tiles, prefix_tiles; int own, parts; };
 
-constexpr int kAttnMaxSplit = 8, kAttnRowsKeys = 128;      // CTAs of a cluster, keys that all warps of a CTA take at once (rows kernel)
+constexpr int kAttnMaxSplit = 8, kAttnRowsKeys = 128, kAttnTilesKeys = 64;      // CTAs of a cluster, keys that all warps of a CTA take at once (rows kernel), keys per unit (tcgen05)
 
 bool attn_pdl_enabled();
 

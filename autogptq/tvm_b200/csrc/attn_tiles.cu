@@ -2,24 +2,27 @@
 //
 //   S = Q K^T,  w = softmax(scale S) over the visible keys,  O = w V
 //
-// A CTA takes two tiles of 128 rows of Q that share a key head (rows are (token, head of the group), so that shared key heads fill a tile) and streams tiles
-// of 128 keys that either of them sees: 2 hd multiplications and one exponential per row and key, and of the latter an SM makes 16 per clock where the
-// tensor cores make 4096 of the former, so for 128 dims both take as long and have to run at once:
+// A CTA takes two tiles of 128 rows of Q that share a key head (rows are (token, head of the group), so that shared key heads fill a tile) and streams units
+// of 64 keys that either of them sees: 2 hd multiplications and one exponential per row and key, and of the latter an SM makes 16 per clock where the
+// tensor cores make 4096 of the former, so for 128 dims both take as long (512 clk per unit and tile of Q) and have to run at once:
 //
 //   warps 0..3, 4..7  softmax of one tile of Q each, a thread per row: S from tensor memory into registers, the weights (16 bits) back over it.  O is
 //                     only rescaled when a row's maximum grows by more than 2^8 over the one in use (no weight is above 2^8; fp32 sums)
-//   warp 8            TMA: K and V tiles into a ring, in the order K0 V0 K1 V1 ..
-//   warp 9            tcgen05.mma: PV of one tile of Q and QK of its next keys while the other tile's softmax runs.  Products are retired in order, so
-//                     that S of the next keys may overwrite the weights, and the arrival of S says that O is complete up to the keys before
+//   warp 8            TMA: K and V of the units into a ring, in the order in which they are multiplied, K0 K1 V0 K2 V1 ..
+//   warps 9, 10       tcgen05.mma for one tile of Q each: S of the unit after next as soon as the weights of this one have been multiplied, so that the
+//                     softmax always finds the next S there and waits for no product
 //
-// Tensor memory: S of both tiles (2 x 128 columns; the weights lie over the first 64), O of both (2 x hd).  The weights are the A operand from
+// Units of 128 keys with one S per tile of Q, so that softmax and products of a tile took turns, took 3900 to 4600 clk per 128 keys, with two threads per
+// row (which exchange its maximum) 4100: 1550 of them the products, 2500 the softmax.
+//
+// Tensor memory: two S per tile of Q (64 columns each; the weights lie over the first 32), O of both (2 x hd).  The weights are the A operand from
 // tensor memory, V is the B operand as it lies (MN-major, keys along K).
 //
 // Rows of V that no row of the tiles sees are zeroed in shared memory before they are multiplied (a weight of zero times a NaN is one).  Where rows of the
 // tiles see different keys and one of these holds a NaN or an infinity, the rows that come out not finite are done again, key by key.
 //
 // PACKED: the rows are (sequence, token, head of the group) of the whole batch against the shared prefix, split over CTAs, sums to scratch.  Up to 128 rows: both
-// tiles of Q are the same rows, one takes the even tiles of keys and the other the odd ones.
+// tiles of Q are the same rows, one takes the even units of keys and the other the odd ones.
 #include <cuda.h>
 
 #include <algorithm>
@@ -33,12 +36,13 @@
 namespace b200gptq {
 namespace {
 
-constexpr int kRows = 128, kKeys = 128, kLoadWarp = 8, kMmaWarp = 9, kThreads = 320;
-constexpr int kTmemCols = 512, kColO = 256;          // S of tile q at 128 q, O at 256 + 128 q
+constexpr int kRows = 128, kKeys = kAttnTilesKeys, kSoftmaxWarps = 8, kLoadWarp = 8, kMmaWarp = 9, kThreads = 384;
+constexpr int kTmemCols = 512, kColO = 256;          // S of tile q, buffer b at 128 q + 64 b, O at 256 + 128 q
 constexpr float kGrow = 8.f;                         // log2 of what a maximum may grow before O is rescaled
 
 template <int HD> struct Smem {
-    static constexpr int tile = kKeys * HD * 2, stages = HD == 128 ? 4 : 6, q = 0, ring = 2 * tile, total = ring + stages * tile + 1024;
+    static constexpr int q_tile = kRows * HD * 2, unit = kKeys * HD * 2, stages = HD == 128 ? 8 : 10, ring = 2 * q_tile, total = ring + stages * unit + 1024;
+    static_assert(stages * unit >= 2 * kRows * HD * 4 || HD == 64, "");
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -119,6 +123,15 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
         "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
         ::"r"(taddr), B200GPTQ_I8(r, 0), B200GPTQ_I8(r, 8), B200GPTQ_I8(r, 16), B200GPTQ_I8(r, 24) : "memory");
 }
+// Pairs of fp32 in one instruction.
+__device__ __forceinline__ void fma2(float& x, float& y, float a, float b, float m, float c) {
+    asm("{\n\t.reg .b64 u, v, w;\n\tmov.b64 u, {%2, %3};\n\tmov.b64 v, {%4, %4};\n\tmov.b64 w, {%5, %5};\n\t"
+        "fma.rn.f32x2 u, u, v, w;\n\tmov.b64 {%0, %1}, u;\n\t}" : "=f"(x), "=f"(y) : "f"(a), "f"(b), "f"(m), "f"(c));
+}
+__device__ __forceinline__ void add2(float& x, float& y, float a, float b) {
+    asm("{\n\t.reg .b64 u, v;\n\tmov.b64 u, {%0, %1};\n\tmov.b64 v, {%2, %3};\n\tadd.rn.f32x2 u, u, v;\n\tmov.b64 {%0, %1}, u;\n\t}"
+        : "+f"(x), "+f"(y) : "f"(a), "f"(b));
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -139,7 +152,7 @@ struct TileArgs {
     b200gptq_attn_args a;
     float* part;
     float sl2;                // |scale| log2 e, and Q is negated where the scale is negative
-    int negate, pairs, splits, part_splits, prefix_tiles;
+    int negate, pairs, splits, prefix_units;
 };
 
 template <typename T, int HD, bool PACKED>
@@ -147,28 +160,37 @@ __global__ void __launch_bounds__(kThreads, 1)
 attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_kp,
                   const __grid_constant__ CUtensorMap map_vp, const __grid_constant__ TileArgs p) {
     using SM = Smem<HD>;
-    constexpr int ST = SM::stages, BOX = kKeys * 128, HALVES = HD / 64;
+    constexpr int ST = SM::stages, QBOX = kRows * 128, BOX = kKeys * 128, HALVES = HD / 64;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     uint8_t* base_ptr = smem_raw + (base - raw);
-    __shared__ __align__(8) uint64_t bars[2 * ST + 8];
+    __shared__ __align__(8) uint64_t bars[2 * ST + 15];
     __shared__ uint32_t tmem_base_holder;
     __shared__ volatile int abort_flag;
+    __shared__ float stats[2][2][kRows];         // [tile][maximum, denominator][row] (PACKED)
 
     const b200gptq_attn_args& a = p.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t bar_base = smem_u32(bars);
     auto full = [&](int s) { return bar_base + 8u * s; };
     auto empty = [&](int s) { return bar_base + 8u * (ST + s); };
-    auto q_full = [&](int q) { return bar_base + 8u * (2 * ST + q); };
-    auto s_full = [&](int q) { return bar_base + 8u * (2 * ST + 2 + q); };
-    auto p_full = [&](int q) { return bar_base + 8u * (2 * ST + 4 + q); };
-    auto o_full = [&](int q) { return bar_base + 8u * (2 * ST + 6 + q); };
+    auto s_full = [&](int q, int b) { return bar_base + 8u * (2 * ST + 2 * q + b); };
+    auto p_full = [&](int q, int b) { return bar_base + 8u * (2 * ST + 4 + 2 * q + b); };
+    auto q_full = [&](int q) { return bar_base + 8u * (2 * ST + 8 + q); };
+    auto o_done = [&](int q) { return bar_base + 8u * (2 * ST + 10 + q); };     // O has the unit's products
+    auto retired = [&](int q) { return bar_base + 8u * (2 * ST + 12 + q); };    // all products of the tile
+    const uint32_t all_met = bar_base + 8u * (2 * ST + 14);
 
     if (threadIdx.x == 0) {
         abort_flag = 0;
-        for (int s = 0; s < ST; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
-        for (int q = 0; q < 2; ++q) { mbar_init(q_full(q), 4); mbar_init(s_full(q), 1); mbar_init(p_full(q), 4); mbar_init(o_full(q), 1); }
+        for (int s = 0; s < ST; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 2); }
+        for (int q = 0; q < 2; ++q) {
+            for (int b = 0; b < 2; ++b) { mbar_init(s_full(q, b), 1); mbar_init(p_full(q, b), 4); }
+            mbar_init(q_full(q), 4);
+            mbar_init(o_done(q), 1);
+            mbar_init(retired(q), 1);
+        }
+        mbar_init(all_met, kSoftmaxWarps);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kMmaWarp) {
@@ -184,9 +206,9 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 
     // ---- which rows, which keys.  The last rows of a prompt see most, and come first. ----
     const int G = a.heads / a.kv_heads, window = a.window ? a.window : 1 << 30;
-    const int split = PACKED ? blockIdx.x % p.splits : 0, unit = PACKED ? blockIdx.x / p.splits : blockIdx.x;
-    const int kh = unit % a.kv_heads, b0 = PACKED ? 0 : unit / a.kv_heads % a.batch;
-    const int pair = p.pairs - 1 - unit / a.kv_heads / (PACKED ? 1 : a.batch), row0 = pair * 2 * kRows;
+    const int split = PACKED ? blockIdx.x % p.splits : 0, part_unit = PACKED ? blockIdx.x / p.splits : blockIdx.x;
+    const int kh = part_unit % a.kv_heads, b0 = PACKED ? 0 : part_unit / a.kv_heads % a.batch;
+    const int pair = p.pairs - 1 - part_unit / a.kv_heads / (PACKED ? 1 : a.batch), row0 = pair * 2 * kRows;
     const int pos0 = PACKED ? 0 : attn_pos(a, b0);
     const int rows_all = PACKED ? a.batch * a.tokens * G : attn_count(a, b0) * G;
     const bool alt = PACKED && rows_all <= kRows;       // both tiles are the same rows
@@ -198,53 +220,60 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         p_lo[q] = pos0 + r / G;
         p_hi[q] = pos0 + (r + max(nrows[q], 1) - 1) / G;
     }
-    int n_tiles = 0, n_s = 0, first = 0;
+    auto of = [](const int (&v)[2], int q) { return q ? v[1] : v[0]; };       // (registers, not an array that is indexed)
+    int n_units = 0, n_s = 0, first = 0;
     AttnRange range = {0, 0, 0};
     if (nrows[0] > 0) {
         if constexpr (PACKED) {
-            first = (int)((long long)p.prefix_tiles * split / p.splits);
-            n_tiles = (int)((long long)p.prefix_tiles * (split + 1) / p.splits) - first;
+            first = (int)((long long)p.prefix_units * split / p.splits);
+            n_units = (int)((long long)p.prefix_units * (split + 1) / p.splits) - first;
         } else {
             range = attn_range(p_lo[0], nrows[1] > 0 ? p_hi[1] : p_hi[0], window, a.sinks, a.max_seq);
             n_s = (range.s_end + kKeys - 1) / kKeys;
-            n_tiles = p.prefix_tiles + n_s + (range.w_end - range.w_start + kKeys - 1) / kKeys;
+            n_units = p.prefix_units + n_s + (range.w_end - range.w_start + kKeys - 1) / kKeys;
         }
     }
     struct Keys { int j0, end; bool prefix; };
     auto keys_at = [&](int i) {
         Keys k;
         if constexpr (PACKED) { k.prefix = true; k.j0 = (first + i) * kKeys; k.end = a.prefix; return k; }
-        k.prefix = i < p.prefix_tiles;
-        i -= p.prefix_tiles;
-        k.j0 = k.prefix ? (i + p.prefix_tiles) * kKeys : i < n_s ? i * kKeys : range.w_start + (i - n_s) * kKeys;
+        k.prefix = i < p.prefix_units;
+        i -= p.prefix_units;
+        k.j0 = k.prefix ? (i + p.prefix_units) * kKeys : i < n_s ? i * kKeys : range.w_start + (i - n_s) * kKeys;
         k.end = k.prefix ? a.prefix : i < n_s ? range.s_end : range.w_end;
         return k;
     };
     auto needs = [&](int q, int i) {          // whether any row of tile q sees any of the keys
-        if (nrows[q] <= 0) return false;
+        if (of(nrows, q) <= 0) return false;
         if (alt) return (i & 1) == q;
         if (PACKED) return true;
         const Keys k = keys_at(i);
-        return k.prefix || (k.j0 <= p_hi[q] && (k.j0 + kKeys - 1 > p_lo[q] - window || k.j0 < a.sinks));
+        return k.prefix || (k.j0 <= of(p_hi, q) && (k.j0 + kKeys - 1 > of(p_lo, q) - window || k.j0 < a.sinks));
+    };
+    // Load n of 2 n_units: K0 K1 V0 K2 V1 .. K(n - 1) V(n - 2) V(n - 1)
+    auto load_at = [&](int n, bool& value) {
+        value = n == 2 * n_units - 1 || (n > 0 && (n & 1) == 0);
+        return n == 2 * n_units - 1 ? n_units - 1 : value ? n / 2 - 1 : (n + 1) / 2;
     };
 
     bool ok = true;
     if (warp == kLoadWarp) {
         // ===== keys and values =====
         if (elect_one()) {
-            int n = 0;                        // loads issued: K i is number 2 i, V i number 2 i + 1
-            for (; n < 2 * n_tiles && ok; ++n) {
-                const int s = n % ST;
-                if (n >= ST) ok = mbar_wait(empty(s), (n / ST - 1) & 1, &abort_flag);
+            int n = 0;
+            for (int s = 0, round = 0; n < 2 * n_units; ++n) {
+                if (round > 0) ok = mbar_wait(empty(s), (round - 1) & 1, &abort_flag);
                 if (!ok) break;
-                const Keys k = keys_at(n / 2);
-                const uint32_t dst = base + SM::ring + s * SM::tile, bar = full(s);
-                mbar_expect(bar, SM::tile);
+                bool value;
+                const Keys k = keys_at(load_at(n, value));
+                const uint32_t dst = base + SM::ring + s * SM::unit, bar = full(s);
+                mbar_expect(bar, SM::unit);
 #pragma unroll
                 for (int h = 0; h < HALVES; ++h) {
-                    if (k.prefix) tma_3d(dst + h * BOX, (n & 1) ? &map_vp : &map_kp, 64 * h, k.j0, kh, bar);
-                    else tma_4d(dst + h * BOX, (n & 1) ? &map_v : &map_k, 64 * h, k.j0, kh, b0, bar);
+                    if (k.prefix) tma_3d(dst + h * BOX, value ? &map_vp : &map_kp, 64 * h, k.j0, kh, bar);
+                    else tma_4d(dst + h * BOX, value ? &map_v : &map_k, 64 * h, k.j0, kh, b0, bar);
                 }
+                if (++s == ST) { s = 0; ++round; }
             }
             if (!ok) {                        // what is on its way lands before the CTA ends
                 int never = 0;
@@ -252,98 +281,94 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             }
         }
         __syncwarp();
-    } else if (warp == kMmaWarp) {
-        // ===== products =====
+    } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
+        // ===== products of tile q, load by load =====
         constexpr uint32_t type = std::is_same<T, __half>::value ? 0u : 1u;
         constexpr uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(kRows >> 4) << 24);
         constexpr uint32_t idesc_qk = idesc | ((uint32_t)(kKeys >> 3) << 17), idesc_pv = idesc | (1u << 16) | ((uint32_t)(HD >> 3) << 17);
-        int started[2] = {0, 0}, mixed[2] = {0, 0};      // QK and PV issued
-        auto wait_load = [&](int n) { if (ok) ok = mbar_wait(full(n % ST), (n / ST) & 1, &abort_flag); ok = __all_sync(0xffffffffu, ok); };
-        auto release = [&](int n) { if (elect_one()) mma_commit(empty(n % ST)); __syncwarp(); };
-        auto qk = [&](int q, int i) {
-            if (started[q]++ == 0) {
-                ok = mbar_wait(q_full(alt ? 0 : q), 0, &abort_flag);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) return;
-            }
-            tc_after();
-            if (elect_one()) {
-                const uint64_t ad = smem_desc(base + SM::q + (alt ? 0 : q) * SM::tile, 0), bd = smem_desc(base + SM::ring + (2 * i) % ST * SM::tile, 0);
+        const int q = warp - kMmaWarp;
+        const uint64_t qd = smem_desc(base + (alt ? 0 : q) * SM::q_tile, 0);
+        const uint32_t ts = tmem + 128u * q, to = tmem + kColO + 128u * q;
+        auto wait = [&](uint32_t bar, int parity) {
+            ok = mbar_wait(bar, parity & 1, &abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+        };
+        int started = 0, mixed = 0;           // S begun, weights multiplied
+        for (int n = 0, s = 0, round = 0; n < 2 * n_units; ++n) {
+            bool value;
+            const int i = load_at(n, value);
+            wait(full(s), round);
+            if (!ok) break;
+            const uint32_t at = base + SM::ring + s * SM::unit;
+            if (!needs(q, i)) {
+                if (lane == 0) mbar_arrive(empty(s));
+            } else if (!value) {
+                if (started == 0) wait(q_full(alt ? 0 : q), 0);
+                if (!ok) break;
+                tc_after();
+                if (elect_one()) {
+                    const uint64_t kd = smem_desc(at, 0);
 #pragma unroll
-                for (int k = 0; k < HD / 16; ++k) {
-                    const uint32_t off = (k / 4 * BOX + k % 4 * 32) >> 4;
-                    mma_ss(tmem + 128u * q, ad + off, bd + off, idesc_qk, k > 0 ? 1u : 0u);
+                    for (int k = 0; k < HD / 16; ++k)
+                        mma_ss(ts + 64u * (started & 1), qd + ((k / 4 * QBOX + k % 4 * 32) >> 4), kd + ((k / 4 * BOX + k % 4 * 32) >> 4), idesc_qk, k > 0 ? 1u : 0u);
+                    mma_commit(s_full(q, started & 1));
+                    mma_commit(empty(s));
                 }
-                mma_commit(s_full(q));
+                ++started;
+            } else {
+                const Keys k = keys_at(i);
+                if (k.j0 + kKeys > k.end) {   // rows that nobody sees (both warps write the same zeros)
+                    for (int x = lane; x < (k.j0 + kKeys - k.end) * HALVES * 8; x += 32) {
+                        const int r = k.end - k.j0 + x / (HALVES * 8), c = x % (HALVES * 8);
+                        *reinterpret_cast<uint4*>(base_ptr + (at - base) + (c / 8) * BOX + r * 128 + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                }
+                wait(p_full(q, mixed & 1), mixed >> 1);
+                if (!ok) break;
+                tc_after();
+                if (elect_one()) {
+                    const uint64_t vd = smem_desc(at, BOX);
+#pragma unroll
+                    for (int k = 0; k < kKeys / 16; ++k)
+                        mma_ts(to, ts + 64u * (mixed & 1) + 8u * k, vd + k * (2048 >> 4), idesc_pv, (mixed > 0 || k > 0) ? 1u : 0u);
+                    mma_commit(empty(s));
+                    mma_commit(o_done(q));
+                }
+                ++mixed;
             }
             __syncwarp();
-        };
-        if (n_tiles > 0) {
-            wait_load(0);
-            for (int q = 0; q < 2 && ok; ++q)
-                if (needs(q, 0)) qk(q, 0);
-            release(0);
+            if (++s == ST) { s = 0; ++round; }
         }
-        for (int i = 0; i < n_tiles && ok; ++i) {
-            const int v = 2 * i + 1, s = v % ST;
-            const uint32_t vt = base + SM::ring + s * SM::tile;
-            wait_load(v);
-            if (!ok) break;
-            const Keys k = keys_at(i);
-            if (k.j0 + kKeys > k.end) {       // rows that nobody sees
-                for (int x = lane; x < (k.j0 + kKeys - k.end) * HALVES * 8; x += 32) {
-                    const int r = k.end - k.j0 + x / (HALVES * 8), c = x % (HALVES * 8);
-                    *reinterpret_cast<uint4*>(base_ptr + (vt - base) + (c / 8) * BOX + r * 128 + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-            }
-            for (int q = 0; q < 2 && ok; ++q) {
-                if (needs(q, i)) {
-                    ok = mbar_wait(p_full(q), mixed[q] & 1, &abort_flag);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    tc_after();
-                    if (elect_one()) {
-                        const uint64_t bd = smem_desc(vt, BOX);
-#pragma unroll
-                        for (int k16 = 0; k16 < kKeys / 16; ++k16)
-                            mma_ts(tmem + kColO + 128u * q, tmem + 128u * q + 8u * k16, bd + k16 * (2048 >> 4), idesc_pv, (mixed[q] > 0 || k16 > 0) ? 1u : 0u);
-                    }
-                    __syncwarp();
-                    ++mixed[q];
-                }
-                if (i + 1 < n_tiles) {
-                    wait_load(v + 1);
-                    if (ok && needs(q, i + 1)) qk(q, i + 1);
-                }
-            }
-            if (!ok) break;
-            release(v);
-            if (i + 1 < n_tiles) release(v + 1);
-        }
-        if (elect_one()) { mma_commit(o_full(0)); mma_commit(o_full(1)); }
+        if (elect_one()) mma_commit(retired(q));
         __syncwarp();
         int never = 0;                        // (also after a wait that ran out: nothing is in flight when tensor memory is freed)
-        mbar_wait(o_full(1), 0, &never);
-    } else {
+        mbar_wait(retired(q), 0, &never);
+    } else if (warp < kSoftmaxWarps) {
         // ===== softmax of tile q, one row per thread =====
-        const int q = warp >> 2, r = threadIdx.x & 127, rows = nrows[q], row_first = row0 + (alt ? 0 : q * kRows);
-        const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16, ts = tmem + 128u * q + lane_off, to = tmem + kColO + 128u * q + lane_off;
-        const bool mine = 32 * (warp & 3) < rows;       // the warp has rows at all
-        // Q, in the swizzled layout of the tiles
+        const int q = warp >> 2, quarter = warp & 3, r = 32 * quarter + lane, rows = of(nrows, q), row_first = row0 + (alt ? 0 : q * kRows);
+        const uint32_t lane_off = (uint32_t)(32 * quarter) << 16, ts = tmem + 128u * q + lane_off, to = tmem + kColO + 128u * q + lane_off;
+        const bool mine = 32 * quarter < rows;          // the warp has rows at all
+        // Q, in the swizzled layout of the tiles: 16 bytes per thread and turn, eight of them on their way at once
         if (!(alt && q == 1)) {
-            uint8_t* dst = base_ptr + SM::q + q * SM::tile;
-            for (int x = lane; x < 32 * HD / 8; x += 32) {
-                const int rr = 32 * (warp & 3) + x / (HD / 8), c = x % (HD / 8);
-                uint4 val = make_uint4(0, 0, 0, 0);
-                if (rr < rows) {
-                    const int idx = row_first + rr, tok = idx / G, head = kh * G + idx - tok * G;
+            uint8_t* dst = base_ptr + q * SM::q_tile;
+#pragma unroll 1
+            for (int x0 = 0; x0 < HD / 8; x0 += 8) {
+                uint4 val[8];
+#pragma unroll
+                for (int x = 0; x < 8; ++x) {
+                    const int rr = 32 * quarter + ((x0 + x) * 32 + lane) / (HD / 8), c = lane % (HD / 8), idx = row_first + rr, tok = idx / G, head = kh * G + idx - tok * G;
                     const int b = PACKED ? tok / a.tokens : b0, t = PACKED ? tok - b * a.tokens : tok;
-                    val = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + b * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2] + 8 * c));
-                    if (p.negate) { val.x ^= 0x80008000u; val.y ^= 0x80008000u; val.z ^= 0x80008000u; val.w ^= 0x80008000u; }
+                    val[x] = make_uint4(0, 0, 0, 0);
+                    if (rr < rows) val[x] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + b * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2] + 8 * c));
                 }
-                *reinterpret_cast<uint4*>(dst + (c / 8) * BOX + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = val;
+#pragma unroll
+                for (int x = 0; x < 8; ++x) {
+                    const int rr = 32 * quarter + ((x0 + x) * 32 + lane) / (HD / 8), c = lane % (HD / 8);
+                    if (p.negate) { val[x].x ^= 0x80008000u; val[x].y ^= 0x80008000u; val[x].z ^= 0x80008000u; val[x].w ^= 0x80008000u; }
+                    *reinterpret_cast<uint4*>(dst + (c / 8) * QBOX + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = val[x];
+                }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -352,22 +377,23 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         const int pr = pos0 + (row_first + min(r, max(rows, 1) - 1)) / G;
         float m = -INFINITY, l = 0.f;           // the maximum in use (of scores, not scaled), the denominator
         int turn = 0;
-        for (int i = 0; i < n_tiles; ++i) {
+        for (int i = 0; i < n_units; ++i) {
             if (!needs(q, i)) continue;
-            ok = mbar_wait(s_full(q), turn & 1, &abort_flag);
+            const uint32_t tb = ts + 64u * (turn & 1);
+            ok = mbar_wait(s_full(q, turn & 1), (turn >> 1) & 1, &abort_flag);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_after();
             if (mine) {
-                uint32_t s[4][32];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32u * c, s[c]);
+                uint32_t s[2][32];
+                tmem_ld32(tb, s[0]);
+                tmem_ld32(tb + 32u, s[1]);
                 tmem_wait_ld();
-#pragma unroll
-                for (int c = 0; c < 4; ++c) after_wait(s[c]);
+                after_wait(s[0]);
+                after_wait(s[1]);
                 const Keys k = keys_at(i);
                 bool whole = k.j0 + kKeys <= k.end;
-                if (!k.prefix) whole = whole && k.j0 + kKeys - 1 <= p_lo[q] && (k.j0 > p_hi[q] - window || k.j0 + kKeys <= a.sinks);
+                if (!k.prefix) whole = whole && k.j0 + kKeys - 1 <= of(p_lo, q) && (k.j0 > of(p_hi, q) - window || k.j0 + kKeys <= a.sinks);
                 if (!whole) {
                     // columns [0, front) and [lo, hi) are seen
                     int front = k.end - k.j0, lo = 0, hi = 0;
@@ -377,19 +403,17 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                         hi = min(pr + 1, k.end) - k.j0;
                     }
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            const int x = 32 * c + e;
-                            if (!(x < front || (x >= lo && x < hi))) s[c][e] = 0xff800000u;       // -infinity
-                        }
+                    for (int x = 0; x < kKeys; ++x)
+                        if (!(x < front || (x >= lo && x < hi))) s[x / 32][x % 32] = 0xff800000u;       // -infinity
                 }
                 float top[4];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    top[c] = __uint_as_float(s[c][0]);
+                for (int g = 0; g < 4; ++g) {
+                    top[g] = __uint_as_float(s[g / 2][g % 2 * 16]);
 #pragma unroll
-                    for (int e = 1; e < 32; ++e) top[c] = fmaxf(top[c], __uint_as_float(s[c][e]));
+                    for (int e = 1; e < 15; e += 2)
+                        top[g] = fmaxf(top[g], fmaxf(__uint_as_float(s[g / 2][g % 2 * 16 + e]), __uint_as_float(s[g / 2][g % 2 * 16 + e + 1])));
+                    top[g] = fmaxf(top[g], __uint_as_float(s[g / 2][g % 2 * 16 + 15]));
                 }
                 const float up = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
                 const bool grow = up > m && (m == -INFINITY || (up - m) * p.sl2 > kGrow);
@@ -397,6 +421,10 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                     const float corr = grow ? exp2_fast((m - up) * p.sl2) : 1.f;
                     if (grow) { m = up; l *= corr; }
                     if (turn > 0) {             // (the first products overwrite O)
+                        ok = mbar_wait(o_done(q), (turn - 1) & 1, &abort_flag);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        tc_after();
                         uint32_t o[32];
 #pragma unroll 1
                         for (int c = 0; c < HD / 32; ++c) {
@@ -411,97 +439,119 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                 }
                 const float off = m == -INFINITY ? 0.f : -m * p.sl2;
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                uint32_t w[32];
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    uint32_t w[32];
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        const int c = 2 * half + e / 16;
-                        const float x0 = exp2_fast(fmaf(__uint_as_float(s[c][e % 16 * 2]), p.sl2, off));
-                        const float x1 = exp2_fast(fmaf(__uint_as_float(s[c][e % 16 * 2 + 1]), p.sl2, off));
-                        sum[e & 1] += x0;
-                        sum[2 + (e & 1)] += x1;
-                        w[e] = Half<T>::pack(x0, x1);
-                    }
-                    tmem_st32(ts + 32u * half, w);
+                for (int e = 0; e < 32; ++e) {
+                    float x0, x1;
+                    fma2(x0, x1, __uint_as_float(s[e / 16][e % 16 * 2]), __uint_as_float(s[e / 16][e % 16 * 2 + 1]), p.sl2, off);
+                    x0 = exp2_fast(x0);
+                    x1 = exp2_fast(x1);
+                    add2(sum[2 * (e & 1)], sum[2 * (e & 1) + 1], x0, x1);
+                    w[e] = Half<T>::pack(x0, x1);
                 }
+                tmem_st32(tb, w);
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 tmem_wait_st();
             }
             tc_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(p_full(q));
+            if (lane == 0) mbar_arrive(p_full(q, turn & 1));
             ++turn;
         }
         // ---- O ----
-        if (ok && rows > 0) {
-            if (turn > 0) {
-                ok = mbar_wait(o_full(q), 0, &abort_flag);
-                ok = __all_sync(0xffffffffu, ok);
-            }
+        if (ok && turn > 0) {
+            ok = mbar_wait(retired(q), 0, &abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+        }
+        tc_after();
+        const long long rows_total = (long long)a.batch * a.tokens * a.heads;
+        if constexpr (PACKED) {
+            // Sums in fp32, through shared memory so that rows are written whole (with one thread per row 4 us more); up to 128 rows both tiles add up.  For 128
+            // dims the tiles lie where the ring was, for 64 over Q too: what each tile multiplies has been multiplied when both have met here.
+            constexpr int CH = HD / 4;          // 16-byte pieces of a row
+            float4* stage = reinterpret_cast<float4*>(base_ptr + (HD == 128 ? SM::ring : 0));
+            tc_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(all_met);
+            if (ok) ok = mbar_wait(all_met, 0, &abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
             tc_after();
-            const long long rows_total = (long long)a.batch * a.tokens * a.heads;
-            const float inv = l != 0.f ? 1.f / l : 0.f;
-            bool bad = false;
-            uint8_t* stage = base_ptr + SM::q + q * SM::tile;            // (the products with Q are done)
-            const int idx = row_first + min(r, rows - 1);
-            const long long at = (PACKED ? (alt ? 2 * split + q : split) * rows_total : 0LL) + (long long)(idx / G) * a.heads + kh * G + idx % G;
-            if (ok && mine)
+            if (ok && mine) {
+                stats[q][0][r] = m * p.sl2;
+                stats[q][1][r] = l;
 #pragma unroll 1
                 for (int c = 0; c < HD / 32; ++c) {
                     uint32_t o[32];
-                    if (turn > 0) {
-                        tmem_ld32(to + 32u * c, o);
-                        tmem_wait_ld();
-                        after_wait(o);
-                    } else {
+                    tmem_ld32(to + 32u * c, o);
+                    tmem_wait_ld();
+                    after_wait(o);
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = 0u;
-                    }
-                    if constexpr (PACKED) {
-                        if (r < rows) {
-                            float4* dst = reinterpret_cast<float4*>(p.part + at * HD + 32 * c);
-#pragma unroll
-                            for (int e = 0; e < 8; ++e)
-                                dst[e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            float f[8];
-#pragma unroll
-                            for (int x = 0; x < 8; ++x) {
-                                // (nothing seen: zero; a NaN or an infinity in V that the row does not see: done again below)
-                                f[x] = l == 0.f ? 0.f : __uint_as_float(o[8 * e + x]) * inv;
-                                bad = bad || !isfinite(f[x]);
-                            }
-                            const uint4 h = make_uint4(Half<T>::pack(f[0], f[1]), Half<T>::pack(f[2], f[3]), Half<T>::pack(f[4], f[5]), Half<T>::pack(f[6], f[7]));
-                            const int chunk = 4 * c + e;
-                            *reinterpret_cast<uint4*>(stage + r * HD * 2 + ((chunk ^ (r & 7)) << 4)) = h;
-                        }
+                    for (int e = 0; e < 8; ++e) {
+                        float4 f = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
+                        if (turn == 0) f = make_float4(0.f, 0.f, 0.f, 0.f);       // (no keys)
+                        stage[(q * kRows + r) * CH + ((8 * c + e) ^ (r & 7))] = f;
                     }
                 }
-            if constexpr (PACKED) {
-                if (ok && r < rows) {
-                    float* ml = p.part + p.part_splits * rows_total * HD + 2 * at;
-                    ml[0] = m * p.sl2;
-                    ml[1] = l;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(all_met);
+            if (ok) ok = mbar_wait(all_met, 1, &abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+            float* ml = p.part + p.splits * rows_total * HD;
+            const int all = alt ? nrows[0] : nrows[0] + nrows[1];
+            for (int x = threadIdx.x; ok && x < all * CH; x += kSoftmaxWarps * 32) {
+                const int row = x / CH, chunk = x % CH, idx = row0 + row;
+                const long long at = split * rows_total + (long long)(idx / G) * a.heads + kh * G + idx % G;
+                float4 f = stage[row * CH + (chunk ^ (row & 7))];
+                float tm = stats[row / kRows][0][row % kRows], tl = stats[row / kRows][1][row % kRows];
+                if (alt) {
+                    const float4 g = stage[(kRows + row) * CH + (chunk ^ (row & 7))];
+                    const float um = stats[1][0][row], both = fmaxf(tm, um), safe = both == -INFINITY ? 0.f : both, e0 = exp2_fast(tm - safe), e1 = exp2_fast(um - safe);
+                    f = make_float4(f.x * e0 + g.x * e1, f.y * e0 + g.y * e1, f.z * e0 + g.z * e1, f.w * e0 + g.w * e1);
+                    tl = tl * e0 + stats[1][1][row] * e1;
+                    tm = both;
                 }
-            } else {
-                __syncwarp();                   // (a warp stores its own rows)
-                const int last = min(32, rows - 32 * (warp & 3));
-                for (int x = lane; ok && x < last * (HD / 8); x += 32) {
-                    const int rr = 32 * (warp & 3) + x / (HD / 8), c = x % (HD / 8), id = row_first + rr, t = id / G, head = kh * G + id - t * G;
-                    *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + b0 * a.out_stride[0] + t * a.out_stride[1] + head * a.out_stride[2] + 8 * c) =
-                        *reinterpret_cast<const uint4*>(stage + rr * HD * 2 + ((c ^ (rr & 7)) << 4));
+                *reinterpret_cast<float4*>(p.part + at * HD + 4 * chunk) = f;
+                if (chunk == 0) *reinterpret_cast<float2*>(ml + 2 * at) = make_float2(tm, tl);
+            }
+        } else if (ok && mine) {
+            const float inv = l != 0.f ? 1.f / l : 0.f;
+            bool bad = false;
+            uint8_t* stage = base_ptr + q * SM::q_tile;                  // (the products with Q are done; a warp stores what it has staged)
+#pragma unroll 1
+            for (int c = 0; c < HD / 32; ++c) {
+                uint32_t o[32];
+                if (turn > 0) {
+                    tmem_ld32(to + 32u * c, o);
+                    tmem_wait_ld();
+                    after_wait(o);
                 }
-                __syncwarp();
-                unsigned again = __ballot_sync(0xffffffffu, bad && r < rows && ok);
-                while (again) {
-                    const int rr = 32 * (warp & 3) + __ffs(again) - 1, id = row_first + rr, t = id / G;
-                    again &= again - 1;
-                    attn_row_again<T, HD>(a, b0, t, kh * G + id - t * G, pos0 + t, 0, HD);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float f[8];
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) {
+                        // (nothing seen: zero; a NaN or an infinity in V that the row does not see: done again below)
+                        f[x] = turn == 0 || l == 0.f ? 0.f : __uint_as_float(o[8 * e + x]) * inv;
+                        bad = bad || !isfinite(f[x]);
+                    }
+                    const uint4 h = make_uint4(Half<T>::pack(f[0], f[1]), Half<T>::pack(f[2], f[3]), Half<T>::pack(f[4], f[5]), Half<T>::pack(f[6], f[7]));
+                    *reinterpret_cast<uint4*>(stage + r * HD * 2 + (((4 * c + e) ^ (r & 7)) << 4)) = h;
                 }
+            }
+            __syncwarp();
+            const int last = min(32, rows - 32 * quarter);
+            for (int x = lane; x < last * (HD / 8); x += 32) {
+                const int rr = 32 * quarter + x / (HD / 8), c = x % (HD / 8), id = row_first + rr, t = id / G, head = kh * G + id - t * G;
+                *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + b0 * a.out_stride[0] + t * a.out_stride[1] + head * a.out_stride[2] + 8 * c) =
+                    *reinterpret_cast<const uint4*>(stage + rr * HD * 2 + ((c ^ (rr & 7)) << 4));
+            }
+            __syncwarp();
+            unsigned again = __ballot_sync(0xffffffffu, bad && r < rows);
+            while (again) {
+                const int rr = 32 * quarter + __ffs(again) - 1, id = row_first + rr, t = id / G;
+                again &= again - 1;
+                attn_row_again<T, HD>(a, b0, t, kh * G + id - t * G, pos0 + t, 0, HD);
             }
         }
     }
@@ -526,7 +576,7 @@ bool encode(CUtensorMap* m, bool bf16, int hd, const void* ptr, int rank, const 
 }
 
 template <typename T, int HD, bool PACKED>
-int run(const b200gptq_attn_args& a, float* part, int splits, int part_splits, cudaStream_t stream) {
+int run(const b200gptq_attn_args& a, float* part, int splits, cudaStream_t stream) {
     static std::once_flag once[64];
     static cudaError_t result[64];
     auto* kernel = attn_tiles_kernel<T, HD, PACKED>;
@@ -551,8 +601,7 @@ int run(const b200gptq_attn_args& a, float* part, int splits, int part_splits, c
     t.sl2 = std::max(std::fabs(a.scale) * kLog2e, 1e-30f);        // (a scale of zero: all weights alike, and no infinity times zero)
     t.negate = a.scale < 0.f;
     t.splits = splits;
-    t.part_splits = part_splits;
-    t.prefix_tiles = (int)((a.prefix + kKeys - 1) / kKeys);
+    t.prefix_units = (int)((a.prefix + kKeys - 1) / kKeys);
     const long long rows = (long long)a.tokens * (a.heads / a.kv_heads) * (PACKED ? a.batch : 1);
     t.pairs = (int)((rows + 2 * kRows - 1) / (2 * kRows));
     const long long ctas = (long long)t.pairs * a.kv_heads * (PACKED ? splits : a.batch);
@@ -572,10 +621,10 @@ int run(const b200gptq_attn_args& a, float* part, int splits, int part_splits, c
 }
 
 template <bool PACKED>
-int run_any(const b200gptq_attn_args& a, float* part, int splits, int part_splits, cudaStream_t stream) {
+int run_any(const b200gptq_attn_args& a, float* part, int splits, cudaStream_t stream) {
     if (a.dtype == B200GPTQ_F16)
-        return a.hd == 128 ? run<__half, 128, PACKED>(a, part, splits, part_splits, stream) : run<__half, 64, PACKED>(a, part, splits, part_splits, stream);
-    return a.hd == 128 ? run<__nv_bfloat16, 128, PACKED>(a, part, splits, part_splits, stream) : run<__nv_bfloat16, 64, PACKED>(a, part, splits, part_splits, stream);
+        return a.hd == 128 ? run<__half, 128, PACKED>(a, part, splits, stream) : run<__half, 64, PACKED>(a, part, splits, stream);
+    return a.hd == 128 ? run<__nv_bfloat16, 128, PACKED>(a, part, splits, stream) : run<__nv_bfloat16, 64, PACKED>(a, part, splits, stream);
 }
 
 }  // namespace
@@ -592,12 +641,8 @@ bool attn_tiles_maps(const b200gptq_attn_args& a, bool prefix) {
     return true;
 }
 
-int attn_tiles_dispatch(const b200gptq_attn_args& a, cudaStream_t stream) { return run_any<false>(a, nullptr, 1, 0, stream); }
+int attn_tiles_dispatch(const b200gptq_attn_args& a, cudaStream_t stream) { return run_any<false>(a, nullptr, 1, stream); }
 
-// `parts` sums per row: runs of the prefix, or two of each (up to 128 rows).
-int attn_tiles_prefix(const b200gptq_attn_args& a, float* part, int parts, cudaStream_t stream) {
-    const bool alt = (long long)a.batch * a.tokens * (a.heads / a.kv_heads) <= kRows;
-    return run_any<true>(a, part, alt ? parts / 2 : parts, parts, stream);
-}
+int attn_tiles_prefix(const b200gptq_attn_args& a, float* part, int parts, cudaStream_t stream) { return run_any<true>(a, part, parts, stream); }
 
 }  // namespace b200gptq
