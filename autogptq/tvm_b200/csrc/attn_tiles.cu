@@ -8,7 +8,7 @@
 //
 //   warps 0..3, 4..7  softmax of one tile of Q each, a thread per row: S from tensor memory into registers, the weights (16 bits) back over it.  O is
 //                     only rescaled when a row's maximum grows by more than 2^8 over the one in use (no weight is above 2^8; fp32 sums)
-//   warp 8            TMA: K and V of the units into a ring, in the order in which they are multiplied, K0 K1 V0 K2 V1 ..
+//   warp 8            TMA: K and V of the units into a ring, in the order in which they are multiplied: K0 and K1, V0 and K2, V1 and K3 ..
 //   warps 9, 10       tcgen05.mma for one tile of Q each: S of the unit after next as soon as the weights of this one have been multiplied, so that the
 //                     softmax always finds the next S there and waits for no product
 //
@@ -41,8 +41,8 @@ constexpr int kTmemCols = 512, kColO = 256;          // S of tile q, buffer b at
 constexpr float kGrow = 8.f;                         // log2 of what a maximum may grow before O is rescaled
 
 template <int HD> struct Smem {
-    static constexpr int q_tile = kRows * HD * 2, unit = kKeys * HD * 2, stages = HD == 128 ? 8 : 10, ring = 2 * q_tile, total = ring + stages * unit + 1024;
-    static_assert(stages * unit >= 2 * kRows * HD * 4 || HD == 64, "");
+    static constexpr int q_tile = kRows * HD * 2, unit = kKeys * HD * 2, stages = HD == 128 ? 4 : 6, ring = 2 * q_tile, total = ring + stages * 2 * unit + 1024;
+    static_assert(stages * 2 * unit >= 2 * kRows * HD * 4, "");
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -88,20 +88,23 @@ __device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap* map, int
     asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
                  ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void mma_commit(uint32_t bar) {       // arrives when all products issued so far have retired
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+// Issued by the one thread for which `lead` is set.  The others come along, so that addresses and descriptors are the warp's (uniform registers): inside
+// a branch of one thread an mma took 69 clk to issue, whatever its size.
+__device__ __forceinline__ void mma_commit(uint32_t bar, uint32_t lead) {       // arrives when all products issued so far have retired
+    asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+                 "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(lead) : "memory");
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate, uint32_t lead) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(lead) : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate, uint32_t lead) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(lead) : "memory");
 }
 #define B200GPTQ_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
 #define B200GPTQ_RW8(r, i) "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7])
@@ -127,6 +130,11 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
 __device__ __forceinline__ void fma2(float& x, float& y, float a, float b, float m, float c) {
     asm("{\n\t.reg .b64 u, v, w;\n\tmov.b64 u, {%2, %3};\n\tmov.b64 v, {%4, %4};\n\tmov.b64 w, {%5, %5};\n\t"
         "fma.rn.f32x2 u, u, v, w;\n\tmov.b64 {%0, %1}, u;\n\t}" : "=f"(x), "=f"(y) : "f"(a), "f"(b), "f"(m), "f"(c));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float m;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+    return m;
 }
 __device__ __forceinline__ void add2(float& x, float& y, float a, float b) {
     asm("{\n\t.reg .b64 u, v;\n\tmov.b64 u, {%0, %1};\n\tmov.b64 v, {%2, %3};\n\tadd.rn.f32x2 u, u, v;\n\tmov.b64 {%0, %1}, u;\n\t}"
@@ -170,7 +178,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     __shared__ float stats[2][2][kRows];         // [tile][maximum, denominator][row] (PACKED)
 
     const b200gptq_attn_args& a = p.a;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t bar_base = smem_u32(bars);
     auto full = [&](int s) { return bar_base + 8u * s; };
     auto empty = [&](int s) { return bar_base + 8u * (ST + s); };
@@ -200,7 +208,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     tc_before();
     __syncthreads();
     tc_after();
-    const uint32_t tmem = tmem_base_holder;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base_holder, 0);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
 
@@ -221,58 +229,59 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         p_hi[q] = pos0 + (r + max(nrows[q], 1) - 1) / G;
     }
     auto of = [](const int (&v)[2], int q) { return q ? v[1] : v[0]; };       // (registers, not an array that is indexed)
-    int n_units = 0, n_s = 0, first = 0;
-    AttnRange range = {0, 0, 0};
+    // Units of three regions, one after the other: the prefix, the sinks, the window (which begin where the keys begin; where sinks and window meet, they
+    // are one run of keys, cut at a multiple of 64).
+    int n_units = 0, n_p = 0, n_s = 0, first = 0, s_end = 0, w_base = 0, w_end = 0;
     if (nrows[0] > 0) {
         if constexpr (PACKED) {
             first = (int)((long long)p.prefix_units * split / p.splits);
-            n_units = (int)((long long)p.prefix_units * (split + 1) / p.splits) - first;
+            n_units = n_p = (int)((long long)p.prefix_units * (split + 1) / p.splits) - first;
         } else {
-            range = attn_range(p_lo[0], nrows[1] > 0 ? p_hi[1] : p_hi[0], window, a.sinks, a.max_seq);
-            n_s = (range.s_end + kKeys - 1) / kKeys;
-            n_units = p.prefix_units + n_s + (range.w_end - range.w_start + kKeys - 1) / kKeys;
+            const AttnRange range = attn_range(p_lo[0], nrows[1] > 0 ? p_hi[1] : p_hi[0], window, a.sinks, a.max_seq);
+            const bool one = range.w_start == 0;
+            w_end = range.w_end;
+            s_end = one ? w_end : range.s_end;
+            n_p = p.prefix_units;
+            n_s = (min(a.sinks, s_end) + kKeys - 1) / kKeys;
+            w_base = one ? n_s * kKeys : range.w_start;
+            n_units = n_p + n_s + max(0, w_end - w_base + kKeys - 1) / kKeys;
         }
     }
-    struct Keys { int j0, end; bool prefix; };
-    auto keys_at = [&](int i) {
-        Keys k;
-        if constexpr (PACKED) { k.prefix = true; k.j0 = (first + i) * kKeys; k.end = a.prefix; return k; }
-        k.prefix = i < p.prefix_units;
-        i -= p.prefix_units;
-        k.j0 = k.prefix ? (i + p.prefix_units) * kKeys : i < n_s ? i * kKeys : range.w_start + (i - n_s) * kKeys;
-        k.end = k.prefix ? a.prefix : i < n_s ? range.s_end : range.w_end;
-        return k;
+    struct Region { int begin, end, j_first, j_end; };           // units, key of unit `begin`, end of the keys
+    // What rows of tile q see of region g
+    auto region = [&](int q, int g) {
+        Region v = {0, 0, 0, 0};
+        if (of(nrows, q) <= 0) return v;
+        if (g == 0) return Region{0, n_p, first * kKeys, a.prefix};
+        if (PACKED) return v;
+        const int hi = of(p_hi, q);
+        if (g == 1) return Region{n_p, n_p + (hi < 0 ? 0 : min(n_s, hi / kKeys + 1)), 0, s_end};
+        const int n_w = n_units - n_p - n_s, from = max(0, (of(p_lo, q) - window + 1 - w_base) >> 6), to = max(from, min(n_w, ((hi - w_base) >> 6) + 1));
+        return Region{n_p + n_s + from, n_p + n_s + to, w_base + from * kKeys, w_end};
     };
-    auto needs = [&](int q, int i) {          // whether any row of tile q sees any of the keys
-        if (of(nrows, q) <= 0) return false;
-        if (alt) return (i & 1) == q;
-        if (PACKED) return true;
-        const Keys k = keys_at(i);
-        return k.prefix || (k.j0 <= of(p_hi, q) && (k.j0 + kKeys - 1 > of(p_lo, q) - window || k.j0 < a.sinks));
-    };
-    // Load n of 2 n_units: K0 K1 V0 K2 V1 .. K(n - 1) V(n - 2) V(n - 1)
-    auto load_at = [&](int n, bool& value) {
-        value = n == 2 * n_units - 1 || (n > 0 && (n & 1) == 0);
-        return n == 2 * n_units - 1 ? n_units - 1 : value ? n / 2 - 1 : (n + 1) / 2;
-    };
-
+    static_assert(kKeys == 64, "");
     bool ok = true;
     if (warp == kLoadWarp) {
         // ===== keys and values =====
         if (elect_one()) {
-            int n = 0;
-            for (int s = 0, round = 0; n < 2 * n_units; ++n) {
-                if (round > 0) ok = mbar_wait(empty(s), (round - 1) & 1, &abort_flag);
-                if (!ok) break;
-                bool value;
-                const Keys k = keys_at(load_at(n, value));
-                const uint32_t dst = base + SM::ring + s * SM::unit, bar = full(s);
-                mbar_expect(bar, SM::unit);
+            auto load = [&](int i, uint32_t dst, uint32_t bar, bool value) {
+                const bool prefix = i < n_p;
+                const int j0 = prefix ? (first + i) * kKeys : i < n_p + n_s ? (i - n_p) * kKeys : w_base + (i - n_p - n_s) * kKeys;
 #pragma unroll
                 for (int h = 0; h < HALVES; ++h) {
-                    if (k.prefix) tma_3d(dst + h * BOX, value ? &map_vp : &map_kp, 64 * h, k.j0, kh, bar);
-                    else tma_4d(dst + h * BOX, value ? &map_v : &map_k, 64 * h, k.j0, kh, b0, bar);
+                    if (prefix) tma_3d(dst + h * BOX, value ? &map_vp : &map_kp, 64 * h, j0, kh, bar);
+                    else tma_4d(dst + h * BOX, value ? &map_v : &map_k, 64 * h, j0, kh, b0, bar);
                 }
+            };
+            int n = 0;                        // slots: K0 and K1, then V i and K i + 2
+            for (int s = 0, round = 0; n_units > 0 && n <= n_units; ++n) {
+                if (round > 0) ok = mbar_wait(empty(s), (round - 1) & 1, &abort_flag);
+                if (!ok) break;
+                const uint32_t dst = base + SM::ring + s * 2 * SM::unit, bar = full(s);
+                mbar_expect(bar, n < 1 ? min(2, n_units) * SM::unit : n + 1 < n_units ? 2 * SM::unit : SM::unit);
+                if (n == 0) load(0, dst, bar, false);
+                else load(n - 1, dst, bar, true);
+                if (n + 1 < n_units) load(n + 1, dst + SM::unit, bar, false);
                 if (++s == ST) { s = 0; ++round; }
             }
             if (!ok) {                        // what is on its way lands before the CTA ends
@@ -283,65 +292,78 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         __syncwarp();
     } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
         // ===== products of tile q, load by load =====
+        const uint32_t lead = elect_one();
         constexpr uint32_t type = std::is_same<T, __half>::value ? 0u : 1u;
         constexpr uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(kRows >> 4) << 24);
         constexpr uint32_t idesc_qk = idesc | ((uint32_t)(kKeys >> 3) << 17), idesc_pv = idesc | (1u << 16) | ((uint32_t)(HD >> 3) << 17);
         const int q = warp - kMmaWarp;
         const uint64_t qd = smem_desc(base + (alt ? 0 : q) * SM::q_tile, 0);
         const uint32_t ts = tmem + 128u * q, to = tmem + kColO + 128u * q;
-        auto wait = [&](uint32_t bar, int parity) {
-            ok = mbar_wait(bar, parity & 1, &abort_flag);
-            ok = __all_sync(0xffffffffu, ok);
+        const Region r0 = region(q, 0), r1 = region(q, 1), r2 = region(q, 2);
+        auto needs = [&](int i) {
+            return alt ? i < r0.end && (i & 1) == q : (i >= r0.begin && i < r0.end) || (i >= r1.begin && i < r1.end) || (i >= r2.begin && i < r2.end);
         };
         int started = 0, mixed = 0;           // S begun, weights multiplied
-        for (int n = 0, s = 0, round = 0; n < 2 * n_units; ++n) {
-            bool value;
-            const int i = load_at(n, value);
-            wait(full(s), round);
-            if (!ok) break;
-            const uint32_t at = base + SM::ring + s * SM::unit;
-            if (!needs(q, i)) {
-                if (lane == 0) mbar_arrive(empty(s));
-            } else if (!value) {
-                if (started == 0) wait(q_full(alt ? 0 : q), 0);
-                if (!ok) break;
-                tc_after();
-                if (elect_one()) {
-                    const uint64_t kd = smem_desc(at, 0);
+        auto qk = [&](uint32_t at) {
+            const uint64_t kd = smem_desc(at, 0);
 #pragma unroll
-                    for (int k = 0; k < HD / 16; ++k)
-                        mma_ss(ts + 64u * (started & 1), qd + ((k / 4 * QBOX + k % 4 * 32) >> 4), kd + ((k / 4 * BOX + k % 4 * 32) >> 4), idesc_qk, k > 0 ? 1u : 0u);
-                    mma_commit(s_full(q, started & 1));
-                    mma_commit(empty(s));
-                }
-                ++started;
-            } else {
-                const Keys k = keys_at(i);
-                if (k.j0 + kKeys > k.end) {   // rows that nobody sees (both warps write the same zeros)
-                    for (int x = lane; x < (k.j0 + kKeys - k.end) * HALVES * 8; x += 32) {
-                        const int r = k.end - k.j0 + x / (HALVES * 8), c = x % (HALVES * 8);
-                        *reinterpret_cast<uint4*>(base_ptr + (at - base) + (c / 8) * BOX + r * 128 + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                }
-                wait(p_full(q, mixed & 1), mixed >> 1);
-                if (!ok) break;
+            for (int k = 0; k < HD / 16; ++k)
+                mma_ss(ts + 64u * (started & 1), qd + ((k / 4 * QBOX + k % 4 * 32) >> 4), kd + ((k / 4 * BOX + k % 4 * 32) >> 4), idesc_qk, k > 0 ? 1u : 0u, lead);
+            mma_commit(s_full(q, started & 1), lead);
+        };
+        // One thread does it all, with one barrier for both loads of a turn: what a turn costs here besides the products (each wait 150 to 250 clk, also one
+        // that is over already) is time in which the tensor cores idle.  (A wait that runs out is not looked at: those after it give up at once,
+        // and the results are not defined then.)
+        if (n_units > 0) {
+            {
+                if (of(nrows, q) > 0) mbar_wait(q_full(alt ? 0 : q), 0, &abort_flag);
+                mbar_wait(full(0), 0, &abort_flag);
                 tc_after();
-                if (elect_one()) {
+            }
+            for (int i = 0; i < min(2, n_units); ++i)
+                if (needs(i)) {
+                    qk(base + SM::ring + i * SM::unit);
+                    ++started;
+                }
+            if (started) mma_commit(empty(0), lead);
+            else if (lead) mbar_arrive(empty(0));
+        }
+        for (int i = 0, s = 1, round = 0; i < n_units; ++i) {
+            const bool mine = needs(i), mine2 = i + 2 < n_units && needs(i + 2);
+            const uint32_t at = base + SM::ring + s * 2 * SM::unit;
+            const int seen = i < n_p ? r0.j_end - r0.j_first - i * kKeys : i < n_p + n_s ? r1.j_end - (i - n_p) * kKeys : r2.j_end - r2.j_first - (i - r2.begin) * kKeys;
+            if (mine && seen < kKeys) {       // rows that nobody sees (both warps write the same zeros)
+                mbar_wait(full(s), round & 1, &abort_flag);
+                __syncwarp();
+                for (int x = lane; x < (kKeys - seen) * HALVES * 8; x += 32) {
+                    const int r = seen + x / (HALVES * 8), c = x % (HALVES * 8);
+                    *reinterpret_cast<uint4*>(base_ptr + (at - base) + (c / 8) * BOX + r * 128 + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+            }
+            {
+                mbar_wait(full(s), round & 1, &abort_flag);
+                if (mine) mbar_wait(p_full(q, mixed & 1), (mixed >> 1) & 1, &abort_flag);
+                __syncwarp();
+                tc_after();
+                if (mine) {
                     const uint64_t vd = smem_desc(at, BOX);
 #pragma unroll
                     for (int k = 0; k < kKeys / 16; ++k)
-                        mma_ts(to, ts + 64u * (mixed & 1) + 8u * k, vd + k * (2048 >> 4), idesc_pv, (mixed > 0 || k > 0) ? 1u : 0u);
-                    mma_commit(empty(s));
-                    mma_commit(o_done(q));
+                        mma_ts(to, ts + 64u * (mixed & 1) + 8u * k, vd + k * (2048 >> 4), idesc_pv, (mixed > 0 || k > 0) ? 1u : 0u, lead);
+                    mma_commit(o_done(q), lead);
                 }
-                ++mixed;
+                if (mine2) qk(at + SM::unit);
+                if (mine || mine2) mma_commit(empty(s), lead);
+                else if (lead) mbar_arrive(empty(s));
             }
+            mixed += mine;
+            started += mine2;
             __syncwarp();
             if (++s == ST) { s = 0; ++round; }
         }
-        if (elect_one()) mma_commit(retired(q));
+        mma_commit(retired(q), lead);
         __syncwarp();
         int never = 0;                        // (also after a wait that ran out: nothing is in flight when tensor memory is freed)
         mbar_wait(retired(q), 0, &never);
@@ -376,13 +398,21 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         }
         const int pr = pos0 + (row_first + min(r, max(rows, 1) - 1)) / G;
         float m = -INFINITY, l = 0.f;           // the maximum in use (of scores, not scaled), the denominator
+        float off = 0.f;                        // -m, scaled (m = -infinity: 0, every weight is then 0)
         int turn = 0;
-        for (int i = 0; i < n_units; ++i) {
-            if (!needs(q, i)) continue;
+#pragma unroll 1
+        for (int g = 0; g < 3; ++g) {
+          const Region v = region(q, g);
+          // A unit whose keys all rows of the tile see: from key `least` to key `most`
+          const int most = min(g == 1 ? min(v.j_end, a.sinks) : v.j_end, g == 0 ? v.j_end : of(p_lo, q) + 1) - kKeys, least = g == 2 ? of(p_hi, q) - window + 1 : 0;
+          int j0 = v.j_first + (alt ? q * kKeys : 0);
+          const int step = alt ? 2 : 1;
+#pragma unroll 1
+          for (int i = v.begin + (alt ? q : 0); i < v.end; i += step, j0 += step * kKeys) {
             const uint32_t tb = ts + 64u * (turn & 1);
-            ok = mbar_wait(s_full(q, turn & 1), (turn >> 1) & 1, &abort_flag);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
+            // (A wait that runs out is not looked at before the end: those after it give up at once, and the results are not defined then.)
+            mbar_wait(s_full(q, turn & 1), (turn >> 1) & 1, &abort_flag);
+            __syncwarp();
             tc_after();
             if (mine) {
                 uint32_t s[2][32];
@@ -391,16 +421,13 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                 tmem_wait_ld();
                 after_wait(s[0]);
                 after_wait(s[1]);
-                const Keys k = keys_at(i);
-                bool whole = k.j0 + kKeys <= k.end;
-                if (!k.prefix) whole = whole && k.j0 + kKeys - 1 <= of(p_lo, q) && (k.j0 > of(p_hi, q) - window || k.j0 + kKeys <= a.sinks);
-                if (!whole) {
+                if (j0 > most || j0 < least) {
                     // columns [0, front) and [lo, hi) are seen
-                    int front = k.end - k.j0, lo = 0, hi = 0;
-                    if (!k.prefix) {
-                        front = min(min(a.sinks, pr + 1), k.end) - k.j0;
-                        lo = pr - window + 1 - k.j0;
-                        hi = min(pr + 1, k.end) - k.j0;
+                    int front = v.j_end - j0, lo = 0, hi = 0;
+                    if (g != 0) {
+                        front = min(min(a.sinks, pr + 1), v.j_end) - j0;
+                        lo = pr - window + 1 - j0;
+                        hi = min(pr + 1, v.j_end) - j0;
                     }
 #pragma unroll
                     for (int x = 0; x < kKeys; ++x)
@@ -412,18 +439,17 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                     top[g] = __uint_as_float(s[g / 2][g % 2 * 16]);
 #pragma unroll
                     for (int e = 1; e < 15; e += 2)
-                        top[g] = fmaxf(top[g], fmaxf(__uint_as_float(s[g / 2][g % 2 * 16 + e]), __uint_as_float(s[g / 2][g % 2 * 16 + e + 1])));
+                        top[g] = max3(top[g], __uint_as_float(s[g / 2][g % 2 * 16 + e]), __uint_as_float(s[g / 2][g % 2 * 16 + e + 1]));
                     top[g] = fmaxf(top[g], __uint_as_float(s[g / 2][g % 2 * 16 + 15]));
                 }
-                const float up = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-                const bool grow = up > m && (m == -INFINITY || (up - m) * p.sl2 > kGrow);
+                const float up = fmaxf(max3(top[0], top[1], top[2]), top[3]);
+                const bool grow = (up - m) * p.sl2 > kGrow;         // (from -infinity too, but not where both are)
                 if (__any_sync(0xffffffffu, grow)) {
                     const float corr = grow ? exp2_fast((m - up) * p.sl2) : 1.f;
-                    if (grow) { m = up; l *= corr; }
+                    if (grow) { m = up; l *= corr; off = -m * p.sl2; }
                     if (turn > 0) {             // (the first products overwrite O)
-                        ok = mbar_wait(o_done(q), (turn - 1) & 1, &abort_flag);
-                        ok = __all_sync(0xffffffffu, ok);
-                        if (!ok) break;
+                        mbar_wait(o_done(q), (turn - 1) & 1, &abort_flag);
+                        __syncwarp();
                         tc_after();
                         uint32_t o[32];
 #pragma unroll 1
@@ -437,7 +463,6 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                         }
                     }
                 }
-                const float off = m == -INFINITY ? 0.f : -m * p.sl2;
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
                 uint32_t w[32];
 #pragma unroll
@@ -457,12 +482,11 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             __syncwarp();
             if (lane == 0) mbar_arrive(p_full(q, turn & 1));
             ++turn;
+          }
         }
         // ---- O ----
-        if (ok && turn > 0) {
-            ok = mbar_wait(retired(q), 0, &abort_flag);
-            ok = __all_sync(0xffffffffu, ok);
-        }
+        if (turn > 0) mbar_wait(retired(q), 0, &abort_flag);
+        ok = __all_sync(0xffffffffu, !abort_flag);
         tc_after();
         const long long rows_total = (long long)a.batch * a.tokens * a.heads;
         if constexpr (PACKED) {
