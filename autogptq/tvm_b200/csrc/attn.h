@@ -7,11 +7,12 @@
 
 namespace b200gptq {
 
-// How a call is carried out.  tiles: one launch of the tcgen05 kernel.  Otherwise the rows kernel takes each sequence's own keys in `own` runs, and the
-// prefix goes before it in `parts` runs (sums in scratch), by the tcgen05 kernel (prefix_tiles) or by the rows kernel.
-struct AttnPlan { bool tiles, prefix_tiles; int own, parts; };
+// How a call is carried out.  tiles: one launch of the tcgen05 kernel.  Otherwise the rows kernel takes each sequence's own keys, with `own` CTAs of `warps`
+// warps per tile of rows; the prefix is among them, or goes before in `parts` runs (sums in scratch), by the tcgen05 kernel (prefix_tiles) or by the rows kernel.
+struct AttnPlan { bool tiles, prefix_tiles; int own, warps, parts; };
 
-constexpr int kAttnMaxSplit = 8, kAttnRowsKeys = 128, kAttnTilesKeys = 64;      // CTAs of a cluster, keys that all warps of a CTA take at once (rows kernel), keys per unit (tcgen05)
+constexpr int kAttnMaxSplit = 8;         // CTAs of a cluster (rows kernel)
+constexpr int kAttnTilesKeys = 64;       // keys of a unit (tcgen05 kernel)
 
 bool attn_pdl_enabled();
 

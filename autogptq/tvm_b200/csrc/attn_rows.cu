@@ -3,18 +3,21 @@
 //
 //   S = Q K^T,  w = softmax(scale S) over the visible keys,  O = w V
 //
-// The bytes of K and V bound it (4 flop per byte and row of Q), so a CTA holds up to 16 or 32 rows of Q (all that share a key head: the heads
+// The bytes of K and V bound it (4 flop per byte and row of Q), so a CTA holds up to 8, 16 or 32 rows of Q (all that share a key head: the heads
 // of its group, the tokens of a short run, and with a prefix all sequences of the batch) and streams the keys once.  Every warp takes blocks of 16
 // keys on its own and goes from global memory to mma.sync fragments without shared memory:
-//   * Q K^T: operand B of m16n8k16 wants, from lane (g, c) = (lane / 4, lane % 4), the pairs 2c and 2c + 8 of key g.  Any order of the 16 dims
+//   * Q K^T: an operand of m16n8k16 wants, from lane (g, c) = (lane / 4, lane % 4), the pairs 2c and 2c + 8 of key g.  Any order of the 16 dims
 //     serves as long as Q has the same, so a lane loads 16 bytes = 8 adjacent dims of key g, which are the operand of two products;
-//   * w V: operand B wants pairs of keys of one dim.  A lane loads 8 adjacent dims of keys 2c, 2c + 1, 2c + 8, 2c + 9 and pairs them with byte
-//     permutations; column g of product (h, i) is dim 64 h + 8 g + i;
-//   * the accumulators of S are operand A of the second product as they lie.
-// The next block's keys are requested when this block's have been multiplied, its values likewise, so that 6 to 8 KB per warp are on their way.
+//   * w V: an operand wants pairs of keys of one dim.  A lane loads 8 adjacent dims of keys 2c, 2c + 1, 2c + 8, 2c + 9 and pairs them with byte
+//     permutations; index g of product (h, i) is dim 64 h + 8 g + i;
+//   * up to 8 rows: keys are the 16, rows the 8 (half the accumulators: two CTAs per SM); the weights change hands by movmatrix.  More: rows are the 16, and the
+//     accumulators of S are operand A of the second product as they lie.
+// The next block's keys are requested when this block's have been multiplied, its values likewise, so that 6 to 8 KB per warp are on their way.  Rows are
+// only rescaled when a score is more than 2^8 above the maximum in use (no weight is above 2^8; fp32 sums).
 //
-// The key range is split over a cluster of up to 8 CTAs, which add up through distributed shared memory, each a slice of the dims.  With a prefix
-// there are two launches: the first takes the prefix, split over CTAs whose sums (fp32) go to scratch; the second takes each sequence's own rows
+// The key range is split over the warps of a CTA and a cluster of up to 8 CTAs, which add up through distributed shared memory, each a slice of the dims.
+// A prefix is part of every sequence's keys where reading it again from L2 takes less time than a second launch (4 us); else
+// there are two: the first takes the prefix, split over CTAs whose sums (fp32) go to scratch; the second takes each sequence's own rows
 // meanwhile, waits for the first (griddepcontrol.wait) and adds everything up.  All sums are in a fixed order.
 #include <algorithm>
 #include <mutex>
@@ -26,8 +29,8 @@
 namespace b200gptq {
 namespace {
 
-constexpr int kWarps = 8, kThreads = kWarps * 32, kBlock = 16, kMaxSplit = kAttnMaxSplit;
-static_assert(kWarps * kBlock == kAttnRowsKeys, "");
+constexpr int kBlock = 16, kMaxSplit = kAttnMaxSplit;
+constexpr float kGrow = 8.f;             // log2 of what a score may be above the maximum in use
 
 template <typename T>
 __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -45,30 +48,35 @@ __device__ __forceinline__ void st_cluster(const float* local, int rank, float v
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v) : "memory");
 }
 
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {      // of an 8 x 8 matrix of 16-bit values, a pair of a row per lane
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
 // Shared memory, in floats: the warps' sums [warp][row][HD + 4], their maxima and denominators, the slices that the CTAs of the cluster push
 // [split][row][HD / splits] with maxima and denominators, a flag per row; the queries (padded rows).
-template <int HD, int MT> struct Lay {
-    static constexpr int R = 16 * MT, LD = HD + 4, QLD = HD + 8;
-    static constexpr int acc = 0, ml = acc + kWarps * R * LD, slice = ml + 2 * kWarps * R, slice_ml = slice + R * HD,
-                         flags = slice_ml + 2 * kMaxSplit * R, q = flags + R, total = q + R * QLD / 2;
+template <int HD, int R, int W> struct Lay {
+    static constexpr int LD = HD + 4, QLD = HD + 8, acc = 0, ml = acc + W * R * LD, slice = ml + 2 * W * R, slice_ml = slice + R * HD,
+                         flags = slice_ml + 2 * kMaxSplit * R, q = flags + (R < 16 ? 16 : R), total = q + R * QLD / 2;
 };
 
 // PREFIX: rows (b, t, g) of one key head against the prefix, sums to `part`.  Otherwise: rows (t, g) of one sequence and key head against its cache
-// (and the sums of the prefix).  A row tile is blockIdx.x / splits % row_tiles.
-template <typename T, int HD, int MT, bool PREFIX>
-__global__ void __launch_bounds__(kThreads, 1)
-attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict__ part, int splits, int row_tiles, int parts) {
-    using L = Lay<HD, MT>;
-    constexpr int R = L::R, SEG = HD / 32, HH = HD / 64;
+// (and the prefix itself, where with_prefix, or its `parts` sums).  A tile of R rows is blockIdx.x / splits % row_tiles.
+template <typename T, int HD, int R, int W, bool PREFIX>
+__global__ void __launch_bounds__(W * 32, R == 8 ? 16 / W : 1)
+attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict__ part, int splits, int row_tiles, int parts, int with_prefix) {
+    using L = Lay<HD, R, W>;
+    constexpr int MT = R == 8 ? 1 : R / 16, SEG = HD / 32, HH = HD / 64, kThreads = W * 32;
     extern __shared__ __align__(16) float sm[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int G = a.heads / a.kv_heads, window = a.window ? a.window : 1 << 30;
     const int split = blockIdx.x % splits, unit = blockIdx.x / splits, tile = unit % row_tiles;
     const int kh = unit / row_tiles % a.kv_heads, b0 = unit / row_tiles / a.kv_heads;        // (PREFIX: b0 = 0)
-    // What is read below was written before the launch in front of this one ended (window) or began (behind the prefix launch, which lets this one
+    // What is read below was written before the launch in front of this one ended, or began (behind the prefix launch, which lets this one
     // start only after it has itself waited; the loads by-pass L1).
     if (!PREFIX && splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-    if (PREFIX || !a.prefix) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (PREFIX || !parts) asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
 
     const int row0 = tile * R, rows_all = (PREFIX ? a.batch : 1) * a.tokens * G;
@@ -76,45 +84,40 @@ attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict
     if constexpr (!PREFIX) { p0 = attn_pos(a, b0); count = attn_count(a, b0); }
     const int nrows = min(R, (PREFIX ? rows_all : count * G) - row0);
     if (nrows <= 0) {                         // padding: every CTA of the cluster leaves
-        if (!PREFIX && a.prefix) asm volatile("griddepcontrol.wait;" ::: "memory");
+        if (!PREFIX && parts) asm volatile("griddepcontrol.wait;" ::: "memory");
         return;
     }
-    // ---- queries ----
-    T* qs = reinterpret_cast<T*>(sm + L::q);
-    for (int i = threadIdx.x; i < R * HD / 8; i += kThreads) {
-        const int r = i / (HD / 8), d = i % (HD / 8) * 8, idx = row0 + min(r, nrows - 1), head = kh * G + idx % G, tok = idx / G;
-        const int bb = PREFIX ? tok / a.tokens : b0, t = PREFIX ? tok - bb * a.tokens : tok;
-        *reinterpret_cast<uint4*>(qs + r * L::QLD + d) = __ldcg(reinterpret_cast<const uint4*>(
-            static_cast<const T*>(a.q) + bb * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2] + d));
-    }
-    // ---- keys ----
-    AttnRange range = {0, 0, a.prefix};
+    // ---- keys: the prefix, the sinks, the window ----
+    AttnRange range = {0, 0, 0};
     const int p_lo = p0 + row0 / G, p_hi = p0 + (row0 + nrows - 1) / G;
     if constexpr (!PREFIX) range = attn_range(p_lo, p_hi, window, a.sinks, a.max_seq);
-    const int nb_s = (range.s_end + kBlock - 1) / kBlock, nb = nb_s + (range.w_end - range.w_start + kBlock - 1) / kBlock;
+    const int n_p = PREFIX || with_prefix ? (a.prefix + kBlock - 1) / kBlock : 0, n_s = n_p + (range.s_end + kBlock - 1) / kBlock,
+              nb = n_s + (range.w_end - range.w_start + kBlock - 1) / kBlock;
     const int first = (int)((long long)nb * split / splits), last = (int)((long long)nb * (split + 1) / splits);
-    const T *kb, *vb;
-    long long ks, vs;
-    if constexpr (PREFIX) {
-        kb = static_cast<const T*>(a.k_prefix) + kh * a.k_prefix_stride[0]; ks = a.k_prefix_stride[1];
-        vb = static_cast<const T*>(a.v_prefix) + kh * a.v_prefix_stride[0]; vs = a.v_prefix_stride[1];
-    } else {
-        kb = static_cast<const T*>(a.k_cache) + b0 * a.k_stride[0] + kh * a.k_stride[1]; ks = a.k_stride[2];
-        vb = static_cast<const T*>(a.v_cache) + b0 * a.v_stride[0] + kh * a.v_stride[1]; vs = a.v_stride[2];
+    const T *k_own = nullptr, *v_own = nullptr, *k_front = nullptr, *v_front = nullptr;
+    if constexpr (!PREFIX) {
+        k_own = static_cast<const T*>(a.k_cache) + b0 * a.k_stride[0] + kh * a.k_stride[1];
+        v_own = static_cast<const T*>(a.v_cache) + b0 * a.v_stride[0] + kh * a.v_stride[1];
+    }
+    if (n_p) {
+        k_front = static_cast<const T*>(a.k_prefix) + kh * a.k_prefix_stride[0];
+        v_front = static_cast<const T*>(a.v_prefix) + kh * a.v_prefix_stride[0];
     }
     uint4 kr[2][SEG], vr[4][HH];
     auto block = [&](int i, int& j0, int& end) {
-        const bool s = i < nb_s;
-        j0 = s ? kBlock * i : range.w_start + kBlock * (i - nb_s);
-        end = s ? range.s_end : range.w_end;
+        j0 = i < n_p ? kBlock * i : i < n_s ? kBlock * (i - n_p) : range.w_start + kBlock * (i - n_s);
+        end = i < n_p ? a.prefix : i < n_s ? range.s_end : range.w_end;
     };
     // (rows behind the end of the range: its last row again, with weight zero)
     auto load_k = [&](int i) {
         int j0, end;
         block(i, j0, end);
+        const bool front = PREFIX || i < n_p;
+        const T* base = (front ? k_front : k_own) + 8 * c;
+        const long long stride = front ? a.k_prefix_stride[1] : a.k_stride[2];
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-            const T* src = kb + min(j0 + 8 * n + g, end - 1) * ks + 8 * c;
+            const T* src = base + min(j0 + 8 * n + g, end - 1) * stride;
 #pragma unroll
             for (int s = 0; s < SEG; ++s) kr[n][s] = __ldcg(reinterpret_cast<const uint4*>(src + 32 * s));
         }
@@ -122,128 +125,201 @@ attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict
     auto load_v = [&](int i) {
         int j0, end;
         block(i, j0, end);
+        const bool front = PREFIX || i < n_p;
+        const T* base = (front ? v_front : v_own) + 8 * g;
+        const long long stride = front ? a.v_prefix_stride[1] : a.v_stride[2];
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-            const T* src = vb + min(j0 + 2 * c + (n & 1) + 4 * (n & 2), end - 1) * vs + 8 * g;
+            const T* src = base + min(j0 + 2 * c + (n & 1) + 4 * (n & 2), end - 1) * stride;
 #pragma unroll
             for (int h = 0; h < HH; ++h) vr[n][h] = __ldcg(reinterpret_cast<const uint4*>(src + 64 * h));
         }
     };
     int i = first + warp;
     if (i < last) { load_k(i); load_v(i); }
+    // ---- queries ----
+    T* qs = reinterpret_cast<T*>(sm + L::q);
+    for (int x = threadIdx.x; x < R * HD / 8; x += kThreads) {
+        const int r = x / (HD / 8), d = x % (HD / 8) * 8, idx = row0 + min(r, nrows - 1), head = kh * G + idx % G, tok = idx / G;
+        const int bb = PREFIX ? tok / a.tokens : b0, t = PREFIX ? tok - bb * a.tokens : tok;
+        *reinterpret_cast<uint4*>(qs + r * L::QLD + d) = __ldcg(reinterpret_cast<const uint4*>(
+            static_cast<const T*>(a.q) + bb * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2] + d));
+    }
+    if (threadIdx.x < R) reinterpret_cast<int*>(sm + L::flags)[threadIdx.x] = 0;
     __syncthreads();
 
     const float scale = a.scale * kLog2e;
-    float acc[MT][8 * HH][4], m[MT][2], l[MT][2];
-    int pr[MT][2];                            // positions of the lane's rows
-    uint4 qf[MT == 1 ? MT : 1][SEG][2];       // (two row tiles read theirs from shared memory each time: registers)
+    float acc[MT][R == 8 ? 4 * HH : 8 * HH][4], m[MT][2], l[MT][2];
+    // Rows of the lane: 2 c, 2 c + 1 (up to 8 rows), else g, g + 8 of each 16; pr: their positions
+    int pr[MT][2];
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
 #pragma unroll
-        for (int n = 0; n < 8 * HH; ++n) acc[t][n][0] = acc[t][n][1] = acc[t][n][2] = acc[t][n][3] = 0.f;
+        for (int n = 0; n < (R == 8 ? 4 * HH : 8 * HH); ++n) acc[t][n][0] = acc[t][n][1] = acc[t][n][2] = acc[t][n][3] = 0.f;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             m[t][r] = -INFINITY; l[t][r] = 0.f;
-            pr[t][r] = p0 + (row0 + min(16 * t + 8 * r + g, nrows - 1)) / G;
-            if constexpr (MT == 1)
-#pragma unroll
-                for (int s = 0; s < SEG; ++s) qf[t][s][r] = *reinterpret_cast<const uint4*>(qs + (8 * r + g) * L::QLD + 32 * s + 8 * c);
+            pr[t][r] = p0 + (row0 + min(R == 8 ? 2 * c + r : 16 * t + 8 * r + g, nrows - 1)) / G;
         }
     }
-    for (; i < last; i += kWarps) {
+    for (; i < last; i += W) {
         int j0, end;
         block(i, j0, end);
-        float s[MT][2][4];
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-#pragma unroll
-            for (int n = 0; n < 2; ++n) s[t][n][0] = s[t][n][1] = s[t][n][2] = s[t][n][3] = 0.f;
+        const bool front = PREFIX || i < n_p;
+        bool whole = j0 + kBlock <= end;      // every row of the tile sees the whole block
+        if constexpr (!PREFIX) whole = whole && (front || (j0 + kBlock - 1 <= p_lo && (j0 > p_hi - window || j0 + kBlock <= a.sinks)));
+        auto sees = [&](int j, int p) { return j < end && (front || attn_sees(p, j, window, a.sinks)); };
+        if constexpr (R == 8) {
+            float s[4] = {0.f, 0.f, 0.f, 0.f};        // keys g (0, 1) and g + 8 (2, 3), rows 2 c and 2 c + 1
 #pragma unroll
             for (int e = 0; e < SEG; ++e) {
-                uint4 x, y;
-                if constexpr (MT == 1) { x = qf[t][e][0]; y = qf[t][e][1]; }
-                else {
-                    x = *reinterpret_cast<const uint4*>(qs + (16 * t + g) * L::QLD + 32 * e + 8 * c);
-                    y = *reinterpret_cast<const uint4*>(qs + (16 * t + 8 + g) * L::QLD + 32 * e + 8 * c);
-                }
-                const uint32_t a0[4] = {x.x, y.x, x.y, y.y}, a1[4] = {x.z, y.z, x.w, y.w};
+                const uint4 x = *reinterpret_cast<const uint4*>(qs + g * L::QLD + 32 * e + 8 * c);
+                const uint32_t a0[4] = {kr[0][e].x, kr[1][e].x, kr[0][e].y, kr[1][e].y}, a1[4] = {kr[0][e].z, kr[1][e].z, kr[0][e].w, kr[1][e].w};
+                mma16<T>(s, a0, x.x, x.y);
+                mma16<T>(s, a1, x.z, x.w);
+            }
+            if (i + W < last) load_k(i + W);
 #pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    mma16<T>(s[t][n], a0, kr[n][e].x, kr[n][e].y);
-                    mma16<T>(s[t][n], a1, kr[n][e].z, kr[n][e].w);
+            for (int e = 0; e < 4; ++e) {
+                s[e] *= scale;
+                if (!whole) s[e] = sees(j0 + g + 8 * (e >> 1), pr[0][e & 1]) ? s[e] : -INFINITY;
+            }
+            if (__any_sync(0xffffffffu, fmaxf(s[0], s[2]) - m[0][0] > kGrow || fmaxf(s[1], s[3]) - m[0][1] > kGrow)) {
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    float up = fmaxf(fmaxf(s[r], s[2 + r]), m[0][r]);
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, o));
+                    const float corr = up == -INFINITY ? 1.f : exp2_fast(m[0][r] - up);
+                    m[0][r] = up;
+                    l[0][r] *= corr;
+#pragma unroll
+                    for (int n = 0; n < 4 * HH; ++n) { acc[0][n][r] *= corr; acc[0][n][2 + r] *= corr; }
                 }
             }
-        }
-        if (i + kWarps < last) load_k(i + kWarps);
-        bool whole = j0 + kBlock <= end;      // every row of the tile sees the whole block
-        if constexpr (!PREFIX) whole = whole && j0 + kBlock - 1 <= p_lo && (j0 > p_hi - window || j0 + kBlock <= a.sinks);
-        uint32_t w[MT][4];
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                float x[4];
+                const float safe = m[0][r] == -INFINITY ? 0.f : m[0][r];
+                s[r] = exp2_fast(s[r] - safe);
+                s[2 + r] = exp2_fast(s[2 + r] - safe);
+                l[0][r] += s[r] + s[2 + r];
+            }
+            const uint32_t w0 = transposed(Half<T>::pack(s[0], s[1])), w1 = transposed(Half<T>::pack(s[2], s[3]));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    x[e] = s[t][e >> 1][2 * r + (e & 1)] * scale;
-                    if (!whole) {
-                        const int j = j0 + 8 * (e >> 1) + 2 * c + (e & 1);
-                        bool see = j < end;
-                        if constexpr (!PREFIX) see = see && attn_sees(pr[t][r], j, window, a.sinks);
-                        x[e] = see ? x[e] : -INFINITY;
+            for (int h = 0; h < HH; ++h)
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {         // dims 64 h + 8 g + 2 n (rows 0 .. 7 of the product) and + 1 (8 .. 15)
+                    const uint32_t x[4] = {__byte_perm(word(vr[0][h], n), word(vr[1][h], n), 0x5410u), __byte_perm(word(vr[0][h], n), word(vr[1][h], n), 0x7632u),
+                                           __byte_perm(word(vr[2][h], n), word(vr[3][h], n), 0x5410u), __byte_perm(word(vr[2][h], n), word(vr[3][h], n), 0x7632u)};
+                    mma16<T>(acc[0][4 * h + n], x, w0, w1);
+                }
+            if (i + W < last) load_v(i + W);
+        } else {
+            float s[MT][2][4];
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+#pragma unroll
+                for (int n = 0; n < 2; ++n) s[t][n][0] = s[t][n][1] = s[t][n][2] = s[t][n][3] = 0.f;
+#pragma unroll
+                for (int e = 0; e < SEG; ++e) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(qs + (16 * t + g) * L::QLD + 32 * e + 8 * c);
+                    const uint4 y = *reinterpret_cast<const uint4*>(qs + (16 * t + 8 + g) * L::QLD + 32 * e + 8 * c);
+                    const uint32_t a0[4] = {x.x, y.x, x.y, y.y}, a1[4] = {x.z, y.z, x.w, y.w};
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        mma16<T>(s[t][n], a0, kr[n][e].x, kr[n][e].y);
+                        mma16<T>(s[t][n], a1, kr[n][e].z, kr[n][e].w);
                     }
                 }
-                float up = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-                up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, 1));
-                up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, 2));
-                up = fmaxf(up, m[t][r]);
-                const float safe = up == -INFINITY ? 0.f : up, corr = exp2_fast(m[t][r] - safe);
-                m[t][r] = up;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = exp2_fast(x[e] - safe);
-                l[t][r] = l[t][r] * corr + ((x[0] + x[1]) + (x[2] + x[3]));
-#pragma unroll
-                for (int n = 0; n < 8 * HH; ++n) { acc[t][n][2 * r] *= corr; acc[t][n][2 * r + 1] *= corr; }
-                w[t][r] = Half<T>::pack(x[0], x[1]);
-                w[t][2 + r] = Half<T>::pack(x[2], x[3]);
             }
+            if (i + W < last) load_k(i + W);
+            bool grow = false;
 #pragma unroll
-        for (int h = 0; h < HH; ++h)
+            for (int t = 0; t < MT; ++t)
 #pragma unroll
-            for (int n = 0; n < 8; ++n) {
-                const uint32_t pick = (n & 1) ? 0x7632u : 0x5410u;
-                const uint32_t y0 = __byte_perm(word(vr[0][h], n / 2), word(vr[1][h], n / 2), pick);
-                const uint32_t y1 = __byte_perm(word(vr[2][h], n / 2), word(vr[3][h], n / 2), pick);
+                for (int r = 0; r < 2; ++r) {
 #pragma unroll
-                for (int t = 0; t < MT; ++t) mma16<T>(acc[t][8 * h + n], w[t], y0, y1);
+                    for (int e = 0; e < 4; ++e) {
+                        float& x = s[t][e >> 1][2 * r + (e & 1)];
+                        x *= scale;
+                        if (!whole) x = sees(j0 + 8 * (e >> 1) + 2 * c + (e & 1), pr[t][r]) ? x : -INFINITY;
+                    }
+                    grow = grow || fmaxf(fmaxf(s[t][0][2 * r], s[t][0][2 * r + 1]), fmaxf(s[t][1][2 * r], s[t][1][2 * r + 1])) - m[t][r] > kGrow;
+                }
+            if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        float up = fmaxf(fmaxf(s[t][0][2 * r], s[t][0][2 * r + 1]), fmaxf(s[t][1][2 * r], s[t][1][2 * r + 1]));
+                        up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, 1));
+                        up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, 2));
+                        up = fmaxf(up, m[t][r]);
+                        const float corr = up == -INFINITY ? 1.f : exp2_fast(m[t][r] - up);
+                        m[t][r] = up;
+                        l[t][r] *= corr;
+#pragma unroll
+                        for (int n = 0; n < 8 * HH; ++n) { acc[t][n][2 * r] *= corr; acc[t][n][2 * r + 1] *= corr; }
+                    }
             }
-        if (i + kWarps < last) load_v(i + kWarps);
+            uint32_t w[MT][4];
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float safe = m[t][r] == -INFINITY ? 0.f : m[t][r];
+                    float x[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = exp2_fast(s[t][e >> 1][2 * r + (e & 1)] - safe);
+                    l[t][r] += (x[0] + x[1]) + (x[2] + x[3]);
+                    w[t][r] = Half<T>::pack(x[0], x[1]);
+                    w[t][2 + r] = Half<T>::pack(x[2], x[3]);
+                }
+#pragma unroll
+            for (int h = 0; h < HH; ++h)
+#pragma unroll
+                for (int n = 0; n < 8; ++n) {
+                    const uint32_t pick = (n & 1) ? 0x7632u : 0x5410u;
+                    const uint32_t y0 = __byte_perm(word(vr[0][h], n / 2), word(vr[1][h], n / 2), pick);
+                    const uint32_t y1 = __byte_perm(word(vr[2][h], n / 2), word(vr[3][h], n / 2), pick);
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) mma16<T>(acc[t][8 * h + n], w[t], y0, y1);
+                }
+            if (i + W < last) load_v(i + W);
+        }
     }
-    // ---- the warps' sums ----
+    // ---- the warps' sums: rows, 8 adjacent dims each ----
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             float sum = l[t][r];
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            const int row = 16 * t + 8 * r + g;
+#pragma unroll
+            for (int o = R == 8 ? 4 : 1; o < (R == 8 ? 32 : 4); o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            const int row = R == 8 ? 2 * c + r : 16 * t + 8 * r + g;
             if (row < nrows) {
-                if (c == 0) { sm[L::ml + 2 * (warp * R + row)] = m[t][r]; sm[L::ml + 2 * (warp * R + row) + 1] = sum; }
+                if (R == 8 ? g == 0 : c == 0) { sm[L::ml + 2 * (warp * R + row)] = m[t][r]; sm[L::ml + 2 * (warp * R + row) + 1] = sum; }
                 float* dst = sm + L::acc + (warp * R + row) * L::LD;
 #pragma unroll
-                for (int h = 0; h < HH; ++h)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {         // columns 2 c + e: dims 64 h + 8 (2 c + e) ..
-                        float4* to = reinterpret_cast<float4*>(dst + 64 * h + 8 * (2 * c + e));
+                for (int h = 0; h < HH; ++h) {
+                    if constexpr (R == 8) {
+                        float4* to = reinterpret_cast<float4*>(dst + 64 * h + 8 * g);
 #pragma unroll
                         for (int x = 0; x < 2; ++x)
-                            to[x] = make_float4(acc[t][8 * h + 4 * x][2 * r + e], acc[t][8 * h + 4 * x + 1][2 * r + e],
-                                                acc[t][8 * h + 4 * x + 2][2 * r + e], acc[t][8 * h + 4 * x + 3][2 * r + e]);
+                            to[x] = make_float4(acc[t][4 * h + 2 * x][r], acc[t][4 * h + 2 * x][2 + r], acc[t][4 * h + 2 * x + 1][r], acc[t][4 * h + 2 * x + 1][2 + r]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {         // columns 2 c + e: dims 64 h + 8 (2 c + e) ..
+                            float4* to = reinterpret_cast<float4*>(dst + 64 * h + 8 * (2 * c + e));
+#pragma unroll
+                            for (int x = 0; x < 2; ++x)
+                                to[x] = make_float4(acc[t][8 * h + 4 * x][2 * r + e], acc[t][8 * h + 4 * x + 1][2 * r + e],
+                                                    acc[t][8 * h + 4 * x + 2][2 * r + e], acc[t][8 * h + 4 * x + 3][2 * r + e]);
+                        }
                     }
+                }
             }
         }
-    if (threadIdx.x < R) reinterpret_cast<int*>(sm + L::flags)[threadIdx.x] = 0;
     __syncthreads();
     if (!PREFIX && splits > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");      // (all CTAs of the cluster run)
     // ---- the CTA's sums: to the scratch, or slice by slice to the CTAs of the cluster ----
@@ -253,10 +329,10 @@ attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict
         const int row = x / HD, d = x % HD;
         float cm = -INFINITY, cl = 0.f, ca = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) cm = fmaxf(cm, sm[L::ml + 2 * (w * R + row)]);
+        for (int w = 0; w < W; ++w) cm = fmaxf(cm, sm[L::ml + 2 * (w * R + row)]);
         const float safe = cm == -INFINITY ? 0.f : cm;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
+        for (int w = 0; w < W; ++w) {
             const float e = exp2_fast(sm[L::ml + 2 * (w * R + row)] - safe);
             cl += sm[L::ml + 2 * (w * R + row) + 1] * e;
             ca += sm[L::acc + (w * R + row) * L::LD + d] * e;
@@ -265,10 +341,7 @@ attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict
             const int idx = row0 + row;
             const long long at = split * rows_total + (long long)(idx / G) * a.heads + kh * G + idx % G;
             part[at * HD + d] = ca;
-            if (d == 0) {
-                float* ml = part + splits * rows_total * HD + 2 * at;
-                ml[0] = cm; ml[1] = cl;
-            }
+            if (d == 0) *reinterpret_cast<float2*>(part + splits * rows_total * HD + 2 * at) = make_float2(cm, cl);
         } else {
             const int to = d / slice;
             st_cluster(sm + L::slice + (split * R + row) * slice + d - to * slice, to, ca);
@@ -281,7 +354,7 @@ attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict
     if constexpr (PREFIX) return;
     if (splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     else __syncthreads();
-    if (a.prefix) asm volatile("griddepcontrol.wait;" ::: "memory");                        // the prefix's sums
+    if (parts) asm volatile("griddepcontrol.wait;" ::: "memory");                           // the prefix's sums
     // ---- this CTA's slice of the dims ----
     int* flags = reinterpret_cast<int*>(sm + L::flags);
     const float* part_ml = part + parts * rows_total * HD;
@@ -297,6 +370,7 @@ attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict
             tl += sm[L::slice_ml + 2 * (r * R + row) + 1] * e;
             ta += sm[L::slice + (r * R + row) * slice + d] * e;
         }
+#pragma unroll 4
         for (int r = 0; r < parts; ++r) {
             const float2 ml = __ldcg(reinterpret_cast<const float2*>(part_ml + 2 * (r * rows_total + at)));
             const float e = exp2_fast(ml.x - safe);
@@ -310,7 +384,7 @@ attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict
     // rows of several tokens in one tile: a NaN may come from a row of the cache that this one does not see
     if (p_hi > p_lo) {
         __syncthreads();
-        for (int row = warp; row < nrows; row += kWarps)
+        for (int row = warp; row < nrows; row += W)
             if (flags[row]) {
                 const int idx = row0 + row;
                 attn_row_again<T, HD>(a, b0, idx / G, kh * G + idx % G, p0 + idx / G, split * slice, (split + 1) * slice);
@@ -318,60 +392,55 @@ attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict
     }
 }
 
-template <typename K>
-int launch(K* kernel, const b200gptq_attn_args& a, int smem, long long ctas, int cluster, bool pdl, float* part, int splits, int row_tiles,
-           int parts, cudaStream_t stream) {
-    if (ctas > 0x7fffffff) return B200GPTQ_ERR_TOO_LARGE;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)ctas);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    int n = 0;
-    if (cluster > 1) {
-        attr[n].id = cudaLaunchAttributeClusterDimension;
-        attr[n].val.clusterDim.x = cluster;
-        attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
-        ++n;
-    }
-    if (pdl) {
-        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[n].val.programmaticStreamSerializationAllowed = 1;
-        ++n;
-    }
-    cfg.attrs = attr;
-    cfg.numAttrs = n;
-    B200GPTQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a, part, splits, row_tiles, parts));
-    return B200GPTQ_OK;
-}
-
-template <typename T, int HD, int MT, bool PREFIX>
+template <typename T, int HD, int R, int W, bool PREFIX>
 int run(const b200gptq_attn_args& a, float* part, const AttnPlan& s, cudaStream_t stream) {
     static std::once_flag once[64];
     static cudaError_t result[64];
-    auto* kernel = attn_rows_kernel<T, HD, MT, PREFIX>;
-    constexpr int smem = Lay<HD, MT>::total * 4;
+    auto* kernel = attn_rows_kernel<T, HD, R, W, PREFIX>;
+    constexpr int smem = Lay<HD, R, W>::total * 4;
     int dev = 0;
     B200GPTQ_CUDA_TRY(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64) return B200GPTQ_ERR_TOO_LARGE;
     std::call_once(once[dev], [&] { result[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
     B200GPTQ_CUDA_TRY(result[dev]);
     const long long rows = (long long)a.tokens * (a.heads / a.kv_heads) * (PREFIX ? a.batch : 1);
-    const int tiles = (int)((rows + 16 * MT - 1) / (16 * MT));
-    const long long units = (long long)tiles * a.kv_heads * (PREFIX ? 1 : a.batch);
-    const int splits = PREFIX ? s.parts : s.own;
-    return launch(kernel, a, smem, units * splits, PREFIX ? 1 : splits, attn_pdl_enabled(), part, splits, tiles, s.parts, stream);
+    const int tiles = (int)((rows + R - 1) / R), splits = PREFIX ? s.parts : s.own;
+    const long long ctas = (long long)tiles * a.kv_heads * (PREFIX ? 1 : a.batch) * splits;
+    if (ctas > 0x7fffffff) return B200GPTQ_ERR_TOO_LARGE;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(W * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (!PREFIX && splits > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = splits;
+        attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    if (attn_pdl_enabled()) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n].val.programmaticStreamSerializationAllowed = 1;
+        ++n;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
+    B200GPTQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a, part, splits, tiles, s.parts, a.prefix && !s.parts ? 1 : 0));
+    return B200GPTQ_OK;
 }
 
 template <typename T, int HD>
 int run_all(const b200gptq_attn_args& a, float* part, const AttnPlan& s, cudaStream_t stream) {
-    const long long per_sequence = (long long)a.tokens * (a.heads / a.kv_heads);
-    if (a.prefix && !s.prefix_tiles) {
-        const int st = per_sequence * a.batch <= 16 ? run<T, HD, 1, true>(a, part, s, stream) : run<T, HD, 2, true>(a, part, s, stream);
+    const long long rows = (long long)a.tokens * (a.heads / a.kv_heads), all = rows * a.batch;
+    if (s.parts && !s.prefix_tiles) {
+        const int st = all <= 8 ? run<T, HD, 8, 8, true>(a, part, s, stream) : all <= 16 ? run<T, HD, 16, 8, true>(a, part, s, stream) : run<T, HD, 32, 8, true>(a, part, s, stream);
         if (st != B200GPTQ_OK) return st;
     }
-    return per_sequence <= 16 ? run<T, HD, 1, false>(a, part, s, stream) : run<T, HD, 2, false>(a, part, s, stream);
+    if (rows <= 8)
+        return s.warps == 2 ? run<T, HD, 8, 2, false>(a, part, s, stream) : s.warps == 4 ? run<T, HD, 8, 4, false>(a, part, s, stream) : run<T, HD, 8, 8, false>(a, part, s, stream);
+    return rows <= 16 ? run<T, HD, 16, 8, false>(a, part, s, stream) : run<T, HD, 32, 8, false>(a, part, s, stream);
 }
 
 }  // namespace

@@ -111,14 +111,14 @@ def test_attention_with_a_window_or_a_prefix_refuses_on_the_host():
         (dict(q=A + 8), -4), (dict(k_cache=A + 2), -4), (dict(v_cache=A + 8), -4), (dict(out=A + 8), -4), (dict(pos=A + 4), -4), (dict(counts=A + 4), -4),
         (dict(q_stride=(512, 64, 68)), -4), (dict(k_stride=(4, 64, 64)), -4), (dict(v_stride=(512, 4, 64)), -4), (dict(out_stride=(512, 64, 1)), -4),
         (dict(window=0, prefix=5, k_prefix=A, v_prefix=A + 8), -4), (dict(window=0, prefix=5, k_prefix=A, v_prefix=A, v_prefix_stride=(512, 4)), -4),
-        (dict(window=0, prefix=5, k_prefix=A, v_prefix=A), -5),
+        (dict(window=0, prefix=200000, k_prefix=A, v_prefix=A), -5),
     ]:
         assert call(**change) == status, change
     assert call(fn=_lib.lib.b200gptq_attn_workspace_bytes) == 0
-    need = call(fn=_lib.lib.b200gptq_attn_workspace_bytes, window=0, prefix=500)
+    need = call(fn=_lib.lib.b200gptq_attn_workspace_bytes, window=0, prefix=200000)
     assert need > 0 and need % (2 * 8 * 66 * 4) == 0
-    assert call(window=0, prefix=500, k_prefix=A, v_prefix=A, ws=A, ws_bytes=need - 1) == -5
-    assert call(window=0, prefix=500, k_prefix=A, v_prefix=A, ws=A + 8, ws_bytes=need) == -4
+    assert call(window=0, prefix=200000, k_prefix=A, v_prefix=A, ws=A, ws_bytes=need - 1) == -5
+    assert call(window=0, prefix=200000, k_prefix=A, v_prefix=A, ws=A + 8, ws_bytes=need) == -4
     assert call(fn=_lib.lib.b200gptq_attn_workspace_bytes, hd=96) == -3
 
 

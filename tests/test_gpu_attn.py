@@ -129,6 +129,15 @@ PREFIX = [
     (1, 150, 2, 1, 128, 180, [20], 128),
     (2, 131, 1, 1, 64, 140, [0, 9], 3),
     (1, 1, 32, 1, 128, 64, [40], 700),
+    # so much that it goes before, in parts: up to 8, 16, 32, 128, 256 and more rows per key head
+    (2, 1, 2, 2, 128, 40, [0, 39], 40001),
+    (12, 1, 1, 1, 128, 40, list(range(12)), 6100),
+    (8, 1, 6, 2, 64, 40, list(range(8)), 10007),
+    (70, 1, 4, 4, 64, 8, [i % 8 for i in range(70)], 1500),
+    (130, 1, 2, 2, 64, 8, [i % 8 - 1 for i in range(130)], 600),
+    (11, 3, 10, 2, 128, 40, list(range(11)), 3333),
+    (90, 1, 4, 1, 128, 5, [i % 5 for i in range(90)], 1111),
+    (5, 60, 1, 1, 64, 70, list(range(5)), 40000),
 ]
 
 
