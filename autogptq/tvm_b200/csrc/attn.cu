@@ -36,13 +36,13 @@ AttnPlan plan_of(const b200gptq_attn_args& a) {
         p.tiles = true;
         return p;
     }
-    // Warps per tile of rows: as many as the SMs hold (16 each, or 8 where a tile has more than 8 rows), two blocks of 16 keys for each at least.
+    // Warps per tile of rows: as many as the SMs hold (16 each, or 8 where a tile has more than 8 rows), a block of 16 keys for each at least.
     const long long tile = rows <= 8 ? 8 : rows <= 16 ? 16 : 32, held = sms * (rows <= 8 ? 16 : 8), units = (rows + tile - 1) / tile * a.kv_heads * a.batch;
     // The prefix among each sequence's keys: read `again` times more, from L2.  A second launch costs 4 us.
     const double again = (double)(a.batch - 1) * a.kv_heads * a.prefix * a.hd * 4;
     const bool apart = a.prefix && again > 32e6;
     const long long keys = (a.window ? std::min<long long>(a.max_seq, (long long)a.window + a.sinks + a.tokens) : a.max_seq) + (apart ? 0 : a.prefix);
-    long long warps = 2;
+    long long warps = rows > 8 ? 8 : keys < 256 ? 1 : 2;
     while (warps < 8 * kAttnMaxSplit && units * warps * 2 <= held && keys >= warps * 2 * 16) warps *= 2;
     p.warps = rows <= 8 ? (int)std::min(warps, 8LL) : 8;
     p.own = (int)std::max(1LL, warps / 8);
@@ -50,10 +50,10 @@ AttnPlan plan_of(const b200gptq_attn_args& a) {
         p.prefix_tiles = all > 32 && attn_tiles_maps(a, true);
         if (p.prefix_tiles) {
             const long long blocks = (a.prefix + kAttnTilesKeys - 1) / kAttnTilesKeys, ctas = (all + 255) / 256 * a.kv_heads;
-            p.parts = (int)std::max<long long>(1, std::min(sms / ctas, blocks / 4));
+            p.parts = (int)std::max<long long>(1, std::min(std::min<long long>(sms / ctas, kAttnMaxParts), blocks / 4));
         } else {
             const long long ctas = (all <= 16 ? 1 : (all + 31) / 32) * a.kv_heads;
-            p.parts = (int)std::max<long long>(1, std::min<long long>(std::min<long long>(2 * sms / ctas, 64), a.prefix / 128));
+            p.parts = (int)std::max<long long>(1, std::min<long long>(std::min<long long>(2 * sms / ctas, kAttnMaxParts), a.prefix / 128));
         }
     }
     return p;

@@ -12,6 +12,7 @@ namespace b200gptq {
 struct AttnPlan { bool tiles, prefix_tiles; int own, warps, parts; };
 
 constexpr int kAttnMaxSplit = 8;         // CTAs of a cluster (rows kernel)
+constexpr int kAttnMaxParts = 64;        // runs of a prefix
 constexpr int kAttnTilesKeys = 64;       // keys of a unit (tcgen05 kernel)
 
 bool attn_pdl_enabled();

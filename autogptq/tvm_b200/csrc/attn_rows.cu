@@ -57,8 +57,9 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {      // of an 8 x 8
 // Shared memory, in floats: the warps' sums [warp][row][HD + 4], their maxima and denominators, the slices that the CTAs of the cluster push
 // [split][row][HD / splits] with maxima and denominators, a flag per row; the queries (padded rows).
 template <int HD, int R, int W> struct Lay {
-    static constexpr int LD = HD + 4, QLD = HD + 8, acc = 0, ml = acc + W * R * LD, slice = ml + 2 * W * R, slice_ml = slice + R * HD,
-                         flags = slice_ml + 2 * kMaxSplit * R, q = flags + (R < 16 ? 16 : R), total = q + R * QLD / 2;
+    static constexpr int LD = HD + 4, QLD = HD + 8, acc = 0, weights = 2 * R * ((W == 8 ? kMaxSplit : 1) + kAttnMaxParts),
+                         ml = acc + (W * R * LD > weights ? W * R * LD : weights), slice = ml + 2 * W * R, slice_ml = slice + R * HD,
+                         flags = slice_ml + 2 * kMaxSplit * R, places = flags + (R < 16 ? 16 : R), q = places + 6 * R, total = q + R * QLD / 2;
 };
 
 // PREFIX: rows (b, t, g) of one key head against the prefix, sums to `part`.  Otherwise: rows (t, g) of one sequence and key head against its cache
@@ -137,15 +138,22 @@ attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict
     };
     int i = first + warp;
     if (i < last) { load_k(i); load_v(i); }
-    // ---- queries ----
+    // ---- the rows' places in q, out and the scratch (divisions once per row), queries ----
+    long long* places = reinterpret_cast<long long*>(sm + L::places);
+    if (threadIdx.x < R) {
+        const int idx = row0 + min((int)threadIdx.x, nrows - 1), tok = idx / G, head = kh * G + idx - tok * G;
+        const int bb = PREFIX ? tok / a.tokens : b0, t = PREFIX ? tok - bb * a.tokens : tok;
+        places[threadIdx.x] = bb * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2];
+        places[R + threadIdx.x] = bb * a.out_stride[0] + t * a.out_stride[1] + head * a.out_stride[2];
+        places[2 * R + threadIdx.x] = ((long long)bb * a.tokens + t) * a.heads + head;
+        reinterpret_cast<int*>(sm + L::flags)[threadIdx.x] = 0;
+    }
+    __syncthreads();
     T* qs = reinterpret_cast<T*>(sm + L::q);
     for (int x = threadIdx.x; x < R * HD / 8; x += kThreads) {
-        const int r = x / (HD / 8), d = x % (HD / 8) * 8, idx = row0 + min(r, nrows - 1), head = kh * G + idx % G, tok = idx / G;
-        const int bb = PREFIX ? tok / a.tokens : b0, t = PREFIX ? tok - bb * a.tokens : tok;
-        *reinterpret_cast<uint4*>(qs + r * L::QLD + d) = __ldcg(reinterpret_cast<const uint4*>(
-            static_cast<const T*>(a.q) + bb * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2] + d));
+        const int r = x / (HD / 8), d = x % (HD / 8) * 8;
+        *reinterpret_cast<uint4*>(qs + r * L::QLD + d) = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + places[r] + d));
     }
-    if (threadIdx.x < R) reinterpret_cast<int*>(sm + L::flags)[threadIdx.x] = 0;
     __syncthreads();
 
     const float scale = a.scale * kLog2e;
@@ -338,8 +346,7 @@ attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict
             ca += sm[L::acc + (w * R + row) * L::LD + d] * e;
         }
         if constexpr (PREFIX) {
-            const int idx = row0 + row;
-            const long long at = split * rows_total + (long long)(idx / G) * a.heads + kh * G + idx % G;
+            const long long at = split * rows_total + places[2 * R + row];
             part[at * HD + d] = ca;
             if (d == 0) *reinterpret_cast<float2*>(part + splits * rows_total * HD + 2 * at) = make_float2(cm, cl);
         } else {
@@ -355,31 +362,65 @@ attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict
     if (splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     else __syncthreads();
     if (parts) asm volatile("griddepcontrol.wait;" ::: "memory");                           // the prefix's sums
-    // ---- this CTA's slice of the dims ----
+    // ---- this CTA's slice of the dims.  With a prefix's sums, first the weights of all runs of all rows, where the warps' sums were: 0 .. splits - 1 those of
+    //      the cluster, then the prefix's.  (Maxima and denominators read by every thread, one run after the other: 8 us more for 18 runs.) ----
     int* flags = reinterpret_cast<int*>(sm + L::flags);
-    const float* part_ml = part + parts * rows_total * HD;
-    for (int x = threadIdx.x; x < nrows * slice; x += kThreads) {
-        const int row = x / slice, d = x - row * slice, idx = row0 + row, t = idx / G, head = kh * G + idx % G;
-        const long long at = ((long long)b0 * a.tokens + t) * a.heads + head;
-        float tm = -INFINITY, tl = 0.f, ta = 0.f;
-        for (int r = 0; r < splits; ++r) tm = fmaxf(tm, sm[L::slice_ml + 2 * (r * R + row)]);
-        for (int r = 0; r < parts; ++r) tm = fmaxf(tm, __ldcg(part_ml + 2 * (r * rows_total + at)));
-        const float safe = tm == -INFINITY ? 0.f : tm;
-        for (int r = 0; r < splits; ++r) {
-            const float e = exp2_fast(sm[L::slice_ml + 2 * (r * R + row)] - safe);
-            tl += sm[L::slice_ml + 2 * (r * R + row) + 1] * e;
-            ta += sm[L::slice + (r * R + row) * slice + d] * e;
+    float2* wl = reinterpret_cast<float2*>(sm);       // (maximum, denominator), then (weight, -)
+    const int runs = splits + parts;
+    if (parts) {
+        const float* part_ml = part + parts * rows_total * HD;
+        for (int x = threadIdx.x; x < nrows * runs; x += kThreads) {
+            const int row = x / runs, r = x - row * runs;
+            const long long at = places[2 * R + row];
+            wl[x] = r < splits ? *reinterpret_cast<const float2*>(sm + L::slice_ml + 2 * (r * R + row)) : __ldcg(reinterpret_cast<const float2*>(part_ml + 2 * ((r - splits) * rows_total + at)));
         }
-#pragma unroll 4
-        for (int r = 0; r < parts; ++r) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(part_ml + 2 * (r * rows_total + at)));
-            const float e = exp2_fast(ml.x - safe);
-            tl += ml.y * e;
-            ta += __ldcg(part + (r * rows_total + at) * HD + split * slice + d) * e;
+        __syncthreads();
+        for (int row = warp; row < nrows; row += W) {
+            float tm = -INFINITY, tl = 0.f;
+            for (int r = lane; r < runs; r += 32) tm = fmaxf(tm, wl[row * runs + r].x);
+    #pragma unroll
+            for (int o = 16; o > 0; o >>= 1) tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, o));
+            const float safe = tm == -INFINITY ? 0.f : tm;
+            for (int r = lane; r < runs; r += 32) {
+                const float e = exp2_fast(wl[row * runs + r].x - safe);
+                tl += wl[row * runs + r].y * e;
+                wl[row * runs + r].x = e;
+            }
+    #pragma unroll
+            for (int o = 16; o > 0; o >>= 1) tl += __shfl_xor_sync(0xffffffffu, tl, o);
+            if (lane == 0) sm[L::slice_ml + row] = tl;    // (what lay there has been copied)
         }
-        const float o = tl != 0.f ? ta / tl : 0.f;
-        static_cast<T*>(a.out)[b0 * a.out_stride[0] + t * a.out_stride[1] + head * a.out_stride[2] + split * slice + d] = Half<T>::round(o);
-        if (!isfinite(o)) flags[row] = 1;
+        __syncthreads();
+    }
+    for (int x = threadIdx.x; x < nrows * (slice / 4); x += kThreads) {
+        const int row = x / (slice / 4), d = (x - row * (slice / 4)) * 4;
+        const long long at = places[2 * R + row];
+        const float2* w = wl + row * runs;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto add = [&](const float4& f, float e) { o.x += f.x * e; o.y += f.y * e; o.z += f.z * e; o.w += f.w * e; };
+        float tl = 0.f;
+        if (parts) {
+            tl = sm[L::slice_ml + row];
+            for (int r = 0; r < splits; ++r) add(*reinterpret_cast<const float4*>(sm + L::slice + (r * R + row) * slice + d), w[r].x);
+        } else {
+            const float2* ml = reinterpret_cast<const float2*>(sm + L::slice_ml) + row;
+            float tm = -INFINITY;
+            for (int r = 0; r < splits; ++r) tm = fmaxf(tm, ml[r * R].x);
+            const float safe = tm == -INFINITY ? 0.f : tm;
+            for (int r = 0; r < splits; ++r) {
+                const float e = exp2_fast(ml[r * R].x - safe);
+                tl += ml[r * R].y * e;
+                add(*reinterpret_cast<const float4*>(sm + L::slice + (r * R + row) * slice + d), e);
+            }
+        }
+        const float* src = part + at * HD + split * slice + d;
+#pragma unroll 8
+        for (int r = 0; r < parts; ++r) add(__ldcg(reinterpret_cast<const float4*>(src + r * rows_total * HD)), w[splits + r].x);
+        const bool none = tl == 0.f;
+        o = make_float4(none ? 0.f : o.x / tl, none ? 0.f : o.y / tl, none ? 0.f : o.z / tl, none ? 0.f : o.w / tl);
+        *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + places[R + row] + split * slice + d) =
+            make_uint2(Half<T>::pack(o.x, o.y), Half<T>::pack(o.z, o.w));
+        if (!isfinite(o.x) || !isfinite(o.y) || !isfinite(o.z) || !isfinite(o.w)) flags[row] = 1;
     }
     // rows of several tokens in one tile: a NaN may come from a row of the cache that this one does not see
     if (p_hi > p_lo) {
@@ -439,7 +480,7 @@ int run_all(const b200gptq_attn_args& a, float* part, const AttnPlan& s, cudaStr
         if (st != B200GPTQ_OK) return st;
     }
     if (rows <= 8)
-        return s.warps == 2 ? run<T, HD, 8, 2, false>(a, part, s, stream) : s.warps == 4 ? run<T, HD, 8, 4, false>(a, part, s, stream) : run<T, HD, 8, 8, false>(a, part, s, stream);
+        return s.warps == 1 ? run<T, HD, 8, 1, false>(a, part, s, stream) : s.warps == 2 ? run<T, HD, 8, 2, false>(a, part, s, stream) : s.warps == 4 ? run<T, HD, 8, 4, false>(a, part, s, stream) : run<T, HD, 8, 8, false>(a, part, s, stream);
     return rows <= 16 ? run<T, HD, 16, 8, false>(a, part, s, stream) : run<T, HD, 32, 8, false>(a, part, s, stream);
 }
 

@@ -41,7 +41,7 @@ constexpr int kTmemCols = 512, kColO = 256;          // S of tile q, buffer b at
 constexpr float kGrow = 8.f;                         // log2 of what a maximum may grow before O is rescaled
 
 template <int HD> struct Smem {
-    static constexpr int q_tile = kRows * HD * 2, unit = kKeys * HD * 2, stages = HD == 128 ? 4 : 6, ring = 2 * q_tile, total = ring + stages * 2 * unit + 1024;
+    static constexpr int q_tile = kRows * HD * 2, unit = kKeys * HD * 2, stages = HD == 128 ? 5 : 8, ring = 2 * q_tile, total = ring + stages * 2 * unit + 1024;
     static_assert(stages * 2 * unit >= 2 * kRows * HD * 4, "");
 };
 
@@ -160,7 +160,7 @@ struct TileArgs {
     b200gptq_attn_args a;
     float* part;
     float sl2;                // |scale| log2 e, and Q is negated where the scale is negative
-    int negate, pairs, splits, prefix_units;
+    int negate, pairs, splits, prefix_units, group;
 };
 
 template <typename T, int HD, bool PACKED>
@@ -175,7 +175,6 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     __shared__ __align__(8) uint64_t bars[2 * ST + 15];
     __shared__ uint32_t tmem_base_holder;
     __shared__ volatile int abort_flag;
-    __shared__ float stats[2][2][kRows];         // [tile][maximum, denominator][row] (PACKED)
 
     const b200gptq_attn_args& a = p.a;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -213,7 +212,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     asm volatile("griddepcontrol.launch_dependents;");
 
     // ---- which rows, which keys.  The last rows of a prompt see most, and come first. ----
-    const int G = a.heads / a.kv_heads, window = a.window ? a.window : 1 << 30;
+    const int G = p.group, window = a.window ? a.window : 1 << 30;
     const int split = PACKED ? blockIdx.x % p.splits : 0, part_unit = PACKED ? blockIdx.x / p.splits : blockIdx.x;
     const int kh = part_unit % a.kv_heads, b0 = PACKED ? 0 : part_unit / a.kv_heads % a.batch;
     const int pair = p.pairs - 1 - part_unit / a.kv_heads / (PACKED ? 1 : a.batch), row0 = pair * 2 * kRows;
@@ -372,6 +371,11 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         const int q = warp >> 2, quarter = warp & 3, r = 32 * quarter + lane, rows = of(nrows, q), row_first = row0 + (alt ? 0 : q * kRows);
         const uint32_t lane_off = (uint32_t)(32 * quarter) << 16, ts = tmem + 128u * q + lane_off, to = tmem + kColO + 128u * q + lane_off;
         const bool mine = 32 * quarter < rows;          // the warp has rows at all
+        // The thread's row.  (The divisions once per row; where other threads need its place they ask for it.  With the divisions where Q is loaded and where O
+        // is stored these took 6500 and 4000 clk.)
+        const int idx = row_first + min(r, max(rows, 1) - 1), token = idx / G, head = kh * G + idx - token * G;
+        const int b = PACKED ? token / a.tokens : b0, t = PACKED ? token - b * a.tokens : token, pr = pos0 + token;
+        const long long q_at = b * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2];
         // Q, in the swizzled layout of the tiles: 16 bytes per thread and turn, eight of them on their way at once
         if (!(alt && q == 1)) {
             uint8_t* dst = base_ptr + q * SM::q_tile;
@@ -380,10 +384,10 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                 uint4 val[8];
 #pragma unroll
                 for (int x = 0; x < 8; ++x) {
-                    const int rr = 32 * quarter + ((x0 + x) * 32 + lane) / (HD / 8), c = lane % (HD / 8), idx = row_first + rr, tok = idx / G, head = kh * G + idx - tok * G;
-                    const int b = PACKED ? tok / a.tokens : b0, t = PACKED ? tok - b * a.tokens : tok;
+                    const int rw = ((x0 + x) * 32 + lane) / (HD / 8), c = lane % (HD / 8);
+                    const long long from = __shfl_sync(0xffffffffu, q_at, rw);
                     val[x] = make_uint4(0, 0, 0, 0);
-                    if (rr < rows) val[x] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + b * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2] + 8 * c));
+                    if (32 * quarter + rw < rows) val[x] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + from + 8 * c));
                 }
 #pragma unroll
                 for (int x = 0; x < 8; ++x) {
@@ -396,7 +400,6 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full(q));
         }
-        const int pr = pos0 + (row_first + min(r, max(rows, 1) - 1)) / G;
         float m = -INFINITY, l = 0.f;           // the maximum in use (of scores, not scaled), the denominator
         float off = 0.f;                        // -m, scaled (m = -infinity: 0, every weight is then 0)
         int turn = 0;
@@ -494,6 +497,9 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             // dims the tiles lie where the ring was, for 64 over Q too: what each tile multiplies has been multiplied when both have met here.
             constexpr int CH = HD / 4;          // 16-byte pieces of a row
             float4* stage = reinterpret_cast<float4*>(base_ptr + (HD == 128 ? SM::ring : 0));
+            float (*stats)[2][kRows] = reinterpret_cast<float (*)[2][kRows]>(stage + 2 * kRows * CH);              // behind them: [tile][maximum, denominator][row]
+            long long (*places)[kRows] = reinterpret_cast<long long (*)[kRows]>(stats + 2);                         // and the rows' places among the sums
+            static_assert((HD == 128 ? SM::ring : 0) + 2 * kRows * HD * 4 + 2 * kRows * 16 <= SM::total - 1024, "");
             tc_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(all_met);
@@ -501,6 +507,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             ok = __all_sync(0xffffffffu, ok);
             tc_after();
             if (ok && mine) {
+                places[q][r] = split * rows_total + (long long)token * a.heads + head;
                 stats[q][0][r] = m * p.sl2;
                 stats[q][1][r] = l;
 #pragma unroll 1
@@ -524,8 +531,8 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             float* ml = p.part + p.splits * rows_total * HD;
             const int all = alt ? nrows[0] : nrows[0] + nrows[1];
             for (int x = threadIdx.x; ok && x < all * CH; x += kSoftmaxWarps * 32) {
-                const int row = x / CH, chunk = x % CH, idx = row0 + row;
-                const long long at = split * rows_total + (long long)(idx / G) * a.heads + kh * G + idx % G;
+                const int row = x / CH, chunk = x % CH;
+                const long long at = places[row / kRows][row % kRows];
                 float4 f = stage[row * CH + (chunk ^ (row & 7))];
                 float tm = stats[row / kRows][0][row % kRows], tl = stats[row / kRows][1][row % kRows];
                 if (alt) {
@@ -540,6 +547,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             }
         } else if (ok && mine) {
             const float inv = l != 0.f ? 1.f / l : 0.f;
+            const long long out_at = b * a.out_stride[0] + t * a.out_stride[1] + head * a.out_stride[2];
             bool bad = false;
             uint8_t* stage = base_ptr + q * SM::q_tile;                  // (the products with Q are done; a warp stores what it has staged)
 #pragma unroll 1
@@ -565,17 +573,19 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             }
             __syncwarp();
             const int last = min(32, rows - 32 * quarter);
-            for (int x = lane; x < last * (HD / 8); x += 32) {
-                const int rr = 32 * quarter + x / (HD / 8), c = x % (HD / 8), id = row_first + rr, t = id / G, head = kh * G + id - t * G;
-                *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + b0 * a.out_stride[0] + t * a.out_stride[1] + head * a.out_stride[2] + 8 * c) =
-                    *reinterpret_cast<const uint4*>(stage + rr * HD * 2 + ((c ^ (rr & 7)) << 4));
+#pragma unroll 4
+            for (int x = 0; x < HD / 8; ++x) {
+                const int rw = (x * 32 + lane) / (HD / 8), rr = 32 * quarter + rw, c = lane % (HD / 8);
+                const long long to_row = __shfl_sync(0xffffffffu, out_at, rw);
+                if (rw < last)
+                    *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + to_row + 8 * c) = *reinterpret_cast<const uint4*>(stage + rr * HD * 2 + ((c ^ (rr & 7)) << 4));
             }
             __syncwarp();
             unsigned again = __ballot_sync(0xffffffffu, bad && r < rows);
             while (again) {
-                const int rr = 32 * quarter + __ffs(again) - 1, id = row_first + rr, t = id / G;
+                const int from = __ffs(again) - 1, t2 = __shfl_sync(0xffffffffu, t, from);
                 again &= again - 1;
-                attn_row_again<T, HD>(a, b0, t, kh * G + id - t * G, pos0 + t, 0, HD);
+                attn_row_again<T, HD>(a, b0, t2, __shfl_sync(0xffffffffu, head, from), pos0 + t2, 0, HD);
             }
         }
     }
@@ -625,6 +635,7 @@ int run(const b200gptq_attn_args& a, float* part, int splits, cudaStream_t strea
     t.sl2 = std::max(std::fabs(a.scale) * kLog2e, 1e-30f);        // (a scale of zero: all weights alike, and no infinity times zero)
     t.negate = a.scale < 0.f;
     t.splits = splits;
+    t.group = a.heads / a.kv_heads;
     t.prefix_units = (int)((a.prefix + kKeys - 1) / kKeys);
     const long long rows = (long long)a.tokens * (a.heads / a.kv_heads) * (PACKED ? a.batch : 1);
     t.pairs = (int)((rows + 2 * kRows - 1) / (2 * kRows));
