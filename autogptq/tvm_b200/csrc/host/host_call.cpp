@@ -579,7 +579,7 @@ PyObject* logits_checked(PyObject* const* args) {
     need(t[1] || (!t[3] && !t[4] && !t[5] && !t[6]), "history", "is needed for penalties");
     if (t[1]) {
         need_type(*t[1], at::kLong, "history");
-        need(t[1]->dim() == 2 && t[1]->size(0) == R && t[1]->size(1) <= (1 << 30) && (t[1]->size(1) <= 1 || t[1]->stride(1) == 1), "history", "must be [rows, positions], dense in its last dimension");
+        need(t[1]->dim() == 2 && t[1]->size(0) == R && t[1]->size(1) < (1 << 30) && (t[1]->size(1) <= 1 || t[1]->stride(1) == 1), "history", "must be [rows, positions], dense in its last dimension");
         a.history_len = (int)t[1]->size(1);
         a.history = a.history_len ? static_cast<const int64_t*>(data_of(*t[1])) : nullptr;
         a.history_stride = R == 1 ? 0 : t[1]->stride(0);

@@ -149,6 +149,15 @@ def test_infinities_and_nan():
     assert float(call(s)[0, 5]) == 1.0
 
 
+@pytest.mark.parametrize("L,N", [(65535, 32767), (65536, 20), (70, 32768), (66000, 33000)])
+def test_long_texts_and_long_lists(L, N):
+    """Counts and entries that fit a token's word just so, and those that have words of their own."""
+    s = make(2, 3000, L, N, True, torch.float32, seed=L)
+    s["history"][:, ::3] = 1234
+    s["bias_tokens"][:, -1] = 77              # the last entry of all
+    check(call(s), s)
+
+
 def test_same_token_throughout():
     s = {"logits": torch.ones(2, 5000, dtype=torch.float32), "history": torch.full((2, 100000), 4321), "lengths": torch.tensor([100000, 99999]),
          "prompt_lens": torch.tensor([1, 0]), "frequency": torch.tensor([0.25, 0.5]), "presence": torch.tensor([1.0, 2.0])}
