@@ -3,9 +3,9 @@
 // A CTA takes a slice of one row's vocabulary.  It goes through the row's whole history and counts the tokens of its slice in shared memory
 // (integers: the order of the additions does not matter), notes for each token the last entry among the biases, and lists the tokens that occur at all.  It
 // copies its slice of the logits, with what the mask forbids, and then does the listed tokens: there are few, and in the loop over all tokens nearly every
-// warp had one and went through all the branches (128 rows of 100003: 41 us and bound by instructions, now LLL).
+// warp had one and went through all the branches (128 rows of 100003: 41 us and bound by instructions, now 32).
 // What bounds it: a few rows, the launch and the round trips to memory, of which there are two, everything else is asked for at once in front
-// of them (64 rows of 50272: lengths, history, biases and logits one after the other 14.7 us, now LLM); many rows, the logits' bytes and the L2 reads of the
+// of them (64 rows of 50272: lengths, history, biases and logits one after the other 14.7 us, now 7.7); many rows, the logits' bytes and the L2 reads of the
 // history, 8 bytes per token and slice.  (A cluster of eight CTAs that shares the work on the history: 3 to 18 us slower.)
 #include <cuda_bf16.h>
 
@@ -45,7 +45,7 @@ template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kThreads, kPerSm)
 adjust_kernel(const __grid_constant__ b200gptq_logit_args a, int slice, int slices) {
     extern __shared__ __align__(16) unsigned smem[];
-    constexpr int V = 16 / sizeof(T), VECS = kMaxSlice / V / kThreads, H = 2, L = 2;
+    constexpr int V = 16 / sizeof(T), VECS = kMaxSlice / V / kThreads, H = 2, L = 1;
     unsigned *count = smem, *listed = count + slice + slice / 2, *mask = listed + 4, *entry = mask + slice / 32;
     unsigned short* list = reinterpret_cast<unsigned short*>(count + slice);
     const int tid = threadIdx.x, row = blockIdx.x / slices, base = (blockIdx.x - row * slices) * slice, n = min(slice, a.vocab - base);
@@ -64,11 +64,7 @@ adjust_kernel(const __grid_constant__ b200gptq_logit_args a, int slice, int slic
     const float* bias_values = a.bias_values + (size_t)row * a.biases;
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    // ---- all that can be asked for at once ----
-    uint4 raw[VECS];
-#pragma unroll
-    for (int k = 0; k < VECS; ++k)
-        if (tid + k * kThreads < vecs) raw[k] = *reinterpret_cast<const uint4*>(in + head + (tid + k * kThreads) * V);
+    // ---- all that can be asked for at once, what is waited for first in front (the logits first: 128 rows of 100003 40 us, now 32) ----
     const int limit = a.history ? a.history_len : 0;
     // The history, two tokens at a time where it lies on 16 bytes; the first of them before it is known how many there are.
     const bool paired = (reinterpret_cast<uintptr_t>(history) & 15u) == 0;
@@ -90,6 +86,10 @@ adjust_kernel(const __grid_constant__ b200gptq_logit_args a, int slice, int slic
     auto held = [&](const int64_t* p, int otherwise) { return p ? (int)max(min((long long)p[row], (long long)limit), 0LL) : otherwise; };
     const int length = held(a.history ? a.lengths : nullptr, limit), prompt = held(a.prompt_lens, 0);
     const float rep = a.repetition ? a.repetition[row] : 1.f, freq = a.frequency ? a.frequency[row] : 0.f, pres = a.presence ? a.presence[row] : 0.f;
+    uint4 raw[VECS];
+#pragma unroll
+    for (int k = 0; k < VECS; ++k)
+        if (tid + k * kThreads < vecs) raw[k] = *reinterpret_cast<const uint4*>(in + head + (tid + k * kThreads) * V);
     if (a.mask)
         for (int i = tid; i < (n + 31) / 32; i += kThreads) mask[i] = (unsigned)a.mask[row * a.mask_stride + base / 32 + i];
     __syncthreads();

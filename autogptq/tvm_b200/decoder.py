@@ -22,7 +22,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
-from typing import List, Optional
+from typing import Dict, List, Optional, Sequence, Union
 
 import torch
 import torch.distributed as dist
@@ -50,6 +50,9 @@ class DecoderConfig:
     # overflow fp16 within one decoder layer; the harness shrinks the scales so that values stay finite
     # (kernel time does not depend on the values).
     scale_mult: float = 1.0 / 16.0
+    # Attention sees the last `window` positions and the first `sinks` of a text; None: all of it.
+    window: Optional[int] = None
+    sinks: int = 0
 
     @property
     def head_dim(self) -> int:
@@ -66,6 +69,44 @@ def check_positions(pos: int, steps: int, max_seq: int) -> None:
     captured graph can advance it), which leaves this host-side check as the place where a bad request is reported."""
     if pos < 0 or steps < 0 or pos + steps > max_seq:
         raise ValueError(f"{steps} steps from position {pos} do not fit the KV caches (max_seq = {max_seq})")
+
+
+@dataclass
+class LogitRules:
+    """What a request asks of the logits before the pick (:func:`ops.adjust_logits`), by sequence or one for all.  ``frequency`` and ``presence`` look at
+    the generated tokens, ``repetition`` at the prompt too.  ``bias``: token -> number.  ``mask`` int32 ``[batch or 1, ceil(vocab / 32)]``: a bit per token that
+    may come next; the caller may write into it between steps (a grammar)."""
+    repetition: Union[None, float, Sequence[float]] = None
+    frequency: Union[None, float, Sequence[float]] = None
+    presence: Union[None, float, Sequence[float]] = None
+    bias: Union[None, Dict[int, float], Sequence[Dict[int, float]]] = None
+    mask: Optional[torch.Tensor] = None
+
+    def arguments(self, batch: int, vocab: int, device) -> dict:
+        """The keyword arguments of :func:`ops.adjust_logits` that do not change from step to step."""
+        out = {}
+        for name in ("repetition", "frequency", "presence"):
+            v = getattr(self, name)
+            if v is not None:
+                v = [float(v)] * batch if isinstance(v, (int, float)) else [float(x) for x in v]
+                if len(v) != batch or not all(math.isfinite(x) for x in v) or (name == "repetition" and min(v) <= 0):
+                    raise ValueError(f"{name}: a finite number for each of {batch} sequences" + (", above 0" if name == "repetition" else ""))
+                out[name] = torch.tensor(v, dtype=torch.float32, device=device)
+        if self.bias is not None:
+            rows = [self.bias] * batch if isinstance(self.bias, dict) else list(self.bias)
+            if len(rows) != batch or any(not 0 <= int(t) < vocab for r in rows for t in r):
+                raise ValueError(f"bias: a dict for each of {batch} sequences, of tokens of the vocabulary")
+            width = max(1, max(len(r) for r in rows))
+            tokens, values = torch.full((batch, width), -1, dtype=torch.long), torch.zeros(batch, width)
+            for i, r in enumerate(rows):
+                tokens[i, :len(r)] = torch.tensor([int(t) for t in r], dtype=torch.long)
+                values[i, :len(r)] = torch.tensor([float(x) for x in r.values()])
+            out["bias_tokens"], out["bias_values"] = tokens.to(device), values.to(device)
+        if self.mask is not None:
+            if self.mask.dtype != torch.int32 or tuple(self.mask.shape) not in ((batch, -(-vocab // 32)), (1, -(-vocab // 32))):
+                raise ValueError(f"mask: int32 [{batch} or 1, {-(-vocab // 32)}]")
+            out["mask"] = self.mask.to(device)
+        return out
 
 
 def _full_layer(cfg: DecoderConfig, K: int, N: int, bias: bool, seed: int, device) -> synth.PackedLayer:
@@ -125,6 +166,8 @@ class DecoderLayer:
             self.norm2_b = torch.zeros(cfg.hidden, device=device, dtype=torch.float16)
         self.k_cache: Optional[torch.Tensor] = None
         self.v_cache: Optional[torch.Tensor] = None
+        self.k_prefix: Optional[torch.Tensor] = None     # [heads, positions, hd]: of a text that all sequences begin with
+        self.v_prefix: Optional[torch.Tensor] = None
 
     def linear_bytes(self) -> int:
         tot = 0
@@ -151,7 +194,9 @@ def one_launch_pays(bits: int, hidden: int, max_seq: int, sms: int) -> bool:
 
 
 class GPTQDecoder:
-    """Batch of sequences, one token per step after the prompt; greedy sampling."""
+    """Batch of sequences, one token per step after the prompt; greedy sampling, under rules for the logits where :meth:`set_rules` has some.  Attention sees
+    the whole text, the last ``cfg.window`` positions and the first ``cfg.sinks``, or a prefix that all sequences share (:meth:`share_prefix`) and
+    each one's own text."""
 
     def __init__(self, cfg: DecoderConfig, batch: int = 1, device="cuda", group=None, fused: bool = True,
                  single: bool = False, fused_allreduce: bool = False, fold_activation: Optional[bool] = None):
@@ -163,6 +208,8 @@ class GPTQDecoder:
         where the slices are short and a launch is a larger share of the step (536 against 508 tok/s at TP 2).
         ``None`` picks accordingly, and leaves the step of one sequence to the one launch for all layers where that takes
         the model (:meth:`_step_plan`); with ``True`` or ``False`` the kernels are launched one by one."""
+        if cfg.window is not None and cfg.window < 1 or cfg.sinks < 0:
+            raise ValueError("window must be at least 1, sinks at least 0")
         self.cfg, self.batch = cfg, batch
         self._fold_request = fold_activation
         self.fused = fused and cfg.head_dim in (64, 128)   # decode steps use the fused helper kernels
@@ -208,9 +255,12 @@ class GPTQDecoder:
         for L in self.layers:
             L.k_cache = torch.zeros(batch, L.heads_local, cfg.max_seq, hd, device=dev, dtype=torch.float16)
             L.v_cache = torch.zeros_like(L.k_cache)
-        inv = 1.0 / (cfg.rope_theta ** (torch.arange(0, hd, 2, device=dev).float() / hd))
-        ang = torch.arange(cfg.max_seq, device=dev).float()[:, None] * inv[None, :]
-        self.cos, self.sin = ang.cos().half(), ang.sin().half()
+        self.cos, self.sin = self._angles(0)
+        self.prefix: Optional[torch.Tensor] = None       # tokens that all sequences begin with (share_prefix)
+        self.rules: Optional[LogitRules] = None
+        self._rule_arguments: dict = {}
+        self.history: Optional[torch.Tensor] = None      # [B, prefix + max_seq], with rules: prefix, prompt and what was generated
+        self._first = torch.zeros(1, dtype=torch.long, device=dev)
         # device-side step state, so that a decode step can be replayed from a CUDA graph
         self.pos = torch.zeros(1, dtype=torch.long, device=dev)
         self.tokens = torch.zeros(batch, dtype=torch.long, device=dev)
@@ -222,6 +272,13 @@ class GPTQDecoder:
         self._pos_host = 0   # host copy of the position, for range checks
 
     # ---- pieces ----
+    def _angles(self, first: int):
+        """Cosines and sines of positions ``first .. first + max_seq - 1``."""
+        hd, dev = self.cfg.head_dim, self.device
+        inv = 1.0 / (self.cfg.rope_theta ** (torch.arange(0, hd, 2, device=dev).float() / hd))
+        ang = torch.arange(first, first + self.cfg.max_seq, device=dev).float()[:, None] * inv[None, :]
+        return ang.cos().half(), ang.sin().half()
+
     def _norm(self, x, w, b):
         if self.cfg.arch == "llama":
             return _rmsnorm(x, w)
@@ -262,8 +319,10 @@ class GPTQDecoder:
         L.k_cache.index_copy_(2, pos_idx, k)
         L.v_cache.index_copy_(2, pos_idx, v)
         if decode:
-            mask = (self.positions <= self.pos)[None, None, None, :]          # attend to the cache up to this step
+            mask = self._sight(self.positions, self.pos)[None, None, None, :]  # attend to the cache up to this step
             att = F.scaled_dot_product_attention(q, L.k_cache, L.v_cache, attn_mask=mask)
+        elif cfg.window is not None:
+            att = F.scaled_dot_product_attention(q, k, v, attn_mask=self._sight(pos_idx[None, :], pos_idx[:, None])[None, None])
         else:
             att = F.scaled_dot_product_attention(q, k, v, is_causal=True)
         att = att.transpose(1, 2).reshape(B * S, L.heads_local * hd)
@@ -277,16 +336,35 @@ class GPTQDecoder:
         x = x + self._row(L.down, act.contiguous()).reshape(B, S, cfg.hidden)
         return x
 
-    def _embed(self, tokens, pos_idx):
-        x = self.embed.index_select(0, tokens.reshape(-1)).reshape(self.batch, -1, self.cfg.hidden)
+    def _sight(self, key, query):
+        """Whether the query at one position sees the key at another."""
+        seen = key <= query
+        if self.cfg.window is not None:
+            seen = seen & ((key > query - self.cfg.window) | (key < self.cfg.sinks))
+        return seen
+
+    def _embed(self, tokens, pos_idx, before: int = 0):
+        """``before``: positions of a shared prefix, which ``pos_idx`` does not count."""
+        x = self.embed.index_select(0, tokens.reshape(-1)).reshape(tokens.shape[0], -1, self.cfg.hidden)
         if self.pos_embed is not None:
-            x = x + self.pos_embed.index_select(0, pos_idx + 2)[None]
+            x = x + self.pos_embed.index_select(0, pos_idx + (2 + before))[None]
         return x
 
     def _sample(self, x_last):
         h = self._norm(x_last, self.final_norm_w, self.final_norm_b)
         self.last_hidden = h
-        return self._pick(self._project(h))                                    # [B, vocab_local]
+        return self._pick(self._ruled(self._project(h)))                       # [B, vocab_local]
+
+    def _ruled(self, logits):
+        """The logits of the next token with the rules applied, in place; ``self.history`` ends with the token at ``self.pos``."""
+        if self.rules is None:
+            return logits
+        logits = logits.reshape(self.batch, -1)
+        before = 0 if self.prefix is None else self.prefix.numel()
+        torch.add(self.pos.expand(self.batch), before + 1, out=self._lengths)
+        v = logits[:, :self.cfg.vocab]
+        ops.adjust_logits(v, self.history, self._lengths, prompt_lens=self._prompt_lens, out=v, **self._rule_arguments)
+        return logits
 
     def _project(self, h):
         """Vocabulary projection of this rank's slice: the library's dense GEMV for a decode batch, the framework's
@@ -334,35 +412,103 @@ class GPTQDecoder:
     def prefill(self, prompt: torch.Tensor):
         """prompt: int64 [B, S]; fills the KV cache and leaves the first generated token in self.tokens."""
         B, S = prompt.shape
-        check_positions(0, S, self.cfg.max_seq)
+        before = 0 if self.prefix is None else self.prefix.numel()
+        check_positions(0, S, self._room())
         self._pos_host = S
         pos_idx = torch.arange(S, device=self.device)
-        x = self._embed(prompt, pos_idx)
+        x = self._embed(prompt, pos_idx, before)
         if self.fused and S <= 65535:
             x = self._prompt_layers(x, S)
+        elif self.prefix is not None:
+            raise ValueError("a prompt behind a shared prefix has at most 65535 tokens")
         else:
             for L in self.layers:
                 x = self._layer(L, x, pos_idx, S, decode=False)
+        if self.rules is not None:
+            self.history[:, before:before + S] = prompt
+            self._prompt_lens.fill_(before + S)
+            self.pos.fill_(S - 1)
         self.tokens.copy_(self._sample(x[:, -1]))
         self.pos.fill_(S)
 
-    def _prompt_layers(self, x, S: int):
+    def _room(self) -> int:
+        """Positions that a sequence has of its own: its rows of the caches, and behind a shared prefix what learned positions leave."""
+        taken = self.prefix.numel() if self.prefix is not None and self.pos_embed is not None else 0
+        return self.cfg.max_seq - taken
+
+    @torch.no_grad()
+    def share_prefix(self, tokens: Optional[torch.Tensor]):
+        """Let every sequence begin with ``tokens`` (int64 ``[P]``): their keys and values are computed and held once, and :meth:`prefill` and the steps
+        after it count the positions behind them.  ``None`` or no tokens: no prefix.  A captured step is dropped."""
+        cfg = self.cfg
+        if tokens is not None and (tokens.dim() != 1 or tokens.dtype != torch.long):
+            raise ValueError("a prefix is int64 [positions]")
+        P = 0 if tokens is None else tokens.numel()
+        if P and cfg.window is not None:
+            raise ValueError("a shared prefix goes with attention over the whole text")
+        if P and not self.fused:
+            raise ValueError("a shared prefix needs the fused helper kernels (heads of 64 or 128 dims)")
+        if P > 65535 or (self.pos_embed is not None and P >= cfg.max_seq):
+            raise ValueError(f"a prefix of {P} positions is too long")
+        self.graph = self._graph_plan = None
+        self.prefix = None
+        self.cos, self.sin = self._angles(0)
+        for L in self.layers:
+            L.k_prefix = L.v_prefix = None
+        if P:
+            tokens = tokens.to(self.device)
+            caches = [tuple(torch.empty(1, L.heads_local, P, cfg.head_dim, dtype=torch.float16, device=self.device) for _ in range(2)) for L in self.layers]
+            cos, sin = self.cos, self.sin
+            if P > cfg.max_seq:
+                more = [self._angles(i) for i in range(cfg.max_seq, P, cfg.max_seq)]
+                cos, sin = torch.cat([cos] + [c for c, _ in more]), torch.cat([sin] + [s for _, s in more])
+            self._prompt_layers(self._embed(tokens[None], torch.arange(P, device=self.device)), P, caches, cos, sin)
+            for L, (k, v) in zip(self.layers, caches):
+                L.k_prefix, L.v_prefix = k[0], v[0]
+            self.prefix = tokens
+            self.cos, self.sin = self._angles(P)
+        self.set_rules(self.rules)
+
+    def set_rules(self, rules: Optional[LogitRules]):
+        """Rules for the logits of every pick from now on (the next :meth:`prefill` starts their history), or None.  A captured step is dropped."""
+        if rules is not None and self.world > 1:
+            raise ValueError("rules look at the whole vocabulary: one rank")
+        self._rule_arguments = {} if rules is None else rules.arguments(self.batch, self.cfg.vocab, self.device)
+        self.rules, self.graph, self._graph_plan = rules, None, None
+        self.history = None
+        if rules is not None:
+            before = 0 if self.prefix is None else self.prefix.numel()
+            self.history = torch.full((self.batch, before + self.cfg.max_seq), -1, dtype=torch.long, device=self.device)
+            if before:
+                self.history[:, :before] = self.prefix
+            self._lengths, self._prompt_lens = (torch.full((self.batch,), before, dtype=torch.long, device=self.device) for _ in range(2))
+
+    def _prompt_layers(self, x, S: int, caches=None, cos=None, sin=None):
         """The decoder layers over a prompt with the fused helper kernels: per layer 5 small launches around the linears and
         the framework's attention (as framework element-wise kernels it was fifty, and the host could not keep up:
-        15.7 ms for 512 tokens of the Llama-7B architecture, 13 of them on the GPU)."""
-        cfg, B = self.cfg, self.batch
+        15.7 ms for 512 tokens of the Llama-7B architecture, 13 of them on the GPU).  ``caches``, ``cos``, ``sin``: those of a text of its own, one
+        sequence (the prefix)."""
+        cfg, B = self.cfg, x.shape[0]
+        alone = caches is not None
+        cos, sin = (cos, sin) if alone else (self.cos, self.sin)
         hd, rms = cfg.head_dim, cfg.arch == "llama"
         eps = 1e-6 if rms else 1e-5
         x = x.reshape(B * S, cfg.hidden).contiguous()
         h = torch.empty_like(x)
         delta = None   # output of the previous row-parallel linear, added to the residual by the next norm
-        for L in self.layers:
+        for i, L in enumerate(self.layers):
+            k_cache, v_cache = caches[i] if alone else (L.k_cache, L.v_cache)
             ops.add_norm(x, delta, L.norm1_w, L.norm1_b, h, eps, rms)
             qkv = L.qkv(h)
             q = torch.empty((B, S, L.heads_local, hd), dtype=torch.float16, device=self.device)
-            ops.rope_prompt(qkv, self.cos, self.sin, q, L.k_cache, L.v_cache, S, L.heads_local, hd, rms)
-            att = F.scaled_dot_product_attention(q.transpose(1, 2), L.k_cache[:, :, :S], L.v_cache[:, :, :S], is_causal=True)
-            delta = self._row(L.o, att.transpose(1, 2).reshape(B * S, L.heads_local * hd))
+            ops.rope_prompt(qkv, cos, sin, q, k_cache, v_cache, S, L.heads_local, hd, rms)
+            if cfg.window is not None:
+                att = ops.attn_window(q, k_cache, v_cache, self._first, cfg.window, cfg.sinks)
+            elif L.k_prefix is not None:
+                att = ops.attn_prefix(q, L.k_prefix, L.v_prefix, k_cache, v_cache, self._first)
+            else:
+                att = F.scaled_dot_product_attention(q.transpose(1, 2), k_cache[:, :, :S], v_cache[:, :, :S], is_causal=True).transpose(1, 2)
+            delta = self._row(L.o, att.reshape(B * S, L.heads_local * hd))
             ops.add_norm(x, delta, L.norm2_w, L.norm2_b, h, eps, rms)
             u = L.up(h)
             a = torch.empty((B * S, L.inter_local), dtype=torch.float16, device=self.device)
@@ -372,6 +518,9 @@ class GPTQDecoder:
 
     @torch.no_grad()
     def _decode_step(self):
+        if self.rules is not None:
+            before = 0 if self.prefix is None else self.prefix.numel()
+            self.history[:, before:].index_copy_(1, self.pos, self.tokens[:, None])
         if self.fused:
             return self._decode_step_fused()
         x = self._embed(self.tokens, self.pos)
@@ -385,8 +534,8 @@ class GPTQDecoder:
         kernels of a layer are launched one by one.  Everything that the plan points to is looked at in every step that is not replayed."""
         cfg = self.cfg
         if (self.world > 1 or self.batch != 1 or self.one_launch is False or self._fold_request is not None or self.fold_activation
-                or _module._global_forward_hooks or _module._global_forward_pre_hooks):
-            return None                            # (who says how the activation is launched gets it launched that way)
+                or _module._global_forward_hooks or _module._global_forward_pre_hooks or self.cfg.window is not None or self.prefix is not None):
+            return None                            # (its attention sees the whole of one text; who says how the activation is launched gets it launched that way)
         H, rms = cfg.hidden, cfg.arch == "llama"
         if self.one_launch is None and not one_launch_pays(cfg.bits, H, cfg.max_seq, torch.cuda.get_device_properties(self.device).multi_processor_count):
             return None
@@ -435,7 +584,7 @@ class GPTQDecoder:
         cfg, B = self.cfg, self.batch
         hd, rms = cfg.head_dim, cfg.arch == "llama"
         eps = 1e-6 if rms else 1e-5
-        x = self._embed(self.tokens, self.pos).reshape(B, cfg.hidden).contiguous()
+        x = self._embed(self.tokens, self.pos, 0 if self.prefix is None else self.prefix.numel()).reshape(B, cfg.hidden).contiguous()
         h = torch.empty_like(x)
         delta = None   # output of the previous row-parallel linear, added to the residual by the next norm
         plan = self._step_plan()
@@ -444,8 +593,16 @@ class GPTQDecoder:
             ops.add_norm(x, delta, L.norm1_w, L.norm1_b, h, eps, rms)
             qkv = L.qkv(h)
             att = torch.empty((B, L.heads_local * hd), dtype=torch.float16, device=self.device)
-            # rotary embedding, cache write and single-query attention in one launch
-            ops.attn_step(qkv, self.cos, self.sin, self.pos, L.k_cache, L.v_cache, att, L.heads_local, hd, rms)
+            if cfg.window is not None or L.k_prefix is not None:
+                q = torch.empty((B, 1, L.heads_local, hd), dtype=torch.float16, device=self.device)
+                ops.rope_cache(qkv, self.cos, self.sin, self.pos, q, L.k_cache, L.v_cache, L.heads_local, hd, rms)
+                if cfg.window is not None:
+                    ops.attn_window(q, L.k_cache, L.v_cache, self.pos, cfg.window, cfg.sinks, out=att.view_as(q))
+                else:
+                    ops.attn_prefix(q, L.k_prefix, L.v_prefix, L.k_cache, L.v_cache, self.pos, out=att.view_as(q))
+            else:
+                # rotary embedding, cache write and single-query attention in one launch
+                ops.attn_step(qkv, self.cos, self.sin, self.pos, L.k_cache, L.v_cache, att, L.heads_local, hd, rms)
             o = self._row(L.o, att)
             ops.add_norm(x, o, L.norm2_w, L.norm2_b, h, eps, rms)
             u = L.up(h)
@@ -458,7 +615,7 @@ class GPTQDecoder:
                 delta = self._row(L.down, a)
         ops.add_norm(x, delta, self.final_norm_w, self.final_norm_b, h, eps, rms)
         self.last_hidden = h
-        logits = self._project(h)
+        logits = self._ruled(self._project(h))
         if (logits.dtype is torch.float16 and logits.is_contiguous()
                 and (self.world == 1 or (self.exchange is not None and B <= 8))):   # the exchange takes up to 8 rows
             # greedy pick and the step's position in the library's kernels: one launch on one GPU, two around the
@@ -479,7 +636,7 @@ class GPTQDecoder:
 
     def capture(self):
         """Warm up (allocates scratch, builds run-time views) and capture one decode step in a CUDA graph."""
-        check_positions(self._pos_host, 3, self.cfg.max_seq)   # two warm-up steps and the captured one
+        check_positions(self._pos_host, 3, self._room())   # two warm-up steps and the captured one
         saved_pos, saved_tok = self.pos.clone(), self.tokens.clone()
         if self.fused:
             self._step_plan()                      # its memory is the caller's stream's, where the graph is replayed, not the warm-up's
@@ -512,7 +669,7 @@ class GPTQDecoder:
         Returns {kind: tuning}; a batch of more than 8 rows is left alone."""
         kinds = ("qkv", "o", "up", "down")
         chosen = {k: getattr(self.layers[0], k).gemv_tuning for k in kinds}
-        if self.batch > 8 or self._pos_host + steps + 3 > self.cfg.max_seq:
+        if self.batch > 8 or self._pos_host + steps + 3 > self._room():
             return chosen
         dev = self.device
 
@@ -553,7 +710,7 @@ class GPTQDecoder:
         return chosen
 
     def decode(self, steps: int) -> torch.Tensor:
-        check_positions(self._pos_host, steps, self.cfg.max_seq)
+        check_positions(self._pos_host, steps, self._room())
         self._pos_host += steps
         out = torch.empty(steps, self.batch, dtype=torch.long, device=self.device)
         for i in range(steps):
@@ -571,7 +728,7 @@ class GPTQDecoder:
         import collections
         from torch.profiler import ProfilerActivity, profile
         torch.cuda.synchronize(self.device)
-        if self._pos_host >= self.cfg.max_seq:     # the caches are full: trace a repeat of the last position
+        if self._pos_host >= self._room():     # the caches are full: trace a repeat of the last position
             self._pos_host -= 1
             self.pos.sub_(1)
         with profile(activities=[ProfilerActivity.CUDA]) as prof:
