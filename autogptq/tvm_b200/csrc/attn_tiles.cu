@@ -21,8 +21,8 @@
 // Rows of V that no row of the tiles sees are zeroed in shared memory before they are multiplied (a weight of zero times a NaN is one).  Where rows of the
 // tiles see different keys and one of these holds a NaN or an infinity, the rows that come out not finite are done again, key by key.
 //
-// PACKED: the rows are (sequence, token, head of the group) of the whole batch against the shared prefix, split over CTAs, sums to scratch.  Up to 128 rows: both
-// tiles of Q are the same rows, one takes the even units of keys and the other the odd ones.
+// PACKED: the rows are (sequence, token, head of the group) of the whole batch against the shared prefix, split over CTAs, sums to scratch.
+// ALT (few rows): both tiles of Q are the same rows, one takes the even units of keys and the other the odd ones; they add up at the end.
 #include <cuda.h>
 
 #include <algorithm>
@@ -160,7 +160,7 @@ struct TileArgs {
     b200gptq_attn_args a;
     float* part;
     float sl2;                // |scale| log2 e, and Q is negated where the scale is negative
-    int negate, pairs, splits, prefix_units, group;
+    int negate, tiles, splits, prefix_units, group, alt;
 };
 
 template <typename T, int HD, bool PACKED>
@@ -215,10 +215,10 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     const int G = p.group, window = a.window ? a.window : 1 << 30;
     const int split = PACKED ? blockIdx.x % p.splits : 0, part_unit = PACKED ? blockIdx.x / p.splits : blockIdx.x;
     const int kh = part_unit % a.kv_heads, b0 = PACKED ? 0 : part_unit / a.kv_heads % a.batch;
-    const int pair = p.pairs - 1 - part_unit / a.kv_heads / (PACKED ? 1 : a.batch), row0 = pair * 2 * kRows;
+    const bool alt = p.alt;                   // both tiles are the same rows
+    const int row0 = (p.tiles - 1 - part_unit / a.kv_heads / (PACKED ? 1 : a.batch)) * (alt ? kRows : 2 * kRows);
     const int pos0 = PACKED ? 0 : attn_pos(a, b0);
     const int rows_all = PACKED ? a.batch * a.tokens * G : attn_count(a, b0) * G;
-    const bool alt = PACKED && rows_all <= kRows;       // both tiles are the same rows
     int nrows[2], p_lo[2], p_hi[2];
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
@@ -300,7 +300,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         const uint32_t ts = tmem + 128u * q, to = tmem + kColO + 128u * q;
         const Region r0 = region(q, 0), r1 = region(q, 1), r2 = region(q, 2);
         auto needs = [&](int i) {
-            return alt ? i < r0.end && (i & 1) == q : (i >= r0.begin && i < r0.end) || (i >= r1.begin && i < r1.end) || (i >= r2.begin && i < r2.end);
+            return (!alt || (i & 1) == q) && ((i >= r0.begin && i < r0.end) || (i >= r1.begin && i < r1.end) || (i >= r2.begin && i < r2.end));
         };
         int started = 0, mixed = 0;           // S begun, weights multiplied
         auto qk = [&](uint32_t at) {
@@ -341,24 +341,34 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
             }
-            {
-                mbar_wait(full(s), round & 1, &abort_flag);
-                if (mine) mbar_wait(p_full(q, mixed & 1), (mixed >> 1) & 1, &abort_flag);
+            mbar_wait(full(s), round & 1, &abort_flag);
+            __syncwarp();
+            // (an S that is free already, as where the tile takes every other unit, is filled at once, the softmax need not wait for it)
+            bool next = mine2;
+            if (next && started - mixed < 2) {
+                tc_after();
+                qk(at + SM::unit);
+                ++started;
+                next = false;
+            }
+            if (mine) {
+                mbar_wait(p_full(q, mixed & 1), (mixed >> 1) & 1, &abort_flag);
                 __syncwarp();
                 tc_after();
-                if (mine) {
-                    const uint64_t vd = smem_desc(at, BOX);
+                const uint64_t vd = smem_desc(at, BOX);
 #pragma unroll
-                    for (int k = 0; k < kKeys / 16; ++k)
-                        mma_ts(to, ts + 64u * (mixed & 1) + 8u * k, vd + k * (2048 >> 4), idesc_pv, (mixed > 0 || k > 0) ? 1u : 0u, lead);
-                    mma_commit(o_done(q), lead);
-                }
-                if (mine2) qk(at + SM::unit);
-                if (mine || mine2) mma_commit(empty(s), lead);
-                else if (lead) mbar_arrive(empty(s));
+                for (int k = 0; k < kKeys / 16; ++k)
+                    mma_ts(to, ts + 64u * (mixed & 1) + 8u * k, vd + k * (2048 >> 4), idesc_pv, (mixed > 0 || k > 0) ? 1u : 0u, lead);
+                mma_commit(o_done(q), lead);
+                ++mixed;
             }
-            mixed += mine;
-            started += mine2;
+            if (next) {
+                tc_after();
+                qk(at + SM::unit);
+                ++started;
+            }
+            if (mine || mine2) mma_commit(empty(s), lead);
+            else if (lead) mbar_arrive(empty(s));
             __syncwarp();
             if (++s == ST) { s = 0; ++round; }
         }
@@ -376,21 +386,22 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         const int idx = row_first + min(r, max(rows, 1) - 1), token = idx / G, head = kh * G + idx - token * G;
         const int b = PACKED ? token / a.tokens : b0, t = PACKED ? token - b * a.tokens : token, pr = pos0 + token;
         const long long q_at = b * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2];
-        // Q, in the swizzled layout of the tiles: 16 bytes per thread and turn, eight of them on their way at once
+        // Q, in the swizzled layout of the tiles: 16 bytes per thread and turn, all of them on their way at once
         if (!(alt && q == 1)) {
+            constexpr int QB = HD / 8;
             uint8_t* dst = base_ptr + q * SM::q_tile;
 #pragma unroll 1
-            for (int x0 = 0; x0 < HD / 8; x0 += 8) {
-                uint4 val[8];
+            for (int x0 = 0; x0 < HD / 8; x0 += QB) {
+                uint4 val[QB];
 #pragma unroll
-                for (int x = 0; x < 8; ++x) {
+                for (int x = 0; x < QB; ++x) {
                     const int rw = ((x0 + x) * 32 + lane) / (HD / 8), c = lane % (HD / 8);
                     const long long from = __shfl_sync(0xffffffffu, q_at, rw);
                     val[x] = make_uint4(0, 0, 0, 0);
                     if (32 * quarter + rw < rows) val[x] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + from + 8 * c));
                 }
 #pragma unroll
-                for (int x = 0; x < 8; ++x) {
+                for (int x = 0; x < QB; ++x) {
                     const int rr = 32 * quarter + ((x0 + x) * 32 + lane) / (HD / 8), c = lane % (HD / 8);
                     if (p.negate) { val[x].x ^= 0x80008000u; val[x].y ^= 0x80008000u; val[x].z ^= 0x80008000u; val[x].w ^= 0x80008000u; }
                     *reinterpret_cast<uint4*>(dst + (c / 8) * QBOX + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = val[x];
@@ -408,10 +419,10 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           const Region v = region(q, g);
           // A unit whose keys all rows of the tile see: from key `least` to key `most`
           const int most = min(g == 1 ? min(v.j_end, a.sinks) : v.j_end, g == 0 ? v.j_end : of(p_lo, q) + 1) - kKeys, least = g == 2 ? of(p_hi, q) - window + 1 : 0;
-          int j0 = v.j_first + (alt ? q * kKeys : 0);
-          const int step = alt ? 2 : 1;
+          const int skip = alt ? (v.begin ^ q) & 1 : 0, step = alt ? 2 : 1;
+          int j0 = v.j_first + skip * kKeys;
 #pragma unroll 1
-          for (int i = v.begin + (alt ? q : 0); i < v.end; i += step, j0 += step * kKeys) {
+          for (int i = v.begin + skip; i < v.end; i += step, j0 += step * kKeys) {
             const uint32_t tb = ts + 64u * (turn & 1);
             // (A wait that runs out is not looked at before the end: those after it give up at once, and the results are not defined then.)
             mbar_wait(s_full(q, turn & 1), (turn >> 1) & 1, &abort_flag);
@@ -492,24 +503,29 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         ok = __all_sync(0xffffffffu, !abort_flag);
         tc_after();
         const long long rows_total = (long long)a.batch * a.tokens * a.heads;
-        if constexpr (PACKED) {
-            // Sums in fp32, through shared memory so that rows are written whole (with one thread per row 4 us more); up to 128 rows both tiles add up.  For 128
-            // dims the tiles lie where the ring was, for 64 over Q too: what each tile multiplies has been multiplied when both have met here.
+        if (PACKED || alt) {
+            // Sums in fp32, through shared memory: so that rows are written whole (with one thread per row 4 us more), and that two tiles which are the same rows
+            // add up.  For 128 dims they lie where the ring was, for 64 over Q too: what each tile multiplies has been multiplied when both have met here.
             constexpr int CH = HD / 4;          // 16-byte pieces of a row
             float4* stage = reinterpret_cast<float4*>(base_ptr + (HD == 128 ? SM::ring : 0));
             float (*stats)[2][kRows] = reinterpret_cast<float (*)[2][kRows]>(stage + 2 * kRows * CH);              // behind them: [tile][maximum, denominator][row]
-            long long (*places)[kRows] = reinterpret_cast<long long (*)[kRows]>(stats + 2);                         // and the rows' places among the sums
-            static_assert((HD == 128 ? SM::ring : 0) + 2 * kRows * HD * 4 + 2 * kRows * 16 <= SM::total - 1024, "");
-            tc_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(all_met);
-            if (ok) ok = mbar_wait(all_met, 0, &abort_flag);
-            ok = __all_sync(0xffffffffu, ok);
-            tc_after();
+            long long (*places)[kRows] = reinterpret_cast<long long (*)[kRows]>(stats + 2);                         // the rows' places among the sums, or in out
+            int* flags = reinterpret_cast<int*>(places + 2);                                                        // rows that are done again
+            static_assert((HD == 128 ? SM::ring : 0) + 2 * kRows * HD * 4 + 2 * kRows * 16 + kRows * 4 <= SM::total - 1024, "");
+            auto meet = [&](int phase) {
+                tc_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(all_met);
+                if (ok) ok = mbar_wait(all_met, phase & 1, &abort_flag);
+                ok = __all_sync(0xffffffffu, ok);
+                tc_after();
+            };
+            meet(0);
             if (ok && mine) {
-                places[q][r] = split * rows_total + (long long)token * a.heads + head;
+                places[q][r] = PACKED ? split * rows_total + (long long)token * a.heads + head : b * a.out_stride[0] + t * a.out_stride[1] + head * a.out_stride[2];
                 stats[q][0][r] = m * p.sl2;
                 stats[q][1][r] = l;
+                if (q == 0) flags[r] = 0;
 #pragma unroll 1
                 for (int c = 0; c < HD / 32; ++c) {
                     uint32_t o[32];
@@ -524,10 +540,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                     }
                 }
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(all_met);
-            if (ok) ok = mbar_wait(all_met, 1, &abort_flag);
-            ok = __all_sync(0xffffffffu, ok);
+            meet(1);
             float* ml = p.part + p.splits * rows_total * HD;
             const int all = alt ? nrows[0] : nrows[0] + nrows[1];
             for (int x = threadIdx.x; ok && x < all * CH; x += kSoftmaxWarps * 32) {
@@ -542,8 +555,26 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                     tl = tl * e0 + stats[1][1][row] * e1;
                     tm = both;
                 }
-                *reinterpret_cast<float4*>(p.part + at * HD + 4 * chunk) = f;
-                if (chunk == 0) *reinterpret_cast<float2*>(ml + 2 * at) = make_float2(tm, tl);
+                if constexpr (PACKED) {
+                    *reinterpret_cast<float4*>(p.part + at * HD + 4 * chunk) = f;
+                    if (chunk == 0) *reinterpret_cast<float2*>(ml + 2 * at) = make_float2(tm, tl);
+                } else {
+                    // (nothing seen: zero; a NaN or an infinity in V that the row does not see: done again below)
+                    const float inv = tl != 0.f ? 1.f / tl : 0.f;
+                    if (tl == 0.f) f = make_float4(0.f, 0.f, 0.f, 0.f);
+                    f = make_float4(f.x * inv, f.y * inv, f.z * inv, f.w * inv);
+                    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at + 4 * chunk) = make_uint2(Half<T>::pack(f.x, f.y), Half<T>::pack(f.z, f.w));
+                    if (!isfinite(f.x) || !isfinite(f.y) || !isfinite(f.z) || !isfinite(f.w)) flags[row] = 1;
+                }
+            }
+            if constexpr (!PACKED) {
+                meet(2);
+                unsigned again = __ballot_sync(0xffffffffu, ok && q == 0 && r < rows && flags[r]);
+                while (again) {
+                    const int from = __ffs(again) - 1, t2 = __shfl_sync(0xffffffffu, t, from);
+                    again &= again - 1;
+                    attn_row_again<T, HD>(a, b0, t2, __shfl_sync(0xffffffffu, head, from), pos0 + t2, 0, HD);
+                }
             }
         } else if (ok && mine) {
             const float inv = l != 0.f ? 1.f / l : 0.f;
@@ -610,7 +641,7 @@ bool encode(CUtensorMap* m, bool bf16, int hd, const void* ptr, int rank, const 
 }
 
 template <typename T, int HD, bool PACKED>
-int run(const b200gptq_attn_args& a, float* part, int splits, cudaStream_t stream) {
+int run(const b200gptq_attn_args& a, float* part, int splits, bool alt, cudaStream_t stream) {
     static std::once_flag once[64];
     static cudaError_t result[64];
     auto* kernel = attn_tiles_kernel<T, HD, PACKED>;
@@ -636,10 +667,12 @@ int run(const b200gptq_attn_args& a, float* part, int splits, cudaStream_t strea
     t.negate = a.scale < 0.f;
     t.splits = splits;
     t.group = a.heads / a.kv_heads;
+    t.alt = alt;
     t.prefix_units = (int)((a.prefix + kKeys - 1) / kKeys);
     const long long rows = (long long)a.tokens * (a.heads / a.kv_heads) * (PACKED ? a.batch : 1);
-    t.pairs = (int)((rows + 2 * kRows - 1) / (2 * kRows));
-    const long long ctas = (long long)t.pairs * a.kv_heads * (PACKED ? splits : a.batch);
+    const int per_cta = alt ? kRows : 2 * kRows;
+    t.tiles = (int)((rows + per_cta - 1) / per_cta);
+    const long long ctas = (long long)t.tiles * a.kv_heads * (PACKED ? splits : a.batch);
     if (ctas > 0x7fffffff) return B200GPTQ_ERR_TOO_LARGE;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)ctas);
@@ -656,10 +689,10 @@ int run(const b200gptq_attn_args& a, float* part, int splits, cudaStream_t strea
 }
 
 template <bool PACKED>
-int run_any(const b200gptq_attn_args& a, float* part, int splits, cudaStream_t stream) {
+int run_any(const b200gptq_attn_args& a, float* part, int splits, bool alt, cudaStream_t stream) {
     if (a.dtype == B200GPTQ_F16)
-        return a.hd == 128 ? run<__half, 128, PACKED>(a, part, splits, stream) : run<__half, 64, PACKED>(a, part, splits, stream);
-    return a.hd == 128 ? run<__nv_bfloat16, 128, PACKED>(a, part, splits, stream) : run<__nv_bfloat16, 64, PACKED>(a, part, splits, stream);
+        return a.hd == 128 ? run<__half, 128, PACKED>(a, part, splits, alt, stream) : run<__half, 64, PACKED>(a, part, splits, alt, stream);
+    return a.hd == 128 ? run<__nv_bfloat16, 128, PACKED>(a, part, splits, alt, stream) : run<__nv_bfloat16, 64, PACKED>(a, part, splits, alt, stream);
 }
 
 }  // namespace
@@ -676,8 +709,14 @@ bool attn_tiles_maps(const b200gptq_attn_args& a, bool prefix) {
     return true;
 }
 
-int attn_tiles_dispatch(const b200gptq_attn_args& a, cudaStream_t stream) { return run_any<false>(a, nullptr, 1, stream); }
+// One tile of rows per CTA, its units shared by both halves, where all tiles then run at once; else two.
+int attn_tiles_dispatch(const b200gptq_attn_args& a, cudaStream_t stream) {
+    const long long tiles = ((long long)a.tokens * (a.heads / a.kv_heads) + kRows - 1) / kRows * a.kv_heads * a.batch;
+    return run_any<false>(a, nullptr, 1, tiles <= sm_count(), stream);
+}
 
-int attn_tiles_prefix(const b200gptq_attn_args& a, float* part, int parts, cudaStream_t stream) { return run_any<true>(a, part, parts, stream); }
+int attn_tiles_prefix(const b200gptq_attn_args& a, float* part, int parts, cudaStream_t stream) {
+    return run_any<true>(a, part, parts, (long long)a.batch * a.tokens * (a.heads / a.kv_heads) <= kRows, stream);
+}
 
 }  // namespace b200gptq
