@@ -66,14 +66,17 @@ template <int HD, int R, int W> struct Lay {
 // (and the prefix itself, where with_prefix, or its `parts` sums).  A tile of R rows is blockIdx.x / splits % row_tiles.
 template <typename T, int HD, int R, int W, bool PREFIX>
 __global__ void __launch_bounds__(W * 32, R == 8 ? 16 / W : 1)
-attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict__ part, int splits, int row_tiles, int parts, int with_prefix) {
+attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict__ part, int split_bits, int row_tiles, int parts, int with_prefix, int G) {
     using L = Lay<HD, R, W>;
     constexpr int MT = R == 8 ? 1 : R / 16, SEG = HD / 32, HH = HD / 64, kThreads = W * 32;
     extern __shared__ __align__(16) float sm[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const int G = a.heads / a.kv_heads, window = a.window ? a.window : 1 << 30;
-    const int split = blockIdx.x % splits, unit = blockIdx.x / splits, tile = unit % row_tiles;
-    const int kh = unit / row_tiles % a.kv_heads, b0 = unit / row_tiles / a.kv_heads;        // (PREFIX: b0 = 0)
+    // (Divisions are few, and not of 64 bits: a call for one token lasts 6 us, and each takes 50 to 200 ns.)
+    const int window = a.window ? a.window : 1 << 30, splits = PREFIX ? parts : 1 << split_bits;
+    const unsigned per_unit = PREFIX ? blockIdx.x / splits : blockIdx.x >> split_bits, unit = row_tiles == 1 ? per_unit : per_unit / row_tiles;
+    const int split = blockIdx.x - per_unit * splits, tile = per_unit - unit * row_tiles;
+    const int b0 = PREFIX ? 0 : unit / (unsigned)a.kv_heads, kh = unit - b0 * a.kv_heads;
+    auto token_of = [&](int idx) { return !PREFIX && a.tokens == 1 ? 0 : (int)((unsigned)idx / (unsigned)G); };       // of row idx
     // What is read below was written before the launch in front of this one ended, or began (behind the prefix launch, which lets this one
     // start only after it has itself waited; the loads by-pass L1).
     if (!PREFIX && splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
@@ -90,11 +93,13 @@ attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict
     }
     // ---- keys: the prefix, the sinks, the window ----
     AttnRange range = {0, 0, 0};
-    const int p_lo = p0 + row0 / G, p_hi = p0 + (row0 + nrows - 1) / G;
+    const int p_lo = PREFIX ? 0 : p0 + token_of(row0), p_hi = PREFIX ? 0 : p0 + token_of(row0 + nrows - 1);
     if constexpr (!PREFIX) range = attn_range(p_lo, p_hi, window, a.sinks, a.max_seq);
     const int n_p = PREFIX || with_prefix ? (a.prefix + kBlock - 1) / kBlock : 0, n_s = n_p + (range.s_end + kBlock - 1) / kBlock,
               nb = n_s + (range.w_end - range.w_start + kBlock - 1) / kBlock;
-    const int first = (int)((long long)nb * split / splits), last = (int)((long long)nb * (split + 1) / splits);
+    int first, last;
+    if constexpr (PREFIX) { first = (int)((long long)nb * split / splits); last = (int)((long long)nb * (split + 1) / splits); }
+    else { first = (int)((long long)nb * split >> split_bits); last = (int)((long long)nb * (split + 1) >> split_bits); }
     const T *k_own = nullptr, *v_own = nullptr, *k_front = nullptr, *v_front = nullptr;
     if constexpr (!PREFIX) {
         k_own = static_cast<const T*>(a.k_cache) + b0 * a.k_stride[0] + kh * a.k_stride[1];
@@ -141,7 +146,7 @@ attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict
     // ---- the rows' places in q, out and the scratch (divisions once per row), queries ----
     long long* places = reinterpret_cast<long long*>(sm + L::places);
     if (threadIdx.x < R) {
-        const int idx = row0 + min((int)threadIdx.x, nrows - 1), tok = idx / G, head = kh * G + idx - tok * G;
+        const int idx = row0 + min((int)threadIdx.x, nrows - 1), tok = token_of(idx), head = kh * G + idx - tok * G;
         const int bb = PREFIX ? tok / a.tokens : b0, t = PREFIX ? tok - bb * a.tokens : tok;
         places[threadIdx.x] = bb * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2];
         places[R + threadIdx.x] = bb * a.out_stride[0] + t * a.out_stride[1] + head * a.out_stride[2];
@@ -167,7 +172,7 @@ attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             m[t][r] = -INFINITY; l[t][r] = 0.f;
-            pr[t][r] = p0 + (row0 + min(R == 8 ? 2 * c + r : 16 * t + 8 * r + g, nrows - 1)) / G;
+            pr[t][r] = PREFIX ? 0 : p0 + token_of(row0 + min(R == 8 ? 2 * c + r : 16 * t + 8 * r + g, nrows - 1));
         }
     }
     for (; i < last; i += W) {
@@ -331,7 +336,8 @@ attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict
     __syncthreads();
     if (!PREFIX && splits > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");      // (all CTAs of the cluster run)
     // ---- the CTA's sums: to the scratch, or slice by slice to the CTAs of the cluster ----
-    const int slice = PREFIX ? HD : HD / splits;
+    const int slice = PREFIX ? HD : HD >> split_bits;
+    constexpr int HD_BITS = HD == 128 ? 7 : 6;
     const long long rows_total = (long long)a.batch * a.tokens * a.heads;
     for (int x = threadIdx.x; x < nrows * HD; x += kThreads) {
         const int row = x / HD, d = x % HD;
@@ -350,7 +356,7 @@ attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict
             part[at * HD + d] = ca;
             if (d == 0) *reinterpret_cast<float2*>(part + splits * rows_total * HD + 2 * at) = make_float2(cm, cl);
         } else {
-            const int to = d / slice;
+            const int to = d >> (HD_BITS - split_bits);
             st_cluster(sm + L::slice + (split * R + row) * slice + d - to * slice, to, ca);
             if (d - to * slice == 0) {
                 st_cluster(sm + L::slice_ml + 2 * (split * R + row), to, cm);
@@ -393,7 +399,7 @@ attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict
         __syncthreads();
     }
     for (int x = threadIdx.x; x < nrows * (slice / 4); x += kThreads) {
-        const int row = x / (slice / 4), d = (x - row * (slice / 4)) * 4;
+        const int row = x >> (HD_BITS - split_bits - 2), d = (x - row * (slice / 4)) * 4;
         const long long at = places[2 * R + row];
         const float2* w = wl + row * runs;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -427,8 +433,8 @@ attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict
         __syncthreads();
         for (int row = warp; row < nrows; row += W)
             if (flags[row]) {
-                const int idx = row0 + row;
-                attn_row_again<T, HD>(a, b0, idx / G, kh * G + idx % G, p0 + idx / G, split * slice, (split + 1) * slice);
+                const int idx = row0 + row, t = token_of(idx);
+                attn_row_again<T, HD>(a, b0, t, kh * G + idx - t * G, p0 + t, split * slice, (split + 1) * slice);
             }
     }
 }
@@ -468,7 +474,9 @@ int run(const b200gptq_attn_args& a, float* part, const AttnPlan& s, cudaStream_
     }
     cfg.attrs = attr;
     cfg.numAttrs = n;
-    B200GPTQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a, part, splits, tiles, s.parts, a.prefix && !s.parts ? 1 : 0));
+    int bits = 0;
+    while ((1 << bits) < splits) ++bits;      // (a cluster has 1, 2, 4 or 8 CTAs)
+    B200GPTQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a, part, bits, tiles, s.parts, a.prefix && !s.parts ? 1 : 0, a.heads / a.kv_heads));
     return B200GPTQ_OK;
 }
 
