@@ -426,17 +426,16 @@ attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict
         o = make_float4(none ? 0.f : o.x / tl, none ? 0.f : o.y / tl, none ? 0.f : o.z / tl, none ? 0.f : o.w / tl);
         *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + places[R + row] + split * slice + d) =
             make_uint2(Half<T>::pack(o.x, o.y), Half<T>::pack(o.z, o.w));
-        if (!isfinite(o.x) || !isfinite(o.y) || !isfinite(o.z) || !isfinite(o.w)) flags[row] = 1;
+        if (isfinite(tl) && (!isfinite(o.x) || !isfinite(o.y) || !isfinite(o.z) || !isfinite(o.w))) flags[row] = 1;
     }
-    // rows of several tokens in one tile: a NaN may come from a row of the cache that this one does not see
-    if (p_hi > p_lo) {
-        __syncthreads();
-        for (int row = warp; row < nrows; row += W)
-            if (flags[row]) {
-                const int idx = row0 + row, t = token_of(idx);
-                attn_row_again<T, HD>(a, b0, t, kh * G + idx - t * G, p0 + t, split * slice, (split + 1) * slice);
-            }
-    }
+    // A weight of zero times a NaN or an infinity, of a key that the row does not see or that stands in for one behind the end: the row is done again.  (Not
+    // where the denominator is not finite: then a score that the row sees is a NaN.)
+    __syncthreads();
+    for (int row = warp; row < nrows; row += W)
+        if (flags[row]) {
+            const int idx = row0 + row, t = token_of(idx);
+            attn_row_again<T, HD>(a, b0, t, kh * G + idx - t * G, p0 + t, split * slice, (split + 1) * slice);
+        }
 }
 
 template <typename T, int HD, int R, int W, bool PREFIX>

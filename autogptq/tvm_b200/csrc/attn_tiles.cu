@@ -213,10 +213,11 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 
     // ---- which rows, which keys.  The last rows of a prompt see most, and come first. ----
     const int G = p.group, window = a.window ? a.window : 1 << 30;
-    const int split = PACKED ? blockIdx.x % p.splits : 0, part_unit = PACKED ? blockIdx.x / p.splits : blockIdx.x;
-    const int kh = part_unit % a.kv_heads, b0 = PACKED ? 0 : part_unit / a.kv_heads % a.batch;
+    const unsigned part_unit = PACKED ? blockIdx.x / (unsigned)p.splits : blockIdx.x, over_heads = part_unit / (unsigned)a.kv_heads;
+    const unsigned row_tile = PACKED ? over_heads : over_heads / (unsigned)a.batch;
+    const int split = PACKED ? blockIdx.x - part_unit * p.splits : 0, kh = part_unit - over_heads * a.kv_heads, b0 = PACKED ? 0 : over_heads - row_tile * a.batch;
     const bool alt = p.alt;                   // both tiles are the same rows
-    const int row0 = (p.tiles - 1 - part_unit / a.kv_heads / (PACKED ? 1 : a.batch)) * (alt ? kRows : 2 * kRows);
+    const int row0 = (p.tiles - 1 - (int)row_tile) * (alt ? kRows : 2 * kRows);
     const int pos0 = PACKED ? 0 : attn_pos(a, b0);
     const int rows_all = PACKED ? a.batch * a.tokens * G : attn_count(a, b0) * G;
     int nrows[2], p_lo[2], p_hi[2];
@@ -224,8 +225,8 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     for (int q = 0; q < 2; ++q) {
         const int r = row0 + (alt ? 0 : q * kRows);
         nrows[q] = max(0, min(kRows, rows_all - r));
-        p_lo[q] = pos0 + r / G;
-        p_hi[q] = pos0 + (r + max(nrows[q], 1) - 1) / G;
+        p_lo[q] = PACKED ? 0 : pos0 + (int)((unsigned)r / (unsigned)G);
+        p_hi[q] = PACKED ? 0 : pos0 + (int)((unsigned)(r + max(nrows[q], 1) - 1) / (unsigned)G);
     }
     auto of = [](const int (&v)[2], int q) { return q ? v[1] : v[0]; };       // (registers, not an array that is indexed)
     // Units of three regions, one after the other: the prefix, the sinks, the window (which begin where the keys begin; where sinks and window meet, they
@@ -383,8 +384,8 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         const bool mine = 32 * quarter < rows;          // the warp has rows at all
         // The thread's row.  (The divisions once per row; where other threads need its place they ask for it.  With the divisions where Q is loaded and where O
         // is stored these took 6500 and 4000 clk.)
-        const int idx = row_first + min(r, max(rows, 1) - 1), token = idx / G, head = kh * G + idx - token * G;
-        const int b = PACKED ? token / a.tokens : b0, t = PACKED ? token - b * a.tokens : token, pr = pos0 + token;
+        const int idx = row_first + min(r, max(rows, 1) - 1), token = (int)((unsigned)idx / (unsigned)G), head = kh * G + idx - token * G;
+        const int b = PACKED ? (int)((unsigned)token / (unsigned)a.tokens) : b0, t = PACKED ? token - b * a.tokens : token, pr = pos0 + token;
         const long long q_at = b * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2];
         // Q, in the swizzled layout of the tiles: 16 bytes per thread and turn, all of them on their way at once
         if (!(alt && q == 1)) {
@@ -541,35 +542,53 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                 }
             }
             meet(1);
-            float* ml = p.part + p.splits * rows_total * HD;
-            const int all = alt ? nrows[0] : nrows[0] + nrows[1];
-            for (int x = threadIdx.x; ok && x < all * CH; x += kSoftmaxWarps * 32) {
-                const int row = x / CH, chunk = x % CH;
-                const long long at = places[row / kRows][row % kRows];
-                float4 f = stage[row * CH + (chunk ^ (row & 7))];
-                float tm = stats[row / kRows][0][row % kRows], tl = stats[row / kRows][1][row % kRows];
+            // A warp takes whole rows; a lane knows one of them: what its tiles' sums count, and where it goes.
+            const int all = alt ? nrows[0] : nrows[0] + nrows[1], per_warp = alt ? kRows / kSoftmaxWarps : 2 * kRows / kSoftmaxWarps, row_0 = warp * per_warp;
+            float w0 = 1.f, w1 = 0.f;
+            long long place = 0;
+            if (ok && lane < per_warp && row_0 + lane < all) {
+                const int row = row_0 + lane, tile = row / kRows, at = row % kRows;
+                place = places[tile][at];
+                float tm = stats[tile][0][at], tl = stats[tile][1][at];
                 if (alt) {
-                    const float4 g = stage[(kRows + row) * CH + (chunk ^ (row & 7))];
-                    const float um = stats[1][0][row], both = fmaxf(tm, um), safe = both == -INFINITY ? 0.f : both, e0 = exp2_fast(tm - safe), e1 = exp2_fast(um - safe);
-                    f = make_float4(f.x * e0 + g.x * e1, f.y * e0 + g.y * e1, f.z * e0 + g.z * e1, f.w * e0 + g.w * e1);
-                    tl = tl * e0 + stats[1][1][row] * e1;
+                    const float um = stats[1][0][at], both = fmaxf(tm, um), safe = both == -INFINITY ? 0.f : both;
+                    w0 = exp2_fast(tm - safe);
+                    w1 = exp2_fast(um - safe);
+                    tl = tl * w0 + stats[1][1][at] * w1;
                     tm = both;
                 }
                 if constexpr (PACKED) {
-                    *reinterpret_cast<float4*>(p.part + at * HD + 4 * chunk) = f;
-                    if (chunk == 0) *reinterpret_cast<float2*>(ml + 2 * at) = make_float2(tm, tl);
+                    *reinterpret_cast<float2*>(p.part + p.splits * rows_total * HD + 2 * place) = make_float2(tm, tl);
                 } else {
-                    // (nothing seen: zero; a NaN or an infinity in V that the row does not see: done again below)
-                    const float inv = tl != 0.f ? 1.f / tl : 0.f;
-                    if (tl == 0.f) f = make_float4(0.f, 0.f, 0.f, 0.f);
-                    f = make_float4(f.x * inv, f.y * inv, f.z * inv, f.w * inv);
-                    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at + 4 * chunk) = make_uint2(Half<T>::pack(f.x, f.y), Half<T>::pack(f.z, f.w));
-                    if (!isfinite(f.x) || !isfinite(f.y) || !isfinite(f.z) || !isfinite(f.w)) flags[row] = 1;
+                    const float inv = tl != 0.f ? 1.f / tl : 0.f;         // (nothing seen: zero)
+                    if (!isfinite(tl)) flags[at] = -1;                    // (a score that the row sees is a NaN)
+                    w0 *= inv;
+                    w1 *= inv;
                 }
             }
+            if (ok)
+#pragma unroll 4
+                for (int x = 0; x < per_warp * CH / 32; ++x) {
+                    const int rw = (x * 32 + lane) / CH, row = row_0 + rw, chunk = lane % CH;
+                    const float e0 = __shfl_sync(0xffffffffu, w0, rw), e1 = __shfl_sync(0xffffffffu, w1, rw);
+                    const long long at = __shfl_sync(0xffffffffu, place, rw);
+                    if (row >= all) continue;
+                    float4 f = stage[row * CH + (chunk ^ (row & 7))];
+                    if (alt) {
+                        const float4 g = stage[(kRows + row) * CH + (chunk ^ (row & 7))];
+                        f = make_float4(f.x * e0 + g.x * e1, f.y * e0 + g.y * e1, f.z * e0 + g.z * e1, f.w * e0 + g.w * e1);
+                    }
+                    if constexpr (PACKED) {
+                        *reinterpret_cast<float4*>(p.part + at * HD + 4 * chunk) = f;
+                    } else {
+                        *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at + 4 * chunk) = make_uint2(Half<T>::pack(f.x, f.y), Half<T>::pack(f.z, f.w));
+                        // (a NaN or an infinity in V that the row does not see: done again below)
+                        if (!isfinite(f.x + f.y + f.z + f.w)) atomicOr(flags + row, 1);
+                    }
+                }
             if constexpr (!PACKED) {
                 meet(2);
-                unsigned again = __ballot_sync(0xffffffffu, ok && q == 0 && r < rows && flags[r]);
+                unsigned again = __ballot_sync(0xffffffffu, ok && q == 0 && r < rows && flags[r] > 0);
                 while (again) {
                     const int from = __ffs(again) - 1, t2 = __shfl_sync(0xffffffffu, t, from);
                     again &= again - 1;
@@ -612,7 +631,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                     *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + to_row + 8 * c) = *reinterpret_cast<const uint4*>(stage + rr * HD * 2 + ((c ^ (rr & 7)) << 4));
             }
             __syncwarp();
-            unsigned again = __ballot_sync(0xffffffffu, bad && r < rows);
+            unsigned again = __ballot_sync(0xffffffffu, bad && isfinite(l) && r < rows);     // (no finite denominator: a score that the row sees is a NaN)
             while (again) {
                 const int from = __ffs(again) - 1, t2 = __shfl_sync(0xffffffffu, t, from);
                 again &= again - 1;

@@ -204,6 +204,44 @@ def test_rows_that_are_not_seen_do_not_matter(T, window, sinks, junk):
         assert bool(got[:, sees].isnan().any()) or junk == -math.inf
 
 
+@pytest.mark.parametrize("T", [1, 5, 150, 3000])
+def test_nan_that_is_seen_is_passed_on(T):
+    """A NaN in one query, in one key or in one dim of one value: those rows and dims are NaN, and no others."""
+    S, p, W = T + 300, 200, 40
+    q, k, v = inputs(1, T, 2, 1, 64, S, F16)
+    clean = ops.attn_window(q, k, v, at(p), W, 2)
+    bad = q.clone()
+    bad[0, T // 2, 1, 7] = math.nan
+    got = ops.attn_window(bad, k, v, at(p), W, 2)
+    assert bool(got[0, T // 2, 1].isnan().all())
+    got[0, T // 2, 1] = clean[0, T // 2, 1]
+    assert torch.equal(got, clean)
+    j = p + T // 2
+    sees = torch.tensor([j <= p + t < j + W for t in range(T)])
+    bad = k.clone()
+    bad[0, 0, j, 3] = math.nan
+    got = ops.attn_window(q, bad, v, at(p), W, 2)[0].cpu()
+    assert bool(got[sees].isnan().all()) and not bool(got[~sees].isnan().any())
+    bad = v.clone()
+    bad[0, 0, j, 3] = math.inf
+    got = ops.attn_window(q, k, bad, at(p), W, 2)[0].cpu()
+    assert bool((got[sees][..., 3] == math.inf).all()) and bool(torch.isfinite(got[~sees]).all())
+    assert bool(torch.isfinite(got[..., :3]).all()) and bool(torch.isfinite(got[..., 4:]).all())
+    assert bool(ops.attn_window(q * math.nan, k, v, at(p), W, 2).isnan().all())
+
+
+@pytest.mark.parametrize("T", [1, 140])
+def test_caches_that_repeat(T):
+    """Batches and heads that are one (stride 0), which a tensor map cannot say."""
+    q, k, v = inputs(3, T, 4, 2, 64, 200, F16)
+    k, v = k[:1, :1].expand(3, 2, 200, 64), v[:1].expand(3, 2, 200, 64)
+    check(ops.attn_window(q, k, v, at(3, 9, 40), 30, 2), *reference(q, k, v, [3, 9, 40], 30, 2))
+    kp, vp = inputs(1, 1, 1, 1, 64, 99, F16, seed=5)[1:]
+    kp, vp = kp[0].expand(2, 99, 64), vp[0].expand(2, 99, 64)
+    check(ops.attn_prefix(q, kp, vp, k, v, at(3, 9, 40)), *reference(q, k, v, [3, 9, 40], kp=kp, vp=vp))
+    check(ops.attn_prefix(q[:1].expand(3, T, 4, 64), kp, vp, k, v, at(3, 9, 40)), *reference(q[:1].expand(3, T, 4, 64), k, v, [3, 9, 40], kp=kp, vp=vp))
+
+
 def test_junk_behind_the_own_rows_with_a_prefix():
     for T in (1, 5, 140):
         q, k, v, kp, vp = inputs(3, T, 4, 2, 128, 200, F16, P=100)
