@@ -38,14 +38,12 @@ AttnPlan plan_of(const b200gptq_attn_args& a) {
     }
     // Warps per tile of rows: as many as the SMs hold (16 each, or 8 where a tile has more than 8 rows), a block of 16 keys for each at least.
     const long long tile = rows <= 8 ? 8 : rows <= 16 ? 16 : 32, held = sms * (rows <= 8 ? 16 : 8), units = (rows + tile - 1) / tile * a.kv_heads * a.batch;
-    // The prefix among each sequence's keys: read `again` times more, from L2.  A second launch costs 4 us.
+    // The prefix among each sequence's keys: `again` bytes more, from L2.  Two more launches cost 5 us.
     const double again = (double)(a.batch - 1) * a.kv_heads * a.prefix * a.hd * 4;
     const bool apart = a.prefix && again > 32e6;
     const long long keys = (a.window ? std::min<long long>(a.max_seq, (long long)a.window + a.sinks + a.tokens) : a.max_seq) + (apart ? 0 : a.prefix);
     long long warps = rows > 8 ? 8 : keys < 256 ? 1 : 2;
     while (warps < 8 * kAttnMaxSplit && units * warps * 2 <= held && keys >= warps * 2 * 16) warps *= 2;
-    p.warps = rows <= 8 ? (int)std::min(warps, 8LL) : 8;
-    p.own = (int)std::max(1LL, warps / 8);
     if (apart) {
         p.prefix_tiles = all > 32 && attn_tiles_maps(a, true);
         if (p.prefix_tiles) {
@@ -56,11 +54,15 @@ AttnPlan plan_of(const b200gptq_attn_args& a) {
             p.parts = (int)std::max<long long>(1, std::min<long long>(std::min<long long>(2 * sms / ctas, kAttnMaxParts), a.prefix / 128));
         }
     }
+    // (beside the tcgen05 kernel an SM has registers for four warps)
+    const long long most = rows <= 8 && p.prefix_tiles ? 4 : 8;
+    p.warps = rows <= 8 ? (int)std::min(warps, most) : 8;
+    p.own = (int)std::max(1LL, std::min<long long>(warps / most, kAttnMaxSplit));
     return p;
 }
 
 size_t scratch_bytes(const b200gptq_attn_args& a, const AttnPlan& p) {
-    return (size_t)p.parts * a.batch * a.tokens * a.heads * (a.hd + 2) * sizeof(float);
+    return (size_t)(p.parts ? p.parts + 1 : 0) * a.batch * a.tokens * a.heads * (a.hd + 2) * sizeof(float);
 }
 
 }  // namespace

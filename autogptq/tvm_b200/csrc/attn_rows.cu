@@ -16,9 +16,10 @@
 // only rescaled when a score is more than 2^8 above the maximum in use (no weight is above 2^8; fp32 sums).
 //
 // The key range is split over the warps of a CTA and a cluster of up to 8 CTAs, which add up through distributed shared memory, each a slice of the dims.
-// A prefix is part of every sequence's keys where reading it again from L2 takes less time than a second launch (4 us); else
-// there are two: the first takes the prefix, split over CTAs whose sums (fp32) go to scratch; the second takes each sequence's own rows
-// meanwhile, waits for the first (griddepcontrol.wait) and adds everything up.  All sums are in a fixed order.
+// A prefix is part of every sequence's keys where reading it again from L2 takes less time than more launches; else there are three: the first
+// takes the prefix, split over CTAs, the second each sequence's own rows, beside it, on what registers and shared memory it leaves, and both leave their
+// sums (fp32) in scratch; the third adds them up.  All sums are in a fixed order.  (Two launches, the second of which adds up: its CTAs wait for the first
+// one's sums where they are, so that few ran beside it: 32 sequences behind 8192 positions 34 us, now TTT; 64 behind 16384 98, now UUU.)
 #include <algorithm>
 #include <mutex>
 #include <type_traits>
@@ -57,13 +58,12 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {      // of an 8 x 8
 // Shared memory, in floats: the warps' sums [warp][row][HD + 4], their maxima and denominators, the slices that the CTAs of the cluster push
 // [split][row][HD / splits] with maxima and denominators, a flag per row; the queries (padded rows).
 template <int HD, int R, int W> struct Lay {
-    static constexpr int LD = HD + 4, QLD = HD + 8, acc = 0, weights = 2 * R * ((W == 8 ? kMaxSplit : 1) + kAttnMaxParts),
-                         ml = acc + (W * R * LD > weights ? W * R * LD : weights), slice = ml + 2 * W * R, slice_ml = slice + R * HD,
+    static constexpr int LD = HD + 4, QLD = HD + 8, acc = 0, ml = acc + W * R * LD, slice = ml + 2 * W * R, slice_ml = slice + R * HD,
                          flags = slice_ml + 2 * kMaxSplit * R, places = flags + (R < 16 ? 16 : R), q = places + 6 * R, total = q + R * QLD / 2;
 };
 
-// PREFIX: rows (b, t, g) of one key head against the prefix, sums to `part`.  Otherwise: rows (t, g) of one sequence and key head against its cache
-// (and the prefix itself, where with_prefix, or its `parts` sums).  A tile of R rows is blockIdx.x / splits % row_tiles.
+// PREFIX: rows (b, t, g) of one key head against the prefix, sums to runs 0 .. parts - 1 of `part`.  Otherwise: rows (t, g) of one sequence and key head against
+// its cache (and the prefix, where with_prefix); with parts, sums to run `parts`.  A tile of R rows is blockIdx.x / splits % row_tiles.
 template <typename T, int HD, int R, int W, bool PREFIX>
 __global__ void __launch_bounds__(W * 32, R == 8 ? 16 / W : 1)
 attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict__ part, int split_bits, int row_tiles, int parts, int with_prefix, int G) {
@@ -77,8 +77,8 @@ attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict
     const int split = blockIdx.x - per_unit * splits, tile = per_unit - unit * row_tiles;
     const int b0 = PREFIX ? 0 : unit / (unsigned)a.kv_heads, kh = unit - b0 * a.kv_heads;
     auto token_of = [&](int idx) { return !PREFIX && a.tokens == 1 ? 0 : (int)((unsigned)idx / (unsigned)G); };       // of row idx
-    // What is read below was written before the launch in front of this one ended, or began (behind the prefix launch, which lets this one
-    // start only after it has itself waited; the loads by-pass L1).
+    // What is read below was written before the launch in front of this one ended, or began (beside the prefix launch, which lets this one
+    // start only after it has itself waited; the loads by-pass L1).  One CTA waits for the prefix launch at its end, so that this launch does not end before it.
     if (!PREFIX && splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     if (PREFIX || !parts) asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
@@ -88,7 +88,7 @@ attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict
     if constexpr (!PREFIX) { p0 = attn_pos(a, b0); count = attn_count(a, b0); }
     const int nrows = min(R, (PREFIX ? rows_all : count * G) - row0);
     if (nrows <= 0) {                         // padding: every CTA of the cluster leaves
-        if (!PREFIX && parts) asm volatile("griddepcontrol.wait;" ::: "memory");
+        if (!PREFIX && parts && blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
         return;
     }
     // ---- keys: the prefix, the sinks, the window ----
@@ -354,7 +354,7 @@ attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict
         if constexpr (PREFIX) {
             const long long at = split * rows_total + places[2 * R + row];
             part[at * HD + d] = ca;
-            if (d == 0) *reinterpret_cast<float2*>(part + splits * rows_total * HD + 2 * at) = make_float2(cm, cl);
+            if (d == 0) *reinterpret_cast<float2*>(part + (parts + 1) * rows_total * HD + 2 * at) = make_float2(cm, cl);
         } else {
             const int to = d >> (HD_BITS - split_bits);
             st_cluster(sm + L::slice + (split * R + row) * slice + d - to * slice, to, ca);
@@ -367,66 +367,36 @@ attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict
     if constexpr (PREFIX) return;
     if (splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     else __syncthreads();
-    if (parts) asm volatile("griddepcontrol.wait;" ::: "memory");                           // the prefix's sums
-    // ---- this CTA's slice of the dims.  With a prefix's sums, first the weights of all runs of all rows, where the warps' sums were: 0 .. splits - 1 those of
-    //      the cluster, then the prefix's.  (Maxima and denominators read by every thread, one run after the other: 8 us more for 18 runs.) ----
+    // ---- this CTA's slice of the dims ----
     int* flags = reinterpret_cast<int*>(sm + L::flags);
-    float2* wl = reinterpret_cast<float2*>(sm);       // (maximum, denominator), then (weight, -)
-    const int runs = splits + parts;
-    if (parts) {
-        const float* part_ml = part + parts * rows_total * HD;
-        for (int x = threadIdx.x; x < nrows * runs; x += kThreads) {
-            const int row = x / runs, r = x - row * runs;
-            const long long at = places[2 * R + row];
-            wl[x] = r < splits ? *reinterpret_cast<const float2*>(sm + L::slice_ml + 2 * (r * R + row)) : __ldcg(reinterpret_cast<const float2*>(part_ml + 2 * ((r - splits) * rows_total + at)));
-        }
-        __syncthreads();
-        for (int row = warp; row < nrows; row += W) {
-            float tm = -INFINITY, tl = 0.f;
-            for (int r = lane; r < runs; r += 32) tm = fmaxf(tm, wl[row * runs + r].x);
-    #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, o));
-            const float safe = tm == -INFINITY ? 0.f : tm;
-            for (int r = lane; r < runs; r += 32) {
-                const float e = exp2_fast(wl[row * runs + r].x - safe);
-                tl += wl[row * runs + r].y * e;
-                wl[row * runs + r].x = e;
-            }
-    #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) tl += __shfl_xor_sync(0xffffffffu, tl, o);
-            if (lane == 0) sm[L::slice_ml + row] = tl;    // (what lay there has been copied)
-        }
-        __syncthreads();
-    }
     for (int x = threadIdx.x; x < nrows * (slice / 4); x += kThreads) {
         const int row = x >> (HD_BITS - split_bits - 2), d = (x - row * (slice / 4)) * 4;
-        const long long at = places[2 * R + row];
-        const float2* w = wl + row * runs;
+        const float2* ml = reinterpret_cast<const float2*>(sm + L::slice_ml) + row;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        auto add = [&](const float4& f, float e) { o.x += f.x * e; o.y += f.y * e; o.z += f.z * e; o.w += f.w * e; };
-        float tl = 0.f;
-        if (parts) {
-            tl = sm[L::slice_ml + row];
-            for (int r = 0; r < splits; ++r) add(*reinterpret_cast<const float4*>(sm + L::slice + (r * R + row) * slice + d), w[r].x);
-        } else {
-            const float2* ml = reinterpret_cast<const float2*>(sm + L::slice_ml) + row;
-            float tm = -INFINITY;
-            for (int r = 0; r < splits; ++r) tm = fmaxf(tm, ml[r * R].x);
-            const float safe = tm == -INFINITY ? 0.f : tm;
-            for (int r = 0; r < splits; ++r) {
-                const float e = exp2_fast(ml[r * R].x - safe);
-                tl += ml[r * R].y * e;
-                add(*reinterpret_cast<const float4*>(sm + L::slice + (r * R + row) * slice + d), e);
-            }
+        float tm = -INFINITY, tl = 0.f;
+        for (int r = 0; r < splits; ++r) tm = fmaxf(tm, ml[r * R].x);
+        const float safe = tm == -INFINITY ? 0.f : tm;
+        for (int r = 0; r < splits; ++r) {
+            const float e = exp2_fast(ml[r * R].x - safe);
+            const float4 f = *reinterpret_cast<const float4*>(sm + L::slice + (r * R + row) * slice + d);
+            tl += ml[r * R].y * e;
+            o.x += f.x * e; o.y += f.y * e; o.z += f.z * e; o.w += f.w * e;
         }
-        const float* src = part + at * HD + split * slice + d;
-#pragma unroll 8
-        for (int r = 0; r < parts; ++r) add(__ldcg(reinterpret_cast<const float4*>(src + r * rows_total * HD)), w[splits + r].x);
+        if (parts) {
+            const long long at = parts * rows_total + places[2 * R + row];
+            *reinterpret_cast<float4*>(part + at * HD + split * slice + d) = o;
+            if (split * slice + d == 0) *reinterpret_cast<float2*>(part + (parts + 1) * rows_total * HD + 2 * at) = make_float2(tm, tl);
+            continue;
+        }
         const bool none = tl == 0.f;
         o = make_float4(none ? 0.f : o.x / tl, none ? 0.f : o.y / tl, none ? 0.f : o.z / tl, none ? 0.f : o.w / tl);
         *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + places[R + row] + split * slice + d) =
             make_uint2(Half<T>::pack(o.x, o.y), Half<T>::pack(o.z, o.w));
         if (isfinite(tl) && (!isfinite(o.x) || !isfinite(o.y) || !isfinite(o.z) || !isfinite(o.w))) flags[row] = 1;
+    }
+    if (parts) {
+        if (blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
+        return;
     }
     // A weight of zero times a NaN or an infinity, of a key that the row does not see or that stands in for one behind the end: the row is done again.  (Not
     // where the denominator is not finite: then a score that the row sees is a NaN.)
@@ -436,6 +406,68 @@ attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict
             const int idx = row0 + row, t = token_of(idx);
             attn_row_again<T, HD>(a, b0, t, kh * G + idx - t * G, p0 + t, split * slice, (split + 1) * slice);
         }
+}
+
+// The sums of all runs of a row, a warp per row: lane l knows runs l, l + 32 .. and, later, adds 4 dims.
+template <typename T, int HD>
+__global__ void __launch_bounds__(256)
+attn_sum_kernel(const __grid_constant__ b200gptq_attn_args a, const float* __restrict__ part, int runs) {
+    constexpr int LANES = HD / 4, MOST = (kAttnMaxParts + 1 + 31) / 32;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");
+    const int lane = threadIdx.x & 31;
+    const long long rows_total = (long long)a.batch * a.tokens * a.heads, at = blockIdx.x * 8LL + (threadIdx.x >> 5);
+    if (at >= rows_total) return;
+    const unsigned token = (unsigned)(at / a.heads);          // (below 2^29)
+    const int head = (int)(at - (long long)token * a.heads), b = token / (unsigned)a.tokens, t = token - b * a.tokens;
+    if (t >= attn_count(a, b)) return;
+    float m[MOST], l[MOST], tm = -INFINITY, tl = 0.f;
+#pragma unroll
+    for (int k = 0; k < MOST; ++k) {
+        const int r = lane + 32 * k;
+        const float2 v = r < runs ? __ldcg(reinterpret_cast<const float2*>(part + runs * rows_total * HD + 2 * (r * rows_total + at))) : make_float2(-INFINITY, 0.f);
+        m[k] = v.x;
+        l[k] = v.y;
+        tm = fmaxf(tm, v.x);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, o));
+    const float safe = tm == -INFINITY ? 0.f : tm;
+#pragma unroll
+    for (int k = 0; k < MOST; ++k) {
+        m[k] = exp2_fast(m[k] - safe);
+        tl += l[k] * m[k];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) tl += __shfl_xor_sync(0xffffffffu, tl, o);
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float* src = part + at * HD + 4 * (lane % LANES);
+    // (64 dims: the halves of the warp take every other run)
+    constexpr int STEP = 32 / LANES;
+#pragma unroll
+    for (int k = 0; k < MOST; ++k)
+#pragma unroll 8
+        for (int r = 32 * k; r < min(runs, 32 * k + 32); r += STEP) {
+            const int mine = r + lane / LANES;
+            const float w = __shfl_sync(0xffffffffu, m[k], mine & 31);
+            if (mine < runs) {
+                const float4 f = __ldcg(reinterpret_cast<const float4*>(src + mine * rows_total * HD));
+                sum.x += f.x * w; sum.y += f.y * w; sum.z += f.z * w; sum.w += f.w * w;
+            }
+        }
+    if constexpr (STEP == 2) {
+        sum.x += __shfl_xor_sync(0xffffffffu, sum.x, 16); sum.y += __shfl_xor_sync(0xffffffffu, sum.y, 16);
+        sum.z += __shfl_xor_sync(0xffffffffu, sum.z, 16); sum.w += __shfl_xor_sync(0xffffffffu, sum.w, 16);
+    }
+    const bool none = tl == 0.f;
+    sum = make_float4(none ? 0.f : sum.x / tl, none ? 0.f : sum.y / tl, none ? 0.f : sum.z / tl, none ? 0.f : sum.w / tl);
+    if (lane < LANES)
+        *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + b * a.out_stride[0] + t * a.out_stride[1] + head * a.out_stride[2] + 4 * lane) =
+            make_uint2(Half<T>::pack(sum.x, sum.y), Half<T>::pack(sum.z, sum.w));
+    __syncwarp();
+    // (as in attn_rows_kernel)
+    if (__any_sync(0xffffffffu, isfinite(tl) && !(isfinite(sum.x) && isfinite(sum.y) && isfinite(sum.z) && isfinite(sum.w))))
+        attn_row_again<T, HD>(a, b, t, head, attn_pos(a, b) + t, 0, HD);
 }
 
 template <typename T, int HD, int R, int W, bool PREFIX>
@@ -491,11 +523,34 @@ int run_all(const b200gptq_attn_args& a, float* part, const AttnPlan& s, cudaStr
     return rows <= 16 ? run<T, HD, 16, 8, false>(a, part, s, stream) : run<T, HD, 32, 8, false>(a, part, s, stream);
 }
 
+template <typename T, int HD>
+int run_sum(const b200gptq_attn_args& a, const float* part, int runs, cudaStream_t stream) {
+    const long long ctas = ((long long)a.batch * a.tokens * a.heads + 7) / 8;
+    if (ctas > 0x7fffffff) return B200GPTQ_ERR_TOO_LARGE;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(256);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = attn_pdl_enabled() ? 1 : 0;
+    B200GPTQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, attn_sum_kernel<T, HD>, a, part, runs));
+    return B200GPTQ_OK;
+}
+
+template <typename T, int HD>
+int run_both(const b200gptq_attn_args& a, float* part, const AttnPlan& s, cudaStream_t stream) {
+    const int st = run_all<T, HD>(a, part, s, stream);
+    return st != B200GPTQ_OK || !s.parts ? st : run_sum<T, HD>(a, part, s.parts + 1, stream);
+}
+
 }  // namespace
 
 int attn_rows_dispatch(const b200gptq_attn_args& a, float* part, const AttnPlan& s, cudaStream_t stream) {
-    if (a.dtype == B200GPTQ_F16) return a.hd == 128 ? run_all<__half, 128>(a, part, s, stream) : run_all<__half, 64>(a, part, s, stream);
-    return a.hd == 128 ? run_all<__nv_bfloat16, 128>(a, part, s, stream) : run_all<__nv_bfloat16, 64>(a, part, s, stream);
+    if (a.dtype == B200GPTQ_F16) return a.hd == 128 ? run_both<__half, 128>(a, part, s, stream) : run_both<__half, 64>(a, part, s, stream);
+    return a.hd == 128 ? run_both<__nv_bfloat16, 128>(a, part, s, stream) : run_both<__nv_bfloat16, 64>(a, part, s, stream);
 }
 
 }  // namespace b200gptq

@@ -41,7 +41,7 @@ constexpr int kTmemCols = 512, kColO = 256;          // S of tile q, buffer b at
 constexpr float kGrow = 8.f;                         // log2 of what a maximum may grow before O is rescaled
 
 template <int HD> struct Smem {
-    static constexpr int q_tile = kRows * HD * 2, unit = kKeys * HD * 2, stages = HD == 128 ? 5 : 8, ring = 2 * q_tile, total = ring + stages * 2 * unit + 1024;
+    static constexpr int q_tile = kRows * HD * 2, unit = kKeys * HD * 2, stages = HD == 128 ? 5 : 8, total = 2 * q_tile + stages * 2 * unit + 1024;
     static_assert(stages * 2 * unit >= 2 * kRows * HD * 4, "");
 };
 
@@ -177,6 +177,8 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     __shared__ volatile int abort_flag;
 
     const b200gptq_attn_args& a = p.a;
+    const bool alt = p.alt;                   // both tiles are the same rows
+    const uint32_t ring = alt ? SM::q_tile : 2 * SM::q_tile;       // where it begins, behind one or two tiles of Q
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t bar_base = smem_u32(bars);
     auto full = [&](int s) { return bar_base + 8u * s; };
@@ -216,7 +218,6 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     const unsigned part_unit = PACKED ? blockIdx.x / (unsigned)p.splits : blockIdx.x, over_heads = part_unit / (unsigned)a.kv_heads;
     const unsigned row_tile = PACKED ? over_heads : over_heads / (unsigned)a.batch;
     const int split = PACKED ? blockIdx.x - part_unit * p.splits : 0, kh = part_unit - over_heads * a.kv_heads, b0 = PACKED ? 0 : over_heads - row_tile * a.batch;
-    const bool alt = p.alt;                   // both tiles are the same rows
     const int row0 = (p.tiles - 1 - (int)row_tile) * (alt ? kRows : 2 * kRows);
     const int pos0 = PACKED ? 0 : attn_pos(a, b0);
     const int rows_all = PACKED ? a.batch * a.tokens * G : attn_count(a, b0) * G;
@@ -277,7 +278,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             for (int s = 0, round = 0; n_units > 0 && n <= n_units; ++n) {
                 if (round > 0) ok = mbar_wait(empty(s), (round - 1) & 1, &abort_flag);
                 if (!ok) break;
-                const uint32_t dst = base + SM::ring + s * 2 * SM::unit, bar = full(s);
+                const uint32_t dst = base + ring + s * 2 * SM::unit, bar = full(s);
                 mbar_expect(bar, n < 1 ? min(2, n_units) * SM::unit : n + 1 < n_units ? 2 * SM::unit : SM::unit);
                 if (n == 0) load(0, dst, bar, false);
                 else load(n - 1, dst, bar, true);
@@ -322,7 +323,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             }
             for (int i = 0; i < min(2, n_units); ++i)
                 if (needs(i)) {
-                    qk(base + SM::ring + i * SM::unit);
+                    qk(base + ring + i * SM::unit);
                     ++started;
                 }
             if (started) mma_commit(empty(0), lead);
@@ -330,7 +331,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         }
         for (int i = 0, s = 1, round = 0; i < n_units; ++i) {
             const bool mine = needs(i), mine2 = i + 2 < n_units && needs(i + 2);
-            const uint32_t at = base + SM::ring + s * 2 * SM::unit;
+            const uint32_t at = base + ring + s * 2 * SM::unit;
             const int seen = i < n_p ? r0.j_end - r0.j_first - i * kKeys : i < n_p + n_s ? r1.j_end - (i - n_p) * kKeys : r2.j_end - r2.j_first - (i - r2.begin) * kKeys;
             if (mine && seen < kKeys) {       // rows that nobody sees (both warps write the same zeros)
                 mbar_wait(full(s), round & 1, &abort_flag);
@@ -508,11 +509,11 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             // Sums in fp32, through shared memory: so that rows are written whole (with one thread per row 4 us more), and that two tiles which are the same rows
             // add up.  For 128 dims they lie where the ring was, for 64 over Q too: what each tile multiplies has been multiplied when both have met here.
             constexpr int CH = HD / 4;          // 16-byte pieces of a row
-            float4* stage = reinterpret_cast<float4*>(base_ptr + (HD == 128 ? SM::ring : 0));
+            float4* stage = reinterpret_cast<float4*>(base_ptr + (HD == 128 ? ring : 0));
             float (*stats)[2][kRows] = reinterpret_cast<float (*)[2][kRows]>(stage + 2 * kRows * CH);              // behind them: [tile][maximum, denominator][row]
             long long (*places)[kRows] = reinterpret_cast<long long (*)[kRows]>(stats + 2);                         // the rows' places among the sums, or in out
             int* flags = reinterpret_cast<int*>(places + 2);                                                        // rows that are done again
-            static_assert((HD == 128 ? SM::ring : 0) + 2 * kRows * HD * 4 + 2 * kRows * 16 + kRows * 4 <= SM::total - 1024, "");
+            static_assert((HD == 128 ? SM::q_tile : 0) + 2 * kRows * HD * 4 + 2 * kRows * 16 + kRows * 4 <= SM::total - SM::q_tile - 1024, "");
             auto meet = [&](int phase) {
                 tc_before();
                 __syncwarp();
@@ -558,7 +559,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                     tm = both;
                 }
                 if constexpr (PACKED) {
-                    *reinterpret_cast<float2*>(p.part + p.splits * rows_total * HD + 2 * place) = make_float2(tm, tl);
+                    *reinterpret_cast<float2*>(p.part + (p.splits + 1) * rows_total * HD + 2 * place) = make_float2(tm, tl);
                 } else {
                     const float inv = tl != 0.f ? 1.f / tl : 0.f;         // (nothing seen: zero)
                     if (!isfinite(tl)) flags[at] = -1;                    // (a score that the row sees is a NaN)
@@ -696,7 +697,7 @@ int run(const b200gptq_attn_args& a, float* part, int splits, bool alt, cudaStre
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)ctas);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = Smem<HD>::total;
+    cfg.dynamicSmemBytes = Smem<HD>::total - (alt ? Smem<HD>::q_tile : 0);
     cfg.stream = stream;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
