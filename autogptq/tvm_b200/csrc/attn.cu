@@ -23,7 +23,7 @@ int check_sizes(const b200gptq_attn_args& a) {
     if (a.dtype != B200GPTQ_F16 && a.dtype != B200GPTQ_BF16) return B200GPTQ_ERR_SHAPE;
     if (a.batch < 1 || a.tokens < 1 || a.heads < 1 || a.kv_heads < 1 || a.heads % a.kv_heads || (a.hd != 64 && a.hd != 128)) return B200GPTQ_ERR_SHAPE;
     if (a.max_seq < 1 || a.prefix < 0 || a.window < 0 || a.sinks < 0 || (a.window && a.prefix) || (!a.window && a.sinks)) return B200GPTQ_ERR_SHAPE;
-    if (a.batch > kMost || a.tokens > kMost || a.max_seq > kMost || a.prefix > kMost || a.window > kMost || a.sinks > kMost ||
+    if (a.batch > kMost || a.tokens > kMost || a.heads > kMost || a.max_seq > kMost || a.prefix > kMost || a.window > kMost || a.sinks > kMost ||
         (long long)a.batch * a.tokens > kMost || (long long)a.batch * a.tokens * (a.heads / a.kv_heads) > kMost)
         return B200GPTQ_ERR_TOO_LARGE;
     return B200GPTQ_OK;
@@ -48,7 +48,11 @@ AttnPlan plan_of(const b200gptq_attn_args& a) {
         p.prefix_tiles = all > 32 && attn_tiles_maps(a, true);
         if (p.prefix_tiles) {
             const long long blocks = (a.prefix + kAttnTilesKeys - 1) / kAttnTilesKeys, ctas = (all + 255) / 256 * a.kv_heads;
-            p.parts = (int)std::max<long long>(1, std::min(std::min<long long>(sms / ctas, kAttnMaxParts), blocks / 4));
+            // SMs by bytes, the caches taken to be half full, a third at least: the sequences' own launch runs on the others.  32 sequences, 8 key
+            // heads of 128, 8192 keys before 130 of 640 each: 23.9 us, 32.4 where the prefix takes every SM; 64 sequences, 4096 before 500 of 1024:
+            // 46.5 and 84.9 (43 without the third); 48 sequences, 12000 before 150 of 2048: 42.9 and 47.2 (65 without the third).
+            const double share = std::max(1. / 3, a.prefix / (a.prefix + 0.5 * a.batch * a.max_seq));
+            p.parts = (int)std::max<long long>(1, std::min(std::min<long long>((long long)(sms * share) / ctas, kAttnMaxParts), blocks / 4));
         } else {
             const long long ctas = (all <= 16 ? 1 : (all + 31) / 32) * a.kv_heads;
             p.parts = (int)std::max<long long>(1, std::min<long long>(std::min<long long>(2 * sms / ctas, kAttnMaxParts), a.prefix / 128));

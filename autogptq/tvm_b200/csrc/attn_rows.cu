@@ -19,7 +19,7 @@
 // A prefix is part of every sequence's keys where reading it again from L2 takes less time than more launches; else there are three: the first
 // takes the prefix, split over CTAs, the second each sequence's own rows, beside it, on what registers and shared memory it leaves, and both leave their
 // sums (fp32) in scratch; the third adds them up.  All sums are in a fixed order.  (Two launches, the second of which adds up: its CTAs wait for the first
-// one's sums where they are, so that few ran beside it: 32 sequences behind 8192 positions 34 us, now TTT; 64 behind 16384 98, now UUU.)
+// one's sums where they are, so that few ran beside it: 32 sequences behind 8192 positions 34 us, now 24; 64 behind 16384 98, now 81.)
 #include <algorithm>
 #include <mutex>
 #include <type_traits>
@@ -515,11 +515,16 @@ template <typename T, int HD>
 int run_all(const b200gptq_attn_args& a, float* part, const AttnPlan& s, cudaStream_t stream) {
     const long long rows = (long long)a.tokens * (a.heads / a.kv_heads), all = rows * a.batch;
     if (s.parts && !s.prefix_tiles) {
-        const int st = all <= 8 ? run<T, HD, 8, 8, true>(a, part, s, stream) : all <= 16 ? run<T, HD, 16, 8, true>(a, part, s, stream) : run<T, HD, 32, 8, true>(a, part, s, stream);
+        const int st = all <= 8    ? run<T, HD, 8, 8, true>(a, part, s, stream)
+                       : all <= 16 ? run<T, HD, 16, 8, true>(a, part, s, stream)
+                                   : run<T, HD, 32, 8, true>(a, part, s, stream);
         if (st != B200GPTQ_OK) return st;
     }
-    if (rows <= 8)
-        return s.warps == 1 ? run<T, HD, 8, 1, false>(a, part, s, stream) : s.warps == 2 ? run<T, HD, 8, 2, false>(a, part, s, stream) : s.warps == 4 ? run<T, HD, 8, 4, false>(a, part, s, stream) : run<T, HD, 8, 8, false>(a, part, s, stream);
+    if (rows <= 8) {
+        if (s.warps == 1) return run<T, HD, 8, 1, false>(a, part, s, stream);
+        if (s.warps == 2) return run<T, HD, 8, 2, false>(a, part, s, stream);
+        return s.warps == 4 ? run<T, HD, 8, 4, false>(a, part, s, stream) : run<T, HD, 8, 8, false>(a, part, s, stream);
+    }
     return rows <= 16 ? run<T, HD, 16, 8, false>(a, part, s, stream) : run<T, HD, 32, 8, false>(a, part, s, stream);
 }
 

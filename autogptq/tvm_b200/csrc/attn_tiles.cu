@@ -144,7 +144,7 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// Operand tiles are boxes of 64 dims (128 bytes, swizzled) by 128 rows, one after the other.  Q and K: K-major, 8-row groups 1024 bytes apart.  V: MN-major,
+// Operand tiles are boxes of 64 dims (128 bytes, swizzled) by 128 rows of Q or 64 keys, one after the other.  Q and K: K-major, 8-row groups 1024 bytes apart.  V: MN-major,
 // groups of 8 keys 1024 bytes apart, the next 64 dims a box further on.
 __device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t leading) {
     uint64_t d = 0;
@@ -312,15 +312,12 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                 mma_ss(ts + 64u * (started & 1), qd + ((k / 4 * QBOX + k % 4 * 32) >> 4), kd + ((k / 4 * BOX + k % 4 * 32) >> 4), idesc_qk, k > 0 ? 1u : 0u, lead);
             mma_commit(s_full(q, started & 1), lead);
         };
-        // One thread does it all, with one barrier for both loads of a turn: what a turn costs here besides the products (each wait 150 to 250 clk, also one
-        // that is over already) is time in which the tensor cores idle.  (A wait that runs out is not looked at: those after it give up at once,
-        // and the results are not defined then.)
+        // One barrier for both loads of a turn: what a turn costs here besides the products (each wait 150 to 250 clk, also one that is over already) is
+        // time in which the tensor cores idle.  (A wait that runs out is not looked at: those after it give up at once, and the results are not defined then.)
         if (n_units > 0) {
-            {
-                if (of(nrows, q) > 0) mbar_wait(q_full(alt ? 0 : q), 0, &abort_flag);
-                mbar_wait(full(0), 0, &abort_flag);
-                tc_after();
-            }
+            if (of(nrows, q) > 0) mbar_wait(q_full(alt ? 0 : q), 0, &abort_flag);
+            mbar_wait(full(0), 0, &abort_flag);
+            tc_after();
             for (int i = 0; i < min(2, n_units); ++i)
                 if (needs(i)) {
                     qk(base + ring + i * SM::unit);
@@ -388,26 +385,23 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         const int idx = row_first + min(r, max(rows, 1) - 1), token = (int)((unsigned)idx / (unsigned)G), head = kh * G + idx - token * G;
         const int b = PACKED ? (int)((unsigned)token / (unsigned)a.tokens) : b0, t = PACKED ? token - b * a.tokens : token, pr = pos0 + token;
         const long long q_at = b * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2];
-        // Q, in the swizzled layout of the tiles: 16 bytes per thread and turn, all of them on their way at once
+        // Q, in the swizzled layout of the tiles: 16 bytes per thread and load, all of them on their way at once
         if (!(alt && q == 1)) {
-            constexpr int QB = HD / 8;
             uint8_t* dst = base_ptr + q * SM::q_tile;
-#pragma unroll 1
-            for (int x0 = 0; x0 < HD / 8; x0 += QB) {
-                uint4 val[QB];
+            const int c = lane % (HD / 8);
+            uint4 val[HD / 8];
 #pragma unroll
-                for (int x = 0; x < QB; ++x) {
-                    const int rw = ((x0 + x) * 32 + lane) / (HD / 8), c = lane % (HD / 8);
-                    const long long from = __shfl_sync(0xffffffffu, q_at, rw);
-                    val[x] = make_uint4(0, 0, 0, 0);
-                    if (32 * quarter + rw < rows) val[x] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + from + 8 * c));
-                }
+            for (int x = 0; x < HD / 8; ++x) {
+                const int rw = (x * 32 + lane) / (HD / 8);
+                const long long from = __shfl_sync(0xffffffffu, q_at, rw);
+                val[x] = make_uint4(0, 0, 0, 0);
+                if (32 * quarter + rw < rows) val[x] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + from + 8 * c));
+            }
 #pragma unroll
-                for (int x = 0; x < QB; ++x) {
-                    const int rr = 32 * quarter + ((x0 + x) * 32 + lane) / (HD / 8), c = lane % (HD / 8);
-                    if (p.negate) { val[x].x ^= 0x80008000u; val[x].y ^= 0x80008000u; val[x].z ^= 0x80008000u; val[x].w ^= 0x80008000u; }
-                    *reinterpret_cast<uint4*>(dst + (c / 8) * QBOX + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = val[x];
-                }
+            for (int x = 0; x < HD / 8; ++x) {
+                const int rr = 32 * quarter + (x * 32 + lane) / (HD / 8);
+                if (p.negate) { val[x].x ^= 0x80008000u; val[x].y ^= 0x80008000u; val[x].z ^= 0x80008000u; val[x].w ^= 0x80008000u; }
+                *reinterpret_cast<uint4*>(dst + (c / 8) * QBOX + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = val[x];
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -418,87 +412,87 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         int turn = 0;
 #pragma unroll 1
         for (int g = 0; g < 3; ++g) {
-          const Region v = region(q, g);
-          // A unit whose keys all rows of the tile see: from key `least` to key `most`
-          const int most = min(g == 1 ? min(v.j_end, a.sinks) : v.j_end, g == 0 ? v.j_end : of(p_lo, q) + 1) - kKeys, least = g == 2 ? of(p_hi, q) - window + 1 : 0;
-          const int skip = alt ? (v.begin ^ q) & 1 : 0, step = alt ? 2 : 1;
-          int j0 = v.j_first + skip * kKeys;
+            const Region v = region(q, g);
+            // A unit whose keys all rows of the tile see: from key `least` to key `most`
+            const int most = min(g == 1 ? min(v.j_end, a.sinks) : v.j_end, g == 0 ? v.j_end : of(p_lo, q) + 1) - kKeys, least = g == 2 ? of(p_hi, q) - window + 1 : 0;
+            const int skip = alt ? (v.begin ^ q) & 1 : 0, step = alt ? 2 : 1;
+            int j0 = v.j_first + skip * kKeys;
 #pragma unroll 1
-          for (int i = v.begin + skip; i < v.end; i += step, j0 += step * kKeys) {
-            const uint32_t tb = ts + 64u * (turn & 1);
-            // (A wait that runs out is not looked at before the end: those after it give up at once, and the results are not defined then.)
-            mbar_wait(s_full(q, turn & 1), (turn >> 1) & 1, &abort_flag);
-            __syncwarp();
-            tc_after();
-            if (mine) {
-                uint32_t s[2][32];
-                tmem_ld32(tb, s[0]);
-                tmem_ld32(tb + 32u, s[1]);
-                tmem_wait_ld();
-                after_wait(s[0]);
-                after_wait(s[1]);
-                if (j0 > most || j0 < least) {
-                    // columns [0, front) and [lo, hi) are seen
-                    int front = v.j_end - j0, lo = 0, hi = 0;
-                    if (g != 0) {
-                        front = min(min(a.sinks, pr + 1), v.j_end) - j0;
-                        lo = pr - window + 1 - j0;
-                        hi = min(pr + 1, v.j_end) - j0;
+            for (int i = v.begin + skip; i < v.end; i += step, j0 += step * kKeys) {
+                const uint32_t tb = ts + 64u * (turn & 1);
+                // (A wait that runs out is not looked at before the end: those after it give up at once, and the results are not defined then.)
+                mbar_wait(s_full(q, turn & 1), (turn >> 1) & 1, &abort_flag);
+                __syncwarp();
+                tc_after();
+                if (mine) {
+                    uint32_t s[2][32];
+                    tmem_ld32(tb, s[0]);
+                    tmem_ld32(tb + 32u, s[1]);
+                    tmem_wait_ld();
+                    after_wait(s[0]);
+                    after_wait(s[1]);
+                    if (j0 > most || j0 < least) {
+                        // columns [0, front) and [lo, hi) are seen
+                        int front = v.j_end - j0, lo = 0, hi = 0;
+                        if (g != 0) {
+                            front = min(min(a.sinks, pr + 1), v.j_end) - j0;
+                            lo = pr - window + 1 - j0;
+                            hi = min(pr + 1, v.j_end) - j0;
+                        }
+#pragma unroll
+                        for (int x = 0; x < kKeys; ++x)
+                            if (!(x < front || (x >= lo && x < hi))) s[x / 32][x % 32] = 0xff800000u;       // -infinity
                     }
+                    float top[4];
 #pragma unroll
-                    for (int x = 0; x < kKeys; ++x)
-                        if (!(x < front || (x >= lo && x < hi))) s[x / 32][x % 32] = 0xff800000u;       // -infinity
-                }
-                float top[4];
+                    for (int g = 0; g < 4; ++g) {
+                        top[g] = __uint_as_float(s[g / 2][g % 2 * 16]);
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    top[g] = __uint_as_float(s[g / 2][g % 2 * 16]);
-#pragma unroll
-                    for (int e = 1; e < 15; e += 2)
-                        top[g] = max3(top[g], __uint_as_float(s[g / 2][g % 2 * 16 + e]), __uint_as_float(s[g / 2][g % 2 * 16 + e + 1]));
-                    top[g] = fmaxf(top[g], __uint_as_float(s[g / 2][g % 2 * 16 + 15]));
-                }
-                const float up = fmaxf(max3(top[0], top[1], top[2]), top[3]);
-                const bool grow = (up - m) * p.sl2 > kGrow;         // (from -infinity too, but not where both are)
-                if (__any_sync(0xffffffffu, grow)) {
-                    const float corr = grow ? exp2_fast((m - up) * p.sl2) : 1.f;
-                    if (grow) { m = up; l *= corr; off = -m * p.sl2; }
-                    if (turn > 0) {             // (the first products overwrite O)
-                        mbar_wait(o_done(q), (turn - 1) & 1, &abort_flag);
-                        __syncwarp();
-                        tc_after();
-                        uint32_t o[32];
+                        for (int e = 1; e < 15; e += 2)
+                            top[g] = max3(top[g], __uint_as_float(s[g / 2][g % 2 * 16 + e]), __uint_as_float(s[g / 2][g % 2 * 16 + e + 1]));
+                        top[g] = fmaxf(top[g], __uint_as_float(s[g / 2][g % 2 * 16 + 15]));
+                    }
+                    const float up = fmaxf(max3(top[0], top[1], top[2]), top[3]);
+                    const bool grow = (up - m) * p.sl2 > kGrow;         // (from -infinity too, but not where both are)
+                    if (__any_sync(0xffffffffu, grow)) {
+                        const float corr = grow ? exp2_fast((m - up) * p.sl2) : 1.f;
+                        if (grow) { m = up; l *= corr; off = -m * p.sl2; }
+                        if (turn > 0) {             // (the first products overwrite O)
+                            mbar_wait(o_done(q), (turn - 1) & 1, &abort_flag);
+                            __syncwarp();
+                            tc_after();
+                            uint32_t o[32];
 #pragma unroll 1
-                        for (int c = 0; c < HD / 32; ++c) {
-                            tmem_ld32(to + 32u * c, o);
-                            tmem_wait_ld();
-                            after_wait(o);
+                            for (int c = 0; c < HD / 32; ++c) {
+                                tmem_ld32(to + 32u * c, o);
+                                tmem_wait_ld();
+                                after_wait(o);
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-                            tmem_st32(to + 32u * c, o);
+                                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+                                tmem_st32(to + 32u * c, o);
+                            }
                         }
                     }
-                }
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
-                uint32_t w[32];
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    uint32_t w[32];
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    float x0, x1;
-                    fma2(x0, x1, __uint_as_float(s[e / 16][e % 16 * 2]), __uint_as_float(s[e / 16][e % 16 * 2 + 1]), p.sl2, off);
-                    x0 = exp2_fast(x0);
-                    x1 = exp2_fast(x1);
-                    add2(sum[2 * (e & 1)], sum[2 * (e & 1) + 1], x0, x1);
-                    w[e] = Half<T>::pack(x0, x1);
+                    for (int e = 0; e < 32; ++e) {
+                        float x0, x1;
+                        fma2(x0, x1, __uint_as_float(s[e / 16][e % 16 * 2]), __uint_as_float(s[e / 16][e % 16 * 2 + 1]), p.sl2, off);
+                        x0 = exp2_fast(x0);
+                        x1 = exp2_fast(x1);
+                        add2(sum[2 * (e & 1)], sum[2 * (e & 1) + 1], x0, x1);
+                        w[e] = Half<T>::pack(x0, x1);
+                    }
+                    tmem_st32(tb, w);
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    tmem_wait_st();
                 }
-                tmem_st32(tb, w);
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                tmem_wait_st();
+                tc_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full(q, turn & 1));
+                ++turn;
             }
-            tc_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(p_full(q, turn & 1));
-            ++turn;
-          }
         }
         // ---- O ----
         if (turn > 0) mbar_wait(retired(q), 0, &abort_flag);
@@ -647,7 +641,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)kTmemCols) : "memory");
 }
 
-// One tensor map: boxes of 64 dims by 128 rows.  Strides of dimensions of size one are any that the encoder takes.
+// One tensor map: boxes of 64 dims by 64 keys.  Strides of dimensions of size one are any that the encoder takes.
 bool encode(CUtensorMap* m, bool bf16, int hd, const void* ptr, int rank, const int* sizes, const int64_t* strides) {
     const EncodeTiledFn fn = encode_tiled_fn();
     cuuint64_t dims[4] = {(cuuint64_t)hd}, st[3] = {};

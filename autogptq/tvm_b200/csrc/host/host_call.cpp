@@ -482,8 +482,13 @@ PyObject* attn_checked(PyObject* const* args) {
     need(hd == 64 || hd == 128, "q", "must have heads of 64 or 128 dims");
     need(k.size(0) == B && k.size(3) == hd && H % KV == 0, "k_cache", "must be [batch, kv_heads, max_seq, head_dim], kv_heads a divisor of q's heads");
     need(v.sizes() == k.sizes(), "v_cache", "must have the shape of k_cache");
-    need(B * T <= (1 << 29) && B * T * (H / KV) <= (1 << 29) && S <= (1 << 29), "q", "is too large");
-    for (auto [t, name] : {std::pair{&k, "k_cache"}, std::pair{&v, "v_cache"}}) { need_type(*t, type, name); need_device(*t, device, name); need_rows(*t, name); need_no_gradient(*t, name); }
+    need(B * T <= (1 << 29) && H <= (1 << 29) && B * T * (H / KV) <= (1 << 29) && S <= (1 << 29), "q", "is too large");
+    for (auto [t, name] : {std::pair{&k, "k_cache"}, std::pair{&v, "v_cache"}}) {
+        need_type(*t, type, name);
+        need_device(*t, device, name);
+        need_rows(*t, name);
+        need_no_gradient(*t, name);
+    }
     need_rows(q, "q");
     need_no_gradient(q, "q");
     need_type(pos, at::kLong, "pos");
@@ -501,7 +506,11 @@ PyObject* attn_checked(PyObject* const* args) {
         need(kp && vp, "k_prefix", "and v_prefix come together");
         need(kp->dim() == 3 && kp->size(0) == KV && kp->size(2) == hd && kp->size(1) <= (1 << 29), "k_prefix", "must be [kv_heads, positions, head_dim]");
         need(vp->sizes() == kp->sizes(), "v_prefix", "must have the shape of k_prefix");
-        for (auto [t, name] : {std::pair{kp, "k_prefix"}, std::pair{vp, "v_prefix"}}) { need_type(*t, type, name); need_device(*t, device, name); need_no_gradient(*t, name); }
+        for (auto [t, name] : {std::pair{kp, "k_prefix"}, std::pair{vp, "v_prefix"}}) {
+            need_type(*t, type, name);
+            need_device(*t, device, name);
+            need_no_gradient(*t, name);
+        }
         a.prefix = (int)kp->size(1);
         if (a.prefix) {
             need_rows(*kp, "k_prefix");

@@ -227,12 +227,16 @@ extern "C" B200GPTQ_API int b200gptq_adjust_logits(const b200gptq_logit_args* ar
     if (!args) return B200GPTQ_ERR_NULL_POINTER;
     const b200gptq_logit_args& a = *args;
     if (!a.logits || !a.out || (a.history && !a.lengths) || (a.biases && (!a.bias_tokens || !a.bias_values))) return B200GPTQ_ERR_NULL_POINTER;
-    if (a.rows < 1 || a.vocab < 1 || a.vocab > 1 << 30 || a.history_len < 0 || a.history_len >= 1 << 30 || a.biases < 0 || a.biases >= 1 << 30 || a.logits_stride < 0 || a.out_stride < 0) return B200GPTQ_ERR_SHAPE;
+    if (a.rows < 1 || a.vocab < 1 || a.vocab > 1 << 30 || a.history_len < 0 || a.history_len >= 1 << 30 || a.biases < 0 || a.biases >= 1 << 30 ||
+        a.logits_stride < 0 || a.out_stride < 0)
+        return B200GPTQ_ERR_SHAPE;
     const int size = a.dtype == B200GPTQ_F32 ? 4 : 2;
     if (a.dtype != B200GPTQ_F16 && a.dtype != B200GPTQ_BF16 && a.dtype != B200GPTQ_F32) return B200GPTQ_ERR_SHAPE;
     if ((reinterpret_cast<uintptr_t>(a.logits) | reinterpret_cast<uintptr_t>(a.out)) & (size - 1) ||
         (reinterpret_cast<uintptr_t>(a.history) | reinterpret_cast<uintptr_t>(a.bias_tokens) | reinterpret_cast<uintptr_t>(a.lengths) |
-         reinterpret_cast<uintptr_t>(a.prompt_lens)) & 7u)
+         reinterpret_cast<uintptr_t>(a.prompt_lens)) & 7u ||
+        (reinterpret_cast<uintptr_t>(a.repetition) | reinterpret_cast<uintptr_t>(a.frequency) | reinterpret_cast<uintptr_t>(a.presence) |
+         reinterpret_cast<uintptr_t>(a.bias_values) | reinterpret_cast<uintptr_t>(a.mask)) & 3u)
         return B200GPTQ_ERR_ALIGNMENT;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return a.dtype == B200GPTQ_F16 ? launch<__half>(a, s) : a.dtype == B200GPTQ_BF16 ? launch<__nv_bfloat16>(a, s) : launch<float>(a, s);

@@ -449,7 +449,8 @@ B200GPTQ_API int b200gptq_pick_final(const void* slots, int rows, int world, lon
  *   strides    in elements, multiples of 8: q and out {batch, token, head}, caches {batch, head, row}, prefix {head, row}; the last
  *              dimension is dense.  All addresses 16-byte aligned.  out overlaps nothing that is read
  *   status      device word (b200gptq_workspace_status's, or any) that a bounded wait which runs out sets to 1, or NULL
- * b200gptq_attn_workspace_bytes: scratch of a call (0 without a prefix; its contents on entry do not matter and nothing is kept there, so
+ * b200gptq_attn_workspace_bytes: scratch of a call (0 without a prefix, and where a prefix is read with each
+ * sequence's own keys; its contents on entry do not matter and nothing is kept there, so
  * calls that may overlap need scratch of their own).  Negative: a B200GPTQ_ERR_* code for the sizes.
  */
 typedef struct {

@@ -130,7 +130,8 @@ def test_logit_rules_refuse_on_the_host():
     assert _lib.lib.b200gptq_adjust_logits(None, None) == -1
     for change, status in [(dict(logits=None), -1), (dict(out=None), -1), (dict(lengths=None), -1), (dict(bias_tokens=None), -1), (dict(bias_values=None), -1),
                            (dict(rows=0), -3), (dict(vocab=0), -3), (dict(history_len=-1), -3), (dict(biases=-1), -3), (dict(dtype=3), -3), (dict(logits_stride=-1), -3),
-                           (dict(logits=A + 1), -4), (dict(out=A + 2, dtype=2), -4), (dict(history=A + 4), -4), (dict(lengths=A + 4), -4)]:
+                           (dict(logits=A + 1), -4), (dict(out=A + 2, dtype=2), -4), (dict(history=A + 4), -4), (dict(lengths=A + 4), -4),
+                           (dict(repetition=A + 2), -4), (dict(presence=A + 1), -4), (dict(bias_values=A + 2), -4), (dict(mask=A + 2), -4)]:
         assert _lib.lib.b200gptq_adjust_logits(ctypes.byref(_lib.LogitArgs(**dict(good, **change))), None) == status, change
 
 
