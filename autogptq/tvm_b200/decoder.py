@@ -71,11 +71,19 @@ def check_positions(pos: int, steps: int, max_seq: int) -> None:
         raise ValueError(f"{steps} steps from position {pos} do not fit the KV caches (max_seq = {max_seq})")
 
 
+def check_prefix(tokens, vocab: int) -> None:
+    """Refuse what is no text of the vocabulary: the device looks the tokens up unseen."""
+    if not isinstance(tokens, torch.Tensor) or tokens.dim() != 1 or tokens.dtype != torch.long:
+        raise ValueError("a prefix is int64 [positions]")
+    if tokens.numel() and not 0 <= int(tokens.min()) <= int(tokens.max()) < vocab:
+        raise ValueError(f"a prefix has tokens of the vocabulary, 0 .. {vocab - 1}")
+
+
 @dataclass
 class LogitRules:
     """What a request asks of the logits before the pick (:func:`ops.adjust_logits`), by sequence or one for all.  ``frequency`` and ``presence`` look at
     the generated tokens, ``repetition`` at the prompt too.  ``bias``: token -> number.  ``mask`` int32 ``[batch or 1, ceil(vocab / 32)]``: a bit per token that
-    may come next; the caller may write into it between steps (a grammar)."""
+    may come next; the caller may write into it between steps (a grammar), where it is on the model's device (else a copy is taken)."""
     repetition: Union[None, float, Sequence[float]] = None
     frequency: Union[None, float, Sequence[float]] = None
     presence: Union[None, float, Sequence[float]] = None
@@ -441,8 +449,8 @@ class GPTQDecoder:
         """Let every sequence begin with ``tokens`` (int64 ``[P]``): their keys and values are computed and held once, and :meth:`prefill` and the steps
         after it count the positions behind them.  ``None`` or no tokens: no prefix.  A captured step is dropped."""
         cfg = self.cfg
-        if tokens is not None and (tokens.dim() != 1 or tokens.dtype != torch.long):
-            raise ValueError("a prefix is int64 [positions]")
+        if tokens is not None:
+            check_prefix(tokens, cfg.vocab)
         P = 0 if tokens is None else tokens.numel()
         if P and cfg.window is not None:
             raise ValueError("a shared prefix goes with attention over the whole text")
@@ -465,7 +473,7 @@ class GPTQDecoder:
             self._prompt_layers(self._embed(tokens[None], torch.arange(P, device=self.device)), P, caches, cos, sin)
             for L, (k, v) in zip(self.layers, caches):
                 L.k_prefix, L.v_prefix = k[0], v[0]
-            self.prefix = tokens
+            self.prefix = tokens.clone()
             self.cos, self.sin = self._angles(P)
         self.set_rules(self.rules)
 

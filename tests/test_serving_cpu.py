@@ -21,3 +21,14 @@ def test_rules_become_one_row_per_sequence():
 def test_refused_rules(rules):
     with pytest.raises(ValueError):
         decoder.LogitRules(**rules).arguments(2, 100, torch.device("cpu"))
+
+
+@pytest.mark.parametrize("tokens", [torch.zeros(1, 3).long(), torch.zeros(3), torch.tensor([1, 100]), torch.tensor([-1, 5]), [1, 2]])
+def test_refused_prefixes(tokens):
+    with pytest.raises(ValueError):
+        decoder.check_prefix(tokens, 100)
+
+
+def test_prefixes():
+    decoder.check_prefix(torch.tensor([0, 99, 5]), 100)
+    decoder.check_prefix(torch.empty(0, dtype=torch.long), 100)
