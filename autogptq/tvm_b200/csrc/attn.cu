@@ -24,7 +24,8 @@ int check_sizes(const b200gptq_attn_args& a) {
     if (a.batch < 1 || a.tokens < 1 || a.heads < 1 || a.kv_heads < 1 || a.heads % a.kv_heads || (a.hd != 64 && a.hd != 128)) return B200GPTQ_ERR_SHAPE;
     if (a.max_seq < 1 || a.prefix < 0 || a.window < 0 || a.sinks < 0 || (a.window && a.prefix) || (!a.window && a.sinks)) return B200GPTQ_ERR_SHAPE;
     if (a.batch > kMost || a.tokens > kMost || a.heads > kMost || a.max_seq > kMost || a.prefix > kMost || a.window > kMost || a.sinks > kMost ||
-        (long long)a.batch * a.tokens > kMost || (long long)a.batch * a.tokens * (a.heads / a.kv_heads) > kMost)
+        (long long)a.batch * a.tokens > kMost || (long long)a.batch * a.tokens * (a.heads / a.kv_heads) > kMost ||
+        (long long)a.batch * a.tokens * a.heads > 0x7fffffff)
         return B200GPTQ_ERR_TOO_LARGE;
     return B200GPTQ_OK;
 }

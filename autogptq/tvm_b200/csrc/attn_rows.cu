@@ -62,21 +62,23 @@ template <int HD, int R, int W> struct Lay {
                          flags = slice_ml + 2 * kMaxSplit * R, places = flags + (R < 16 ? 16 : R), q = places + 6 * R, total = q + R * QLD / 2;
 };
 
+struct RowDivisors { Divisor parts, row_tiles, kv_heads, group, tokens; };
+
 // PREFIX: rows (b, t, g) of one key head against the prefix, sums to runs 0 .. parts - 1 of `part`.  Otherwise: rows (t, g) of one sequence and key head against
 // its cache (and the prefix, where with_prefix); with parts, sums to run `parts`.  A tile of R rows is blockIdx.x / splits % row_tiles.
 template <typename T, int HD, int R, int W, bool PREFIX>
 __global__ void __launch_bounds__(W * 32, R == 8 ? 16 / W : 1)
-attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict__ part, int split_bits, int row_tiles, int parts, int with_prefix, int G) {
+attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict__ part, int split_bits, int row_tiles, int parts, int with_prefix, int G,
+                 const __grid_constant__ RowDivisors by) {
     using L = Lay<HD, R, W>;
     constexpr int MT = R == 8 ? 1 : R / 16, SEG = HD / 32, HH = HD / 64, kThreads = W * 32;
     extern __shared__ __align__(16) float sm[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    // (Divisions are few, and not of 64 bits: a call for one token lasts 6 us, and each takes 50 to 200 ns.)
     const int window = a.window ? a.window : 1 << 30, splits = PREFIX ? parts : 1 << split_bits;
-    const unsigned per_unit = PREFIX ? blockIdx.x / splits : blockIdx.x >> split_bits, unit = row_tiles == 1 ? per_unit : per_unit / row_tiles;
+    const unsigned per_unit = PREFIX ? over(blockIdx.x, by.parts) : blockIdx.x >> split_bits, unit = over(per_unit, by.row_tiles);
     const int split = blockIdx.x - per_unit * splits, tile = per_unit - unit * row_tiles;
-    const int b0 = PREFIX ? 0 : unit / (unsigned)a.kv_heads, kh = unit - b0 * a.kv_heads;
-    auto token_of = [&](int idx) { return !PREFIX && a.tokens == 1 ? 0 : (int)((unsigned)idx / (unsigned)G); };       // of row idx
+    const int b0 = PREFIX ? 0 : over(unit, by.kv_heads), kh = unit - b0 * a.kv_heads;
+    auto token_of = [&](int idx) { return (int)over((unsigned)idx, by.group); };       // of row idx
     // What is read below was written before the launch in front of this one ended, or began (beside the prefix launch, which lets this one
     // start only after it has itself waited; the loads by-pass L1).  One CTA waits for the prefix launch at its end, so that this launch does not end before it.
     if (!PREFIX && splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
@@ -98,8 +100,14 @@ attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict
     const int n_p = PREFIX || with_prefix ? (a.prefix + kBlock - 1) / kBlock : 0, n_s = n_p + (range.s_end + kBlock - 1) / kBlock,
               nb = n_s + (range.w_end - range.w_start + kBlock - 1) / kBlock;
     int first, last;
-    if constexpr (PREFIX) { first = (int)((long long)nb * split / splits); last = (int)((long long)nb * (split + 1) / splits); }
-    else { first = (int)((long long)nb * split >> split_bits); last = (int)((long long)nb * (split + 1) >> split_bits); }
+    if constexpr (PREFIX) {
+        const int each = over(nb, by.parts), more = nb - each * splits;
+        first = split * each + min(split, more);
+        last = first + each + (split < more ? 1 : 0);
+    } else {
+        first = (int)((long long)nb * split >> split_bits);
+        last = (int)((long long)nb * (split + 1) >> split_bits);
+    }
     const T *k_own = nullptr, *v_own = nullptr, *k_front = nullptr, *v_front = nullptr;
     if constexpr (!PREFIX) {
         k_own = static_cast<const T*>(a.k_cache) + b0 * a.k_stride[0] + kh * a.k_stride[1];
@@ -147,7 +155,7 @@ attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict
     long long* places = reinterpret_cast<long long*>(sm + L::places);
     if (threadIdx.x < R) {
         const int idx = row0 + min((int)threadIdx.x, nrows - 1), tok = token_of(idx), head = kh * G + idx - tok * G;
-        const int bb = PREFIX ? tok / a.tokens : b0, t = PREFIX ? tok - bb * a.tokens : tok;
+        const int bb = PREFIX ? (int)over((unsigned)tok, by.tokens) : b0, t = PREFIX ? tok - bb * a.tokens : tok;
         places[threadIdx.x] = bb * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2];
         places[R + threadIdx.x] = bb * a.out_stride[0] + t * a.out_stride[1] + head * a.out_stride[2];
         places[2 * R + threadIdx.x] = ((long long)bb * a.tokens + t) * a.heads + head;
@@ -411,15 +419,15 @@ attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict
 // The sums of all runs of a row, a warp per row: lane l knows runs l, l + 32 .. and, later, adds 4 dims.
 template <typename T, int HD>
 __global__ void __launch_bounds__(256)
-attn_sum_kernel(const __grid_constant__ b200gptq_attn_args a, const float* __restrict__ part, int runs) {
+attn_sum_kernel(const __grid_constant__ b200gptq_attn_args a, const float* __restrict__ part, int runs, const Divisor by_heads, const Divisor by_tokens) {
     constexpr int LANES = HD / 4, MOST = (kAttnMaxParts + 1 + 31) / 32;
+    const int lane = threadIdx.x & 31;
+    const long long rows_total = (long long)a.batch * a.tokens * a.heads, at = blockIdx.x * 8LL + (threadIdx.x >> 5);       // (below 2^31)
+    const unsigned token = over((unsigned)at, by_heads);
+    const int head = (int)at - (int)token * a.heads, b = over(token, by_tokens), t = token - b * a.tokens;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
-    const int lane = threadIdx.x & 31;
-    const long long rows_total = (long long)a.batch * a.tokens * a.heads, at = blockIdx.x * 8LL + (threadIdx.x >> 5);
     if (at >= rows_total) return;
-    const unsigned token = (unsigned)(at / a.heads);          // (below 2^29)
-    const int head = (int)(at - (long long)token * a.heads), b = token / (unsigned)a.tokens, t = token - b * a.tokens;
     if (t >= attn_count(a, b)) return;
     float m[MOST], l[MOST], tm = -INFINITY, tl = 0.f;
 #pragma unroll
@@ -507,7 +515,8 @@ int run(const b200gptq_attn_args& a, float* part, const AttnPlan& s, cudaStream_
     cfg.numAttrs = n;
     int bits = 0;
     while ((1 << bits) < splits) ++bits;      // (a cluster has 1, 2, 4 or 8 CTAs)
-    B200GPTQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a, part, bits, tiles, s.parts, a.prefix && !s.parts ? 1 : 0, a.heads / a.kv_heads));
+    B200GPTQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a, part, bits, tiles, s.parts, a.prefix && !s.parts ? 1 : 0, a.heads / a.kv_heads,
+                                         RowDivisors{Divisor(std::max(s.parts, 1)), Divisor(tiles), Divisor(a.kv_heads), Divisor(a.heads / a.kv_heads), Divisor(a.tokens)}));
     return B200GPTQ_OK;
 }
 
@@ -541,7 +550,7 @@ int run_sum(const b200gptq_attn_args& a, const float* part, int runs, cudaStream
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = attn_pdl_enabled() ? 1 : 0;
-    B200GPTQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, attn_sum_kernel<T, HD>, a, part, runs));
+    B200GPTQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, attn_sum_kernel<T, HD>, a, part, runs, Divisor(a.heads), Divisor(a.tokens)));
     return B200GPTQ_OK;
 }
 

@@ -12,6 +12,9 @@
 //   warps 9, 10       tcgen05.mma for one tile of Q each: S of the unit after next as soon as the weights of this one have been multiplied, so that the
 //                     softmax always finds the next S there and waits for no product
 //
+// Measured per unit and both tiles, 128 dims: 1 570 clk; the products alone 1 280 (Q and K are 48 KB of shared memory, 384 clk, for 256 of arithmetic), the
+// exponentials, which both tiles do at the same time, 1 030 of a softmax warp's turn.  One prompt of 8192, 32 / 8 heads, window 4096: 355 us, 1 160 TFLOP/s;
+// 411 when it runs for seconds and the power limit holds the clock at 1.6 GHz.
 // Units of 128 keys with one S per tile of Q, so that softmax and products of a tile took turns, took 3900 to 4600 clk per 128 keys, with two threads per
 // row (which exchange its maximum) 4100: 1550 of them the products, 2500 the softmax.
 //
@@ -161,6 +164,8 @@ struct TileArgs {
     float* part;
     float sl2;                // |scale| log2 e, and Q is negated where the scale is negative
     int negate, tiles, splits, prefix_units, group, alt;
+    int units_each, units_more;             // of a run of the prefix; the first units_more runs have one more
+    Divisor by_splits, by_kv_heads, by_batch, by_group, by_tokens;
 };
 
 template <typename T, int HD, bool PACKED>
@@ -210,15 +215,16 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     __syncthreads();
     tc_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base_holder, 0);
+    // ---- which rows, which keys.  The last rows of a prompt see most, and come first. ----
+    const int G = p.group, window = a.window ? a.window : 1 << 30;
+    const unsigned part_unit = PACKED ? over(blockIdx.x, p.by_splits) : blockIdx.x, over_heads = over(part_unit, p.by_kv_heads);
+    const unsigned row_tile = PACKED ? over_heads : over(over_heads, p.by_batch);
+    const int split = PACKED ? blockIdx.x - part_unit * p.splits : 0, kh = part_unit - over_heads * a.kv_heads, b0 = PACKED ? 0 : over_heads - row_tile * a.batch;
+    const int row0 = (p.tiles - 1 - (int)row_tile) * (alt ? kRows : 2 * kRows);
+    // (nothing that another launch has written is read before this)
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
 
-    // ---- which rows, which keys.  The last rows of a prompt see most, and come first. ----
-    const int G = p.group, window = a.window ? a.window : 1 << 30;
-    const unsigned part_unit = PACKED ? blockIdx.x / (unsigned)p.splits : blockIdx.x, over_heads = part_unit / (unsigned)a.kv_heads;
-    const unsigned row_tile = PACKED ? over_heads : over_heads / (unsigned)a.batch;
-    const int split = PACKED ? blockIdx.x - part_unit * p.splits : 0, kh = part_unit - over_heads * a.kv_heads, b0 = PACKED ? 0 : over_heads - row_tile * a.batch;
-    const int row0 = (p.tiles - 1 - (int)row_tile) * (alt ? kRows : 2 * kRows);
     const int pos0 = PACKED ? 0 : attn_pos(a, b0);
     const int rows_all = PACKED ? a.batch * a.tokens * G : attn_count(a, b0) * G;
     int nrows[2], p_lo[2], p_hi[2];
@@ -226,8 +232,8 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     for (int q = 0; q < 2; ++q) {
         const int r = row0 + (alt ? 0 : q * kRows);
         nrows[q] = max(0, min(kRows, rows_all - r));
-        p_lo[q] = PACKED ? 0 : pos0 + (int)((unsigned)r / (unsigned)G);
-        p_hi[q] = PACKED ? 0 : pos0 + (int)((unsigned)(r + max(nrows[q], 1) - 1) / (unsigned)G);
+        p_lo[q] = PACKED ? 0 : pos0 + (int)over((unsigned)r, p.by_group);
+        p_hi[q] = PACKED ? 0 : pos0 + (int)over((unsigned)(r + max(nrows[q], 1) - 1), p.by_group);
     }
     auto of = [](const int (&v)[2], int q) { return q ? v[1] : v[0]; };       // (registers, not an array that is indexed)
     // Units of three regions, one after the other: the prefix, the sinks, the window (which begin where the keys begin; where sinks and window meet, they
@@ -235,8 +241,8 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     int n_units = 0, n_p = 0, n_s = 0, first = 0, s_end = 0, w_base = 0, w_end = 0;
     if (nrows[0] > 0) {
         if constexpr (PACKED) {
-            first = (int)((long long)p.prefix_units * split / p.splits);
-            n_units = n_p = (int)((long long)p.prefix_units * (split + 1) / p.splits) - first;
+            first = split * p.units_each + min(split, p.units_more);
+            n_units = n_p = p.units_each + (split < p.units_more ? 1 : 0);
         } else {
             const AttnRange range = attn_range(p_lo[0], nrows[1] > 0 ? p_hi[1] : p_hi[0], window, a.sinks, a.max_seq);
             const bool one = range.w_start == 0;
@@ -380,10 +386,9 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         const int q = warp >> 2, quarter = warp & 3, r = 32 * quarter + lane, rows = of(nrows, q), row_first = row0 + (alt ? 0 : q * kRows);
         const uint32_t lane_off = (uint32_t)(32 * quarter) << 16, ts = tmem + 128u * q + lane_off, to = tmem + kColO + 128u * q + lane_off;
         const bool mine = 32 * quarter < rows;          // the warp has rows at all
-        // The thread's row.  (The divisions once per row; where other threads need its place they ask for it.  With the divisions where Q is loaded and where O
-        // is stored these took 6500 and 4000 clk.)
-        const int idx = row_first + min(r, max(rows, 1) - 1), token = (int)((unsigned)idx / (unsigned)G), head = kh * G + idx - token * G;
-        const int b = PACKED ? (int)((unsigned)token / (unsigned)a.tokens) : b0, t = PACKED ? token - b * a.tokens : token, pr = pos0 + token;
+        // The thread's row.  (Once per row; where other threads need its place they ask for it.)
+        const int idx = row_first + min(r, max(rows, 1) - 1), token = (int)over((unsigned)idx, p.by_group), head = kh * G + idx - token * G;
+        const int b = PACKED ? (int)over((unsigned)token, p.by_tokens) : b0, t = PACKED ? token - b * a.tokens : token, pr = pos0 + token;
         const long long q_at = b * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2];
         // Q, in the swizzled layout of the tiles: 16 bytes per thread and load, all of them on their way at once
         if (!(alt && q == 1)) {
@@ -683,6 +688,13 @@ int run(const b200gptq_attn_args& a, float* part, int splits, bool alt, cudaStre
     t.group = a.heads / a.kv_heads;
     t.alt = alt;
     t.prefix_units = (int)((a.prefix + kKeys - 1) / kKeys);
+    t.units_each = t.prefix_units / splits;
+    t.units_more = t.prefix_units % splits;
+    t.by_splits = Divisor(splits);
+    t.by_kv_heads = Divisor(a.kv_heads);
+    t.by_batch = Divisor(a.batch);
+    t.by_group = Divisor(t.group);
+    t.by_tokens = Divisor(a.tokens);
     const long long rows = (long long)a.tokens * (a.heads / a.kv_heads) * (PACKED ? a.batch : 1);
     const int per_cta = alt ? kRows : 2 * kRows;
     t.tiles = (int)((rows + per_cta - 1) / per_cta);
