@@ -215,7 +215,8 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     __syncthreads();
     tc_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base_holder, 0);
-    // ---- which rows, which keys.  The last rows of a prompt see most, and come first. ----
+    // ---- which rows, which keys.  The last rows of a prompt see most, and come first (the tiles of one head one after the other read two chunks of 512 of 72
+    //      heads once instead of 1.4 times, which took as long; one prompt of 4096 without a window 158 us, now 136). ----
     const int G = p.group, window = a.window ? a.window : 1 << 30;
     const unsigned part_unit = PACKED ? over(blockIdx.x, p.by_splits) : blockIdx.x, over_heads = over(part_unit, p.by_kv_heads);
     const unsigned row_tile = PACKED ? over_heads : over(over_heads, p.by_batch);
