@@ -103,8 +103,8 @@ adjust_kernel(const __grid_constant__ b200gptq_logit_args a, int slice, int slic
 #pragma unroll
             for (int v = 0; v < 2; ++v) {
                 const int i = i0 + 2 * u * kThreads + v;
-                const unsigned long long at = t[u][v] - (unsigned long long)base;
-                if (i < length && at < (unsigned long long)n) {
+                const unsigned at = (unsigned)t[u][v] - (unsigned)base;          // (the vocabulary has below 2^31 tokens)
+                if (i < length && at < (unsigned)n && !(unsigned)(t[u][v] >> 32)) {
                     const unsigned before = i >= prompt ? atomicAdd(count + at, 1u) : atomicOr(count + at, kSeen);
                     if (before == 0) list[atomicAdd(listed, 1u)] = (unsigned short)at;
                 }
