@@ -419,7 +419,9 @@ class GPTQDecoder:
     @torch.no_grad()
     def prefill(self, prompt: torch.Tensor):
         """prompt: int64 [B, S]; fills the KV cache and leaves the first generated token in self.tokens."""
-        B, S = prompt.shape
+        if prompt.dim() != 2 or prompt.shape[0] != self.batch:
+            raise ValueError(f"a prompt is int64 [{self.batch}, tokens], got {tuple(prompt.shape)}")
+        S = prompt.shape[1]
         before = 0 if self.prefix is None else self.prefix.numel()
         check_positions(0, S, self._room())
         self._pos_host = S

@@ -391,6 +391,10 @@ def rope_prompt(qkv, cos, sin, q_out, k_cache, v_cache, seq: int, heads: int, hd
     """:func:`rope_cache` for a whole prompt: ``qkv`` ``[B * seq, 3*heads*hd]`` of tokens 0 .. seq-1 -> rotated ``q_out``
     ``[B, seq, heads, hd]`` and the caches (``b200gptq_rope_prompt``)."""
     B, max_seq = k_cache.shape[0], k_cache.shape[2]
+    if (qkv.numel() != 3 * B * seq * heads * hd or q_out.numel() != B * seq * heads * hd or k_cache.shape != v_cache.shape
+            or k_cache.shape != (B, heads, max_seq, hd) or rope and min(cos.shape[0], sin.shape[0]) < seq):
+        raise ValueError(f"q|k|v {tuple(qkv.shape)}, q {tuple(q_out.shape)} and caches {tuple(k_cache.shape)} are not those of {B} prompts "
+                         f"of {seq} tokens, {heads} heads of {hd}")
     with torch.cuda.device(qkv.device):
         st = _lib.lib.b200gptq_rope_prompt(_ptr(qkv), _ptr(cos), _ptr(sin), _ptr(q_out), _ptr(k_cache), _ptr(v_cache), B, seq,
                                            heads, hd, max_seq, 1 if rope else 0, _stream(qkv.device))

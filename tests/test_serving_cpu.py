@@ -32,3 +32,26 @@ def test_refused_prefixes(tokens):
 def test_prefixes():
     decoder.check_prefix(torch.tensor([0, 99, 5]), 100)
     decoder.check_prefix(torch.empty(0, dtype=torch.long), 100)
+
+
+def bare(batch, **more):
+    """A decoder without layers: what it checks before anything is computed."""
+    cfg = decoder.DecoderConfig(layers=0, hidden=256, heads=4, inter=512, vocab=103, **{"max_seq": 96, **more})
+    return decoder.GPTQDecoder(cfg, batch=batch, device="cpu")
+
+
+@pytest.mark.parametrize("batch,shape", [(1, (2, 6)), (2, (1, 6)), (2, (3, 6)), (2, (6,)), (1, (1, 2, 3))])
+def test_prompts_of_another_batch_are_refused(batch, shape):
+    """The kernels write a row of the caches for each of the model's sequences."""
+    with pytest.raises(ValueError, match="a prompt is"):
+        bare(batch).prefill(torch.zeros(shape, dtype=torch.long))
+
+
+@pytest.mark.parametrize("change", [dict(qkv=(6, 768)), dict(q=(1, 6, 4, 64)), dict(k=(2, 4, 10, 64), v=(1, 4, 10, 64)), dict(k=(2, 2, 10, 64), v=(2, 2, 10, 64)),
+                                    dict(cos=(5, 32)), dict(sin=(5, 32))])
+def test_rotary_embedding_of_a_prompt_takes_tensors_that_fit(change):
+    from autogptq.tvm_b200 import ops
+    t = {n: torch.zeros(s, dtype=torch.float16) for n, s in dict(dict(qkv=(12, 768), cos=(6, 32), sin=(6, 32), q=(2, 6, 4, 64), k=(2, 4, 10, 64),
+                                                                      v=(2, 4, 10, 64)), **change).items()}
+    with pytest.raises(ValueError, match="are not those of"):
+        ops.rope_prompt(t["qkv"], t["cos"], t["sin"], t["q"], t["k"], t["v"], 6, 4, 64, True)
