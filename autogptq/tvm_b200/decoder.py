@@ -424,13 +424,13 @@ class GPTQDecoder:
         S = prompt.shape[1]
         before = 0 if self.prefix is None else self.prefix.numel()
         check_positions(0, S, self._room())
+        if self.prefix is not None and S > 65535:
+            raise ValueError("a prompt behind a shared prefix has at most 65535 tokens")
         self._pos_host = S
         pos_idx = torch.arange(S, device=self.device)
         x = self._embed(prompt, pos_idx, before)
         if self.fused and S <= 65535:
             x = self._prompt_layers(x, S)
-        elif self.prefix is not None:
-            raise ValueError("a prompt behind a shared prefix has at most 65535 tokens")
         else:
             for L in self.layers:
                 x = self._layer(L, x, pos_idx, S, decode=False)

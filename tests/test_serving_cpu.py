@@ -55,3 +55,11 @@ def test_rotary_embedding_of_a_prompt_takes_tensors_that_fit(change):
                                                                       v=(2, 4, 10, 64)), **change).items()}
     with pytest.raises(ValueError, match="are not those of"):
         ops.rope_prompt(t["qkv"], t["cos"], t["sin"], t["q"], t["k"], t["v"], 6, 4, 64, True)
+
+
+def test_a_prompt_too_long_behind_a_prefix_leaves_the_position():
+    m = bare(1, max_seq=70000)
+    m.prefix, m._pos_host = torch.zeros(3, dtype=torch.long), 5
+    with pytest.raises(ValueError, match="65535"):
+        m.prefill(torch.zeros(1, 65536, dtype=torch.long))
+    assert m._pos_host == 5
