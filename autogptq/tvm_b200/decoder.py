@@ -97,18 +97,19 @@ class LogitRules:
             v = getattr(self, name)
             if v is not None:
                 v = [float(v)] * batch if isinstance(v, (int, float)) else [float(x) for x in v]
-                if len(v) != batch or not all(math.isfinite(x) for x in v) or (name == "repetition" and min(v) <= 0):
-                    raise ValueError(f"{name}: a finite number for each of {batch} sequences" + (", above 0" if name == "repetition" else ""))
-                out[name] = torch.tensor(v, dtype=torch.float32, device=device)
+                t = torch.tensor(v, dtype=torch.float32)         # (looked at as the kernel will see them: 1e-50 is 0 there, 1e50 infinity)
+                if len(v) != batch or not bool(torch.isfinite(t).all()) or (name == "repetition" and float(t.min()) <= 0):
+                    raise ValueError(f"{name}: a finite number for each of {batch} sequences" + (", above 0" if name == "repetition" else "") + ", in 32 bits")
+                out[name] = t.to(device)
         if self.bias is not None:
             rows = [self.bias] * batch if isinstance(self.bias, dict) else list(self.bias)
-            if len(rows) != batch or any(not 0 <= int(t) < vocab for r in rows for t in r):
-                raise ValueError(f"bias: a dict for each of {batch} sequences, of tokens of the vocabulary")
+            if len(rows) != batch or any(not 0 <= int(t) < vocab or math.isnan(x) for r in rows for t, x in r.items()):
+                raise ValueError(f"bias: a dict for each of {batch} sequences, of tokens of the vocabulary and numbers")
             width = max(1, max(len(r) for r in rows))
-            tokens, values = torch.full((batch, width), -1, dtype=torch.long), torch.zeros(batch, width)
+            tokens, values = torch.full((batch, width), -1, dtype=torch.long), torch.zeros(batch, width, dtype=torch.float32)
             for i, r in enumerate(rows):
                 tokens[i, :len(r)] = torch.tensor([int(t) for t in r], dtype=torch.long)
-                values[i, :len(r)] = torch.tensor([float(x) for x in r.values()])
+                values[i, :len(r)] = torch.tensor([float(x) for x in r.values()], dtype=torch.float32)
             out["bias_tokens"], out["bias_values"] = tokens.to(device), values.to(device)
         if self.mask is not None:
             if self.mask.dtype != torch.int32 or tuple(self.mask.shape) not in ((batch, -(-vocab // 32)), (1, -(-vocab // 32))):

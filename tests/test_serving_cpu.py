@@ -63,3 +63,20 @@ def test_a_prompt_too_long_behind_a_prefix_leaves_the_position():
     with pytest.raises(ValueError, match="65535"):
         m.prefill(torch.zeros(1, 65536, dtype=torch.long))
     assert m._pos_host == 5
+
+
+@pytest.mark.parametrize("rules", [dict(repetition=1e-50), dict(repetition=1e50), dict(frequency=[0.0, -1e39]), dict(presence=1e300), dict(bias={3: float("nan")})])
+def test_numbers_are_refused_as_32_bits_hold_them(rules):
+    """A repetition of 1e-50 is above 0 and not infinite, but is divided by as 0."""
+    with pytest.raises(ValueError):
+        decoder.LogitRules(**rules).arguments(2, 100, torch.device("cpu"))
+
+
+def test_biases_are_fp32_whatever_the_default_type():
+    before = torch.get_default_dtype()
+    try:
+        torch.set_default_dtype(torch.float64)
+        a = decoder.LogitRules(bias={1: 0.5, 2: float("-inf")}).arguments(1, 100, torch.device("cpu"))
+    finally:
+        torch.set_default_dtype(before)
+    assert a["bias_values"].dtype == torch.float32 and a["bias_values"].tolist() == [[0.5, float("-inf")]]
