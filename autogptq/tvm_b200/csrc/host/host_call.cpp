@@ -414,8 +414,15 @@ void need_type(const at::Tensor& t, at::ScalarType type, const char* name) {
 void need_device(const at::Tensor& t, int device, const char* name) {
     if (t.get_device() != device) refuse(PyExc_RuntimeError, std::string(name) + " is on another device");
 }
-void need_no_gradient(const at::Tensor& t, const char* name) {
-    if (t.requires_grad() && at::GradMode::is_enabled()) refuse(PyExc_RuntimeError, std::string(name) + " requires a gradient, and this operator has no backward pass");
+// The arguments' names, in the order of the calls below.
+constexpr int kArguments = 11;
+constexpr const char* kAttnNames[kArguments] = {"q", "k_prefix", "v_prefix", "k_cache", "v_cache", "pos", "window", "sinks", "counts", "scale", "out"};
+constexpr const char* kLogitNames[kArguments] = {"logits", "history", "lengths", "prompt_lens", "repetition", "frequency", "presence", "bias_tokens", "bias_values", "mask", "out"};
+// No argument asks for a derivative: penalties and biases could have one as well as the logits.
+void need_no_gradients(PyObject* const* args, const char* const* names) {
+    for (int i = 0; i < kArguments; ++i)
+        if (THPVariable_Check(args[i]) && at::GradMode::is_enabled() && THPVariable_Unpack(args[i]).requires_grad())
+            refuse(PyExc_RuntimeError, std::string(names[i]) + " requires a gradient, and this operator has no backward pass");
 }
 const void* data_of(const at::Tensor& t) { return t.unsafeGetTensorImpl()->data(); }
 // Whether the memory between the first and the last element of the two has a byte in common.
@@ -487,10 +494,8 @@ PyObject* attn_checked(PyObject* const* args) {
         need_type(*t, type, name);
         need_device(*t, device, name);
         need_rows(*t, name);
-        need_no_gradient(*t, name);
     }
     need_rows(q, "q");
-    need_no_gradient(q, "q");
     need_type(pos, at::kLong, "pos");
     need_device(pos, device, "pos");
     need(pos.dim() == 1 && (pos.size(0) == B || pos.size(0) == 1) && (pos.size(0) == 1 || pos.stride(0) == 1), "pos", "must be int64, dense, one number or one for each sequence");
@@ -509,7 +514,6 @@ PyObject* attn_checked(PyObject* const* args) {
         for (auto [t, name] : {std::pair{kp, "k_prefix"}, std::pair{vp, "v_prefix"}}) {
             need_type(*t, type, name);
             need_device(*t, device, name);
-            need_no_gradient(*t, name);
         }
         a.prefix = (int)kp->size(1);
         if (a.prefix) {
@@ -535,7 +539,6 @@ PyObject* attn_checked(PyObject* const* args) {
         need_device(*given, device, "out");
         need(given->sizes() == q.sizes(), "out", "must have the shape of q");
         need_rows(*given, "out");
-        need_no_gradient(*given, "out");
         bool apart = !overlap(*given, q) && !overlap(*given, k) && !overlap(*given, v) && !overlap(*given, pos) && !(counts && overlap(*given, *counts));
         if (a.prefix) apart = apart && !overlap(*given, *kp) && !overlap(*given, *vp);
         for (int i = 0; i < 3; ++i) apart = apart && (given->size(i) == 1 || given->stride(i) != 0);
@@ -567,10 +570,10 @@ PyObject* attn_checked(PyObject* const* args) {
 // adjust_logits(logits, history, lengths, prompt_lens, repetition, frequency, presence, bias_tokens, bias_values, mask, out)
 PyObject* logits_checked(PyObject* const* args) {
     const at::Tensor& x = tensor_of(args[0], "logits");
-    const char* names[11] = {"logits", "history", "lengths", "prompt_lens", "repetition", "frequency", "presence", "bias_tokens", "bias_values", "mask", "out"};
-    const at::Tensor* t[11];
+    const char* const* names = kLogitNames;
+    const at::Tensor* t[kArguments];
     const int device = x.get_device();
-    for (int i = 1; i < 11; ++i) {
+    for (int i = 1; i < kArguments; ++i) {
         t[i] = tensor_or_none(args[i], names[i]);
         if (t[i]) need_device(*t[i], device, names[i]);
     }
@@ -579,7 +582,6 @@ PyObject* logits_checked(PyObject* const* args) {
     if (type != at::kHalf && type != at::kBFloat16 && type != at::kFloat) refuse(PyExc_TypeError, "logits must be float16, bfloat16 or float32");
     a.dtype = type == at::kHalf ? B200GPTQ_F16 : type == at::kBFloat16 ? B200GPTQ_BF16 : B200GPTQ_F32;
     need(x.dim() == 2 && x.numel() > 0 && (x.size(1) == 1 || x.stride(1) == 1) && x.size(0) <= INT32_MAX && x.size(1) <= (1 << 30), "logits", "must be [rows, vocab], dense in its last dimension");
-    need_no_gradient(x, "logits");
     const int64_t R = x.size(0), V = x.size(1);
     a.rows = (int)R; a.vocab = (int)V;
     a.logits = data_of(x);
@@ -622,7 +624,6 @@ PyObject* logits_checked(PyObject* const* args) {
         const at::Tensor& o = *t[10];
         need_type(o, type, "out");
         need(o.sizes() == x.sizes() && (V == 1 || o.stride(1) == 1) && (R == 1 || o.stride(0) >= V), "out", "must have the shape of logits, rows apart and dense in its last dimension");
-        need_no_gradient(o, "out");
         bool apart = (data_of(o) == data_of(x) && (R == 1 || o.stride(0) == x.stride(0))) || !overlap(o, x);
         for (int i = 1; i < 10; ++i) apart = apart && !(t[i] && overlap(o, *t[i]));
         need(apart, "out", "must be logits itself or overlap nothing that is read");
@@ -642,9 +643,10 @@ PyObject* logits_checked(PyObject* const* args) {
     return answer(std::move(out), t[10] != nullptr, st);
 }
 
-PyObject* raising(PyObject* (*call)(PyObject* const*), PyObject* const* args, Py_ssize_t nargs) {
-    if (nargs != 11) { PyErr_SetString(PyExc_TypeError, "11 arguments"); return nullptr; }
+PyObject* raising(PyObject* (*call)(PyObject* const*), const char* const* names, PyObject* const* args, Py_ssize_t nargs) {
+    if (nargs != kArguments) { PyErr_SetString(PyExc_TypeError, "11 arguments"); return nullptr; }
     try {
+        need_no_gradients(args, names);
         return call(args);
     } catch (const Refusal& r) {
         PyErr_SetString(r.type, r.text.c_str());
@@ -656,8 +658,8 @@ PyObject* raising(PyObject* (*call)(PyObject* const*), PyObject* const* args, Py
     }
     return nullptr;
 }
-PyObject* attn(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return raising(attn_checked, args, nargs); }
-PyObject* adjust_logits(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return raising(logits_checked, args, nargs); }
+PyObject* attn(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return raising(attn_checked, kAttnNames, args, nargs); }
+PyObject* adjust_logits(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return raising(logits_checked, kLogitNames, args, nargs); }
 
 PyMethodDef module_methods[] = {
     {"attn", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attn)), METH_FASTCALL, nullptr},

@@ -80,3 +80,32 @@ def test_biases_are_fp32_whatever_the_default_type():
     finally:
         torch.set_default_dtype(before)
     assert a["bias_values"].dtype == torch.float32 and a["bias_values"].tolist() == [[0.5, float("-inf")]]
+
+
+def arguments(op):
+    """(call, its tensors by name), of sizes that fit."""
+    from autogptq.tvm_b200 import ops
+    h = dict(dtype=torch.float16)
+    if op == "logits":
+        return ops.adjust_logits, dict(logits=torch.zeros(2, 40, **h), history=torch.zeros(2, 5).long(), lengths=torch.zeros(2).long(), repetition=torch.ones(2),
+                                       frequency=torch.zeros(2), presence=torch.zeros(2), bias_tokens=torch.zeros(2, 3).long(), bias_values=torch.zeros(2, 3),
+                                       out=torch.zeros(2, 40, **h))
+    t = dict(q=torch.zeros(2, 1, 4, 64, **h), k_cache=torch.zeros(2, 2, 9, 64, **h), v_cache=torch.zeros(2, 2, 9, 64, **h), pos=torch.zeros(1).long(),
+             out=torch.zeros(2, 1, 4, 64, **h))
+    if op == "window":
+        return lambda **kw: ops.attn_window(window=4, **kw), t
+    return ops.attn_prefix, dict(t, k_prefix=torch.zeros(2, 7, 64, **h), v_prefix=torch.zeros(2, 7, 64, **h))
+
+
+FLOATS = [(op, n) for op in ("logits", "window", "prefix") for n, t in arguments(op)[1].items() if t.is_floating_point()]
+
+
+@pytest.mark.parametrize("op,name", FLOATS)
+def test_a_gradient_is_never_dropped(op, name):
+    """There is no backward pass: whichever tensor asks for one, penalties and biases too, is refused (before the device is looked at)."""
+    call, t = arguments(op)
+    t[name].requires_grad_()
+    with pytest.raises(RuntimeError, match=f"{name} requires a gradient"):
+        call(**t)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+        call(**t)
