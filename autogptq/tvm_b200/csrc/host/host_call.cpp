@@ -13,6 +13,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/core/AutogradState.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
@@ -418,11 +419,15 @@ void need_device(const at::Tensor& t, int device, const char* name) {
 constexpr int kArguments = 11;
 constexpr const char* kAttnNames[kArguments] = {"q", "k_prefix", "v_prefix", "k_cache", "v_cache", "pos", "window", "sinks", "counts", "scale", "out"};
 constexpr const char* kLogitNames[kArguments] = {"logits", "history", "lengths", "prompt_lens", "repetition", "frequency", "presence", "bias_tokens", "bias_values", "mask", "out"};
-// No argument asks for a derivative: penalties and biases could have one as well as the logits.
+// No argument asks for a derivative, backward or (a dual number, which knows no no_grad) forward: penalties and biases could as well as the logits.
 void need_no_gradients(PyObject* const* args, const char* const* names) {
-    for (int i = 0; i < kArguments; ++i)
-        if (THPVariable_Check(args[i]) && at::GradMode::is_enabled() && THPVariable_Unpack(args[i]).requires_grad())
-            refuse(PyExc_RuntimeError, std::string(names[i]) + " requires a gradient, and this operator has no backward pass");
+    const bool backward = at::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+    for (int i = 0; i < kArguments; ++i) {
+        if (!THPVariable_Check(args[i])) continue;
+        const at::Tensor& t = THPVariable_Unpack(args[i]);
+        if (backward && t.requires_grad()) refuse(PyExc_RuntimeError, std::string(names[i]) + " requires a gradient, and this operator has no backward pass");
+        if (forward && t._fw_grad(0).defined()) refuse(PyExc_RuntimeError, std::string(names[i]) + " carries a tangent, and this operator has no forward-mode derivative");
+    }
 }
 const void* data_of(const at::Tensor& t) { return t.unsafeGetTensorImpl()->data(); }
 // Whether the memory between the first and the last element of the two has a byte in common.

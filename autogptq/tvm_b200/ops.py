@@ -465,7 +465,8 @@ def attn_window(q, k_cache, v_cache, pos, window: int, sinks: int = 0, counts=No
     and values already; ``pos`` int64 ``[1]`` or ``[B]`` on the device: position of token 0 (token t is at ``pos + t``); ``counts`` int64 ``[B]``:
     how many of a sequence's T tokens are no padding, the rows of ``out`` behind them are left as they were.  ``scale`` is ``hd ** -0.5`` where not
     given.  Views are taken as long as rows begin at multiples of 16 bytes.  A query before position 0 sees nothing and gets zeros; one
-    behind the cache sees what its window has of it.  There is no backward pass.  Returns ``[B, T, heads, hd]``."""
+    behind the cache sees what its window has of it.  There is no backward pass and no forward-mode
+    derivative: what asks for one is refused.  Returns ``[B, T, heads, hd]``."""
     return _checked(_lib._host.attn(q, None, None, k_cache, v_cache, pos, window, sinks, counts, scale, out), "b200gptq_attn")
 
 

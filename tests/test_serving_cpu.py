@@ -109,3 +109,20 @@ def test_a_gradient_is_never_dropped(op, name):
         call(**t)
     with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
         call(**t)
+
+
+@pytest.mark.parametrize("op,name", FLOATS)
+def test_a_tangent_is_never_dropped(op, name):
+    """A dual number of forward mode neither requires a gradient nor is a wrapper; no_grad does not switch its tangent off."""
+    from torch.autograd import forward_ad
+    call, t = arguments(op)
+    plain = t[name]
+    with forward_ad.dual_level():
+        t[name] = forward_ad.make_dual(plain, torch.ones_like(plain))
+        with pytest.raises(RuntimeError, match=f"{name} carries a tangent"):
+            call(**t)
+        with torch.no_grad(), pytest.raises(RuntimeError, match=f"{name} carries a tangent"):
+            call(**t)
+    t[name] = plain
+    with pytest.raises(RuntimeError, match="CUDA"):
+        call(**t)
