@@ -16,9 +16,11 @@
 #include <c10/core/AutogradState.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cmath>
 #include <string>
 #include <unordered_map>
+#include <utility>
 
 #include "../../../../include/b200gptq.h"
 
@@ -446,6 +448,19 @@ bool overlap(const at::Tensor& x, const at::Tensor& y) {
     span(y, c, d);
     return a < d && c < b;
 }
+// Whether the elements of each dimension lie apart: a dimension's stride passes all that the dimensions of smaller strides reach.
+bool apart_from_itself(const at::Tensor& t) {
+    c10::SmallVector<std::pair<int64_t, int64_t>, 4> dims;         // (stride, size)
+    for (int64_t i = 0; i < t.dim(); ++i)
+        if (t.size(i) > 1) dims.emplace_back(t.stride(i), t.size(i));
+    std::sort(dims.begin(), dims.end());
+    int64_t reach = 1;
+    for (auto [stride, size] : dims) {
+        if (stride < reach) return false;
+        reach += (size - 1) * stride;
+    }
+    return true;
+}
 int int_of(PyObject* o, const char* name) {
     const long long v = PyLong_AsLongLong(o);
     if (v == -1 && PyErr_Occurred()) { PyErr_Clear(); refuse(PyExc_TypeError, std::string(name) + " must be an integer"); }
@@ -546,8 +561,7 @@ PyObject* attn_checked(PyObject* const* args) {
         need_rows(*given, "out");
         bool apart = !overlap(*given, q) && !overlap(*given, k) && !overlap(*given, v) && !overlap(*given, pos) && !(counts && overlap(*given, *counts));
         if (a.prefix) apart = apart && !overlap(*given, *kp) && !overlap(*given, *vp);
-        for (int i = 0; i < 3; ++i) apart = apart && (given->size(i) == 1 || given->stride(i) != 0);
-        need(apart, "out", "must not overlap what is read, nor itself");
+        need(apart && apart_from_itself(*given), "out", "must not overlap what is read, nor itself");
     }
     // (rows of padding that nobody has given a value)
     if (counts && !given) refuse(PyExc_ValueError, "counts needs out: the rows of padding keep what it holds");

@@ -384,3 +384,20 @@ def test_a_given_output_counts_a_write():
     before = out._version
     ops.attn_window(q, k, v, at(3), 4, out=out)
     assert out._version == before + 1
+
+
+@pytest.mark.parametrize("strides", [(256, 256, 32, 1), (256, 256, 0, 1), (64, 256, 64, 1), (128, 256, 64, 1)])
+def test_an_output_whose_rows_share_memory_is_refused(strides):
+    q, k, v = inputs(3, 1, 4, 2, 64, 40, F16)
+    out = torch.zeros(2000, device=DEV, dtype=F16).as_strided(q.shape, strides)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.attn_window(q, k, v, at(3), 4, out=out)
+
+
+def test_outputs_in_any_order_of_dimensions_are_taken():
+    q, k, v = inputs(3, 5, 4, 2, 64, 40, F16)
+    want = ops.attn_window(q, k, v, at(3), 9, 1)
+    for order in ((0, 1, 2), (2, 0, 1), (1, 2, 0), (2, 1, 0)):
+        shape = [q.shape[i] for i in order]
+        out = torch.zeros(*shape, 72, device=DEV, dtype=F16)[..., :64].permute(*(order.index(i) for i in range(3)), 3)
+        assert torch.equal(ops.attn_window(q, k, v, at(3), 9, 1, out=out), want)
