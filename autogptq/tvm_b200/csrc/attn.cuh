@@ -3,6 +3,8 @@
 
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace b200gptq {
@@ -72,41 +74,106 @@ __device__ __forceinline__ AttnRange attn_range(int p_lo, int p_hi, int window, 
     return r;
 }
 
-// One query row by one warp, key by key, skipping the rows that it does not see.  The tiles of both kernels multiply weights of zero with whatever
+// One query row by one warp, a few keys at a time, skipping the rows that it does not see.  The tiles of both kernels multiply weights of zero with whatever
 // the rows hold that other queries of the tile see: where that gives a NaN or an infinity the row is done again here.  A lane owns HD / 32 dims.
+// Whether there is anything to do is looked at first, since one such value in a row that all see (a sink) sends every row of a long prompt here:
+//   * the dims that came out finite are right, and so is an infinity in fp16: 2^8 times the largest fp16 number, 2^29 times over, is far from fp32's end, so it
+//     is that of values which the row sees, with weights that are not zero, and of one sign;
+//   * a dim in which the row sees a NaN is one.  Those are looked for without the scores, a few rows of V at a time.
+// One prompt of 8192, 32 / 8 heads of 128, window 4096 (0.36 ms) with one value per key head that is not finite: in a sink 0.57 (NaN) and 0.47 ms (infinity
+// in fp16), 231 where every row was done again one key at a time; in the middle 32 and 21 ms, 176 so; an infinity in bf16, whose rows are all done again, 131.
 template <typename T, int HD>
 __device__ __noinline__ void attn_row_again(const b200gptq_attn_args& a, int b, int t, int head, int p, int d0, int d1) {
-    constexpr int D = HD / 32;
+    constexpr int D = HD / 32, kAgain = 8;    // keys whose loads are on their way at once
     const int lane = threadIdx.x & 31, kh = head / (a.heads / a.kv_heads), window = a.window ? a.window : 1 << 30;
+    T* out = static_cast<T*>(a.out) + b * a.out_stride[0] + t * a.out_stride[1] + head * a.out_stride[2];
+    const AttnRange r = attn_range(p, p, window, a.sinks, a.max_seq);
+    const T *kp = static_cast<const T*>(a.k_prefix) + kh * a.k_prefix_stride[0] + lane * D,
+            *vp = static_cast<const T*>(a.v_prefix) + kh * a.v_prefix_stride[0] + lane * D;
+    const T *kc = static_cast<const T*>(a.k_cache) + b * a.k_stride[0] + kh * a.k_stride[1] + lane * D,
+            *vc = static_cast<const T*>(a.v_cache) + b * a.v_stride[0] + kh * a.v_stride[1] + lane * D;
+    unsigned open = 0;                        // dims of the lane that are not known yet
+#pragma unroll
+    for (int e = 0; e < D; ++e) {
+        const int d = lane * D + e;
+        const float f = d >= d0 && d < d1 ? Half<T>::wide(out[d]) : 0.f;
+        if (isnan(f) || (isinf(f) && !std::is_same<T, __half>::value)) open |= 1u << e;
+    }
+    auto known = [&](const T* v, long long stride, int j, int end) {
+        for (; __any_sync(0xffffffffu, open) && j < end; j += kAgain)
+#pragma unroll
+            for (int u = 0; u < kAgain; ++u) {
+                const uint32_t* row = reinterpret_cast<const uint32_t*>(v + min(j + u, end - 1) * stride);
+#pragma unroll
+                for (int e = 0; e < D; e += 2) {
+                    const float2 f = Half<T>::unpack(row[e / 2]);
+                    if (isnan(f.x)) open &= ~(1u << e);
+                    if (isnan(f.y)) open &= ~(2u << e);
+                }
+            }
+    };
+    known(vp, a.v_prefix_stride[1], 0, a.prefix);
+    known(vc, a.v_stride[2], 0, r.s_end);
+    known(vc, a.v_stride[2], r.w_start, r.w_end);
+    if (!__any_sync(0xffffffffu, open)) return;
     const T* q = static_cast<const T*>(a.q) + b * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2] + lane * D;
     float qf[D], acc[D], m = -INFINITY, l = 0.f;
 #pragma unroll
     for (int e = 0; e < D; ++e) { qf[e] = Half<T>::wide(q[e]) * a.scale * kLog2e; acc[e] = 0.f; }
-    auto key = [&](const T* k, const T* v) {
-        float s = 0.f;
+    auto keys = [&](const T* k, long long k_stride, const T* v, long long v_stride, int j, int end) {
+        for (; j < end; j += kAgain) {
+            uint32_t kw[kAgain][D / 2], vw[kAgain][D / 2];
+            float s[kAgain], up = m;
 #pragma unroll
-        for (int e = 0; e < D; ++e) s = fmaf(qf[e], Half<T>::wide(k[e]), s);
+            for (int u = 0; u < kAgain; ++u) {
+                const long long at = min(j + u, end - 1);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        const float up = fmaxf(m, s), safe = up == -INFINITY ? 0.f : up, corr = exp2_fast(m - safe), w = exp2_fast(s - safe);
-        m = up;
-        l = l * corr + w;
+                for (int e = 0; e < D / 2; ++e) {
+                    kw[u][e] = reinterpret_cast<const uint32_t*>(k + at * k_stride)[e];
+                    vw[u][e] = reinterpret_cast<const uint32_t*>(v + at * v_stride)[e];
+                }
+            }
 #pragma unroll
-        for (int e = 0; e < D; ++e) acc[e] = acc[e] * corr + w * Half<T>::wide(v[e]);
+            for (int u = 0; u < kAgain; ++u) {
+                s[u] = 0.f;
+#pragma unroll
+                for (int e = 0; e < D; e += 2) {
+                    const float2 f = Half<T>::unpack(kw[u][e / 2]);
+                    s[u] = fmaf(qf[e + 1], f.y, fmaf(qf[e], f.x, s[u]));
+                }
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+                for (int u = 0; u < kAgain; ++u) s[u] += __shfl_xor_sync(0xffffffffu, s[u], o);
+#pragma unroll
+            for (int u = 0; u < kAgain; ++u)
+                if (j + u < end) up = fmaxf(up, s[u]);
+            const float safe = up == -INFINITY ? 0.f : up, corr = exp2_fast(m - safe);
+            m = up;
+            l *= corr;
+#pragma unroll
+            for (int e = 0; e < D; ++e) acc[e] *= corr;
+#pragma unroll
+            for (int u = 0; u < kAgain; ++u)
+                if (j + u < end) {
+                    const float w = exp2_fast(s[u] - safe);
+                    l += w;
+#pragma unroll
+                    for (int e = 0; e < D; e += 2) {
+                        const float2 f = Half<T>::unpack(vw[u][e / 2]);
+                        acc[e] = fmaf(w, f.x, acc[e]);
+                        acc[e + 1] = fmaf(w, f.y, acc[e + 1]);
+                    }
+                }
+        }
     };
-    const T *kp = static_cast<const T*>(a.k_prefix) + kh * a.k_prefix_stride[0] + lane * D,
-            *vp = static_cast<const T*>(a.v_prefix) + kh * a.v_prefix_stride[0] + lane * D;
-    for (int j = 0; j < a.prefix; ++j) key(kp + j * a.k_prefix_stride[1], vp + j * a.v_prefix_stride[1]);
-    const T *kc = static_cast<const T*>(a.k_cache) + b * a.k_stride[0] + kh * a.k_stride[1] + lane * D,
-            *vc = static_cast<const T*>(a.v_cache) + b * a.v_stride[0] + kh * a.v_stride[1] + lane * D;
-    const AttnRange r = attn_range(p, p, window, a.sinks, a.max_seq);
-    for (int j = 0; j < r.s_end; ++j) key(kc + j * a.k_stride[2], vc + j * a.v_stride[2]);
-    for (int j = r.w_start; j < r.w_end; ++j) key(kc + j * a.k_stride[2], vc + j * a.v_stride[2]);
-    T* out = static_cast<T*>(a.out) + b * a.out_stride[0] + t * a.out_stride[1] + head * a.out_stride[2];
+    keys(kp, a.k_prefix_stride[1], vp, a.v_prefix_stride[1], 0, a.prefix);
+    keys(kc, a.k_stride[2], vc, a.v_stride[2], 0, r.s_end);
+    keys(kc, a.k_stride[2], vc, a.v_stride[2], r.w_start, r.w_end);
 #pragma unroll
     for (int e = 0; e < D; ++e) {
-        const int d = lane * D + e;
-        if (d >= d0 && d < d1) out[d] = Half<T>::round(l != 0.f ? acc[e] / l : 0.f);       // (a NaN stays one)
+        if (open >> e & 1u) out[lane * D + e] = Half<T>::round(l != 0.f ? acc[e] / l : 0.f);       // (a NaN stays one)
     }
 }
 

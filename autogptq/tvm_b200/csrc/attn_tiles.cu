@@ -578,6 +578,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                     if (alt) {
                         const float4 g = stage[(kRows + row) * CH + (chunk ^ (row & 7))];
                         f = make_float4(f.x * e0 + g.x * e1, f.y * e0 + g.y * e1, f.z * e0 + g.z * e1, f.w * e0 + g.w * e1);
+                        if (e0 == 0.f && e1 == 0.f) f = make_float4(0.f, 0.f, 0.f, 0.f);       // (nothing seen, as above: not zero times a NaN)
                     }
                     if constexpr (PACKED) {
                         *reinterpret_cast<float4*>(p.part + at * HD + 4 * chunk) = f;

@@ -401,3 +401,33 @@ def test_outputs_in_any_order_of_dimensions_are_taken():
         shape = [q.shape[i] for i in order]
         out = torch.zeros(*shape, 72, device=DEV, dtype=F16)[..., :64].permute(*(order.index(i) for i in range(3)), 3)
         assert torch.equal(ops.attn_window(q, k, v, at(3), 9, 1, out=out), want)
+
+
+def microseconds(call, n=5):
+    for _ in range(2):
+        call()
+    e = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+    torch.cuda.synchronize()
+    e[0].record()
+    for _ in range(n):
+        call()
+    e[1].record()
+    e[1].synchronize()
+    return e[0].elapsed_time(e[1]) * 1000 / n
+
+
+@pytest.mark.parametrize("dtype,junk", [(F16, math.nan), (BF16, math.nan), (F16, math.inf), (F16, -math.inf)])
+@pytest.mark.parametrize("T,B", [(4096, 1), (1, 32)])
+def test_one_value_that_is_not_finite_does_not_slow_a_call_down(T, B, dtype, junk):
+    """In one dim of a sink's value, which every row sees: that dim is it in every row, and the call takes about as long as without.  (Where each row
+    is done again key by key it takes hundreds of times as long; the bound of ten leaves room for other users of the machine.)"""
+    q, k, v = inputs(B, T, 8, 8, 128, 4096, dtype)
+    pos = at(4096 - T)
+    clean = ops.attn_window(q, k, v, pos, 2000, 4)
+    before = microseconds(lambda: ops.attn_window(q, k, v, pos, 2000, 4))
+    v[:, :, 0, 77] = junk
+    got = ops.attn_window(q, k, v, pos, 2000, 4)
+    assert bool((got[..., 77].isnan() if math.isnan(junk) else got[..., 77] == junk).all())
+    rest = [d for d in range(128) if d != 77]
+    assert torch.equal(got[..., rest], clean[..., rest])
+    assert microseconds(lambda: ops.attn_window(q, k, v, pos, 2000, 4)) < 10 * before
