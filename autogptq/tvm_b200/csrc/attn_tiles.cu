@@ -601,7 +601,11 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             const float inv = l != 0.f ? 1.f / l : 0.f;
             const long long out_at = b * a.out_stride[0] + t * a.out_stride[1] + head * a.out_stride[2];
             bool bad = false;
-            uint8_t* stage = base_ptr + q * SM::q_tile;                  // (the products with Q are done; a warp stores what it has staged)
+            // A warp stores what it has staged, where other warps have written Q: the products with Q are done, or, in a tile that sees no keys and has
+            // waited for none, Q is there (else it came down on rows that were staged already).
+            uint8_t* stage = base_ptr + q * SM::q_tile;
+            if (turn == 0) mbar_wait(q_full(q), 0, &abort_flag);
+            __syncwarp();
 #pragma unroll 1
             for (int c = 0; c < HD / 32; ++c) {
                 uint32_t o[32];

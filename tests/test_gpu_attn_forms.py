@@ -305,3 +305,18 @@ def test_streams_and_graphs(name):
         for _, x, y, _, _ in graphs:
             assert torch.equal(x, w) and torch.equal(y, w)
     ops.check_status(DEV)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("at,W", [(-1000, 14), (-130, 14), (5000, 14)])
+def test_tiles_that_see_nothing(at, W, hd):
+    """Whole tiles of rows before position 0, or so far behind the cache that the window has left it: zeros.  (The queries are more than the L2 holds, so
+    that the warps of a tile get theirs at different times.)"""
+    B, T, heads = 400, 257, 8
+    q = torch.full((B, T, heads, hd), 3.0, device=DEV, dtype=F16)
+    k = torch.ones(B, heads, 1, hd, device=DEV, dtype=F16)
+    p = at + torch.arange(T, device=DEV)
+    empty = (p < 0) | (p >= W)
+    for _ in range(6):
+        got = ops.attn_window(q, k, k, torch.tensor([at], device=DEV), W, 0)
+        assert bool((got[:, empty] == 0).all()) and bool((got[:, ~empty] == 1).all())
