@@ -33,13 +33,20 @@ int check_sizes(const b200gptq_attn_args& a) {
 AttnPlan plan_of(const b200gptq_attn_args& a) {
     AttnPlan p = {};
     const long long rows = (long long)a.tokens * (a.heads / a.kv_heads), all = rows * a.batch, sms = sm_count();
+    // 64 rows of a key head or more: the tcgen05 kernel, which has all keys of a tile in one CTA; fewer: the rows kernel, which splits them over CTAs.  Measured
+    // (32 / 8 heads of 128, us, tcgen05 kernel and rows kernel).  Many sequences: 64 behind 500 positions, 32 rows 45 and 54, 60 rows 47 and 98; 8 with a
+    // window of 4096, 32 rows 39 and 46, 64 rows 41 and 77, 128 rows 43 and 145.  One sequence has few tiles, and the rows kernel stays ahead up to some 256 rows: behind
+    // 16384, 64 rows 120 and 80, 128 rows 131 and 73, 256 rows 132 and 132, 800 rows 133 and 478; window 4096, 64 rows 39 and 34, 128 rows 41 and 26, 256
+    // rows 41 and 40, 800 rows 42 and 129.  The rule is the many sequences'; one that knows tiles and keys, and a tcgen05 kernel that splits the keys, are not there.
     if (rows >= 64 && attn_tiles_maps(a, false) && (!a.prefix || attn_tiles_maps(a, true))) {
         p.tiles = true;
         return p;
     }
     // Warps per tile of rows: as many as the SMs hold (16 each, or 8 where a tile has more than 8 rows), a block of 16 keys for each at least.
     const long long tile = rows <= 8 ? 8 : rows <= 16 ? 16 : 32, held = sms * (rows <= 8 ? 16 : 8), units = (rows + tile - 1) / tile * a.kv_heads * a.batch;
-    // The prefix among each sequence's keys: `again` bytes more, from L2.  Two more launches cost 5 us.
+    // The prefix among each sequence's keys: `again` bytes more, from L2, or before, with two more launches.  Single tokens, us, among and before: 8 sequences,
+    // 8 key heads of 128, 500 positions (14 MB) 8.0 and 12.1; 4, 32 key heads, 500 (25 MB) 9.4 and 11.6; 5, 8 key heads, 2000 (33 MB) 13.9 and 13.8; 8 of them
+    // (57 MB) 14.1 and 15.0; 16 (123 MB) 22.7 and 14.8; 2, 8 key heads, 16384 (67 MB) 39.3 and 24.5; 64, 8 key heads, 500 (129 MB) 24.2 and 13.0.
     const double again = (double)(a.batch - 1) * a.kv_heads * a.prefix * a.hd * 4;
     const bool apart = a.prefix && again > 32e6;
     const long long keys = (a.window ? std::min<long long>(a.max_seq, (long long)a.window + a.sinks + a.tokens) : a.max_seq) + (apart ? 0 : a.prefix);
@@ -49,9 +56,9 @@ AttnPlan plan_of(const b200gptq_attn_args& a) {
         p.prefix_tiles = all > 32 && attn_tiles_maps(a, true);
         if (p.prefix_tiles) {
             const long long blocks = (a.prefix + kAttnTilesKeys - 1) / kAttnTilesKeys, ctas = (all + 255) / 256 * a.kv_heads;
-            // SMs by bytes, the caches taken to be half full, a third at least: the sequences' own launch runs on the others.  32 sequences, 8 key
-            // heads of 128, 8192 keys before 130 of 640 each: 23.9 us, 32.4 where the prefix takes every SM; 64 sequences, 4096 before 500 of 1024:
-            // 46.5 and 84.9 (43 without the third); 48 sequences, 12000 before 150 of 2048: 42.9 and 47.2 (65 without the third).
+            // SMs by bytes, the caches taken to be half full, a third at least: the sequences' own launch runs on the others.  32 / 8 heads of 128, us,
+            // this share, every SM for the prefix, and without the third: 32 sequences, 8192 keys before 130 of 640 each, 19.6, 25.7 and 19.6; 64, 4096 before
+            // 500 of 1024, 55.4, 57.5 and 45.5; 48, 12000 before 150 of 2048, 44.2, 38.0 and 70.6.  (How full the caches are is known on the device only.)
             const double share = std::max(1. / 3, a.prefix / (a.prefix + 0.5 * a.batch * a.max_seq));
             p.parts = (int)std::max<long long>(1, std::min(std::min<long long>((long long)(sms * share) / ctas, kAttnMaxParts), blocks / 4));
         } else {

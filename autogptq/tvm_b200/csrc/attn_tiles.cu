@@ -22,7 +22,7 @@
 // tensor memory, V is the B operand as it lies (MN-major, keys along K).
 //
 // Rows of V that no row of the tiles sees are zeroed in shared memory before they are multiplied (a weight of zero times a NaN is one).  Where rows of the
-// tiles see different keys and one of these holds a NaN or an infinity, the rows that come out not finite are done again, key by key.
+// tiles see different keys and one of these holds a NaN or an infinity, the rows that come out not finite are done again (attn_row_again).
 //
 // PACKED: the rows are (sequence, token, head of the group) of the whole batch against the shared prefix, split over CTAs, sums to scratch.
 // ALT (few rows): both tiles of Q are the same rows, one takes the even units of keys and the other the odd ones; they add up at the end.
@@ -216,7 +216,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     tc_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base_holder, 0);
     // ---- which rows, which keys.  The last rows of a prompt see most, and come first (the tiles of one head one after the other read two chunks of 512 of 72
-    //      heads once instead of 1.4 times, which took as long; one prompt of 4096 without a window 158 us, now 136). ----
+    //      heads once instead of 1.4 times, which took as long; one prompt of 4096, 32 heads, without a window 158 us, now 137). ----
     const int G = p.group, window = a.window ? a.window : 1 << 30;
     const unsigned part_unit = PACKED ? over(blockIdx.x, p.by_splits) : blockIdx.x, over_heads = over(part_unit, p.by_kv_heads);
     const unsigned row_tile = PACKED ? over_heads : over(over_heads, p.by_batch);

@@ -471,8 +471,8 @@ def attn_window(q, k_cache, v_cache, pos, window: int, sinks: int = 0, counts=No
 
 
 def attn_prefix(q, k_prefix, v_prefix, k_cache, v_cache, pos, counts=None, scale: Optional[float] = None, out=None):
-    """Attention of a batch whose sequences begin with the same text: ``k_prefix`` / ``v_prefix`` ``[kv_heads, P, hd]`` are held and read once
-    for all (P may be 0), the rest of each sequence is in its own rows of the caches ``[B, kv_heads, max_seq, hd]``.  A query sees all P rows and rows
+    """Attention of a batch whose sequences begin with the same text: ``k_prefix`` / ``v_prefix`` ``[kv_heads, P, hd]`` are held once for all, and read once
+    where reading them again for each sequence would pass 32 MB and a sequence has fewer than 64 rows (tokens x heads) per key head (P may be 0), the rest of each sequence is in its own rows of the caches ``[B, kv_heads, max_seq, hd]``.  A query sees all P rows and rows
     ``0 .. pos + t`` of its own; ``pos`` counts the sequence's own rows (-1: none).  Otherwise as :func:`attn_window`."""
     if k_prefix is None or v_prefix is None:
         raise TypeError("k_prefix and v_prefix must be tensors")
