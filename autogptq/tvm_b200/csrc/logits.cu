@@ -182,8 +182,8 @@ adjust_kernel(const __grid_constant__ b200gptq_logit_args a, int slice, int slic
 
 template <typename T, bool WIDE>
 int launch(const b200gptq_logit_args& a, cudaStream_t stream) {
-    // Slices: the first of 1024, 2048, 4096 and 8192 whose grid fits the SMs at once (kPerSm CTAs each; two where words are WIDE, 83 KB for 8192), else the last: every
-    // CTA goes through the history.  Not all grids are whole waves: 64 rows of 50272 are 448 CTAs for 444 places, 128 of 32000 are 512 (7.3 and 6.5 us with penalties alone).
+    // Slices: the first of 1024, 2048, 4096 and 8192 whose grid is at most kPerSm CTAs per SM, else the last, since every CTA goes through the history.  (Where words
+    // are WIDE, 83 KB for 8192, two of the last are on an SM at once.)  Not all grids are whole waves: 64 rows of 50272 are 448 CTAs for 444 places, 128 of 32000 are 512 (7.3 and 6.5 us with penalties alone).
     int slice = 1024;
     while (slice < kMaxSlice && (long long)a.rows * ((a.vocab + slice - 1) / slice) > (long long)kPerSm * sm_count()) slice *= 2;
     const int slices = (a.vocab + slice - 1) / slice;
