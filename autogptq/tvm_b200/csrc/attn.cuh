@@ -32,6 +32,7 @@ template <> struct Half<__half> {
     __device__ static __forceinline__ float2 unpack(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
     __device__ static __forceinline__ __half round(float a) { return __float2half_rn(a); }
     __device__ static __forceinline__ float wide(__half a) { return __half2float(a); }
+    static constexpr float kTop = 65504.f;
 };
 template <> struct Half<__nv_bfloat16> {
     __device__ static __forceinline__ uint32_t pack(float a, float b) {
@@ -41,7 +42,24 @@ template <> struct Half<__nv_bfloat16> {
     __device__ static __forceinline__ float2 unpack(uint32_t u) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u)); }
     __device__ static __forceinline__ __nv_bfloat16 round(float a) { return __float2bfloat16_rn(a); }
     __device__ static __forceinline__ float wide(__nv_bfloat16 a) { return __bfloat162float(a); }
+    static constexpr float kTop = 3.4028235e38f;      // (of fp32: values near bf16's largest number pass its range as they are added up)
 };
+
+// N results of a row, before they are rounded; whether one of them is not finite.  A mean of values is no larger than the largest of them, but with weights that
+// are rounded and a sum that is not it can pass fp16's largest number by 2^-11, which rounds to infinity: it is that number then.  (All are looked at
+// together: two chunks of 512 of 72 heads 61.2 us; 62.2 with each one held by itself, 60.4 with none.)
+template <typename T, int N> __device__ __forceinline__ bool settle(float (&f)[N]) {
+    bool odd = false, bad = false;
+#pragma unroll
+    for (int x = 0; x < N; ++x) odd = odd || !(fabsf(f[x]) <= Half<T>::kTop);
+    if (odd)
+#pragma unroll
+        for (int x = 0; x < N; ++x) {
+            if (isfinite(f[x])) f[x] = fminf(fmaxf(f[x], -Half<T>::kTop), Half<T>::kTop);
+            else bad = true;
+        }
+    return bad;
+}
 
 __device__ __forceinline__ float exp2_fast(float x) {       // 2^x; 0 for -infinity
     float y;

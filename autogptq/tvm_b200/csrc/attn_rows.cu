@@ -397,10 +397,10 @@ attn_rows_kernel(const __grid_constant__ b200gptq_attn_args a, float* __restrict
             continue;
         }
         const bool none = tl == 0.f;
-        o = make_float4(none ? 0.f : o.x / tl, none ? 0.f : o.y / tl, none ? 0.f : o.z / tl, none ? 0.f : o.w / tl);
+        float f[4] = {none ? 0.f : o.x / tl, none ? 0.f : o.y / tl, none ? 0.f : o.z / tl, none ? 0.f : o.w / tl};
+        if (settle<T>(f) && isfinite(tl)) flags[row] = 1;
         *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + places[R + row] + split * slice + d) =
-            make_uint2(Half<T>::pack(o.x, o.y), Half<T>::pack(o.z, o.w));
-        if (isfinite(tl) && (!isfinite(o.x) || !isfinite(o.y) || !isfinite(o.z) || !isfinite(o.w))) flags[row] = 1;
+            make_uint2(Half<T>::pack(f[0], f[1]), Half<T>::pack(f[2], f[3]));
     }
     if (parts) {
         if (blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -468,13 +468,14 @@ attn_sum_kernel(const __grid_constant__ b200gptq_attn_args a, const float* __res
         sum.z += __shfl_xor_sync(0xffffffffu, sum.z, 16); sum.w += __shfl_xor_sync(0xffffffffu, sum.w, 16);
     }
     const bool none = tl == 0.f;
-    sum = make_float4(none ? 0.f : sum.x / tl, none ? 0.f : sum.y / tl, none ? 0.f : sum.z / tl, none ? 0.f : sum.w / tl);
+    float mean[4] = {none ? 0.f : sum.x / tl, none ? 0.f : sum.y / tl, none ? 0.f : sum.z / tl, none ? 0.f : sum.w / tl};
+    const bool bad = settle<T>(mean);
     if (lane < LANES)
         *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + b * a.out_stride[0] + t * a.out_stride[1] + head * a.out_stride[2] + 4 * lane) =
-            make_uint2(Half<T>::pack(sum.x, sum.y), Half<T>::pack(sum.z, sum.w));
+            make_uint2(Half<T>::pack(mean[0], mean[1]), Half<T>::pack(mean[2], mean[3]));
     __syncwarp();
     // (as in attn_rows_kernel)
-    if (__any_sync(0xffffffffu, isfinite(tl) && !(isfinite(sum.x) && isfinite(sum.y) && isfinite(sum.z) && isfinite(sum.w))))
+    if (__any_sync(0xffffffffu, isfinite(tl) && bad))
         attn_row_again<T, HD>(a, b, t, head, attn_pos(a, b) + t, 0, HD);
 }
 

@@ -13,7 +13,7 @@
 //                     softmax always finds the next S there and waits for no product
 //
 // Measured per unit and both tiles, 128 dims: 1 570 clk; the products alone 1 280 (Q and K are 48 KB of shared memory, 384 clk, for 256 of arithmetic), the
-// exponentials, which both tiles do at the same time, 1 030 of a softmax warp's turn.  One prompt of 8192, 32 / 8 heads, window 4096: 355 us, 1 160 TFLOP/s;
+// exponentials, which both tiles do at the same time, 1 030 of a softmax warp's turn.  One prompt of 8192, 32 / 8 heads, window 4096: 357 us, 1 150 TFLOP/s;
 // 411 when it runs for seconds and the power limit holds the clock at 1.6 GHz.
 // Units of 128 keys with one S per tile of Q, so that softmax and products of a tile took turns, took 3900 to 4600 clk per 128 keys, with two threads per
 // row (which exchange its maximum) 4100: 1550 of them the products, 2500 the softmax.
@@ -583,9 +583,10 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                     if constexpr (PACKED) {
                         *reinterpret_cast<float4*>(p.part + at * HD + 4 * chunk) = f;
                     } else {
-                        *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at + 4 * chunk) = make_uint2(Half<T>::pack(f.x, f.y), Half<T>::pack(f.z, f.w));
+                        float mean[4] = {f.x, f.y, f.z, f.w};
                         // (a NaN or an infinity in V that the row does not see: done again below)
-                        if (!isfinite(f.x + f.y + f.z + f.w)) atomicOr(flags + row, 1);
+                        if (settle<T>(mean)) atomicOr(flags + row, 1);
+                        *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at + 4 * chunk) = make_uint2(Half<T>::pack(mean[0], mean[1]), Half<T>::pack(mean[2], mean[3]));
                     }
                 }
             if constexpr (!PACKED) {
@@ -618,11 +619,8 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                 for (int e = 0; e < 4; ++e) {
                     float f[8];
 #pragma unroll
-                    for (int x = 0; x < 8; ++x) {
-                        // (nothing seen: zero; a NaN or an infinity in V that the row does not see: done again below)
-                        f[x] = turn == 0 || l == 0.f ? 0.f : __uint_as_float(o[8 * e + x]) * inv;
-                        bad = bad || !isfinite(f[x]);
-                    }
+                    for (int x = 0; x < 8; ++x) f[x] = turn == 0 || l == 0.f ? 0.f : __uint_as_float(o[8 * e + x]) * inv;       // (nothing seen: zero)
+                    if (settle<T>(f)) bad = true;              // (a NaN or an infinity in V that the row does not see: done again below)
                     const uint4 h = make_uint4(Half<T>::pack(f[0], f[1]), Half<T>::pack(f[2], f[3]), Half<T>::pack(f[4], f[5]), Half<T>::pack(f[6], f[7]));
                     *reinterpret_cast<uint4*>(stage + r * HD * 2 + (((4 * c + e) ^ (r & 7)) << 4)) = h;
                 }
