@@ -67,10 +67,11 @@ __device__ __forceinline__ float exp2_fast(float x) {       // 2^x; 0 for -infin
     return y;
 }
 
-// Position of token 0 of sequence b.  Positions far outside the cache behave like those just outside (all sizes are below 2^30).
+// Position of token 0 of sequence b.  Positions far outside the cache behave like those just outside (all sizes are 2^29 at most: with a window what
+// lies 2^30 out has left the cache behind; without, where a window of 2^30 stands for none, tokens up to 2^29 - 1 further on still see row 0).
 __device__ __forceinline__ int attn_pos(const b200gptq_attn_args& a, int b) {
     const long long p = __ldcg(reinterpret_cast<const long long*>(a.pos) + (a.pos_each ? b : 0));
-    return (int)max(min(p, 1LL << 30), -(1LL << 30));
+    return (int)max(min(p, a.window ? 1LL << 30 : 1LL << 29), -(1LL << 30));
 }
 __device__ __forceinline__ int attn_count(const b200gptq_attn_args& a, int b) {
     if (!a.counts) return a.tokens;

@@ -347,3 +347,27 @@ def test_values_at_the_end_of_fp16(name, monkeypatch):
     some = torch.stack([c.sees(b).any(1) for b in range(c.B)]) | bool(c.P)
     assert bool((got[~some] == 0).all()) and bool(torch.isfinite(got).all())
     assert bool(((got[some].double() - sign.double()).abs() <= 2 * 2.0 ** -11 * top).all())
+
+
+@every_form
+def test_a_negative_scale_is_that_of_the_negated_queries(name):
+    """Bit for bit, as a sign changes no rounding; and a scale of zero is that of queries of zero."""
+    c = Call(name)
+    assert torch.equal(c(scale=-0.1), c(q=-c.q, scale=0.1))
+    assert torch.equal(c(scale=0.0), c(q=torch.zeros_like(c.q), scale=0.1))
+
+
+@every_form
+def test_numbers_far_out_of_range(name):
+    """Positions and counts at the ends of 64 bits are held to what there is."""
+    c = Call(name)
+    ends = torch.tensor([(1 << 63) - 1, -(1 << 63)], device=DEV)
+    out = torch.full_like(c.q, 7.0)
+    c(counts=ends[1].expand(c.B).contiguous(), out=out)
+    assert bool((out == 7).all())
+    want = c()
+    assert torch.equal(c(counts=ends[0].expand(c.B).contiguous(), out=out), want)
+    c.at = [-(1 << 40)] * c.B
+    check(c(pos=ends[1:]), *c.reference())
+    c.at = [1 << 40] * c.B
+    check(c(pos=ends[:1]), *c.reference())
