@@ -371,3 +371,12 @@ def test_numbers_far_out_of_range(name):
     check(c(pos=ends[1:]), *c.reference())
     c.at = [1 << 40] * c.B
     check(c(pos=ends[:1]), *c.reference())
+
+
+@pytest.mark.parametrize("W,S", [(1 << 29, 0), (1 << 29, 1 << 29), (1, 1 << 29), (30, 61)])
+@pytest.mark.parametrize("name", [*(n for n in FORMS if "P" not in FORMS[n]), *SMALL])
+def test_the_largest_windows_and_sinks(name, W, S, monkeypatch):
+    monkeypatch.setitem(FORMS, "here", dict(SMALL.get(name, {}), hd=64, W=60, S=2, parts=None))
+    c = Call(name if name in FORMS else "here")
+    c.W, c.S = W, S
+    check(c(), *c.reference())
