@@ -65,6 +65,8 @@ _SIGNATURES = {
     "b200gptq_attn_workspace_bytes": (ctypes.c_int64, [_c_void_p]),
     "b200gptq_attn": (_c_int, [_c_void_p, _c_void_p, _c_size_t, _c_void_p]),
     "b200gptq_adjust_logits": (_c_int, [_c_void_p, _c_void_p]),
+    "b200gptq_cache_write": (_c_int, [_c_void_p, _c_void_p]),
+    "b200gptq_cache_read": (_c_int, [_c_void_p, _c_void_p]),
     "b200gptq_step_plan_bytes": (_c_size_t, [_c_void_p]),
     "b200gptq_step_table_bytes": (_c_size_t, [_c_int]),
     "b200gptq_step_plan_create": (_c_int, [_c_void_p] * 4),
@@ -101,6 +103,23 @@ class LogitArgs(ctypes.Structure):
                                           "presence", "bias_values", "mask")]
                 + [(n, ctypes.c_int64) for n in ("logits_stride", "out_stride", "history_stride", "mask_stride")]
                 + [(n, _c_int) for n in ("dtype", "rows", "vocab", "history_len", "biases")])
+
+
+class Cache4(ctypes.Structure):
+    _fields_ = ([(n, _c_void_p) for n in ("k", "v", "k_scales", "v_scales")]
+                + [(n, ctypes.c_int64 * 3) for n in ("k_stride", "v_stride", "k_scale_stride", "v_scale_stride")]
+                + [(n, _c_int) for n in ("dtype", "batch", "kv_heads", "max_seq", "hd", "group")])
+
+
+class CacheWriteArgs(ctypes.Structure):
+    _fields_ = ([("cache", Cache4)] + [(n, _c_void_p) for n in ("k", "v", "q", "cos_t", "sin_t", "q_out", "k_out", "v_out", "pos", "counts")]
+                + [(n, ctypes.c_int64 * 3) for n in ("k_stride", "v_stride", "q_stride", "q_out_stride", "k_out_stride", "v_out_stride")]
+                + [(n, _c_int) for n in ("tokens", "heads", "angles", "pos_each")])
+
+
+class CacheReadArgs(ctypes.Structure):
+    _fields_ = ([("cache", Cache4)] + [(n, _c_void_p) for n in ("k_out", "v_out", "lengths")]
+                + [(n, ctypes.c_int64 * 3) for n in ("k_out_stride", "v_out_stride")])
 
 
 def _load() -> ctypes.CDLL:

@@ -419,12 +419,14 @@ void need_device(const at::Tensor& t, int device, const char* name) {
 }
 // The arguments' names, in the order of the calls below.
 constexpr int kArguments = 11;
+constexpr const char* kWriteNames[] = {"k", "v", "cache.k", "cache.v", "cache.k_scales", "cache.v_scales", "pos", "counts", "cos", "sin", "q", "q_out", "k_out", "v_out"};
+constexpr const char* kReadNames[] = {"cache.k", "cache.v", "cache.k_scales", "cache.v_scales", "lengths", "k_out", "v_out"};
 constexpr const char* kAttnNames[kArguments] = {"q", "k_prefix", "v_prefix", "k_cache", "v_cache", "pos", "window", "sinks", "counts", "scale", "out"};
 constexpr const char* kLogitNames[kArguments] = {"logits", "history", "lengths", "prompt_lens", "repetition", "frequency", "presence", "bias_tokens", "bias_values", "mask", "out"};
 // No argument asks for a derivative, backward or (a dual number, which knows no no_grad) forward: penalties and biases could as well as the logits.
-void need_no_gradients(PyObject* const* args, const char* const* names) {
+void need_no_gradients(PyObject* const* args, const char* const* names, int count) {
     const bool backward = at::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
-    for (int i = 0; i < kArguments; ++i) {
+    for (int i = 0; i < count; ++i) {
         // (THPVariable_Check asks Python about what is no tensor: 100 ns each)
         if (args[i] == Py_None || PyLong_CheckExact(args[i]) || PyFloat_CheckExact(args[i]) || !THPVariable_Check(args[i])) continue;
         const at::Tensor& t = THPVariable_Unpack(args[i]);
@@ -663,10 +665,179 @@ PyObject* logits_checked(PyObject* const* args) {
     return answer(std::move(out), t[10] != nullptr, st);
 }
 
-PyObject* raising(PyObject* (*call)(PyObject* const*), const char* const* names, PyObject* const* args, Py_ssize_t nargs) {
-    if (nargs != kArguments) { PyErr_SetString(PyExc_TypeError, "11 arguments"); return nullptr; }
+// ---- the cache held in 4 bits ----
+// Fills `c` from the tensors of an ops.QuantCache: codes, codes, constants, constants.  `written`: its elements have to lie apart.
+void cache_of(const at::Tensor* const (&t)[4], const char* const* names, bool written, b200gptq_cache4& c) {
+    const at::Tensor &k = *t[0], &scales = *t[2];
+    const int device = k.get_device();
+    const at::ScalarType type = scales.scalar_type();
+    if (type != at::kHalf && type != at::kBFloat16) refuse(PyExc_TypeError, std::string(names[2]) + " must be float16 or bfloat16");
+    need(k.dim() == 4 && k.numel() > 0, names[0], "must be [batch, kv_heads, max_seq, head_dim / 2]");
+    const int64_t B = k.size(0), KV = k.size(1), S = k.size(2), hd = 2 * k.size(3);
+    need(hd == 64 || hd == 128, names[0], "must have heads of 64 or 128 dims");
+    need(B <= (1 << 29) && KV <= (1 << 29) && S <= (1 << 29), names[0], "is too large");
+    need(scales.dim() == 5 && scales.size(0) == B && scales.size(1) == KV && scales.size(2) == S && scales.size(4) == 2 &&
+             (scales.size(3) * 32 == hd || scales.size(3) * 64 == hd), names[2], "must be [batch, kv_heads, max_seq, head_dim / group, 2] with groups of 32 or 64");
+    need(t[1]->sizes() == k.sizes(), names[1], "must have the shape of the keys' codes");
+    need(t[3]->sizes() == scales.sizes(), names[3], "must have the shape of the keys' constants");
+    const int64_t groups = scales.size(3);
+    void** at[4] = {&c.k, &c.v, &c.k_scales, &c.v_scales};
+    int64_t(*stride[4])[3] = {&c.k_stride, &c.v_stride, &c.k_scale_stride, &c.v_scale_stride};
+    for (int i = 0; i < 4; ++i) {
+        const at::Tensor& x = *t[i];
+        need_type(x, i < 2 ? at::kByte : type, names[i]);
+        need_device(x, device, names[i]);
+        if (i < 2) {
+            need_rows(x, names[i]);
+        } else {
+            bool ok = x.stride(4) == 1 && (groups == 1 || x.stride(3) == 2) && ((uintptr_t)data_of(x) & (uintptr_t)(4 * groups - 1)) == 0;
+            for (int d = 0; d < 3; ++d) ok = ok && (x.size(d) == 1 || x.stride(d) % (2 * groups) == 0);
+            need(ok, names[i], "must be dense in its last two dimensions, with rows that begin at multiples of their own size");
+        }
+        need(!written || apart_from_itself(x), names[i], "must not overlap itself");
+        *at[i] = const_cast<void*>(data_of(x));
+        strides_of(x, *stride[i], {0, 1, 2});
+    }
+    if (written)
+        for (int i = 0; i < 4; ++i)
+            for (int j = 0; j < i; ++j) need(!overlap(*t[i], *t[j]), names[i], "must not overlap another part of the cache");
+    c.dtype = type == at::kHalf ? B200GPTQ_F16 : B200GPTQ_BF16;
+    c.batch = (int)B; c.kv_heads = (int)KV; c.max_seq = (int)S; c.hd = (int)hd; c.group = (int)(hd / groups);
+}
+void positions_of(const at::Tensor& pos, int device, int64_t batch, const int64_t** at, int* each) {
+    need_type(pos, at::kLong, "pos");
+    need_device(pos, device, "pos");
+    need(pos.dim() == 1 && (pos.size(0) == batch || pos.size(0) == 1) && (pos.size(0) == 1 || pos.stride(0) == 1), "pos", "must be int64, dense, one number or one for each sequence");
+    *at = static_cast<const int64_t*>(data_of(pos));
+    *each = pos.size(0) > 1;
+}
+void wrote(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+// cache_write(k, v, cache.k, cache.v, cache.k_scales, cache.v_scales, pos, counts, cos, sin, q, q_out, k_out, v_out): q_out or None, or a status code
+PyObject* write_checked(PyObject* const* args) {
+    const at::Tensor* t[14];
+    for (int i = 0; i < 14; ++i) t[i] = i < 7 ? &tensor_of(args[i], kWriteNames[i]) : tensor_or_none(args[i], kWriteNames[i]);
+    const char* const* names = kWriteNames;
+    b200gptq_cache_write_args a = {};
+    const at::Tensor* const cache[4] = {t[2], t[3], t[4], t[5]};
+    cache_of(cache, names + 2, true, a.cache);
+    const int device = t[2]->get_device();
+    const at::ScalarType type = t[4]->scalar_type();
+    const int64_t B = a.cache.batch, KV = a.cache.kv_heads, hd = a.cache.hd;
+    need(t[0]->dim() == 4 && t[0]->numel() > 0 && t[0]->size(0) == B && t[0]->size(2) == KV && t[0]->size(3) == hd, "k", "must be [batch, tokens, kv_heads, head_dim] of the cache's sizes");
+    const int64_t T = t[0]->size(1);
+    need(T <= (1 << 29), "k", "is too large");
+    need((t[8] != nullptr) == (t[9] != nullptr), "cos", "and sin come together");
+    need((t[10] != nullptr) == (t[11] != nullptr), "q", "and q_out come together");
+    need((t[12] != nullptr) == (t[13] != nullptr), "k_out", "and v_out come together");
+    need(!t[10] || t[8], "q", "is there to be rotated: cos and sin are missing");
+    positions_of(*t[6], device, B, &a.pos, &a.pos_each);
+    a.counts = whole_numbers(t[7], device, B, "counts");
+    if (t[8]) {
+        for (int i : {8, 9}) {
+            need_type(*t[i], type, names[i]);
+            need_device(*t[i], device, names[i]);
+            need(t[i]->dim() == 2 && t[i]->numel() > 0 && t[i]->size(1) * 2 == hd && t[i]->size(0) <= (1 << 29) && t[i]->is_contiguous() && ((uintptr_t)data_of(*t[i]) & 15u) == 0, names[i],
+                 "must be [positions, head_dim / 2], contiguous and on 16 bytes");
+        }
+        need(t[9]->size(0) == t[8]->size(0), "sin", "must have the shape of cos");
+        a.cos_t = data_of(*t[8]); a.sin_t = data_of(*t[9]);
+        a.angles = (int)t[8]->size(0);
+    }
+    if (t[10]) {
+        need(t[10]->dim() == 4 && t[10]->numel() > 0 && t[10]->size(0) == B && t[10]->size(1) == T && t[10]->size(3) == hd && t[10]->size(2) <= (1 << 29), "q", "must be [batch, tokens, heads, head_dim]");
+        need(t[11]->sizes() == t[10]->sizes(), "q_out", "must have the shape of q");
+        a.heads = (int)t[10]->size(2);
+    }
+    struct { int i; const void** at; int64_t (*stride)[3]; } rows[6] = {{0, &a.k, &a.k_stride}, {1, &a.v, &a.v_stride}, {10, &a.q, &a.q_stride},
+        {11, const_cast<const void**>(&a.q_out), &a.q_out_stride}, {12, const_cast<const void**>(&a.k_out), &a.k_out_stride}, {13, const_cast<const void**>(&a.v_out), &a.v_out_stride}};
+    for (auto& r : rows) {
+        const at::Tensor* x = t[r.i];
+        if (!x) continue;
+        need(r.i == 10 || r.i == 11 || x->sizes() == t[0]->sizes(), names[r.i], "must have the shape of k");
+        need_type(*x, type, names[r.i]);
+        need_device(*x, device, names[r.i]);
+        need_rows(*x, names[r.i]);
+        *r.at = data_of(*x);
+        strides_of(*x, *r.stride, {0, 1, 2});
+    }
+    // what is written overlaps nothing else: the cache (2 .. 5), q_out, k_out, v_out
+    for (int i : {2, 3, 4, 5, 11, 12, 13}) {
+        if (!t[i]) continue;
+        bool apart = i < 6 || apart_from_itself(*t[i]);
+        for (int j = 0; j < 14; ++j) apart = apart && (j == i || !t[j] || (i < 6 && j >= 2 && j < 6) || !overlap(*t[i], *t[j]));
+        need(apart, names[i], "must not overlap another tensor, nor itself");
+    }
+    a.tokens = (int)T;
+    const at::Device on(at::kCUDA, (c10::DeviceIndex)device);
+    const c10::cuda::OptionalCUDAGuard guard(c10::cuda::current_device() != device ? std::optional<at::Device>(on) : std::nullopt);
+    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
+    int st;
+    {
+        const WithoutGil released;
+        st = b200gptq_cache_write(&a, stream);
+    }
+    if (st != B200GPTQ_OK) return PyLong_FromLong(st);
+    for (int i : {2, 3, 4, 5, 11, 12, 13})
+        if (t[i]) wrote(*t[i]);
+    if (!t[11]) Py_RETURN_NONE;
+    Py_INCREF(args[11]);
+    return args[11];
+}
+
+// cache_read(cache.k, cache.v, cache.k_scales, cache.v_scales, lengths, k_out, v_out): (k, v), or a status code
+PyObject* read_checked(PyObject* const* args) {
+    const at::Tensor* t[7];
+    for (int i = 0; i < 7; ++i) t[i] = i < 4 ? &tensor_of(args[i], kReadNames[i]) : tensor_or_none(args[i], kReadNames[i]);
+    b200gptq_cache_read_args a = {};
+    const at::Tensor* const cache[4] = {t[0], t[1], t[2], t[3]};
+    cache_of(cache, kReadNames, false, a.cache);
+    const int device = t[0]->get_device();
+    const at::ScalarType type = t[2]->scalar_type();
+    const int64_t shape[4] = {a.cache.batch, a.cache.kv_heads, a.cache.max_seq, a.cache.hd};
+    a.lengths = whole_numbers(t[4], device, a.cache.batch, "lengths");
+    need((t[5] != nullptr) == (t[6] != nullptr), "k_out", "and v_out come together");
+    if (t[4] && !t[5]) refuse(PyExc_ValueError, "lengths needs k_out and v_out: the rows behind them keep what they hold");
+    for (int i : {5, 6}) {
+        if (!t[i]) continue;
+        need_type(*t[i], type, kReadNames[i]);
+        need_device(*t[i], device, kReadNames[i]);
+        need(t[i]->sizes() == at::IntArrayRef(shape), kReadNames[i], "must be [batch, kv_heads, max_seq, head_dim] of the cache's sizes");
+        need_rows(*t[i], kReadNames[i]);
+        bool apart = apart_from_itself(*t[i]);
+        for (int j = 0; j < 7; ++j) apart = apart && (j == i || !t[j] || !overlap(*t[i], *t[j]));
+        need(apart, kReadNames[i], "must not overlap another tensor, nor itself");
+    }
+    const at::Device on(at::kCUDA, (c10::DeviceIndex)device);
+    const c10::cuda::OptionalCUDAGuard guard(c10::cuda::current_device() != device ? std::optional<at::Device>(on) : std::nullopt);
+    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
+    at::Tensor out[2];
+    int st;
+    {
+        const WithoutGil released;
+        for (int i = 0; i < 2; ++i) out[i] = t[5 + i] ? *t[5 + i] : at::Tensor(at::detail::empty_cuda(at::IntArrayRef(shape), type, on, std::nullopt));
+        a.k_out = out[0].unsafeGetTensorImpl()->mutable_data();
+        a.v_out = out[1].unsafeGetTensorImpl()->mutable_data();
+        strides_of(out[0], a.k_out_stride, {0, 1, 2});
+        strides_of(out[1], a.v_out_stride, {0, 1, 2});
+        st = b200gptq_cache_read(&a, stream);
+    }
+    if (st != B200GPTQ_OK) return PyLong_FromLong(st);
+    PyObject* pair = PyTuple_New(2);
+    for (int i = 0; pair && i < 2; ++i) {
+        if (t[5 + i]) wrote(out[i]);
+        PyTuple_SET_ITEM(pair, i, THPVariable_Wrap(std::move(out[i])));
+    }
+    return pair;
+}
+
+template <int N>
+PyObject* raising(PyObject* (*call)(PyObject* const*), const char* const (&names)[N], PyObject* const* args, Py_ssize_t nargs) {
+    if (nargs != N) { PyErr_SetString(PyExc_TypeError, (std::to_string(N) + " arguments").c_str()); return nullptr; }
     try {
-        need_no_gradients(args, names);
+        need_no_gradients(args, names, N);
         return call(args);
     } catch (const Refusal& r) {
         PyErr_SetString(r.type, r.text.c_str());
@@ -680,10 +851,14 @@ PyObject* raising(PyObject* (*call)(PyObject* const*), const char* const* names,
 }
 PyObject* attn(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return raising(attn_checked, kAttnNames, args, nargs); }
 PyObject* adjust_logits(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return raising(logits_checked, kLogitNames, args, nargs); }
+PyObject* cache_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return raising(write_checked, kWriteNames, args, nargs); }
+PyObject* cache_read(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return raising(read_checked, kReadNames, args, nargs); }
 
 PyMethodDef module_methods[] = {
     {"attn", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attn)), METH_FASTCALL, nullptr},
     {"adjust_logits", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adjust_logits)), METH_FASTCALL, nullptr},
+    {"cache_write", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_write)), METH_FASTCALL, nullptr},
+    {"cache_read", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_read)), METH_FASTCALL, nullptr},
     {"pack", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(pack)), METH_FASTCALL, nullptr},
     {"set_scratch", set_scratch, METH_VARARGS, nullptr},
     {"set_scratch_source", set_scratch_source, METH_O, nullptr},

@@ -7,6 +7,7 @@ status.  Nothing here computes on the host.
 from __future__ import annotations
 
 import sys
+from dataclasses import dataclass
 from typing import Optional, Tuple
 
 import torch
@@ -494,6 +495,48 @@ def adjust_logits(logits, history=None, lengths=None, prompt_lens=None, repetiti
     throughout.  Evaluated in fp32, rounded once."""
     return _checked(_lib._host.adjust_logits(logits, history, lengths, prompt_lens, repetition, frequency, presence, bias_tokens,
                                              bias_values, mask, out), "b200gptq_adjust_logits")
+
+
+@dataclass
+class QuantCache:
+    """Keys and values in 4 bits: ``k`` / ``v`` uint8 ``[batch, kv_heads, max_seq, hd / 2]`` and, for each group of 32 or 64 dims of a row, a scale and a zero
+    ``k_scales`` / ``v_scales`` fp16 or bf16 ``[batch, kv_heads, max_seq, hd / group, 2]``.  A code c stands for ``zero + scale * c``; how the codes lie
+    in a row is said in ``include/b200gptq.h``.  Views are taken as long as rows begin at multiples of 16 bytes (constants: of a row's own size)."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scales: torch.Tensor
+    v_scales: torch.Tensor
+
+    @classmethod
+    def empty(cls, batch: int, kv_heads: int, max_seq: int, hd: int, group: int = 32, dtype=torch.float16, device="cuda") -> "QuantCache":
+        """A cache whose rows all stand for zeros."""
+        if hd not in (64, 128) or group not in (32, 64):
+            raise ValueError("a cache in 4 bits has heads of 64 or 128 dims and groups of 32 or 64")
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise TypeError("a cache in 4 bits stands for float16 or bfloat16")
+        codes = [torch.zeros(batch, kv_heads, max_seq, hd // 2, dtype=torch.uint8, device=device) for _ in range(2)]
+        return cls(*codes, *(torch.zeros(batch, kv_heads, max_seq, hd // group, 2, dtype=dtype, device=device) for _ in range(2)))
+
+    @property
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scales, self.v_scales))
+
+
+def cache_write(cache: QuantCache, k, v, pos, counts=None, cos=None, sin=None, q=None, q_out=None, k_out=None, v_out=None):
+    """New tokens into a cache in 4 bits, in one launch (``b200gptq_cache_write``): token t of sequence b at row ``pos[b] + t``.
+
+    ``k``, ``v`` ``[B, T, kv_heads, hd]`` in the type of the cache's constants; ``pos`` int64 ``[1]`` or ``[B]`` on the device, ``counts`` as for :func:`attn_window`.  With
+    ``cos`` / ``sin`` ``[positions, hd / 2]`` the keys, and the queries ``q`` ``[B, T, heads, hd]`` into ``q_out``, are rotated first (pairs of neighbours, row ``pos[b] + t``).
+    ``k_out`` / ``v_out`` ``[B, T, kv_heads, hd]`` get what the cache then stands for.  Padding, and tokens at positions outside the cache or
+    the angles, are left out everywhere.  A group of dims with a NaN or an infinity in it is NaN throughout.  Returns ``q_out``."""
+    return _checked(_lib._host.cache_write(k, v, cache.k, cache.v, cache.k_scales, cache.v_scales, pos, counts, cos, sin, q, q_out, k_out, v_out),
+                    "b200gptq_cache_write")
+
+
+def cache_read(cache: QuantCache, lengths=None, k_out=None, v_out=None):
+    """``(k, v)`` ``[B, kv_heads, max_seq, hd]``: what a cache in 4 bits stands for, each value rounded once (``b200gptq_cache_read``).  With ``lengths`` (int64
+    ``[B]``) the rows behind them are left as they were."""
+    return _checked(_lib._host.cache_read(cache.k, cache.v, cache.k_scales, cache.v_scales, lengths, k_out, v_out), "b200gptq_cache_read")
 
 
 def act(u, out, inter: int, gated: bool):

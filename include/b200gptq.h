@@ -466,6 +466,62 @@ B200GPTQ_API int64_t b200gptq_attn_workspace_bytes(const b200gptq_attn_args* arg
 B200GPTQ_API int b200gptq_attn(const b200gptq_attn_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * A KV cache held in 4 bits.  No counterpart in the reference, which leaves the cache to transformers
+ * (end2end/autogptq-generation-inference-benchmark.py:26-49).
+ *
+ * A row (one token, one key head, keys or values) is hd / 2 bytes of codes and, for each group of `group` dims, a scale and a zero in dtype:
+ *
+ *   value[d] = zero[d / group] + scale[d / group] * code[d],   code 0 .. 15
+ *
+ * b200gptq_cache_write derives them from the row x in dtype (rotated, where it is, and rounded):  zero = min x,  scale = (max x - min x) / 15 rounded to
+ * dtype,  code = (x - zero) / scale rounded to the nearest, ties to even, and held to 0 .. 15 (0 where scale is 0); all in fp32.  An x is off by half a scale at
+ * most, and 15 roundings of the scale at the upper end; where a value comes out in dtype it is held to dtype's largest number.  A group that holds a NaN or an infinity, or whose range passes fp32, is NaN throughout.
+ * The codes of a row lie as eight 4-bit fields in little-endian 32-bit words, field f at bits 4 f: word w = (hd / 64) i + h (i = 0 .. 7) holds the dims
+ * a + {0, 2, 32, 34, 1, 3, 33, 35}, a = 64 h + 4 i: operands of the tensor cores as they lie, for keys and for values.
+ *
+ *   dtype      B200GPTQ_F16 or B200GPTQ_BF16: of the constants and of all rows that go in and come out;  hd  64 or 128;  group  32 or 64
+ *   k, v       codes [batch, kv_heads, max_seq, hd / 2] bytes, strides {batch, head, row} in bytes, multiples of 16; 16-byte aligned
+ *   k_scales, v_scales  constants [batch, kv_heads, max_seq, hd / group, 2] (scale, zero), strides {batch, head, row} in elements, each row at a multiple of
+ *              its own size (2 hd / group elements); the last two dimensions are dense
+ */
+typedef struct {
+    void *k, *v, *k_scales, *v_scales;
+    int64_t k_stride[3], v_stride[3], k_scale_stride[3], v_scale_stride[3];
+    int dtype, batch, kv_heads, max_seq, hd, group;
+} b200gptq_cache4;
+
+/*
+ * New tokens into the cache: token t of sequence b at row pos[b] + t.
+ *   k, v       [batch, tokens, kv_heads, hd], strides {batch, token, head} in elements, multiples of 8, 16-byte aligned (so are q, q_out, k_out and v_out)
+ *   cos_t, sin_t  [angles, hd / 2] dense in dtype, or NULL: keys (and q) are rotated by row pos[b] + t, pairs of neighbours
+ *              (x0 cos - x1 sin, x0 sin + x1 cos), in fp32, rounded once
+ *   q, q_out   [batch, tokens, heads, hd], both or neither (and only with cos_t): the queries, rotated
+ *   k_out, v_out  what the cache now stands for, in dtype (rounded once), [batch, tokens, kv_heads, hd] each, or NULL
+ *   pos        device int64 [batch], or one for all (pos_each 0);  counts  device int64 [batch] or NULL: tokens t >= counts[b] are padding
+ * Padding, and tokens whose position is outside the cache or the angles, are left out: nothing is written for them anywhere.  No output overlaps
+ * anything that is read.
+ */
+typedef struct {
+    b200gptq_cache4 cache;
+    const void *k, *v, *q, *cos_t, *sin_t;
+    void *q_out, *k_out, *v_out;
+    const int64_t *pos, *counts;
+    int64_t k_stride[3], v_stride[3], q_stride[3], q_out_stride[3], k_out_stride[3], v_out_stride[3];
+    int tokens, heads, angles, pos_each;
+} b200gptq_cache_write_args;
+B200GPTQ_API int b200gptq_cache_write(const b200gptq_cache_write_args* args, void* stream);
+
+/* The cache back in dtype, each value rounded once: rows 0 .. lengths[b] - 1 (device int64 [batch]; NULL: all; held to 0 .. max_seq) into k_out, v_out
+ * [batch, kv_heads, max_seq, hd], strides {batch, head, row} in elements, multiples of 8, 16-byte aligned.  Rows behind them are left as they were. */
+typedef struct {
+    b200gptq_cache4 cache;
+    void *k_out, *v_out;
+    const int64_t* lengths;
+    int64_t k_out_stride[3], v_out_stride[3];
+} b200gptq_cache_read_args;
+B200GPTQ_API int b200gptq_cache_read(const b200gptq_cache_read_args* args, void* stream);
+
+/*
  * Rules on the logits of the next token, before the pick (the reference leaves them to transformers' generate()).  Per row, for token v with logit x:
  *   1. v among history[0 .. length):              x = x > 0 ? x / repetition : x * repetition
  *   2. v n times (n > 0) in history[prompt_len .. length):   x = x - frequency * n - presence
