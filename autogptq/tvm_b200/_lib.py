@@ -67,6 +67,8 @@ _SIGNATURES = {
     "b200gptq_adjust_logits": (_c_int, [_c_void_p, _c_void_p]),
     "b200gptq_cache_write": (_c_int, [_c_void_p, _c_void_p]),
     "b200gptq_cache_read": (_c_int, [_c_void_p, _c_void_p]),
+    "b200gptq_attn_cache_workspace_bytes": (ctypes.c_int64, [_c_void_p]),
+    "b200gptq_attn_cache": (_c_int, [_c_void_p, _c_void_p, _c_size_t, _c_void_p]),
     "b200gptq_step_plan_bytes": (_c_size_t, [_c_void_p]),
     "b200gptq_step_table_bytes": (_c_size_t, [_c_int]),
     "b200gptq_step_plan_create": (_c_int, [_c_void_p] * 4),
@@ -120,6 +122,12 @@ class CacheWriteArgs(ctypes.Structure):
 class CacheReadArgs(ctypes.Structure):
     _fields_ = ([("cache", Cache4)] + [(n, _c_void_p) for n in ("k_out", "v_out", "lengths")]
                 + [(n, ctypes.c_int64 * 3) for n in ("k_out_stride", "v_out_stride")])
+
+
+class AttnCacheArgs(ctypes.Structure):
+    _fields_ = ([("cache", Cache4)] + [(n, _c_void_p) for n in ("q", "out", "pos", "counts", "status")]
+                + [(n, ctypes.c_int64 * 3) for n in ("q_stride", "out_stride")]
+                + [(n, _c_int) for n in ("tokens", "heads", "window", "sinks", "pos_each")] + [("scale", ctypes.c_float)])
 
 
 def _load() -> ctypes.CDLL:

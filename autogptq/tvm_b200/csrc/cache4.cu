@@ -7,7 +7,7 @@
 // Bound by the bytes of long prompts and by the launch for a decode step.
 #include <algorithm>
 
-#include "attn.h"
+#include "attn4.h"
 #include "cache4.cuh"
 
 namespace b200gptq {
@@ -125,24 +125,10 @@ cache_write_kernel(const __grid_constant__ b200gptq_cache_write_args a, unsigned
     }
 }
 
-// A CTA takes ROWS rows of the keys or the values of one sequence and head.
-template <typename T, int HD, int GS>
-__global__ void __launch_bounds__(kThreads)
-cache_read_kernel(const __grid_constant__ b200gptq_cache_read_args a, unsigned chunks, const Divisor by_chunks, const Divisor by_heads) {
-    constexpr int LANES = HD / 8, NG = HD / GS, ROWS = kThreads / LANES;
-    asm volatile("griddepcontrol.launch_dependents;");
-    const b200gptq_cache4& c = a.cache;
-    const unsigned which = over(blockIdx.x, by_chunks), pair = which >> 1, b = over(pair, by_heads);
-    const int head = (int)(pair - b * c.kv_heads), u = threadIdx.x % LANES, g = u & 7, h = u >> 3;
-    const bool is_k = !(which & 1);
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const long long length = a.lengths ? min(__ldcg(reinterpret_cast<const long long*>(a.lengths) + b), (long long)c.max_seq) : c.max_seq;
-    const int j = (int)((blockIdx.x - which * chunks) * ROWS + threadIdx.x / LANES);
-    if (j >= length) return;
-    const uint8_t* codes = static_cast<const uint8_t*>(is_k ? c.k : c.v) + (is_k ? b * c.k_stride[0] + head * c.k_stride[1] + j * c.k_stride[2]
-                                                                                 : b * c.v_stride[0] + head * c.v_stride[1] + j * c.v_stride[2]);
-    const T* constants = static_cast<const T*>(is_k ? c.k_scales : c.v_scales) + (is_k ? b * c.k_scale_stride[0] + head * c.k_scale_stride[1] + j * c.k_scale_stride[2]
-                                                                                       : b * c.v_scale_stride[0] + head * c.v_scale_stride[1] + j * c.v_scale_stride[2]);
+// A row back in 16 bits, HD / 8 lanes (of which this is number u) a row.
+template <typename T, int HD, int GS> __device__ __forceinline__ void read_row(const uint8_t* codes, const T* constants, T* out, int u) {
+    constexpr int NG = HD / GS;
+    const int g = u & 7, h = u >> 3;
     const uint32_t w = __ldcg(reinterpret_cast<const unsigned*>(codes) + (HD / 64) * g + h);
     float2 of[2];                                 // (scale, zero) of the two runs of dims
     of[0] = Half<T>::unpack(__ldcg(reinterpret_cast<const unsigned*>(constants) + h * NG / (HD / 64)));
@@ -152,10 +138,55 @@ cache_read_kernel(const __grid_constant__ b200gptq_cache_read_args a, unsigned c
     float x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = value_of<T>(code[e], of[e / 4].x, of[e / 4].y);
-    T* out = static_cast<T*>(is_k ? a.k_out : a.v_out) + (is_k ? b * a.k_out_stride[0] + head * a.k_out_stride[1] + j * a.k_out_stride[2]
-                                                               : b * a.v_out_stride[0] + head * a.v_out_stride[1] + j * a.v_out_stride[2]) + 64 * h + 4 * g;
+    out += 64 * h + 4 * g;
     *reinterpret_cast<uint2*>(out) = pack4<T>(x);
     *reinterpret_cast<uint2*>(out + 32) = pack4<T>(x + 4);
+}
+
+// A CTA takes ROWS rows of the keys or the values of one sequence and head.
+template <typename T, int HD, int GS>
+__global__ void __launch_bounds__(kThreads)
+cache_read_kernel(const __grid_constant__ b200gptq_cache_read_args a, unsigned chunks, const __grid_constant__ Divisor by_chunks, const __grid_constant__ Divisor by_heads) {
+    constexpr int LANES = HD / 8, ROWS = kThreads / LANES;
+    asm volatile("griddepcontrol.launch_dependents;");
+    const b200gptq_cache4& c = a.cache;
+    const unsigned which = over(blockIdx.x, by_chunks), pair = which >> 1, b = over(pair, by_heads);
+    const int head = (int)(pair - b * c.kv_heads);
+    const bool is_k = !(which & 1);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const long long length = a.lengths ? min(__ldcg(reinterpret_cast<const long long*>(a.lengths) + b), (long long)c.max_seq) : c.max_seq;
+    const int j = (int)((blockIdx.x - which * chunks) * ROWS + threadIdx.x / LANES);
+    if (j >= length) return;
+    const uint8_t* codes = static_cast<const uint8_t*>(is_k ? c.k : c.v) + (is_k ? b * c.k_stride[0] + head * c.k_stride[1] + j * c.k_stride[2]
+                                                                                 : b * c.v_stride[0] + head * c.v_stride[1] + j * c.v_stride[2]);
+    const T* constants = static_cast<const T*>(is_k ? c.k_scales : c.v_scales) + (is_k ? b * c.k_scale_stride[0] + head * c.k_scale_stride[1] + j * c.k_scale_stride[2]
+                                                                                       : b * c.v_scale_stride[0] + head * c.v_scale_stride[1] + j * c.v_scale_stride[2]);
+    T* out = static_cast<T*>(is_k ? a.k_out : a.v_out) + (is_k ? b * a.k_out_stride[0] + head * a.k_out_stride[1] + j * a.k_out_stride[2]
+                                                               : b * a.v_out_stride[0] + head * a.v_out_stride[1] + j * a.v_out_stride[2]);
+    read_row<T, HD, GS>(codes, constants, out, threadIdx.x % LANES);
+}
+
+// For prompts: the rows that the tokens see between them, into dense k and v [batch, kv_heads, max_seq, hd].
+template <typename T, int HD, int GS>
+__global__ void __launch_bounds__(kThreads)
+cache_read_seen_kernel(const __grid_constant__ Attn4Args a, T* __restrict__ k, T* __restrict__ v, unsigned chunks, const __grid_constant__ Divisor by_chunks,
+                       const __grid_constant__ Divisor by_heads) {
+    constexpr int LANES = HD / 8, ROWS = kThreads / LANES;
+    asm volatile("griddepcontrol.launch_dependents;");
+    const b200gptq_cache4& c = a.cache;
+    const unsigned which = over(blockIdx.x, by_chunks), pair = which >> 1, b = over(pair, by_heads);
+    const int head = (int)(pair - b * c.kv_heads);
+    const bool is_k = !(which & 1);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int j = (int)((blockIdx.x - which * chunks) * ROWS + threadIdx.x / LANES);
+    const int p0 = attn_pos(a.attn, b), count = attn_count(a.attn, b);
+    const AttnRange r = attn_range(p0, p0 + count - 1, a.attn.window ? a.attn.window : 1 << 30, a.attn.sinks, c.max_seq);
+    if (!count || j >= r.w_end || (j >= r.s_end && j < r.w_start) || j >= c.max_seq) return;
+    const uint8_t* codes = static_cast<const uint8_t*>(is_k ? c.k : c.v) + (is_k ? b * c.k_stride[0] + head * c.k_stride[1] + j * c.k_stride[2]
+                                                                                 : b * c.v_stride[0] + head * c.v_stride[1] + j * c.v_stride[2]);
+    const T* constants = static_cast<const T*>(is_k ? c.k_scales : c.v_scales) + (is_k ? b * c.k_scale_stride[0] + head * c.k_scale_stride[1] + j * c.k_scale_stride[2]
+                                                                                       : b * c.v_scale_stride[0] + head * c.v_scale_stride[1] + j * c.v_scale_stride[2]);
+    read_row<T, HD, GS>(codes, constants, (is_k ? k : v) + ((long long)pair * c.max_seq + j) * HD, threadIdx.x % LANES);
 }
 
 template <typename... KArgs, typename... Args>
@@ -188,6 +219,15 @@ int read(const b200gptq_cache_read_args& a, cudaStream_t stream) {
     return launch(cache_read_kernel<T, HD, GS>, dim3((unsigned)(ctas * chunks)), stream, a, (unsigned)chunks, Divisor(chunks), Divisor(a.cache.kv_heads));
 }
 
+template <typename T, int HD, int GS>
+int read_seen(const Attn4Args& a, void* k, void* v, cudaStream_t stream) {
+    constexpr int ROWS = kThreads / (HD / 8);
+    const long long chunks = (a.cache.max_seq + ROWS - 1) / ROWS, ctas = 2LL * a.cache.batch * a.cache.kv_heads;
+    if (ctas > 0x7fffffff / chunks) return B200GPTQ_ERR_TOO_LARGE;
+    return launch(cache_read_seen_kernel<T, HD, GS>, dim3((unsigned)(ctas * chunks)), stream, a, static_cast<T*>(k), static_cast<T*>(v), (unsigned)chunks, Divisor(chunks),
+                  Divisor(a.cache.kv_heads));
+}
+
 template <typename T, typename Args> int by_shape(const Args& a, cudaStream_t stream, int (*const (&run)[2][2])(const Args&, cudaStream_t)) {
     return run[a.cache.hd == 128][a.cache.group == 64](a, stream);
 }
@@ -195,6 +235,14 @@ template <typename T, typename Args> int by_shape(const Args& a, cudaStream_t st
 uintptr_t bits_of(const void* p, const int64_t (&stride)[3]) { return p ? reinterpret_cast<uintptr_t>(p) | (uintptr_t)(2 * (stride[0] | stride[1] | stride[2])) : 0; }
 
 }  // namespace
+
+int attn4_read_back(const Attn4Args& a, void* k, void* v, cudaStream_t s) {
+    using F = int (*)(const Attn4Args&, void*, void*, cudaStream_t);
+    static const F run[2][2][2] = {{{read_seen<__half, 64, 32>, read_seen<__half, 64, 64>}, {read_seen<__half, 128, 32>, read_seen<__half, 128, 64>}},
+                                   {{read_seen<__nv_bfloat16, 64, 32>, read_seen<__nv_bfloat16, 64, 64>}, {read_seen<__nv_bfloat16, 128, 32>, read_seen<__nv_bfloat16, 128, 64>}}};
+    return run[a.cache.dtype == B200GPTQ_BF16][a.cache.hd == 128][a.cache.group == 64](a, k, v, s);
+}
+
 }  // namespace b200gptq
 
 using namespace b200gptq;

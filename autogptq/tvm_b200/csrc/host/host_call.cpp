@@ -421,6 +421,7 @@ void need_device(const at::Tensor& t, int device, const char* name) {
 constexpr int kArguments = 11;
 constexpr const char* kWriteNames[] = {"k", "v", "cache.k", "cache.v", "cache.k_scales", "cache.v_scales", "pos", "counts", "cos", "sin", "q", "q_out", "k_out", "v_out"};
 constexpr const char* kReadNames[] = {"cache.k", "cache.v", "cache.k_scales", "cache.v_scales", "lengths", "k_out", "v_out"};
+constexpr const char* kAttnCacheNames[] = {"q", "cache.k", "cache.v", "cache.k_scales", "cache.v_scales", "pos", "window", "sinks", "counts", "scale", "out"};
 constexpr const char* kAttnNames[kArguments] = {"q", "k_prefix", "v_prefix", "k_cache", "v_cache", "pos", "window", "sinks", "counts", "scale", "out"};
 constexpr const char* kLogitNames[kArguments] = {"logits", "history", "lengths", "prompt_lens", "repetition", "frequency", "presence", "bias_tokens", "bias_values", "mask", "out"};
 // No argument asks for a derivative, backward or (a dual number, which knows no no_grad) forward: penalties and biases could as well as the logits.
@@ -833,6 +834,71 @@ PyObject* read_checked(PyObject* const* args) {
     return pair;
 }
 
+// attn_cache(q, cache.k, cache.v, cache.k_scales, cache.v_scales, pos, window, sinks, counts, scale, out): the output, or a status code
+PyObject* attn_cache_checked(PyObject* const* args) {
+    const at::Tensor &q = tensor_of(args[0], "q"), &pos = tensor_of(args[5], "pos");
+    const at::Tensor* cache[4];
+    for (int i = 0; i < 4; ++i) cache[i] = &tensor_of(args[1 + i], kAttnCacheNames[1 + i]);
+    const at::Tensor *counts = tensor_or_none(args[8], "counts"), *given = tensor_or_none(args[10], "out");
+    b200gptq_attn_cache_args a = {};
+    cache_of(cache, kAttnCacheNames + 1, false, a.cache);
+    const int device = cache[0]->get_device();
+    const at::ScalarType type = cache[2]->scalar_type();
+    const int64_t B = a.cache.batch, KV = a.cache.kv_heads;
+    need_type(q, type, "q");
+    need_device(q, device, "q");
+    need(q.dim() == 4 && q.numel() > 0 && q.size(0) == B && q.size(3) == a.cache.hd && q.size(2) % KV == 0, "q", "must be [batch, tokens, heads, head_dim] of the cache's sizes, heads a multiple of its heads");
+    const int64_t T = q.size(1), H = q.size(2);
+    need(B * T <= (1 << 29) && H <= (1 << 29) && B * T * (H / KV) <= (1 << 29), "q", "is too large");
+    need_rows(q, "q");
+    positions_of(pos, device, B, &a.pos, &a.pos_each);
+    a.counts = whole_numbers(counts, device, B, "counts");
+    a.tokens = (int)T; a.heads = (int)H;
+    a.q = data_of(q);
+    strides_of(q, a.q_stride, {0, 1, 2});
+    a.sinks = int_of(args[7], "sinks");
+    if (args[6] != Py_None) {
+        a.window = int_of(args[6], "window");
+        need(a.window >= 1, "window", "must be at least 1");
+    }
+    need(a.window || !a.sinks, "sinks", "go with a window");
+    if (args[9] == Py_None) {
+        a.scale = (float)(1.0 / std::sqrt((double)a.cache.hd));
+    } else {
+        a.scale = (float)PyFloat_AsDouble(args[9]);
+        if (PyErr_Occurred()) { PyErr_Clear(); refuse(PyExc_TypeError, "scale must be a number"); }
+    }
+    if (given) {
+        need_type(*given, type, "out");
+        need_device(*given, device, "out");
+        need(given->sizes() == q.sizes(), "out", "must have the shape of q");
+        need_rows(*given, "out");
+        bool apart = !overlap(*given, q) && !overlap(*given, pos) && !(counts && overlap(*given, *counts));
+        for (const at::Tensor* t : cache) apart = apart && !overlap(*given, *t);
+        need(apart && apart_from_itself(*given), "out", "must not overlap what is read, nor itself");
+    }
+    if (counts && !given) refuse(PyExc_ValueError, "counts needs out: the rows of padding keep what it holds");
+    const at::Device on(at::kCUDA, (c10::DeviceIndex)device);
+    const c10::cuda::OptionalCUDAGuard guard(c10::cuda::current_device() != device ? std::optional<at::Device>(on) : std::nullopt);
+    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
+    Scratch ws;                 // (for its status word: what a wait that runs out raises)
+    if (!scratch_for(device, stream, B200GPTQ_STATUS_BYTES, &ws)) return nullptr;
+    const Held owner(ws.owner);
+    a.status = reinterpret_cast<unsigned int*>(static_cast<char*>(ws.ptr) + B200GPTQ_STATUS_BYTES) - 1;
+    at::Tensor out, scratch;
+    int st;
+    {
+        const WithoutGil released;
+        out = given ? *given : at::Tensor(at::detail::empty_cuda(q.sizes(), type, on, std::nullopt));
+        a.out = out.unsafeGetTensorImpl()->mutable_data();
+        strides_of(out, a.out_stride, {0, 1, 2});
+        const int64_t bytes = b200gptq_attn_cache_workspace_bytes(&a);
+        if (bytes > 0) scratch = at::detail::empty_cuda({bytes}, at::kByte, on, std::nullopt);
+        st = bytes < 0 ? (int)bytes : b200gptq_attn_cache(&a, bytes > 0 ? scratch.unsafeGetTensorImpl()->mutable_data() : nullptr, (size_t)bytes, stream);
+    }
+    return answer(std::move(out), given != nullptr, st);
+}
+
 template <int N>
 PyObject* raising(PyObject* (*call)(PyObject* const*), const char* const (&names)[N], PyObject* const* args, Py_ssize_t nargs) {
     if (nargs != N) { PyErr_SetString(PyExc_TypeError, (std::to_string(N) + " arguments").c_str()); return nullptr; }
@@ -852,12 +918,14 @@ PyObject* raising(PyObject* (*call)(PyObject* const*), const char* const (&names
 PyObject* attn(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return raising(attn_checked, kAttnNames, args, nargs); }
 PyObject* adjust_logits(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return raising(logits_checked, kLogitNames, args, nargs); }
 PyObject* cache_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return raising(write_checked, kWriteNames, args, nargs); }
+PyObject* attn_cache(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return raising(attn_cache_checked, kAttnCacheNames, args, nargs); }
 PyObject* cache_read(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return raising(read_checked, kReadNames, args, nargs); }
 
 PyMethodDef module_methods[] = {
     {"attn", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attn)), METH_FASTCALL, nullptr},
     {"adjust_logits", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adjust_logits)), METH_FASTCALL, nullptr},
     {"cache_write", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_write)), METH_FASTCALL, nullptr},
+    {"attn_cache", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attn_cache)), METH_FASTCALL, nullptr},
     {"cache_read", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_read)), METH_FASTCALL, nullptr},
     {"pack", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(pack)), METH_FASTCALL, nullptr},
     {"set_scratch", set_scratch, METH_VARARGS, nullptr},

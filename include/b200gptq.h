@@ -522,6 +522,27 @@ typedef struct {
 B200GPTQ_API int b200gptq_cache_read(const b200gptq_cache_read_args* args, void* stream);
 
 /*
+ * Attention of new tokens over a cache held in 4 bits: b200gptq_attn's, of a query at position p = pos[b] + t, over the values that the cache stands for.
+ *   window 0: a token sees rows 0 .. p, else the last `window` of them and the first `sinks`; without a window there are no sinks
+ * Everything else (counts, strides, what is not seen, rows that see nothing) is as there.  Statistics and sums are fp32; weights times scales are rounded to fp16 before
+ * they multiply codes.  64 rows of a key head (tokens * heads / kv_heads) or more: the rows that are seen are read back into scratch, each value rounded to dtype, and
+ * multiplied as b200gptq_attn does.
+ * b200gptq_attn_cache_workspace_bytes: scratch of a call, 16-byte aligned, contents on entry do not matter, not shared by calls that may overlap.
+ */
+typedef struct {
+    b200gptq_cache4 cache;
+    const void* q;
+    void* out;
+    const int64_t *pos, *counts;
+    unsigned int* status;
+    int64_t q_stride[3], out_stride[3];
+    int tokens, heads, window, sinks, pos_each;
+    float scale;
+} b200gptq_attn_cache_args;
+B200GPTQ_API int64_t b200gptq_attn_cache_workspace_bytes(const b200gptq_attn_cache_args* args);
+B200GPTQ_API int b200gptq_attn_cache(const b200gptq_attn_cache_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Rules on the logits of the next token, before the pick (the reference leaves them to transformers' generate()).  Per row, for token v with logit x:
  *   1. v among history[0 .. length):              x = x > 0 ? x / repetition : x * repetition
  *   2. v n times (n > 0) in history[prompt_len .. length):   x = x - frequency * n - presence
