@@ -67,6 +67,7 @@ _SIGNATURES = {
     "b200gptq_adjust_logits": (_c_int, [_c_void_p, _c_void_p]),
     "b200gptq_cache_write": (_c_int, [_c_void_p, _c_void_p]),
     "b200gptq_cache_read": (_c_int, [_c_void_p, _c_void_p]),
+    "b200gptq_sample": (_c_int, [_c_void_p, _c_void_p]),
     "b200gptq_attn_cache_workspace_bytes": (ctypes.c_int64, [_c_void_p]),
     "b200gptq_attn_cache": (_c_int, [_c_void_p, _c_void_p, _c_size_t, _c_void_p]),
     "b200gptq_step_plan_bytes": (_c_size_t, [_c_void_p]),
@@ -128,6 +129,11 @@ class AttnCacheArgs(ctypes.Structure):
     _fields_ = ([("cache", Cache4)] + [(n, _c_void_p) for n in ("q", "out", "pos", "counts", "status")]
                 + [(n, ctypes.c_int64 * 3) for n in ("q_stride", "out_stride")]
                 + [(n, _c_int) for n in ("tokens", "heads", "window", "sinks", "pos_each")] + [("scale", ctypes.c_float)])
+
+
+class SampleArgs(ctypes.Structure):
+    _fields_ = ([(n, _c_void_p) for n in ("logits", "uniform", "temperature", "top_p", "min_p", "top_k", "out")]
+                + [("logits_stride", ctypes.c_int64)] + [(n, _c_int) for n in ("dtype", "rows", "vocab")])
 
 
 def _load() -> ctypes.CDLL:

@@ -422,6 +422,7 @@ constexpr int kArguments = 11;
 constexpr const char* kWriteNames[] = {"k", "v", "cache.k", "cache.v", "cache.k_scales", "cache.v_scales", "pos", "counts", "cos", "sin", "q", "q_out", "k_out", "v_out"};
 constexpr const char* kReadNames[] = {"cache.k", "cache.v", "cache.k_scales", "cache.v_scales", "lengths", "k_out", "v_out"};
 constexpr const char* kAttnCacheNames[] = {"q", "cache.k", "cache.v", "cache.k_scales", "cache.v_scales", "pos", "window", "sinks", "counts", "scale", "out"};
+constexpr const char* kSampleNames[] = {"logits", "uniform", "temperature", "top_k", "top_p", "min_p", "out"};
 constexpr const char* kAttnNames[kArguments] = {"q", "k_prefix", "v_prefix", "k_cache", "v_cache", "pos", "window", "sinks", "counts", "scale", "out"};
 constexpr const char* kLogitNames[kArguments] = {"logits", "history", "lengths", "prompt_lens", "repetition", "frequency", "presence", "bias_tokens", "bias_values", "mask", "out"};
 // No argument asks for a derivative, backward or (a dual number, which knows no no_grad) forward: penalties and biases could as well as the logits.
@@ -899,6 +900,53 @@ PyObject* attn_cache_checked(PyObject* const* args) {
     return answer(std::move(out), given != nullptr, st);
 }
 
+// sample(logits, uniform, temperature, top_k, top_p, min_p, out): the tokens, or a status code
+PyObject* sample_checked(PyObject* const* args) {
+    const at::Tensor& x = tensor_of(args[0], "logits");
+    const at::Tensor* t[7] = {&x, &tensor_of(args[1], "uniform")};
+    const int device = x.get_device();
+    for (int i = 1; i < 7; ++i) {
+        if (i > 1) t[i] = tensor_or_none(args[i], kSampleNames[i]);
+        if (t[i]) need_device(*t[i], device, kSampleNames[i]);
+    }
+    b200gptq_sample_args a = {};
+    const at::ScalarType type = x.scalar_type();
+    if (type != at::kHalf && type != at::kBFloat16 && type != at::kFloat) refuse(PyExc_TypeError, "logits must be float16, bfloat16 or float32");
+    a.dtype = type == at::kHalf ? B200GPTQ_F16 : type == at::kBFloat16 ? B200GPTQ_BF16 : B200GPTQ_F32;
+    need(x.dim() == 2 && x.numel() > 0 && (x.size(1) == 1 || x.stride(1) == 1), "logits", "must be [rows, vocab], dense in its last dimension");
+    need(x.size(1) <= (1 << 18) && x.size(0) <= (1 << 27), "logits", "is too large: 2^18 tokens at most");
+    const int64_t R = x.size(0);
+    a.rows = (int)R; a.vocab = (int)x.size(1);
+    a.logits = data_of(x);
+    a.logits_stride = R == 1 ? 0 : x.stride(0);
+    const float** numbers[7] = {nullptr, &a.uniform, &a.temperature, nullptr, &a.top_p, &a.min_p, nullptr};
+    for (int i : {1, 2, 4, 5})
+        if (t[i]) {
+            need_type(*t[i], at::kFloat, kSampleNames[i]);
+            need(t[i]->dim() == 1 && t[i]->size(0) == R && (R == 1 || t[i]->stride(0) == 1), kSampleNames[i], "must be float32, dense, one number for each row");
+            *numbers[i] = static_cast<const float*>(data_of(*t[i]));
+        }
+    for (int i : {3, 6})
+        if (t[i]) {
+            need_type(*t[i], at::kLong, kSampleNames[i]);
+            need(t[i]->dim() == 1 && t[i]->size(0) == R && (R == 1 || t[i]->stride(0) == 1), kSampleNames[i], "must be int64, dense, one number for each row");
+        }
+    if (t[3]) a.top_k = static_cast<const int64_t*>(data_of(*t[3]));
+    for (int i = 0; i < 6 && t[6]; ++i) need(!t[i] || !overlap(*t[6], *t[i]), "out", "must overlap nothing that is read");
+    const at::Device on(at::kCUDA, (c10::DeviceIndex)device);
+    const c10::cuda::OptionalCUDAGuard guard(c10::cuda::current_device() != device ? std::optional<at::Device>(on) : std::nullopt);
+    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
+    at::Tensor out;
+    int st;
+    {
+        const WithoutGil released;
+        out = t[6] ? *t[6] : at::Tensor(at::detail::empty_cuda({R}, at::kLong, on, std::nullopt));
+        a.out = static_cast<int64_t*>(out.unsafeGetTensorImpl()->mutable_data());
+        st = b200gptq_sample(&a, stream);
+    }
+    return answer(std::move(out), t[6] != nullptr, st);
+}
+
 template <int N>
 PyObject* raising(PyObject* (*call)(PyObject* const*), const char* const (&names)[N], PyObject* const* args, Py_ssize_t nargs) {
     if (nargs != N) { PyErr_SetString(PyExc_TypeError, (std::to_string(N) + " arguments").c_str()); return nullptr; }
@@ -919,6 +967,7 @@ PyObject* attn(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return rais
 PyObject* adjust_logits(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return raising(logits_checked, kLogitNames, args, nargs); }
 PyObject* cache_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return raising(write_checked, kWriteNames, args, nargs); }
 PyObject* attn_cache(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return raising(attn_cache_checked, kAttnCacheNames, args, nargs); }
+PyObject* sample(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return raising(sample_checked, kSampleNames, args, nargs); }
 PyObject* cache_read(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return raising(read_checked, kReadNames, args, nargs); }
 
 PyMethodDef module_methods[] = {
@@ -926,6 +975,7 @@ PyMethodDef module_methods[] = {
     {"adjust_logits", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adjust_logits)), METH_FASTCALL, nullptr},
     {"cache_write", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_write)), METH_FASTCALL, nullptr},
     {"attn_cache", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attn_cache)), METH_FASTCALL, nullptr},
+    {"sample", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(sample)), METH_FASTCALL, nullptr},
     {"cache_read", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_read)), METH_FASTCALL, nullptr},
     {"pack", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(pack)), METH_FASTCALL, nullptr},
     {"set_scratch", set_scratch, METH_VARARGS, nullptr},

@@ -545,6 +545,17 @@ def attn_cache(q, cache: QuantCache, pos, window: Optional[int] = None, sinks: i
     return _checked(_lib._host.attn_cache(q, cache.k, cache.v, cache.k_scales, cache.v_scales, pos, window, sinks, counts, scale, out), "b200gptq_attn_cache")
 
 
+def sample(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None, out=None):
+    """The next token of each row of ``logits`` ``[rows, vocab]`` (fp16, bf16 or fp32, up to 2^18 tokens) from a given random number, in one launch
+    (``b200gptq_sample``).  Per row, with weights ``exp((x - max x) / temperature)``, kept are the ``top_k`` largest logits (0: all), of these the fewest whose
+    weights make up ``top_p`` of theirs (1: all), and of these the ones of weight ``min_p`` at least (the largest weight is 1); equal logits count from the lowest token on.  The
+    token is the lowest for which the kept weights up to it pass ``uniform`` times all of them.  Temperature 0: the lowest token of the largest logit.
+
+    ``uniform``, ``temperature``, ``top_p``, ``min_p`` fp32 ``[rows]``, ``top_k`` int64 ``[rows]``, all on the device.  The borders are exact: weights are integers in units
+    of 2^-45 of the largest or less, whose sums have no rounding.  A NaN counts as minus infinity.  Returns int64 ``[rows]``."""
+    return _checked(_lib._host.sample(logits, uniform, temperature, top_k, top_p, min_p, out), "b200gptq_sample")
+
+
 def act(u, out, inter: int, gated: bool):
     with torch.cuda.device(u.device):
         st = _lib.lib.b200gptq_act(_ptr(u), _ptr(out), u.shape[0], inter, 1 if gated else 0, _stream(u.device))

@@ -568,6 +568,31 @@ typedef struct {
 B200GPTQ_API int b200gptq_adjust_logits(const b200gptq_logit_args* args, void* stream);
 
 /*
+ * The next token of each row from a given random number (the reference leaves it to transformers' generate()).  With M the row's largest logit and
+ * weights w_v = exp((x_v - M) / temperature), tokens are ordered by x, larger first, and equal ones by v, lower first; kept are those that are
+ *   among the first top_k (0 or less: all of them),  and
+ *   in the shortest beginning of these whose weights add up to top_p of all of these (1 or more: all of them; the first one always),  and
+ *   of weight min_p at least, the largest weight being 1 (the first one always).
+ * The token is the lowest v for which the kept weights of tokens 0 .. v add up to more than uniform times all kept weights (uniform below 0 counts as 0, 1 or more
+ * as the largest number below 1).  A temperature of 0 (or anything that is not 1e-18 at least), and top_k 1, give the lowest token of the largest logit.
+ * Weights are integers in units of 2^-F, F = min(49, 62 - ceil(log2 vocab)), and everything that follows from them is exact, whatever the order; so a weight below
+ * 2^-(F + 1) is zero.  A NaN counts as minus infinity; where the largest logit is plus infinity, the tokens that have it share all the weight; a row without any
+ * number gives the lowest token of the largest logit, or 0.
+ *   dtype      B200GPTQ_F16, _BF16 or _F32, of logits [rows, vocab] with a row stride (elements);  vocab up to 2^18
+ *   uniform    device fp32 [rows];  temperature, top_p, min_p  device fp32 [rows], each NULL for 1, 1, 0;  top_k  device int64 [rows] or NULL for 0
+ *   out        device int64 [rows]
+ */
+typedef struct {
+    const void* logits;
+    const float *uniform, *temperature, *top_p, *min_p;
+    const int64_t* top_k;
+    int64_t* out;
+    int64_t logits_stride;
+    int dtype, rows, vocab;
+} b200gptq_sample_args;
+B200GPTQ_API int b200gptq_sample(const b200gptq_sample_args* args, void* stream);
+
+/*
  * The decoder layers of one decode step of one sequence as ONE cooperative launch: per layer norm, q|k|v, rotary embedding +
  * cache write + attention, output projection, residual sum, norm, first FFN linear, activation, second FFN linear, residual sum: the
  * arithmetic of the helpers above and of b200gptq_gemv.  The reference has no counterpart (its loop is transformers' generate(),

@@ -63,3 +63,33 @@ def test_a_cache_and_its_size():
         ops.cache_read(c)
     with pytest.raises(RuntimeError):
         ops.cache_write(c, torch.zeros(2, 1, 3, 128, dtype=torch.bfloat16), torch.zeros(2, 1, 3, 128, dtype=torch.bfloat16), torch.zeros(1, dtype=torch.long))
+
+
+def test_attention_refuses():
+    good = dict(q=A, out=A, pos=A, tokens=1, heads=4, window=8, scale=1.0)
+
+    def call(change, cache=None, need=None):
+        a = _lib.AttnCacheArgs(cache=cache4(**(cache or {})), **{**good, **{k: v for k, v in change.items() if "stride" not in k}})
+        for n in ("q_stride", "out_stride"):
+            setattr(a, n, (ctypes.c_int64 * 3)(*change.get(n, (256, 256, 64))))
+        return _lib.lib.b200gptq_attn_cache(ctypes.byref(a), None, 0, None), _lib.lib.b200gptq_attn_cache_workspace_bytes(ctypes.byref(a))
+
+    for change, status in [(dict(q=None), -1), (dict(out=None), -1), (dict(pos=None), -1), (dict(tokens=0), -3), (dict(heads=3), -3), (dict(heads=0), -3), (dict(window=-1), -3),
+                           (dict(sinks=-1), -3), (dict(window=0, sinks=2), -3), (dict(tokens=1 << 29), -8), (dict(window=(1 << 29) + 1), -8), (dict(q=A + 8), -4), (dict(out=A + 2), -4),
+                           (dict(pos=A + 4), -4), (dict(counts=A + 4), -4), (dict(status=A + 2), -4), (dict(q_stride=(256, 256, 4)), -4), (dict(out_stride=(4, 256, 64)), -4),
+                           (dict(tokens=64), -5)]:
+        assert call(change)[0] == status, change
+    for change, status in BAD_CACHES:
+        assert call({}, change)[0] == status, change
+    assert call({})[1] == 0 and call(dict(tokens=64))[1] == 4 * 2 * 2 * 40 * 64 and call(dict(heads=3))[1] == -3
+    assert _lib.lib.b200gptq_attn_cache(None, None, 0, None) == -1
+
+
+def test_sampling_refuses():
+    good = dict(logits=A, uniform=A, out=A, logits_stride=100, dtype=0, rows=2, vocab=100)
+    for change, status in [(dict(logits=None), -1), (dict(uniform=None), -1), (dict(out=None), -1), (dict(dtype=3), -3), (dict(rows=0), -3), (dict(vocab=0), -3),
+                           (dict(logits_stride=-1), -3), (dict(vocab=(1 << 18) + 1), -8), (dict(rows=(1 << 27) + 1), -8), (dict(logits=A + 1), -4), (dict(dtype=2, logits=A + 2), -4),
+                           (dict(out=A + 4), -4), (dict(top_k=A + 4), -4), (dict(uniform=A + 2), -4), (dict(temperature=A + 2), -4), (dict(top_p=A + 1), -4), (dict(min_p=A + 2), -4)]:
+        a = _lib.SampleArgs(**{**good, **change})
+        assert _lib.lib.b200gptq_sample(ctypes.byref(a), None) == status, change
+    assert _lib.lib.b200gptq_sample(None, None) == -1
