@@ -53,6 +53,9 @@ class DecoderConfig:
     # Attention sees the last `window` positions and the first `sinks` of a text; None: all of it.
     window: Optional[int] = None
     sinks: int = 0
+    # Keys and values are held in 16 bits, or in 4 with a scale and a zero for each `cache_group` dims (32 or 64) of a row.
+    cache_bits: int = 16
+    cache_group: int = 32
 
     @property
     def head_dim(self) -> int:
@@ -118,6 +121,31 @@ class LogitRules:
         return out
 
 
+@dataclass
+class Sampling:
+    """How a request draws its tokens (:func:`ops.sample`), each number by sequence or one for all; what is not given does not cut anything off.  The random
+    numbers are drawn from ``seed`` when sampling is set, and anew by every prompt: the n-th prompt of two models with the same seed gets the same ones."""
+    temperature: Union[float, Sequence[float]] = 1.0
+    top_k: Union[None, int, Sequence[int]] = None
+    top_p: Union[None, float, Sequence[float]] = None
+    min_p: Union[None, float, Sequence[float]] = None
+    seed: int = 0
+
+    def arguments(self, batch: int, device) -> dict:
+        """The keyword arguments of :func:`ops.sample` that do not change from step to step."""
+        out = {}
+        for name, low, high in (("temperature", 0, math.inf), ("top_k", 0, math.inf), ("top_p", 0, 1), ("min_p", 0, 1)):
+            v = getattr(self, name)
+            if v is None:
+                continue
+            v = [v] * batch if isinstance(v, (int, float)) else list(v)
+            t = torch.tensor(v, dtype=torch.long if name == "top_k" else torch.float32)
+            if len(v) != batch or name == "top_k" and any(not isinstance(x, int) for x in v) or any(not low <= x <= high for x in v) or not bool(torch.isfinite(t).all()):
+                raise ValueError(f"{name}: a number from {low} to {high} for each of {batch} sequences" + (", whole" if name == "top_k" else ""))
+            out[name] = t.to(device)
+        return out
+
+
 def _full_layer(cfg: DecoderConfig, K: int, N: int, bias: bool, seed: int, device) -> synth.PackedLayer:
     return synth.make_layer(cfg.bits, K, N, cfg.group_size, cfg.desc_act, bias=bias, seed=seed, device=device,
                             scale_mult=cfg.scale_mult)
@@ -175,6 +203,7 @@ class DecoderLayer:
             self.norm2_b = torch.zeros(cfg.hidden, device=device, dtype=torch.float16)
         self.k_cache: Optional[torch.Tensor] = None
         self.v_cache: Optional[torch.Tensor] = None
+        self.cache: Optional[ops.QuantCache] = None      # in their place, where keys and values are held in 4 bits
         self.k_prefix: Optional[torch.Tensor] = None     # [heads, positions, hd]: of a text that all sequences begin with
         self.v_prefix: Optional[torch.Tensor] = None
 
@@ -203,7 +232,8 @@ def one_launch_pays(bits: int, hidden: int, max_seq: int, sms: int) -> bool:
 
 
 class GPTQDecoder:
-    """Batch of sequences, one token per step after the prompt; greedy sampling, under rules for the logits where :meth:`set_rules` has some.  Attention sees
+    """Batch of sequences, one token per step after the prompt; the token of the largest logit, or one drawn as :meth:`set_sampling` says, under rules for the
+    logits where :meth:`set_rules` has some.  Keys and values are held in 16 or 4 bits (``cfg.cache_bits``).  Attention sees
     the whole text, the last ``cfg.window`` positions and the first ``cfg.sinks``, or a prefix that all sequences share (:meth:`share_prefix`) and
     each one's own text."""
 
@@ -219,6 +249,8 @@ class GPTQDecoder:
         the model (:meth:`_step_plan`); with ``True`` or ``False`` the kernels are launched one by one."""
         if cfg.window is not None and cfg.window < 1 or cfg.sinks < 0:
             raise ValueError("window must be at least 1, sinks at least 0")
+        if cfg.cache_bits not in (4, 16) or (cfg.cache_bits == 4 and (cfg.cache_group not in (32, 64) or not fused or cfg.head_dim not in (64, 128))):
+            raise ValueError("caches have 16 bits, or 4 in groups of 32 or 64 with the fused helper kernels (heads of 64 or 128 dims)")
         self.cfg, self.batch = cfg, batch
         self._fold_request = fold_activation
         self.fused = fused and cfg.head_dim in (64, 128)   # decode steps use the fused helper kernels
@@ -262,6 +294,9 @@ class GPTQDecoder:
         del head_t
         hd = cfg.head_dim
         for L in self.layers:
+            if cfg.cache_bits == 4:
+                L.cache = ops.QuantCache.empty(batch, L.heads_local, cfg.max_seq, hd, cfg.cache_group, torch.float16, dev)
+                continue
             L.k_cache = torch.zeros(batch, L.heads_local, cfg.max_seq, hd, device=dev, dtype=torch.float16)
             L.v_cache = torch.zeros_like(L.k_cache)
         self.cos, self.sin = self._angles(0)
@@ -270,6 +305,9 @@ class GPTQDecoder:
         self._rule_arguments: dict = {}
         self.history: Optional[torch.Tensor] = None      # [B, prefix + max_seq], with rules: prefix, prompt and what was generated
         self._first = torch.zeros(1, dtype=torch.long, device=dev)
+        self.sampling: Optional[Sampling] = None
+        self._sampling_arguments: dict = {}
+        self._uniform: Optional[torch.Tensor] = None     # [max_seq, B], with sampling: the random number of the token behind each position
         # device-side step state, so that a decode step can be replayed from a CUDA graph
         self.pos = torch.zeros(1, dtype=torch.long, device=dev)
         self.tokens = torch.zeros(batch, dtype=torch.long, device=dev)
@@ -362,7 +400,14 @@ class GPTQDecoder:
     def _sample(self, x_last):
         h = self._norm(x_last, self.final_norm_w, self.final_norm_b)
         self.last_hidden = h
-        return self._pick(self._ruled(self._project(h)))                       # [B, vocab_local]
+        logits = self._ruled(self._project(h))                                 # [B, vocab_local]
+        return self._pick(logits) if self.sampling is None else self._draw(logits)
+
+    def _draw(self, logits, out=None):
+        """The next tokens by their sampling; the last token is the one at ``self.pos``."""
+        self.last_logits = logits
+        u = self._uniform.index_select(0, self.pos).reshape(-1)
+        return ops.sample(logits[:, :self.cfg.vocab], u, out=out, **self._sampling_arguments)
 
     def _ruled(self, logits):
         """The logits of the next token with the rules applied, in place; ``self.history`` ends with the token at ``self.pos``."""
@@ -425,8 +470,8 @@ class GPTQDecoder:
         S = prompt.shape[1]
         before = 0 if self.prefix is None else self.prefix.numel()
         check_positions(0, S, self._room())
-        if self.prefix is not None and S > 65535:
-            raise ValueError("a prompt behind a shared prefix has at most 65535 tokens")
+        if (self.prefix is not None or self.cfg.cache_bits == 4) and S > 65535:
+            raise ValueError("a prompt behind a shared prefix, or into caches of 4 bits, has at most 65535 tokens")
         self._pos_host = S
         pos_idx = torch.arange(S, device=self.device)
         x = self._embed(prompt, pos_idx, before)
@@ -438,6 +483,9 @@ class GPTQDecoder:
         if self.rules is not None:
             self.history[:, before:before + S] = prompt
             self._prompt_lens.fill_(before + S)
+        if self.sampling is not None:
+            self._uniform.uniform_(generator=self._random)
+        if self.rules is not None or self.sampling is not None:
             self.pos.fill_(S - 1)
         self.tokens.copy_(self._sample(x[:, -1]))
         self.pos.fill_(S)
@@ -457,6 +505,8 @@ class GPTQDecoder:
         P = 0 if tokens is None else tokens.numel()
         if P and cfg.window is not None:
             raise ValueError("a shared prefix goes with attention over the whole text")
+        if P and cfg.cache_bits == 4:
+            raise ValueError("a shared prefix goes with caches of 16 bits")
         if P and not self.fused:
             raise ValueError("a shared prefix needs the fused helper kernels (heads of 64 or 128 dims)")
         if P > 65535 or (self.pos_embed is not None and P >= cfg.max_seq):
@@ -494,6 +544,30 @@ class GPTQDecoder:
                 self.history[:, :before] = self.prefix
             self._lengths, self._prompt_lens = (torch.full((self.batch,), before, dtype=torch.long, device=self.device) for _ in range(2))
 
+    def set_sampling(self, sampling: Optional[Sampling]):
+        """Draw every token from now on (``None``: take the one of the largest logit again), from random numbers of their own.  A captured step is dropped."""
+        if sampling is not None and self.world > 1:
+            raise ValueError("sampling looks at the whole vocabulary: one rank")
+        if sampling is not None and self.cfg.vocab > 1 << 18:
+            raise ValueError("sampling takes vocabularies of up to 2^18 tokens")
+        self._sampling_arguments = {} if sampling is None else sampling.arguments(self.batch, self.device)
+        self.sampling, self.graph, self._graph_plan = sampling, None, None
+        self._uniform = None
+        if sampling is not None:
+            self._random = torch.Generator(device=self.device).manual_seed(sampling.seed)
+            self._uniform = torch.rand(self.cfg.max_seq, self.batch, generator=self._random, device=self.device)
+
+    def _write_cache(self, L: DecoderLayer, qkv, S: int, pos, values=None):
+        """New tokens' keys and values into the layer's cache of 4 bits, and their queries ``[B, S, heads, hd]``; ``values``: where what the cache
+        stands for goes, two tensors ``[B, heads, S, hd]``."""
+        q, k, v = qkv.view(-1, S, 3, L.heads_local, self.cfg.head_dim).unbind(2)
+        out = dict(zip(("k_out", "v_out"), (t.transpose(1, 2) for t in values or ())))
+        if self.cfg.arch != "llama":
+            ops.cache_write(L.cache, k, v, pos, **out)
+            return q
+        rotated = torch.empty(q.shape, dtype=torch.float16, device=self.device)
+        return ops.cache_write(L.cache, k, v, pos, cos=self.cos, sin=self.sin, q=q, q_out=rotated, **out)
+
     def _prompt_layers(self, x, S: int, caches=None, cos=None, sin=None):
         """The decoder layers over a prompt with the fused helper kernels: per layer 5 small launches around the linears and
         the framework's attention (as framework element-wise kernels it was fifty, and the host could not keep up:
@@ -511,8 +585,12 @@ class GPTQDecoder:
             k_cache, v_cache = caches[i] if alone else (L.k_cache, L.v_cache)
             ops.add_norm(x, delta, L.norm1_w, L.norm1_b, h, eps, rms)
             qkv = L.qkv(h)
-            q = torch.empty((B, S, L.heads_local, hd), dtype=torch.float16, device=self.device)
-            ops.rope_prompt(qkv, cos, sin, q, k_cache, v_cache, S, L.heads_local, hd, rms)
+            if L.cache is not None:            # the prompt sees what the steps after it will see: the values that the codes stand for
+                k_cache, v_cache = (torch.empty((B, L.heads_local, S, hd), dtype=torch.float16, device=self.device) for _ in range(2))
+                q = self._write_cache(L, qkv, S, self._first, (k_cache, v_cache))
+            else:
+                q = torch.empty((B, S, L.heads_local, hd), dtype=torch.float16, device=self.device)
+                ops.rope_prompt(qkv, cos, sin, q, k_cache, v_cache, S, L.heads_local, hd, rms)
             if cfg.window is not None:
                 att = ops.attn_window(q, k_cache, v_cache, self._first, cfg.window, cfg.sinks)
             elif L.k_prefix is not None:
@@ -545,7 +623,8 @@ class GPTQDecoder:
         kernels of a layer are launched one by one.  Everything that the plan points to is looked at in every step that is not replayed."""
         cfg = self.cfg
         if (self.world > 1 or self.batch != 1 or self.one_launch is False or self._fold_request is not None or self.fold_activation
-                or _module._global_forward_hooks or _module._global_forward_pre_hooks or self.cfg.window is not None or self.prefix is not None):
+                or _module._global_forward_hooks or _module._global_forward_pre_hooks or self.cfg.window is not None or self.prefix is not None
+                or cfg.cache_bits == 4):
             return None                            # (its attention sees the whole of one text; who says how the activation is launched gets it launched that way)
         H, rms = cfg.hidden, cfg.arch == "llama"
         if self.one_launch is None and not one_launch_pays(cfg.bits, H, cfg.max_seq, torch.cuda.get_device_properties(self.device).multi_processor_count):
@@ -604,7 +683,10 @@ class GPTQDecoder:
             ops.add_norm(x, delta, L.norm1_w, L.norm1_b, h, eps, rms)
             qkv = L.qkv(h)
             att = torch.empty((B, L.heads_local * hd), dtype=torch.float16, device=self.device)
-            if cfg.window is not None or L.k_prefix is not None:
+            if L.cache is not None:
+                q = self._write_cache(L, qkv, 1, self.pos)
+                ops.attn_cache(q, L.cache, self.pos, window=cfg.window, sinks=cfg.sinks if cfg.window is not None else 0, out=att.view(q.shape))
+            elif cfg.window is not None or L.k_prefix is not None:
                 q = torch.empty((B, 1, L.heads_local, hd), dtype=torch.float16, device=self.device)
                 ops.rope_cache(qkv, self.cos, self.sin, self.pos, q, L.k_cache, L.v_cache, L.heads_local, hd, rms)
                 if cfg.window is not None:
@@ -627,7 +709,10 @@ class GPTQDecoder:
         ops.add_norm(x, delta, self.final_norm_w, self.final_norm_b, h, eps, rms)
         self.last_hidden = h
         logits = self._ruled(self._project(h))
-        if (logits.dtype is torch.float16 and logits.is_contiguous()
+        if self.sampling is not None:
+            self._draw(logits, self.tokens)
+            self.pos.add_(1)
+        elif (logits.dtype is torch.float16 and logits.is_contiguous()
                 and (self.world == 1 or (self.exchange is not None and B <= 8))):   # the exchange takes up to 8 rows
             # greedy pick and the step's position in the library's kernels: one launch on one GPU, two around the
             # exchange on several (the framework's route is a dozen element-wise launches)
