@@ -2,8 +2,9 @@
 //
 //   zero = min x,  scale = (max x - min x) / 15,  code = round((x - zero) / scale);   value = zero + scale * code
 //
-// One word (eight codes) per lane: HD / 8 lanes share a row, and since a word's fields come from two runs of four dims (cache4.cuh) a lane reads two times 8
-// bytes and the 8 lanes of a group meet in three shuffles for its minimum and maximum.  A row's words, constants and values leave in whole sectors.
+// Four lanes share a row: lane c has 8 dims of each 32, which are the codes of adjacent words (16 bytes of the row, 8 for 64 dims), 16 bytes of 16-bit values at a
+// time. They meet in two shuffles per group for its minimum and maximum. A code is first taken from the product with 1 / scale, which is off by less than
+// 2^-18, and divided out only where that is nearer than that to the middle between two codes.
 // Bound by the bytes of long prompts and by the launch for a decode step.
 #include <algorithm>
 
@@ -17,11 +18,30 @@ constexpr int kThreads = 256;
 
 struct WriteDivisors { Divisor rows, tokens; };
 
-template <typename T> __device__ __forceinline__ void unpack4(uint2 v, float* x) {
-    const float2 a = Half<T>::unpack(v.x), b = Half<T>::unpack(v.y);
-    x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
+template <typename T> __device__ __forceinline__ void unpack8(const uint4& v, float (&x)[8]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = Half<T>::unpack(w[i]);
+        x[2 * i] = f.x; x[2 * i + 1] = f.y;
+    }
 }
-template <typename T> __device__ __forceinline__ uint2 pack4(const float* x) { return make_uint2(Half<T>::pack(x[0], x[1]), Half<T>::pack(x[2], x[3])); }
+template <typename T> __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
+    return make_uint4(Half<T>::pack(x[0], x[1]), Half<T>::pack(x[2], x[3]), Half<T>::pack(x[4], x[5]), Half<T>::pack(x[6], x[7]));
+}
+template <int N> struct Words { uint32_t w[N]; };                 // 4, 8 or 16 bytes
+template <int N> __device__ __forceinline__ Words<N> load_words(const void* at) {
+    Words<N> r;
+    if constexpr (N == 4) { const uint4 v = __ldcg(static_cast<const uint4*>(at)); r.w[0] = v.x; r.w[1] = v.y; r.w[2] = v.z; r.w[3] = v.w; }
+    else if constexpr (N == 2) { const uint2 v = __ldcg(static_cast<const uint2*>(at)); r.w[0] = v.x; r.w[1] = v.y; }
+    else r.w[0] = __ldcg(static_cast<const unsigned*>(at));
+    return r;
+}
+template <int N> __device__ __forceinline__ void store_words(void* at, const Words<N>& r) {
+    if constexpr (N == 4) *static_cast<uint4*>(at) = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
+    else if constexpr (N == 2) *static_cast<uint2*>(at) = make_uint2(r.w[0], r.w[1]);
+    else *static_cast<uint32_t*>(at) = r.w[0];
+}
 // The value of a code.  (-65504 + 15 scales is 65536 where the scale was rounded up: not an infinity in fp16.)
 template <typename T> __device__ __forceinline__ float value_of(unsigned code, float scale, float zero) {
     constexpr float top = std::is_same<T, __half>::value ? 65504.f : 3.38953139e38f;
@@ -29,14 +49,21 @@ template <typename T> __device__ __forceinline__ float value_of(unsigned code, f
     return x > top ? top : x;                     // (the sum of zero, which is no smaller than -top, and of something that is not negative)
 }
 
+// Code of a number d >= 0 from the group's zero on, which is 15.x scales at most.
+__device__ __forceinline__ unsigned code_of(float d, float scale, float inverse) {
+    float q = d * inverse;
+    if (fabsf(q - floorf(q) - 0.5f) < 0x1p-18f) q = __fdiv_rn(d, scale);
+    return (unsigned)fminf(rintf(q), 15.f);
+}
+
 // Rows: for each token the key heads, the value heads and, where queries are rotated, the query heads.
 template <typename T, int HD, int GS>
 __global__ void __launch_bounds__(kThreads)
 cache_write_kernel(const __grid_constant__ b200gptq_cache_write_args a, unsigned rows, const __grid_constant__ WriteDivisors by) {
-    constexpr int LANES = HD / 8;
+    constexpr int Y = HD / 32, NG = HD / GS, HH = HD / 64;
     asm volatile("griddepcontrol.launch_dependents;");
-    const unsigned row = (unsigned)((blockIdx.x * (unsigned long long)kThreads + threadIdx.x) / LANES);
-    const int lane = threadIdx.x & 31, u = lane % LANES, g = u & 7, h = u >> 3, d = 64 * h + 4 * g;
+    const unsigned row = blockIdx.x * (unsigned)(kThreads / 4) + threadIdx.x / 4;
+    const int c = threadIdx.x & 3;
     const unsigned token = over(min(row, rows - 1), by.rows), b = over(token, by.tokens);
     const int per = 2 * a.cache.kv_heads + (a.q ? a.heads : 0), j = (int)(min(row, rows - 1) - token * per), t = (int)(token - b * a.tokens), kv = a.cache.kv_heads;
     const bool is_k = j < kv, is_v = !is_k && j < 2 * kv, is_q = !is_k && !is_v;
@@ -44,126 +71,147 @@ cache_write_kernel(const __grid_constant__ b200gptq_cache_write_args a, unsigned
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const long long start = __ldcg(reinterpret_cast<const long long*>(a.pos) + (a.pos_each ? b : 0));
     const long long count = a.counts ? __ldcg(reinterpret_cast<const long long*>(a.counts) + b) : a.tokens;
+    const T* src = (is_k   ? static_cast<const T*>(a.k) + b * a.k_stride[0] + t * a.k_stride[1] + head * a.k_stride[2]
+                    : is_v ? static_cast<const T*>(a.v) + b * a.v_stride[0] + t * a.v_stride[1] + head * a.v_stride[2]
+                           : static_cast<const T*>(a.q) + b * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2]) + 8 * c;
+    uint4 raw[Y];                                 // (a row of padding is read too: it is there)
+#pragma unroll
+    for (int y = 0; y < Y; ++y) raw[y] = *reinterpret_cast<const uint4*>(src + 32 * y);
     // (a position near the end of 64 bits must not wrap around to one in the cache)
     const bool valid = row < rows && t < count && start < a.cache.max_seq && start >= -(long long)t && start + t < a.cache.max_seq && (!a.cos_t || start + t < a.angles);
     const int p = valid ? (int)(start + t) : 0;
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (valid) {
-        const T* src = is_k   ? static_cast<const T*>(a.k) + b * a.k_stride[0] + t * a.k_stride[1] + head * a.k_stride[2]
-                       : is_v ? static_cast<const T*>(a.v) + b * a.v_stride[0] + t * a.v_stride[1] + head * a.v_stride[2]
-                              : static_cast<const T*>(a.q) + b * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2];
-        unpack4<T>(*reinterpret_cast<const uint2*>(src + d), x);
-        unpack4<T>(*reinterpret_cast<const uint2*>(src + d + 32), x + 4);
-        if (a.cos_t && !is_v) {
-            const T *cos_t = static_cast<const T*>(a.cos_t) + (long long)p * (HD / 2) + d / 2, *sin_t = static_cast<const T*>(a.sin_t) + (long long)p * (HD / 2) + d / 2;
+    const bool turn = a.cos_t && !is_v;
+    if (turn) {
+        const T *cos_t = static_cast<const T*>(a.cos_t) + (long long)p * (HD / 2) + 4 * c, *sin_t = static_cast<const T*>(a.sin_t) + (long long)p * (HD / 2) + 4 * c;
+#pragma unroll
+        for (int y = 0; y < Y; ++y) {
+            const uint2 cw = *reinterpret_cast<const uint2*>(cos_t + 16 * y), sw = *reinterpret_cast<const uint2*>(sin_t + 16 * y);
+            const uint32_t cs[2] = {cw.x, cw.y}, sn[2] = {sw.x, sw.y};
+            float x[8];
+            unpack8<T>(raw[y], x);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const float2 c = Half<T>::unpack(*reinterpret_cast<const uint32_t*>(cos_t + 16 * i)), s = Half<T>::unpack(*reinterpret_cast<const uint32_t*>(sin_t + 16 * i));
-                float* y = x + 4 * i;
+                const float2 f = Half<T>::unpack(cs[i]), s = Half<T>::unpack(sn[i]);
+                float* z = x + 4 * i;
                 // (products of 16-bit numbers are exact in fp32, so it does not matter whether they are fused with the sum)
-                const float y0 = y[0] * c.x - y[1] * s.x, y1 = y[0] * s.x + y[1] * c.x, y2 = y[2] * c.y - y[3] * s.y, y3 = y[2] * s.y + y[3] * c.y;
-                y[0] = y0; y[1] = y1; y[2] = y2; y[3] = y3;
+                const float z0 = z[0] * f.x - z[1] * s.x, z1 = z[0] * s.x + z[1] * f.x, z2 = z[2] * f.y - z[3] * s.y, z3 = z[2] * s.y + z[3] * f.y;
+                z[0] = z0; z[1] = z1; z[2] = z2; z[3] = z3;
             }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = Half<T>::wide(Half<T>::round(x[i]));
+            raw[y] = pack8<T>(x);
         }
     }
     if (valid && is_q) {
-        T* dst = static_cast<T*>(a.q_out) + b * a.q_out_stride[0] + t * a.q_out_stride[1] + head * a.q_out_stride[2] + d;
-        *reinterpret_cast<uint2*>(dst) = pack4<T>(x);
-        *reinterpret_cast<uint2*>(dst + 32) = pack4<T>(x + 4);
-    }
-    // ---- range of each group: the lane's four dims of it (eight, where both runs are in one group), then the 8 lanes ----
-    float lo[2], hi[2], scale[2], zero[2];
-    unsigned odd[2];                              // of the warp's lanes, those with a NaN or an infinity
+        T* dst = static_cast<T*>(a.q_out) + b * a.q_out_stride[0] + t * a.q_out_stride[1] + head * a.q_out_stride[2] + 8 * c;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const float* y = x + 4 * i;
-        lo[i] = fminf(fminf(y[0], y[1]), fminf(y[2], y[3]));
-        hi[i] = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
+        for (int y = 0; y < Y; ++y) *reinterpret_cast<uint4*>(dst + 32 * y) = raw[y];
+    }
+    if (!__any_sync(0xffffffffu, valid && !is_q)) return;
+    Words<2 * HH> word = {};                      // of gg = 2 c + x, half h: 2 x + h (64 dims: x)
+    Words<NG> constants;
+    T* out = static_cast<T*>(is_k ? a.k_out : a.v_out);
+    const bool writes = valid && !is_q;
+    if (out && writes) out += (is_k ? b * a.k_out_stride[0] + t * a.k_out_stride[1] + head * a.k_out_stride[2] : b * a.v_out_stride[0] + t * a.v_out_stride[1] + head * a.v_out_stride[2]) + 8 * c;
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {                // a group: 32 dims or 64
+        constexpr int SPAN = GS / 32;
+        float x[SPAN][8], lo = INFINITY, hi = -INFINITY;
         bool finite = true;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) finite = finite && isfinite(y[e]);
-        odd[i] = __ballot_sync(0xffffffffu, !finite);
-    }
-    if constexpr (GS == 64) { lo[0] = fminf(lo[0], lo[1]); hi[0] = fmaxf(hi[0], hi[1]); odd[0] |= odd[1]; }
+        for (int y = 0; y < SPAN; ++y) {
+            unpack8<T>(raw[SPAN * n + y], x[y]);
 #pragma unroll
-    for (int i = 0; i < (GS == 64 ? 1 : 2); ++i) {
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) {
-            lo[i] = fminf(lo[i], __shfl_xor_sync(0xffffffffu, lo[i], o));
-            hi[i] = fmaxf(hi[i], __shfl_xor_sync(0xffffffffu, hi[i], o));
+            for (int e = 0; e < 8; ++e) {
+                lo = fminf(lo, x[y][e]);
+                hi = fmaxf(hi, x[y][e]);
+                finite = finite && isfinite(x[y][e]);
+            }
         }
-        scale[i] = Half<T>::wide(Half<T>::round(__fdiv_rn(__fsub_rn(hi[i], lo[i]), 15.f)));
-        zero[i] = lo[i];
-        if ((odd[i] >> (lane & ~7) & 0xffu) || !isfinite(scale[i])) scale[i] = zero[i] = __int_as_float(0x7fc00000);
-    }
-    if constexpr (GS == 64) { scale[1] = scale[0]; zero[1] = zero[0]; }
-    if (!valid || is_q) return;
-    unsigned code[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float s = scale[e / 4];
-        code[e] = s > 0.f ? (unsigned)fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[e], zero[e / 4]), s)), 0.f), 15.f) : 0u;
-        x[e] = value_of<T>(code[e], s, zero[e / 4]);
+        for (int o = 1; o < 4; o <<= 1) {
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        }
+        const unsigned odd = __ballot_sync(0xffffffffu, !finite) >> (threadIdx.x & 28) & 15u;
+        float scale = Half<T>::wide(Half<T>::round(__fdiv_rn(__fsub_rn(hi, lo), 15.f))), zero = lo;
+        if (odd || !isfinite(scale)) scale = zero = __int_as_float(0x7fc00000);
+        constants.w[n] = Half<T>::pack(scale, zero);
+        const float inverse = __frcp_rn(scale);
+#pragma unroll
+        for (int y = 0; y < SPAN; ++y) {
+            const int at = SPAN * n + y, h = at >> 1;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                // (a scale that is subnormal in fp32 has no reciprocal there: bf16 below 2^-126)
+                const float d = __fsub_rn(x[y][e], zero);
+                const unsigned code = !(scale > 0.f) ? 0u : inverse < INFINITY ? code_of(d, scale, inverse) : (unsigned)fminf(rintf(__fdiv_rn(d, scale)), 15.f);
+                // fields of dims 0, 2 (of four), 1, 3: 0, 1, 4, 5; in the second half of 64 dims two further on
+                word.w[HH * (e >> 2) + h] |= code << 4 * ((at & 1) * 2 + (e & 1) * 4 + (e & 3) / 2);
+                x[y][e] = value_of<T>(code, scale, zero);
+            }
+            if (out && writes) *reinterpret_cast<uint4*>(out + 32 * at) = pack8<T>(x[y]);
+        }
     }
-    const b200gptq_cache4& c = a.cache;
-    uint8_t* codes = static_cast<uint8_t*>(is_k ? c.k : c.v) + (is_k ? b * c.k_stride[0] + head * c.k_stride[1] + p * c.k_stride[2]
-                                                                     : b * c.v_stride[0] + head * c.v_stride[1] + p * c.v_stride[2]);
-    reinterpret_cast<uint32_t*>(codes)[(HD / 64) * g + h] = cache4_word(code);
-    if (g == 0) {
-        T* constants = static_cast<T*>(is_k ? c.k_scales : c.v_scales) + (is_k ? b * c.k_scale_stride[0] + head * c.k_scale_stride[1] + p * c.k_scale_stride[2]
-                                                                               : b * c.v_scale_stride[0] + head * c.v_scale_stride[1] + p * c.v_scale_stride[2]);
-        if constexpr (GS == 64) reinterpret_cast<uint32_t*>(constants)[h] = Half<T>::pack(scale[0], zero[0]);
-        else reinterpret_cast<uint2*>(constants)[h] = make_uint2(Half<T>::pack(scale[0], zero[0]), Half<T>::pack(scale[1], zero[1]));
-    }
-    T* out = static_cast<T*>(is_k ? a.k_out : a.v_out);
-    if (out) {
-        out += (is_k ? b * a.k_out_stride[0] + t * a.k_out_stride[1] + head * a.k_out_stride[2] : b * a.v_out_stride[0] + t * a.v_out_stride[1] + head * a.v_out_stride[2]) + d;
-        *reinterpret_cast<uint2*>(out) = pack4<T>(x);
-        *reinterpret_cast<uint2*>(out + 32) = pack4<T>(x + 4);
+    if (!writes) return;
+    const b200gptq_cache4& cache = a.cache;
+    uint8_t* codes = static_cast<uint8_t*>(is_k ? cache.k : cache.v) + (is_k ? b * cache.k_stride[0] + head * cache.k_stride[1] + p * cache.k_stride[2]
+                                                                             : b * cache.v_stride[0] + head * cache.v_stride[1] + p * cache.v_stride[2]);
+    store_words<2 * HH>(codes + 8 * HH * c, word);
+    if (c == 0)
+        store_words<NG>(static_cast<T*>(is_k ? cache.k_scales : cache.v_scales) + (is_k ? b * cache.k_scale_stride[0] + head * cache.k_scale_stride[1] + p * cache.k_scale_stride[2]
+                                                                                        : b * cache.v_scale_stride[0] + head * cache.v_scale_stride[1] + p * cache.v_scale_stride[2]),
+                        constants);
+}
+
+// Lane c's part of a row back in 16 bits.
+template <typename T, int HD, int GS> __device__ __forceinline__ void unpack_row(const Words<HD / 32>& word, const Words<HD / GS>& constants, T* out, int c) {
+    constexpr int HH = HD / 64;
+#pragma unroll
+    for (int y = 0; y < HD / 32; ++y) {
+        const float2 of = Half<T>::unpack(constants.w[GS == 32 ? y : y >> 1]);        // (scale, zero)
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = value_of<T>(word.w[HH * (e >> 2) + (y >> 1)] >> 4 * ((y & 1) * 2 + (e & 1) * 4 + (e & 3) / 2) & 15u, of.x, of.y);
+        *reinterpret_cast<uint4*>(out + 32 * y + 8 * c) = pack8<T>(x);
     }
 }
 
-// A row back in 16 bits, HD / 8 lanes (of which this is number u) a row.
-template <typename T, int HD, int GS> __device__ __forceinline__ void read_row(const uint8_t* codes, const T* constants, T* out, int u) {
-    constexpr int NG = HD / GS;
-    const int g = u & 7, h = u >> 3;
-    const uint32_t w = __ldcg(reinterpret_cast<const unsigned*>(codes) + (HD / 64) * g + h);
-    float2 of[2];                                 // (scale, zero) of the two runs of dims
-    of[0] = Half<T>::unpack(__ldcg(reinterpret_cast<const unsigned*>(constants) + h * NG / (HD / 64)));
-    of[1] = GS == 64 ? of[0] : Half<T>::unpack(__ldcg(reinterpret_cast<const unsigned*>(constants) + 2 * h + 1));
-    unsigned code[8];
-    cache4_codes(w, code);
-    float x[8];
+// A CTA takes kRowsPerCta rows of the keys or the values of one sequence and head; a lane kDeep of them, all asked for at once.
+constexpr int kDeep = 4, kRowsPerCta = kThreads / 4 * kDeep;
+template <typename T, int HD, int GS, typename Wanted, typename Out>
+__device__ __forceinline__ void read_rows(const b200gptq_cache4& cache, unsigned b, int head, bool is_k, int j0, Wanted wanted, Out out) {
+    const int c = threadIdx.x & 3;
+    const uint8_t* codes = static_cast<const uint8_t*>(is_k ? cache.k : cache.v) + (is_k ? b * cache.k_stride[0] + head * cache.k_stride[1] : b * cache.v_stride[0] + head * cache.v_stride[1]);
+    const T* constants = static_cast<const T*>(is_k ? cache.k_scales : cache.v_scales) +
+                         (is_k ? b * cache.k_scale_stride[0] + head * cache.k_scale_stride[1] : b * cache.v_scale_stride[0] + head * cache.v_scale_stride[1]);
+    const long long stride = is_k ? cache.k_stride[2] : cache.v_stride[2], scale_stride = is_k ? cache.k_scale_stride[2] : cache.v_scale_stride[2];
+    Words<HD / 32> word[kDeep];
+    Words<HD / GS> of[kDeep];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = value_of<T>(code[e], of[e / 4].x, of[e / 4].y);
-    out += 64 * h + 4 * g;
-    *reinterpret_cast<uint2*>(out) = pack4<T>(x);
-    *reinterpret_cast<uint2*>(out + 32) = pack4<T>(x + 4);
+    for (int i = 0; i < kDeep; ++i) {
+        const int j = j0 + i * (kThreads / 4);
+        if (!wanted(j)) continue;
+        word[i] = load_words<HD / 32>(codes + j * stride + HD / 8 * c);
+        of[i] = load_words<HD / GS>(constants + j * scale_stride);
+    }
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i) {
+        const int j = j0 + i * (kThreads / 4);
+        if (wanted(j)) unpack_row<T, HD, GS>(word[i], of[i], out(j), c);
+    }
 }
 
-// A CTA takes ROWS rows of the keys or the values of one sequence and head.
 template <typename T, int HD, int GS>
 __global__ void __launch_bounds__(kThreads)
 cache_read_kernel(const __grid_constant__ b200gptq_cache_read_args a, unsigned chunks, const __grid_constant__ Divisor by_chunks, const __grid_constant__ Divisor by_heads) {
-    constexpr int LANES = HD / 8, ROWS = kThreads / LANES;
     asm volatile("griddepcontrol.launch_dependents;");
-    const b200gptq_cache4& c = a.cache;
     const unsigned which = over(blockIdx.x, by_chunks), pair = which >> 1, b = over(pair, by_heads);
-    const int head = (int)(pair - b * c.kv_heads);
+    const int head = (int)(pair - b * a.cache.kv_heads), j0 = (int)((blockIdx.x - which * chunks) * kRowsPerCta + threadIdx.x / 4);
     const bool is_k = !(which & 1);
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const long long length = a.lengths ? min(__ldcg(reinterpret_cast<const long long*>(a.lengths) + b), (long long)c.max_seq) : c.max_seq;
-    const int j = (int)((blockIdx.x - which * chunks) * ROWS + threadIdx.x / LANES);
-    if (j >= length) return;
-    const uint8_t* codes = static_cast<const uint8_t*>(is_k ? c.k : c.v) + (is_k ? b * c.k_stride[0] + head * c.k_stride[1] + j * c.k_stride[2]
-                                                                                 : b * c.v_stride[0] + head * c.v_stride[1] + j * c.v_stride[2]);
-    const T* constants = static_cast<const T*>(is_k ? c.k_scales : c.v_scales) + (is_k ? b * c.k_scale_stride[0] + head * c.k_scale_stride[1] + j * c.k_scale_stride[2]
-                                                                                       : b * c.v_scale_stride[0] + head * c.v_scale_stride[1] + j * c.v_scale_stride[2]);
-    T* out = static_cast<T*>(is_k ? a.k_out : a.v_out) + (is_k ? b * a.k_out_stride[0] + head * a.k_out_stride[1] + j * a.k_out_stride[2]
-                                                               : b * a.v_out_stride[0] + head * a.v_out_stride[1] + j * a.v_out_stride[2]);
-    read_row<T, HD, GS>(codes, constants, out, threadIdx.x % LANES);
+    const long long length = a.lengths ? min(__ldcg(reinterpret_cast<const long long*>(a.lengths) + b), (long long)a.cache.max_seq) : a.cache.max_seq;
+    T* out = static_cast<T*>(is_k ? a.k_out : a.v_out) + (is_k ? b * a.k_out_stride[0] + head * a.k_out_stride[1] : b * a.v_out_stride[0] + head * a.v_out_stride[1]);
+    const long long stride = is_k ? a.k_out_stride[2] : a.v_out_stride[2];
+    read_rows<T, HD, GS>(a.cache, b, head, is_k, j0, [&](int j) { return j < length; }, [&](int j) { return out + j * stride; });
 }
 
 // For prompts: the rows that the tokens see between them, into dense k and v [batch, kv_heads, max_seq, hd].
@@ -171,22 +219,16 @@ template <typename T, int HD, int GS>
 __global__ void __launch_bounds__(kThreads)
 cache_read_seen_kernel(const __grid_constant__ Attn4Args a, T* __restrict__ k, T* __restrict__ v, unsigned chunks, const __grid_constant__ Divisor by_chunks,
                        const __grid_constant__ Divisor by_heads) {
-    constexpr int LANES = HD / 8, ROWS = kThreads / LANES;
     asm volatile("griddepcontrol.launch_dependents;");
-    const b200gptq_cache4& c = a.cache;
     const unsigned which = over(blockIdx.x, by_chunks), pair = which >> 1, b = over(pair, by_heads);
-    const int head = (int)(pair - b * c.kv_heads);
+    const int head = (int)(pair - b * a.cache.kv_heads), j0 = (int)((blockIdx.x - which * chunks) * kRowsPerCta + threadIdx.x / 4);
     const bool is_k = !(which & 1);
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int j = (int)((blockIdx.x - which * chunks) * ROWS + threadIdx.x / LANES);
     const int p0 = attn_pos(a.attn, b), count = attn_count(a.attn, b);
-    const AttnRange r = attn_range(p0, p0 + count - 1, a.attn.window ? a.attn.window : 1 << 30, a.attn.sinks, c.max_seq);
-    if (!count || j >= r.w_end || (j >= r.s_end && j < r.w_start) || j >= c.max_seq) return;
-    const uint8_t* codes = static_cast<const uint8_t*>(is_k ? c.k : c.v) + (is_k ? b * c.k_stride[0] + head * c.k_stride[1] + j * c.k_stride[2]
-                                                                                 : b * c.v_stride[0] + head * c.v_stride[1] + j * c.v_stride[2]);
-    const T* constants = static_cast<const T*>(is_k ? c.k_scales : c.v_scales) + (is_k ? b * c.k_scale_stride[0] + head * c.k_scale_stride[1] + j * c.k_scale_stride[2]
-                                                                                       : b * c.v_scale_stride[0] + head * c.v_scale_stride[1] + j * c.v_scale_stride[2]);
-    read_row<T, HD, GS>(codes, constants, (is_k ? k : v) + ((long long)pair * c.max_seq + j) * HD, threadIdx.x % LANES);
+    const AttnRange r = attn_range(p0, p0 + count - 1, a.attn.window ? a.attn.window : 1 << 30, a.attn.sinks, a.cache.max_seq);
+    const int end = count ? min(r.w_end, a.cache.max_seq) : 0;
+    T* out = (is_k ? k : v) + (long long)pair * a.cache.max_seq * HD;
+    read_rows<T, HD, GS>(a.cache, b, head, is_k, j0, [&](int j) { return j < end && (j < r.s_end || j >= r.w_start); }, [&](int j) { return out + (long long)j * HD; });
 }
 
 template <typename... KArgs, typename... Args>
@@ -208,21 +250,19 @@ template <typename T, int HD, int GS>
 int write(const b200gptq_cache_write_args& a, cudaStream_t stream) {
     const long long per = 2LL * a.cache.kv_heads + (a.q ? a.heads : 0), rows = per * a.cache.batch * a.tokens;
     const WriteDivisors by = {Divisor(per), Divisor(a.tokens)};
-    return launch(cache_write_kernel<T, HD, GS>, dim3((unsigned)((rows * (HD / 8) + kThreads - 1) / kThreads)), stream, a, (unsigned)rows, by);
+    return launch(cache_write_kernel<T, HD, GS>, dim3((unsigned)((rows * 4 + kThreads - 1) / kThreads)), stream, a, (unsigned)rows, by);
 }
 
 template <typename T, int HD, int GS>
 int read(const b200gptq_cache_read_args& a, cudaStream_t stream) {
-    constexpr int ROWS = kThreads / (HD / 8);
-    const long long chunks = (a.cache.max_seq + ROWS - 1) / ROWS, ctas = 2LL * a.cache.batch * a.cache.kv_heads;
+    const long long chunks = (a.cache.max_seq + kRowsPerCta - 1) / kRowsPerCta, ctas = 2LL * a.cache.batch * a.cache.kv_heads;
     if (ctas > 0x7fffffff / chunks) return B200GPTQ_ERR_TOO_LARGE;
     return launch(cache_read_kernel<T, HD, GS>, dim3((unsigned)(ctas * chunks)), stream, a, (unsigned)chunks, Divisor(chunks), Divisor(a.cache.kv_heads));
 }
 
 template <typename T, int HD, int GS>
 int read_seen(const Attn4Args& a, void* k, void* v, cudaStream_t stream) {
-    constexpr int ROWS = kThreads / (HD / 8);
-    const long long chunks = (a.cache.max_seq + ROWS - 1) / ROWS, ctas = 2LL * a.cache.batch * a.cache.kv_heads;
+    const long long chunks = (a.cache.max_seq + kRowsPerCta - 1) / kRowsPerCta, ctas = 2LL * a.cache.batch * a.cache.kv_heads;
     if (ctas > 0x7fffffff / chunks) return B200GPTQ_ERR_TOO_LARGE;
     return launch(cache_read_seen_kernel<T, HD, GS>, dim3((unsigned)(ctas * chunks)), stream, a, static_cast<T*>(k), static_cast<T*>(v), (unsigned)chunks, Divisor(chunks),
                   Divisor(a.cache.kv_heads));
@@ -259,7 +299,7 @@ B200GPTQ_API int b200gptq_cache_write(const b200gptq_cache_write_args* args, voi
     // (rows are numbered in 31 bits)
     if (a.tokens > kCacheMost || (a.q && a.heads > kCacheMost)) return B200GPTQ_ERR_TOO_LARGE;
     const double rows = (2.0 * a.cache.kv_heads + (a.q ? a.heads : 0)) * a.cache.batch * a.tokens;
-    if (rows * (a.cache.hd / 8) > 2147483647.0) return B200GPTQ_ERR_TOO_LARGE;
+    if (rows > 2147483647.0) return B200GPTQ_ERR_TOO_LARGE;
     st = cache4_check_memory(a.cache);
     if (st != B200GPTQ_OK) return st;
     if ((bits_of(a.k, a.k_stride) | bits_of(a.v, a.v_stride) | bits_of(a.q, a.q_stride) | bits_of(a.q_out, a.q_out_stride) | bits_of(a.k_out, a.k_out_stride) |

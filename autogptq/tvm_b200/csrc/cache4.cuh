@@ -26,9 +26,6 @@ inline int cache4_check_memory(const b200gptq_cache4& c) {
 
 // Lane u of the HD / 8 that share a row has word (HD / 64) (u % 8) + u / 8 of it: dims a .. a + 3 in its fields 0, 4, 1, 5 and dims a + 32 .. a + 35 in 2, 6, 3, 7,
 // with a = 64 (u / 8) + 4 (u % 8).  x[0 .. 3] are the former, x[4 .. 7] the latter.
-__device__ __forceinline__ uint32_t cache4_word(const unsigned (&c)[8]) {
-    return c[0] | c[2] << 4 | c[4] << 8 | c[6] << 12 | c[1] << 16 | c[3] << 20 | c[5] << 24 | c[7] << 28;
-}
 __device__ __forceinline__ void cache4_codes(uint32_t w, unsigned (&c)[8]) {
     c[0] = w & 15u; c[2] = w >> 4 & 15u; c[4] = w >> 8 & 15u; c[6] = w >> 12 & 15u;
     c[1] = w >> 16 & 15u; c[3] = w >> 20 & 15u; c[5] = w >> 24 & 15u; c[7] = w >> 28;

@@ -12,6 +12,7 @@
 // through distributed shared memory and all come to the same results.
 #include <cuda_bf16.h>
 
+#include <cstddef>
 #include <cstdlib>
 #include <mutex>
 
@@ -20,7 +21,7 @@
 namespace b200gptq {
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 1024, kMostCtas = 8, kTable = 64;
+constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 1024, kFine = 512, kFineBits = 9, kMostCtas = 8, kTable = 64;
 constexpr float kColdest = 1e-18f;       // temperatures below count as 0, so that no scale leaves fp32
 typedef unsigned long long u64;
 
@@ -47,14 +48,13 @@ __device__ __forceinline__ unsigned ld_remote(uint32_t at) {
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
     return v;
 }
-__device__ __forceinline__ u64 ld_remote64(uint32_t at) {
-    u64 v;
-    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(at) : "memory");
+__device__ __forceinline__ uint2 ld_remote2(uint32_t at) {
+    uint2 v;
+    asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
     return v;
 }
 __device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ u64 shfl_up(u64 v, int o) { return __shfl_up_sync(0xffffffffu, v, o); }
 template <typename V> __device__ __forceinline__ V warp_total(V v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -84,14 +84,15 @@ __device__ __forceinline__ u64 share(float f, u64 s, bool up) {
     return q + (up && rest ? 1 : 0);
 }
 
-struct Bins { unsigned count[kBins], low[kBins], high[kBins]; };
+template <int N> struct Bins { unsigned count[N], low[N], high[N]; };
 struct Warp { u64 mass; unsigned ties, unused; };       // of a warp's tokens: sum above the border, how many are at it
 struct Shared {
-    Bins bins[2];
+    Bins<kBins> bins;
+    Bins<kFine> fine[2];
     double table[kTable];
     Warp warps[kWarps];
-    u64 scan_mass[kWarps], found_mass, found_below;
-    unsigned scan_count[kWarps], found_count, found_inside;
+    u64 scan_mass[kWarps], found_mass;
+    unsigned scan_count[kWarps], found_count;
     float top, warp_top[kWarps];
     int found;
 };
@@ -126,64 +127,92 @@ __device__ __forceinline__ int bin_of(float x, const Row& r) {
     return f < (float)kBins ? (int)f : kBins;                                                // (a NaN: kBins)
 }
 
-// The bins of all CTAs of the cluster added up, and the first bin, from the top on, with which count or mass reaches its target: leaves the bin, what lies
-// above it and what is in it in `s` (found: -1 where the target is not reached).  Begins with a barrier of the cluster.
-__device__ void find_bin(Shared& s, const Bins& mine, int ctas, bool by_count, u64 target, u64 above) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (ctas > 1) cluster_sync();
-    else __syncthreads();
-    constexpr int PER = kBins / kThreads;
-    unsigned n[PER];
-    u64 m[PER], count = 0, mass = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        n[i] = 0;
-        m[i] = 0;
-        const int bin = tid * PER + i;
-        for (int c = 0; c < ctas; ++c) {
-            if (ctas > 1) {
-                n[i] += ld_remote(remote_of(mine.count + bin, c));
-                m[i] += (u64)ld_remote(remote_of(mine.high + bin, c)) << 32;
-                m[i] += ld_remote(remote_of(mine.low + bin, c));
-            } else {
-                n[i] = mine.count[bin];
-                m[i] = ((u64)mine.high[bin] << 32) + mine.low[bin];
-            }
-        }
-        count += n[i];
-        mass += m[i];
-    }
-    u64 count_to = warp_prefix(count, lane), mass_to = warp_prefix(mass, lane);
-    if (lane == 31) { s.scan_count[warp] = (unsigned)count_to; s.scan_mass[warp] = mass_to; }
-    if (tid == 0) s.found = -1;
-    __syncthreads();
-    for (int w = 0; w < warp; ++w) { count_to += s.scan_count[w]; mass_to += s.scan_mass[w]; }
-    count_to -= count;
-    mass_to -= mass;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const u64 before = above + (by_count ? count_to : mass_to), after = before + (by_count ? n[i] : m[i]);
-        if (before < target && after >= target) {
-            s.found = tid * PER + i;
-            s.found_count = (unsigned)count_to;
-            s.found_mass = mass_to;
-            s.found_inside = n[i];
-        }
-        count_to += n[i];
-        mass_to += m[i];
-    }
-    if (tid == kThreads - 1) s.found_below = mass_to;        // all of it
-    __syncthreads();
-}
-
-__device__ __forceinline__ void put(Bins& h, unsigned at, u64 w) {
-    atomicAdd(h.count + at, 1u);
+template <int N> __device__ __forceinline__ void put(Bins<N>& h, unsigned at, u64 w, bool counts) {
+    if (counts) atomicAdd(h.count + at, 1u);
     const unsigned low = (unsigned)w, old = atomicAdd(h.low + at, low), high = (unsigned)(w >> 32) + (old + low < low ? 1u : 0u);
     if (high) atomicAdd(h.high + at, high);
 }
 
+// The thread's bins (PER adjacent ones) of all CTAs of the cluster added up, and what lies above them.  The CTAs have met before.
+template <int PER> struct Sums {
+    unsigned n[PER];
+    u64 m[PER], count_before, mass_before, mass_all;
+
+    template <int N> __device__ __forceinline__ void add_up(Shared& s, const Bins<N>& mine, int ctas, bool counts) {
+        static_assert(N == PER * kThreads, "");
+        const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) n[i] = 0, m[i] = 0;
+        if (ctas == 1) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                n[i] = mine.count[tid * PER + i];
+                m[i] = ((u64)mine.high[tid * PER + i] << 32) + mine.low[tid * PER + i];
+            }
+        } else {
+            const int bin = tid * PER;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {        // (all loads of four CTAs on their way at once)
+                uint2 c[4], l[4], h[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    c[r] = l[r] = h[r] = make_uint2(0, 0);
+                    if (4 * half + r >= ctas) continue;
+                    if constexpr (PER == 2) {
+                        if (counts) c[r] = ld_remote2(remote_of(mine.count + bin, 4 * half + r));
+                        l[r] = ld_remote2(remote_of(mine.low + bin, 4 * half + r));
+                        h[r] = ld_remote2(remote_of(mine.high + bin, 4 * half + r));
+                    } else {
+                        if (counts) c[r].x = ld_remote(remote_of(mine.count + bin, 4 * half + r));
+                        l[r].x = ld_remote(remote_of(mine.low + bin, 4 * half + r));
+                        h[r].x = ld_remote(remote_of(mine.high + bin, 4 * half + r));
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    n[0] += c[r].x;
+                    m[0] += ((u64)h[r].x << 32) + l[r].x;
+                    if constexpr (PER == 2) { n[1] += c[r].y; m[1] += ((u64)h[r].y << 32) + l[r].y; }
+                }
+            }
+        }
+        u64 count = 0, mass = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) { count += n[i]; mass += m[i]; }
+        const u64 count_to = counts ? warp_prefix(count, lane) : 0, mass_to = warp_prefix(mass, lane);
+        if (lane == 31) { s.scan_count[warp] = (unsigned)count_to; s.scan_mass[warp] = mass_to; }
+        if (tid == 0) s.found = -1;
+        __syncthreads();
+        count_before = count_to - count;
+        mass_before = mass_to - mass;
+        mass_all = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) { count_before += s.scan_count[w]; mass_before += s.scan_mass[w]; }
+            mass_all += s.scan_mass[w];
+        }
+    }
+    // The first bin, from the top on, with which count or mass (and what lies `above` all of them) reaches its target, with what lies above it among
+    // the bins, in `s`; s.found is -1 on entry and where there is none.
+    __device__ __forceinline__ void find(Shared& s, bool by_count, u64 target, u64 above) const {
+        u64 count_to = count_before, mass_to = mass_before;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const u64 before = above + (by_count ? count_to : mass_to), after = before + (by_count ? n[i] : m[i]);
+            if (before < target && after >= target) {
+                s.found = threadIdx.x * PER + i;
+                s.found_count = (unsigned)count_to;
+                s.found_mass = mass_to;
+            }
+            count_to += n[i];
+            mass_to += m[i];
+        }
+        __syncthreads();
+    }
+};
+
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 2)
 sample_kernel(const __grid_constant__ b200gptq_sample_args a, int slice, int cluster_bits, int bits) {
     extern __shared__ __align__(16) unsigned char smem[];
     Shared& s = *reinterpret_cast<Shared*>(smem);
@@ -192,7 +221,12 @@ sample_kernel(const __grid_constant__ b200gptq_sample_args a, int slice, int clu
     const int base = min(rank * slice, a.vocab), n = min(slice, a.vocab - base);
     // A warp's tokens: a run of the slice
     const int run = (slice + kWarps - 1) / kWarps, first = min(warp * run, n), last = min(first + run, n);
-    for (int i = tid; i < kBins * 3 * 2; i += kThreads) reinterpret_cast<unsigned*>(s.bins)[i] = 0;
+    static_assert(offsetof(Shared, fine) == sizeof(Bins<kBins>), "");
+    for (int i = tid; i < kBins * 3 + 2 * kFine * 3; i += kThreads) reinterpret_cast<unsigned*>(&s.bins)[i] = 0;
+    auto meet = [&] {
+        if (ctas > 1) cluster_sync();
+        else __syncthreads();
+    };
     if (tid < kTable) s.table[tid] = exp2((double)tid / kTable);
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -225,11 +259,16 @@ sample_kernel(const __grid_constant__ b200gptq_sample_args a, int slice, int clu
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         if (tid == 0) s.top = top;
     }
-    if (ctas > 1) cluster_sync();
-    else __syncthreads();
+    meet();
     Row r;
     r.top = s.top;
-    for (int c = 0; c < ctas && ctas > 1; ++c) r.top = fmaxf(r.top, __uint_as_float(ld_remote(remote_of(&s.top, c))));
+    if (ctas > 1) {
+        float others[kMostCtas];
+#pragma unroll
+        for (int c = 0; c < kMostCtas; ++c) others[c] = c < ctas ? __uint_as_float(ld_remote(remote_of(&s.top, c))) : -INFINITY;
+#pragma unroll
+        for (int c = 0; c < kMostCtas; ++c) r.top = fmaxf(r.top, others[c]);
+    }
     r.bits = bits;
     const bool greedy = !(temperature >= kColdest) || top_k == 1 || min_p > 1.f || r.top == -INFINITY;
     r.step = greedy ? 0.0 : 64 * 1.4426950408889634074 / (double)temperature;
@@ -240,16 +279,21 @@ sample_kernel(const __grid_constant__ b200gptq_sample_args a, int slice, int clu
         border = key_of(r.top);
         ties = 1;
     } else if (top_k > 0 || top_p < 1.f) {
+        const bool counts = top_k > 0;
+#pragma unroll 4
         for (int i = first + lane; i < last; i += 32) {
             const float v = wide(x[i]);
             const int bin = bin_of(v, r);
-            if (bin >= kBins) continue;
-            put(s.bins[0], bin, weight(v, r, s.table));
+            if (bin < kBins) put(s.bins, bin, weight(v, r, s.table), counts);
         }
-        u64 sum = 0;                     // of what top-k keeps
-        // One value of x: the border of the first `target` tokens (by_count) or of the shortest beginning that weighs `target`.
-        auto search = [&](bool by_count, u64 target, unsigned& key, unsigned& above_count, u64& above_mass, unsigned& inside) {
-            find_bin(s, s.bins[0], ctas, by_count, target, 0);
+        meet();
+        Sums<kBins / kThreads> whole;
+        whole.add_up(s, s.bins, ctas, counts);
+        int level = 0;
+        u64 above_count = 0, above_mass = 0;
+        // The value of x at which the first `target` tokens (by_count), or the shortest beginning that weighs `target`, end, and what lies above it
+        auto search = [&](bool by_count, u64 target, unsigned& key) {
+            whole.find(s, by_count, target, 0);
             const int bin = s.found;
             if (bin < 0) return false;
             above_count = s.found_count;
@@ -260,49 +304,43 @@ sample_kernel(const __grid_constant__ b200gptq_sample_args a, int slice, int clu
             unsigned lo = key_of(far) > 2 ? key_of(far) - 2 : 0, hi = max(key_of(fminf(near, r.top)), 3u) + (bin == 0 ? 0 : 2);
             int shift;
             do {
-                __syncthreads();         // (what the last search found has been read)
-                shift = max(0, 32 - __clz(hi - lo) - 10);
-                Bins& h = s.bins[1];
-                for (int i = tid; i < kBins * 3; i += kThreads) reinterpret_cast<unsigned*>(&h)[i] = 0;
-                __syncthreads();
+                shift = max(0, 32 - __clz(hi - lo) - kFineBits);
+                Bins<kFine>& h = s.fine[level & 1];
+#pragma unroll 4
                 for (int i = first + lane; i < last; i += 32) {
                     const float v = wide(x[i]);
-                    if (bin_of(v, r) != bin) continue;
                     const unsigned k = key_of(v);
-                    if (k < lo || k > hi) continue;
-                    put(h, (hi - k) >> shift, weight(v, r, s.table));
+                    if (k >= lo && k <= hi && bin_of(v, r) == bin) put(h, (hi - k) >> shift, weight(v, r, s.table), counts);
                 }
-                find_bin(s, h, ctas, by_count, target, by_count ? above_count : above_mass);
+                meet();
+                // (the other one has been read by all: it was added up before they met)
+                ++level;
+                for (int i = tid; i < kFine * 3; i += kThreads) reinterpret_cast<unsigned*>(s.fine + (level & 1))[i] = 0;
+                Sums<kFine / kThreads> part;
+                part.add_up(s, h, ctas, counts);
+                part.find(s, by_count, target, by_count ? above_count : above_mass);
                 above_count += s.found_count;
                 above_mass += s.found_mass;
-                inside = s.found_inside;
                 hi -= (unsigned)s.found << shift;
                 lo = max(lo, hi - ((1u << shift) - 1));
-                if (ctas > 1) cluster_sync();        // (the bins have been read by all)
+                __syncthreads();         // (what was found has been read)
+                if (tid == 0) s.found = -1;
             } while (shift > 0);
+            __syncthreads();
             key = hi;
             return true;
         };
-        unsigned above_count = 0, inside = 0;
-        u64 above_mass = 0;
-        bool cut = false;
-        if (top_k > 0) {
-            cut = search(true, (u64)top_k, border, above_count, above_mass, inside);
-            if (cut) {
-                ties = (unsigned)(top_k - above_count);
-                sum = above_mass + ties * weight(of_key(border), r, s.table);
-            }
+        u64 sum = whole.mass_all;        // of what top-k keeps
+        const bool cut = top_k > 0 && search(true, (u64)top_k, border);
+        if (cut) {
+            ties = (unsigned)(top_k - above_count);
+            sum = above_mass + ties * weight(of_key(border), r, s.table);
         }
         if (top_p < 1.f) {
-            if (!cut) {
-                if (top_k <= 0) find_bin(s, s.bins[0], ctas, true, ~0ull, 0);
-                sum = s.found_below;
-                __syncthreads();
-            }
             u64 target = share(top_p, sum, true);
             if (target == 0) target = 1;
             unsigned key = 0;
-            if (search(false, target, key, above_count, above_mass, inside)) {
+            if (search(false, target, key)) {
                 const u64 w = weight(of_key(key), r, s.table), need = (target - above_mass + w - 1) / w;
                 ties = key == border && cut ? min(ties, (unsigned)need) : (unsigned)need;
                 border = key;
@@ -314,6 +352,7 @@ sample_kernel(const __grid_constant__ b200gptq_sample_args a, int slice, int clu
     // (what min-p leaves out has a smaller key than all that it keeps)
     auto kept_weight = [&](float v) { const u64 w = greedy ? 1 : weight(v, r, s.table); return w >= least || v == r.top ? w : 0; };
     Warp mine = {0, 0, 0};
+#pragma unroll 4
     for (int i = first + lane; i < last; i += 32) {
         const float v = wide(x[i]);
         const unsigned k = key_of(v);
@@ -323,8 +362,7 @@ sample_kernel(const __grid_constant__ b200gptq_sample_args a, int slice, int clu
     mine.mass = warp_total(mine.mass);
     mine.ties = warp_total(mine.ties);
     if (lane == 0) s.warps[warp] = mine;
-    if (ctas > 1) cluster_sync();
-    else __syncthreads();
+    meet();
     const u64 border_w = border ? kept_weight(of_key(border)) : 0;
     // every warp looks at all warps of the cluster, 32 at a time: those before it, and all
     u64 before = 0, total = 0;
@@ -335,7 +373,8 @@ sample_kernel(const __grid_constant__ b200gptq_sample_args a, int slice, int clu
         if (w < ctas * kWarps) {
             if (ctas > 1) {
                 const uint32_t at = remote_of(s.warps + (w % kWarps), w / kWarps);
-                other.mass = ld_remote64(at);
+                const uint2 mass = ld_remote2(at);
+                other.mass = (u64)mass.y << 32 | mass.x;
                 other.ties = ld_remote(at + 8);
             } else {
                 other = s.warps[w];
@@ -388,10 +427,12 @@ sample_kernel(const __grid_constant__ b200gptq_sample_args a, int slice, int clu
 
 template <typename T>
 int launch(const b200gptq_sample_args& a, cudaStream_t stream) {
+    // CTAs per row: as many as the SMs hold three of, a slice of 1024 tokens or more, and enough that a slice leaves an SM room for three (51 KB; what eight cannot
+    // hold so takes more).
     int cluster_bits = 0;
-    while (cluster_bits < 3 && (long long)a.rows << (cluster_bits + 1) <= 2LL * sm_count() && a.vocab >> (cluster_bits + 1) >= 1024) ++cluster_bits;
-    constexpr int most = 128 * 1024 / sizeof(T);       // tokens of a slice
-    while ((a.vocab + (1 << cluster_bits) - 1) >> cluster_bits > most) ++cluster_bits;
+    while (cluster_bits < 3 && ((long long)a.rows << (cluster_bits + 1) <= 3LL * sm_count() || (long long)a.vocab * sizeof(T) > 51200LL << cluster_bits) &&
+           a.vocab >> (cluster_bits + 1) >= 1024)
+        ++cluster_bits;
     // (slices begin at multiples of 16 bytes)
     const int slice = (((a.vocab + (1 << cluster_bits) - 1) >> cluster_bits) + 7) / 8 * 8;
     int log2v = 0;
