@@ -2,14 +2,17 @@
 //
 //   w_v = exp((x_v - max x) / T),  kept: a beginning of the order "larger x, then lower v",  token: the first v whose kept sum passes u * (sum of all kept)
 //
-// All that decides is exact: weights are integers (units of 2^-F of the largest, F so that the vocabulary's sum fits 62 bits; exp2 in 64 bits from a table of 64 powers
-// and a Taylor polynomial of degree 5, after P. T. P. Tang, "Table-driven implementation of the exponential function", 1989), their sums have no order, and the
-// products p * S and u * S are taken in 128 bits. Sums in fp32 would put the border off by more than what lies between two tokens of a large vocabulary.
+// What decides are sums over the vocabulary, and a random number may fall anywhere between two tokens: sums in fp32 put borders off by more than what lies
+// between neighbours.  Weights are integers here (units of 2^-F of the largest, F so that the vocabulary's sum fits 62 bits; off by 2^-32 relative at most: the logarithm in fixed
+// point of 32 fractional bits, by one FMA in 64 bits, a table of 256 powers and a Taylor polynomial of degree 3, after P. T. P. Tang, "Table-driven implementation of the
+// exponential function", 1989), their sums have neither order nor rounding, and the products p * S and u * S are taken in 128 bits.
 //
-// A cluster of CTAs shares a row, each keeps a slice of the logits in shared memory. The number of kept tokens follows from histograms: 1024 bins, linear in
-// the logarithm of the weight, with the number and the sum of the tokens in each (the order of x and of the bins is the same), then the bin in which top-k or top-p ends
-// again by the bits of x until one value is left. Tokens of that value are kept from the lowest on. The CTAs of a cluster read each other's bins
-// through distributed shared memory and all come to the same results.
+// A cluster of CTAs shares a row, each keeps a slice of the logits in shared memory.  Where top-k or top-p ends follows from histograms: 1024 bins, linear in
+// the logarithm of the weight, of the tokens' number (top-k) or weight (top-p; the order of x and of the bins is the same), then the bin in which the search ends
+// again by the bits of x until one value is left.  Tokens of that value are kept from the lowest on.  After the first bins only the tokens down to where the
+// search ended are looked at again: each warp moves its own together.  The CTAs of the cluster read each other's sums through distributed shared memory and all come
+// to the same results.
+// Bound by instructions, a pass over all tokens with their weights and two without, and for a few rows by the chain of passes and exchanges.
 #include <cuda_bf16.h>
 
 #include <cstddef>
@@ -21,7 +24,7 @@
 namespace b200gptq {
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 1024, kFine = 512, kFineBits = 9, kMostCtas = 8, kTable = 64;
+constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 1024, kBinBits = 10, kMostCtas = 8, kTableBits = 8, kTable = 1 << kTableBits;
 constexpr float kColdest = 1e-18f;       // temperatures below count as 0, so that no scale leaves fp32
 typedef unsigned long long u64;
 
@@ -30,13 +33,18 @@ template <> __device__ __forceinline__ float wide(float x) { return x; }
 template <> __device__ __forceinline__ float wide(__half x) { return __half2float(x); }
 template <> __device__ __forceinline__ float wide(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// Larger x, larger key; a NaN counts as minus infinity.
-__device__ __forceinline__ unsigned key_of(float x) {
+// Larger x, larger key; a NaN counts as minus infinity.  (The last 13 or 16 bits of a number of 16 bits say nothing in fp32.)
+template <typename T> struct Key { static constexpr int shift = 0; };
+template <> struct Key<__half> { static constexpr int shift = 13; };
+template <> struct Key<__nv_bfloat16> { static constexpr int shift = 16; };
+template <typename T> __device__ __forceinline__ unsigned key_of(float x) {
     const unsigned b = __float_as_uint(x == 0.f ? 0.f : x);
-    return x != x ? 0u : b & 0x80000000u ? ~b : b | 0x80000000u;
+    return x != x ? 0u : (b & 0x80000000u ? ~b : b | 0x80000000u) >> Key<T>::shift;
 }
-
-__device__ __forceinline__ float of_key(unsigned k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+template <typename T> __device__ __forceinline__ float of_key(unsigned k) {
+    const unsigned b = k << Key<T>::shift;
+    return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~(b | ((1u << Key<T>::shift) - 1)));
+}
 
 __device__ __forceinline__ uint32_t remote_of(const void* local, int rank) {
     uint32_t r;
@@ -51,6 +59,11 @@ __device__ __forceinline__ unsigned ld_remote(uint32_t at) {
 __device__ __forceinline__ uint2 ld_remote2(uint32_t at) {
     uint2 v;
     asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint4 ld_remote4(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
     return v;
 }
 __device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
@@ -84,42 +97,42 @@ __device__ __forceinline__ u64 share(float f, u64 s, bool up) {
     return q + (up && rest ? 1 : 0);
 }
 
-template <int N> struct Bins { unsigned count[N], low[N], high[N]; };
-struct Warp { u64 mass; unsigned ties, unused; };       // of a warp's tokens: sum above the border, how many are at it
+struct Power { unsigned whole; float part; };       // 2^(30 + j / kTable), as a whole number and in fp32
+// A bin's weight in three words of 17 bits and what they pass over, so that adding takes no carry (a slice has below 2^15 tokens); its number of tokens is in the first.
+struct Bins { unsigned part[3][kBins]; };
+constexpr int kPart = 17;
+struct __align__(16) Warp { u64 mass; unsigned ties, unused; };       // of a warp's tokens: sum above the border, how many are at it
 struct Shared {
-    Bins<kBins> bins;
-    Bins<kFine> fine[2];
-    double table[kTable];
+    Bins bins[3];                         // in turn: this pass's, the last one's, the next one's
+    u64 groups[3][kBins / 32];            // sums of 32 bins
+    Power table[kTable];
     Warp warps[kWarps];
-    u64 scan_mass[kWarps], found_mass;
-    unsigned scan_count[kWarps], found_count;
+    u64 found_above, all, target, before;
+    unsigned ties_before;
     float top, warp_top[kWarps];
-    int found;
+    int found, owner;
 };
 
 // Everything of a row that the CTAs of its cluster agree on.
 struct Row {
     float top, half_scale;               // largest logit; bins per half a unit of x
-    double step;                         // 64 log2(e) / T
+    double step;                         // log2(e) / T
     int bits;                            // F
 };
-__device__ __forceinline__ u64 weight(float x, const Row& r, const double* table) {
-    if (x == r.top) return 1ull << r.bits;
-    const double z = ((double)x - (double)r.top) * r.step;
-    if (!(z > -64.0 * 64)) return 0;
-    const double magic = 6755399441055744.0, y = z + magic, f = z - (y - magic);             // z = i + f, |f| <= 1/2
-    const int i = (int)(unsigned)__double_as_longlong(y);
-    constexpr double l = 0.69314718055994530942 / kTable;
-    double p = fma(f, l * l * l * l * l / 120, l * l * l * l / 24);
-    p = fma(f, p, l * l * l / 6);
-    p = fma(f, p, l * l / 2);
-    p = fma(f, p, l);
-    p = fma(f, p, 1.0);
-    const u64 b = (u64)__double_as_longlong(p * table[i & (kTable - 1)]);                    // [1/2, 2): near 1 the polynomial may be below it
-    const int e = (int)(b >> 52) - 1023 + (i >> 6) + r.bits, down = 52 - e;
-    const u64 m = (b & ((1ull << 52) - 1)) | 1ull << 52;
-    return down > 54 ? 0 : ((m >> (down - 1)) + 1) >> 1;                                     // (down is 3 at least: F is 49 at most)
+__device__ __forceinline__ u64 weight(float x, const Row& r, const Power* table) {        // (no branches: several at once hide each other's latency)
+    // 1.5 2^20 + log2 of the weight: the number's last word is the fraction of the logarithm, the first its whole part
+    const long long y = __double_as_longlong(fma((double)x - (double)r.top, r.step, 1572864.0));
+    const int hi = (int)(y >> 32), down = 0x41380000 - hi;                               // (a NaN, minus infinity: far outside)
+    const unsigned f = (unsigned)y;
+    const Power p = table[f >> (32 - kTableBits)];
+    constexpr float ln2 = 0.693147181f;
+    const float z = (float)(f & ((1u << (32 - kTableBits)) - 1)) * (ln2 * 0x1p-32f), e = fmaf(z * z, fmaf(z, 1.f / 6, 0.5f), z);        // 2^(rest) - 1 below 2^-8.5
+    const u64 m = (u64)(p.whole + __float2uint_rn(p.part * e)) << (r.bits - 29);         // twice the weight, before it is shifted down
+    const u64 w = ((m >> max(0, min(down, 63))) + 1) >> 1;
+    return x == r.top ? 1ull << r.bits : (unsigned)down < 64u ? w : 0;
 }
+// The same where it is not worth its code.
+__device__ __noinline__ u64 weight_apart(float x, const Row& r, const Power* table) { return weight(x, r, table); }
 // Bin of x, kBins or more where its weight is zero.
 __device__ __forceinline__ int bin_of(float x, const Row& r) {
     if (x == r.top) return 0;
@@ -127,107 +140,79 @@ __device__ __forceinline__ int bin_of(float x, const Row& r) {
     return f < (float)kBins ? (int)f : kBins;                                                // (a NaN: kBins)
 }
 
-template <int N> __device__ __forceinline__ void put(Bins<N>& h, unsigned at, u64 w, bool counts) {
-    if (counts) atomicAdd(h.count + at, 1u);
-    const unsigned low = (unsigned)w, old = atomicAdd(h.low + at, low), high = (unsigned)(w >> 32) + (old + low < low ? 1u : 0u);
-    if (high) atomicAdd(h.high + at, high);
+__device__ __forceinline__ u64 sum_of(unsigned a, unsigned b, unsigned c) { return a + ((u64)b << kPart) + ((u64)c << 2 * kPart); }
+__device__ __forceinline__ void put(Bins& h, unsigned at, u64 w) {
+    const unsigned a = (unsigned)w & ((1u << kPart) - 1), b = (unsigned)(w >> kPart) & ((1u << kPart) - 1), c = (unsigned)(w >> 2 * kPart);
+    if (a) atomicAdd(h.part[0] + at, a);
+    if (b) atomicAdd(h.part[1] + at, b);
+    if (c) atomicAdd(h.part[2] + at, c);
 }
 
-// The thread's bins (PER adjacent ones) of all CTAs of the cluster added up, and what lies above them.  The CTAs have met before.
-template <int PER> struct Sums {
-    unsigned n[PER];
-    u64 m[PER], count_before, mass_before, mass_all;
+// The sums of 32 bins each, by all warps.
+__device__ __forceinline__ void add_groups(const Bins& h, u64* groups) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int g = threadIdx.x >> 5; g < kBins / 32; g += kWarps) {
+        const u64 sum = warp_total(sum_of(h.part[0][32 * g + lane], h.part[1][32 * g + lane], h.part[2][32 * g + lane]));
+        if (lane == 0) groups[g] = sum;
+    }
+}
 
-    template <int N> __device__ __forceinline__ void add_up(Shared& s, const Bins<N>& mine, int ctas, bool counts) {
-        static_assert(N == PER * kThreads, "");
-        const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+// One warp of each CTA, when the CTAs have met: the first bin of all of them added up, from the top on, with which the sum (and what lies `above` all bins)
+// reaches its target, which may be a share of all, and the sum above it; -1 where it does not.  (Reading all bins of all CTAs instead, 96 KB each through the cluster's network, took 2.7 us.)
+template <typename Target> __device__ __forceinline__ void find(Shared& s, const Bins& h, const u64* groups, int ctas, u64 above, Target target_of) {
+    static_assert(kBins == 32 * 32, "");
+    const int lane = threadIdx.x & 31;
+    uint2 v[kMostCtas];
 #pragma unroll
-        for (int i = 0; i < PER; ++i) n[i] = 0, m[i] = 0;
-        if (ctas == 1) {
+    for (int r = 0; r < kMostCtas; ++r) v[r] = r < ctas ? ld_remote2(remote_of(groups + lane, r)) : make_uint2(0, 0);
+    u64 sum = 0;
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                n[i] = mine.count[tid * PER + i];
-                m[i] = ((u64)mine.high[tid * PER + i] << 32) + mine.low[tid * PER + i];
-            }
-        } else {
-            const int bin = tid * PER;
+    for (int r = 0; r < kMostCtas; ++r) sum += ((u64)v[r].y << 32) + v[r].x;
+    u64 to = above + warp_prefix(sum, lane);
+    const u64 all = __shfl_sync(0xffffffffu, to, 31), target = target_of(all);
+    if (lane == 0) { s.all = all; s.target = target; }
+    const unsigned hit = __ballot_sync(0xffffffffu, to >= target);
+    if (lane == 0) s.found = -1;
+    if (!hit) return;
+    const int g = __ffs(hit) - 1;
+    above = __shfl_sync(0xffffffffu, to - sum, g);
+    unsigned n[kMostCtas][3];
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {        // (all loads of four CTAs on their way at once)
-                uint2 c[4], l[4], h[4];
+    for (int r = 0; r < kMostCtas; ++r)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    c[r] = l[r] = h[r] = make_uint2(0, 0);
-                    if (4 * half + r >= ctas) continue;
-                    if constexpr (PER == 2) {
-                        if (counts) c[r] = ld_remote2(remote_of(mine.count + bin, 4 * half + r));
-                        l[r] = ld_remote2(remote_of(mine.low + bin, 4 * half + r));
-                        h[r] = ld_remote2(remote_of(mine.high + bin, 4 * half + r));
-                    } else {
-                        if (counts) c[r].x = ld_remote(remote_of(mine.count + bin, 4 * half + r));
-                        l[r].x = ld_remote(remote_of(mine.low + bin, 4 * half + r));
-                        h[r].x = ld_remote(remote_of(mine.high + bin, 4 * half + r));
-                    }
-                }
+        for (int i = 0; i < 3; ++i) n[r][i] = r < ctas ? ld_remote(remote_of(h.part[i] + 32 * g + lane, r)) : 0;
+    sum = 0;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    n[0] += c[r].x;
-                    m[0] += ((u64)h[r].x << 32) + l[r].x;
-                    if constexpr (PER == 2) { n[1] += c[r].y; m[1] += ((u64)h[r].y << 32) + l[r].y; }
-                }
-            }
-        }
-        u64 count = 0, mass = 0;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) { count += n[i]; mass += m[i]; }
-        const u64 count_to = counts ? warp_prefix(count, lane) : 0, mass_to = warp_prefix(mass, lane);
-        if (lane == 31) { s.scan_count[warp] = (unsigned)count_to; s.scan_mass[warp] = mass_to; }
-        if (tid == 0) s.found = -1;
-        __syncthreads();
-        count_before = count_to - count;
-        mass_before = mass_to - mass;
-        mass_all = 0;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            if (w < warp) { count_before += s.scan_count[w]; mass_before += s.scan_mass[w]; }
-            mass_all += s.scan_mass[w];
-        }
+    for (int r = 0; r < kMostCtas; ++r) sum += sum_of(n[r][0], n[r][1], n[r][2]);
+    to = above + warp_prefix(sum, lane);
+    const unsigned in = __ballot_sync(0xffffffffu, to >= target);
+    if (lane == __ffs(in) - 1) {
+        s.found = 32 * g + lane;
+        s.found_above = to - sum;
     }
-    // The first bin, from the top on, with which count or mass (and what lies `above` all of them) reaches its target, with what lies above it among
-    // the bins, in `s`; s.found is -1 on entry and where there is none.
-    __device__ __forceinline__ void find(Shared& s, bool by_count, u64 target, u64 above) const {
-        u64 count_to = count_before, mass_to = mass_before;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const u64 before = above + (by_count ? count_to : mass_to), after = before + (by_count ? n[i] : m[i]);
-            if (before < target && after >= target) {
-                s.found = threadIdx.x * PER + i;
-                s.found_count = (unsigned)count_to;
-                s.found_mass = mass_to;
-            }
-            count_to += n[i];
-            mass_to += m[i];
-        }
-        __syncthreads();
-    }
-};
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 2)
-sample_kernel(const __grid_constant__ b200gptq_sample_args a, int slice, int cluster_bits, int bits) {
+sample_kernel(const __grid_constant__ b200gptq_sample_args a, int slice, int cluster_bits, int bits, int room) {
     extern __shared__ __align__(16) unsigned char smem[];
     Shared& s = *reinterpret_cast<Shared*>(smem);
-    T* x = reinterpret_cast<T*>(smem + (sizeof(Shared) + 15) / 16 * 16);
+    T* x = reinterpret_cast<T*>(smem + (sizeof(Shared) + 15) / 16 * 16);                  // the slice, later what each warp has kept of its run of it
+    unsigned short* places = reinterpret_cast<unsigned short*>(x + slice);                // and where that stood in the run (where there is room for both)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, ctas = 1 << cluster_bits, row = blockIdx.x >> cluster_bits, rank = blockIdx.x & (ctas - 1);
     const int base = min(rank * slice, a.vocab), n = min(slice, a.vocab - base);
     // A warp's tokens: a run of the slice
     const int run = (slice + kWarps - 1) / kWarps, first = min(warp * run, n), last = min(first + run, n);
-    static_assert(offsetof(Shared, fine) == sizeof(Bins<kBins>), "");
-    for (int i = tid; i < kBins * 3 + 2 * kFine * 3; i += kThreads) reinterpret_cast<unsigned*>(&s.bins)[i] = 0;
+    for (int i = tid; i < (int)sizeof(s.bins) / 16; i += kThreads) reinterpret_cast<uint4*>(s.bins)[i] = make_uint4(0, 0, 0, 0);
     auto meet = [&] {
         if (ctas > 1) cluster_sync();
         else __syncthreads();
     };
-    if (tid < kTable) s.table[tid] = exp2((double)tid / kTable);
+    if (tid < kTable) {
+        const double power = exp2(30 + (double)tid / kTable);
+        s.table[tid] = {(unsigned)__double2uint_rn(power), (float)power};
+    }
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride + base;
@@ -271,166 +256,220 @@ sample_kernel(const __grid_constant__ b200gptq_sample_args a, int slice, int clu
     }
     r.bits = bits;
     const bool greedy = !(temperature >= kColdest) || top_k == 1 || min_p > 1.f || r.top == -INFINITY;
-    r.step = greedy ? 0.0 : 64 * 1.4426950408889634074 / (double)temperature;
-    r.half_scale = (float)(r.step * (2.0 * kBins / 64) / (bits + 1));
+    r.step = greedy ? 0.0 : 1.4426950408889634074 / (double)temperature;
+    r.half_scale = (float)(r.step * (2.0 * kBins) / (bits + 1));
     // ---- the border: tokens of larger keys are kept, and of those at it the first `ties` ----
-    unsigned border = 0, ties = 0xffffffffu;
-    if (greedy) {
-        border = key_of(r.top);
-        ties = 1;
-    } else if (top_k > 0 || top_p < 1.f) {
-        const bool counts = top_k > 0;
+    enum { kNumber, kWeight, kKept };            // tokens into bins, for top-k; weights into bins, for top-p; sums of what is kept
+    unsigned border = greedy ? key_of<T>(r.top) : 0, ties = greedy ? 1 : 0xffffffffu, lo = 0, hi = 0xffffffffu;
+    int mode = greedy ? kKept : top_k > 0 ? kNumber : top_p < 1.f ? kWeight : kKept, bin = -1, shift = 0, turn = 0;        // bin -1: by the logarithm
+    u64 above = 0, target = (u64)top_k;
+    bool cut = false, moved = false;
+    const u64 least = share(min_p, 1ull << bits, true);
+    // (what min-p leaves out has a smaller key than all that it keeps)
+    auto keeps = [&](float v, u64 w) { return w >= least || v == r.top ? w : 0; };
+    Warp mine = {0, 0, 0};
+    const T* run_x = x + first;
+    int many = last - first;                     // of the warp's run
+    while (mode != kKept) {
+        Bins& h = s.bins[turn];
+        if (bin < 0 && mode == kNumber) {
 #pragma unroll 4
-        for (int i = first + lane; i < last; i += 32) {
-            const float v = wide(x[i]);
-            const int bin = bin_of(v, r);
-            if (bin < kBins) put(s.bins, bin, weight(v, r, s.table), counts);
-        }
-        meet();
-        Sums<kBins / kThreads> whole;
-        whole.add_up(s, s.bins, ctas, counts);
-        int level = 0;
-        u64 above_count = 0, above_mass = 0;
-        // The value of x at which the first `target` tokens (by_count), or the shortest beginning that weighs `target`, end, and what lies above it
-        auto search = [&](bool by_count, u64 target, unsigned& key) {
-            whole.find(s, by_count, target, 0);
-            const int bin = s.found;
-            if (bin < 0) return false;
-            above_count = s.found_count;
-            above_mass = s.found_mass;
-            // The keys of that bin lie between those of its ends, a little further out (rounding of bin_of)
-            const double unit = 64.0 * (bits + 1) / kBins / r.step;
-            const float far = fmaxf((float)((double)r.top - (bin + 1.01) * unit), -3.4028235e38f), near = bin == 0 ? r.top : (float)((double)r.top - (bin - 0.01) * unit);
-            unsigned lo = key_of(far) > 2 ? key_of(far) - 2 : 0, hi = max(key_of(fminf(near, r.top)), 3u) + (bin == 0 ? 0 : 2);
-            int shift;
-            do {
-                shift = max(0, 32 - __clz(hi - lo) - kFineBits);
-                Bins<kFine>& h = s.fine[level & 1];
-#pragma unroll 4
-                for (int i = first + lane; i < last; i += 32) {
-                    const float v = wide(x[i]);
-                    const unsigned k = key_of(v);
-                    if (k >= lo && k <= hi && bin_of(v, r) == bin) put(h, (hi - k) >> shift, weight(v, r, s.table), counts);
-                }
-                meet();
-                // (the other one has been read by all: it was added up before they met)
-                ++level;
-                for (int i = tid; i < kFine * 3; i += kThreads) reinterpret_cast<unsigned*>(s.fine + (level & 1))[i] = 0;
-                Sums<kFine / kThreads> part;
-                part.add_up(s, h, ctas, counts);
-                part.find(s, by_count, target, by_count ? above_count : above_mass);
-                above_count += s.found_count;
-                above_mass += s.found_mass;
-                hi -= (unsigned)s.found << shift;
-                lo = max(lo, hi - ((1u << shift) - 1));
-                __syncthreads();         // (what was found has been read)
-                if (tid == 0) s.found = -1;
-            } while (shift > 0);
-            __syncthreads();
-            key = hi;
-            return true;
-        };
-        u64 sum = whole.mass_all;        // of what top-k keeps
-        const bool cut = top_k > 0 && search(true, (u64)top_k, border);
-        if (cut) {
-            ties = (unsigned)(top_k - above_count);
-            sum = above_mass + ties * weight(of_key(border), r, s.table);
-        }
-        if (top_p < 1.f) {
-            u64 target = share(top_p, sum, true);
-            if (target == 0) target = 1;
-            unsigned key = 0;
-            if (search(false, target, key)) {
-                const u64 w = weight(of_key(key), r, s.table), need = (target - above_mass + w - 1) / w;
-                ties = key == border && cut ? min(ties, (unsigned)need) : (unsigned)need;
-                border = key;
+            for (int i = lane; i < many; i += 32) {
+                const int at = bin_of(wide(run_x[i]), r);
+                if (at < kBins) atomicAdd(h.part[0] + at, 1u);
             }
+        } else if (bin < 0) {
+#pragma unroll 4
+            for (int i = lane; i < many; i += 32) {
+                const float v = wide(run_x[i]);
+                const int at = bin_of(v, r);
+                put(h, min(at, kBins - 1), at < kBins && key_of<T>(v) > border ? weight(v, r, s.table) : 0);
+            }
+        } else {
+            for (int i = lane; i < many; i += 32) {
+                const float v = wide(run_x[i]);
+                const unsigned k = key_of<T>(v);
+                if (k > border && k >= lo && k <= hi && bin_of(v, r) == bin) put(h, (hi - k) >> shift, mode == kNumber ? 1 : weight_apart(v, r, s.table));
+            }
+        }
+        __syncthreads();
+        add_groups(h, s.groups[turn]);
+        meet();
+        // (the last turn's bins have been read by all: before they met)
+        const int last_turn = turn == 0 ? 2 : turn - 1;
+        if (warp == 0) {
+            find(s, h, s.groups[turn], ctas, bin < 0 ? 0 : above, [&](u64 sum) {
+                if (mode != kWeight || bin >= 0) return target;
+                // (of all, or of what top-k keeps; one token at least)
+                return max(share(top_p, cut ? sum + ties * weight_apart(of_key<T>(border), r, s.table) : sum, true), (u64)1);
+            });
+        } else {
+            for (int i = tid - 32; i < (int)sizeof(Bins) / 16; i += kThreads - 32) reinterpret_cast<uint4*>(s.bins + last_turn)[i] = make_uint4(0, 0, 0, 0);
+        }
+        turn = turn == 2 ? 0 : turn + 1;
+        __syncthreads();
+        const int found = s.found;
+        const u64 all = s.all;
+        target = s.target;
+        if (found >= 0) above = s.found_above;
+        __syncthreads();                         // (what was found has been read)
+        if (found >= 0) {
+            if (bin < 0) {
+                // The keys of that bin lie between those of its ends, a little further out (rounding of bin_of)
+                bin = found;
+                const double unit = (double)(bits + 1) / kBins / r.step;
+                const float far = fmaxf((float)((double)r.top - (bin + 1.01) * unit), -3.4028235e38f), near = bin == 0 ? r.top : (float)((double)r.top - (bin - 0.01) * unit);
+                lo = key_of<T>(far) > 2 ? key_of<T>(far) - 2 : 0;
+                hi = max(key_of<T>(fminf(near, r.top)), 3u) + (bin == 0 ? 0 : 2);
+                shift = max(0, 32 - __clz(hi - lo) - kBinBits);
+                if (!moved && room) {            // nothing below the keys of this bin will be kept: the others move to the front of the run
+                    int held = 0;
+                    for (int i0 = 0; i0 < many; i0 += 32) {
+                        const int i = i0 + lane;
+                        const T v = i < many ? run_x[i] : T(0.f);
+                        const bool in = i < many && key_of<T>(wide(v)) >= lo;
+                        const unsigned whom = __ballot_sync(0xffffffffu, in);
+                        __syncwarp();
+                        const int to = held + __popc(whom & ((1u << lane) - 1));
+                        if (in) { x[first + to] = v; places[first + to] = (unsigned short)i; }
+                        held += __popc(whom);
+                        __syncwarp();
+                    }
+                    many = held;
+                    moved = true;
+                }
+                continue;
+            }
+            hi -= (unsigned)found << shift;
+            lo = max(lo, hi - ((1u << shift) - 1));
+            if (shift > 0) {
+                shift = max(0, 32 - __clz(hi - lo) - kBinBits);
+                continue;
+            }
+        }
+        // ---- a search has ended, at the value of key hi ----
+        if (mode == kNumber) {
+            if (found >= 0) {                    // (else top-k keeps all that have a weight)
+                cut = true;
+                border = hi;
+                ties = (unsigned)(top_k - above);
+            }
+            mode = top_p < 1.f ? kWeight : kKept;
+            bin = -1;
+        } else {
+            if (found >= 0) {
+                const u64 w = weight_apart(of_key<T>(hi), r, s.table);
+                border = hi;
+                ties = (unsigned)((target - above + w - 1) / w);
+            } else {                             // among those at top-k's border
+                const u64 w = weight_apart(of_key<T>(border), r, s.table);
+                ties = min(ties, (unsigned)((target - all + w - 1) / w));
+            }
+            mode = kKept;
         }
     }
     // ---- sums of the kept tokens by warp, in the vocabulary's order ----
-    const u64 least = share(min_p, 1ull << bits, true);
-    // (what min-p leaves out has a smaller key than all that it keeps)
-    auto kept_weight = [&](float v) { const u64 w = greedy ? 1 : weight(v, r, s.table); return w >= least || v == r.top ? w : 0; };
-    Warp mine = {0, 0, 0};
-#pragma unroll 4
-    for (int i = first + lane; i < last; i += 32) {
-        const float v = wide(x[i]);
-        const unsigned k = key_of(v);
-        if (k > border) mine.mass += kept_weight(v);
-        else if (k == border) ++mine.ties;
+#pragma unroll 2
+    for (int i = lane; i < many; i += 32) {
+        const float v = wide(run_x[i]);
+        const unsigned k = key_of<T>(v);
+        const u64 w = greedy ? 1 : weight(v, r, s.table);
+        if (k > border) mine.mass += keeps(v, w);
+        if (k == border) ++mine.ties;
     }
     mine.mass = warp_total(mine.mass);
     mine.ties = warp_total(mine.ties);
     if (lane == 0) s.warps[warp] = mine;
     meet();
-    const u64 border_w = border ? kept_weight(of_key(border)) : 0;
-    // every warp looks at all warps of the cluster, 32 at a time: those before it, and all
-    u64 before = 0, total = 0;
-    unsigned ties_before = 0, ties_all = 0;
-    for (int w0 = 0; w0 < ctas * kWarps; w0 += 32) {
-        const int w = w0 + lane;
-        Warp other = {0, 0, 0};
-        if (w < ctas * kWarps) {
-            if (ctas > 1) {
-                const uint32_t at = remote_of(s.warps + (w % kWarps), w / kWarps);
-                const uint2 mass = ld_remote2(at);
-                other.mass = (u64)mass.y << 32 | mass.x;
-                other.ties = ld_remote(at + 8);
-            } else {
-                other = s.warps[w];
-            }
+    auto kept_weight = [&](float v) { return keeps(v, greedy ? 1 : weight_apart(v, r, s.table)); };
+    const u64 border_w = border ? kept_weight(of_key<T>(border)) : 0;
+    // ---- warp 0 of each CTA looks for the warp of the cluster that has the token; lane l has kPer warps in their order ----
+    constexpr int kPer = kMostCtas * kWarps / 32;
+    if (warp == 0) {
+        uint4 v[kPer];
+        unsigned lane_ties = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int w = kPer * lane + i;
+            v[i] = make_uint4(0, 0, 0, 0);
+            if (w < ctas * kWarps) v[i] = ld_remote4(remote_of(s.warps + w % kWarps, w / kWarps));
+            lane_ties += v[i].z;
         }
-        const u64 to = ties_all + warp_prefix((u64)other.ties, lane);
-        const u64 taken = min(to, (u64)ties) - min(to - other.ties, (u64)ties);
-        const u64 mass = other.mass + taken * border_w;
-        const bool earlier = w < rank * kWarps + warp;
-        before += warp_total(earlier ? mass : 0);
-        total += warp_total(mass);
-        ties_before += warp_total(earlier ? other.ties : 0u);
-        ties_all += warp_total(other.ties);
+        unsigned to = warp_prefix(lane_ties, lane) - lane_ties;          // (equal tokens before)
+        u64 mass[kPer], sum = 0;
+        unsigned ties_to[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            ties_to[i] = to;
+            to += v[i].z;
+            mass[i] = ((u64)v[i].y << 32) + v[i].x + (u64)(min(to, ties) - min(ties_to[i], ties)) * border_w;
+            sum += mass[i];
+        }
+        u64 before = warp_prefix(sum, lane);
+        const u64 total = __shfl_sync(0xffffffffu, before, 31);
+        before -= sum;
+        u64 target = share(u, total, false);
+        if (total > 0 && target >= total) target = total - 1;
+        if (lane == 0) s.owner = -1;
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            if (target >= before && target < before + mass[i]) {
+                s.owner = kPer * lane + i;
+                s.before = before;
+                s.ties_before = ties_to[i];
+                s.found_above = target;
+            }
+            before += mass[i];
+        }
     }
-    if (ctas > 1) cluster_sync();                 // (nobody leaves while others read)
-    u64 target = share(u, total, false);
-    if (total > 0 && target >= total) target = total - 1;
-    if (total == 0) {                             // nothing to choose from
+    meet();                                       // (nobody leaves while others read)
+    if (s.owner < 0) {                            // nothing to choose from
         if (rank == 0 && tid == 0) a.out[row] = 0;
         return;
     }
-    const u64 own = mine.mass + (min((u64)ties_before + mine.ties, (u64)ties) - min((u64)ties_before, (u64)ties)) * border_w;
-    if (target < before || target >= before + own) return;
-    // ---- this warp's run has the token: a run of it per lane, then that one again, a token per lane ----
-    int begin = first, end = last;
-    unsigned at_border = ties_before;
-    while (true) {
-        const int each = (end - begin + 31) / 32, from = min(begin + lane * each, end), to = min(from + each, end);
-        u64 mass = 0;
-        unsigned mine_ties = 0;
-        for (int i = from; i < to; ++i) {
-            const float v = wide(x[i]);
-            const unsigned k = key_of(v);
-            if (k > border) mass += kept_weight(v);
-            else if (k == border) ++mine_ties;
+    if (s.owner != rank * kWarps + warp) return;
+    // ---- this warp's run has the token: what is kept, 32 at a time, in order ----
+    u64 before = s.before;
+    target = s.found_above;
+    unsigned at_border = s.ties_before;
+    int* next = reinterpret_cast<int*>(s.bins) + warp * 64;                   // (the bins are done with)
+    int held = 0;
+    for (int i0 = 0; i0 < many || held > 0; i0 += 32) {
+        const int i = i0 + lane;
+        const unsigned k = i < many ? key_of<T>(wide(run_x[i])) : 0;
+        const unsigned tie = __ballot_sync(0xffffffffu, i < many && k == border), earlier = (1u << lane) - 1;
+        const bool in = i < many && (k > border || (k == border && at_border + __popc(tie & earlier) < ties));
+        at_border += __popc(tie);
+        const unsigned whom = __ballot_sync(0xffffffffu, in);
+        if (in) next[held + __popc(whom & earlier)] = i;
+        held += __popc(whom);
+        __syncwarp();
+        if (held < 32 && i0 + 32 < many) continue;
+        const int now = min(held, 32), place = lane < now ? next[lane] : -1, rest = next[32 + lane];
+        __syncwarp();
+        const u64 to = before + warp_prefix(place >= 0 ? kept_weight(wide(run_x[place])) : 0, lane);
+        const unsigned hit = __ballot_sync(0xffffffffu, target < to);
+        if (hit) {
+            if (lane == __ffs(hit) - 1) a.out[row] = base + first + (moved ? (int)places[first + place] : place);
+            return;
         }
-        const unsigned ties_to = at_border + warp_prefix(mine_ties, lane);
-        mass += (u64)(min(ties_to, ties) - min(ties_to - mine_ties, ties)) * border_w;
-        const u64 to_here = before + warp_prefix(mass, lane);
-        const unsigned hit = __ballot_sync(0xffffffffu, target < to_here);
-        const int who = __ffs(hit) - 1;
-        begin = __shfl_sync(0xffffffffu, from, who);
-        end = __shfl_sync(0xffffffffu, to, who);
-        before = __shfl_sync(0xffffffffu, to_here - mass, who);
-        at_border = __shfl_sync(0xffffffffu, ties_to - mine_ties, who);
-        if (end - begin <= 1) break;
+        before = __shfl_sync(0xffffffffu, to, 31);
+        held -= now;
+        if (lane < held) next[lane] = rest;
+        __syncwarp();
     }
-    if (lane == 0) a.out[row] = base + begin;
 }
+
+constexpr size_t kMostShared = 227 * 1024;
+size_t shared_bytes(int slice, size_t size) { return (sizeof(Shared) + 15) / 16 * 16 + slice * size; }
 
 template <typename T>
 int launch(const b200gptq_sample_args& a, cudaStream_t stream) {
-    // CTAs per row: as many as the SMs hold three of, a slice of 1024 tokens or more, and enough that a slice leaves an SM room for three (51 KB; what eight cannot
-    // hold so takes more).
+    // CTAs per row: as many as the SMs hold two of, a slice of 1024 tokens or more, and enough that a slice leaves an SM room for two (what eight cannot hold so
+    // takes more)
     int cluster_bits = 0;
-    while (cluster_bits < 3 && ((long long)a.rows << (cluster_bits + 1) <= 3LL * sm_count() || (long long)a.vocab * sizeof(T) > 51200LL << cluster_bits) &&
+    while (cluster_bits < 3 && ((long long)a.rows << (cluster_bits + 1) <= 2LL * sm_count() || shared_bytes((a.vocab >> cluster_bits) + 8, sizeof(T) + sizeof(unsigned short)) > 113 * 1024) &&
            a.vocab >> (cluster_bits + 1) >= 1024)
         ++cluster_bits;
     // (slices begin at multiples of 16 bytes)
@@ -438,7 +477,9 @@ int launch(const b200gptq_sample_args& a, cudaStream_t stream) {
     int log2v = 0;
     while (1 << log2v < a.vocab) ++log2v;
     const int bits = 62 - log2v < 49 ? 62 - log2v : 49;
-    const size_t smem = (sizeof(Shared) + 15) / 16 * 16 + (size_t)slice * sizeof(T);
+    // (a vocabulary near 2^18 in fp32 leaves no room to move tokens together)
+    const bool room = shared_bytes(slice, sizeof(T) + sizeof(unsigned short)) <= kMostShared;
+    const size_t smem = shared_bytes(slice, sizeof(T) + (room ? sizeof(unsigned short) : 0));
     static const bool pdl = [] {
         const char* e = std::getenv("B200GPTQ_PDL");
         return !(e && e[0] == '0');
@@ -449,7 +490,7 @@ int launch(const b200gptq_sample_args& a, cudaStream_t stream) {
     B200GPTQ_CUDA_TRY(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64) return B200GPTQ_ERR_TOO_LARGE;
     auto* kernel = sample_kernel<T>;
-    std::call_once(once[dev], [&] { result[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)((sizeof(Shared) + 15) / 16 * 16 + 128 * 1024 + 64)); });
+    std::call_once(once[dev], [&] { result[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostShared); });
     B200GPTQ_CUDA_TRY(result[dev]);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)a.rows << cluster_bits);
@@ -471,7 +512,7 @@ int launch(const b200gptq_sample_args& a, cudaStream_t stream) {
     }
     cfg.attrs = attr;
     cfg.numAttrs = n;
-    B200GPTQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a, slice, cluster_bits, bits));
+    B200GPTQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a, slice, cluster_bits, bits, room ? 1 : 0));
     return B200GPTQ_OK;
 }
 
