@@ -37,7 +37,7 @@ Attn4Plan plan_of(const b200gptq_attn_cache_args& a) {
 
 int64_t scratch_bytes(const b200gptq_attn_cache_args& a, const Attn4Plan& p) {
     if (p.read) return (int64_t)a.cache.batch * a.cache.kv_heads * a.cache.max_seq * a.cache.hd * 4;
-    return p.flat ? 2LL * p.ctas * 8 * p.tiles8 * (a.cache.hd + 2) * (int)sizeof(float) : 0;
+    return p.flat ? 2LL * kAttn4Warps * p.ctas * 8 * p.tiles8 * (a.cache.hd + 2) * (int)sizeof(float) : 0;
 }
 
 }  // namespace
@@ -66,6 +66,9 @@ B200GPTQ_API int b200gptq_attn_cache(const b200gptq_attn_cache_args* args, void*
     uintptr_t bits = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out);
     for (int i = 0; i < 3; ++i) bits |= (uintptr_t)(2 * (a.q_stride[i] | a.out_stride[i]));
     if (bits & 15u) return B200GPTQ_ERR_ALIGNMENT;
+    // (the rows kernel multiplies rows and their steps, in bytes, in 32 bits each)
+    for (int64_t step : {a.cache.k_stride[2], a.cache.v_stride[2], 2 * a.cache.k_scale_stride[2], 2 * a.cache.v_scale_stride[2]})
+        if (step < 0 || step > 0xffffffffLL) return B200GPTQ_ERR_TOO_LARGE;
     if ((reinterpret_cast<uintptr_t>(a.pos) | reinterpret_cast<uintptr_t>(a.counts)) & 7u || reinterpret_cast<uintptr_t>(a.status) & 3u) return B200GPTQ_ERR_ALIGNMENT;
     if (need && (!workspace || workspace_bytes < (size_t)need)) return B200GPTQ_ERR_WORKSPACE;
     if (reinterpret_cast<uintptr_t>(workspace) & 15u) return B200GPTQ_ERR_ALIGNMENT;

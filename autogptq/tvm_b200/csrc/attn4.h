@@ -7,6 +7,7 @@
 namespace b200gptq {
 
 constexpr int kAttn4MaxSplit = 8;        // CTAs of a cluster
+constexpr int kAttn4Warps = 8;           // of a CTA; each has scratch for two (sequence, key head, tile of rows) that it does a part of
 
 // The queries, positions and sizes as b200gptq_attn has them (without caches), and the cache.
 struct Attn4Args {
@@ -16,7 +17,7 @@ struct Attn4Args {
 struct Attn4Divisors { Divisor row_tiles, kv_heads, group; };
 
 // How a call is carried out.  read: the rows that are seen are read back into scratch and the tcgen05 kernel of b200gptq_attn takes them.  Otherwise the rows kernel, with
-// 8 * tiles8 rows of Q per tile, FLAT over `ctas` CTAs or with 2^split_bits CTAs for each tile.
+// 8 * tiles8 rows of Q per tile, with even runs of all keys for the warps of `ctas` CTAs (flat) or with 2^split_bits CTAs for each tile.
 struct Attn4Plan { bool read, flat; int tiles8, split_bits, ctas; };
 
 int attn4_rows_dispatch(const Attn4Args& a, float* part, const Attn4Plan& p, cudaStream_t stream);

@@ -5,18 +5,21 @@
 // A row of the cache is 68 to 80 bytes for 128 dims and has to be multiplied by up to 8, 16 or 32 rows of Q, so bytes and instructions bound it alike, and the codes go
 // to the tensor cores as they are: a field of four bits that is masked in place, at bits 0 .. 3 or 4 .. 7 of 16, is the fp16 number c 2^-24 or 16 c 2^-24 (subnormal,
 // exact), so eight codes cost a shift and four masks.  Scales and zeros are applied beside the products:
-//   S(key, row) = sum over groups of  sK (q . cK) + zK (sum of q)      one product chain per group, then two fp32 FMAs
+//   S(key, row) = sum over groups of  sK (q . cK) + zK (sum of q)      one product chain per group, then an fp32 FMA; the zeros in a product of their own, with
+//                                                                      the sums of q in two numbers each (16 bits or more together)
 //   O(dim, row) = sum over keys of  (w sV) cV + w zV                   w sV is what is rounded to fp16; w zV is summed in fp32, per group
 // Q is scaled by a power of two per row (to below 2^15, exact for what is above 2^-38 of the row's largest; so bf16 queries are exact in fp16), w sV by one per
 // warp that follows the largest scale seen, so neither leaves fp16's range.
 //
-// Every warp takes blocks of 16 keys on its own, through a ring of cp.async stages in shared memory.  Keys are the 16 of m16n8k16, rows the 8: 8 bytes (128
+// Every warp takes parts of 16 keys on its own, through a ring of cp.async stages in shared memory.  Keys are the 16 of m16n8k16, rows the 8: 8 bytes (128
 // dims: 16) of a key are the operand of S as they lie, two keys' words paired by byte permutations that of O (include/b200gptq.h has the order of the codes).
 // Rows are only rescaled when a score is more than 2^8 above the maximum in use (no weight is above 2^8; fp32 sums).
 //
-// FLAT: the blocks of all sequences and key heads lie one behind the other, and each CTA takes an even run of them, whatever the texts' lengths, which are known
-// on the device only.  Where a run ends inside a (sequence, key head) the sums go to scratch, and a second launch adds them up in order.
-// Otherwise a cluster of 1 to 8 CTAs shares a (sequence, key head), and they add up through distributed shared memory.
+// attn4_cluster_kernel: a cluster of 1 to 8 CTAs shares a (sequence, key head, tile of rows), and they add up through distributed shared memory.
+// attn4_flat_kernel: for long caches.  The parts of all sequences and key heads lie one behind the other, and each WARP takes an even run of them, whatever the texts'
+// lengths, which are known on the device only.  Where a run ends inside a (sequence, key head) the sums go to scratch, and a second launch adds them up in
+// order.  (A run for each CTA, whose warps shared a sequence's part of it: 16 texts of 900 to 15900 tokens, 32 / 8 heads, 66 us and SMs idle for a quarter of it, at the ends
+// of sequences and at the end.)
 #include <algorithm>
 #include <mutex>
 #include <type_traits>
@@ -27,13 +30,26 @@
 namespace b200gptq {
 namespace {
 
-constexpr int kBlock = 16, kWarps = 8, kThreads = kWarps * 32, kStages = 4;
+constexpr int kPart = 16, kWarps = kAttn4Warps, kThreads = kWarps * 32, kStages = 4;
 constexpr float kGrow = 8.f;             // log2 of what a score may be above the maximum in use
 constexpr unsigned kLow = 0x000f000fu, kHigh = 0x00f000f0u;
 
 __device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The same without a sum before it.
+__device__ __forceinline__ void mma16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+template <typename T> __device__ __forceinline__ void mma8_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+    if constexpr (std::is_same<T, __half>::value)
+        asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(b0), "f"(0.f));
+    else
+        asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(b0), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {      // of an 8 x 8 matrix of 16-bit values, a pair of a row per lane
     uint32_t r;
@@ -58,85 +74,367 @@ template <int N> __device__ __forceinline__ Words<N> lds(uint32_t at) {
     return r;
 }
 
-// One block of 16 keys in shared memory, in bytes: codes of K as they lie; codes of V, 16 bytes at a time, where each 128 bytes (2 or 4 rows) are permuted so that
+// A part in shared memory, in bytes: codes of K as they lie; codes of V, 16 bytes at a time, where each 128 bytes (2 or 4 rows) are permuted so that
 // the lanes of a load (rows 2c) meet no bank twice; constants of K and of V.
 template <int HD, int GS> struct Stage {
-    static constexpr int row = HD / 2, groups = HD / GS, constants = 4 * groups, k = 0, v = kBlock * row, kc = 2 * kBlock * row, vc = kc + kBlock * constants,
-                         total = vc + kBlock * constants;
-    __device__ static __forceinline__ int v_at(int r, int byte) {
+    static constexpr int row = HD / 2, groups = HD / GS, constants = 4 * groups, k = 0, v = kPart * row, kc = 2 * kPart * row, vc = kc + kPart * constants,
+                         total = vc + kPart * constants;
+    __host__ __device__ static constexpr int v_at(int r, int byte) {
         const int line = r * row / 128, chunk = (r * row % 128 + byte) / 16;
         return v + line * 128 + ((chunk ^ (2 * (line & (HD == 128 ? 3 : 1)))) * 16 + byte % 16);
     }
 };
 
-// Shared memory, in floats: the ring [warp][stage], over which the warps' sums [warp][row][HD + 4] come to lie; their maxima and denominators; the slices that the
-// CTAs of the cluster push [split][row][HD / splits] with maxima and denominators; a flag per row; the rows' places (q, out); sums of q by group and row, factor of a
-// row; the operand made of Q.
+// Shared memory, in floats.  A warp's ring, and with 32 rows its operand made of Q, which registers do not hold (a slot for each lane).  attn4_cluster_kernel, over the
+// rings: the warps' sums [warp][row][HD + 4]; behind them their maxima and denominators, the slices that the CTAs of the cluster push [split][row][HD / splits] with maxima
+// and denominators, a flag per row.
 template <int HD, int GS, int NT> struct Lay {
-    static constexpr int R = 8 * NT, LD = HD + 4, ring = kWarps * kStages * Stage<HD, GS>::total / 4, sums = kWarps * R * LD, ml = ring > sums ? ring : sums,
-                         slice = ml + 2 * kWarps * R, slice_ml = slice + R * HD, flags = slice_ml + 2 * kAttn4MaxSplit * R, places = flags + R, qsum = places + 4 * R,
-                         factor = qsum + 4 * R, where = factor + R, q = where + 8, total = q + NT * (HD / 32) * 32 * 4;
-    static_assert(places % 2 == 0 && q % 4 == 0 && slice % 4 == 0, "");
+    static constexpr int R = 8 * NT, LD = HD + 4, q = kStages * Stage<HD, GS>::total / 4, warp = q + (NT == 4 ? NT * (HD / 32) * 32 * 4 : 0), rings = kWarps * warp,
+                         sums = kWarps * R * LD, ml = rings > sums ? rings : sums, slice = ml + 2 * kWarps * R, slice_ml = slice + R * HD,
+                         flags = slice_ml + 2 * kAttn4MaxSplit * R, total = flags + R;
+    static_assert(slice % 4 == 0 && q % 4 == 0 && warp % 4 == 0, "");
 };
 
-// Blocks of a sequence: those that its tokens see between them; one at least where there are tokens, since their rows get zeros when they see nothing.
+// Parts of a sequence: those that its tokens see between them; one at least where there are tokens, since their rows get zeros when they see nothing.
 struct Span { AttnRange range; int p0, count, n_s, nb; };
 __device__ __forceinline__ Span span_of(const Attn4Args& a, int b) {
     Span s;
     s.p0 = attn_pos(a.attn, b);
     s.count = attn_count(a.attn, b);
     s.range = attn_range(s.p0, s.p0 + max(s.count, 1) - 1, a.attn.window ? a.attn.window : 1 << 30, a.attn.sinks, a.attn.max_seq);
-    s.n_s = (s.range.s_end + kBlock - 1) / kBlock;
-    s.nb = s.count ? max(1, s.n_s + (s.range.w_end - s.range.w_start + kBlock - 1) / kBlock) : 0;
+    s.n_s = (s.range.s_end + kPart - 1) / kPart;
+    s.nb = s.count ? max(1, s.n_s + (s.range.w_end - s.range.w_start + kPart - 1) / kPart) : 0;
     return s;
 }
-// Of the CTAs of a FLAT launch, number i begins with block total * i / ctas.
-__device__ __forceinline__ long long flat_begin(long long total, int i, int ctas) { return total * i / ctas; }
 
-// The sequence in which block `at` of the flat order lies, and the block with which that sequence begins; the total where at < 0.  All threads of a CTA
-// call it; `where` has room for 8 floats.
-struct Found { int b; long long begin, total; };
-__device__ Found flat_find(const Attn4Args& a, int units, int cta, int ctas, long long offset, long long* where) {
-    __shared__ long long scan[kWarps + 1];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    Found f = {0, 0, 0};
-    for (int b = threadIdx.x; b < a.attn.batch; b += kThreads) f.total += (long long)span_of(a, b).nb * units;
+// What a warp does: parts first, first + step .. below last of a (sequence, key head, tile of rows).
+struct Job { int b, kh, row0, nrows, first, last, step; };
+
+// A warp's sums: of rows 8 t + 2 c and + 1; O without the zeros, in units of limit 2^-24 (dims 64 h + 32 y + 4 g + {0, 2} in acc[4 h + 2 y], {1, 3} in the next), and what the zeros
+// add, by group, of the lane's keys.
+template <int HD, int GS, int NT> struct Sums {
+    static constexpr int HH = HD / 64, NG = HD / GS;
+    float acc[NT][4 * HH][4], zacc[NT][2][NG], m[NT][2], l[NT][2], limit;
+
+    // The lanes' shares of denominators and zeros added up.
+    __device__ __forceinline__ void settle_lanes() {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) f.total += __shfl_xor_sync(0xffffffffu, f.total, o);
-    if (lane == 0) scan[warp] = f.total;
-    __syncthreads();
-    f.total = 0;
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) f.total += scan[w];
-    __syncthreads();
-    const long long at = flat_begin(f.total, cta, ctas) + offset;
-    if (threadIdx.x == 0) { where[0] = -1; where[1] = 0; }
-    long long before = 0;
-    for (int b0 = 0; b0 < a.attn.batch; b0 += kThreads) {
-        const int b = b0 + threadIdx.x;
-        const long long mine = b < a.attn.batch ? (long long)span_of(a, b).nb * units : 0;
-        long long sum = mine;
+            for (int r = 0; r < 2; ++r)
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long x = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += x;
-        }
-        if (lane == 31) scan[warp] = sum;
-        __syncthreads();
-        long long lower = before, all = before;
+                for (int o = 4; o < 32; o <<= 1) {
+                    l[t][r] += __shfl_xor_sync(0xffffffffu, l[t][r], o);
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            if (w < warp) lower += scan[w];
-            all += scan[w];
-        }
-        if (at >= lower + sum - mine && at < lower + sum) { where[0] = b; where[1] = lower + sum - mine; }
-        before = all;
-        __syncthreads();
-        if (before > at) break;
+                    for (int n = 0; n < NG; ++n) zacc[t][r][n] += __shfl_xor_sync(0xffffffffu, zacc[t][r][n], o);
+                }
     }
-    f.b = (int)where[0];
-    f.begin = where[1];
-    return f;
+    // Dims 64 h + 32 y + 4 g .. of row r.  (Fields at bits 4 .. 7 were 16 times as large.)
+    __device__ __forceinline__ float4 four(int t, int r, int h, int y) const {
+        const float z = zacc[t][r][GS == 32 ? 2 * h + y : h];
+        const float *even = acc[t][4 * h + 2 * y], *odd = acc[t][4 * h + 2 * y + 1];
+        return make_float4(fmaf(even[r] * 0x1p24f, limit, z), fmaf(odd[r] * 0x1p24f, limit, z), fmaf(even[2 + r] * 0x1p20f, limit, z), fmaf(odd[2 + r] * 0x1p20f, limit, z));
+    }
+};
+
+template <typename T, int HD, int GS, int NT>
+__device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, const Span& span, int G, const Divisor& by_group, uint32_t* own, Sums<HD, GS, NT>& sums) {
+    using St = Stage<HD, GS>;
+    using L = Lay<HD, GS, NT>;
+    constexpr int NG = HD / GS, HH = HD / 64, KW = HD / 32, VW = HD / 64;      // words of a key per lane, for S and for O
+    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3, window = a.attn.window ? a.attn.window : 1 << 30;
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(own);
+    auto token_of = [&](int idx) { return (int)over((unsigned)idx, by_group); };       // of row idx
+    const AttnRange range = span.range;
+    const int p_lo = span.p0 + token_of(job.row0), p_hi = span.p0 + token_of(job.row0 + job.nrows - 1), last = job.last;
+    const uint8_t *kb = static_cast<const uint8_t*>(a.cache.k) + job.b * a.cache.k_stride[0] + job.kh * a.cache.k_stride[1],
+                  *vb = static_cast<const uint8_t*>(a.cache.v) + job.b * a.cache.v_stride[0] + job.kh * a.cache.v_stride[1];
+    const T *kcb = static_cast<const T*>(a.cache.k_scales) + job.b * a.cache.k_scale_stride[0] + job.kh * a.cache.k_scale_stride[1],
+            *vcb = static_cast<const T*>(a.cache.v_scales) + job.b * a.cache.v_scale_stride[0] + job.kh * a.cache.v_scale_stride[1];
+    auto part = [&](int i, int& j0, int& end) {
+        j0 = i < span.n_s ? kPart * i : range.w_start + kPart * (i - span.n_s);
+        end = i < span.n_s ? range.s_end : range.w_end;
+    };
+    // A lane's share of a part: 16 bytes of row lane / CHUNKS (128 dims: and of the row 8 further on) of K and of V, the constants of row lane % 16 of K or V.
+    constexpr int CHUNKS = St::row / 16;
+    const unsigned k_step = (unsigned)a.cache.k_stride[2], v_step = (unsigned)a.cache.v_stride[2],
+                   c_step = 2u * (unsigned)(lane < 16 ? a.cache.k_scale_stride[2] : a.cache.v_scale_stride[2]);
+    const int r = lane / CHUNKS, byte = lane % CHUNKS * 16;
+    const uint8_t *kl = kb + byte, *vl = vb + byte, *cl = reinterpret_cast<const uint8_t*>(lane < 16 ? kcb : vcb);
+    const uint32_t k_to = St::k + r * St::row + byte, v_to = St::v_at(r, byte), c_to = (lane < 16 ? St::kc : St::vc) + (lane & 15) * St::constants;
+    static_assert(HD == 64 || (Stage<128, GS>::v_at(9, 16) - Stage<128, GS>::v_at(1, 16) == 512), "");
+    auto fetch = [&](int i, uint32_t at) {
+        if (i < last) {
+            int j0, end;
+            part(i, j0, end);
+            // (rows behind the end of the range: its last row again, or row 0 of a range that is empty, which may lie behind the cache, with weight zero)
+            const int top = max(min(end, a.attn.max_seq) - 1, 0);
+            const unsigned j = min(j0 + r, top);
+            copy_async<16>(at + k_to, kl + (unsigned long long)j * k_step);
+            copy_async<16>(at + v_to, vl + (unsigned long long)j * v_step);
+            if constexpr (HD == 128) {
+                const unsigned j8 = min(j0 + r + 8, top);
+                copy_async<16>(at + k_to + 512, kl + (unsigned long long)j8 * k_step);
+                copy_async<16>(at + v_to + 512, vl + (unsigned long long)j8 * v_step);
+            }
+            copy_async<St::constants>(at + c_to, cl + (unsigned long long)(unsigned)min(j0 + (lane & 15), top) * c_step);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    int i = job.first;
+#pragma unroll
+    for (int s = 0; s < kStages; ++s) fetch(i + s * job.step, ring + s * St::total);
+    // ---- the operand made of Q: lane (g, c) has dims 32 y + 8 c .. of row 8 t + g, scaled by a power of two, the third and fourth of four by 1 / 16; sums by group ----
+    uint4 qr[NT <= 2 ? NT : 1][KW];
+    uint4* q_at = reinterpret_cast<uint4*>(own + L::q) + lane;
+    uint32_t qz[NT];
+    float factor[NT][2];
+    int pr[NT][2];
+    float (&acc)[NT][4 * HH][4] = sums.acc, (&zacc)[NT][2][NG] = sums.zacc, (&m)[NT][2] = sums.m, (&l)[NT][2] = sums.l, &limit = sums.limit, inverse = 0.f;
+    limit = 0.f;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int idx = job.row0 + min(8 * t + g, job.nrows - 1), tok = token_of(idx), head = job.kh * G + idx - tok * G;
+        const T* q = static_cast<const T*>(a.attn.q) + job.b * a.attn.q_stride[0] + tok * a.attn.q_stride[1] + head * a.attn.q_stride[2] + 8 * c;
+        uint4 raw[KW];
+        float most = 0.f;
+#pragma unroll
+        for (int y = 0; y < KW; ++y) raw[y] = __ldcg(reinterpret_cast<const uint4*>(q + 32 * y));
+#pragma unroll
+        for (int y = 0; y < KW; ++y) {
+            const uint32_t w[4] = {raw[y].x, raw[y].y, raw[y].z, raw[y].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 two = Half<T>::unpack(w[e]);
+                most = fmaxf(most, fmaxf(fabsf(two.x), fabsf(two.y)));
+            }
+        }
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        int up = 15;
+        if (most > 0.f && most < INFINITY) frexpf(most, &up);
+        // (2^(15 - up) in two factors: bf16's smallest numbers need more than fp32 has)
+        const float scale0 = __int_as_float((127 + (15 - up) / 2) << 23), scale1 = __int_as_float((127 + 15 - up - (15 - up) / 2) << 23);
+        float of[NG];
+#pragma unroll
+        for (int y = 0; y < KW; ++y) {
+            const uint32_t w[4] = {raw[y].x, raw[y].y, raw[y].z, raw[y].w};
+            float f[8], sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 two = Half<T>::unpack(w[e]);
+                f[2 * e] = two.x * scale0 * scale1;
+                f[2 * e + 1] = two.y * scale0 * scale1;
+                sum += f[2 * e] + f[2 * e + 1];
+            }
+            const uint4 made = make_uint4(Half<__half>::pack(f[0], f[1]), Half<__half>::pack(f[2] * 0.0625f, f[3] * 0.0625f), Half<__half>::pack(f[4], f[5]),
+                                          Half<__half>::pack(f[6] * 0.0625f, f[7] * 0.0625f));
+            if constexpr (NT <= 2) qr[t][y] = made;
+            else q_at[(t * KW + y) * 32] = made;
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            if (GS == 64 && (y & 1)) of[y >> 1] += sum;
+            else of[GS == 64 ? y >> 1 : y] = sum;
+        }
+        // the sums in two numbers each, times 2^-6: factors 0 .. NG - 1 and NG .. 2 NG - 1 of the eight of a product; lane (g, c) has factors 2 c and 2 c + 1
+        float upper[2], lower[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const float sum = (NG == 4 ? (c & 1 ? of[(2 + e) % NG] : of[e % NG]) : of[e % NG]) * 0x1p-6f;
+            upper[e] = Half<T>::wide(Half<T>::round(sum));
+            lower[e] = sum - upper[e];
+        }
+        if constexpr (NG == 4) qz[t] = c < 2 ? Half<T>::pack(upper[0], upper[1]) : Half<T>::pack(lower[0], lower[1]);
+        else if constexpr (NG == 2) qz[t] = c == 0 ? Half<T>::pack(upper[0], upper[1]) : c == 1 ? Half<T>::pack(lower[0], lower[1]) : 0u;
+        else qz[t] = c == 0 ? Half<T>::pack(upper[0], lower[0]) : 0u;
+        const float mine = ldexpf(a.attn.scale * kLog2e, 24 + up - 15);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            m[t][e] = -INFINITY; l[t][e] = 0.f;
+            factor[t][e] = __shfl_sync(0xffffffffu, mine, 4 * (2 * c + e));
+            pr[t][e] = span.p0 + token_of(job.row0 + min(8 * t + 2 * c + e, job.nrows - 1));
+#pragma unroll
+            for (int n = 0; n < NG; ++n) zacc[t][e][n] = 0.f;
+        }
+#pragma unroll
+        for (int n = 0; n < 4 * HH; ++n) acc[t][n][0] = acc[t][n][1] = acc[t][n][2] = acc[t][n][3] = 0.f;
+    }
+    for (uint32_t from = ring; i < last; i += job.step) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+        __syncwarp();
+        int j0, end;
+        part(i, j0, end);
+        // every row of the tile sees the whole part
+        const bool whole = j0 + kPart <= end && j0 + kPart - 1 <= p_lo && (j0 > p_hi - window || j0 + kPart <= a.attn.sinks);
+        // ---- S: keys g (0, 1) and g + 8 (2, 3), rows 2 c and 2 c + 1 ----
+        float s[NT][4], widest = 0.f;
+        {
+            // the zeros of groups 2 (c % 2) and + 1 (where there are fewer groups: of those there are), the same for both halves of a sum of q
+            const Words<NG == 1 ? 1 : 2> z0 = lds<NG == 1 ? 1 : 2>(from + St::kc + g * St::constants + (NG == 4 ? 8 * (c & 1) : 0)),
+                                         z1 = lds<NG == 1 ? 1 : 2>(from + St::kc + (g + 8) * St::constants + (NG == 4 ? 8 * (c & 1) : 0));
+            const uint32_t a0 = __byte_perm(z0.w[0], z0.w[NG == 1 ? 0 : 1], 0x7632u), a1 = __byte_perm(z1.w[0], z1.w[NG == 1 ? 0 : 1], 0x7632u);
+            const Words<KW> k0 = lds<KW>(from + St::k + g * St::row + 4 * KW * c), k1 = lds<KW>(from + St::k + (g + 8) * St::row + 4 * KW * c);
+            const Words<NG> c0 = lds<NG>(from + St::kc + g * St::constants), c1 = lds<NG>(from + St::kc + (g + 8) * St::constants);
+            const Words<NG> u0 = lds<NG>(from + St::vc + g * St::constants), u1 = lds<NG>(from + St::vc + (g + 8) * St::constants);
+#pragma unroll
+            for (int n = 0; n < NG; ++n) widest = fmaxf(widest, fmaxf(Half<T>::unpack(u0.w[n]).x, Half<T>::unpack(u1.w[n]).x));
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                mma8_first<T>(s[t], a0, a1, qz[t]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[t][e] *= 0x1p-18f;
+            }
+            float d[NT][4];
+#pragma unroll
+            for (int y = 0; y < KW; ++y) {        // 32 dims
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const uint32_t w0 = k0.w[HH * x + (y >> 1)] >> (y & 1 ? 8 : 0), w1 = k1.w[HH * x + (y >> 1)] >> (y & 1 ? 8 : 0);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        uint32_t b0, b1;
+                        if constexpr (NT <= 2) {
+                            b0 = x ? qr[t][y].z : qr[t][y].x;
+                            b1 = x ? qr[t][y].w : qr[t][y].y;
+                        } else {
+                            const uint2 two = reinterpret_cast<const uint2*>(q_at + (t * KW + y) * 32)[x];
+                            b0 = two.x;
+                            b1 = two.y;
+                        }
+                        if (x == 0 && (GS == 32 || !(y & 1))) mma16_first(d[t], w0 & kLow, w1 & kLow, w0 & kHigh, w1 & kHigh, b0, b1);
+                        else mma16(d[t], w0 & kLow, w1 & kLow, w0 & kHigh, w1 & kHigh, b0, b1);
+                    }
+                }
+                if (GS == 32 || (y & 1)) {
+                    const int n = GS == 32 ? y : y >> 1;
+                    const float f0 = Half<T>::unpack(c0.w[n]).x, f1 = Half<T>::unpack(c1.w[n]).x;
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[t][e] = fmaf(e < 2 ? f0 : f1, d[t][e], s[t][e]);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[t][e] *= factor[t][e & 1];
+        }
+        if (__builtin_expect(!whole, 0)) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int j = j0 + g + 8 * (e >> 1);
+                        s[t][e] = j < end && attn_sees(pr[t][e & 1], j, window, a.attn.sinks) ? s[t][e] : -INFINITY;
+                    }
+        }
+        bool grow = widest > 8.f * limit;
+        float top[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                top[t][r] = fmaxf(s[t][r], s[t][2 + r]);
+                grow = grow || top[t][r] - m[t][r] > kGrow;
+            }
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) widest = fmaxf(widest, __shfl_xor_sync(0xffffffffu, widest, o));
+            float shrink = 1.f;
+            if (widest > limit) {                 // the power of two at or below it
+                const float now = fminf(fmaxf(__uint_as_float(__float_as_uint(widest) & 0x7f800000u), 0x1p-100f), 0x1p126f);
+                shrink = limit == 0.f ? 0.f : limit / now;
+                limit = now;
+                inverse = 1.f / now;
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    float up = fmaxf(top[t][r], m[t][r]);
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, o));
+                    const float corr = up == -INFINITY ? 1.f : exp2_fast(m[t][r] - up), both = corr * shrink;
+                    m[t][r] = up;
+                    l[t][r] *= corr;
+#pragma unroll
+                    for (int n = 0; n < NG; ++n) zacc[t][r][n] *= corr;
+#pragma unroll
+                    for (int n = 0; n < 4 * HH; ++n) { acc[t][n][r] *= both; acc[t][n][2 + r] *= both; }
+                }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float safe = m[t][r] == -INFINITY ? 0.f : m[t][r];
+                {
+                    s[t][r] = exp2_fast(s[t][r] - safe);
+                    s[t][2 + r] = exp2_fast(s[t][2 + r] - safe);
+                    l[t][r] += s[t][r] + s[t][2 + r];
+                }
+            }
+        // ---- O: codes of keys 2c, 2c + 1 and 2c + 8, 2c + 9 in pairs ----
+        {
+            // constants of V; those of keys behind the end count for nothing
+            const Words<NG> u0 = lds<NG>(from + St::vc + g * St::constants), u1 = lds<NG>(from + St::vc + (g + 8) * St::constants);
+            float sv[2][NG];
+            {
+                float zv[2][NG];
+#pragma unroll
+                for (int n = 0; n < NG; ++n) {
+                    const float2 f0 = Half<T>::unpack(u0.w[n]), f1 = Half<T>::unpack(u1.w[n]);
+                    sv[0][n] = f0.x; zv[0][n] = f0.y; sv[1][n] = f1.x; zv[1][n] = f1.y;
+                }
+                if (__builtin_expect(!whole, 0)) {
+#pragma unroll
+                    for (int n = 0; n < NG; ++n) {
+                        if (j0 + g >= end) sv[0][n] = zv[0][n] = 0.f;
+                        if (j0 + g + 8 >= end) sv[1][n] = zv[1][n] = 0.f;
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+#pragma unroll
+                        for (int n = 0; n < NG; ++n) zacc[t][r][n] = fmaf(s[t][r], zv[0][n], fmaf(s[t][2 + r], zv[1][n], zacc[t][r][n]));
+                        s[t][r] *= inverse;
+                        s[t][2 + r] *= inverse;
+                    }
+            }
+            Words<VW> v[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) v[n] = lds<VW>(from + St::v_at(2 * c + (n & 1) + 4 * (n & 2), 4 * VW * g));
+#pragma unroll
+            for (int h = 0; h < HH; ++h) {
+                const uint32_t x[2][2] = {{__byte_perm(v[0].w[h], v[1].w[h], 0x5410u), __byte_perm(v[2].w[h], v[3].w[h], 0x5410u)},
+                                          {__byte_perm(v[0].w[h], v[1].w[h], 0x7632u), __byte_perm(v[2].w[h], v[3].w[h], 0x7632u)}};
+                uint32_t b0[NT], b1[NT];
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {     // dims 64 h + 32 y + 4 g + {0, 2} and {1, 3}
+                    if (GS == 32 || y == 0) {
+                        const int n = GS == 32 ? 2 * h + y : h;
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) {
+                            b0[t] = transposed(Half<__half>::pack(s[t][0] * sv[0][n], s[t][1] * sv[0][n]));
+                            b1[t] = transposed(Half<__half>::pack(s[t][2] * sv[1][n], s[t][3] * sv[1][n]));
+                        }
+                    }
+#pragma unroll
+                    for (int z = 0; z < 2; ++z) {
+                        const uint32_t k01 = x[z][0] >> (8 * y), k89 = x[z][1] >> (8 * y);
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) mma16(acc[t][4 * h + 2 * y + z], k01 & kLow, k01 & kHigh, k89 & kLow, k89 & kHigh, b0[t], b1[t]);
+                    }
+                }
+            }
+        }
+        __syncwarp();                             // (the part has been read)
+        fetch(i + kStages * job.step, from);
+        from = from + St::total == ring + kStages * St::total ? ring : from + St::total;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // The row once more by one warp, a few keys at a time and only those that it sees: see attn_row_again in attn.cuh, of which this is the plain form (all dims of
@@ -202,492 +500,343 @@ __device__ __noinline__ void attn4_row_again(const Attn4Args& a, int b, int t, i
     }
 }
 
-template <typename T, int HD, int GS, int NT, bool FLAT>
+template <typename T, int HD, int GS, int NT>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
-attn4_rows_kernel(const __grid_constant__ Attn4Args a, float* __restrict__ part, int split_bits, int row_tiles, int G, const __grid_constant__ Attn4Divisors by) {
+attn4_cluster_kernel(const __grid_constant__ Attn4Args a, int split_bits, int row_tiles, int G, const __grid_constant__ Attn4Divisors by) {
     using L = Lay<HD, GS, NT>;
-    using St = Stage<HD, GS>;
-    constexpr int R = 8 * NT, NG = HD / GS, HH = HD / 64, KW = HD / 32, VW = HD / 64;      // words of a key per lane, for S and for O
+    constexpr int R = 8 * NT, HH = HD / 64;
     extern __shared__ __align__(16) float sm[];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const int window = a.attn.window ? a.attn.window : 1 << 30, splits = FLAT ? 1 : 1 << split_bits, units = a.attn.kv_heads * row_tiles;
-    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(sm) + warp * kStages * St::total;
-    auto token_of = [&](int idx) { return (int)over((unsigned)idx, by.group); };       // of row idx
-    if (!FLAT && splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3, splits = 1 << split_bits;
+    if (splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    const unsigned per_unit = blockIdx.x >> split_bits, unit = over(per_unit, by.row_tiles), b = over(unit, by.kv_heads);
+    const int split = blockIdx.x - (per_unit << split_bits), kh = unit - b * a.attn.kv_heads;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
-
-    const unsigned per_unit = blockIdx.x >> split_bits;
-    const int split = FLAT ? 0 : blockIdx.x - (per_unit << split_bits);
-    int b = 0, tile = 0, kh = 0;
-    long long cur = 0, begin = 0, hi = 0, seq = 0;             // FLAT: the next block, the first one and the end of the run, the sequence's first
-    if constexpr (FLAT) {
-        const Found f = flat_find(a, units, blockIdx.x, gridDim.x, 0, reinterpret_cast<long long*>(sm + L::where));
-        begin = cur = flat_begin(f.total, blockIdx.x, gridDim.x);
-        hi = flat_begin(f.total, blockIdx.x + 1, gridDim.x);
-        b = f.b;
-        seq = f.begin;
-        if (cur >= hi) return;
-    } else {
-        const unsigned unit = over(per_unit, by.row_tiles);
-        tile = per_unit - unit * row_tiles;
-        b = over(unit, by.kv_heads);
-        kh = unit - b * a.attn.kv_heads;
+    const Span span = span_of(a, b);
+    Job job = {(int)b, kh, (int)(per_unit - unit * row_tiles) * R, 0, (int)((long long)span.nb * split >> split_bits) + warp, (int)((long long)span.nb * (split + 1) >> split_bits), kWarps};
+    job.nrows = min(R, span.count * G - job.row0);
+    const int nrows = job.nrows;
+    if (nrows <= 0) return;                       // padding: every CTA of the cluster leaves
+    int* flags = reinterpret_cast<int*>(sm + L::flags);
+    if (threadIdx.x < R) flags[threadIdx.x] = 0;
+    Sums<HD, GS, NT> sums;
+    run_parts<T, HD, GS, NT>(a, job, span, G, by.group, reinterpret_cast<uint32_t*>(sm + warp * L::warp), sums);
+    sums.settle_lanes();
+    __syncthreads();                              // (the rings have been read)
+    // ---- the warps' sums: rows, four adjacent dims each ----
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int row = 8 * t + 2 * c + r;
+            if (row < nrows) {
+                if (g == 0) { sm[L::ml + 2 * (warp * R + row)] = sums.m[t][r]; sm[L::ml + 2 * (warp * R + row) + 1] = sums.l[t][r]; }
+#pragma unroll
+                for (int h = 0; h < HH; ++h)
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) *reinterpret_cast<float4*>(sm + (warp * R + row) * L::LD + 64 * h + 32 * y + 4 * g) = sums.four(t, r, h, y);
+            }
+        }
+    __syncthreads();
+    if (splits > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");      // (all CTAs of the cluster run)
+    // ---- the CTA's sums: out, or slice by slice to the CTAs of the cluster ----
+    const int slice = HD >> split_bits;
+    constexpr int HD_BITS = HD == 128 ? 7 : 6;
+    auto out_of = [&](int row) {
+        const int idx = job.row0 + row, t = (int)over((unsigned)idx, by.group), head = kh * G + idx - t * G;
+        return static_cast<T*>(a.attn.out) + b * a.attn.out_stride[0] + t * a.attn.out_stride[1] + head * a.attn.out_stride[2];
+    };
+    for (int x = threadIdx.x; x < nrows * (HD / 4); x += kThreads) {
+        const int row = x / (HD / 4), d = x % (HD / 4) * 4;
+        float cm = -INFINITY, cl = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) cm = fmaxf(cm, sm[L::ml + 2 * (w * R + row)]);
+        const float safe = cm == -INFINITY ? 0.f : cm;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float e = exp2_fast(sm[L::ml + 2 * (w * R + row)] - safe);
+            const float4 f = *reinterpret_cast<const float4*>(sm + (w * R + row) * L::LD + d);
+            cl += sm[L::ml + 2 * (w * R + row) + 1] * e;
+            o.x += f.x * e; o.y += f.y * e; o.z += f.z * e; o.w += f.w * e;
+        }
+        if (splits == 1) {
+            const bool none = cl == 0.f;
+            float f[4] = {none ? 0.f : o.x / cl, none ? 0.f : o.y / cl, none ? 0.f : o.z / cl, none ? 0.f : o.w / cl};
+            if (settle<T>(f) && isfinite(cl)) flags[row] = 1;
+            *reinterpret_cast<uint2*>(out_of(row) + d) = make_uint2(Half<T>::pack(f[0], f[1]), Half<T>::pack(f[2], f[3]));
+        } else {
+            const float f[4] = {o.x, o.y, o.z, o.w};
+            const int to = d >> (HD_BITS - split_bits);        // (a slice has 8 dims at least)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) st_cluster(sm + L::slice + (split * R + row) * slice + d + e - to * slice, to, f[e]);
+            if (d - to * slice == 0) {
+                st_cluster(sm + L::slice_ml + 2 * (split * R + row), to, cm);
+                st_cluster(sm + L::slice_ml + 2 * (split * R + row) + 1, to, cl);
+            }
+        }
     }
-    Span span = span_of(a, b);
-    while (true) {
-        // ---- what is to be done: blocks first .. last of a (sequence, key head, tile of rows) ----
-        int first, last, n_unit = 0;
-        bool complete = true;
-        if constexpr (FLAT) {
-            n_unit = (int)((cur - seq) / span.nb);
-            first = (int)(cur - seq - (long long)n_unit * span.nb);
-            last = (int)min((long long)span.nb, first + (hi - cur));
-            kh = n_unit / row_tiles;
-            tile = n_unit - kh * row_tiles;
-            complete = first == 0 && last == span.nb;
-        } else {
-            first = (int)((long long)span.nb * split >> split_bits);
-            last = (int)((long long)span.nb * (split + 1) >> split_bits);
+    if (splits > 1) {
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        for (int x = threadIdx.x; x < nrows * (slice / 4); x += kThreads) {           // this CTA's slice of the dims
+            const int row = x >> (HD_BITS - split_bits - 2), d = (x - row * (slice / 4)) * 4;
+            const float2* ml = reinterpret_cast<const float2*>(sm + L::slice_ml) + row;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            float tm = -INFINITY, tl = 0.f;
+            for (int r = 0; r < splits; ++r) tm = fmaxf(tm, ml[r * R].x);
+            const float safe = tm == -INFINITY ? 0.f : tm;
+            for (int r = 0; r < splits; ++r) {
+                const float e = exp2_fast(ml[r * R].x - safe);
+                const float4 f = *reinterpret_cast<const float4*>(sm + L::slice + (r * R + row) * slice + d);
+                tl += ml[r * R].y * e;
+                o.x += f.x * e; o.y += f.y * e; o.z += f.z * e; o.w += f.w * e;
+            }
+            const bool none = tl == 0.f;
+            float f[4] = {none ? 0.f : o.x / tl, none ? 0.f : o.y / tl, none ? 0.f : o.z / tl, none ? 0.f : o.w / tl};
+            if (settle<T>(f) && isfinite(tl)) flags[row] = 1;
+            *reinterpret_cast<uint2*>(out_of(row) + split * slice + d) = make_uint2(Half<T>::pack(f[0], f[1]), Half<T>::pack(f[2], f[3]));
         }
-        const int row0 = tile * R, nrows = min(R, span.count * G - row0);
-        if (nrows <= 0) {                         // padding
-            if constexpr (!FLAT) return;          // (every CTA of the cluster)
-        } else {
-        const AttnRange range = span.range;
-        const int p_lo = span.p0 + token_of(row0), p_hi = span.p0 + token_of(row0 + nrows - 1);
-        const uint8_t *kb = static_cast<const uint8_t*>(a.cache.k) + b * a.cache.k_stride[0] + kh * a.cache.k_stride[1],
-                      *vb = static_cast<const uint8_t*>(a.cache.v) + b * a.cache.v_stride[0] + kh * a.cache.v_stride[1];
-        const T *kcb = static_cast<const T*>(a.cache.k_scales) + b * a.cache.k_scale_stride[0] + kh * a.cache.k_scale_stride[1],
-                *vcb = static_cast<const T*>(a.cache.v_scales) + b * a.cache.v_scale_stride[0] + kh * a.cache.v_scale_stride[1];
-        auto block = [&](int i, int& j0, int& end) {
-            j0 = i < span.n_s ? kBlock * i : range.w_start + kBlock * (i - span.n_s);
-            end = i < span.n_s ? range.s_end : range.w_end;
-        };
-        // (rows behind the end of the range: its last row again, or row 0 of a range that is empty, with weight zero)
-        auto fetch = [&](int i, int stage) {
-            if (i < last) {
-                int j0, end;
-                block(i, j0, end);
-                const int top = max(min(end, a.attn.max_seq) - 1, 0);       // (an empty range may lie behind the cache)
-                const uint32_t at = ring + stage * St::total;
-                constexpr int CHUNKS = St::row / 16;
-#pragma unroll
-                for (int x = 0; x < kBlock * CHUNKS / 32; ++x) {
-                    const int r = (lane + 32 * x) / CHUNKS, byte = (lane + 32 * x) % CHUNKS * 16;
-                    const long long j = min(j0 + r, top);
-                    copy_async<16>(at + St::k + r * St::row + byte, kb + j * a.cache.k_stride[2] + byte);
-                    copy_async<16>(at + St::v_at(r, byte), vb + j * a.cache.v_stride[2] + byte);
-                }
-                const long long j = min(j0 + (lane & 15), top);
-                const T* from = lane < 16 ? kcb + j * a.cache.k_scale_stride[2] : vcb + j * a.cache.v_scale_stride[2];
-                copy_async<St::constants>(at + (lane < 16 ? St::kc : St::vc) + (lane & 15) * St::constants, from);
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        };
-        int i = first + warp;
-#pragma unroll
-        for (int s = 0; s < kStages - 1; ++s) fetch(i + s * kWarps, s);
-        // ---- the rows' places, the operand made of Q, its sums ----
-        long long* places = reinterpret_cast<long long*>(sm + L::places);
-        if (threadIdx.x < R) {
-            const int idx = row0 + min((int)threadIdx.x, nrows - 1), t = token_of(idx), head = kh * G + idx - t * G;
-            places[threadIdx.x] = b * a.attn.q_stride[0] + t * a.attn.q_stride[1] + head * a.attn.q_stride[2];
-            places[R + threadIdx.x] = b * a.attn.out_stride[0] + t * a.attn.out_stride[1] + head * a.attn.out_stride[2];
-            reinterpret_cast<int*>(sm + L::flags)[threadIdx.x] = 0;
+    }
+    // A weight of zero times a NaN, of a key that the row does not see: the row is done again.  (Not where the denominator is not finite: then a score that the row
+    // sees is a NaN.)
+    __syncthreads();
+    for (int row = warp; row < nrows; row += kWarps)
+        if (flags[row]) {
+            const int idx = job.row0 + row, t = (int)over((unsigned)idx, by.group);
+            attn4_row_again<T, HD, GS>(a, b, t, kh * G + idx - t * G, span.p0 + t, split * slice, (split + 1) * slice);
         }
-        __syncthreads();
-        // eight dims (32 y + 8 c ..) of row r per thread: HD / 8 threads of a warp share a row
-        for (int x = threadIdx.x; x < R * HD / 8; x += kThreads) {
-            const int r = x / (HD / 8), e8 = x % (HD / 8), y = e8 >> 2;
-            const uint4 raw = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.attn.q) + places[r] + 8 * e8));
-            const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-            float f[8], most = 0.f;
+}
+
+// ---- the parts of all sequences and key heads one behind the other ----
+// Run i of `runs` begins with part total * i / runs.
+__device__ __forceinline__ long long run_begin(long long total, int i, int runs) { return total * i / runs; }
+__device__ __forceinline__ long long warp_sum(long long v) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 two = Half<T>::unpack(w[e]);
-                f[2 * e] = two.x; f[2 * e + 1] = two.y;
-                most = fmaxf(most, fmaxf(fabsf(two.x), fabsf(two.y)));
-            }
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+// All parts, by a warp; `units`: key heads times tiles of rows, which have the same parts each.
+__device__ __forceinline__ long long parts_of_all(const Attn4Args& a, int units) {
+    long long sum = 0;
+    for (int b = threadIdx.x & 31; b < a.attn.batch; b += 32) sum += (long long)span_of(a, b).nb * units;
+    return warp_sum(sum);
+}
+// The sequence in which part `at` lies and the part with which it begins (b < 0: at is behind all); the part with which sequence `b` begins, where stop is one.
+struct Place { int b; long long begin; };
+__device__ __forceinline__ Place place_of(const Attn4Args& a, int units, long long at, int stop) {
+    const int lane = threadIdx.x & 31;
+    long long before = 0;
+    for (int b0 = 0; b0 < a.attn.batch; b0 += 32) {
+        const int b = b0 + lane;
+        const long long mine = b < a.attn.batch ? (long long)span_of(a, b).nb * units : 0;
+        long long to = mine;
 #pragma unroll
-            for (int o = 1; o < HD / 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-            int up = 15;
-            if (most > 0.f && most < INFINITY) frexpf(most, &up);
-            float sum = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                f[e] = ldexpf(f[e], 15 - up);
-                sum += f[e];
-            }
-#pragma unroll
-            for (int o = 1; o < GS / 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (e8 % (GS / 8) == 0) sm[L::qsum + (e8 / (GS / 8)) * R + r] = ldexpf(sum, -24);
-            if (e8 == 0) sm[L::factor + r] = ldexpf(a.attn.scale * kLog2e, 24 + up - 15);
-            *reinterpret_cast<uint4*>(sm + L::q + (((r >> 3) * KW + y) * 32 + (r & 7) * 4 + (e8 & 3)) * 4) =
-                make_uint4(Half<__half>::pack(f[0], f[1]), Half<__half>::pack(f[2] * 0.0625f, f[3] * 0.0625f), Half<__half>::pack(f[4], f[5]),
-                           Half<__half>::pack(f[6] * 0.0625f, f[7] * 0.0625f));
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long x = __shfl_up_sync(0xffffffffu, to, o);
+            if (lane >= o) to += x;
         }
-        __syncthreads();
-        // Rows of the lane: 8 t + 2 c and + 1
-        float acc[NT][4 * HH][4], zacc[NT][2][NG], m[NT][2], l[NT][2], factor[NT][2], limit = 0.f, inverse = 0.f;
-        int pr[NT][2];
-        uint4 qr[NT <= 2 ? NT : 1][KW];
-        float qs[NT <= 2 ? NT : 1][NG][2];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-#pragma unroll
-            for (int n = 0; n < 4 * HH; ++n) acc[t][n][0] = acc[t][n][1] = acc[t][n][2] = acc[t][n][3] = 0.f;
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                m[t][r] = -INFINITY; l[t][r] = 0.f;
-                factor[t][r] = sm[L::factor + 8 * t + 2 * c + r];
-                pr[t][r] = span.p0 + token_of(row0 + min(8 * t + 2 * c + r, nrows - 1));
-#pragma unroll
-                for (int n = 0; n < NG; ++n) {
-                    zacc[t][r][n] = 0.f;
-                    if constexpr (NT <= 2) qs[t][n][r] = sm[L::qsum + n * R + 8 * t + 2 * c + r];
-                }
-            }
-            if constexpr (NT <= 2)
-#pragma unroll
-                for (int y = 0; y < KW; ++y) qr[t][y] = *reinterpret_cast<const uint4*>(sm + L::q + ((t * KW + y) * 32 + lane) * 4);
+        const unsigned hit = __ballot_sync(0xffffffffu, b < a.attn.batch && (stop >= 0 ? b == stop : before + to > at));
+        if (hit) {
+            const int who = __ffs(hit) - 1;
+            return {b0 + who, before + __shfl_sync(0xffffffffu, to - mine, who)};
         }
-        for (int stage = 0; i < last; i += kWarps) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-            __syncwarp();
-            fetch(i + (kStages - 1) * kWarps, stage == 0 ? kStages - 1 : stage - 1);
-            const uint32_t at = ring + stage * St::total;
-            stage = stage + 1 == kStages ? 0 : stage + 1;
-            int j0, end;
-            block(i, j0, end);
-            // every row of the tile sees the whole block
-            const bool whole = j0 + kBlock <= end && j0 + kBlock - 1 <= p_lo && (j0 > p_hi - window || j0 + kBlock <= a.attn.sinks);
-            // ---- S: keys g (0, 1) and g + 8 (2, 3), rows 2 c and 2 c + 1 ----
-            float s[NT][4];
-#pragma unroll
-            for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
-            {
-                const Words<KW> k0 = lds<KW>(at + St::k + g * St::row + 4 * KW * c), k1 = lds<KW>(at + St::k + (g + 8) * St::row + 4 * KW * c);
-                const Words<NG> c0 = lds<NG>(at + St::kc + g * St::constants), c1 = lds<NG>(at + St::kc + (g + 8) * St::constants);
-                float d[NT][4];
-#pragma unroll
-                for (int y = 0; y < KW; ++y) {        // 32 dims
-                    if (GS == 32 || !(y & 1)) {
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) d[t][0] = d[t][1] = d[t][2] = d[t][3] = 0.f;
-                    }
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const uint32_t w0 = k0.w[HH * x + (y >> 1)] >> (y & 1 ? 8 : 0), w1 = k1.w[HH * x + (y >> 1)] >> (y & 1 ? 8 : 0);
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            uint32_t b0, b1;
-                            if constexpr (NT <= 2) {
-                                b0 = x ? qr[t][y].z : qr[t][y].x;
-                                b1 = x ? qr[t][y].w : qr[t][y].y;
-                            } else {
-                                const uint2 two = *reinterpret_cast<const uint2*>(sm + L::q + ((t * KW + y) * 32 + lane) * 4 + 2 * x);
-                                b0 = two.x;
-                                b1 = two.y;
-                            }
-                            mma16(d[t], w0 & kLow, w1 & kLow, w0 & kHigh, w1 & kHigh, b0, b1);
-                        }
-                    }
-                    if (GS == 32 || (y & 1)) {
-                        const int n = GS == 32 ? y : y >> 1;
-                        const float2 f0 = Half<T>::unpack(c0.w[n]), f1 = Half<T>::unpack(c1.w[n]);       // (scale, zero)
-#pragma unroll
-                        for (int t = 0; t < NT; ++t)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                float sum;
-                                if constexpr (NT <= 2) sum = qs[t][n][e & 1];
-                                else sum = sm[L::qsum + n * R + 8 * t + 2 * c + (e & 1)];
-                                s[t][e] = fmaf(e < 2 ? f0.x : f1.x, d[t][e], fmaf(e < 2 ? f0.y : f1.y, sum, s[t][e]));
-                            }
-                    }
-                }
-            }
-            // ---- constants of V; those of keys behind the end count for nothing ----
-            const Words<NG> u0 = lds<NG>(at + St::vc + g * St::constants), u1 = lds<NG>(at + St::vc + (g + 8) * St::constants);
-            float sv[2][NG], zv[2][NG], widest = 0.f;
-#pragma unroll
-            for (int n = 0; n < NG; ++n) {
-                const float2 f0 = Half<T>::unpack(u0.w[n]), f1 = Half<T>::unpack(u1.w[n]);
-                sv[0][n] = f0.x; zv[0][n] = f0.y; sv[1][n] = f1.x; zv[1][n] = f1.y;
-                if (!whole) {
-                    if (j0 + g >= end) sv[0][n] = zv[0][n] = 0.f;
-                    if (j0 + g + 8 >= end) sv[1][n] = zv[1][n] = 0.f;
-                }
-                widest = fmaxf(widest, fmaxf(sv[0][n], sv[1][n]));
-            }
-            bool grow = widest > 8.f * limit;
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    s[t][e] *= factor[t][e & 1];
-                    if (!whole) {
-                        const int j = j0 + g + 8 * (e >> 1);
-                        s[t][e] = j < end && attn_sees(pr[t][e & 1], j, window, a.attn.sinks) ? s[t][e] : -INFINITY;
-                    }
-                }
-                grow = grow || fmaxf(s[t][0], s[t][2]) - m[t][0] > kGrow || fmaxf(s[t][1], s[t][3]) - m[t][1] > kGrow;
-            }
-            if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) widest = fmaxf(widest, __shfl_xor_sync(0xffffffffu, widest, o));
-                float shrink = 1.f;
-                if (widest > limit) {                 // the power of two at or below it
-                    const float now = fminf(fmaxf(__uint_as_float(__float_as_uint(widest) & 0x7f800000u), 0x1p-100f), 0x1p126f);
-                    shrink = limit == 0.f ? 0.f : limit / now;
-                    limit = now;
-                    inverse = 1.f / now;
-                }
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        float up = fmaxf(fmaxf(s[t][r], s[t][2 + r]), m[t][r]);
-#pragma unroll
-                        for (int o = 4; o < 32; o <<= 1) up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, o));
-                        const float corr = up == -INFINITY ? 1.f : exp2_fast(m[t][r] - up), both = corr * shrink;
-                        m[t][r] = up;
-                        l[t][r] *= corr;
-#pragma unroll
-                        for (int n = 0; n < NG; ++n) zacc[t][r][n] *= corr;
-#pragma unroll
-                        for (int n = 0; n < 4 * HH; ++n) { acc[t][n][r] *= both; acc[t][n][2 + r] *= both; }
-                    }
-            }
+        before += __shfl_sync(0xffffffffu, to, 31);
+    }
+    return {-1, before};
+}
+// Scratch of a run: what it did of the (sequence, key head, tile) in which it began, and of that in which it ended.
+template <int HD, int NT> __device__ __forceinline__ float* scratch_of(float* part, int run, bool second) { return part + (2LL * run + second) * (8 * NT * (HD + 2)); }
+
+template <typename T, int HD, int GS, int NT>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
+attn4_flat_kernel(const __grid_constant__ Attn4Args a, float* __restrict__ part, int row_tiles, int G, const __grid_constant__ Attn4Divisors by) {
+    using L = Lay<HD, GS, NT>;
+    constexpr int R = 8 * NT, HH = HD / 64;
+    extern __shared__ __align__(16) float sm[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3, units = a.attn.kv_heads * row_tiles, runs = gridDim.x * kWarps,
+              run = blockIdx.x * kWarps + warp;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");
+    const long long total = parts_of_all(a, units), begin = run_begin(total, run, runs), end = run_begin(total, run + 1, runs);
+    if (begin >= end) return;
+    Place at = place_of(a, units, begin, -1);
+    for (long long cur = begin; cur < end;) {
+        const Span span = span_of(a, at.b);
+        if (cur >= at.begin + (long long)span.nb * units) {      // the next sequence
+            at.begin += (long long)span.nb * units;
+            ++at.b;
+            continue;
+        }
+        const int unit = (int)((cur - at.begin) / span.nb);
+        Job job;
+        job.b = at.b;
+        job.kh = unit / row_tiles;
+        job.row0 = (unit - job.kh * row_tiles) * R;
+        job.nrows = min(R, span.count * G - job.row0);
+        job.first = (int)(cur - at.begin - (long long)unit * span.nb);
+        job.last = (int)min((long long)span.nb, job.first + (end - cur));
+        job.step = 1;
+        const bool second = cur != begin;
+        cur += job.last - job.first;
+        if (job.nrows <= 0) continue;             // padding
+        Sums<HD, GS, NT> sums;
+        run_parts<T, HD, GS, NT>(a, job, span, G, by.group, reinterpret_cast<uint32_t*>(sm + warp * L::warp), sums);
+        sums.settle_lanes();
+        __syncwarp();                             // (the ring has been read)
+        if (job.first > 0 || job.last < span.nb) {
+            float* to = scratch_of<HD, NT>(part, run, second);
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const float safe = m[t][r] == -INFINITY ? 0.f : m[t][r];
-                    s[t][r] = exp2_fast(s[t][r] - safe);
-                    s[t][2 + r] = exp2_fast(s[t][2 + r] - safe);
-                    l[t][r] += s[t][r] + s[t][2 + r];
+                    const int row = 8 * t + 2 * c + r;
+                    if (row >= job.nrows) continue;
+                    if (g == 0) *reinterpret_cast<float2*>(to + R * HD + 2 * row) = make_float2(sums.m[t][r], sums.l[t][r]);
 #pragma unroll
-                    for (int n = 0; n < NG; ++n) zacc[t][r][n] = fmaf(s[t][r], zv[0][n], fmaf(s[t][2 + r], zv[1][n], zacc[t][r][n]));
+                    for (int h = 0; h < HH; ++h)
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) *reinterpret_cast<float4*>(to + row * HD + 64 * h + 32 * y + 4 * g) = sums.four(t, r, h, y);
                 }
-            // ---- O: codes of keys 2c, 2c + 1 and 2c + 8, 2c + 9 in pairs ----
-            Words<VW> v[4];
-#pragma unroll
-            for (int n = 0; n < 4; ++n) v[n] = lds<VW>(at + St::v_at(2 * c + (n & 1) + 4 * (n & 2), 4 * VW * g));
-#pragma unroll
-            for (int h = 0; h < HH; ++h) {
-                const uint32_t x[2][2] = {{__byte_perm(v[0].w[h], v[1].w[h], 0x5410u), __byte_perm(v[2].w[h], v[3].w[h], 0x5410u)},
-                                          {__byte_perm(v[0].w[h], v[1].w[h], 0x7632u), __byte_perm(v[2].w[h], v[3].w[h], 0x7632u)}};
-                uint32_t b0[NT], b1[NT];
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {         // dims 64 h + 32 y + 4 g + {0, 2} and {1, 3}
-                    if (GS == 32 || y == 0) {
-                        const int n = GS == 32 ? 2 * h + y : h;
-                        const float w0 = sv[0][n] * inverse, w1 = sv[1][n] * inverse;
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            b0[t] = transposed(Half<__half>::pack(s[t][0] * w0, s[t][1] * w0));
-                            b1[t] = transposed(Half<__half>::pack(s[t][2] * w1, s[t][3] * w1));
-                        }
-                    }
-#pragma unroll
-                    for (int z = 0; z < 2; ++z) {
-                        const uint32_t k01 = x[z][0] >> (8 * y), k89 = x[z][1] >> (8 * y);
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) mma16(acc[t][4 * h + 2 * y + z], k01 & kLow, k01 & kHigh, k89 & kLow, k89 & kHigh, b0[t], b1[t]);
-                    }
-                }
-            }
+            continue;
         }
-        // ---- the warps' sums: rows, four adjacent dims each ----
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        __syncthreads();                          // (the ring has been read)
+        unsigned bad[NT][2];                      // lanes with a result that is not finite beside a denominator that is
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                const int row = 8 * t + 2 * c + r;
-                float sum = l[t][r];
+                const int row = 8 * t + 2 * c + r, idx = job.row0 + min(row, job.nrows - 1), tok = (int)over((unsigned)idx, by.group), head = job.kh * G + idx - tok * G;
+                T* out = static_cast<T*>(a.attn.out) + job.b * a.attn.out_stride[0] + tok * a.attn.out_stride[1] + head * a.attn.out_stride[2];
+                const float l = sums.l[t][r];
+                const bool none = l == 0.f;
+                bool odd = false;
 #pragma unroll
-                for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                for (int h = 0; h < HH; ++h)
 #pragma unroll
-                for (int n = 0; n < NG; ++n)
-#pragma unroll
-                    for (int o = 4; o < 32; o <<= 1) zacc[t][r][n] += __shfl_xor_sync(0xffffffffu, zacc[t][r][n], o);
-                if (row < nrows) {
-                    if (g == 0) { sm[L::ml + 2 * (warp * R + row)] = m[t][r]; sm[L::ml + 2 * (warp * R + row) + 1] = sum; }
-#pragma unroll
-                    for (int h = 0; h < HH; ++h)
-#pragma unroll
-                        for (int y = 0; y < 2; ++y) {
-                            const float z = zacc[t][r][GS == 32 ? 2 * h + y : h];
-                            const float *even = acc[t][4 * h + 2 * y], *odd = acc[t][4 * h + 2 * y + 1];
-                            // (fields at bits 4 .. 7 were 16 times as large)
-                            *reinterpret_cast<float4*>(sm + (warp * R + row) * L::LD + 64 * h + 32 * y + 4 * g) =
-                                make_float4(fmaf(even[r] * 0x1p24f, limit, z), fmaf(odd[r] * 0x1p24f, limit, z), fmaf(even[2 + r] * 0x1p20f, limit, z), fmaf(odd[2 + r] * 0x1p20f, limit, z));
-                        }
-                }
+                    for (int y = 0; y < 2; ++y) {
+                        const float4 o = sums.four(t, r, h, y);
+                        float f[4] = {none ? 0.f : o.x / l, none ? 0.f : o.y / l, none ? 0.f : o.z / l, none ? 0.f : o.w / l};
+                        odd = settle<T>(f) || odd;
+                        if (row < job.nrows) *reinterpret_cast<uint2*>(out + 64 * h + 32 * y + 4 * g) = make_uint2(Half<T>::pack(f[0], f[1]), Half<T>::pack(f[2], f[3]));
+                    }
+                bad[t][r] = __ballot_sync(0xffffffffu, odd && isfinite(l) && row < job.nrows);
             }
-        __syncthreads();
-        if (!FLAT && splits > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");      // (all CTAs of the cluster run)
-        // ---- the CTA's sums: to the scratch or out, or slice by slice to the CTAs of the cluster ----
-        const int slice = FLAT ? HD : HD >> split_bits;
-        constexpr int HD_BITS = HD == 128 ? 7 : 6;
-        int* flags = reinterpret_cast<int*>(sm + L::flags);
-        float* run = FLAT ? part + (2LL * blockIdx.x + (cur != begin)) * R * (HD + 2) : nullptr;
-        for (int x = threadIdx.x; x < nrows * (HD / 4); x += kThreads) {
-            const int row = x / (HD / 4), d = x % (HD / 4) * 4;
-            float cm = -INFINITY, cl = 0.f;
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        __syncwarp();
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) cm = fmaxf(cm, sm[L::ml + 2 * (w * R + row)]);
-            const float safe = cm == -INFINITY ? 0.f : cm;
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float e = exp2_fast(sm[L::ml + 2 * (w * R + row)] - safe);
-                const float4 f = *reinterpret_cast<const float4*>(sm + (w * R + row) * L::LD + d);
-                cl += sm[L::ml + 2 * (w * R + row) + 1] * e;
-                o.x += f.x * e; o.y += f.y * e; o.z += f.z * e; o.w += f.w * e;
-            }
-            if (FLAT && !complete) {
-                *reinterpret_cast<float4*>(run + row * HD + d) = o;
-                if (d == 0) *reinterpret_cast<float2*>(run + R * HD + 2 * row) = make_float2(cm, cl);
-            } else if (FLAT || splits == 1) {
-                const bool none = cl == 0.f;
-                float f[4] = {none ? 0.f : o.x / cl, none ? 0.f : o.y / cl, none ? 0.f : o.z / cl, none ? 0.f : o.w / cl};
-                if (settle<T>(f) && isfinite(cl)) flags[row] = 1;
-                *reinterpret_cast<uint2*>(static_cast<T*>(a.attn.out) + places[R + row] + d) = make_uint2(Half<T>::pack(f[0], f[1]), Half<T>::pack(f[2], f[3]));
-            } else {
-                const float f[4] = {o.x, o.y, o.z, o.w};
-                const int to = d >> (HD_BITS - split_bits);        // (a slice has 8 dims at least)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) st_cluster(sm + L::slice + (split * R + row) * slice + d + e - to * slice, to, f[e]);
-                if (d - to * slice == 0) {
-                    st_cluster(sm + L::slice_ml + 2 * (split * R + row), to, cm);
-                    st_cluster(sm + L::slice_ml + 2 * (split * R + row) + 1, to, cl);
-                }
-            }
-        }
-        if (!FLAT && splits > 1) {
-            asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-            for (int x = threadIdx.x; x < nrows * (slice / 4); x += kThreads) {       // this CTA's slice of the dims
-                const int row = x >> (HD_BITS - split_bits - 2), d = (x - row * (slice / 4)) * 4;
-                const float2* ml = reinterpret_cast<const float2*>(sm + L::slice_ml) + row;
-                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-                float tm = -INFINITY, tl = 0.f;
-                for (int r = 0; r < splits; ++r) tm = fmaxf(tm, ml[r * R].x);
-                const float safe = tm == -INFINITY ? 0.f : tm;
-                for (int r = 0; r < splits; ++r) {
-                    const float e = exp2_fast(ml[r * R].x - safe);
-                    const float4 f = *reinterpret_cast<const float4*>(sm + L::slice + (r * R + row) * slice + d);
-                    tl += ml[r * R].y * e;
-                    o.x += f.x * e; o.y += f.y * e; o.z += f.z * e; o.w += f.w * e;
-                }
-                const bool none = tl == 0.f;
-                float f[4] = {none ? 0.f : o.x / tl, none ? 0.f : o.y / tl, none ? 0.f : o.z / tl, none ? 0.f : o.w / tl};
-                if (settle<T>(f) && isfinite(tl)) flags[row] = 1;
-                *reinterpret_cast<uint2*>(static_cast<T*>(a.attn.out) + places[R + row] + split * slice + d) = make_uint2(Half<T>::pack(f[0], f[1]), Half<T>::pack(f[2], f[3]));
-            }
-        }
-        // A weight of zero times a NaN, of a key that the row does not see: the row is done again.  (Not where the denominator is not finite: then a score
-        // that the row sees is a NaN.)
-        __syncthreads();
-        if (complete)
-            for (int row = warp; row < nrows; row += kWarps)
-                if (flags[row]) {
-                    const int idx = row0 + row, t = token_of(idx);
-                    attn4_row_again<T, HD, GS>(a, b, t, kh * G + idx - t * G, span.p0 + t, FLAT ? 0 : split * slice, FLAT ? HD : (split + 1) * slice);
-                }
-        }
-        if constexpr (!FLAT) {
-            return;
-        } else {
-            cur += last - first;
-            if (cur >= hi) return;
-            __syncthreads();                      // (the sums and flags have been read)
-            while (cur >= seq + (long long)span.nb * units) {
-                seq += (long long)span.nb * units;
-                span = span_of(a, ++b);
-            }
-        }
+            for (int r = 0; r < 2; ++r)
+                for (int x = 0; x < 4 && bad[t][r]; ++x)
+                    if (bad[t][r] & 0x11111111u << x) {
+                        const int idx = job.row0 + 8 * t + 2 * x + r, tok = (int)over((unsigned)idx, by.group);
+                        attn4_row_again<T, HD, GS>(a, job.b, tok, job.kh * G + idx - tok * G, span.p0 + tok, 0, HD);
+                    }
     }
 }
 
-// The runs of each (sequence, key head, tile of rows) in which a run of the FLAT launch ends: CTA i takes the one in which run i does, if that is the first there.
+// A CTA for each row: the runs that share its (sequence, key head, tile), taken in turn by the warps (64 dims: halves of warps), which add up at the end, in order.
+// What lies before the wait was written before the launch in front of this one let it start, when all its CTAs had waited themselves; the loads by-pass L1.
 template <typename T, int HD, int GS, int NT>
 __global__ void __launch_bounds__(kThreads)
-attn4_sum_kernel(const __grid_constant__ Attn4Args a, const float* __restrict__ part, int row_tiles, int G, int ctas, const __grid_constant__ Attn4Divisors by) {
-    constexpr int R = 8 * NT;
-    __shared__ long long where[4];
-    __shared__ int flags[R];
+attn4_sum_kernel(const __grid_constant__ Attn4Args a, float* __restrict__ part, int row_tiles, int G, int runs, const __grid_constant__ Attn4Divisors by) {
+    constexpr int R = 8 * NT, LANES = HD / 4, TAKERS = kThreads / LANES, DEEP = 4;
+    __shared__ float4 sum[TAKERS][LANES];
+    __shared__ float2 ml[TAKERS];
+    const int units = a.attn.kv_heads * row_tiles, taker = threadIdx.x / LANES, d = threadIdx.x % LANES * 4;
+    const unsigned unit_all = blockIdx.x / R, per_kh = over(unit_all, by.row_tiles), b = over(per_kh, by.kv_heads);
+    const int row = blockIdx.x % R, tile = unit_all - per_kh * row_tiles, kh = per_kh - b * a.attn.kv_heads, idx = tile * R + row;
+    const Span span = span_of(a, b);
+    const bool there = idx < span.count * G;
+    const long long total = parts_of_all(a, units), start = place_of(a, units, 0, b).begin + (long long)(kh * row_tiles + tile) * span.nb, end = start + span.nb;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
-    const int units = a.attn.kv_heads * row_tiles, warp = threadIdx.x >> 5;
-    const Found f = flat_find(a, units, blockIdx.x + 1, ctas, 0, where);
-    const long long at = flat_begin(f.total, blockIdx.x + 1, ctas);
-    if (f.b < 0) return;
-    const Span span = span_of(a, f.b);
-    const int n_unit = (int)((at - f.begin) / span.nb), kh = n_unit / row_tiles, tile = n_unit - kh * row_tiles;
-    const long long start = f.begin + (long long)n_unit * span.nb, end = start + span.nb, mine = flat_begin(f.total, blockIdx.x, ctas);
-    if (at == start || mine > start) return;                  // run i ends where the next one begins, or did not begin this one
-    if (mine == at) return;                                   // (an empty run)
-    const int row0 = tile * R, nrows = min(R, span.count * G - row0);
-    if (nrows <= 0) return;
-    int runs = 1;                                             // runs blockIdx.x .. + runs - 1
-    while (flat_begin(f.total, blockIdx.x + runs, ctas) < end) ++runs;
-    if (threadIdx.x < R) flags[threadIdx.x] = 0;
-    __syncthreads();
-    auto slot = [&](int r) { return part + (2LL * (blockIdx.x + r) + (r == 0 && mine != start)) * R * (HD + 2); };
-    for (int x = threadIdx.x; x < nrows * (HD / 4); x += kThreads) {
-        const int row = x / (HD / 4), d = x % (HD / 4) * 4;
-        float tm = -INFINITY, tl = 0.f;
-        for (int r = 0; r < runs; ++r)
-            if (r == 0 || flat_begin(f.total, blockIdx.x + r, ctas) < flat_begin(f.total, blockIdx.x + r + 1, ctas)) tm = fmaxf(tm, slot(r)[R * HD + 2 * row]);
-        const float safe = tm == -INFINITY ? 0.f : tm;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int r = 0; r < runs; ++r) {
-            if (r > 0 && flat_begin(f.total, blockIdx.x + r, ctas) >= flat_begin(f.total, blockIdx.x + r + 1, ctas)) continue;
-            const float2 ml = *reinterpret_cast<const float2*>(slot(r) + R * HD + 2 * row);
-            const float4 p = *reinterpret_cast<const float4*>(slot(r) + row * HD + d);
-            const float e = exp2_fast(ml.x - safe);
-            tl += ml.y * e;
-            o.x += p.x * e; o.y += p.y * e; o.z += p.z * e; o.w += p.w * e;
+    if (!there) return;
+    int first = (int)(start * runs / total);                  // the run that has part `start`
+    while (run_begin(total, first + 1, runs) <= start) ++first;
+    while (run_begin(total, first, runs) > start) --first;
+    if (run_begin(total, first + 1, runs) >= end) return;     // it has all of it
+    const bool second = run_begin(total, first, runs) < start;
+    float m = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int r0 = first + taker; r0 < runs && run_begin(total, r0, runs) < end; r0 += DEEP * TAKERS) {
+        float2 of[DEEP];
+        float4 v[DEEP];
+        float up = m;
+#pragma unroll
+        for (int x = 0; x < DEEP; ++x) {
+            const int r = r0 + x * TAKERS;
+            const long long at = run_begin(total, r, runs);
+            // (an empty run has left nothing; there are such where there are fewer parts than runs)
+            const bool has = r < runs && at < end && at < run_begin(total, r + 1, runs);
+            const float* from = scratch_of<HD, NT>(part, has ? r : first, has ? r == first && second : second);
+            of[x] = __ldcg(reinterpret_cast<const float2*>(from + R * HD + 2 * row));
+            v[x] = __ldcg(reinterpret_cast<const float4*>(from + row * HD + d));
+            if (!has) of[x] = make_float2(-INFINITY, 0.f);
+            up = fmaxf(up, of[x].x);
         }
-        const bool none = tl == 0.f;
-        float v[4] = {none ? 0.f : o.x / tl, none ? 0.f : o.y / tl, none ? 0.f : o.z / tl, none ? 0.f : o.w / tl};
-        if (settle<T>(v) && isfinite(tl)) flags[row] = 1;
-        const int idx = row0 + row, t = (int)over((unsigned)idx, by.group), head = kh * G + idx - t * G;
-        *reinterpret_cast<uint2*>(static_cast<T*>(a.attn.out) + f.b * a.attn.out_stride[0] + t * a.attn.out_stride[1] + head * a.attn.out_stride[2] + d) =
-            make_uint2(Half<T>::pack(v[0], v[1]), Half<T>::pack(v[2], v[3]));
+        const float safe = up == -INFINITY ? 0.f : up, corr = exp2_fast(m - safe);
+        m = up;
+        l *= corr;
+        o.x *= corr; o.y *= corr; o.z *= corr; o.w *= corr;
+#pragma unroll
+        for (int x = 0; x < DEEP; ++x) {
+            if (of[x].x == -INFINITY) continue;               // (nothing seen, or nothing there)
+            const float e = exp2_fast(of[x].x - safe);
+            l += of[x].y * e;
+            o.x += v[x].x * e; o.y += v[x].y * e; o.z += v[x].z * e; o.w += v[x].w * e;
+        }
     }
+    sum[taker][d / 4] = o;
+    if (d == 0) ml[taker] = make_float2(m, l);
     __syncthreads();
-    for (int row = warp; row < nrows; row += kWarps)
-        if (flags[row]) {
-            const int idx = row0 + row, t = (int)over((unsigned)idx, by.group);
-            attn4_row_again<T, HD, GS>(a, f.b, t, kh * G + idx - t * G, span.p0 + t, 0, HD);
-        }
+    if (threadIdx.x >= 32) return;
+    float tm = -INFINITY, tl = 0.f;
+#pragma unroll
+    for (int x = 0; x < TAKERS; ++x) tm = fmaxf(tm, ml[x].x);
+    const float safe = tm == -INFINITY ? 0.f : tm;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int x = 0; x < TAKERS; ++x) {
+        const float e = exp2_fast(ml[x].x - safe);
+        const float4 v = sum[x][d / 4];
+        tl += ml[x].y * e;
+        o.x += v.x * e; o.y += v.y * e; o.z += v.z * e; o.w += v.w * e;
+    }
+    const bool none = tl == 0.f;
+    float f[4] = {none ? 0.f : o.x / tl, none ? 0.f : o.y / tl, none ? 0.f : o.z / tl, none ? 0.f : o.w / tl};
+    const bool bad = settle<T>(f);
+    const int t = (int)over((unsigned)idx, by.group), head = kh * G + idx - t * G;
+    if (threadIdx.x < LANES)
+        *reinterpret_cast<uint2*>(static_cast<T*>(a.attn.out) + b * a.attn.out_stride[0] + t * a.attn.out_stride[1] + head * a.attn.out_stride[2] + d) =
+            make_uint2(Half<T>::pack(f[0], f[1]), Half<T>::pack(f[2], f[3]));
+    __syncwarp();
+    if (__any_sync(0xffffffffu, bad && isfinite(tl))) attn4_row_again<T, HD, GS>(a, b, t, head, span.p0 + t, 0, HD);      // (as in attn4_cluster_kernel)
 }
 
-template <typename T, int HD, int GS, int NT, bool FLAT>
+// A kernel's limit of shared memory, once per device.
+struct Allowed {
+    std::once_flag once[64];
+    cudaError_t result[64];
+    template <typename Kernel> int shared(Kernel* kernel, int bytes) {
+        int dev = 0;
+        B200GPTQ_CUDA_TRY(cudaGetDevice(&dev));
+        if (dev < 0 || dev >= 64) return B200GPTQ_ERR_TOO_LARGE;
+        std::call_once(once[dev], [&] { result[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
+        B200GPTQ_CUDA_TRY(result[dev]);
+        return B200GPTQ_OK;
+    }
+};
+
+template <typename T, int HD, int GS, int NT>
 int run(const Attn4Args& a, float* part, const Attn4Plan& p, cudaStream_t stream) {
-    static std::once_flag once[64];
-    static cudaError_t result[64];
-    auto* kernel = attn4_rows_kernel<T, HD, GS, NT, FLAT>;
-    constexpr int smem = Lay<HD, GS, NT>::total * 4;
-    int dev = 0;
-    B200GPTQ_CUDA_TRY(cudaGetDevice(&dev));
-    if (dev < 0 || dev >= 64) return B200GPTQ_ERR_TOO_LARGE;
-    std::call_once(once[dev], [&] { result[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
-    B200GPTQ_CUDA_TRY(result[dev]);
+    static Allowed cluster_allowed, flat_allowed;
+    constexpr int smem = Lay<HD, GS, NT>::total * 4, flat_smem = Lay<HD, GS, NT>::rings * 4;
     const int G = a.attn.heads / a.attn.kv_heads;
-    const long long tiles = ((long long)a.attn.tokens * G + 8 * NT - 1) / (8 * NT), ctas = FLAT ? p.ctas : tiles * a.attn.kv_heads * a.attn.batch << p.split_bits;
-    if (ctas > 0x7fffffff) return B200GPTQ_ERR_TOO_LARGE;
+    const long long tiles = ((long long)a.attn.tokens * G + 8 * NT - 1) / (8 * NT), units = tiles * a.attn.kv_heads * a.attn.batch, ctas = p.flat ? p.ctas : units << p.split_bits;
+    if (ctas > 0x7fffffff || units * 8 * NT > 0x7fffffff) return B200GPTQ_ERR_TOO_LARGE;
     const Attn4Divisors by = {Divisor(tiles), Divisor(a.attn.kv_heads), Divisor(G)};
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)ctas);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     int n = 0;
@@ -698,26 +847,34 @@ int run(const Attn4Args& a, float* part, const Attn4Plan& p, cudaStream_t stream
     }
     cfg.attrs = attr;
     cfg.numAttrs = n;
-    if (!FLAT && p.split_bits) {
-        attr[n].id = cudaLaunchAttributeClusterDimension;
-        attr[n].val.clusterDim.x = 1 << p.split_bits;
-        attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
-        cfg.numAttrs = n + 1;
+    if (!p.flat) {
+        auto* kernel = attn4_cluster_kernel<T, HD, GS, NT>;
+        const int st = cluster_allowed.shared(kernel, smem);
+        if (st != B200GPTQ_OK) return st;
+        cfg.dynamicSmemBytes = smem;
+        if (p.split_bits) {
+            attr[n].id = cudaLaunchAttributeClusterDimension;
+            attr[n].val.clusterDim.x = 1 << p.split_bits;
+            attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+            cfg.numAttrs = n + 1;
+        }
+        B200GPTQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a, p.split_bits, (int)tiles, G, by));
+        return B200GPTQ_OK;
     }
-    B200GPTQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a, part, FLAT ? 0 : p.split_bits, (int)tiles, G, by));
-    if (!FLAT || ctas < 2) return B200GPTQ_OK;
-    cfg.gridDim = dim3((unsigned)ctas - 1);
+    auto* kernel = attn4_flat_kernel<T, HD, GS, NT>;
+    const int st = flat_allowed.shared(kernel, flat_smem);
+    if (st != B200GPTQ_OK) return st;
+    cfg.dynamicSmemBytes = flat_smem;
+    B200GPTQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a, part, (int)tiles, G, by));
+    cfg.gridDim = dim3((unsigned)(units * 8 * NT));
     cfg.dynamicSmemBytes = 0;
-    cfg.numAttrs = n;
-    B200GPTQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, attn4_sum_kernel<T, HD, GS, NT>, a, (const float*)part, (int)tiles, G, (int)ctas, by));
+    B200GPTQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, attn4_sum_kernel<T, HD, GS, NT>, a, part, (int)tiles, G, (int)ctas * kWarps, by));
     return B200GPTQ_OK;
 }
 
 template <typename T, int HD, int GS>
 int run_rows(const Attn4Args& a, float* part, const Attn4Plan& p, cudaStream_t stream) {
-    if (p.tiles8 == 1) return p.flat ? run<T, HD, GS, 1, true>(a, part, p, stream) : run<T, HD, GS, 1, false>(a, part, p, stream);
-    if (p.tiles8 == 2) return p.flat ? run<T, HD, GS, 2, true>(a, part, p, stream) : run<T, HD, GS, 2, false>(a, part, p, stream);
-    return p.flat ? run<T, HD, GS, 4, true>(a, part, p, stream) : run<T, HD, GS, 4, false>(a, part, p, stream);
+    return p.tiles8 == 1 ? run<T, HD, GS, 1>(a, part, p, stream) : p.tiles8 == 2 ? run<T, HD, GS, 2>(a, part, p, stream) : run<T, HD, GS, 4>(a, part, p, stream);
 }
 
 template <typename T>
