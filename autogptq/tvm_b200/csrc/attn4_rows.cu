@@ -61,16 +61,16 @@ __device__ __forceinline__ void st_cluster(const float* local, int rank, float v
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"((uint32_t)__cvta_generic_to_shared(local)), "r"(rank));
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v) : "memory");
 }
-template <int N> __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
-    if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
+template <int N, int OFF = 0> __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+    if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0 + %2], [%1], 16;" ::"r"(dst), "l"(src), "n"(OFF) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0 + %3], [%1], %2;" ::"r"(dst), "l"(src), "n"(N), "n"(OFF) : "memory");
 }
 template <int N> struct Words { uint32_t w[N]; };
-template <int N> __device__ __forceinline__ Words<N> lds(uint32_t at) {
+template <int N, int OFF> __device__ __forceinline__ Words<N> lds(uint32_t at) {       // (the offset in the instruction)
     Words<N> r;
-    if constexpr (N == 4) asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]) : "r"(at));
-    else if constexpr (N == 2) asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(r.w[0]), "=r"(r.w[1]) : "r"(at));
-    else asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r.w[0]) : "r"(at));
+    if constexpr (N == 4) asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4 + %5];" : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]) : "r"(at), "n"(OFF));
+    else if constexpr (N == 2) asm volatile("ld.shared.v2.b32 {%0,%1}, [%2 + %3];" : "=r"(r.w[0]), "=r"(r.w[1]) : "r"(at), "n"(OFF));
+    else asm volatile("ld.shared.b32 %0, [%1 + %2];" : "=r"(r.w[0]) : "r"(at), "n"(OFF));
     return r;
 }
 
@@ -94,6 +94,15 @@ template <int HD, int GS, int NT> struct Lay {
                          flags = slice_ml + 2 * kAttn4MaxSplit * R, total = flags + R;
     static_assert(slice % 4 == 0 && q % 4 == 0 && warp % 4 == 0, "");
 };
+
+// The largest scale of two rows' constants, (scale, zero) in a word each, which are compared together; NaN counts for nothing.
+template <typename T, int N> __device__ __forceinline__ float widest_scale(const Words<N>& u, const Words<N>& v) {
+    using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+    T2 most = __hmax2(*reinterpret_cast<const T2*>(&u.w[0]), *reinterpret_cast<const T2*>(&v.w[0]));
+#pragma unroll
+    for (int n = 1; n < N; ++n) most = __hmax2(most, __hmax2(*reinterpret_cast<const T2*>(&u.w[n]), *reinterpret_cast<const T2*>(&v.w[n])));
+    return fmaxf(Half<T>::wide(most.x), 0.f);
+}
 
 // Parts of a sequence: those that its tokens see between them; one at least where there are tokens, since their rows get zeros when they see nothing.
 struct Span { AttnRange range; int p0, count, n_s, nb; };
@@ -151,10 +160,6 @@ __device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, co
                   *vb = static_cast<const uint8_t*>(a.cache.v) + job.b * a.cache.v_stride[0] + job.kh * a.cache.v_stride[1];
     const T *kcb = static_cast<const T*>(a.cache.k_scales) + job.b * a.cache.k_scale_stride[0] + job.kh * a.cache.k_scale_stride[1],
             *vcb = static_cast<const T*>(a.cache.v_scales) + job.b * a.cache.v_scale_stride[0] + job.kh * a.cache.v_scale_stride[1];
-    auto part = [&](int i, int& j0, int& end) {
-        j0 = i < span.n_s ? kPart * i : range.w_start + kPart * (i - span.n_s);
-        end = i < span.n_s ? range.s_end : range.w_end;
-    };
     // A lane's share of a part: 16 bytes of row lane / CHUNKS (128 dims: and of the row 8 further on) of K and of V, the constants of row lane % 16 of K or V.
     constexpr int CHUNKS = St::row / 16;
     const unsigned k_step = (unsigned)a.cache.k_stride[2], v_step = (unsigned)a.cache.v_stride[2],
@@ -163,27 +168,57 @@ __device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, co
     const uint8_t *kl = kb + byte, *vl = vb + byte, *cl = reinterpret_cast<const uint8_t*>(lane < 16 ? kcb : vcb);
     const uint32_t k_to = St::k + r * St::row + byte, v_to = St::v_at(r, byte), c_to = (lane < 16 ? St::kc : St::vc) + (lane & 15) * St::constants;
     static_assert(HD == 64 || (Stage<128, GS>::v_at(9, 16) - Stage<128, GS>::v_at(1, 16) == 512), "");
-    auto fetch = [&](int i, uint32_t at) {
-        if (i < last) {
-            int j0, end;
-            part(i, j0, end);
-            // (rows behind the end of the range: its last row again, or row 0 of a range that is empty, which may lie behind the cache, with weight zero)
-            const int top = max(min(end, a.attn.max_seq) - 1, 0);
-            const unsigned j = min(j0 + r, top);
-            copy_async<16>(at + k_to, kl + (unsigned long long)j * k_step);
-            copy_async<16>(at + v_to, vl + (unsigned long long)j * v_step);
-            if constexpr (HD == 128) {
-                const unsigned j8 = min(j0 + r + 8, top);
-                copy_async<16>(at + k_to + 512, kl + (unsigned long long)j8 * k_step);
-                copy_async<16>(at + v_to + 512, vl + (unsigned long long)j8 * v_step);
+    // Where the warp is: the row with which a part begins, the end of its range, and between which rows all rows of the tile see all of a part.  Twice: for the part that is
+    // fetched and for the one that is multiplied.
+    struct Walk { int i, j0, end, whole_from, whole_to; };
+    auto enter = [&](Walk& w) {
+        const bool sink = w.i < span.n_s;
+        w.j0 = sink ? kPart * w.i : range.w_start + kPart * (w.i - span.n_s);
+        w.end = sink ? range.s_end : range.w_end;
+        w.whole_from = sink ? 0 : p_hi - window + 1;
+        w.whole_to = min(sink ? min(range.s_end, a.attn.sinks) : range.w_end, p_lo + 1) - kPart;
+    };
+    auto advance = [&](Walk& w) {
+        const bool sink = w.i < span.n_s;
+        w.i += job.step;
+        w.j0 += kPart * job.step;
+        if (sink && w.i >= span.n_s) enter(w);
+    };
+    auto fetch = [&](Walk& w, uint32_t at) {
+        if (w.i < last) {
+            const uint32_t k_at = at + k_to, v_at = at + v_to, c_at = at + c_to;
+            if (w.j0 + kPart <= w.end) {
+                const uint8_t *k = kl + (unsigned long long)(unsigned)(w.j0 + r) * k_step, *v = vl + (unsigned long long)(unsigned)(w.j0 + r) * v_step;
+                copy_async<16>(k_at, k);
+                copy_async<16>(v_at, v);
+                if constexpr (HD == 128) {
+                    copy_async<16, 512>(k_at, k + 8ull * k_step);
+                    copy_async<16, 512>(v_at, v + 8ull * v_step);
+                }
+                copy_async<St::constants>(c_at, cl + (unsigned long long)(unsigned)(w.j0 + (lane & 15)) * c_step);
+            } else {
+                // (rows behind the end of the range: its last row again, or row 0 of a range that is empty, which may lie behind the cache, with weight zero)
+                const int top = max(min(w.end, a.attn.max_seq) - 1, 0);
+                const unsigned j = min(w.j0 + r, top);
+                copy_async<16>(k_at, kl + (unsigned long long)j * k_step);
+                copy_async<16>(v_at, vl + (unsigned long long)j * v_step);
+                if constexpr (HD == 128) {
+                    const unsigned j8 = min(w.j0 + r + 8, top);
+                    copy_async<16, 512>(k_at, kl + (unsigned long long)j8 * k_step);
+                    copy_async<16, 512>(v_at, vl + (unsigned long long)j8 * v_step);
+                }
+                copy_async<St::constants>(c_at, cl + (unsigned long long)(unsigned)min(w.j0 + (lane & 15), top) * c_step);
             }
-            copy_async<St::constants>(at + c_to, cl + (unsigned long long)(unsigned)min(j0 + (lane & 15), top) * c_step);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
+        advance(w);
     };
-    int i = job.first;
+    Walk ahead, now;
+    ahead.i = now.i = job.first;
+    enter(ahead);
+    enter(now);
 #pragma unroll
-    for (int s = 0; s < kStages; ++s) fetch(i + s * job.step, ring + s * St::total);
+    for (int s = 0; s < kStages; ++s) fetch(ahead, ring + s * St::total);
     // ---- the operand made of Q: lane (g, c) has dims 32 y + 8 c .. of row 8 t + g, scaled by a power of two, the third and fourth of four by 1 / 16; sums by group ----
     uint4 qr[NT <= 2 ? NT : 1][KW];
     uint4* q_at = reinterpret_cast<uint4*>(own + L::q) + lane;
@@ -259,25 +294,26 @@ __device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, co
 #pragma unroll
         for (int n = 0; n < 4 * HH; ++n) acc[t][n][0] = acc[t][n][1] = acc[t][n][2] = acc[t][n][3] = 0.f;
     }
-    for (uint32_t from = ring; i < last; i += job.step) {
+    // The lane's places in a part: codes and constants of keys g and g + 8, zeros, codes of keys 2c, 2c + 8 and 2c + 1, 2c + 9.
+    const uint32_t k_lane = St::k + g * St::row + 4 * KW * c, c_lane = St::kc + g * St::constants, z_lane = c_lane + (NG == 4 ? 8 * (c & 1) : 0),
+                   even_lane = St::v_at(2 * c, 4 * VW * g), odd_lane = St::v_at(2 * c + 1, 4 * VW * g);
+    for (uint32_t from = ring; now.i < last; advance(now)) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
         __syncwarp();
-        int j0, end;
-        part(i, j0, end);
-        // every row of the tile sees the whole part
-        const bool whole = j0 + kPart <= end && j0 + kPart - 1 <= p_lo && (j0 > p_hi - window || j0 + kPart <= a.attn.sinks);
+        const int j0 = now.j0, end = now.end;
+        const bool whole = j0 >= now.whole_from && j0 <= now.whole_to;
+        const uint32_t k_from = from + k_lane, c_from = from + c_lane, z_from = from + z_lane, even_from = from + even_lane, odd_from = from + odd_lane;
         // ---- S: keys g (0, 1) and g + 8 (2, 3), rows 2 c and 2 c + 1 ----
         float s[NT][4], widest = 0.f;
         {
             // the zeros of groups 2 (c % 2) and + 1 (where there are fewer groups: of those there are), the same for both halves of a sum of q
-            const Words<NG == 1 ? 1 : 2> z0 = lds<NG == 1 ? 1 : 2>(from + St::kc + g * St::constants + (NG == 4 ? 8 * (c & 1) : 0)),
-                                         z1 = lds<NG == 1 ? 1 : 2>(from + St::kc + (g + 8) * St::constants + (NG == 4 ? 8 * (c & 1) : 0));
+            const Words<NG == 1 ? 1 : 2> z0 = lds<NG == 1 ? 1 : 2, 0>(z_from),
+                                         z1 = lds<NG == 1 ? 1 : 2, 8 * St::constants>(z_from);
             const uint32_t a0 = __byte_perm(z0.w[0], z0.w[NG == 1 ? 0 : 1], 0x7632u), a1 = __byte_perm(z1.w[0], z1.w[NG == 1 ? 0 : 1], 0x7632u);
-            const Words<KW> k0 = lds<KW>(from + St::k + g * St::row + 4 * KW * c), k1 = lds<KW>(from + St::k + (g + 8) * St::row + 4 * KW * c);
-            const Words<NG> c0 = lds<NG>(from + St::kc + g * St::constants), c1 = lds<NG>(from + St::kc + (g + 8) * St::constants);
-            const Words<NG> u0 = lds<NG>(from + St::vc + g * St::constants), u1 = lds<NG>(from + St::vc + (g + 8) * St::constants);
-#pragma unroll
-            for (int n = 0; n < NG; ++n) widest = fmaxf(widest, fmaxf(Half<T>::unpack(u0.w[n]).x, Half<T>::unpack(u1.w[n]).x));
+            const Words<KW> k0 = lds<KW, 0>(k_from), k1 = lds<KW, 8 * St::row>(k_from);
+            const Words<NG> c0 = lds<NG, 0>(c_from), c1 = lds<NG, 8 * St::constants>(c_from);
+            const Words<NG> u0 = lds<NG, kPart * St::constants>(c_from), u1 = lds<NG, (kPart + 8) * St::constants>(c_from);
+            widest = widest_scale<T, NG>(u0, u1);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 mma8_first<T>(s[t], a0, a1, qz[t]);
@@ -377,7 +413,7 @@ __device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, co
         // ---- O: codes of keys 2c, 2c + 1 and 2c + 8, 2c + 9 in pairs ----
         {
             // constants of V; those of keys behind the end count for nothing
-            const Words<NG> u0 = lds<NG>(from + St::vc + g * St::constants), u1 = lds<NG>(from + St::vc + (g + 8) * St::constants);
+            const Words<NG> u0 = lds<NG, kPart * St::constants>(c_from), u1 = lds<NG, (kPart + 8) * St::constants>(c_from);
             float sv[2][NG];
             {
                 float zv[2][NG];
@@ -403,9 +439,8 @@ __device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, co
                         s[t][2 + r] *= inverse;
                     }
             }
-            Words<VW> v[4];
-#pragma unroll
-            for (int n = 0; n < 4; ++n) v[n] = lds<VW>(from + St::v_at(2 * c + (n & 1) + 4 * (n & 2), 4 * VW * g));
+            constexpr int EIGHT = St::v_at(8, 0) - St::v_at(0, 0);
+            const Words<VW> v[4] = {lds<VW, 0>(even_from), lds<VW, 0>(odd_from), lds<VW, EIGHT>(even_from), lds<VW, EIGHT>(odd_from)};
 #pragma unroll
             for (int h = 0; h < HH; ++h) {
                 const uint32_t x[2][2] = {{__byte_perm(v[0].w[h], v[1].w[h], 0x5410u), __byte_perm(v[2].w[h], v[3].w[h], 0x5410u)},
@@ -431,7 +466,7 @@ __device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, co
             }
         }
         __syncwarp();                             // (the part has been read)
-        fetch(i + kStages * job.step, from);
+        fetch(ahead, from);
         from = from + St::total == ring + kStages * St::total ? ring : from + St::total;
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -608,42 +643,55 @@ attn4_cluster_kernel(const __grid_constant__ Attn4Args a, int split_bits, int ro
 }
 
 // ---- the parts of all sequences and key heads one behind the other ----
-// Run i of `runs` begins with part total * i / runs.
-__device__ __forceinline__ long long run_begin(long long total, int i, int runs) { return total * i / runs; }
-__device__ __forceinline__ long long warp_sum(long long v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+__device__ __forceinline__ long long divided(long long n, int d) {       // n >= 0, d > 0 (a division of 64 bits takes some 100 instructions)
+    return n >> 32 ? n / d : (long long)((unsigned)n / (unsigned)d);
 }
-// All parts, by a warp; `units`: key heads times tiles of rows, which have the same parts each.
-__device__ __forceinline__ long long parts_of_all(const Attn4Args& a, int units) {
-    long long sum = 0;
-    for (int b = threadIdx.x & 31; b < a.attn.batch; b += 32) sum += (long long)span_of(a, b).nb * units;
-    return warp_sum(sum);
-}
-// The sequence in which part `at` lies and the part with which it begins (b < 0: at is behind all); the part with which sequence `b` begins, where stop is one.
-struct Place { int b; long long begin; };
-__device__ __forceinline__ Place place_of(const Attn4Args& a, int units, long long at, int stop) {
-    const int lane = threadIdx.x & 31;
-    long long before = 0;
-    for (int b0 = 0; b0 < a.attn.batch; b0 += 32) {
-        const int b = b0 + lane;
-        const long long mine = b < a.attn.batch ? (long long)span_of(a, b).nb * units : 0;
-        long long to = mine;
+// The runs: the first `more` have `each` + 1 parts, the others `each`.
+struct Runs {
+    long long each;
+    int more;
+    __device__ __forceinline__ Runs(long long total, int runs) : each(divided(total, runs)), more((int)(total - each * runs)) {}
+    __device__ __forceinline__ long long begin(int i) const { return each * i + min(i, more); }
+    // The run that has part `at` of them.
+    __device__ __forceinline__ int of(long long at) const {
+        const long long longer = (each + 1) * more;
+        return at < longer ? (int)divided(at, (int)(each + 1)) : more + (int)divided(at - longer, (int)each);
+    }
+};
+// The sequences' parts as a warp sees them, 32 sequences at a time; `units`: key heads times tiles of rows, which have the same parts each.
+struct Parts {
+    long long mine, to, before;               // of the lane's sequence; with those before it among the 32; before these
+    int b0;
+
+    __device__ __forceinline__ void look(const Attn4Args& a, int units, int first) {
+        const int lane = threadIdx.x & 31;
+        b0 = first;
+        mine = b0 + lane < a.attn.batch ? (long long)span_of(a, b0 + lane).nb * units : 0;
+        to = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const long long x = __shfl_up_sync(0xffffffffu, to, o);
             if (lane >= o) to += x;
         }
-        const unsigned hit = __ballot_sync(0xffffffffu, b < a.attn.batch && (stop >= 0 ? b == stop : before + to > at));
-        if (hit) {
-            const int who = __ffs(hit) - 1;
-            return {b0 + who, before + __shfl_sync(0xffffffffu, to - mine, who)};
-        }
-        before += __shfl_sync(0xffffffffu, to, 31);
     }
-    return {-1, before};
-}
+    // Leaves the first 32 sequences, so that there is nothing to be looked at again where there are no more.
+    __device__ __forceinline__ long long all(const Attn4Args& a, int units) {
+        long long sum = 0;
+        for (int first = (a.attn.batch - 1) / 32 * 32; first >= 0; first -= 32) {
+            look(a, units, first);
+            sum += __shfl_sync(0xffffffffu, to, 31);
+        }
+        before = 0;
+        return sum;
+    }
+    __device__ __forceinline__ void next(const Attn4Args& a, int units) {
+        const long long sum = before + __shfl_sync(0xffffffffu, to, 31);
+        look(a, units, b0 + 32);
+        before = sum;
+    }
+    // The part with which lane who's sequence begins.
+    __device__ __forceinline__ long long begin_of(int who) const { return before + __shfl_sync(0xffffffffu, to - mine, who); }
+};
 // Scratch of a run: what it did of the (sequence, key head, tile) in which it began, and of that in which it ended.
 template <int HD, int NT> __device__ __forceinline__ float* scratch_of(float* part, int run, bool second) { return part + (2LL * run + second) * (8 * NT * (HD + 2)); }
 
@@ -657,23 +705,27 @@ attn4_flat_kernel(const __grid_constant__ Attn4Args a, float* __restrict__ part,
               run = blockIdx.x * kWarps + warp;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
-    const long long total = parts_of_all(a, units), begin = run_begin(total, run, runs), end = run_begin(total, run + 1, runs);
+    Parts parts;
+    const Runs by_run(parts.all(a, units), runs);
+    const long long begin = by_run.begin(run), end = by_run.begin(run + 1);
     if (begin >= end) return;
-    Place at = place_of(a, units, begin, -1);
+    unsigned hit;
+    while (!(hit = __ballot_sync(0xffffffffu, parts.mine && parts.before + parts.to > begin))) parts.next(a, units);
+    Job job;
+    job.b = parts.b0 + __ffs(hit) - 1;
+    long long sequence = parts.begin_of(__ffs(hit) - 1);         // the part with which it begins
     for (long long cur = begin; cur < end;) {
-        const Span span = span_of(a, at.b);
-        if (cur >= at.begin + (long long)span.nb * units) {      // the next sequence
-            at.begin += (long long)span.nb * units;
-            ++at.b;
+        const Span span = span_of(a, job.b);
+        if (cur >= sequence + (long long)span.nb * units) {      // the next sequence
+            sequence += (long long)span.nb * units;
+            ++job.b;
             continue;
         }
-        const int unit = (int)((cur - at.begin) / span.nb);
-        Job job;
-        job.b = at.b;
-        job.kh = unit / row_tiles;
+        const int unit = (int)divided(cur - sequence, span.nb);
+        job.kh = (int)over((unsigned)unit, by.row_tiles);
         job.row0 = (unit - job.kh * row_tiles) * R;
         job.nrows = min(R, span.count * G - job.row0);
-        job.first = (int)(cur - at.begin - (long long)unit * span.nb);
+        job.first = (int)(cur - sequence - (long long)unit * span.nb);
         job.last = (int)min((long long)span.nb, job.first + (end - cur));
         job.step = 1;
         const bool second = cur != begin;
@@ -746,27 +798,28 @@ attn4_sum_kernel(const __grid_constant__ Attn4Args a, float* __restrict__ part, 
     const int row = blockIdx.x % R, tile = unit_all - per_kh * row_tiles, kh = per_kh - b * a.attn.kv_heads, idx = tile * R + row;
     const Span span = span_of(a, b);
     const bool there = idx < span.count * G;
-    const long long total = parts_of_all(a, units), start = place_of(a, units, 0, b).begin + (long long)(kh * row_tiles + tile) * span.nb, end = start + span.nb;
+    Parts parts;
+    const Runs by_run(parts.all(a, units), runs);
+    while (parts.b0 + 32 <= (int)b) parts.next(a, units);
+    const long long start = parts.begin_of((int)b - parts.b0) + (long long)(kh * row_tiles + tile) * span.nb, end = start + span.nb;
+    const int first = there ? by_run.of(start) : 0;           // the run that has part `start`
+    const bool whole = by_run.begin(first + 1) >= end;
+    const bool second = by_run.begin(first) < start;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
-    if (!there) return;
-    int first = (int)(start * runs / total);                  // the run that has part `start`
-    while (run_begin(total, first + 1, runs) <= start) ++first;
-    while (run_begin(total, first, runs) > start) --first;
-    if (run_begin(total, first + 1, runs) >= end) return;     // it has all of it
-    const bool second = run_begin(total, first, runs) < start;
+    if (!there || whole) return;
     float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int r0 = first + taker; r0 < runs && run_begin(total, r0, runs) < end; r0 += DEEP * TAKERS) {
+    for (int r0 = first + taker; r0 < runs && by_run.begin(r0) < end; r0 += DEEP * TAKERS) {
         float2 of[DEEP];
         float4 v[DEEP];
         float up = m;
 #pragma unroll
         for (int x = 0; x < DEEP; ++x) {
             const int r = r0 + x * TAKERS;
-            const long long at = run_begin(total, r, runs);
+            const long long at = by_run.begin(r);
             // (an empty run has left nothing; there are such where there are fewer parts than runs)
-            const bool has = r < runs && at < end && at < run_begin(total, r + 1, runs);
+            const bool has = r < runs && at < end && at < by_run.begin(r + 1);
             const float* from = scratch_of<HD, NT>(part, has ? r : first, has ? r == first && second : second);
             of[x] = __ldcg(reinterpret_cast<const float2*>(from + R * HD + 2 * row));
             v[x] = __ldcg(reinterpret_cast<const float4*>(from + row * HD + d));
