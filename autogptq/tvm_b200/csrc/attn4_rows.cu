@@ -168,63 +168,37 @@ __device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, co
     const uint8_t *kl = kb + byte, *vl = vb + byte, *cl = reinterpret_cast<const uint8_t*>(lane < 16 ? kcb : vcb);
     const uint32_t k_to = St::k + r * St::row + byte, v_to = St::v_at(r, byte), c_to = (lane < 16 ? St::kc : St::vc) + (lane & 15) * St::constants;
     static_assert(HD == 64 || (Stage<128, GS>::v_at(9, 16) - Stage<128, GS>::v_at(1, 16) == 512), "");
-    // Where the warp is: the row with which a part begins, the end of its range, and between which rows all rows of the tile see all of a part.  Twice: for the part that is
-    // fetched and for the one that is multiplied.
-    struct Walk { int i, j0, end, whole_from, whole_to; };
-    auto enter = [&](Walk& w) {
-        const bool sink = w.i < span.n_s;
-        w.j0 = sink ? kPart * w.i : range.w_start + kPart * (w.i - span.n_s);
-        w.end = sink ? range.s_end : range.w_end;
-        w.whole_from = sink ? 0 : p_hi - window + 1;
-        w.whole_to = min(sink ? min(range.s_end, a.attn.sinks) : range.w_end, p_lo + 1) - kPart;
-    };
-    auto advance = [&](Walk& w) {
-        const bool sink = w.i < span.n_s;
-        w.i += job.step;
-        w.j0 += kPart * job.step;
-        if (sink && w.i >= span.n_s) enter(w);
-    };
-    auto fetch = [&](Walk& w, uint32_t at) {
-        if (w.i < last) {
-            const uint32_t k_at = at + k_to, v_at = at + v_to, c_at = at + c_to;
-            if (w.j0 + kPart <= w.end) {
-                const uint8_t *k = kl + (unsigned long long)(unsigned)(w.j0 + r) * k_step, *v = vl + (unsigned long long)(unsigned)(w.j0 + r) * v_step;
-                copy_async<16>(k_at, k);
-                copy_async<16>(v_at, v);
-                if constexpr (HD == 128) {
-                    copy_async<16, 512>(k_at, k + 8ull * k_step);
-                    copy_async<16, 512>(v_at, v + 8ull * v_step);
-                }
-                copy_async<St::constants>(c_at, cl + (unsigned long long)(unsigned)(w.j0 + (lane & 15)) * c_step);
-            } else {
-                // (rows behind the end of the range: its last row again, or row 0 of a range that is empty, which may lie behind the cache, with weight zero)
-                const int top = max(min(w.end, a.attn.max_seq) - 1, 0);
-                const unsigned j = min(w.j0 + r, top);
-                copy_async<16>(k_at, kl + (unsigned long long)j * k_step);
-                copy_async<16>(v_at, vl + (unsigned long long)j * v_step);
-                if constexpr (HD == 128) {
-                    const unsigned j8 = min(w.j0 + r + 8, top);
-                    copy_async<16, 512>(k_at, kl + (unsigned long long)j8 * k_step);
-                    copy_async<16, 512>(v_at, vl + (unsigned long long)j8 * v_step);
-                }
-                copy_async<St::constants>(c_at, cl + (unsigned long long)(unsigned)min(w.j0 + (lane & 15), top) * c_step);
+    // The parts lie in two ranges of rows, the sinks and the window; the ring is filled anew for the second.  (Rows behind the end of a range may be read, with weight
+    // zero, those behind the cache not.)
+    const int most_row = a.attn.max_seq - 1;
+    auto fetch = [&](int j0, int behind, uint32_t at) {
+        if (j0 < behind) {
+            const unsigned j = min(j0 + r, most_row);
+            copy_async<16>(at + k_to, kl + (unsigned long long)j * k_step);
+            copy_async<16>(at + v_to, vl + (unsigned long long)j * v_step);
+            if constexpr (HD == 128) {
+                const unsigned j8 = min(j0 + r + 8, most_row);
+                copy_async<16, 512>(at + k_to, kl + (unsigned long long)j8 * k_step);
+                copy_async<16, 512>(at + v_to, vl + (unsigned long long)j8 * v_step);
             }
+            copy_async<St::constants>(at + c_to, cl + (unsigned long long)(unsigned)min(j0 + (lane & 15), most_row) * c_step);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        advance(w);
     };
-    Walk ahead, now;
-    ahead.i = now.i = job.first;
-    enter(ahead);
-    enter(now);
+    bool sink = job.first < span.n_s;
+    int j0, behind;                               // first row of the warp's next part, a row behind its last one's first
+    auto enter = [&](int first) {                 // part `first` of the job's, in the range that it lies in
+        j0 = sink ? kPart * first : range.w_start + kPart * (first - span.n_s);
+        behind = sink ? kPart * min(last, span.n_s) : range.w_start + kPart * (last - span.n_s);
 #pragma unroll
-    for (int s = 0; s < kStages; ++s) fetch(ahead, ring + s * St::total);
+        for (int s = 0; s < kStages; ++s) fetch(j0 + s * kPart * job.step, behind, ring + s * St::total);
+    };
+    enter(job.first);
     // ---- the operand made of Q: lane (g, c) has dims 32 y + 8 c .. of row 8 t + g, scaled by a power of two, the third and fourth of four by 1 / 16; sums by group ----
     uint4 qr[NT <= 2 ? NT : 1][KW];
     uint4* q_at = reinterpret_cast<uint4*>(own + L::q) + lane;
     uint32_t qz[NT];
     float factor[NT][2];
-    int pr[NT][2];
     float (&acc)[NT][4 * HH][4] = sums.acc, (&zacc)[NT][2][NG] = sums.zacc, (&m)[NT][2] = sums.m, (&l)[NT][2] = sums.l, &limit = sums.limit, inverse = 0.f;
     limit = 0.f;
 #pragma unroll
@@ -287,7 +261,6 @@ __device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, co
         for (int e = 0; e < 2; ++e) {
             m[t][e] = -INFINITY; l[t][e] = 0.f;
             factor[t][e] = __shfl_sync(0xffffffffu, mine, 4 * (2 * c + e));
-            pr[t][e] = span.p0 + token_of(job.row0 + min(8 * t + 2 * c + e, job.nrows - 1));
 #pragma unroll
             for (int n = 0; n < NG; ++n) zacc[t][e][n] = 0.f;
         }
@@ -297,11 +270,14 @@ __device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, co
     // The lane's places in a part: codes and constants of keys g and g + 8, zeros, codes of keys 2c, 2c + 8 and 2c + 1, 2c + 9.
     const uint32_t k_lane = St::k + g * St::row + 4 * KW * c, c_lane = St::kc + g * St::constants, z_lane = c_lane + (NG == 4 ? 8 * (c & 1) : 0),
                    even_lane = St::v_at(2 * c, 4 * VW * g), odd_lane = St::v_at(2 * c + 1, 4 * VW * g);
-    for (uint32_t from = ring; now.i < last; advance(now)) {
+    const int step = kPart * job.step;
+    while (true) {
+    // Parts that begin between these rows are seen as a whole by all rows of the tile.
+    const int end = sink ? range.s_end : range.w_end, whole_from = sink ? 0 : p_hi - window + 1, whole_to = min(sink ? min(end, a.attn.sinks) : end, p_lo + 1) - kPart;
+    for (uint32_t from = ring; j0 < behind; j0 += step) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
         __syncwarp();
-        const int j0 = now.j0, end = now.end;
-        const bool whole = j0 >= now.whole_from && j0 <= now.whole_to;
+        const bool whole = j0 >= whole_from && j0 <= whole_to;
         const uint32_t k_from = from + k_lane, c_from = from + c_lane, z_from = from + z_lane, even_from = from + even_lane, odd_from = from + odd_lane;
         // ---- S: keys g (0, 1) and g + 8 (2, 3), rows 2 c and 2 c + 1 ----
         float s[NT][4], widest = 0.f;
@@ -355,14 +331,17 @@ __device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, co
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[t][e] *= factor[t][e & 1];
         }
-        if (__builtin_expect(!whole, 0)) {
+        if (!whole) {
+            __syncwarp();                         // (so that it stays a branch: with predicates instead each part took 45 instructions more)
+            const Words<NG> u0 = lds<NG, kPart * St::constants>(c_from), u1 = lds<NG, (kPart + 8) * St::constants>(c_from);
+            widest = fmaxf(j0 + g < end ? widest_scale<T, NG>(u0, u0) : 0.f, j0 + g + 8 < end ? widest_scale<T, NG>(u1, u1) : 0.f);
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int j = j0 + g + 8 * (e >> 1);
-                        s[t][e] = j < end && attn_sees(pr[t][e & 1], j, window, a.attn.sinks) ? s[t][e] : -INFINITY;
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    const int j = j0 + g + 8 * (e >> 1), p = span.p0 + token_of(job.row0 + min(8 * t + 2 * c + (e & 1), job.nrows - 1));
+                    s[t][e] = j < end && attn_sees(p, j, window, a.attn.sinks) ? s[t][e] : -INFINITY;
+                }
         }
         bool grow = widest > 8.f * limit;
         float top[NT][2];
@@ -422,7 +401,8 @@ __device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, co
                     const float2 f0 = Half<T>::unpack(u0.w[n]), f1 = Half<T>::unpack(u1.w[n]);
                     sv[0][n] = f0.x; zv[0][n] = f0.y; sv[1][n] = f1.x; zv[1][n] = f1.y;
                 }
-                if (__builtin_expect(!whole, 0)) {
+                if (!whole) {
+                    __syncwarp();
 #pragma unroll
                     for (int n = 0; n < NG; ++n) {
                         if (j0 + g >= end) sv[0][n] = zv[0][n] = 0.f;
@@ -466,10 +446,16 @@ __device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, co
             }
         }
         __syncwarp();                             // (the part has been read)
-        fetch(ahead, from);
+        fetch(j0 + kStages * step, behind, from);
         from = from + St::total == ring + kStages * St::total ? ring : from + St::total;
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
+    // on to the window: the job's first part behind the sinks
+    if (!sink || last <= span.n_s) break;
+    __syncwarp();                                 // (the ring has been read)
+    sink = false;
+    enter(job.first + (span.n_s - job.first + job.step - 1) / job.step * job.step);
+    }
 }
 
 // The row once more by one warp, a few keys at a time and only those that it sees: see attn_row_again in attn.cuh, of which this is the plain form (all dims of

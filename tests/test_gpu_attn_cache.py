@@ -191,6 +191,20 @@ def test_what_is_not_seen_does_not_matter(S, T, dtype):
         check(got[0, -1, :, group:], want[0, -1, :, group:], bound[0, -1, :, group:])
 
 
+@pytest.mark.parametrize("S,T,window", [(80, 1, None), (2300, 1, None), (2300, 5, 40), (90, 6, 20), (90, 40, None)])
+def test_rows_of_an_older_text_do_not_matter(S, T, window):
+    """What lies behind the last token and in front of the window: numbers as large as there are, which must not widen what weights are scaled by."""
+    q, cache = inputs(2, T, 4, 2, 128, S, F16)
+    pos, sinks = [S - T - 7, 37], 2 if window else 0
+    want, bound = reference(q, cache, pos, window, sinks)
+    for b, p in enumerate(pos):
+        for t in (cache.k_scales, cache.v_scales):
+            t[b, :, p + T:] = 8736.0 if t is cache.v_scales else -60000.0
+            if window:
+                t[b, :, sinks:max(sinks, p - window + 1)] = 8736.0
+    check(ops.attn_cache(q, cache, at(*pos), window=window, sinks=sinks), want, bound)
+
+
 def test_queries_and_values_of_all_sizes():
     """Scales of V from the smallest to the largest, queries from 2^-20 to 2^14 in one row and between rows."""
     for dtype in (F16, BF16):
