@@ -35,8 +35,27 @@ Attn4Plan plan_of(const b200gptq_attn_cache_args& a) {
     return p;
 }
 
+// What is read back at once: all of it, as long as that is 1 GB at most, or as many key heads of sequences as have a tile of 128 rows for each SM where that is
+// more; else in turns of equal size.  (Turns that leave the rows in L2 until they have been multiplied are no gain: 2 chunks of 512 behind 3500, 72 heads of
+// 128, 311 MB at once 244 us, 4 turns of 18 heads, whose tiles fill the SMs once, 266.)
+struct Turns { int batch, heads; };          // sequences and key heads of a turn
+Turns turns_of(const b200gptq_attn_cache_args& a) {
+    const b200gptq_cache4& c = a.cache;
+    const long long tiles = ((long long)a.tokens * (a.heads / c.kv_heads) + 127) / 128, fill = (sm_count() + tiles - 1) / tiles,
+                    pairs = std::max((long long)(1e9 / (4.0 * c.max_seq * c.hd)), fill);
+    auto even = [](long long all, long long fit) {         // the smallest size with as few turns
+        const long long turns = (all + fit - 1) / fit;
+        return (int)((all + turns - 1) / turns);
+    };
+    if (pairs >= c.batch) return {c.batch, even(c.kv_heads, pairs / c.batch)};
+    return {even(c.batch, pairs), 1};
+}
+
 int64_t scratch_bytes(const b200gptq_attn_cache_args& a, const Attn4Plan& p) {
-    if (p.read) return (int64_t)a.cache.batch * a.cache.kv_heads * a.cache.max_seq * a.cache.hd * 4;
+    if (p.read) {
+        const Turns t = turns_of(a);
+        return (int64_t)t.batch * t.heads * a.cache.max_seq * a.cache.hd * 4;
+    }
     return p.flat ? 2LL * kAttn4Warps * p.ctas * 8 * p.tiles8 * (a.cache.hd + 2) * (int)sizeof(float) : 0;
 }
 
@@ -51,9 +70,7 @@ B200GPTQ_API int64_t b200gptq_attn_cache_workspace_bytes(const b200gptq_attn_cac
     if (!args) return B200GPTQ_ERR_NULL_POINTER;
     const int st = check_sizes(*args);
     if (st != B200GPTQ_OK) return st;
-    const double most = 4.0 * args->cache.batch * args->cache.kv_heads * args->cache.max_seq * args->cache.hd;
-    const Attn4Plan p = plan_of(*args);
-    return p.read && most > 9e18 ? B200GPTQ_ERR_TOO_LARGE : scratch_bytes(*args, p);
+    return scratch_bytes(*args, plan_of(*args));
 }
 
 B200GPTQ_API int b200gptq_attn_cache(const b200gptq_attn_cache_args* args, void* workspace, size_t workspace_bytes, void* stream) {
@@ -73,7 +90,7 @@ B200GPTQ_API int b200gptq_attn_cache(const b200gptq_attn_cache_args* args, void*
     if (need && (!workspace || workspace_bytes < (size_t)need)) return B200GPTQ_ERR_WORKSPACE;
     if (reinterpret_cast<uintptr_t>(workspace) & 15u) return B200GPTQ_ERR_ALIGNMENT;
     const Attn4Plan p = plan_of(a);
-    const cudaStream_t at = static_cast<cudaStream_t>(stream);
+    const cudaStream_t at_stream = static_cast<cudaStream_t>(stream);
     const b200gptq_cache4& c = a.cache;
     Attn4Args all = {};
     all.cache = c;
@@ -83,15 +100,35 @@ B200GPTQ_API int b200gptq_attn_cache(const b200gptq_attn_cache_args* args, void*
     std::copy(a.out_stride, a.out_stride + 3, f.out_stride);
     f.dtype = c.dtype; f.batch = c.batch; f.tokens = a.tokens; f.heads = a.heads; f.kv_heads = c.kv_heads; f.hd = c.hd; f.max_seq = c.max_seq;
     f.window = a.window; f.sinks = a.sinks; f.pos_each = a.pos_each; f.scale = a.scale;
-    if (!p.read) return attn4_rows_dispatch(all, static_cast<float*>(workspace), p, at);
+    if (!p.read) return attn4_rows_dispatch(all, static_cast<float*>(workspace), p, at_stream);
     f.k_cache = workspace;
     f.v_cache = static_cast<char*>(workspace) + need / 2;
-    const int64_t stride[3] = {(int64_t)c.kv_heads * c.max_seq * c.hd, (int64_t)c.max_seq * c.hd, c.hd};
-    std::copy(stride, stride + 3, f.k_stride);
-    std::copy(stride, stride + 3, f.v_stride);
+    const Turns turn = turns_of(a);
+    const int group = a.heads / c.kv_heads;
+    f.k_stride[2] = f.v_stride[2] = c.hd;
+    f.k_stride[1] = f.v_stride[1] = (int64_t)c.max_seq * c.hd;
+    f.k_stride[0] = f.v_stride[0] = turn.heads * f.k_stride[1];
     if (!attn_tiles_maps(f, false)) return B200GPTQ_ERR_TOO_LARGE;
-    st = attn4_read_back(all, workspace, static_cast<char*>(workspace) + need / 2, at);
-    return st != B200GPTQ_OK ? st : attn_tiles_dispatch(f, at);
+    for (int b = 0; b < c.batch; b += turn.batch)
+        for (int h = 0; h < c.kv_heads; h += turn.heads) {
+            Attn4Args part = all;
+            part.cache.batch = part.attn.batch = std::min(turn.batch, c.batch - b);
+            part.cache.kv_heads = part.attn.kv_heads = std::min(turn.heads, c.kv_heads - h);
+            part.attn.heads = part.attn.kv_heads * group;
+            auto at = [&](const void* p, const int64_t (&stride)[3], int size) { return const_cast<char*>(static_cast<const char*>(p)) + (b * stride[0] + h * stride[1]) * size; };
+            part.cache.k = at(c.k, c.k_stride, 1);
+            part.cache.v = at(c.v, c.v_stride, 1);
+            part.cache.k_scales = at(c.k_scales, c.k_scale_stride, 2);
+            part.cache.v_scales = at(c.v_scales, c.v_scale_stride, 2);
+            part.attn.q = static_cast<const char*>(a.q) + (b * a.q_stride[0] + (int64_t)h * group * a.q_stride[2]) * 2;
+            part.attn.out = static_cast<char*>(a.out) + (b * a.out_stride[0] + (int64_t)h * group * a.out_stride[2]) * 2;
+            if (a.pos_each) part.attn.pos = a.pos + b;
+            if (a.counts) part.attn.counts = a.counts + b;
+            st = attn4_read_back(part, workspace, static_cast<char*>(workspace) + need / 2, at_stream);
+            if (st == B200GPTQ_OK) st = attn_tiles_dispatch(part.attn, at_stream);
+            if (st != B200GPTQ_OK) return st;
+        }
+    return B200GPTQ_OK;
 }
 
 }  // extern "C"

@@ -21,7 +21,7 @@ struct Attn4Divisors { Divisor row_tiles, kv_heads, group; };
 struct Attn4Plan { bool read, flat; int tiles8, split_bits, ctas; };
 
 int attn4_rows_dispatch(const Attn4Args& a, float* part, const Attn4Plan& p, cudaStream_t stream);
-// The rows of the cache that any query sees, into k, v [batch, kv_heads, max_seq, hd] (cache4.cu).
+// The rows of the cache that any query sees, into k, v with the strides of a.attn's caches (cache4.cu).
 int attn4_read_back(const Attn4Args& a, void* k, void* v, cudaStream_t stream);
 
 }  // namespace b200gptq

@@ -3,8 +3,8 @@
 //   zero = min x,  scale = (max x - min x) / 15,  code = round((x - zero) / scale);   value = zero + scale * code
 //
 // Four lanes share a row: lane c has 8 dims of each 32, which are the codes of adjacent words (16 bytes of the row, 8 for 64 dims), 16 bytes of 16-bit values at a
-// time. They meet in two shuffles per group for its minimum and maximum. A code is first taken from the product with 1 / scale, which is off by less than
-// 2^-18, and divided out only where that is nearer than that to the middle between two codes.
+// time. They meet in two shuffles per group for its minimum and maximum, of pairs of 16-bit numbers. A code is first taken from the product with 1 / scale, which
+// is off by less than 2^-18, and divided out only where that is nearer than that to the middle between two codes.
 // Bound by the bytes of long prompts and by the launch for a decode step.
 #include <algorithm>
 
@@ -43,50 +43,69 @@ template <int N> __device__ __forceinline__ void store_words(void* at, const Wor
     else *static_cast<uint32_t*>(at) = r.w[0];
 }
 // The value of a code.  (-65504 + 15 scales is 65536 where the scale was rounded up: not an infinity in fp16.)
+template <typename T> constexpr float kLargest = std::is_same<T, __half>::value ? 65504.f : 3.38953139e38f;
 template <typename T> __device__ __forceinline__ float value_of(unsigned code, float scale, float zero) {
-    constexpr float top = std::is_same<T, __half>::value ? 65504.f : 3.38953139e38f;
     const float x = fmaf((float)code, scale, zero);
-    return x > top ? top : x;                     // (the sum of zero, which is no smaller than -top, and of something that is not negative)
+    return x > kLargest<T> ? kLargest<T> : x;                     // (the sum of zero, which is no smaller than -top, and of something that is not negative)
 }
 
-// Code of a number d >= 0 from the group's zero on, which is 15.x scales at most.
-__device__ __forceinline__ unsigned code_of(float d, float scale, float inverse) {
-    float q = d * inverse;
-    if (fabsf(q - floorf(q) - 0.5f) < 0x1p-18f) q = __fdiv_rn(d, scale);
-    return (unsigned)fminf(rintf(q), 15.f);
+// The smaller or larger of pairs of 16-bit numbers; a NaN where one of them is one.
+template <typename T> struct Pair;
+template <> struct Pair<__half> { typedef __half2 type; };
+template <> struct Pair<__nv_bfloat16> { typedef __nv_bfloat162 type; };
+template <typename T> __device__ __forceinline__ uint32_t lower2(uint32_t a, uint32_t b) {
+    using P = typename Pair<T>::type;
+    const P r = __hmin2_nan(*reinterpret_cast<const P*>(&a), *reinterpret_cast<const P*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
 }
+template <typename T> __device__ __forceinline__ uint32_t upper2(uint32_t a, uint32_t b) {
+    using P = typename Pair<T>::type;
+    const P r = __hmax2_nan(*reinterpret_cast<const P*>(&a), *reinterpret_cast<const P*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+constexpr float kRound = 12582912.f;          // 1.5 2^23: a number below 2^22 that is added to it is rounded to a whole one, ties to even
 
-// Rows: for each token the key heads, the value heads and, where queries are rotated, the query heads.
-template <typename T, int HD, int GS>
-__global__ void __launch_bounds__(kThreads)
-cache_write_kernel(const __grid_constant__ b200gptq_cache_write_args a, unsigned rows, const __grid_constant__ WriteDivisors by) {
-    constexpr int Y = HD / 32, NG = HD / GS, HH = HD / 64;
-    asm volatile("griddepcontrol.launch_dependents;");
-    const unsigned row = blockIdx.x * (unsigned)(kThreads / 4) + threadIdx.x / 4;
-    const int c = threadIdx.x & 3;
-    const unsigned token = over(min(row, rows - 1), by.rows), b = over(token, by.tokens);
-    const int per = 2 * a.cache.kv_heads + (a.q ? a.heads : 0), j = (int)(min(row, rows - 1) - token * per), t = (int)(token - b * a.tokens), kv = a.cache.kv_heads;
-    const bool is_k = j < kv, is_v = !is_k && j < 2 * kv, is_q = !is_k && !is_v;
-    const int head = is_k ? j : is_v ? j - kv : j - 2 * kv;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const long long start = __ldcg(reinterpret_cast<const long long*>(a.pos) + (a.pos_each ? b : 0));
-    const long long count = a.counts ? __ldcg(reinterpret_cast<const long long*>(a.counts) + b) : a.tokens;
-    const T* src = (is_k   ? static_cast<const T*>(a.k) + b * a.k_stride[0] + t * a.k_stride[1] + head * a.k_stride[2]
-                    : is_v ? static_cast<const T*>(a.v) + b * a.v_stride[0] + t * a.v_stride[1] + head * a.v_stride[2]
-                           : static_cast<const T*>(a.q) + b * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2]) + 8 * c;
-    uint4 raw[Y];                                 // (a row of padding is read too: it is there)
+// A lane's part of a row.  Rows: for each token the key heads, the value heads and, where queries are rotated, the query heads.
+template <typename T, int HD> struct WriteRow {
+    static constexpr int Y = HD / 32, HH = HD / 64;
+    unsigned b;
+    int t, head, c, p;
+    bool is_k, is_v, is_q, there, valid;
+    uint4 raw[Y];
+    uint2 cos_w[Y], sin_w[Y];
+
+    __device__ __forceinline__ void place(const b200gptq_cache_write_args& a, unsigned row, unsigned rows, const WriteDivisors& by) {
+        c = threadIdx.x & 3;
+        there = row < rows;
+        row = min(row, rows - 1);
+        const unsigned token = over(row, by.rows);
+        const int per = 2 * a.cache.kv_heads + (a.q ? a.heads : 0), j = (int)(row - token * per), kv = a.cache.kv_heads;
+        b = over(token, by.tokens);
+        t = (int)(token - b * a.tokens);
+        is_k = j < kv; is_v = !is_k && j < 2 * kv; is_q = !is_k && !is_v;
+        head = is_k ? j : is_v ? j - kv : j - 2 * kv;
+    }
+    __device__ __forceinline__ void fetch(const b200gptq_cache_write_args& a) {
+        const long long start = __ldcg(reinterpret_cast<const long long*>(a.pos) + (a.pos_each ? b : 0));
+        const long long count = a.counts ? __ldcg(reinterpret_cast<const long long*>(a.counts) + b) : a.tokens;
+        const T* src = (is_k   ? static_cast<const T*>(a.k) + b * a.k_stride[0] + t * a.k_stride[1] + head * a.k_stride[2]
+                        : is_v ? static_cast<const T*>(a.v) + b * a.v_stride[0] + t * a.v_stride[1] + head * a.v_stride[2]
+                               : static_cast<const T*>(a.q) + b * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2]) + 8 * c;
 #pragma unroll
-    for (int y = 0; y < Y; ++y) raw[y] = *reinterpret_cast<const uint4*>(src + 32 * y);
-    // (a position near the end of 64 bits must not wrap around to one in the cache)
-    const bool valid = row < rows && t < count && start < a.cache.max_seq && start >= -(long long)t && start + t < a.cache.max_seq && (!a.cos_t || start + t < a.angles);
-    const int p = valid ? (int)(start + t) : 0;
-    const bool turn = a.cos_t && !is_v;
-    if (turn) {
-        const T *cos_t = static_cast<const T*>(a.cos_t) + (long long)p * (HD / 2) + 4 * c, *sin_t = static_cast<const T*>(a.sin_t) + (long long)p * (HD / 2) + 4 * c;
+        for (int y = 0; y < Y; ++y) raw[y] = *reinterpret_cast<const uint4*>(src + 32 * y);       // (a row of padding is read too: it is there)
+        // (a position near the end of 64 bits must not wrap around to one in the cache)
+        valid = there && t < count && start < a.cache.max_seq && start >= -(long long)t && start + t < a.cache.max_seq && (!a.cos_t || start + t < a.angles);
+        p = valid ? (int)(start + t) : 0;
+        if (a.cos_t && !is_v) {
+            const T *cos_t = static_cast<const T*>(a.cos_t) + (long long)p * (HD / 2) + 4 * c, *sin_t = static_cast<const T*>(a.sin_t) + (long long)p * (HD / 2) + 4 * c;
+#pragma unroll
+            for (int y = 0; y < Y; ++y) { cos_w[y] = *reinterpret_cast<const uint2*>(cos_t + 16 * y); sin_w[y] = *reinterpret_cast<const uint2*>(sin_t + 16 * y); }
+        }
+    }
+    __device__ __forceinline__ void turn() {
 #pragma unroll
         for (int y = 0; y < Y; ++y) {
-            const uint2 cw = *reinterpret_cast<const uint2*>(cos_t + 16 * y), sw = *reinterpret_cast<const uint2*>(sin_t + 16 * y);
-            const uint32_t cs[2] = {cw.x, cw.y}, sn[2] = {sw.x, sw.y};
+            const uint32_t cs[2] = {cos_w[y].x, cos_w[y].y}, sn[2] = {sin_w[y].x, sin_w[y].y};
             float x[8];
             unpack8<T>(raw[y], x);
 #pragma unroll
@@ -100,66 +119,94 @@ cache_write_kernel(const __grid_constant__ b200gptq_cache_write_args a, unsigned
             raw[y] = pack8<T>(x);
         }
     }
-    if (valid && is_q) {
-        T* dst = static_cast<T*>(a.q_out) + b * a.q_out_stride[0] + t * a.q_out_stride[1] + head * a.q_out_stride[2] + 8 * c;
+    template <int GS> __device__ __forceinline__ void store(const b200gptq_cache_write_args& a) {
+        constexpr int NG = HD / GS;
+        if (a.cos_t && !is_v) turn();
+        if (valid && is_q) {
+            T* dst = static_cast<T*>(a.q_out) + b * a.q_out_stride[0] + t * a.q_out_stride[1] + head * a.q_out_stride[2] + 8 * c;
 #pragma unroll
-        for (int y = 0; y < Y; ++y) *reinterpret_cast<uint4*>(dst + 32 * y) = raw[y];
-    }
-    if (!__any_sync(0xffffffffu, valid && !is_q)) return;
-    Words<2 * HH> word = {};                      // of gg = 2 c + x, half h: 2 x + h (64 dims: x)
-    Words<NG> constants;
-    T* out = static_cast<T*>(is_k ? a.k_out : a.v_out);
-    const bool writes = valid && !is_q;
-    if (out && writes) out += (is_k ? b * a.k_out_stride[0] + t * a.k_out_stride[1] + head * a.k_out_stride[2] : b * a.v_out_stride[0] + t * a.v_out_stride[1] + head * a.v_out_stride[2]) + 8 * c;
+            for (int y = 0; y < Y; ++y) *reinterpret_cast<uint4*>(dst + 32 * y) = raw[y];
+        }
+        const bool writes = valid && !is_q;
+        if (!__any_sync(0xffffffffu, writes)) return;
+        Words<2 * HH> word = {};                  // of words (HD / 64) (2 c + x) + h of the row: HH x + h
+        Words<NG> constants;
+        T* out = static_cast<T*>(is_k ? a.k_out : a.v_out);
+        if (out && writes)
+            out += (is_k ? b * a.k_out_stride[0] + t * a.k_out_stride[1] + head * a.k_out_stride[2] : b * a.v_out_stride[0] + t * a.v_out_stride[1] + head * a.v_out_stride[2]) + 8 * c;
 #pragma unroll
-    for (int n = 0; n < NG; ++n) {                // a group: 32 dims or 64
-        constexpr int SPAN = GS / 32;
-        float x[SPAN][8], lo = INFINITY, hi = -INFINITY;
-        bool finite = true;
+        for (int n = 0; n < NG; ++n) {            // a group: 32 dims or 64
+            constexpr int SPAN = GS / 32;
+            uint32_t lo = raw[SPAN * n].x, hi = lo;
 #pragma unroll
-        for (int y = 0; y < SPAN; ++y) {
-            unpack8<T>(raw[SPAN * n + y], x[y]);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                lo = fminf(lo, x[y][e]);
-                hi = fmaxf(hi, x[y][e]);
-                finite = finite && isfinite(x[y][e]);
+            for (int y = 0; y < SPAN; ++y) {
+                const uint4 v = raw[SPAN * n + y];
+                lo = lower2<T>(lower2<T>(lo, v.x), lower2<T>(lower2<T>(v.y, v.z), v.w));
+                hi = upper2<T>(upper2<T>(hi, v.x), upper2<T>(upper2<T>(v.y, v.z), v.w));
             }
-        }
 #pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        }
-        const unsigned odd = __ballot_sync(0xffffffffu, !finite) >> (threadIdx.x & 28) & 15u;
-        float scale = Half<T>::wide(Half<T>::round(__fdiv_rn(__fsub_rn(hi, lo), 15.f))), zero = lo;
-        if (odd || !isfinite(scale)) scale = zero = __int_as_float(0x7fc00000);
-        constants.w[n] = Half<T>::pack(scale, zero);
-        const float inverse = __frcp_rn(scale);
+            for (int o = 1; o < 4; o <<= 1) {
+                lo = lower2<T>(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+                hi = upper2<T>(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+            }
+            const float2 lo2 = Half<T>::unpack(lower2<T>(lo, lo >> 16 | lo << 16)), hi2 = Half<T>::unpack(upper2<T>(hi, hi >> 16 | hi << 16));
+            float scale = Half<T>::wide(Half<T>::round(__fdiv_rn(__fsub_rn(hi2.x, lo2.x), 15.f))), zero = lo2.x;
+            if (!isfinite(scale)) scale = zero = __int_as_float(0x7fc00000);
+            constants.w[n] = Half<T>::pack(scale, zero);
+            // (a scale of zero: all codes are 0; one that is subnormal in fp32, bf16 below 2^-126, has no reciprocal there)
+            const float inverse = scale > 0.f ? __frcp_rn(scale) : 0.f;
+            const bool high = fmaf(15.f, scale, zero) > kLargest<T> || !(inverse < INFINITY);
 #pragma unroll
-        for (int y = 0; y < SPAN; ++y) {
-            const int at = SPAN * n + y, h = at >> 1;
+            for (int y = 0; y < SPAN; ++y) {
+                const int at = SPAN * n + y, h = at >> 1;
+                float x[8], code[8], off = 0.f;
+                unpack8<T>(raw[at], x);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                // (a scale that is subnormal in fp32 has no reciprocal there: bf16 below 2^-126)
-                const float d = __fsub_rn(x[y][e], zero);
-                const unsigned code = !(scale > 0.f) ? 0u : inverse < INFINITY ? code_of(d, scale, inverse) : (unsigned)fminf(rintf(__fdiv_rn(d, scale)), 15.f);
+                for (int e = 0; e < 8; ++e) {
+                    const float d = __fsub_rn(x[e], zero), q = fminf(d * inverse, 15.f);
+                    code[e] = __fsub_rn(__fadd_rn(q, kRound), kRound);
+                    off = fmaxf(off, fabsf(q - code[e]));
+                }
+                if (off > 0.5f - 0x1p-18f || high) {           // near the middle between two codes, or a range that is not ordinary: by the definition
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) code[e] = scale > 0.f ? fminf(rintf(__fdiv_rn(__fsub_rn(x[e], zero), scale)), 15.f) : 0.f;
+                }
                 // fields of dims 0, 2 (of four), 1, 3: 0, 1, 4, 5; in the second half of 64 dims two further on
-                word.w[HH * (e >> 2) + h] |= code << 4 * ((at & 1) * 2 + (e & 1) * 4 + (e & 3) / 2);
-                x[y][e] = value_of<T>(code, scale, zero);
+#pragma unroll
+                for (int x4 = 0; x4 < 2; ++x4) {
+                    const float *c4 = code + 4 * x4;
+                    const unsigned two = __float_as_uint(__fadd_rn(fmaf(c4[2], 16.f, c4[0]), kRound)) & 0xffu, other = __float_as_uint(__fadd_rn(fmaf(c4[3], 16.f, c4[1]), kRound)) & 0xffu;
+                    word.w[HH * x4 + h] |= (two | other << 16) << (at & 1) * 8;
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = fmaf(code[e], scale, zero);
+                if (high)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = value_of<T>((unsigned)code[e], scale, zero);
+                if (out && writes) *reinterpret_cast<uint4*>(out + 32 * at) = pack8<T>(x);
             }
-            if (out && writes) *reinterpret_cast<uint4*>(out + 32 * at) = pack8<T>(x[y]);
         }
+        if (!writes) return;
+        const b200gptq_cache4& cache = a.cache;
+        uint8_t* codes = static_cast<uint8_t*>(is_k ? cache.k : cache.v) + (is_k ? b * cache.k_stride[0] + head * cache.k_stride[1] + p * cache.k_stride[2]
+                                                                                 : b * cache.v_stride[0] + head * cache.v_stride[1] + p * cache.v_stride[2]);
+        store_words<2 * HH>(codes + 8 * HH * c, word);
+        if (c == 0)
+            store_words<NG>(static_cast<T*>(is_k ? cache.k_scales : cache.v_scales) + (is_k ? b * cache.k_scale_stride[0] + head * cache.k_scale_stride[1] + p * cache.k_scale_stride[2]
+                                                                                            : b * cache.v_scale_stride[0] + head * cache.v_scale_stride[1] + p * cache.v_scale_stride[2]),
+                            constants);
     }
-    if (!writes) return;
-    const b200gptq_cache4& cache = a.cache;
-    uint8_t* codes = static_cast<uint8_t*>(is_k ? cache.k : cache.v) + (is_k ? b * cache.k_stride[0] + head * cache.k_stride[1] + p * cache.k_stride[2]
-                                                                             : b * cache.v_stride[0] + head * cache.v_stride[1] + p * cache.v_stride[2]);
-    store_words<2 * HH>(codes + 8 * HH * c, word);
-    if (c == 0)
-        store_words<NG>(static_cast<T*>(is_k ? cache.k_scales : cache.v_scales) + (is_k ? b * cache.k_scale_stride[0] + head * cache.k_scale_stride[1] + p * cache.k_scale_stride[2]
-                                                                                        : b * cache.v_scale_stride[0] + head * cache.v_scale_stride[1] + p * cache.v_scale_stride[2]),
-                        constants);
+};
+
+template <typename T, int HD, int GS>
+__global__ void __launch_bounds__(kThreads)
+cache_write_kernel(const __grid_constant__ b200gptq_cache_write_args a, unsigned rows, const __grid_constant__ WriteDivisors by) {
+    asm volatile("griddepcontrol.launch_dependents;");
+    WriteRow<T, HD> row;
+    row.place(a, blockIdx.x * (unsigned)(kThreads / 4) + threadIdx.x / 4, rows, by);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    row.fetch(a);
+    row.template store<GS>(a);
 }
 
 // Lane c's part of a row back in 16 bits.
@@ -214,7 +261,7 @@ cache_read_kernel(const __grid_constant__ b200gptq_cache_read_args a, unsigned c
     read_rows<T, HD, GS>(a.cache, b, head, is_k, j0, [&](int j) { return j < length; }, [&](int j) { return out + j * stride; });
 }
 
-// For prompts: the rows that the tokens see between them, into dense k and v [batch, kv_heads, max_seq, hd].
+// For prompts: the rows that the tokens see between them, into k and v with the strides of the attention's caches.
 template <typename T, int HD, int GS>
 __global__ void __launch_bounds__(kThreads)
 cache_read_seen_kernel(const __grid_constant__ Attn4Args a, T* __restrict__ k, T* __restrict__ v, unsigned chunks, const __grid_constant__ Divisor by_chunks,
@@ -227,7 +274,7 @@ cache_read_seen_kernel(const __grid_constant__ Attn4Args a, T* __restrict__ k, T
     const int p0 = attn_pos(a.attn, b), count = attn_count(a.attn, b);
     const AttnRange r = attn_range(p0, p0 + count - 1, a.attn.window ? a.attn.window : 1 << 30, a.attn.sinks, a.cache.max_seq);
     const int end = count ? min(r.w_end, a.cache.max_seq) : 0;
-    T* out = (is_k ? k : v) + (long long)pair * a.cache.max_seq * HD;
+    T* out = (is_k ? k : v) + b * a.attn.k_stride[0] + head * a.attn.k_stride[1];
     read_rows<T, HD, GS>(a.cache, b, head, is_k, j0, [&](int j) { return j < end && (j < r.s_end || j >= r.w_start); }, [&](int j) { return out + (long long)j * HD; });
 }
 

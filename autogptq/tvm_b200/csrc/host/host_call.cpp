@@ -437,22 +437,22 @@ void need_no_gradients(PyObject* const* args, const char* const* names, int coun
     }
 }
 const void* data_of(const at::Tensor& t) { return t.unsafeGetTensorImpl()->data(); }
-// Whether the memory between the first and the last element of the two has a byte in common.
-bool overlap(const at::Tensor& x, const at::Tensor& y) {
-    auto span = [](const at::Tensor& t, uintptr_t& lo, uintptr_t& hi) {
+// The memory between a tensor's first and last element, and whether that of two has a byte in common.
+struct Memory {
+    uintptr_t lo = 0, hi = 0;
+    Memory() = default;
+    explicit Memory(const at::Tensor& t) {
         int64_t last = 0;
         for (int64_t i = 0; i < t.dim(); ++i) {
-            if (t.size(i) == 0) { lo = hi = 0; return; }
+            if (t.size(i) == 0) return;
             last += (t.size(i) - 1) * t.stride(i);
         }
         lo = (uintptr_t)data_of(t);
         hi = lo + (uintptr_t)((last + 1) * t.element_size());
-    };
-    uintptr_t a, b, c, d;
-    span(x, a, b);
-    span(y, c, d);
-    return a < d && c < b;
-}
+    }
+    bool meets(const Memory& o) const { return lo < o.hi && o.lo < hi; }
+};
+bool overlap(const at::Tensor& x, const at::Tensor& y) { return Memory(x).meets(Memory(y)); }
 // Whether the elements of each dimension lie apart: a dimension's stride passes all that the dimensions of smaller strides reach.
 bool apart_from_itself(const at::Tensor& t) {
     c10::SmallVector<std::pair<int64_t, int64_t>, 4> dims;         // (stride, size)
@@ -700,9 +700,6 @@ void cache_of(const at::Tensor* const (&t)[4], const char* const* names, bool wr
         *at[i] = const_cast<void*>(data_of(x));
         strides_of(x, *stride[i], {0, 1, 2});
     }
-    if (written)
-        for (int i = 0; i < 4; ++i)
-            for (int j = 0; j < i; ++j) need(!overlap(*t[i], *t[j]), names[i], "must not overlap another part of the cache");
     c.dtype = type == at::kHalf ? B200GPTQ_F16 : B200GPTQ_BF16;
     c.batch = (int)B; c.kv_heads = (int)KV; c.max_seq = (int)S; c.hd = (int)hd; c.group = (int)(hd / groups);
 }
@@ -765,11 +762,14 @@ PyObject* write_checked(PyObject* const* args) {
         *r.at = data_of(*x);
         strides_of(*x, *r.stride, {0, 1, 2});
     }
-    // what is written overlaps nothing else: the cache (2 .. 5), q_out, k_out, v_out
+    // what is written overlaps nothing else: the cache (2 .. 5, whose parts have been found apart from themselves), q_out, k_out, v_out
+    Memory memory[14];
+    for (int i = 0; i < 14; ++i)
+        if (t[i]) memory[i] = Memory(*t[i]);
     for (int i : {2, 3, 4, 5, 11, 12, 13}) {
         if (!t[i]) continue;
         bool apart = i < 6 || apart_from_itself(*t[i]);
-        for (int j = 0; j < 14; ++j) apart = apart && (j == i || !t[j] || (i < 6 && j >= 2 && j < 6) || !overlap(*t[i], *t[j]));
+        for (int j = 0; j < 14; ++j) apart = apart && (j == i || !memory[i].meets(memory[j]));
         need(apart, names[i], "must not overlap another tensor, nor itself");
     }
     a.tokens = (int)T;

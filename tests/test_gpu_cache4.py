@@ -173,6 +173,23 @@ def test_ranges_at_the_edges(dtype, group):
     assert torch.equal(out[0, :3].cpu(), x[0, :3].cpu())     # one value, or two zeros
 
 
+@pytest.mark.parametrize("group", [32, 64])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_values_near_the_largest_number(dtype, group):
+    """A scale that was rounded up puts the last code above the type's largest number; what comes out is that number."""
+    top = torch.finfo(dtype).max
+    x = torch.zeros(40, 128)
+    for i in range(40):
+        x[i] = top * torch.linspace(0.02 * i, 1, 128)
+    x = x.to(dtype).to(DEV)[None, :, None]
+    cache, out = ops.QuantCache.empty(1, 1, 40, 128, group, dtype, DEV), torch.empty_like(x)
+    ops.cache_write(cache, x, -x, at(0), k_out=out, v_out=torch.empty_like(x))
+    assert bool(torch.isfinite(out).all()) and torch.equal(out[0, :, 0].double().cpu(), rounded(values(cache, "k")[0, 0], dtype))
+    assert float((values(cache, "k") > top).double().sum()) > 0                # (there are such)
+    assert torch.equal(codes_of(cache.k)[0, 0], defined(x, group)[0][0, :, 0]) and torch.equal(codes_of(cache.v)[0, 0], defined(-x, group)[0][0, :, 0])
+    assert all(bool(torch.isfinite(t).all()) for t in ops.cache_read(cache))
+
+
 def test_padding_and_positions_outside():
     B, T, kv, hd, S = 6, 4, 2, 64, 10
     k, v = rows(B, T, kv, hd, dtype=F16), rows(B, T, kv, hd, dtype=F16, seed=1)
