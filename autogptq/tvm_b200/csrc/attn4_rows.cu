@@ -7,7 +7,8 @@
 // exact), so eight codes cost a shift and four masks.  Scales and zeros are applied beside the products:
 //   S(key, row) = sum over groups of  sK (q . cK) + zK (sum of q)      one product chain per group, then an fp32 FMA; the zeros in a product of their own, with
 //                                                                      the sums of q in two numbers each (16 bits or more together)
-//   O(dim, row) = sum over keys of  (w sV) cV + w zV                   w sV is what is rounded to fp16; w zV is summed in fp32, per group
+//   O(dim, row) = sum over keys of  (w sV) (cV - 8) + w (zV + 8 sV)    w sV is what is rounded to fp16, and codes of both signs make half of its error of codes from 0 to 15
+//                                                                      (by one subtraction in fp16, exact); the second term is summed in fp32, per group
 // Q is scaled by a power of two per row (to below 2^15, exact for what is above 2^-38 of the row's largest; so bf16 queries are exact in fp16), w sV by one per
 // warp that follows the largest scale seen, so neither leaves fp16's range.
 //
@@ -94,6 +95,13 @@ template <int HD, int GS, int NT> struct Lay {
                          flags = slice_ml + 2 * kAttn4MaxSplit * R, total = flags + R;
     static_assert(slice % 4 == 0 && q % 4 == 0 && warp % 4 == 0, "");
 };
+
+// Two codes less 8, in units of 2^-24 (or 16 times that): exact.
+template <unsigned EIGHT> __device__ __forceinline__ uint32_t centred(uint32_t codes) {
+    constexpr uint32_t eight = EIGHT | EIGHT << 16;
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&codes), *reinterpret_cast<const __half2*>(&eight));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
 
 // The largest scale of two rows' constants, (scale, zero) in a word each, which are compared together; NaN counts for nothing.
 template <typename T, int N> __device__ __forceinline__ float widest_scale(const Words<N>& u, const Words<N>& v) {
@@ -399,7 +407,7 @@ __device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, co
 #pragma unroll
                 for (int n = 0; n < NG; ++n) {
                     const float2 f0 = Half<T>::unpack(u0.w[n]), f1 = Half<T>::unpack(u1.w[n]);
-                    sv[0][n] = f0.x; zv[0][n] = f0.y; sv[1][n] = f1.x; zv[1][n] = f1.y;
+                    sv[0][n] = f0.x; zv[0][n] = fmaf(8.f, f0.x, f0.y); sv[1][n] = f1.x; zv[1][n] = fmaf(8.f, f1.x, f1.y);
                 }
                 if (!whole) {
                     __syncwarp();
@@ -439,8 +447,9 @@ __device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, co
 #pragma unroll
                     for (int z = 0; z < 2; ++z) {
                         const uint32_t k01 = x[z][0] >> (8 * y), k89 = x[z][1] >> (8 * y);
+                        const uint32_t a0 = centred<8>(k01 & kLow), a1 = centred<128>(k01 & kHigh), a2 = centred<8>(k89 & kLow), a3 = centred<128>(k89 & kHigh);
 #pragma unroll
-                        for (int t = 0; t < NT; ++t) mma16(acc[t][4 * h + 2 * y + z], k01 & kLow, k01 & kHigh, k89 & kLow, k89 & kHigh, b0[t], b1[t]);
+                        for (int t = 0; t < NT; ++t) mma16(acc[t][4 * h + 2 * y + z], a0, a1, a2, a3, b0[t], b1[t]);
                     }
                 }
             }

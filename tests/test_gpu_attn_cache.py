@@ -1,11 +1,12 @@
 """Attention over a cache in 4 bits (ops.attn_cache), against 64 bits.
 
 The bound, per output element, with u = half a step of the type (2^-11 fp16, 2^-8 bf16), K and V the values zero + scale code that the cache stands for,
-|K|+ = |zero| + scale code (the two are added up apart), A = sum_j w_j |V_j|+ / sum_j w_j, s the largest scale of V and n visible keys:
+|K|+ = |zero| + scale code, |V|+ = |zero + 8 scale| + scale |code - 8| (each as the two that are added up apart), A = sum_j w_j |V_j|+ / sum_j w_j, s the largest scale of V
+and n visible keys:
 
     u |o|                             the result's rounding
-    + 2^-11 A                         each weight times scale is rounded to fp16 before it multiplies a code (relative)
-    + n 2^-25 15 s                    and below 2^-14 of the largest scale to half a step of fp16's subnormal numbers; codes are 15 at most
+    + 2^-11 A                         each weight times scale is rounded to fp16 before it multiplies a code less 8 (relative)
+    + n 2^-25 8 s                     and below 2^-14 of the largest scale to half a step of fp16's subnormal numbers; codes less 8 are 8 at most
     + 2 d A                           d: error of a score in fp32, hd products and sums, each off by 2^-22 of the sum of |q| |K|+ at most
                                       (2^-24 for rounded sums; the tensor cores may truncate), which moves a weight and the denominator
     + (n 2^-22 + 2^-18) A             sums of n products in fp32 likewise; exp2, scale, merging of parts: a few steps of 2^-22 each
@@ -60,13 +61,15 @@ def reference(q, cache, pos, window=None, sinks=0, scale=None, counts=None):
                 n = int(seen.sum())
                 if n == 0:
                     continue
-                K, V, Kp, Vp = kc[seen] + kz[seen], vc[seen] + vz[seen], kc[seen] + kz[seen].abs(), vc[seen] + vz[seen].abs()
+                K, V, Kp = kc[seen] + kz[seen], vc[seen] + vz[seen], kc[seen] + kz[seen].abs()
+                eight = 8 * cache.v_scales[b, h][seen][..., 0].double().repeat_interleave(hd // cache.v_scales.shape[3], -1)
+                Vp = (vz[seen] + eight).abs() + (vc[seen] - eight).abs()
                 Q = q[b, t, h * G:h * G + G].double()
                 w = torch.softmax(Q @ K.t() * scale, dim=1)
                 o, A = w @ V, w @ Vp
                 d = hd * 2.0 ** -22 * (Q.abs() @ Kp.t()).amax(1, keepdim=True) * abs(scale)
                 top = cache.v_scales[b, h][seen][..., 0].double().amax()
-                err = u * o.abs() + n * 2.0 ** -25 * 15 * top + 2.0 ** -11 * A
+                err = u * o.abs() + n * 2.0 ** -25 * 8 * top + 2.0 ** -11 * A
                 if many:
                     d = d + u * (Q.abs() @ K.abs().t()).amax(1, keepdim=True) * abs(scale)
                     err = err + 2 * u * A + (n * 2.0 ** -25 * V.abs().max() if q.dtype is F16 else 0)

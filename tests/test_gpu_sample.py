@@ -116,6 +116,21 @@ def test_a_border_among_equal_logits(dtype):
         check(few, u, **kw)
 
 
+@pytest.mark.parametrize("dtype,V", [(F32, 1 << 18), (F32, 150001), (F16, 1 << 18), (F16, 9000)])
+def test_a_crowd_of_equal_logits_below_the_largest(dtype, V):
+    """Sums of one number many times over, whose bits do not end: nothing passes over in the bins."""
+    x = torch.full((6, V), -1.2345, device=DEV)
+    x[:, 77], x[:, 4001] = 0.0, -0.3
+    x[5, ::2] = -1.5
+    u = torch.tensor([0.1234, 0.5555, 0.91, 0.3, 0.77, 0.6], device=DEV)
+    p = torch.tensor([0.5, 0.31, 0.9, 0.777, 0.123, 0.66], device=DEV)
+    k = torch.tensor([V // 2, V // 3, 5000, V - 3, 100, V - V // 3], device=DEV)
+    x = x.to(dtype)
+    check(x, u, top_p=p)
+    check(x, u, top_k=k)
+    check(x, u, top_p=p, top_k=k, temperature=torch.full((6,), 0.9, device=DEV))
+
+
 def test_values_around_zero_and_of_all_sizes():
     """The bits of x between two close values span many powers of two near zero."""
     g = torch.Generator().manual_seed(4)
