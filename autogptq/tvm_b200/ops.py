@@ -551,8 +551,8 @@ def sample(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None
     weights make up ``top_p`` of theirs (1: all), and of these the ones of weight ``min_p`` at least (the largest weight is 1); equal logits count from the lowest token on.  The
     token is the lowest for which the kept weights up to it pass ``uniform`` times all of them.  Temperature 0: the lowest token of the largest logit.
 
-    ``uniform``, ``temperature``, ``top_p``, ``min_p`` fp32 ``[rows]``, ``top_k`` int64 ``[rows]``, all on the device.  The borders are exact: weights are integers in units
-    of 2^-45 of the largest or less, whose sums have no rounding.  A NaN counts as minus infinity.  Returns int64 ``[rows]``."""
+    ``uniform``, ``temperature``, ``top_p``, ``min_p`` fp32 ``[rows]``, ``top_k`` int64 ``[rows]``, all on the device.  Weights are integers in units of 2^-44 of
+    the largest or less, off by 2^-32 of themselves at most, and what follows from them has no rounding.  A NaN counts as minus infinity.  Returns int64 ``[rows]``."""
     return _checked(_lib._host.sample(logits, uniform, temperature, top_k, top_p, min_p, out), "b200gptq_sample")
 
 

@@ -575,8 +575,8 @@ B200GPTQ_API int b200gptq_adjust_logits(const b200gptq_logit_args* args, void* s
  *   of weight min_p at least, the largest weight being 1 (the first one always).
  * The token is the lowest v for which the kept weights of tokens 0 .. v add up to more than uniform times all kept weights (uniform below 0 counts as 0, 1 or more
  * as the largest number below 1).  A temperature of 0 (or anything that is not 1e-18 at least), and top_k 1, give the lowest token of the largest logit.
- * Weights are integers in units of 2^-F, F = min(49, 62 - ceil(log2 vocab)), and everything that follows from them is exact, whatever the order; so a weight below
- * 2^-(F + 1) is zero.  A NaN counts as minus infinity; where the largest logit is plus infinity, the tokens that have it share all the weight; a row without any
+ * Weights are integers in units of 2^-F, F = min(49, 62 - ceil(log2 vocab)), each off by half a unit and 2^-32 of itself at most; everything that follows from them
+ * is exact, whatever the order.  A weight below 2^-(F + 1) is zero.  A NaN counts as minus infinity; where the largest logit is plus infinity, the tokens that have it share all the weight; a row without any
  * number gives the lowest token of the largest logit, or 0.
  *   dtype      B200GPTQ_F16, _BF16 or _F32, of logits [rows, vocab] with a row stride (elements);  vocab up to 2^18
  *   uniform    device fp32 [rows];  temperature, top_p, min_p  device fp32 [rows], each NULL for 1, 1, 0;  top_k  device int64 [rows] or NULL for 0

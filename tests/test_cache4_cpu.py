@@ -93,3 +93,44 @@ def test_sampling_refuses():
         a = _lib.SampleArgs(**{**good, **change})
         assert _lib.lib.b200gptq_sample(ctypes.byref(a), None) == status, change
     assert _lib.lib.b200gptq_sample(None, None) == -1
+
+
+def arguments(op):
+    """(call, its tensors by name), of sizes that fit."""
+    h = dict(dtype=torch.float16)
+    if op == "sample":
+        return ops.sample, dict(logits=torch.zeros(2, 40, **h), uniform=torch.zeros(2), temperature=torch.ones(2), top_k=torch.zeros(2).long(), top_p=torch.ones(2), min_p=torch.zeros(2),
+                                out=torch.zeros(2).long())
+    c = ops.QuantCache.empty(2, 2, 9, 64, 32, device="cpu")
+    t = dict(k=c.k, v=c.v, k_scales=c.k_scales, v_scales=c.v_scales)
+    rows = {n: torch.zeros(2, 1, 2, 64, **h) for n in ("k", "v", "q", "q_out", "k_out", "v_out")}
+    parts = {f"cache.{n}": x for n, x in t.items()}
+
+    def with_cache(call):
+        return lambda **kw: call(cache=ops.QuantCache(*(kw.pop(f"cache.{n}") for n in t)), **kw)
+
+    if op == "write":
+        return with_cache(ops.cache_write), dict(parts, **rows, pos=torch.zeros(1).long(), cos=torch.ones(9, 32, **h), sin=torch.zeros(9, 32, **h))
+    if op == "read":
+        return with_cache(ops.cache_read), dict(parts, k_out=torch.zeros(2, 2, 9, 64, **h), v_out=torch.zeros(2, 2, 9, 64, **h))
+    return with_cache(ops.attn_cache), dict(parts, q=torch.zeros(2, 1, 4, 64, **h), pos=torch.zeros(1).long(), out=torch.zeros(2, 1, 4, 64, **h))
+
+
+FLOATS = [(op, n) for op in ("write", "read", "attend", "sample") for n, t in arguments(op)[1].items() if t.is_floating_point()]
+
+
+@pytest.mark.parametrize("op,name", FLOATS)
+def test_a_gradient_or_a_tangent_is_never_dropped(op, name):
+    """There is no derivative: whichever tensor asks for one, the constants of a cache too, is refused (before the device is looked at)."""
+    from torch.autograd import forward_ad
+    call, t = arguments(op)
+    plain = t[name]
+    with forward_ad.dual_level():
+        t[name] = forward_ad.make_dual(plain, torch.ones_like(plain))
+        with torch.no_grad(), pytest.raises(RuntimeError, match="carries a tangent"):
+            call(**t)
+    t[name] = plain.requires_grad_()
+    with pytest.raises(RuntimeError, match=f"{name} requires a gradient"):
+        call(**t)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+        call(**t)

@@ -1,7 +1,8 @@
 """Sampling (ops.sample) against the definition in 64 bits, whole numbers: no tolerance.
 
 A token may only differ from the definition's where a random number, a share of top-p or min-p falls within rounding of a border.  The kernel's weights are off by
-half a unit of 2^-F each (F is 45 at 100000 tokens) and 64 bits by 2^-52 relative; the reference says for each row whether any decision lay within 2^-30 of a
+2^-32 of themselves and half a unit of 2^-F each (F is 45 at 100000 tokens), so two sums differ by 2^-31 of themselves
+and 2^-46 per token at most, and 64 bits by 2^-52 relative; the reference says for each row whether any decision lay within 2^-30 of a
 border, and such rows are not drawn: the seeds here have none (asserted).
 """
 import math
