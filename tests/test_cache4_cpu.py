@@ -68,20 +68,26 @@ def test_a_cache_and_its_size():
 def test_attention_refuses():
     good = dict(q=A, out=A, pos=A, tokens=1, heads=4, window=8, scale=1.0)
 
-    def call(change, cache=None, need=None):
+    def arguments_of(change, cache=None):
         a = _lib.AttnCacheArgs(cache=cache4(**(cache or {})), **{**good, **{k: v for k, v in change.items() if "stride" not in k}})
         for n in ("q_stride", "out_stride"):
             setattr(a, n, (ctypes.c_int64 * 3)(*change.get(n, (256, 256, 64))))
-        return _lib.lib.b200gptq_attn_cache(ctypes.byref(a), None, 0, None), _lib.lib.b200gptq_attn_cache_workspace_bytes(ctypes.byref(a))
+        return ctypes.byref(a)
+
+    def call(change, cache=None):              # (never with what is not refused: the addresses are made up, and there may be a GPU)
+        return _lib.lib.b200gptq_attn_cache(arguments_of(change, cache), None, 0, None)
+
+    def scratch(change):
+        return _lib.lib.b200gptq_attn_cache_workspace_bytes(arguments_of(change))
 
     for change, status in [(dict(q=None), -1), (dict(out=None), -1), (dict(pos=None), -1), (dict(tokens=0), -3), (dict(heads=3), -3), (dict(heads=0), -3), (dict(window=-1), -3),
                            (dict(sinks=-1), -3), (dict(window=0, sinks=2), -3), (dict(tokens=1 << 29), -8), (dict(window=(1 << 29) + 1), -8), (dict(q=A + 8), -4), (dict(out=A + 2), -4),
                            (dict(pos=A + 4), -4), (dict(counts=A + 4), -4), (dict(status=A + 2), -4), (dict(q_stride=(256, 256, 4)), -4), (dict(out_stride=(4, 256, 64)), -4),
                            (dict(tokens=64), -5)]:
-        assert call(change)[0] == status, change
+        assert call(change) == status, change
     for change, status in BAD_CACHES:
-        assert call({}, change)[0] == status, change
-    assert call({})[1] == 0 and call(dict(tokens=64))[1] == 4 * 2 * 2 * 40 * 64 and call(dict(heads=3))[1] == -3
+        assert call({}, change) == status, change
+    assert scratch({}) == 0 and scratch(dict(tokens=64)) == 4 * 2 * 2 * 40 * 64 and scratch(dict(heads=3)) == -3
     assert _lib.lib.b200gptq_attn_cache(None, None, 0, None) == -1
 
 
