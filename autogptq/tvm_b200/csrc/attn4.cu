@@ -1,5 +1,6 @@
 // b200gptq_attn_cache: checks of the arguments and choice of the kernel.  See include/b200gptq.h.
 #include <algorithm>
+#include <cmath>
 
 #include "attn4.h"
 #include "cache4.cuh"
@@ -22,15 +23,29 @@ int check_sizes(const b200gptq_attn_cache_args& a) {
 Attn4Plan plan_of(const b200gptq_attn_cache_args& a) {
     Attn4Plan p = {};
     const long long rows = (long long)a.tokens * (a.heads / a.cache.kv_heads), sms = sm_count();
-    if (rows >= 64) {
-        p.read = true;
-        return p;
+    const long long keys = a.window ? std::min<long long>(a.cache.max_seq, (long long)a.window + a.sinks + a.tokens) : a.cache.max_seq, pairs = (long long)a.cache.batch * a.cache.kv_heads;
+    // Read back from 64 rows per key head on (as b200gptq_attn does), and otherwise where the sizes make one way much the longer, by rates in us that were measured at 128
+    // dims: the rows kernel does 6500 keys of a tile of 32 rows in one, a CTA of the tcgen05 kernel 128 keys of its 128 rows, 8500 rows are read back.  32 / 8 heads of
+    // 128, us, read back and not: 1 sequence behind 16000 positions, 16 tokens 137 and 48, 64 tokens 147 and 139, 200 tokens 148 and 490; behind 30000, 12
+    // tokens 249 and 69; 4 sequences behind 8000, 16 tokens 95 and 87; 16 behind 3000, 12 tokens 82 and 111 to 149; 30 behind 300, 12 tokens 29 and 53; 8 behind 900, 16 tokens
+    // 23 and 24; 64 behind 300, 8 tokens 58 and 57.
+    p.read = rows >= 64;
+    if (rows > 16) {
+        const double size = (double)keys * a.cache.hd / 128, direct = (double)((rows + 31) / 32) * pairs * size / 6500,
+                     read = (double)(((rows + 127) / 128 * pairs + sms - 1) / sms) * size / 128 + pairs * size / 8500;
+        if (std::fabs(direct - read) > 10) p.read = read < direct;
     }
+    if (p.read) return p;
+    // A tile has 8, 16 or 32 rows.  Two CTAs of 8 rows fit an SM, one of more.
     p.tiles8 = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
-    const long long units = (rows + 8 * p.tiles8 - 1) / (8 * p.tiles8) * a.cache.kv_heads * a.cache.batch, held = sms * (p.tiles8 == 1 ? 2 : 1);
-    const long long keys = a.window ? std::min<long long>(a.cache.max_seq, (long long)a.window + a.sinks + a.tokens) : a.cache.max_seq;
+    const long long units = (rows + 8 * p.tiles8 - 1) / (8 * p.tiles8) * pairs, held = sms * (p.tiles8 == 1 ? 2 : 1);
+    // As many CTAs for a tile as the SMs hold, a part for each warp at least.
     while (p.split_bits < 3 && units << (p.split_bits + 1) <= held && keys >> (p.split_bits + 1) >= 128) ++p.split_bits;
-    p.flat = keys > 2048;
+    // Even runs of all keys, and a second launch whose work grows with the number of tiles, where a warp of a cluster has many parts, as the longest text has them.  Single
+    // tokens, 32 / 8 heads of 128 (with 8 rows), us, runs and clusters: 1 text of 4000 12.6 and 8.2, of 16000 18.6 and 18.6, of 131000 57 and 117; 16 texts of
+    // 200 to 4000 28 and 24, of 900 to 15900 62 and 78 (all of 15900: 99 and 96); 32 of 900 to 15900 111 and 149, 40 137 and 164; 64 of 200 to 4000 94 and 64, of 900 to 7900
+    // 139 and 120.  16 rows: 2 texts of 16000 26 and 46, 16 of 900 to 7900 57 and 66.  32 rows: 1 of 30000 45 and 69, 8 of 900 to 7900 64 and 71, 16 of 900 to 3900 84 and 70.
+    p.flat = 6 * (keys >> (p.split_bits + 7)) > 72 + units;
     p.ctas = (int)held;
     return p;
 }

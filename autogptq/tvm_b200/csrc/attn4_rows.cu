@@ -17,10 +17,14 @@
 // Rows are only rescaled when a score is more than 2^8 above the maximum in use (no weight is above 2^8; fp32 sums).
 //
 // attn4_cluster_kernel: a cluster of 1 to 8 CTAs shares a (sequence, key head, tile of rows), and they add up through distributed shared memory.
-// attn4_flat_kernel: for long caches.  The parts of all sequences and key heads lie one behind the other, and each WARP takes an even run of them, whatever the texts'
-// lengths, which are known on the device only.  Where a run ends inside a (sequence, key head) the sums go to scratch, and a second launch adds them up in
-// order.  (A run for each CTA, whose warps shared a sequence's part of it: 16 texts of 900 to 15900 tokens, 32 / 8 heads, 66 us and SMs idle for a quarter of it, at the ends
-// of sequences and at the end.)
+// attn4_flat_kernel: for many keys per tile.  The parts of all sequences and key heads lie one behind the other, and each WARP takes an even run of them, whatever the texts'
+// lengths, which are known on the device only.  Where a run ends inside a (sequence, key head) the sums go to scratch, of the eight warps together where the whole CTA is in
+// one, and a second launch adds them up in order.  (A run for each CTA, whose warps shared a sequence's part of it: 16 texts of 900 to 15900 tokens, 32 / 8 heads, 66 us and SMs
+// idle for a quarter of it, at the ends of sequences and at the end; sums of single warps alone: 1 text of 16000 26 us, with those of CTAs 19.)
+//
+// Measured (32 / 8 heads of 128): those 16 texts 62 us, 2.8 TB/s; 1 text of 700, 32 heads, 7.1.  A part takes 490 instructions, 62 % of the issue slots of the SMs are in use and half
+// of the integer pipe's, and neither memory (42 %) nor the tensor pipe: what is left over are the waits of 4 warps per scheduler for each other's chains (loads from shared memory,
+// products, exponentials).
 #include <algorithm>
 #include <mutex>
 #include <type_traits>
@@ -702,13 +706,25 @@ attn4_flat_kernel(const __grid_constant__ Attn4Args a, float* __restrict__ part,
     asm volatile("griddepcontrol.launch_dependents;");
     Parts parts;
     const Runs by_run(parts.all(a, units), runs);
-    const long long begin = by_run.begin(run), end = by_run.begin(run + 1);
-    if (begin >= end) return;
+    const long long begin = by_run.begin(run), end = by_run.begin(run + 1), cta_begin = by_run.begin(run - warp), cta_end = by_run.begin(run - warp + kWarps);
+    if (cta_begin >= cta_end) return;
     unsigned hit;
-    while (!(hit = __ballot_sync(0xffffffffu, parts.mine && parts.before + parts.to > begin))) parts.next(a, units);
+    while (!(hit = __ballot_sync(0xffffffffu, parts.mine && parts.before + parts.to > cta_begin))) parts.next(a, units);
     Job job;
     job.b = parts.b0 + __ffs(hit) - 1;
     long long sequence = parts.begin_of(__ffs(hit) - 1);         // the part with which it begins
+    // All that the CTA does may lie in one (sequence, key head, tile): then its warps add up and leave one set of sums.
+    const int nb0 = (int)divided(__shfl_sync(0xffffffffu, parts.mine, __ffs(hit) - 1), units), unit0 = (int)divided(cta_begin - sequence, nb0);
+    const bool together = cta_end <= sequence + (long long)(unit0 + 1) * nb0;
+    if (!together) {
+        if (begin >= end) return;
+        while (!(hit = __ballot_sync(0xffffffffu, parts.mine && parts.before + parts.to > begin))) parts.next(a, units);
+        job.b = parts.b0 + __ffs(hit) - 1;
+        sequence = parts.begin_of(__ffs(hit) - 1);
+    }
+    float* sums_at = sm + warp * L::warp;         // in place of the ring: [row][HD + 4], maximum and denominator behind a row
+    static_assert(R * L::LD <= L::warp, "");
+    if (together && begin >= end && lane < R) *reinterpret_cast<float2*>(sums_at + lane * L::LD + HD) = make_float2(-INFINITY, 0.f);
     for (long long cur = begin; cur < end;) {
         const Span span = span_of(a, job.b);
         if (cur >= sequence + (long long)span.nb * units) {      // the next sequence
@@ -730,19 +746,20 @@ attn4_flat_kernel(const __grid_constant__ Attn4Args a, float* __restrict__ part,
         run_parts<T, HD, GS, NT>(a, job, span, G, by.group, reinterpret_cast<uint32_t*>(sm + warp * L::warp), sums);
         sums.settle_lanes();
         __syncwarp();                             // (the ring has been read)
-        if (job.first > 0 || job.last < span.nb) {
-            float* to = scratch_of<HD, NT>(part, run, second);
+        if (together || job.first > 0 || job.last < span.nb) {
+            float* to = together ? sums_at : scratch_of<HD, NT>(part, run, second);
+            const int row_step = together ? L::LD : HD;
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                     const int row = 8 * t + 2 * c + r;
                     if (row >= job.nrows) continue;
-                    if (g == 0) *reinterpret_cast<float2*>(to + R * HD + 2 * row) = make_float2(sums.m[t][r], sums.l[t][r]);
+                    if (g == 0) *reinterpret_cast<float2*>(to + (together ? row * L::LD + HD : R * HD + 2 * row)) = make_float2(sums.m[t][r], sums.l[t][r]);
 #pragma unroll
                     for (int h = 0; h < HH; ++h)
 #pragma unroll
-                        for (int y = 0; y < 2; ++y) *reinterpret_cast<float4*>(to + row * HD + 64 * h + 32 * y + 4 * g) = sums.four(t, r, h, y);
+                        for (int y = 0; y < 2; ++y) *reinterpret_cast<float4*>(to + row * row_step + 64 * h + 32 * y + 4 * g) = sums.four(t, r, h, y);
                 }
             continue;
         }
@@ -778,6 +795,28 @@ attn4_flat_kernel(const __grid_constant__ Attn4Args a, float* __restrict__ part,
                         attn4_row_again<T, HD, GS>(a, job.b, tok, job.kh * G + idx - tok * G, span.p0 + tok, 0, HD);
                     }
     }
+    if (!together) return;
+    __syncthreads();
+    const int row0 = (unit0 - (int)over((unsigned)unit0, by.row_tiles) * row_tiles) * R, nrows = min(R, attn_count(a.attn, job.b) * G - row0);
+    float* to = scratch_of<HD, NT>(part, run - warp, false);
+    for (int x = threadIdx.x; x < nrows * (HD / 4); x += kThreads) {
+        const int row = x / (HD / 4), d = x % (HD / 4) * 4;
+        float cm = -INFINITY, cl = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) cm = fmaxf(cm, sm[w * L::warp + row * L::LD + HD]);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float2 ml = *reinterpret_cast<const float2*>(sm + w * L::warp + row * L::LD + HD);
+            if (ml.x == -INFINITY) continue;      // (nothing seen, or no part)
+            const float e = exp2_fast(ml.x - cm);
+            const float4 f = *reinterpret_cast<const float4*>(sm + w * L::warp + row * L::LD + d);
+            cl += ml.y * e;
+            o.x += f.x * e; o.y += f.y * e; o.z += f.z * e; o.w += f.w * e;
+        }
+        *reinterpret_cast<float4*>(to + row * HD + d) = o;
+        if (d == 0) *reinterpret_cast<float2*>(to + R * HD + 2 * row) = make_float2(cm, cl);
+    }
 }
 
 // A CTA for each row: the runs that share its (sequence, key head, tile), taken in turn by the warps (64 dims: halves of warps), which add up at the end, in order.
@@ -797,25 +836,29 @@ attn4_sum_kernel(const __grid_constant__ Attn4Args a, float* __restrict__ part, 
     const Runs by_run(parts.all(a, units), runs);
     while (parts.b0 + 32 <= (int)b) parts.next(a, units);
     const long long start = parts.begin_of((int)b - parts.b0) + (long long)(kh * row_tiles + tile) * span.nb, end = start + span.nb;
-    const int first = there ? by_run.of(start) : 0;           // the run that has part `start`
-    const bool whole = by_run.begin(first + 1) >= end;
+    // What there is: sums of runs, or of CTAs where all that a CTA did is in this unit; `early` runs, `ctas` CTAs from `cta` on, `late` runs.
+    const int first = there ? by_run.of(start) : 0, last = there ? by_run.of(end - 1) : 0, cta0 = first / kWarps, cta1 = last / kWarps;
+    auto inside = [&](int i) { return by_run.begin(i * kWarps) >= start && by_run.begin(i * kWarps + kWarps) <= end; };
+    const bool in0 = inside(cta0), in1 = inside(cta1);
+    const int early = in0 ? 0 : min(last + 1, (cta0 + 1) * kWarps) - first, cta = in0 ? cta0 : cta0 + 1, ctas = max(0, (in1 ? cta1 : cta1 - 1) - cta + 1),
+              late = cta1 > cta0 && !in1 ? last - cta1 * kWarps + 1 : 0, records = early + ctas + late;
+    const bool whole = !in0 && first == last;
     const bool second = by_run.begin(first) < start;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
     if (!there || whole) return;
     float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int r0 = first + taker; r0 < runs && by_run.begin(r0) < end; r0 += DEEP * TAKERS) {
+    for (int i0 = taker; i0 < records; i0 += DEEP * TAKERS) {
         float2 of[DEEP];
         float4 v[DEEP];
         float up = m;
 #pragma unroll
         for (int x = 0; x < DEEP; ++x) {
-            const int r = r0 + x * TAKERS;
-            const long long at = by_run.begin(r);
-            // (an empty run has left nothing; there are such where there are fewer parts than runs)
-            const bool has = r < runs && at < end && at < by_run.begin(r + 1);
-            const float* from = scratch_of<HD, NT>(part, has ? r : first, has ? r == first && second : second);
+            const int i = i0 + x * TAKERS;
+            const bool has = i < records;
+            const int r = !has ? (early ? first : cta * kWarps) : i < early ? first + i : i < early + ctas ? (cta + i - early) * kWarps : cta1 * kWarps + i - early - ctas;
+            const float* from = scratch_of<HD, NT>(part, r, r == first && second);
             of[x] = __ldcg(reinterpret_cast<const float2*>(from + R * HD + 2 * row));
             v[x] = __ldcg(reinterpret_cast<const float4*>(from + row * HD + d));
             if (!has) of[x] = make_float2(-INFINITY, 0.f);

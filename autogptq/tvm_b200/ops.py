@@ -541,7 +541,8 @@ def cache_read(cache: QuantCache, lengths=None, k_out=None, v_out=None):
 
 def attn_cache(q, cache: QuantCache, pos, window: Optional[int] = None, sinks: int = 0, counts=None, scale: Optional[float] = None, out=None):
     """:func:`attn_window` over a cache in 4 bits (``b200gptq_attn_cache``); ``window`` None: a token sees the whole text up to it.  The new tokens are in the
-    cache already (:func:`cache_write`).  64 rows (tokens x heads) per key head or more take scratch for the cache's rows in 16 bits."""
+    cache already (:func:`cache_write`).  Many rows (tokens x heads) per key
+    head may take scratch for the cache's rows in 16 bits."""
     return _checked(_lib._host.attn_cache(q, cache.k, cache.v, cache.k_scales, cache.v_scales, pos, window, sinks, counts, scale, out), "b200gptq_attn_cache")
 
 
