@@ -57,15 +57,10 @@ __device__ __forceinline__ unsigned ld_remote(uint32_t at) {
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
     return v;
 }
-__device__ __forceinline__ uint2 ld_remote2(uint32_t at) {
-    uint2 v;
-    asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
-    return v;
-}
-__device__ __forceinline__ uint4 ld_remote4(uint32_t at) {
-    uint4 v;
-    asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
-    return v;
+__device__ __forceinline__ void st_remote(uint32_t at, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory"); }
+__device__ __forceinline__ void st_remote(uint32_t at, unsigned long long v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory"); }
+__device__ __forceinline__ void st_remote(uint32_t at, const uint4& v) {
+    asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 __device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
@@ -103,14 +98,15 @@ struct Power { unsigned whole; float part; };       // 2^(30 + j / kTable), as a
 struct Bins { unsigned part[3][kBins]; };
 constexpr int kPart = 17;
 struct __align__(16) Warp { u64 mass; unsigned ties, unused; };       // of a warp's tokens: sum above the border, how many are at it
+// (What all CTAs want of each other they push before they meet: reading it after that cost a round trip of some 700 clk more.)
 struct Shared {
-    Bins bins[3];                         // in turn: this pass's, the last one's, the next one's
-    u64 groups[3][kBins / 32];            // sums of 32 bins
+    Bins bins[2];                         // in turn: this pass's, and the last one's, which become the next one's
+    u64 groups[2][kMostCtas][kBins / 32]; // sums of 32 bins of each CTA
     Power table[kTable];
-    Warp warps[kWarps];
+    Warp warps[kMostCtas * kWarps];       // of all CTAs
     u64 found_above, all, target, before;
     unsigned ties_before;
-    float top, warp_top[kWarps];
+    float tops[kMostCtas], warp_top[kWarps];
     int found, owner;
 };
 
@@ -149,13 +145,15 @@ __device__ __forceinline__ void put(Bins& h, unsigned at, u64 w) {
     if (c) atomicAdd(h.part[2] + at, c);
 }
 
-// The sums of 32 bins each, by all warps.
-__device__ __forceinline__ void add_groups(const Bins& h, u64* groups) {
+// The sums of 32 bins each, by all warps, to all CTAs; a bin's sum into its first two words.
+__device__ __forceinline__ void add_groups(Bins& h, u64* groups, int rank, int ctas) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int g = threadIdx.x >> 5; g < kBins / 32; g += kWarps) {
-        const u64 sum = warp_total(sum_of(h.part[0][32 * g + lane], h.part[1][32 * g + lane], h.part[2][32 * g + lane]));
-        if (lane == 0) groups[g] = sum;
+        const u64 bin = sum_of(h.part[0][32 * g + lane], h.part[1][32 * g + lane], h.part[2][32 * g + lane]), sum = warp_total(bin);
+        h.part[0][32 * g + lane] = (unsigned)bin;
+        h.part[1][32 * g + lane] = (unsigned)(bin >> 32);
+        if (lane < ctas) st_remote(remote_of(groups + rank * (kBins / 32) + g, lane), sum);
     }
 }
 
@@ -164,12 +162,9 @@ __device__ __forceinline__ void add_groups(const Bins& h, u64* groups) {
 template <typename Target> __device__ __forceinline__ void find(Shared& s, const Bins& h, const u64* groups, int ctas, u64 above, Target target_of) {
     static_assert(kBins == 32 * 32, "");
     const int lane = threadIdx.x & 31;
-    uint2 v[kMostCtas];
-#pragma unroll
-    for (int r = 0; r < kMostCtas; ++r) v[r] = r < ctas ? ld_remote2(remote_of(groups + lane, r)) : make_uint2(0, 0);
     u64 sum = 0;
 #pragma unroll
-    for (int r = 0; r < kMostCtas; ++r) sum += ((u64)v[r].y << 32) + v[r].x;
+    for (int r = 0; r < kMostCtas; ++r) sum += r < ctas ? groups[r * (kBins / 32) + lane] : 0;
     u64 to = above + warp_prefix(sum, lane);
     const u64 all = __shfl_sync(0xffffffffu, to, 31), target = target_of(all);
     if (lane == 0) { s.all = all; s.target = target; }
@@ -178,14 +173,14 @@ template <typename Target> __device__ __forceinline__ void find(Shared& s, const
     if (!hit) return;
     const int g = __ffs(hit) - 1;
     above = __shfl_sync(0xffffffffu, to - sum, g);
-    unsigned n[kMostCtas][3];
+    unsigned n[kMostCtas][2];
 #pragma unroll
     for (int r = 0; r < kMostCtas; ++r)
 #pragma unroll
-        for (int i = 0; i < 3; ++i) n[r][i] = r < ctas ? ld_remote(remote_of(h.part[i] + 32 * g + lane, r)) : 0;
+        for (int i = 0; i < 2; ++i) n[r][i] = r < ctas ? ld_remote(remote_of(h.part[i] + 32 * g + lane, r)) : 0;
     sum = 0;
 #pragma unroll
-    for (int r = 0; r < kMostCtas; ++r) sum += sum_of(n[r][0], n[r][1], n[r][2]);
+    for (int r = 0; r < kMostCtas; ++r) sum += ((u64)n[r][1] << 32) + n[r][0];
     to = above + warp_prefix(sum, lane);
     const unsigned in = __ballot_sync(0xffffffffu, to >= target);
     if (lane == __ffs(in) - 1) {
@@ -206,6 +201,7 @@ sample_kernel(const __grid_constant__ b200gptq_sample_args a, int slice, int clu
     // A warp's tokens: a run of the slice
     const int run = (slice + kWarps - 1) / kWarps, first = min(warp * run, n), last = min(first + run, n);
     for (int i = tid; i < (int)sizeof(s.bins) / 16; i += kThreads) reinterpret_cast<uint4*>(s.bins)[i] = make_uint4(0, 0, 0, 0);
+    if (ctas > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     auto meet = [&] {
         if (ctas > 1) cluster_sync();
         else __syncthreads();
@@ -219,6 +215,7 @@ sample_kernel(const __grid_constant__ b200gptq_sample_args a, int slice, int clu
     const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride + base;
     const float temperature = a.temperature ? a.temperature[row] : 1.f, top_p = a.top_p ? a.top_p[row] : 1.f, min_p = a.min_p ? a.min_p[row] : 0.f, u = a.uniform[row];
     const long long top_k = a.top_k ? a.top_k[row] : 0;
+    const double step = 1.4426950408889634074 / (double)temperature;                     // (of no use where the temperature is 0)
     // ---- the slice, and the row's largest logit ----
     float top = -INFINITY;
     if ((reinterpret_cast<uintptr_t>(in) & 15u) == 0) {
@@ -243,21 +240,17 @@ sample_kernel(const __grid_constant__ b200gptq_sample_args a, int slice, int clu
         top = tid < kWarps ? s.warp_top[tid] : -INFINITY;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (tid == 0) s.top = top;
     }
+    if (ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");      // (all CTAs of the cluster run)
+    if (tid < ctas) st_remote(remote_of(s.tops + rank, tid), top);
     meet();
     Row r;
-    r.top = s.top;
-    if (ctas > 1) {
-        float others[kMostCtas];
+    r.top = s.tops[0];
 #pragma unroll
-        for (int c = 0; c < kMostCtas; ++c) others[c] = c < ctas ? __uint_as_float(ld_remote(remote_of(&s.top, c))) : -INFINITY;
-#pragma unroll
-        for (int c = 0; c < kMostCtas; ++c) r.top = fmaxf(r.top, others[c]);
-    }
+    for (int c = 1; c < kMostCtas; ++c) r.top = c < ctas ? fmaxf(r.top, s.tops[c]) : r.top;
     r.bits = bits;
     const bool greedy = !(temperature >= kColdest) || top_k == 1 || min_p > 1.f || r.top == -INFINITY;
-    r.step = greedy ? 0.0 : 1.4426950408889634074 / (double)temperature;
+    r.step = greedy ? 0.0 : step;
     r.half_scale = (float)(r.step * (2.0 * kBins) / (bits + 1));
     // ---- the border: tokens of larger keys are kept, and of those at it the first `ties` ----
     enum { kNumber, kWeight, kKept };            // tokens into bins, for top-k; weights into bins, for top-p; sums of what is kept
@@ -294,20 +287,19 @@ sample_kernel(const __grid_constant__ b200gptq_sample_args a, int slice, int clu
             }
         }
         __syncthreads();
-        add_groups(h, s.groups[turn]);
+        add_groups(h, s.groups[turn][0], rank, ctas);
         meet();
-        // (the last turn's bins have been read by all: before they met)
-        const int last_turn = turn == 0 ? 2 : turn - 1;
+        // (the last turn's bins have been read by all: before they met; so have its groups)
         if (warp == 0) {
-            find(s, h, s.groups[turn], ctas, bin < 0 ? 0 : above, [&](u64 sum) {
+            find(s, h, s.groups[turn][0], ctas, bin < 0 ? 0 : above, [&](u64 sum) {
                 if (mode != kWeight || bin >= 0) return target;
                 // (of all, or of what top-k keeps; one token at least)
                 return max(share(top_p, cut ? sum + ties * weight_apart(of_key<T>(border), r, s.table) : sum, true), (u64)1);
             });
         } else {
-            for (int i = tid - 32; i < (int)sizeof(Bins) / 16; i += kThreads - 32) reinterpret_cast<uint4*>(s.bins + last_turn)[i] = make_uint4(0, 0, 0, 0);
+            for (int i = tid - 32; i < (int)sizeof(Bins) / 16; i += kThreads - 32) reinterpret_cast<uint4*>(s.bins + (turn ^ 1))[i] = make_uint4(0, 0, 0, 0);
         }
-        turn = turn == 2 ? 0 : turn + 1;
+        turn ^= 1;
         __syncthreads();
         const int found = s.found;
         const u64 all = s.all;
@@ -325,17 +317,24 @@ sample_kernel(const __grid_constant__ b200gptq_sample_args a, int slice, int clu
                 shift = max(0, 32 - __clz(hi - lo) - kBinBits);
                 if (!moved && room) {            // nothing below the keys of this bin will be kept: the others move to the front of the run
                     int held = 0;
-                    for (int i0 = 0; i0 < many; i0 += 32) {
-                        const int i = i0 + lane;
-                        const T v = i < many ? run_x[i] : T(0.f);
-                        const bool in = i < many && key_of<T>(wide(v)) >= lo;
-                        const unsigned whom = __ballot_sync(0xffffffffu, in);
-                        __syncwarp();
-                        const int to = held + __popc(whom & ((1u << lane) - 1));
-                        if (in) { x[first + to] = v; places[first + to] = (unsigned short)i; }
-                        held += __popc(whom);
-                        __syncwarp();
+                    constexpr int DEEP = 4;
+                    const float least_x = lo <= key_of<T>(-INFINITY) ? -INFINITY : of_key<T>(lo);       // (not a NaN)
+                    for (int i0 = 0; i0 < many; i0 += 32 * DEEP) {
+                        T v[DEEP];
+#pragma unroll
+                        for (int e = 0; e < DEEP; ++e) v[e] = i0 + 32 * e + lane < many ? run_x[i0 + 32 * e + lane] : T(0.f);
+                        __syncwarp();            // (read, by all lanes, before anything is put there)
+#pragma unroll
+                        for (int e = 0; e < DEEP; ++e) {
+                            const int i = i0 + 32 * e + lane;
+                            const bool in = i < many && wide(v[e]) >= least_x;
+                            const unsigned whom = __ballot_sync(0xffffffffu, in);
+                            const int to = held + __popc(whom & ((1u << lane) - 1));
+                            if (in) { x[first + to] = v[e]; places[first + to] = (unsigned short)i; }
+                            held += __popc(whom);
+                        }
                     }
+                    __syncwarp();
                     many = held;
                     moved = true;
                 }
@@ -380,7 +379,7 @@ sample_kernel(const __grid_constant__ b200gptq_sample_args a, int slice, int clu
     }
     mine.mass = warp_total(mine.mass);
     mine.ties = warp_total(mine.ties);
-    if (lane == 0) s.warps[warp] = mine;
+    if (lane < ctas) st_remote(remote_of(s.warps + rank * kWarps + warp, lane), make_uint4((unsigned)mine.mass, (unsigned)(mine.mass >> 32), mine.ties, 0));
     meet();
     auto kept_weight = [&](float v) { return keeps(v, greedy ? 1 : weight_apart(v, r, s.table)); };
     const u64 border_w = border ? kept_weight(of_key<T>(border)) : 0;
@@ -393,7 +392,7 @@ sample_kernel(const __grid_constant__ b200gptq_sample_args a, int slice, int clu
         for (int i = 0; i < kPer; ++i) {
             const int w = kPer * lane + i;
             v[i] = make_uint4(0, 0, 0, 0);
-            if (w < ctas * kWarps) v[i] = ld_remote4(remote_of(s.warps + w % kWarps, w / kWarps));
+            if (w < ctas * kWarps) v[i] = reinterpret_cast<const uint4*>(s.warps)[w];
             lane_ties += v[i].z;
         }
         unsigned to = warp_prefix(lane_ties, lane) - lane_ties;          // (equal tokens before)
@@ -424,7 +423,7 @@ sample_kernel(const __grid_constant__ b200gptq_sample_args a, int slice, int clu
             before += mass[i];
         }
     }
-    meet();                                       // (nobody leaves while others read)
+    __syncthreads();                              // (what the CTAs push has arrived before they met: each may leave)
     if (s.owner < 0) {                            // nothing to choose from
         if (rank == 0 && tid == 0) a.out[row] = 0;
         return;
