@@ -13,7 +13,8 @@
 // search ended are looked at again: each warp moves its own together.  The CTAs of the cluster read each other's sums through distributed shared memory and all come
 // to the same results.
 // Bound by the chain of searches (2 to 5 after one another, some 5000 clk each: bins, a meeting, sums from the other CTAs, a decision) and, with many rows, by the
-// instructions of the pass over all weights.  Measured: 1 row of 32000 19.5 us, 64 rows of 50272 31.5 (45 % of the issue slots in use), 128 of 100003 in fp32 136 (51 %).
+// instructions of the pass over all weights.  Measured: 1 row of 32000 17.6 us, 64 rows of 50272 30.0, 128 of 100003 in fp32 127 (half of
+// the issue slots in use).
 #include <cuda_bf16.h>
 
 #include <cstddef>
@@ -467,8 +468,8 @@ size_t shared_bytes(int slice, size_t size) { return (sizeof(Shared) + 15) / 16 
 template <typename T>
 int launch(const b200gptq_sample_args& a, cudaStream_t stream) {
     // CTAs per row: as many as the SMs hold two of, a slice of 1024 tokens or more, and enough that a slice leaves an SM room for two (what eight cannot hold so
-    // takes more).  Measured, us, with this and with other numbers of CTAs per row: 1 row of 32000, 8 CTAs 16.0, 4 18.7; 64 rows of 32000, 4 27.3, 8 40.9; 300 of 4099, 1
-    // 20.6, 4 60.7; 20 of 100003 in fp32, 8 37.9, 4 43.3; 128 of them, 8 135, 4, which leave an SM one CTA, 158.
+    // takes more).  Measured, us, with this and with other numbers of CTAs per row: 1 row of 32000, 8 CTAs 14.5, 4 17.0; 64 rows of 32000, 4 26.1, 8 38.4; 300 of 4099, 1
+    // 21.0, 4 56.7; 20 of 100003 in fp32, 8 36.2, 4 39.5; 128 of them, 8 127, 4, which leave an SM one CTA, 143.
     int cluster_bits = 0;
     while (cluster_bits < 3 && ((long long)a.rows << (cluster_bits + 1) <= 2LL * sm_count() || shared_bytes((a.vocab >> cluster_bits) + 8, sizeof(T) + sizeof(unsigned short)) > 113 * 1024) &&
            a.vocab >> (cluster_bits + 1) >= 1024)
