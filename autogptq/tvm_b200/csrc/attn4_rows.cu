@@ -9,12 +9,15 @@
 //                                                                      the sums of q in two numbers each (16 bits or more together)
 //   O(dim, row) = sum over keys of  (w sV) (cV - 8) + w (zV + 8 sV)    w sV is what is rounded to fp16, and codes of both signs make half of its error of codes from 0 to 15
 //                                                                      (by one subtraction in fp16, exact); the second term is summed in fp32, per group
-// Q is scaled by a power of two per row (to below 2^15, exact for what is above 2^-38 of the row's largest; so bf16 queries are exact in fp16), w sV by one per
-// warp that follows the largest scale seen, so neither leaves fp16's range.
+// Q is scaled by a power of two per row (to below 2^15, exact for what is above 2^-38 of the row's largest; so bf16 queries are exact in fp16).  So is w sV, per
+// row and group of dims: the largest so far lies between 2^6 and 2^16, so what becomes a subnormal number is off by 2^-31 of it at most.  (One power per warp that followed the largest
+// scale alone was wrong: a key of large scale, whatever its weight, or another group's, took the low bits of all others.)  They are a byte each, since there are no registers
+// left for numbers, and what the sums are in: while weights shrink with a growing maximum, sums stay and their units shrink.
 //
 // Every warp takes parts of 16 keys on its own, through a ring of cp.async stages in shared memory.  Keys are the 16 of m16n8k16, rows the 8: 8 bytes (128
 // dims: 16) of a key are the operand of S as they lie, two keys' words paired by byte permutations that of O (include/b200gptq.h has the order of the codes).
-// Rows are only rescaled when a score is more than 2^8 above the maximum in use (no weight is above 2^8; fp32 sums).
+// Rows are only rescaled when a score is more than 8 (log2) above the maximum in use (no weight is above 2^-16; fp32 sums), which is a whole number, so that all factors are
+// powers of two.
 //
 // attn4_cluster_kernel: a cluster of 1 to 8 CTAs shares a (sequence, key head, tile of rows), and they add up through distributed shared memory.
 // attn4_flat_kernel: for many keys per tile.  The parts of all sequences and key heads lie one behind the other, and each WARP takes an even run of them, whatever the texts'
@@ -22,7 +25,7 @@
 // one, and a second launch adds them up in order.  (A run for each CTA, whose warps shared a sequence's part of it: 16 texts of 900 to 15900 tokens, 32 / 8 heads, 66 us and SMs
 // idle for a quarter of it, at the ends of sequences and at the end; sums of single warps alone: 1 text of 16000 26 us, with those of CTAs 19.)
 //
-// Measured (32 / 8 heads of 128): those 16 texts 62 us, 2.8 TB/s; 1 text of 700, 32 heads, 7.1.  A part takes 490 instructions, 62 % of the issue slots of the SMs are in use and half
+// Measured (32 / 8 heads of 128): those 16 texts 64 us, 2.7 TB/s (62.9 with a power per warp); 1 text of 700, 32 heads, 7.2.  A part takes 490 instructions, 62 % of the issue slots of the SMs are in use and half
 // of the integer pipe's, and neither memory (42 %) nor the tensor pipe: what is left over are the waits of 4 warps per scheduler for each other's chains (loads from shared memory,
 // products, exponentials).
 #include <algorithm>
@@ -37,6 +40,7 @@ namespace {
 
 constexpr int kPart = 16, kWarps = kAttn4Warps, kThreads = kWarps * 32, kStages = 4;
 constexpr float kGrow = 8.f;             // log2 of what a score may be above the maximum in use
+constexpr float kBelow = 24.f;           // log2 of what that maximum's weight lies below 1, so that a million of bf16's largest values add up in fp32
 constexpr unsigned kLow = 0x000f000fu, kHigh = 0x00f000f0u;
 
 __device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -107,14 +111,8 @@ template <unsigned EIGHT> __device__ __forceinline__ uint32_t centred(uint32_t c
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// The largest scale of two rows' constants, (scale, zero) in a word each, which are compared together; NaN counts for nothing.
-template <typename T, int N> __device__ __forceinline__ float widest_scale(const Words<N>& u, const Words<N>& v) {
-    using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
-    T2 most = __hmax2(*reinterpret_cast<const T2*>(&u.w[0]), *reinterpret_cast<const T2*>(&v.w[0]));
-#pragma unroll
-    for (int n = 1; n < N; ++n) most = __hmax2(most, __hmax2(*reinterpret_cast<const T2*>(&u.w[n]), *reinterpret_cast<const T2*>(&v.w[n])));
-    return fmaxf(Half<T>::wide(most.x), 0.f);
-}
+// 2^e; 0 below fp32's normal numbers.
+__device__ __forceinline__ float power(int e) { return e < -126 ? 0.f : __uint_as_float((unsigned)(e + 127) << 23); }
 
 // Parts of a sequence: those that its tokens see between them; one at least where there are tokens, since their rows get zeros when they see nothing.
 struct Span { AttnRange range; int p0, count, n_s, nb; };
@@ -131,11 +129,25 @@ __device__ __forceinline__ Span span_of(const Attn4Args& a, int b) {
 // What a warp does: parts first, first + step .. below last of a (sequence, key head, tile of rows).
 struct Job { int b, kh, row0, nrows, first, last, step; };
 
-// A warp's sums: of rows 8 t + 2 c and + 1; O without the zeros, in units of limit 2^-24 (dims 64 h + 32 y + 4 g + {0, 2} in acc[4 h + 2 y], {1, 3} in the next), and what the zeros
-// add, by group, of the lane's keys.
+// A warp's sums: of rows 8 t + 2 c and + 1; O without the zeros, in units of 2^-24 / fit (dims 64 h + 32 y + 4 g + {0, 2} in acc[4 h + 2 y], {1, 3} in the next), and what the zeros
+// add, by group, of the lane's keys.  fit: what w sV is multiplied by, a power of two for each row and group; byte n holds the exponent field of group n's.
 template <int HD, int GS, int NT> struct Sums {
     static constexpr int HH = HD / 64, NG = HD / GS;
-    float acc[NT][4 * HH][4], zacc[NT][2][NG], m[NT][2], l[NT][2], limit;
+    static constexpr int kFitMost = 253;          // 2^126: times a weight still a number
+    float acc[NT][4 * HH][4], zacc[NT][2][NG], m[NT][2], l[NT][2];
+    unsigned fit[NT][2];
+
+    static __device__ __forceinline__ int field(unsigned all, int n) { return (int)(all >> 8 * n & 0xffu); }
+    static __device__ __forceinline__ float number(unsigned all, int n) { return __uint_as_float((n < 3 ? all << (23 - 8 * n) : all >> 1) & 0x7f800000u); }
+    // Row (t, r)'s sums of group n are multiplied by f.
+    __device__ __forceinline__ void scale(int t, int r, int n, float f) {
+#pragma unroll
+        for (int x = 0; x < GS / 16; ++x) {
+            float (&a)[4] = acc[t][GS / 16 * n + x];
+            a[r] *= f;
+            a[2 + r] *= f;
+        }
+    }
 
     // The lanes' shares of denominators and zeros added up.
     __device__ __forceinline__ void settle_lanes() {
@@ -152,7 +164,8 @@ template <int HD, int GS, int NT> struct Sums {
     }
     // Dims 64 h + 32 y + 4 g .. of row r.  (Fields at bits 4 .. 7 were 16 times as large.)
     __device__ __forceinline__ float4 four(int t, int r, int h, int y) const {
-        const float z = zacc[t][r][GS == 32 ? 2 * h + y : h];
+        const int n = GS == 32 ? 2 * h + y : h;
+        const float z = zacc[t][r][n], limit = power(127 - field(fit[t][r], n));
         const float *even = acc[t][4 * h + 2 * y], *odd = acc[t][4 * h + 2 * y + 1];
         return make_float4(fmaf(even[r] * 0x1p24f, limit, z), fmaf(odd[r] * 0x1p24f, limit, z), fmaf(even[2 + r] * 0x1p20f, limit, z), fmaf(odd[2 + r] * 0x1p20f, limit, z));
     }
@@ -211,8 +224,9 @@ __device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, co
     uint4* q_at = reinterpret_cast<uint4*>(own + L::q) + lane;
     uint32_t qz[NT];
     float factor[NT][2];
-    float (&acc)[NT][4 * HH][4] = sums.acc, (&zacc)[NT][2][NG] = sums.zacc, (&m)[NT][2] = sums.m, (&l)[NT][2] = sums.l, &limit = sums.limit, inverse = 0.f;
-    limit = 0.f;
+    float (&acc)[NT][4 * HH][4] = sums.acc, (&zacc)[NT][2][NG] = sums.zacc, (&m)[NT][2] = sums.m, (&l)[NT][2] = sums.l;
+    using Fit = Sums<HD, GS, NT>;
+    unsigned (&fit)[NT][2] = sums.fit;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         const int idx = job.row0 + min(8 * t + g, job.nrows - 1), tok = token_of(idx), head = job.kh * G + idx - tok * G;
@@ -272,6 +286,7 @@ __device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, co
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             m[t][e] = -INFINITY; l[t][e] = 0.f;
+            fit[t][e] = Fit::kFitMost * 0x01010101u;
             factor[t][e] = __shfl_sync(0xffffffffu, mine, 4 * (2 * c + e));
 #pragma unroll
             for (int n = 0; n < NG; ++n) zacc[t][e][n] = 0.f;
@@ -283,6 +298,7 @@ __device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, co
     const uint32_t k_lane = St::k + g * St::row + 4 * KW * c, c_lane = St::kc + g * St::constants, z_lane = c_lane + (NG == 4 ? 8 * (c & 1) : 0),
                    even_lane = St::v_at(2 * c, 4 * VW * g), odd_lane = St::v_at(2 * c + 1, 4 * VW * g);
     const int step = kPart * job.step;
+    bool fresh = true;                            // the warp's first part: all sums are zero
     while (true) {
     // Parts that begin between these rows are seen as a whole by all rows of the tile.
     const int end = sink ? range.s_end : range.w_end, whole_from = sink ? 0 : p_hi - window + 1, whole_to = min(sink ? min(end, a.attn.sinks) : end, p_lo + 1) - kPart;
@@ -292,7 +308,7 @@ __device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, co
         const bool whole = j0 >= whole_from && j0 <= whole_to;
         const uint32_t k_from = from + k_lane, c_from = from + c_lane, z_from = from + z_lane, even_from = from + even_lane, odd_from = from + odd_lane;
         // ---- S: keys g (0, 1) and g + 8 (2, 3), rows 2 c and 2 c + 1 ----
-        float s[NT][4], widest = 0.f;
+        float s[NT][4];
         {
             // the zeros of groups 2 (c % 2) and + 1 (where there are fewer groups: of those there are), the same for both halves of a sum of q
             const Words<NG == 1 ? 1 : 2> z0 = lds<NG == 1 ? 1 : 2, 0>(z_from),
@@ -300,8 +316,6 @@ __device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, co
             const uint32_t a0 = __byte_perm(z0.w[0], z0.w[NG == 1 ? 0 : 1], 0x7632u), a1 = __byte_perm(z1.w[0], z1.w[NG == 1 ? 0 : 1], 0x7632u);
             const Words<KW> k0 = lds<KW, 0>(k_from), k1 = lds<KW, 8 * St::row>(k_from);
             const Words<NG> c0 = lds<NG, 0>(c_from), c1 = lds<NG, 8 * St::constants>(c_from);
-            const Words<NG> u0 = lds<NG, kPart * St::constants>(c_from), u1 = lds<NG, (kPart + 8) * St::constants>(c_from);
-            widest = widest_scale<T, NG>(u0, u1);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 mma8_first<T>(s[t], a0, a1, qz[t]);
@@ -345,8 +359,6 @@ __device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, co
         }
         if (!whole) {
             __syncwarp();                         // (so that it stays a branch: with predicates instead each part took 45 instructions more)
-            const Words<NG> u0 = lds<NG, kPart * St::constants>(c_from), u1 = lds<NG, (kPart + 8) * St::constants>(c_from);
-            widest = fmaxf(j0 + g < end ? widest_scale<T, NG>(u0, u0) : 0.f, j0 + g + 8 < end ? widest_scale<T, NG>(u1, u1) : 0.f);
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -355,39 +367,38 @@ __device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, co
                     s[t][e] = j < end && attn_sees(p, j, window, a.attn.sinks) ? s[t][e] : -INFINITY;
                 }
         }
-        bool grow = widest > 8.f * limit;
+        bool grow = false;
         float top[NT][2];
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 top[t][r] = fmaxf(s[t][r], s[t][2 + r]);
-                grow = grow || top[t][r] - m[t][r] > kGrow;
+                grow = grow || top[t][r] - m[t][r] > kGrow - kBelow;
             }
         if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) widest = fmaxf(widest, __shfl_xor_sync(0xffffffffu, widest, o));
-            float shrink = 1.f;
-            if (widest > limit) {                 // the power of two at or below it
-                const float now = fminf(fmaxf(__uint_as_float(__float_as_uint(widest) & 0x7f800000u), 0x1p-100f), 0x1p126f);
-                shrink = limit == 0.f ? 0.f : limit / now;
-                limit = now;
-                inverse = 1.f / now;
-            }
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    float up = fmaxf(top[t][r], m[t][r]);
+                    float up = fmaxf(ceilf(top[t][r]) + kBelow, m[t][r]);
 #pragma unroll
                     for (int o = 4; o < 32; o <<= 1) up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, o));
-                    const float corr = up == -INFINITY ? 1.f : exp2_fast(m[t][r] - up), both = corr * shrink;
+                    // (from minus infinity, or to infinity: all there was counts for nothing)
+                    const int down = up == m[t][r] ? 0 : (int)fmaxf(m[t][r] - up, -1024.f);
                     m[t][r] = up;
+                    if (fresh) continue;
+                    const float corr = power(down);
                     l[t][r] *= corr;
+                    unsigned fits = 0;
 #pragma unroll
-                    for (int n = 0; n < NG; ++n) zacc[t][r][n] *= corr;
-#pragma unroll
-                    for (int n = 0; n < 4 * HH; ++n) { acc[t][n][r] *= both; acc[t][n][2 + r] *= both; }
+                    for (int n = 0; n < NG; ++n) {            // what was the largest w sV is smaller by as much: the sums stay as they are in units that do so too
+                        const int old = Fit::field(fit[t][r], n), now = min(old - down, Fit::kFitMost);
+                        zacc[t][r][n] *= corr;
+                        sums.scale(t, r, n, power(now - old + down));
+                        fits |= (unsigned)now << 8 * n;
+                    }
+                    fit[t][r] = fits;
                 }
         }
 #pragma unroll
@@ -424,40 +435,71 @@ __device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, co
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
+                    for (int r = 0; r < 2; ++r)
 #pragma unroll
                         for (int n = 0; n < NG; ++n) zacc[t][r][n] = fmaf(s[t][r], zv[0][n], fmaf(s[t][2 + r], zv[1][n], zacc[t][r][n]));
-                        s[t][r] *= inverse;
-                        s[t][2 + r] *= inverse;
-                    }
             }
-            constexpr int EIGHT = St::v_at(8, 0) - St::v_at(0, 0);
-            const Words<VW> v[4] = {lds<VW, 0>(even_from), lds<VW, 0>(odd_from), lds<VW, EIGHT>(even_from), lds<VW, EIGHT>(odd_from)};
+            // w sV as operands, of as many groups at once as registers hold
+            constexpr int ONCE = NT <= 2 ? NG : 1, EIGHT = St::v_at(8, 0) - St::v_at(0, 0);
+            Words<VW> v[4];
 #pragma unroll
-            for (int h = 0; h < HH; ++h) {
-                const uint32_t x[2][2] = {{__byte_perm(v[0].w[h], v[1].w[h], 0x5410u), __byte_perm(v[2].w[h], v[3].w[h], 0x5410u)},
-                                          {__byte_perm(v[0].w[h], v[1].w[h], 0x7632u), __byte_perm(v[2].w[h], v[3].w[h], 0x7632u)}};
-                uint32_t b0[NT], b1[NT];
+            for (int n0 = 0; n0 < NG; n0 += ONCE) {
+                uint32_t b0[NT][ONCE], b1[NT][ONCE];
+                auto products = [&] {             // (the weight first: a large scale alone may pass fp32 in units for small products)
+                    __half2 most = __float2half2_rn(0.f);        // (a NaN, 0 times an infinity that is not seen, counts for nothing)
 #pragma unroll
-                for (int y = 0; y < 2; ++y) {     // dims 64 h + 32 y + 4 g + {0, 2} and {1, 3}
-                    if (GS == 32 || y == 0) {
-                        const int n = GS == 32 ? 2 * h + y : h;
+                    for (int t = 0; t < NT; ++t)
 #pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            b0[t] = transposed(Half<__half>::pack(s[t][0] * sv[0][n], s[t][1] * sv[0][n]));
-                            b1[t] = transposed(Half<__half>::pack(s[t][2] * sv[1][n], s[t][3] * sv[1][n]));
+                        for (int i = 0; i < ONCE; ++i) {
+                            const int n = n0 + i;
+                            const float f0 = Fit::number(fit[t][0], n), f1 = Fit::number(fit[t][1], n);
+                            b0[t][i] = Half<__half>::pack(s[t][0] * f0 * sv[0][n], s[t][1] * f1 * sv[0][n]);
+                            b1[t][i] = Half<__half>::pack(s[t][2] * f0 * sv[1][n], s[t][3] * f1 * sv[1][n]);
+                            most = __hmax2(most, __hmax2(__habs2(*reinterpret_cast<const __half2*>(&b0[t][i])), __habs2(*reinterpret_cast<const __half2*>(&b1[t][i]))));
                         }
+                    return most;
+                };
+                if (__any_sync(0xffffffffu, !__hble2(products(), __float2half2_rn(32768.f)))) {      // units in which the largest product is 2^6 or a little more
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r)
+#pragma unroll
+                            for (int i = 0; i < ONCE; ++i) {
+                                const int n = n0 + i, old = Fit::field(fit[t][r], n);
+                                float large = fmaxf(fmaxf(fabsf(s[t][r] * sv[0][n]), fabsf(s[t][2 + r] * sv[1][n])), 0.f);
+#pragma unroll
+                                for (int o = 4; o < 32; o <<= 1) large = fmaxf(large, __shfl_xor_sync(0xffffffffu, large, o));
+                                const int now = min(old, 2 * 127 + 6 - (int)(__float_as_uint(large) >> 23));
+                                if (!fresh) sums.scale(t, r, n, power(now - old));
+                                fit[t][r] += (unsigned)(now - old) << 8 * n;
+                            }
+                    products();
+                }
+                if (n0 == 0) { v[0] = lds<VW, 0>(even_from); v[1] = lds<VW, 0>(odd_from); v[2] = lds<VW, EIGHT>(even_from); v[3] = lds<VW, EIGHT>(odd_from); }
+#pragma unroll
+                for (int i = 0; i < ONCE; ++i) {
+                    const int n = n0 + i, h = GS == 32 ? n >> 1 : n;
+                    const uint32_t x[2][2] = {{__byte_perm(v[0].w[h], v[1].w[h], 0x5410u), __byte_perm(v[2].w[h], v[3].w[h], 0x5410u)},
+                                              {__byte_perm(v[0].w[h], v[1].w[h], 0x7632u), __byte_perm(v[2].w[h], v[3].w[h], 0x7632u)}};
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        b0[t][i] = transposed(b0[t][i]);
+                        b1[t][i] = transposed(b1[t][i]);
                     }
 #pragma unroll
-                    for (int z = 0; z < 2; ++z) {
-                        const uint32_t k01 = x[z][0] >> (8 * y), k89 = x[z][1] >> (8 * y);
-                        const uint32_t a0 = centred<8>(k01 & kLow), a1 = centred<128>(k01 & kHigh), a2 = centred<8>(k89 & kLow), a3 = centred<128>(k89 & kHigh);
+                    for (int y = GS == 32 ? n & 1 : 0; y < (GS == 32 ? (n & 1) + 1 : 2); ++y)        // dims 64 h + 32 y + 4 g + {0, 2} and {1, 3}
 #pragma unroll
-                        for (int t = 0; t < NT; ++t) mma16(acc[t][4 * h + 2 * y + z], a0, a1, a2, a3, b0[t], b1[t]);
-                    }
+                        for (int z = 0; z < 2; ++z) {
+                            const uint32_t k01 = x[z][0] >> (8 * y), k89 = x[z][1] >> (8 * y);
+                            const uint32_t a0 = centred<8>(k01 & kLow), a1 = centred<128>(k01 & kHigh), a2 = centred<8>(k89 & kLow), a3 = centred<128>(k89 & kHigh);
+#pragma unroll
+                            for (int t = 0; t < NT; ++t) mma16(acc[t][4 * h + 2 * y + z], a0, a1, a2, a3, b0[t][i], b1[t][i]);
+                        }
                 }
             }
         }
+        fresh = false;
         __syncwarp();                             // (the part has been read)
         fetch(j0 + kStages * step, behind, from);
         from = from + St::total == ring + kStages * St::total ? ring : from + St::total;

@@ -525,7 +525,8 @@ B200GPTQ_API int b200gptq_cache_read(const b200gptq_cache_read_args* args, void*
  * Attention of new tokens over a cache held in 4 bits: b200gptq_attn's, of a query at position p = pos[b] + t, over the values that the cache stands for.
  *   window 0: a token sees rows 0 .. p, else the last `window` of them and the first `sinks`; without a window there are no sinks
  * Everything else (counts, strides, what is not seen, rows that see nothing) is as there.  Statistics and sums are fp32; weights times scales are rounded to fp16 before
- * they multiply codes.  64 rows of a key head (tokens * heads / kv_heads) or more, and 17 or more over many keys: where that pays the rows that are seen are read back into
+ * they multiply codes, by row and group of dims: each is off by 2^-11 of itself or 2^-31 of the largest that the row has in that
+ * group (of 2^-96 where that is less).  64 rows of a key head (tokens * heads / kv_heads) or more, and 17 or more over many keys: where that pays the rows that are seen are read back into
  * scratch, each value rounded to dtype, and multiplied as b200gptq_attn does.
  * b200gptq_attn_cache_workspace_bytes: scratch of a call, 16-byte aligned, contents on entry do not matter, not shared by calls that may overlap.
  */
