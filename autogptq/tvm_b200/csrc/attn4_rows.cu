@@ -11,8 +11,8 @@
 //                                                                      (by one subtraction in fp16, exact); the second term is summed in fp32, per group
 // Q is scaled by a power of two per row (to below 2^15, exact for what is above 2^-38 of the row's largest; so bf16 queries are exact in fp16).  So is w sV, per
 // row and group of dims: the largest so far lies between 2^6 and 2^16, so what becomes a subnormal number is off by 2^-31 of it at most.  (One power per warp that followed the largest
-// scale alone was wrong: a key of large scale, whatever its weight, or another group's, took the low bits of all others.)  They are a byte each, since there are no registers
-// left for numbers, and what the sums are in: while weights shrink with a growing maximum, sums stay and their units shrink.
+// scale alone was wrong: a key of large scale, whatever its weight, or another group's, took the low bits of all others.)  They are 16 bits each, since there are no
+// registers left for numbers, and what the sums are in: while weights shrink with a growing maximum, sums stay and their units shrink.
 //
 // Every warp takes parts of 16 keys on its own, through a ring of cp.async stages in shared memory.  Keys are the 16 of m16n8k16, rows the 8: 8 bytes (128
 // dims: 16) of a key are the operand of S as they lie, two keys' words paired by byte permutations that of O (include/b200gptq.h has the order of the codes).
@@ -25,7 +25,8 @@
 // one, and a second launch adds them up in order.  (A run for each CTA, whose warps shared a sequence's part of it: 16 texts of 900 to 15900 tokens, 32 / 8 heads, 66 us and SMs
 // idle for a quarter of it, at the ends of sequences and at the end; sums of single warps alone: 1 text of 16000 26 us, with those of CTAs 19.)
 //
-// Measured (32 / 8 heads of 128): those 16 texts 64 us, 2.7 TB/s (62.9 with a power per warp); 1 text of 700, 32 heads, 7.2.  A part takes 490 instructions, 62 % of the issue slots of the SMs are in use and half
+// Measured (32 / 8 heads of 128): those 16 texts 62 us, 2.8 TB/s; 1 text of 700, 32 heads, 7.4; 2 texts of 16000 and 16 rows 28.8, 1 and 64 rows 56 (26.8 and 48.6
+// with a power of two per warp; one copy of the products in a loop, instead of a branch with a second one: 16 texts 69).  A part takes 490 instructions, 62 % of the issue slots of the SMs are in use and half
 // of the integer pipe's, and neither memory (42 %) nor the tensor pipe: what is left over are the waits of 4 warps per scheduler for each other's chains (loads from shared memory,
 // products, exponentials).
 #include <algorithm>
@@ -111,6 +112,20 @@ template <unsigned EIGHT> __device__ __forceinline__ uint32_t centred(uint32_t c
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+// a b and a b + c, each of two.
+__device__ __forceinline__ float2 times(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 u, v;\n\tmov.b64 u, {%2, %3};\n\tmov.b64 v, {%4, %5};\n\tmul.rn.f32x2 u, u, v;\n\tmov.b64 {%0, %1}, u;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 times_plus(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{\n\t.reg .b64 u, v, w;\n\tmov.b64 u, {%2, %3};\n\tmov.b64 v, {%4, %5};\n\tmov.b64 w, {%6, %7};\n\tfma.rn.f32x2 u, u, v, w;\n\tmov.b64 {%0, %1}, u;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+__device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
 // 2^e; 0 below fp32's normal numbers.
 __device__ __forceinline__ float power(int e) { return e < -126 ? 0.f : __uint_as_float((unsigned)(e + 127) << 23); }
 
@@ -130,15 +145,16 @@ __device__ __forceinline__ Span span_of(const Attn4Args& a, int b) {
 struct Job { int b, kh, row0, nrows, first, last, step; };
 
 // A warp's sums: of rows 8 t + 2 c and + 1; O without the zeros, in units of 2^-24 / fit (dims 64 h + 32 y + 4 g + {0, 2} in acc[4 h + 2 y], {1, 3} in the next), and what the zeros
-// add, by group, of the lane's keys.  fit: what w sV is multiplied by, a power of two for each row and group; byte n holds the exponent field of group n's.
+// add, by group, of the lane's keys.  fit: what w sV is multiplied by, a power of two for each row and group, whose upper 16 bits are all of it.
 template <int HD, int GS, int NT> struct Sums {
     static constexpr int HH = HD / 64, NG = HD / GS;
-    static constexpr int kFitMost = 253;          // 2^126: times a weight still a number
-    float acc[NT][4 * HH][4], zacc[NT][2][NG], m[NT][2], l[NT][2];
-    unsigned fit[NT][2];
+    static constexpr unsigned kFitMost = 0x7e807e80u;            // 2^126: times a weight still a number
+    float acc[NT][4 * HH][4], m[NT][2], l[NT][2];
+    float2 zacc[NT][NG];                          // (x, y: r = 0, 1)
+    unsigned fit[NT][NG];                         // (lower half, upper half)
 
-    static __device__ __forceinline__ int field(unsigned all, int n) { return (int)(all >> 8 * n & 0xffu); }
-    static __device__ __forceinline__ float number(unsigned all, int n) { return __uint_as_float((n < 3 ? all << (23 - 8 * n) : all >> 1) & 0x7f800000u); }
+    static __device__ __forceinline__ int field(unsigned both, int r) { return (int)(r ? both >> 23 : both >> 7 & 0xffu); }       // the exponent's
+    static __device__ __forceinline__ float2 numbers(unsigned both) { return make_float2(__uint_as_float(both << 16), __uint_as_float(both & 0xffff0000u)); }
     // Row (t, r)'s sums of group n are multiplied by f.
     __device__ __forceinline__ void scale(int t, int r, int n, float f) {
 #pragma unroll
@@ -159,13 +175,13 @@ template <int HD, int GS, int NT> struct Sums {
                 for (int o = 4; o < 32; o <<= 1) {
                     l[t][r] += __shfl_xor_sync(0xffffffffu, l[t][r], o);
 #pragma unroll
-                    for (int n = 0; n < NG; ++n) zacc[t][r][n] += __shfl_xor_sync(0xffffffffu, zacc[t][r][n], o);
+                    for (int n = 0; n < NG; ++n) (r ? zacc[t][n].y : zacc[t][n].x) += __shfl_xor_sync(0xffffffffu, r ? zacc[t][n].y : zacc[t][n].x, o);
                 }
     }
     // Dims 64 h + 32 y + 4 g .. of row r.  (Fields at bits 4 .. 7 were 16 times as large.)
     __device__ __forceinline__ float4 four(int t, int r, int h, int y) const {
         const int n = GS == 32 ? 2 * h + y : h;
-        const float z = zacc[t][r][n], limit = power(127 - field(fit[t][r], n));
+        const float z = r ? zacc[t][n].y : zacc[t][n].x, limit = power(127 - field(fit[t][n], r));
         const float *even = acc[t][4 * h + 2 * y], *odd = acc[t][4 * h + 2 * y + 1];
         return make_float4(fmaf(even[r] * 0x1p24f, limit, z), fmaf(odd[r] * 0x1p24f, limit, z), fmaf(even[2 + r] * 0x1p20f, limit, z), fmaf(odd[2 + r] * 0x1p20f, limit, z));
     }
@@ -224,9 +240,10 @@ __device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, co
     uint4* q_at = reinterpret_cast<uint4*>(own + L::q) + lane;
     uint32_t qz[NT];
     float factor[NT][2];
-    float (&acc)[NT][4 * HH][4] = sums.acc, (&zacc)[NT][2][NG] = sums.zacc, (&m)[NT][2] = sums.m, (&l)[NT][2] = sums.l;
+    float (&acc)[NT][4 * HH][4] = sums.acc, (&m)[NT][2] = sums.m, (&l)[NT][2] = sums.l;
+    float2 (&zacc)[NT][NG] = sums.zacc;
     using Fit = Sums<HD, GS, NT>;
-    unsigned (&fit)[NT][2] = sums.fit;
+    unsigned (&fit)[NT][NG] = sums.fit;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         const int idx = job.row0 + min(8 * t + g, job.nrows - 1), tok = token_of(idx), head = job.kh * G + idx - tok * G;
@@ -286,11 +303,10 @@ __device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, co
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             m[t][e] = -INFINITY; l[t][e] = 0.f;
-            fit[t][e] = Fit::kFitMost * 0x01010101u;
             factor[t][e] = __shfl_sync(0xffffffffu, mine, 4 * (2 * c + e));
-#pragma unroll
-            for (int n = 0; n < NG; ++n) zacc[t][e][n] = 0.f;
         }
+#pragma unroll
+        for (int n = 0; n < NG; ++n) { zacc[t][n] = both(0.f); fit[t][n] = Fit::kFitMost; }
 #pragma unroll
         for (int n = 0; n < 4 * HH; ++n) acc[t][n][0] = acc[t][n][1] = acc[t][n][2] = acc[t][n][3] = 0.f;
     }
@@ -349,7 +365,11 @@ __device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, co
 #pragma unroll
                     for (int t = 0; t < NT; ++t)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) s[t][e] = fmaf(e < 2 ? f0 : f1, d[t][e], s[t][e]);
+                        for (int e = 0; e < 4; e += 2) {
+                            const float2 two = times_plus(both(e ? f1 : f0), make_float2(d[t][e], d[t][e + 1]), make_float2(s[t][e], s[t][e + 1]));
+                            s[t][e] = two.x;
+                            s[t][e + 1] = two.y;
+                        }
                 }
             }
 #pragma unroll
@@ -378,28 +398,29 @@ __device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, co
             }
         if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+            for (int t = 0; t < NT; ++t) {
+                int down[2];
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                     float up = fmaxf(ceilf(top[t][r]) + kBelow, m[t][r]);
 #pragma unroll
                     for (int o = 4; o < 32; o <<= 1) up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, o));
                     // (from minus infinity, or to infinity: all there was counts for nothing)
-                    const int down = up == m[t][r] ? 0 : (int)fmaxf(m[t][r] - up, -1024.f);
+                    down[r] = up == m[t][r] ? 0 : (int)fminf(up - m[t][r], 255.f);
                     m[t][r] = up;
-                    if (fresh) continue;
-                    const float corr = power(down);
-                    l[t][r] *= corr;
-                    unsigned fits = 0;
-#pragma unroll
-                    for (int n = 0; n < NG; ++n) {            // what was the largest w sV is smaller by as much: the sums stay as they are in units that do so too
-                        const int old = Fit::field(fit[t][r], n), now = min(old - down, Fit::kFitMost);
-                        zacc[t][r][n] *= corr;
-                        sums.scale(t, r, n, power(now - old + down));
-                        fits |= (unsigned)now << 8 * n;
-                    }
-                    fit[t][r] = fits;
+                    if (!fresh) l[t][r] *= power(-down[r]);
                 }
+                if (fresh) continue;
+                const float2 corr = make_float2(power(-down[0]), power(-down[1]));
+#pragma unroll
+                for (int n = 0; n < NG; ++n) {    // what was the largest w sV is smaller by as much: the sums stay as they are in units that do so too
+                    const unsigned old = fit[t][n], now = __vminu2(old + ((unsigned)down[0] << 7 | (unsigned)down[1] << 23), Fit::kFitMost);
+                    zacc[t][n] = times(zacc[t][n], corr);
+                    fit[t][n] = now;
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) sums.scale(t, r, n, power(Fit::field(now, r) - Fit::field(old, r) - down[r]));
+                }
+            }
         }
 #pragma unroll
         for (int t = 0; t < NT; ++t)
@@ -435,9 +456,8 @@ __device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, co
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
-                    for (int r = 0; r < 2; ++r)
-#pragma unroll
-                        for (int n = 0; n < NG; ++n) zacc[t][r][n] = fmaf(s[t][r], zv[0][n], fmaf(s[t][2 + r], zv[1][n], zacc[t][r][n]));
+                    for (int n = 0; n < NG; ++n)
+                        zacc[t][n] = times_plus(make_float2(s[t][0], s[t][1]), both(zv[0][n]), times_plus(make_float2(s[t][2], s[t][3]), both(zv[1][n]), zacc[t][n]));
             }
             // w sV as operands, of as many groups at once as registers hold
             constexpr int ONCE = NT <= 2 ? NG : 1, EIGHT = St::v_at(8, 0) - St::v_at(0, 0);
@@ -452,9 +472,11 @@ __device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, co
 #pragma unroll
                         for (int i = 0; i < ONCE; ++i) {
                             const int n = n0 + i;
-                            const float f0 = Fit::number(fit[t][0], n), f1 = Fit::number(fit[t][1], n);
-                            b0[t][i] = Half<__half>::pack(s[t][0] * f0 * sv[0][n], s[t][1] * f1 * sv[0][n]);
-                            b1[t][i] = Half<__half>::pack(s[t][2] * f0 * sv[1][n], s[t][3] * f1 * sv[1][n]);
+                            const float2 f = Fit::numbers(fit[t][n]),
+                                         p0 = times(times(make_float2(s[t][0], s[t][1]), f), both(sv[0][n])),
+                                         p1 = times(times(make_float2(s[t][2], s[t][3]), f), both(sv[1][n]));
+                            b0[t][i] = Half<__half>::pack(p0.x, p0.y);
+                            b1[t][i] = Half<__half>::pack(p1.x, p1.y);
                             most = __hmax2(most, __hmax2(__habs2(*reinterpret_cast<const __half2*>(&b0[t][i])), __habs2(*reinterpret_cast<const __half2*>(&b1[t][i]))));
                         }
                     return most;
@@ -463,17 +485,20 @@ __device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, co
 #pragma unroll
                     for (int t = 0; t < NT; ++t)
 #pragma unroll
-                        for (int r = 0; r < 2; ++r)
+                        for (int i = 0; i < ONCE; ++i) {         // (of each row: upper halves of numbers, whose order is theirs)
+                            const int n = n0 + i;
+                            const float2 p0 = times(make_float2(s[t][0], s[t][1]), both(sv[0][n])), p1 = times(make_float2(s[t][2], s[t][3]), both(sv[1][n]));
+                            const float x = fmaxf(fmaxf(fabsf(p0.x), fabsf(p1.x)), 0.f), y = fmaxf(fmaxf(fabsf(p0.y), fabsf(p1.y)), 0.f);
+                            unsigned large = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632u);
 #pragma unroll
-                            for (int i = 0; i < ONCE; ++i) {
-                                const int n = n0 + i, old = Fit::field(fit[t][r], n);
-                                float large = fmaxf(fmaxf(fabsf(s[t][r] * sv[0][n]), fabsf(s[t][2 + r] * sv[1][n])), 0.f);
+                            for (int o = 4; o < 32; o <<= 1) large = __vmaxu2(large, __shfl_xor_sync(0xffffffffu, large, o));
+                            // (exponent fields: 127 for 1, so 254 + 6 less that of the largest)
+                            const unsigned old = fit[t][n], now = __vminu2(old, (260u << 7 | 260u << 23) - (large & 0x7f807f80u));
+                            fit[t][n] = now;
+                            if (!fresh)
 #pragma unroll
-                                for (int o = 4; o < 32; o <<= 1) large = fmaxf(large, __shfl_xor_sync(0xffffffffu, large, o));
-                                const int now = min(old, 2 * 127 + 6 - (int)(__float_as_uint(large) >> 23));
-                                if (!fresh) sums.scale(t, r, n, power(now - old));
-                                fit[t][r] += (unsigned)(now - old) << 8 * n;
-                            }
+                                for (int r = 0; r < 2; ++r) sums.scale(t, r, n, power(Fit::field(now, r) - Fit::field(old, r)));
+                        }
                     products();
                 }
                 if (n0 == 0) { v[0] = lds<VW, 0>(even_from); v[1] = lds<VW, 0>(odd_from); v[2] = lds<VW, EIGHT>(even_from); v[3] = lds<VW, EIGHT>(odd_from); }
