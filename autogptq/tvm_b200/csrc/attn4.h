@@ -21,7 +21,8 @@ struct Attn4Divisors { Divisor row_tiles, kv_heads, group; };
 struct Attn4Plan { bool read, flat; int tiles8, split_bits, ctas; };
 
 int attn4_rows_dispatch(const Attn4Args& a, float* part, const Attn4Plan& p, cudaStream_t stream);
-// The rows of the cache that any query sees, into k, v with the strides of a.attn's caches (cache4.cu).
-int attn4_read_back(const Attn4Args& a, void* k, void* v, cudaStream_t stream);
+// The rows of the cache that any query sees, into k, v [batch, kv_heads, rows, hd] (cache4.cu).  Where `rows` is less than the cache has, which a window allows, rows behind the sinks move
+// up so that the last one that is seen is the last there is, and `pos` gets the positions of token 0 among them.
+int attn4_read_back(const Attn4Args& a, void* k, void* v, int rows, int64_t* pos, cudaStream_t stream);
 
 }  // namespace b200gptq

@@ -225,8 +225,8 @@ template <typename T, int HD, int GS> __device__ __forceinline__ void unpack_row
 
 // A CTA takes kRowsPerCta rows of the keys or the values of one sequence and head; a lane kDeep of them, all asked for at once.
 constexpr int kDeep = 4, kRowsPerCta = kThreads / 4 * kDeep;
-template <typename T, int HD, int GS, typename Wanted, typename Out>
-__device__ __forceinline__ void read_rows(const b200gptq_cache4& cache, unsigned b, int head, bool is_k, int j0, Wanted wanted, Out out) {
+template <typename T, int HD, int GS, typename From, typename Out>
+__device__ __forceinline__ void read_rows(const b200gptq_cache4& cache, unsigned b, int head, bool is_k, int j0, From from, Out out) {
     const int c = threadIdx.x & 3;
     const uint8_t* codes = static_cast<const uint8_t*>(is_k ? cache.k : cache.v) + (is_k ? b * cache.k_stride[0] + head * cache.k_stride[1] : b * cache.v_stride[0] + head * cache.v_stride[1]);
     const T* constants = static_cast<const T*>(is_k ? cache.k_scales : cache.v_scales) +
@@ -237,14 +237,15 @@ __device__ __forceinline__ void read_rows(const b200gptq_cache4& cache, unsigned
 #pragma unroll
     for (int i = 0; i < kDeep; ++i) {
         const int j = j0 + i * (kThreads / 4);
-        if (!wanted(j)) continue;
-        word[i] = load_words<HD / 32>(codes + j * stride + HD / 8 * c);
-        of[i] = load_words<HD / GS>(constants + j * scale_stride);
+        const int row = from(j);                  // of the cache; -1: none
+        if (row < 0) continue;
+        word[i] = load_words<HD / 32>(codes + row * stride + HD / 8 * c);
+        of[i] = load_words<HD / GS>(constants + row * scale_stride);
     }
 #pragma unroll
     for (int i = 0; i < kDeep; ++i) {
         const int j = j0 + i * (kThreads / 4);
-        if (wanted(j)) unpack_row<T, HD, GS>(word[i], of[i], out(j), c);
+        if (from(j) >= 0) unpack_row<T, HD, GS>(word[i], of[i], out(j), c);
     }
 }
 
@@ -259,13 +260,13 @@ cache_read_kernel(const __grid_constant__ b200gptq_cache_read_args a, unsigned c
     const long long length = a.lengths ? min(__ldcg(reinterpret_cast<const long long*>(a.lengths) + b), (long long)a.cache.max_seq) : a.cache.max_seq;
     T* out = static_cast<T*>(is_k ? a.k_out : a.v_out) + (is_k ? b * a.k_out_stride[0] + head * a.k_out_stride[1] : b * a.v_out_stride[0] + head * a.v_out_stride[1]);
     const long long stride = is_k ? a.k_out_stride[2] : a.v_out_stride[2];
-    read_rows<T, HD, GS>(a.cache, b, head, is_k, j0, [&](int j) { return j < length; }, [&](int j) { return out + j * stride; });
+    read_rows<T, HD, GS>(a.cache, b, head, is_k, j0, [&](int j) { return j < length ? j : -1; }, [&](int j) { return out + j * stride; });
 }
 
-// For prompts: the rows that the tokens see between them, into k and v with the strides of the attention's caches.
+// For prompts: the rows that the tokens see between them, into k and v of `rows` rows (attn4_read_back).
 template <typename T, int HD, int GS>
 __global__ void __launch_bounds__(kThreads)
-cache_read_seen_kernel(const __grid_constant__ Attn4Args a, T* __restrict__ k, T* __restrict__ v, unsigned chunks, const __grid_constant__ Divisor by_chunks,
+cache_read_seen_kernel(const __grid_constant__ Attn4Args a, T* __restrict__ k, T* __restrict__ v, int rows, long long* __restrict__ pos, unsigned chunks, const __grid_constant__ Divisor by_chunks,
                        const __grid_constant__ Divisor by_heads) {
     asm volatile("griddepcontrol.launch_dependents;");
     const unsigned which = over(blockIdx.x, by_chunks), pair = which >> 1, b = over(pair, by_heads);
@@ -275,8 +276,18 @@ cache_read_seen_kernel(const __grid_constant__ Attn4Args a, T* __restrict__ k, T
     const int p0 = attn_pos(a.attn, b), count = attn_count(a.attn, b);
     const AttnRange r = attn_range(p0, p0 + count - 1, a.attn.window ? a.attn.window : 1 << 30, a.attn.sinks, a.cache.max_seq);
     const int end = count ? min(r.w_end, a.cache.max_seq) : 0;
-    T* out = (is_k ? k : v) + b * a.attn.k_stride[0] + head * a.attn.k_stride[1];
-    read_rows<T, HD, GS>(a.cache, b, head, is_k, j0, [&](int j) { return j < end && (j < r.s_end || j >= r.w_start); }, [&](int j) { return out + (long long)j * HD; });
+    // (There are as many rows as a window, the tokens behind its first one and the sinks make up, so the first row of the window does not come to lie before the sinks' end, and where
+    // the two meet nothing has moved.)
+    const int up = max(0, min(p0 + count, a.cache.max_seq) - rows);
+    if (pos && threadIdx.x == 0 && head == 0 && is_k && blockIdx.x == which * chunks) pos[b] = p0 - up;
+    T* out = (is_k ? k : v) + ((long long)b * a.cache.kv_heads + head) * rows * HD;
+    read_rows<T, HD, GS>(
+        a.cache, b, head, is_k, j0,
+        [&](int j) {
+            const int from = j < r.s_end ? j : j + up;
+            return j < rows && from < end && (from < r.s_end || from >= r.w_start) ? from : -1;
+        },
+        [&](int j) { return out + (long long)j * HD; });
 }
 
 template <typename... KArgs, typename... Args>
@@ -309,11 +320,11 @@ int read(const b200gptq_cache_read_args& a, cudaStream_t stream) {
 }
 
 template <typename T, int HD, int GS>
-int read_seen(const Attn4Args& a, void* k, void* v, cudaStream_t stream) {
-    const long long chunks = (a.cache.max_seq + kRowsPerCta - 1) / kRowsPerCta, ctas = 2LL * a.cache.batch * a.cache.kv_heads;
+int read_seen(const Attn4Args& a, void* k, void* v, int rows, int64_t* pos, cudaStream_t stream) {
+    const long long chunks = (rows + kRowsPerCta - 1) / kRowsPerCta, ctas = 2LL * a.cache.batch * a.cache.kv_heads;
     if (ctas > 0x7fffffff / chunks) return B200GPTQ_ERR_TOO_LARGE;
-    return launch(cache_read_seen_kernel<T, HD, GS>, dim3((unsigned)(ctas * chunks)), stream, a, static_cast<T*>(k), static_cast<T*>(v), (unsigned)chunks, Divisor(chunks),
-                  Divisor(a.cache.kv_heads));
+    return launch(cache_read_seen_kernel<T, HD, GS>, dim3((unsigned)(ctas * chunks)), stream, a, static_cast<T*>(k), static_cast<T*>(v), rows, reinterpret_cast<long long*>(pos), (unsigned)chunks,
+                  Divisor(chunks), Divisor(a.cache.kv_heads));
 }
 
 template <typename T, typename Args> int by_shape(const Args& a, cudaStream_t stream, int (*const (&run)[2][2])(const Args&, cudaStream_t)) {
@@ -324,11 +335,11 @@ uintptr_t bits_of(const void* p, const int64_t (&stride)[3]) { return p ? reinte
 
 }  // namespace
 
-int attn4_read_back(const Attn4Args& a, void* k, void* v, cudaStream_t s) {
-    using F = int (*)(const Attn4Args&, void*, void*, cudaStream_t);
+int attn4_read_back(const Attn4Args& a, void* k, void* v, int rows, int64_t* pos, cudaStream_t s) {
+    using F = int (*)(const Attn4Args&, void*, void*, int, int64_t*, cudaStream_t);
     static const F run[2][2][2] = {{{read_seen<__half, 64, 32>, read_seen<__half, 64, 64>}, {read_seen<__half, 128, 32>, read_seen<__half, 128, 64>}},
                                    {{read_seen<__nv_bfloat16, 64, 32>, read_seen<__nv_bfloat16, 64, 64>}, {read_seen<__nv_bfloat16, 128, 32>, read_seen<__nv_bfloat16, 128, 64>}}};
-    return run[a.cache.dtype == B200GPTQ_BF16][a.cache.hd == 128][a.cache.group == 64](a, k, v, s);
+    return run[a.cache.dtype == B200GPTQ_BF16][a.cache.hd == 128][a.cache.group == 64](a, k, v, rows, pos, s);
 }
 
 }  // namespace b200gptq

@@ -528,7 +528,10 @@ B200GPTQ_API int b200gptq_cache_read(const b200gptq_cache_read_args* args, void*
  * they multiply codes, by row and group of dims: each is off by 2^-11 of itself or 2^-31 of the largest that the row has in that
  * group (of 2^-96 where that is less).  64 rows of a key head (tokens * heads / kv_heads) or more, and 17 or more over many keys: where that pays the rows that are seen are read back into
  * scratch, each value rounded to dtype, and multiplied as b200gptq_attn does.
- * b200gptq_attn_cache_workspace_bytes: scratch of a call, 16-byte aligned, contents on entry do not matter, not shared by calls that may overlap.
+ * b200gptq_attn_cache_workspace_bytes: scratch of a call, 16-byte aligned, contents on entry do not matter, not shared by calls that may overlap.  Rows that are read back take 4 hd
+ * bytes each, as many as the cache has or a window, the sinks and the tokens make up; where that passes 1 GB they are read back in turns of some key heads of some sequences.  A
+ * call that reads back takes less, down to room for one key head of one sequence (and 16 bytes), or more, in as many turns as that makes, with the same result; one that does
+ * not wants all of it.
  */
 typedef struct {
     b200gptq_cache4 cache;
