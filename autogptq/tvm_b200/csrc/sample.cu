@@ -5,7 +5,8 @@
 // What decides are sums over the vocabulary, and a random number may fall anywhere between two tokens: sums in fp32 put borders off by more than what lies
 // between neighbours.  Weights are integers here (units of 2^-F of the largest, F so that the vocabulary's sum fits 62 bits; off by 2^-32 relative at most: the logarithm in fixed
 // point of 32 fractional bits, by one FMA in 64 bits, a table of 256 powers and a Taylor polynomial of degree 3, after P. T. P. Tang, "Table-driven implementation of the
-// exponential function", 1989), their sums have neither order nor rounding, and the products p * S and u * S are taken in 128 bits.
+// exponential function", 1989; the table has 52 bits and the products with it 40, so that the logarithm's last one is what counts, 2^-33.5), their sums have
+// neither order nor rounding, and the products p * S and u * S are taken in 128 bits.
 //
 // A cluster of CTAs shares a row, each keeps a slice of the logits in shared memory.  Where top-k or top-p ends follows from histograms: 1024 bins, linear in
 // the logarithm of the weight, of the tokens' number (top-k) or weight (top-p; the order of x and of the bins is the same), then the bin in which the search ends
@@ -13,7 +14,7 @@
 // search ended are looked at again: each warp moves its own together.  The CTAs of the cluster read each other's sums through distributed shared memory and all come
 // to the same results.
 // Bound by the chain of searches (2 to 5 after one another, some 5000 clk each: bins, a meeting, sums from the other CTAs, a decision) and, with many rows, by the
-// instructions of the pass over all weights.  Measured: 1 row of 32000 17.6 us, 64 rows of 50272 30.0, 128 of 100003 in fp32 127 (half of
+// instructions of the pass over all weights.  Measured: 1 row of 32000 17.7 us, 64 rows of 50272 30.9, 128 of 100003 in fp32 130 (half of
 // the issue slots in use).
 #include <cuda_bf16.h>
 
@@ -94,7 +95,6 @@ __device__ __forceinline__ u64 share(float f, u64 s, bool up) {
     return q + (up && rest ? 1 : 0);
 }
 
-struct Power { unsigned whole; float part; };       // 2^(30 + j / kTable), as a whole number and in fp32
 // A bin's weight in three words of 17 bits and what they pass over, so that adding takes no carry (a slice has below 2^15 tokens); its number of tokens is in the first.
 struct Bins { unsigned part[3][kBins]; };
 constexpr int kPart = 17;
@@ -103,7 +103,7 @@ struct __align__(16) Warp { u64 mass; unsigned ties, unused; };       // of a wa
 struct Shared {
     Bins bins[2];                         // in turn: this pass's, and the last one's, which become the next one's
     u64 groups[2][kMostCtas][kBins / 32]; // sums of 32 bins of each CTA
-    Power table[kTable];
+    u64 table[kTable];                    // 2^(52 + j / kTable)
     Warp warps[kMostCtas * kWarps];       // of all CTAs
     u64 found_above, all, target, before;
     unsigned ties_before;
@@ -117,20 +117,22 @@ struct Row {
     double step;                         // log2(e) / T
     int bits;                            // F
 };
-__device__ __forceinline__ u64 weight(float x, const Row& r, const Power* table) {        // (no branches: several at once hide each other's latency)
+__device__ __forceinline__ u64 weight(float x, const Row& r, const u64* table) {        // (no branches: several at once hide each other's latency)
     // 1.5 2^20 + log2 of the weight: the number's last word is the fraction of the logarithm, the first its whole part
     const long long y = __double_as_longlong(fma((double)x - (double)r.top, r.step, 1572864.0));
-    const int hi = (int)(y >> 32), down = 0x41380000 - hi;                               // (a NaN, minus infinity: far outside)
+    const unsigned down = 0x41380000u - (unsigned)(y >> 32);                             // (a NaN, minus infinity: far outside)
     const unsigned f = (unsigned)y;
-    const Power p = table[f >> (32 - kTableBits)];
-    constexpr float ln2 = 0.693147181f;
-    const float z = (float)(f & ((1u << (32 - kTableBits)) - 1)) * (ln2 * 0x1p-32f), e = fmaf(z * z, fmaf(z, 1.f / 6, 0.5f), z);        // 2^(rest) - 1 below 2^-8.5
-    const u64 m = (u64)(p.whole + __float2uint_rn(p.part * e)) << (r.bits - 29);         // twice the weight, before it is shifted down
-    const u64 w = ((m >> max(0, min(down, 63))) + 1) >> 1;
-    return x == r.top ? 1ull << r.bits : (unsigned)down < 64u ? w : 0;
+    const u64 p = table[f >> (32 - kTableBits)];
+    // 2^rest - 1 in units of 2^-40, below 2^31.5: z + z^2 / 2 + z^3 / 6 with z = ln 2 times the rest, the first of these as a whole number
+    constexpr double ln2 = 0.69314718055994531;
+    const float z = (float)(f & ((1u << (32 - kTableBits)) - 1));                        // (units of 2^-32)
+    const unsigned e = __umulhi(f << kTableBits, (unsigned)(ln2 * 0x1p32 + 0.5)) + __float2uint_rn(z * z * fmaf(z, (float)(ln2 * ln2 * ln2 / 6 * 0x1p-56), (float)(ln2 * ln2 / 2 * 0x1p-24)));
+    const u64 m = p + ((u64)(unsigned)(p >> 21) * e >> 19);                              // the weight in units of 2^-52, before it is shifted down
+    const u64 w = ((m >> min(51 - r.bits + down, 63u)) + 1) >> 1;
+    return x == r.top ? 1ull << r.bits : down < 64u ? w : 0;
 }
 // The same where it is not worth its code.
-__device__ __noinline__ u64 weight_apart(float x, const Row& r, const Power* table) { return weight(x, r, table); }
+__device__ __noinline__ u64 weight_apart(float x, const Row& r, const u64* table) { return weight(x, r, table); }
 // Bin of x, kBins or more where its weight is zero.
 __device__ __forceinline__ int bin_of(float x, const Row& r) {
     if (x == r.top) return 0;
@@ -207,10 +209,7 @@ sample_kernel(const __grid_constant__ b200gptq_sample_args a, int slice, int clu
         if (ctas > 1) cluster_sync();
         else __syncthreads();
     };
-    if (tid < kTable) {
-        const double power = exp2(30 + (double)tid / kTable);
-        s.table[tid] = {(unsigned)__double2uint_rn(power), (float)power};
-    }
+    if (tid < kTable) s.table[tid] = __double2ull_rn(exp2(52 + (double)tid / kTable));
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride + base;
