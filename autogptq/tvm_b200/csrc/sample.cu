@@ -251,7 +251,7 @@ sample_kernel(const __grid_constant__ b200gptq_sample_args a, int slice, int clu
     r.bits = bits;
     const bool greedy = !(temperature >= kColdest) || top_k == 1 || min_p > 1.f || r.top == -INFINITY;
     r.step = greedy ? 0.0 : step;
-    r.half_scale = (float)(r.step * (2.0 * kBins) / (bits + 1));
+    r.half_scale = (float)(r.step * (2.0 * kBins) / (bits + 1) * (1 - 0x1p-20));          // (less than roundings in fp32 may add: no weight that is not zero lies behind the bins)
     // ---- the border: tokens of larger keys are kept, and of those at it the first `ties` ----
     enum { kNumber, kWeight, kKept };            // tokens into bins, for top-k; weights into bins, for top-p; sums of what is kept
     unsigned border = greedy ? key_of<T>(r.top) : 0, ties = greedy ? 1 : 0xffffffffu, lo = 0, hi = 0xffffffffu;

@@ -1,7 +1,9 @@
-"""How far the weights of ops.sample are off: no tolerance but the header's.
+"""How far the weights of ops.sample are off, and that none is lost at the end of the bins: no tolerance but the header's.
 
 A weight w, the largest being 1, is a whole number of units of 2^-49 here (up to 8192 tokens) and off by half a unit and 2^-32 of itself at most.  64 bits are off by 2^-52.
 """
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -53,3 +55,30 @@ def test_a_crowd_of_equal_weights():
     logits[:, 8000] = 0
     out = ops.sample(logits.to(DEV), u[near].to(DEV)).cpu()
     assert torch.equal(out == 8000, (8000 * w < border)[near])
+
+
+def at_the_end():
+    """Temperatures and largest logits for which a logit of 0 has a little more than half a unit of weight and 1024 bins, counted in fp32, end before it."""
+    found = []
+    for t in np.linspace(0.5, 2, 3000).astype(np.float32):
+        step = 1.4426950408889634 / float(t)
+        per_half = np.float32(step * 2048 / 50)
+        near = np.float32(50 / step)
+        for k in range(-6, 7):
+            top = (np.array([near]).view(np.int32) + k).view(np.float32)[0]
+            if 1e-6 < 50 - float(top) * step and np.float32(0.5) * top * per_half >= 1024:
+                found.append((50 - float(top) * step, float(t), float(top)))
+    return sorted(found, reverse=True)[:20]
+
+
+def test_top_k_counts_the_smallest_weights():
+    """Of 998 tokens with half a unit of weight and more, all unlike, top-k keeps the two largest beside the top one, and with no random number the lowest that is kept is drawn."""
+    rows = at_the_end()
+    assert len(rows) == 20
+    small = torch.arange(1, 999, dtype=torch.float64) * 2.0 ** -60
+    logits = torch.stack([torch.cat([small, torch.tensor([top], dtype=torch.float64)]) for _, _, top in rows]).float()
+    temperature = torch.tensor([t for _, t, _ in rows])
+    assert all(0.5 < 2.0 ** 49 * math.exp((float(row[0]) - float(row[-1])) / t) < 0.51 for row, (_, t, _) in zip(logits, rows))
+    k = torch.full((20,), 3, dtype=torch.long)
+    out = ops.sample(logits.to(DEV), torch.zeros(20, device=DEV), temperature=temperature.to(DEV), top_k=k.to(DEV)).cpu()
+    assert bool((out >= 996).all()), out
