@@ -194,11 +194,11 @@ template <typename Target> __device__ __forceinline__ void find(Shared& s, const
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 2)
-sample_kernel(const __grid_constant__ b200gptq_sample_args a, int slice, int cluster_bits, int bits, int room) {
+sample_kernel(const __grid_constant__ b200gptq_sample_args a, int slice, int cluster_bits, int bits) {
     extern __shared__ __align__(16) unsigned char smem[];
     Shared& s = *reinterpret_cast<Shared*>(smem);
     T* x = reinterpret_cast<T*>(smem + (sizeof(Shared) + 15) / 16 * 16);                  // the slice, later what each warp has kept of its run of it
-    unsigned short* places = reinterpret_cast<unsigned short*>(x + slice);                // and where that stood in the run (where there is room for both)
+    unsigned short* places = reinterpret_cast<unsigned short*>(x + slice);                // and where that stood in the run
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, ctas = 1 << cluster_bits, row = blockIdx.x >> cluster_bits, rank = blockIdx.x & (ctas - 1);
     const int base = min(rank * slice, a.vocab), n = min(slice, a.vocab - base);
     // A warp's tokens: a run of the slice
@@ -315,7 +315,7 @@ sample_kernel(const __grid_constant__ b200gptq_sample_args a, int slice, int clu
                 lo = key_of<T>(far) > 2 ? key_of<T>(far) - 2 : 0;
                 hi = max(key_of<T>(fminf(near, r.top)), 3u) + (bin == 0 ? 0 : 2);
                 shift = max(0, 32 - __clz(hi - lo) - kBinBits);
-                if (!moved && room) {            // nothing below the keys of this bin will be kept: the others move to the front of the run
+                if (!moved) {            // nothing below the keys of this bin will be kept: the others move to the front of the run
                     int held = 0;
                     constexpr int DEEP = 4;
                     const float least_x = lo <= key_of<T>(-INFINITY) ? -INFINITY : of_key<T>(lo);       // (not a NaN)
@@ -462,15 +462,19 @@ sample_kernel(const __grid_constant__ b200gptq_sample_args a, int slice, int clu
 }
 
 constexpr size_t kMostShared = 227 * 1024;
-size_t shared_bytes(int slice, size_t size) { return (sizeof(Shared) + 15) / 16 * 16 + slice * size; }
+constexpr int kMostVocab = 1 << 18;
+// Of a slice: logits and 16 bits of place for each.
+constexpr size_t shared_bytes(int slice, size_t size) { return (sizeof(Shared) + 15) / 16 * 16 + slice * (size + sizeof(unsigned short)); }
+static_assert(shared_bytes(kMostVocab / kMostCtas, sizeof(float)) <= kMostShared, "");
 
 template <typename T>
 int launch(const b200gptq_sample_args& a, cudaStream_t stream) {
     // CTAs per row: as many as the SMs hold two of, a slice of 1024 tokens or more, and enough that a slice leaves an SM room for two (what eight cannot hold so
-    // takes more).  Measured, us, with this and with other numbers of CTAs per row: 1 row of 32000, 8 CTAs 14.5, 4 17.0; 64 rows of 32000, 4 26.1, 8 38.4; 300 of 4099, 1
-    // 21.0, 4 56.7; 20 of 100003 in fp32, 8 36.2, 4 39.5; 128 of them, 8 127, 4, which leave an SM one CTA, 143.
+    // takes more).  Measured, us, with this and with other numbers of CTAs per row, temperatures of 0.6 to 1.2.  Top-k 50, then top-p 0.95: 1 row of 32000, 8 CTAs 17.6, 4 18.2, 1
+    // 21.9; 64 rows of 32000, 4 21.8, 2 25.4, 8 41.7; 64 of 50272, 4 24.9, 2 23.8, 8 43.8; 300 of 4099, 1 29.6, 2 52; 20 of 100003 in fp32, 8 31.9, 4 29.0; 128 of them, 8 133, 4, which
+    // leave an SM one CTA, 124.  Top-p 0.95 alone, where more is searched: 64 of 50272, 4 35.8, 2 40.4, 8 46.6; 300 of 4099, 1 28.2, 2 42; 20 of 100003, 8 38.9, 4 42.6; 128, 8 146, 4 159.
     int cluster_bits = 0;
-    while (cluster_bits < 3 && ((long long)a.rows << (cluster_bits + 1) <= 2LL * sm_count() || shared_bytes((a.vocab >> cluster_bits) + 8, sizeof(T) + sizeof(unsigned short)) > 113 * 1024) &&
+    while (cluster_bits < 3 && ((long long)a.rows << (cluster_bits + 1) <= 2LL * sm_count() || shared_bytes((a.vocab >> cluster_bits) + 8, sizeof(T)) > 113 * 1024) &&
            a.vocab >> (cluster_bits + 1) >= 1024)
         ++cluster_bits;
     // (slices begin at multiples of 16 bytes)
@@ -478,9 +482,7 @@ int launch(const b200gptq_sample_args& a, cudaStream_t stream) {
     int log2v = 0;
     while (1 << log2v < a.vocab) ++log2v;
     const int bits = 62 - log2v < 49 ? 62 - log2v : 49;
-    // (a vocabulary near 2^18 in fp32 leaves no room to move tokens together)
-    const bool room = shared_bytes(slice, sizeof(T) + sizeof(unsigned short)) <= kMostShared;
-    const size_t smem = shared_bytes(slice, sizeof(T) + (room ? sizeof(unsigned short) : 0));
+    const size_t smem = shared_bytes(slice, sizeof(T));
     static const bool pdl = [] {
         const char* e = std::getenv("B200GPTQ_PDL");
         return !(e && e[0] == '0');
@@ -513,7 +515,7 @@ int launch(const b200gptq_sample_args& a, cudaStream_t stream) {
     }
     cfg.attrs = attr;
     cfg.numAttrs = n;
-    B200GPTQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a, slice, cluster_bits, bits, room ? 1 : 0));
+    B200GPTQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a, slice, cluster_bits, bits));
     return B200GPTQ_OK;
 }
 
@@ -528,7 +530,7 @@ extern "C" B200GPTQ_API int b200gptq_sample(const b200gptq_sample_args* args, vo
     if (!a.logits || !a.uniform || !a.out) return B200GPTQ_ERR_NULL_POINTER;
     if (a.dtype != B200GPTQ_F16 && a.dtype != B200GPTQ_BF16 && a.dtype != B200GPTQ_F32) return B200GPTQ_ERR_SHAPE;
     if (a.rows < 1 || a.vocab < 1 || a.logits_stride < 0) return B200GPTQ_ERR_SHAPE;
-    if (a.vocab > 1 << 18 || a.rows > 1 << 27) return B200GPTQ_ERR_TOO_LARGE;
+    if (a.vocab > kMostVocab || a.rows > 1 << 27) return B200GPTQ_ERR_TOO_LARGE;
     const int size = a.dtype == B200GPTQ_F32 ? 4 : 2;
     if (reinterpret_cast<uintptr_t>(a.logits) & (size - 1) || (reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.top_k)) & 7u ||
         (reinterpret_cast<uintptr_t>(a.uniform) | reinterpret_cast<uintptr_t>(a.temperature) | reinterpret_cast<uintptr_t>(a.top_p) | reinterpret_cast<uintptr_t>(a.min_p)) & 3u)
