@@ -437,7 +437,7 @@ void need_no_gradients(PyObject* const* args, const char* const* names, int coun
     }
 }
 const void* data_of(const at::Tensor& t) { return t.unsafeGetTensorImpl()->data(); }
-// The memory between a tensor's first and last element, and whether that of two has a byte in common.
+// The memory between a tensor's first and last element.
 struct Memory {
     uintptr_t lo = 0, hi = 0;
     Memory() = default;
@@ -452,7 +452,27 @@ struct Memory {
     }
     bool meets(const Memory& o) const { return lo < o.hi && o.lo < hi; }
 };
-bool overlap(const at::Tensor& x, const at::Tensor& y) { return Memory(x).meets(Memory(y)); }
+// Whether two tensors may have a byte in common.  Where one begins before the other ends they may still alternate (keys and values side by side in one allocation): seen modulo
+// a stride of theirs, dimensions of which it divides the stride stay where they are, and what the others reach may lie apart.
+bool alternate(const at::Tensor& x, const at::Tensor& y) {
+    const uintptr_t at_x = (uintptr_t)data_of(x), at_y = (uintptr_t)data_of(y);
+    auto reach = [](const at::Tensor& t, uintptr_t period) {
+        const uintptr_t size = t.element_size();
+        uintptr_t bytes = size;
+        for (int64_t i = 0; i < t.dim(); ++i)
+            if (t.size(i) > 1 && (uintptr_t)t.stride(i) * size % period) bytes += (uintptr_t)(t.size(i) - 1) * (uintptr_t)t.stride(i) * size;
+        return bytes;
+    };
+    for (const at::Tensor* t : {&x, &y})
+        for (int64_t i = 0; i < t->dim(); ++i) {
+            const uintptr_t period = (uintptr_t)t->stride(i) * t->element_size();
+            if (t->size(i) < 2 || period == 0) continue;
+            const uintptr_t apart = at_y >= at_x ? (at_y - at_x) % period : (period - (at_x - at_y) % period) % period;        // from x on to y
+            if (reach(x, period) <= apart && apart + reach(y, period) <= period) return true;
+        }
+    return false;
+}
+bool overlap(const at::Tensor& x, const at::Tensor& y) { return Memory(x).meets(Memory(y)) && !alternate(x, y); }
 // Whether the elements of each dimension lie apart: a dimension's stride passes all that the dimensions of smaller strides reach.
 bool apart_from_itself(const at::Tensor& t) {
     c10::SmallVector<std::pair<int64_t, int64_t>, 4> dims;         // (stride, size)
@@ -769,7 +789,7 @@ PyObject* write_checked(PyObject* const* args) {
     for (int i : {2, 3, 4, 5, 11, 12, 13}) {
         if (!t[i]) continue;
         bool apart = i < 6 || apart_from_itself(*t[i]);
-        for (int j = 0; j < 14; ++j) apart = apart && (j == i || !memory[i].meets(memory[j]));
+        for (int j = 0; j < 14; ++j) apart = apart && (j == i || !memory[i].meets(memory[j]) || alternate(*t[i], *t[j]));
         need(apart, names[i], "must not overlap another tensor, nor itself");
     }
     a.tokens = (int)T;
