@@ -26,7 +26,7 @@
 // idle for a quarter of it, at the ends of sequences and at the end; sums of single warps alone: 1 text of 16000 26 us, with those of CTAs 19.)
 //
 // Measured (32 / 8 heads of 128): those 16 texts 62 us, 2.8 TB/s; 1 text of 700, 32 heads, 7.4; 2 texts of 16000 and 16 rows 28.8, 1 and 64 rows 56 (26.8 and 48.6
-// with a power of two per warp; one copy of the products in a loop, instead of a branch with a second one: 16 texts 69).  A part takes 490 instructions, 62 % of the issue slots of the SMs are in use and half
+// with a power of two per warp; one copy of the products in a loop, instead of a branch with a second one: 16 texts 69).  A part takes 480 instructions, 60 % of the issue slots of the SMs are in use and half
 // of the integer pipe's, and neither memory (42 %) nor the tensor pipe: what is left over are the waits of 4 warps per scheduler for each other's chains (loads from shared memory,
 // products, exponentials).
 #include <algorithm>

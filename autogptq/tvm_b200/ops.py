@@ -526,7 +526,8 @@ def cache_write(cache: QuantCache, k, v, pos, counts=None, cos=None, sin=None, q
     """New tokens into a cache in 4 bits, in one launch (``b200gptq_cache_write``): token t of sequence b at row ``pos[b] + t``.
 
     ``k``, ``v`` ``[B, T, kv_heads, hd]`` in the type of the cache's constants; ``pos`` int64 ``[1]`` or ``[B]`` on the device, ``counts`` as for :func:`attn_window`.  With
-    ``cos`` / ``sin`` ``[positions, hd / 2]`` the keys, and the queries ``q`` ``[B, T, heads, hd]`` into ``q_out``, are rotated first (pairs of neighbours, row ``pos[b] + t``).
+    ``cos`` / ``sin`` ``[positions, hd / 2]`` the keys, and the queries ``q`` ``[B, T, heads, hd]`` into ``q_out``, are rotated first (pairs of neighbours, row ``pos[b] + t``;
+    dims of models that turn halves are put side by side when their weights are loaded).
     ``k_out`` / ``v_out`` ``[B, T, kv_heads, hd]`` get what the cache then stands for.  Padding, and tokens at positions outside the cache or
     the angles, are left out everywhere.  A group of dims with a NaN or an infinity in it is NaN throughout.  Returns ``q_out``."""
     return _checked(_lib._host.cache_write(k, v, cache.k, cache.v, cache.k_scales, cache.v_scales, pos, counts, cos, sin, q, q_out, k_out, v_out),
@@ -542,7 +543,8 @@ def cache_read(cache: QuantCache, lengths=None, k_out=None, v_out=None):
 def attn_cache(q, cache: QuantCache, pos, window: Optional[int] = None, sinks: int = 0, counts=None, scale: Optional[float] = None, out=None):
     """:func:`attn_window` over a cache in 4 bits (``b200gptq_attn_cache``); ``window`` None: a token sees the whole text up to it.  The new tokens are in the
     cache already (:func:`cache_write`).  Many rows (tokens x heads) per key
-    head may take scratch for the cache's rows in 16 bits."""
+    head may take scratch for rows of the cache in 16 bits, those that a window, sinks and tokens make up, and 1 GB at most (or one key head of one sequence); keys, values and weights
+    are then rounded to their type.  The sizes decide, ``max_seq`` among them."""
     return _checked(_lib._host.attn_cache(q, cache.k, cache.v, cache.k_scales, cache.v_scales, pos, window, sinks, counts, scale, out), "b200gptq_attn_cache")
 
 

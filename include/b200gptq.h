@@ -531,7 +531,7 @@ B200GPTQ_API int b200gptq_cache_read(const b200gptq_cache_read_args* args, void*
  * b200gptq_attn_cache_workspace_bytes: scratch of a call, 16-byte aligned, contents on entry do not matter, not shared by calls that may overlap.  Rows that are read back take 4 hd
  * bytes each, as many as the cache has or a window, the sinks and the tokens make up; where that passes 1 GB they are read back in turns of some key heads of some sequences.  A
  * call that reads back takes less, down to room for one key head of one sequence (and 16 bytes), or more, in as many turns as that makes, with the same result; one that does
- * not wants all of it.
+ * not wants all of it.  Whether a call reads back follows from the sizes alone, capacity included: the same text in a larger cache may be rounded otherwise.
  */
 typedef struct {
     b200gptq_cache4 cache;
