@@ -16,8 +16,8 @@
 //
 // Every warp takes parts of 16 keys on its own, through a ring of cp.async stages in shared memory.  Keys are the 16 of m16n8k16, rows the 8: 8 bytes (128
 // dims: 16) of a key are the operand of S as they lie, two keys' words paired by byte permutations that of O (include/b200gptq.h has the order of the codes).
-// Rows are only rescaled when a score is more than 8 (log2) above the maximum in use (no weight is above 2^-16; fp32 sums), which is a whole number, so that all factors are
-// powers of two.
+// Rows are only rescaled when a score is more than 8 (log2) above the maximum in use (no weight is above 2^-16; fp32 sums), and then to a weight of 2^-24 for the
+// largest: a power of two, which w sV does not round.  (A maximum rounded up to a whole number made all factors powers of two, and the distance of single tokens from 64 bits 2.9e-4 instead of 2.2e-4.)
 //
 // attn4_cluster_kernel: a cluster of 1 to 8 CTAs shares a (sequence, key head, tile of rows), and they add up through distributed shared memory.
 // attn4_flat_kernel: for many keys per tile.  The parts of all sequences and key heads lie one behind the other, and each WARP takes an even run of them, whatever the texts'
@@ -400,25 +400,29 @@ __device__ __forceinline__ void run_parts(const Attn4Args& a, const Job& job, co
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 int down[2];
+                float2 corr, rest;
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    float up = fmaxf(ceilf(top[t][r]) + kBelow, m[t][r]);
+                    float up = top[t][r];
 #pragma unroll
                     for (int o = 4; o < 32; o <<= 1) up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, o));
-                    // (from minus infinity, or to infinity: all there was counts for nothing)
-                    down[r] = up == m[t][r] ? 0 : (int)fminf(up - m[t][r], 255.f);
-                    m[t][r] = up;
-                    if (!fresh) l[t][r] *= power(-down[r]);
+                    up += kBelow;
+                    const float by = up - m[t][r];           // (infinite where there was nothing, or a score is infinite: what there was counts for nothing)
+                    const bool moves = by > kGrow;
+                    if (moves) m[t][r] = up;
+                    down[r] = moves ? (int)fminf(ceilf(by), 255.f) : 0;
+                    (r ? corr.y : corr.x) = moves ? exp2_fast(-by) : 1.f;
+                    (r ? rest.y : rest.x) = moves ? exp2_fast((float)down[r] - by) : 1.f;
+                    if (!fresh) l[t][r] *= r ? corr.y : corr.x;
                 }
                 if (fresh) continue;
-                const float2 corr = make_float2(power(-down[0]), power(-down[1]));
 #pragma unroll
-                for (int n = 0; n < NG; ++n) {    // what was the largest w sV is smaller by as much: the sums stay as they are in units that do so too
+                for (int n = 0; n < NG; ++n) {    // what was the largest w sV is smaller by as much: units of the sums shrink so too, by the power of two that is next
                     const unsigned old = fit[t][n], now = __vminu2(old + ((unsigned)down[0] << 7 | (unsigned)down[1] << 23), Fit::kFitMost);
                     zacc[t][n] = times(zacc[t][n], corr);
                     fit[t][n] = now;
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) sums.scale(t, r, n, power(Fit::field(now, r) - Fit::field(old, r) - down[r]));
+                    for (int r = 0; r < 2; ++r) sums.scale(t, r, n, power(Fit::field(now, r) - Fit::field(old, r) - down[r]) * (r ? rest.y : rest.x));
                 }
             }
         }

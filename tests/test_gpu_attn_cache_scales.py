@@ -160,3 +160,24 @@ def test_the_largest_and_smallest_scales(S):
     cache.v_scales[:, :, :, 1, 1] = 0
     q = queries(2, 1, 4, 128, BF16)
     check(ops.attn_cache(q, cache, at(S - 1, S - 7)), *reference(q, cache, [S - 1, S - 7]))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("S,window", [(40, 1), (3000, None), (20000, None)])
+@pytest.mark.parametrize("heads,group", [(1, 32), (13, 64), (30, 32)])
+def test_the_largest_weight_is_not_rounded(heads, group, S, window, dtype):
+    """A row whose weight lies all on one key comes out as that key's value: the largest weight is a power of two, and times a scale of 16 bits has no rounding.
+
+    u |o| is left, and 2^-17 A for zeros and codes added up in fp32 and the scale's exp2 (a few steps of 2^-22 each).
+    """
+    g = torch.Generator(device=DEV).manual_seed(3)
+    where = torch.full((S,), -60.0, device=DEV)
+    where[S - 1] = 0
+    cache = made(1, S, 1, 128, group, dtype, where)
+    cache.k_scales[..., 1] += cache.k_scales.new_tensor(0.37)                 # (scores that are no whole numbers)
+    cache.v_scales[..., 0] = (0.1 + torch.rand(cache.v_scales.shape[:-1], generator=g, device=DEV)).to(dtype)
+    q = queries(1, 1, heads, 128, dtype)
+    code, scale, zero = (t[0, 0, S - 1] for t in parts(cache.v, cache.v_scales))
+    want = (zero + scale * code)[None, None, None].expand(q.shape)
+    A = (zero.abs() + 16 * scale)[None, None, None]
+    check(ops.attn_cache(q, cache, at(S - 1), window=window), want, torch.finfo(dtype).eps / 2 * want.abs() + 2.0 ** -17 * A)
